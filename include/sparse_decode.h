@@ -253,6 +253,145 @@ int32_t sd_check_device(sd_index* idx, int32_t* flags, sd_stream stream);
 int32_t sd_decode_noalloc(const sd_config* cfg, const sd_arrays* arrays, int64_t offset, const void* q, float scale,
                           void* out, int32_t* sel_out, int32_t* device_flags, sd_stream stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged serving cache: the tokens of many sequences of different lengths in
+ * the pages of one pool, and what a decode step does around it -- norms and
+ * rotary positions of queries and keys, storing the new tokens, copying pages
+ * (fork, compaction) and attention of one new token per sequence.
+ *
+ * These calls keep no state: the caller owns every device array. The
+ * reference caches one sequence batch per layer (KVCacheSimple,
+ * KVCache.swift:315-371) and has no pages; storage formats are its own
+ * (dense rows, or the affine tuple of QuantizedKVCache).
+ * ------------------------------------------------------------------------- */
+
+/* A pool of n_pages pages of page_size tokens for n_layers layers. K and V
+ * are [n_layers, n_pages, n_kv_heads, page_size, D] of dtype, or, for
+ * kv_bits 4 / 8, uint32-packed codes [..., D * kv_bits / 32] with scales and
+ * biases [..., D / 64] of dtype. Every array starts on a 16-byte boundary. */
+typedef struct {
+  void* k_data;
+  void* v_data;
+  void* k_scales;      /* the four scale/bias arrays: quantized pools only, else NULL */
+  void* k_biases;
+  void* v_scales;
+  void* v_biases;
+  int64_t n_pages;     /* n_pages * n_kv_heads * page_size rows must stay below 2^31 */
+  int32_t n_layers;
+  int32_t n_kv_heads;
+  int32_t head_dim;    /* D in {64, 128} */
+  int32_t page_size;   /* tokens: 16, 32, 64, 128 or 256 */
+  int32_t dtype;       /* sd_dtype */
+  int32_t kv_bits;     /* 0, 4 or 8 */
+  int32_t group_size;  /* 64 when kv_bits != 0, else 0 */
+  int32_t reserved;    /* must be 0 */
+} sd_pages;
+
+/* Rows [batch, tokens, heads, D] with contiguous D; strides in elements. */
+typedef struct {
+  void* data;
+  int64_t batch_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+} sd_rows;
+
+/* Norm and rotation of the rows of queries and keys (RoPE with the
+ * reference's `traditional` flag, applied at the cache offset:
+ * Libraries/MLXLMCommon/RoPEApplication.swift:23-27; q_norm / k_norm as
+ * Libraries/MLXLLM/Models/Qwen3.swift:65-96 applies them). For a row x:
+ *   y = x * rsqrt(mean(x^2) + eps) * w                     (if its norm is given)
+ *   (a, b) -> factor * (a cos - b sin, b cos + a sin), angle = position * inv_freq[i],
+ * where pair i < rot_dim / 2 is (y[i], y[i + rot_dim / 2]), or
+ * (y[2i], y[2i + 1]) when traditional; y[rot_dim ..] passes through. All in
+ * fp32, rounded once. Any scaling of positions for long contexts is in
+ * inv_freq and factor. */
+typedef struct {
+  const float* inv_freq;  /* [rot_dim / 2]; may be NULL when rot_dim is 0 */
+  const void* q_norm;     /* [D] of the rows' dtype, or NULL */
+  const void* k_norm;
+  float eps;
+  float factor;
+  int32_t rot_dim;        /* even, 0 .. D */
+  int32_t traditional;
+  int32_t reserved[2];    /* must be 0 */
+} sd_rotation;
+
+/* q_out / k_out = rotated q / k for batch x tokens tokens at
+ * positions[batch * tokens] (int32). k (with n_kv_heads 0) or q (with
+ * n_q_heads 0) may be absent; an output may be its own input. head_dim: even,
+ * 2 .. 256. */
+int32_t sd_rotary(const sd_rotation* rot, int32_t dtype, int32_t head_dim, int32_t batch, int32_t tokens,
+                  const int32_t* positions, int32_t n_q_heads, const sd_rows* q, const sd_rows* q_out,
+                  int32_t n_kv_heads, const sd_rows* k, const sd_rows* k_out, sd_stream stream);
+
+/* Store n_tokens new tokens (k, v: rows [1, n_tokens, n_kv_heads, D]) into
+ * layer `layer` of the pool: token n of sequence seq[n] (NULL: n) at
+ * positions[n] goes to page tables[seq[n], position / page_size], slot
+ * position % page_size; a negative position stores nothing (padding). With
+ * `rot` the keys are normed and rotated on the way, and the queries (n_q_heads
+ * > 0) into q_out, in the same launch. Rows are quantized like sd_append's.
+ * Two tokens of one call must not share a slot. tables [batch, table_width]
+ * int32. An index out of range stores nothing and sets bit 2 of
+ * *device_flags (nullable device int, as sd_check_device's bits). */
+int32_t sd_paged_append(const sd_pages* pages, int32_t layer, int32_t n_tokens, const sd_rows* k, const sd_rows* v,
+                        const int32_t* tables, int32_t batch, int32_t table_width, const int32_t* positions,
+                        const int32_t* seq, const sd_rotation* rot, int32_t n_q_heads, const sd_rows* q,
+                        const sd_rows* q_out, int32_t* device_flags, sd_stream stream);
+
+/* Page dst[i] = page src[i], i < n, in every layer and array of the pool (src,
+ * dst: device int32). The dst pages must be distinct and none of them a src.
+ * A pair out of range copies nothing and sets bit 2 of *device_flags. */
+int32_t sd_copy_pages(const sd_pages* pages, const int32_t* src, const int32_t* dst, int32_t n,
+                      int32_t* device_flags, sd_stream stream);
+
+/* Attention of one new token per sequence (q [batch, n_q_heads, D]) over the
+ * pages: out [batch, n_q_heads, D] = softmax(scale * q K^T) V over the tokens
+ * [max(0, lengths[b] - window), lengths[b]) (window 0: all of them; the last
+ * token is the new one, stored before the call). sinks: [n_q_heads] fp32 as
+ * in sd_set_sinks, or NULL. A length of 0 gives zeros. Query heads per kv
+ * head: 1 .. 16. Lengths and tables are read on the device only. The
+ * workspace (sd_paged_workspace bytes, 16-byte aligned, contents do not
+ * matter) must not be shared by calls that may overlap. Pages past a
+ * sequence's length, or before its window, are not read. An index or length
+ * out of range sets bit 2 of *device_flags; rows of such a page read as 0. */
+int32_t sd_paged_workspace(const sd_pages* pages, int32_t batch, int32_t n_q_heads, int64_t* bytes);
+int32_t sd_paged_decode(const sd_pages* pages, int32_t layer, const void* q, int32_t batch, int32_t n_q_heads,
+                        const int32_t* tables, int32_t table_width, const int32_t* lengths, float scale,
+                        int32_t window, const float* sinks, void* out, void* workspace, int64_t workspace_bytes,
+                        int32_t* device_flags, sd_stream stream);
+
+/* Which sequence holds which page: host bookkeeping of one pool, with pages
+ * shared between forked sequences by reference counts. No call touches the
+ * GPU; those that need page copies return the pairs for sd_copy_pages, to be
+ * copied before the next append (extend) or decode (compact). One map is used
+ * by one host thread at a time. Sequence ids are never reused. */
+typedef struct sd_pagemap sd_pagemap; /* opaque */
+int32_t sd_pagemap_create(int64_t n_pages, int32_t page_size, sd_pagemap** out);
+int32_t sd_pagemap_destroy(sd_pagemap* map);
+int32_t sd_pagemap_add(sd_pagemap* map, int64_t* seq);
+/* A new sequence with the same tokens: every page becomes shared. */
+int32_t sd_pagemap_fork(sd_pagemap* map, int64_t seq, int64_t* forked);
+int32_t sd_pagemap_free(sd_pagemap* map, int64_t seq);
+/* Make room for n_tokens more tokens. If the page that they begin in is
+ * shared, the sequence gets a copy of its own: *n_copies (0 or 1) and the pair
+ * are written. SD_ERR_CAPACITY, and nothing changed, when the pool has too
+ * few free pages. */
+int32_t sd_pagemap_extend(sd_pagemap* map, int64_t seq, int64_t n_tokens, int32_t* src, int32_t* dst,
+                          int32_t* n_copies);
+/* Drop up to n_tokens tokens from the end (KVCache.trim); *trimmed nullable. */
+int32_t sd_pagemap_trim(sd_pagemap* map, int64_t seq, int64_t n_tokens, int64_t* trimmed);
+int32_t sd_pagemap_length(const sd_pagemap* map, int64_t seq, int64_t* tokens);
+/* The table of n sequences, [n, width] int32 on the host, rows padded with -1;
+ * lengths [n] nullable. SD_ERR_SHAPE when a sequence has more than width pages. */
+int32_t sd_pagemap_tables(const sd_pagemap* map, const int64_t* seqs, int32_t n, int32_t width, int32_t* tables,
+                          int32_t* lengths);
+/* The most pages that any of the n sequences holds, at least 1. */
+int32_t sd_pagemap_width(const sd_pagemap* map, const int64_t* seqs, int32_t n, int32_t* width);
+int32_t sd_pagemap_free_pages(const sd_pagemap* map, int64_t* n);
+/* Move pages so that the used ones are the lowest: at most `room` moves into
+ * src / dst (*n of them; 0: nothing left to move). */
+int32_t sd_pagemap_compact(sd_pagemap* map, int32_t* src, int32_t* dst, int32_t room, int32_t* n);
+
 #ifdef __cplusplus
 }
 #endif

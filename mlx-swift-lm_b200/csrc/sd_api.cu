@@ -15,12 +15,16 @@
 
 #include "../../include/sparse_decode.h"
 #include "sd_format.h"
+#include "sd_host.h"
 #include "sd_kernels.h"
 #include "sd_params.h"
 
 namespace {
 
 thread_local std::string g_last_error;
+}  // namespace
+
+namespace sd {
 
 int32_t fail(int32_t status, const char* fmt, ...) {
   char buf[512];
@@ -31,17 +35,6 @@ int32_t fail(int32_t status, const char* fmt, ...) {
   g_last_error = buf;
   return status;
 }
-
-#define SD_CUDA(call)                                                                              \
-  do {                                                                                             \
-    cudaError_t e_ = (call);                                                                       \
-    if (e_ != cudaSuccess) return fail(SD_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), \
-                                       __FILE__, __LINE__);                                        \
-  } while (0)
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
@@ -54,6 +47,40 @@ EncodeTiledFn encode_fn() {
   }
   return fn;
 }
+
+// The K or V arena as a 3-D byte tensor (column box, row, box index): a row
+// of row_bytes is cut into boxes of min(row_bytes, 128) bytes, the widest the
+// swizzle allows, and one copy moves a whole tile of kTileTokens rows with all
+// its boxes, landing as [box][row][box bytes] in shared memory. One TMA
+// operation per tile rather than one per box: the SM's TMA unit spends a fixed
+// time on each operation, which dominates copies of a few KB.
+int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const int box_bytes = std::min(row_bytes, 128);
+  const int nbox = row_bytes / box_bytes;
+  CUtensorMapSwizzle sw = box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                          : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                            : CU_TENSOR_MAP_SWIZZLE_32B;
+  cuuint64_t dims[3] = {cuuint64_t(box_bytes), cuuint64_t(rows), cuuint64_t(nbox)};
+  cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(box_bytes)};
+  cuuint32_t box[3] = {cuuint32_t(box_bytes), cuuint32_t(box_rows), cuuint32_t(nbox)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return SD_OK;
+}
+
+}  // namespace sd
+
+namespace {
+
+using sd::EncodeTiledFn;
+using sd::encode_fn;
+using sd::encode_map;
+using sd::fail;
 
 int elt_size(int dtype) { return dtype == SD_F32 ? 4 : 2; }
 
@@ -172,31 +199,6 @@ int32_t validate(const sd_config* c) {
     if (r != 0) return fail(SD_ERR_INVALID_ARG, "reserved config fields must be 0");
   if (c->shard_count * c->top_k > sd::kUnionMax)
     return fail(SD_ERR_SHAPE, "shard_count * top_k must be <= %d", sd::kUnionMax);
-  return SD_OK;
-}
-
-// The K or V arena as a 3-D byte tensor (column box, row, box index): a row
-// of row_bytes is cut into boxes of min(row_bytes, 128) bytes, the widest the
-// swizzle allows, and one copy moves a whole tile of kTileTokens rows with all
-// its boxes, landing as [box][row][box bytes] in shared memory. One TMA
-// operation per tile rather than one per box: the SM's TMA unit spends a fixed
-// time on each operation, which dominates copies of a few KB.
-int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const int box_bytes = std::min(row_bytes, 128);
-  const int nbox = row_bytes / box_bytes;
-  CUtensorMapSwizzle sw = box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                          : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                            : CU_TENSOR_MAP_SWIZZLE_32B;
-  cuuint64_t dims[3] = {cuuint64_t(box_bytes), cuuint64_t(rows), cuuint64_t(nbox)};
-  cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(box_bytes)};
-  cuuint32_t box[3] = {cuuint32_t(box_bytes), cuuint32_t(box_rows), cuuint32_t(nbox)};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
   return SD_OK;
 }
 

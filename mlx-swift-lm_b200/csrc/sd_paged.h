@@ -1,0 +1,140 @@
+// sd_paged.h -- parameters, launch shapes and kernel tables of the operators
+// on a paged KV pool: decode attention, append (with rotation) and page
+// copies. Included by host and device code.
+#pragma once
+
+#include <stdint.h>
+
+#include "sd_format.h"
+
+namespace sd {
+
+constexpr int kPagedWarps = 4;                          // warps that attend
+constexpr int kPagedThreads = (kPagedWarps + 1) * 32;   // + one producer warp
+constexpr int kPagedMaxBatch = 4096;                    // sequences per decode call
+constexpr int kPagedMaxStages = 16;
+// Two CTAs share an SM: half of its 228 KB each, less 1 KB that every CTA reserves.
+constexpr int kPagedSmem = 115712;
+
+// Stored rows of one pool format: E of ESIZE bytes (dense element, or type of
+// the scales and biases), BITS = 0 / 4 / 8.
+template <int ESIZE, int BITS, int D>
+struct PagedFmt {
+  static constexpr bool kTensor = ESIZE == 2;           // 16-bit formats go through the tensor cores
+  static constexpr int kRowBytes = BITS ? D * BITS / 8 : D * ESIZE;
+  static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;
+  static constexpr int kNBox = kRowBytes / kBoxBytes;
+  static constexpr int kCpb = kBoxBytes / 16;           // 16-byte chunks per box row
+  static constexpr int kNChunk = kRowBytes / 16;
+  static constexpr int kEpc = BITS ? 128 / BITS : 16 / ESIZE;  // elements per chunk
+  static constexpr int kGroups = BITS ? D / 64 : 1;
+  // Tokens of one stage: about 16 to 32 KB for K and V together.
+  static constexpr int kTile = BITS ? 128 : ESIZE == 2 ? 64 : 32;
+  static constexpr int kKvBytes = kTile * kRowBytes;    // K (or V) of a stage
+  static constexpr int kSbBytes = BITS ? kTile * kGroups * ESIZE : 0;  // each of the four scale/bias pieces
+  static constexpr int kStageBytes = (2 * kKvBytes + 4 * kSbBytes + 1023) / 1024 * 1024;
+};
+
+// Floats of one warp's (o, m, l) in the combine buffer -- o rows padded to
+// D + 4, which spreads the fragment stores over the banks -- and of one
+// unfinished segment in the workspace; multiples of 4, as both are read with
+// 16-byte accesses.
+__host__ __device__ constexpr int paged_warp_floats(int G, int D) { return (G * (D + 6) + 3) / 4 * 4; }
+__host__ __device__ constexpr int paged_part_floats(int G, int D) { return (G * (D + 2) + 3) / 4 * 4; }
+
+struct PagedParams {
+  const void* q;          // [B, Hkv * G, D]
+  void* out;              // [B, Hkv * G, D]
+  float* part;            // [grid][2][paged_part_floats]: o [G][D], then (m, l) [G]
+  int* prefix;            // [B + 1] tiles of the sequences before b
+  const int* tables;      // [B, W]
+  const int* lengths;     // [B]
+  const float* sinks;     // [Hkv * G] or null
+  const void *k_scales, *k_biases, *v_scales, *v_biases;  // of this layer
+  int64_t n_pages;
+  int B, Hkv, G, P, W, window;
+  int stages, ncta, min_tiles;
+  int q_off, buf_off, prefix_off, bar_off;  // shared-memory layout
+  float scale_log2;
+  int* flags;
+};
+
+struct PagedSet {
+  const void* decode;  // paged_decode_kernel<E, BITS, D, NB>(PagedParams, CUtensorMap, CUtensorMap)
+  const void* merge;   // paged_merge_kernel<E, D>(PagedParams, int tile)
+  int tile, stage_bytes, row_bytes, groups;
+};
+// nb: blocks of 8 query heads per kv head (1 or 2). Null members without an instantiation.
+PagedSet paged_e0_b0(int D, int nb);
+PagedSet paged_e1_b0(int D, int nb);
+PagedSet paged_e2_b0(int D, int nb);
+PagedSet paged_e0_b4(int D, int nb);
+PagedSet paged_e1_b4(int D, int nb);
+PagedSet paged_e2_b4(int D, int nb);
+PagedSet paged_e0_b8(int D, int nb);
+PagedSet paged_e1_b8(int D, int nb);
+PagedSet paged_e2_b8(int D, int nb);
+
+// ---------------------------------------------------------------------------
+
+// Rows [batch, tokens, heads, D] with D contiguous; strides in elements.
+struct Rows {
+  void* data;
+  int64_t batch, token, head;
+};
+
+struct RotaryParams {
+  Rows q, k, v, q_out, k_out;
+  int Hq, Hkv, Hv;          // heads of q, k and v rows per token (0: none)
+  int R;                    // Hq + Hkv + Hv
+  int D, rot2;              // head_dim, rotated pairs (0: no rotation)
+  int traditional;
+  int L;                    // tokens per batch entry
+  int64_t tasks;            // batch * L * R
+  const int* positions;     // [batch * L]
+  const float* inv_freq;    // [rot2]
+  const void *q_norm, *k_norm;
+  float eps, factor;
+  int span;                 // tokens whose rows one block may touch
+  // append: where the k and v rows go (null tables: k_out)
+  const int* tables;
+  const int* seq;
+  int B, W, P, page_shift;
+  int64_t n_pages;
+  void *k_data, *v_data, *k_scales, *k_biases, *v_scales, *v_biases;
+  int* flags;
+};
+
+constexpr int kRotThreads = 128;
+constexpr int kRotUnroll = 4;  // rows in flight per group of lanes
+// Lanes per row (log2): a power of two with a chunk pair of 2 * vec elements for each, at most a warp.
+__host__ __device__ constexpr int rotary_lanes_log(int D, int vec) {
+  int l = 0;
+  while (l < 5 && (1 << l) < D / (2 * vec)) ++l;
+  return l;
+}
+// Shared floats before the staged rows: cos and sin of `span` tokens, two norms.
+__host__ __device__ constexpr int rotary_stage_at(int span, int rot2, int D) {
+  return (span * 2 * rot2 + 2 * D + 3) / 4 * 4;
+}
+
+// vec: elements per access (1, 2, 4, 8 for 16-bit types; 1, 2, 4 for fp32); null if not instantiated.
+const void* rotary_kernel_for(int dtype, int bits, int vec);
+
+struct CopyParams {
+  const int *src, *dst;
+  int n;
+  int64_t n_pages;
+  int n_layers, n_arrays;
+  uint8_t* array[6];
+  int64_t bytes[6];   // of one page in each array
+  int pieces[6];      // kCopyPiece pieces of one page
+  int per_pair;       // pieces of one page pair in one layer
+  int64_t total;      // n * n_layers * per_pair
+  int* flags;
+};
+constexpr int kCopyPiece = 16384;
+constexpr int kCopyThreads = 256;
+const void* copy_pages_kernel_ptr();
+
+}  // namespace sd

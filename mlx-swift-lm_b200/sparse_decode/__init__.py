@@ -13,6 +13,9 @@ and mirrors the reference's cache/attention API on top of it:
 * `attention_with_cache_update` -- the router
                             (Libraries/MLXLMCommon/AttentionUtils.swift:37-77)
                             with the sparse branch for single-token decode.
+* `PagePool`, `rotary`, `paged_append`, `copy_pages`, `paged_decode`
+                         -- the paged serving cache (paged.py): many sequences
+                            of different lengths in the pages of one pool.
 
 torch is used for device memory and streams only. There is no CPU fallback:
 the native library must be built (`__graft_entry__.build()`), and every
@@ -39,7 +42,10 @@ EXPORTED = ["sd_abi_version", "sd_status_string", "sd_last_error", "sd_index_cre
             "sd_set_offset", "sd_rebuild_summaries", "sd_decode", "sd_shard_candidates", "sd_shard_attend",
             "sd_shard_merge", "sd_check_device", "sd_set_launch_overlap", "sd_decode_noalloc", "sd_comm_create",
             "sd_comm_handle", "sd_comm_open", "sd_comm_open_local", "sd_comm_set_wait_limit", "sd_comm_destroy",
-            "sd_shard_decode", "sd_set_sinks"]
+            "sd_shard_decode", "sd_set_sinks", "sd_rotary", "sd_paged_append", "sd_copy_pages", "sd_paged_workspace",
+            "sd_paged_decode", "sd_pagemap_create", "sd_pagemap_destroy", "sd_pagemap_add", "sd_pagemap_fork",
+            "sd_pagemap_free", "sd_pagemap_extend", "sd_pagemap_trim", "sd_pagemap_length", "sd_pagemap_tables",
+            "sd_pagemap_width", "sd_pagemap_free_pages", "sd_pagemap_compact"]
 COMM_HANDLE_BYTES = 128
 
 
@@ -65,6 +71,23 @@ class SDArrays(ctypes.Structure):
         ("reserved", ctypes.c_int32 * 4)]
 
 
+class SDPages(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_data", "v_data", "k_scales", "k_biases", "v_scales", "v_biases")] + [
+        ("n_pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+            "n_layers", "n_kv_heads", "head_dim", "page_size", "dtype", "kv_bits", "group_size", "reserved")]
+
+
+class SDRows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class SDRotation(ctypes.Structure):
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("factor", ctypes.c_float), ("rot_dim", ctypes.c_int32),
+                ("traditional", ctypes.c_int32), ("reserved", ctypes.c_int32 * 2)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -79,6 +102,8 @@ def lib() -> ctypes.CDLL:
         L = ctypes.CDLL(str(path))
         vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
         pp = ctypes.POINTER(ctypes.c_void_p)
+        pg, pr, prot = ctypes.POINTER(SDPages), ctypes.POINTER(SDRows), ctypes.POINTER(SDRotation)
+        pi32, pi64 = ctypes.POINTER(i32), ctypes.POINTER(i64)
         sig = {
             "sd_abi_version": ([], i32),
             "sd_status_string": ([i32], ctypes.c_char_p),
@@ -109,6 +134,23 @@ def lib() -> ctypes.CDLL:
             "sd_comm_destroy": ([vp], i32),
             "sd_shard_decode": ([vp, vp, vp, vp, vp, f32, vp, vp, vp], i32),
             "sd_set_sinks": ([vp, vp], i32),
+            "sd_rotary": ([prot, i32, i32, i32, i32, vp, i32, pr, pr, i32, pr, pr, vp], i32),
+            "sd_paged_append": ([pg, i32, i32, pr, pr, vp, i32, i32, vp, vp, prot, i32, pr, pr, vp, vp], i32),
+            "sd_copy_pages": ([pg, vp, vp, i32, vp, vp], i32),
+            "sd_paged_workspace": ([pg, i32, i32, pi64], i32),
+            "sd_paged_decode": ([pg, i32, vp, i32, i32, vp, i32, vp, f32, i32, vp, vp, vp, i64, vp, vp], i32),
+            "sd_pagemap_create": ([i64, i32, pp], i32),
+            "sd_pagemap_destroy": ([vp], i32),
+            "sd_pagemap_add": ([vp, pi64], i32),
+            "sd_pagemap_fork": ([vp, i64, pi64], i32),
+            "sd_pagemap_free": ([vp, i64], i32),
+            "sd_pagemap_extend": ([vp, i64, i64, pi32, pi32, pi32], i32),
+            "sd_pagemap_trim": ([vp, i64, i64, pi64], i32),
+            "sd_pagemap_length": ([vp, i64, pi64], i32),
+            "sd_pagemap_tables": ([vp, pi64, i32, i32, pi32, pi32], i32),
+            "sd_pagemap_width": ([vp, pi64, i32, pi32], i32),
+            "sd_pagemap_free_pages": ([vp, pi64], i32),
+            "sd_pagemap_compact": ([vp, pi32, pi32, i32, pi32], i32),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
@@ -441,3 +483,5 @@ def sharded_decode(index, q, k_new=None, v_new=None, scale=None, group=None, sel
 from .cache import SparseKVCache, attention_with_cache_update  # noqa: E402,F401
 from .persist import (load_prompt_cache, make_prompt_cache, maybe_quantize_kv_cache,  # noqa: E402,F401
                       save_prompt_cache)
+from .paged import (KVPages, PagedBatch, PagedLayer, PagePool, copy_pages, paged_append, paged_decode,  # noqa: E402,F401
+                    rotary, rotary_frequencies)

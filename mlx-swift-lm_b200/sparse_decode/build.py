@@ -1,8 +1,10 @@
 """Build libsparse_decode.so (sm_100a) in-tree with nvcc.
 
 The library is compiled from mlx-swift-lm_b200/csrc: one object per storage
-format (sd_inst.cu with SD_E/SD_BITS), plus the C ABI (sd_api.cu). The CUDA
-runtime is linked statically, so the .so only needs the driver at run time.
+format (sd_inst.cu and, for the paged cache, sd_paged_inst.cu, with
+SD_E/SD_BITS), the rotary and page-copy kernels (sd_rotary.cu), plus the C ABI
+(sd_api.cu, sd_pages.cu). The CUDA runtime is linked statically, so the .so
+only needs the driver at run time.
 
 `build(phase_timing=True)` makes a second library, libsparse_decode_phases.so,
 compiled with -DSD_PHASE_TIMING: the decode kernel then writes per-phase
@@ -36,14 +38,16 @@ def _sources() -> list[Path]:
         INCLUDE / "sparse_decode.h"]
 
 
-def _kernel_sources() -> list[Path]:
-    """What the kernel objects (sd_inst.cu) depend on: everything but sd_api.cu."""
-    return [s for s in _sources() if s.name not in ("sd_api.cu", "sparse_decode.h")]
+def _kernel_sources(name: str, skip: set) -> list[Path]:
+    """What a kernel object depends on: its source and csrc's headers, less
+    those of host code and of the other kernels."""
+    return [CSRC / name] + [h for h in sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+                            if h.name not in skip | {"sd_host.h"}]
 
 
-def _api_sources() -> list[Path]:
-    return [CSRC / "sd_api.cu", CSRC / "sd_format.h", CSRC / "sd_params.h", CSRC / "sd_kernels.h",
-            INCLUDE / "sparse_decode.h"]
+def _host_sources(name: str) -> list[Path]:
+    return [CSRC / n for n in (name, "sd_format.h", "sd_params.h", "sd_kernels.h", "sd_host.h", "sd_paged.h")] + [
+        INCLUDE / "sparse_decode.h"]
 
 
 def _stale(target: Path, sources: list[Path] | None = None) -> bool:
@@ -65,20 +69,24 @@ def build(force: bool = False, verbose: bool = False, phase_timing: bool = False
     bdir = PKG_DIR / "_build_phases" if phase_timing else BUILD
     flags = FLAGS + (["-DSD_PHASE_TIMING"] if phase_timing else [])
     bdir.mkdir(exist_ok=True)
-    jobs = []
+    # (object, source, extra flags, files it depends on)
+    units = []
     for e, b in FORMATS:
-        obj = bdir / f"sd_inst_e{e}_b{b}.o"
-        if force or _stale(obj, _kernel_sources()):
-            jobs.append([NVCC, *ARCH, *flags, f"-DSD_E={e}", f"-DSD_BITS={b}", "-c", str(CSRC / "sd_inst.cu"),
-                         "-o", str(obj)])
-    if force or _stale(bdir / "sd_api.o", _api_sources()):
-        jobs.append([NVCC, *ARCH, *flags, "-c", str(CSRC / "sd_api.cu"), "-o", str(bdir / "sd_api.o")])
+        fmt = [f"-DSD_E={e}", f"-DSD_BITS={b}"]
+        units.append((f"sd_inst_e{e}_b{b}.o", "sd_inst.cu", fmt, _kernel_sources("sd_inst.cu", {"sd_paged.cuh", "sd_paged.h"})))
+        units.append((f"sd_paged_e{e}_b{b}.o", "sd_paged_inst.cu", fmt, _kernel_sources("sd_paged_inst.cu", {"sd_decode.cuh"})))
+    units.append(("sd_rotary.o", "sd_rotary.cu", [], _kernel_sources("sd_rotary.cu", {"sd_decode.cuh", "sd_paged.cuh"})))
+    units += [(f"{n}.o", f"{n}.cu", [], _host_sources(f"{n}.cu")) for n in ("sd_api", "sd_pages")]
+    jobs = []
+    for obj, src, extra, deps in units:
+        if force or _stale(bdir / obj, deps):
+            jobs.append([NVCC, *ARCH, *flags, *extra, "-c", str(CSRC / src), "-o", str(bdir / obj)])
     with cf.ThreadPoolExecutor(max_workers=max(2, os.cpu_count() or 2)) as ex:
         for f in cf.as_completed([ex.submit(_run, j) for j in jobs]):
             f.result()
             if verbose:
                 print(".", end="", flush=True)
-    objs = [str(bdir / f"sd_inst_e{e}_b{b}.o") for e, b in FORMATS] + [str(bdir / "sd_api.o")]
+    objs = [str(bdir / obj) for obj, *_ in units]
     if not force and not jobs and not _stale(lib, [Path(o) for o in objs]):
         return lib
     tmp = lib.with_suffix(".so.tmp")

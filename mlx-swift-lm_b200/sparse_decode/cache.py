@@ -260,7 +260,9 @@ def _dequantize(wq, scales, biases, bits: int):
 def attention_with_cache_update(queries, keys, values, cache, scale: float, mask=None, sinks=None):
     """Router (AttentionUtils.swift:37-77; with `sinks`, the sink variant of
     MiMoV2Flash.swift:14-56). queries [B, Hq, L, D]; keys/values
-    [B, Hkv, L, D]; sinks [Hq] or None. Returns [B, Hq, L, D]."""
+    [B, Hkv, L, D]; sinks [Hq] or None. Returns [B, Hq, L, D]. `cache`: None, a
+    SparseKVCache, or a layer of a paged step (PagedBatch.layer)."""
+    from .paged import PagedLayer
     if cache is None:
         return _dense_attention(queries, keys, values, scale, mask, sinks)
     if isinstance(cache, SparseKVCache):
@@ -274,4 +276,6 @@ def attention_with_cache_update(queries, keys, values, cache, scale: float, mask
         else:
             k, v = cache.update(keys, values)
         return _dense_attention(queries, k, v, scale, mask, sinks)
+    if isinstance(cache, PagedLayer):
+        return cache.attend(queries, keys, values, scale, mask, sinks)
     raise TypeError(f"unsupported cache type {type(cache).__name__}")

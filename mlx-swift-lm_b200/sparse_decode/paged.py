@@ -1,0 +1,581 @@
+"""Paged serving cache: rotary positions, page appends and copies, and decode
+attention of many sequences of different lengths over one pool of pages.
+
+The operators (each one launch, decode two) work on the caller's tensors and
+keep nothing between calls:
+
+* `rotary`        -- per-head RMS norm (optional) and rotary positions of
+                     queries and keys;
+* `paged_append`  -- the same, with keys and values stored into their pages
+                     (quantized for 4/8-bit pools);
+* `copy_pages`    -- whole pages copied inside a pool, in every layer;
+* `paged_decode`  -- attention of one new token per sequence over its pages.
+
+`PagePool` owns a pool and the map of sequences to pages (fork, copy-on-write,
+trim, free, compaction); `PagedBatch` is one step's view of some sequences,
+whose layers `attention_with_cache_update` takes as caches.
+
+All calls run on the current device; `stream` defaults to the current stream.
+Tensors last used on another stream must be ordered before the call by the
+caller, as for any torch operation.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Optional, Sequence
+
+from . import DTYPES, SDError, SDPages, SDRotation, SDRows, _check, _torch_dtype, lib
+
+_DTYPE_CODE: dict = {}
+
+
+def _dtype_code(dtype) -> int:
+    if not _DTYPE_CODE:
+        _DTYPE_CODE.update({_torch_dtype(n): c for n, c in DTYPES.items()})
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
+    return code
+
+
+def _device() -> int:
+    import torch
+    return torch.cuda.current_device()
+
+
+def _arg(t, name: str, dtype, dev: int, shape=None) -> Optional[int]:
+    """Device pointer of a contiguous tensor argument (None passes NULL)."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on the current device")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    return t.data_ptr()
+
+
+def _rows(t, name: str, dtype, dev: int, dim: int) -> tuple:
+    """sd_rows of [tokens, heads, D] or [batch, heads, tokens, D] with any
+    strides but the last, as (struct, batch, tokens, heads)."""
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on the current device")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    shape, st = t.shape, t.stride()
+    if len(shape) == 3:
+        n, h, d = shape
+        b, s = 1, (0, st[0], st[1])
+    elif len(shape) == 4:
+        b, h, n, d = shape
+        s = (st[0], st[2], st[1])
+    else:
+        raise ValueError(f"{name} must be [tokens, heads, D] or [batch, heads, tokens, D]")
+    if d != dim:
+        raise ValueError(f"{name} has head_dim {d}, expected {dim}")
+    if st[-1] != 1 and d != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return SDRows(t.data_ptr(), *s), b, n, h
+
+
+def _handle(stream):
+    """(cudaStream_t, context that allocates for it)."""
+    import torch
+    if stream is None:
+        return torch.cuda.current_stream().cuda_stream, contextlib.nullcontext()
+    return stream.cuda_stream, torch.cuda.stream(stream)
+
+
+def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: int, dim: int) -> SDRotation:
+    import torch
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dim() != 1:
+            raise ValueError("inv_freq must be [rot_dim / 2]")
+        rot = 2 * inv_freq.shape[0]
+    return SDRotation(_arg(inv_freq, "inv_freq", torch.float32, dev), _arg(q_norm, "q_norm", dtype, dev, (dim,)),
+                      _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda"):
+    """(inv_freq [rot_dim / 2] fp32 on `device`, factor) for `rotary` and
+    `paged_append`: base^(-2i / rot_dim), computed in 64 bits, with the
+    positions stretched for long contexts by `scaling`, a model
+    configuration's rope_scaling dict:
+
+    * linear:   angles divided by `factor`;
+    * llama3:   only wavelengths beyond original_max_position_embeddings /
+                low_freq_factor are divided, those below .../high_freq_factor
+                are kept, a linear blend between;
+    * yarn:     the same blend by the number of turns over the original
+                context (beta_fast, beta_slow), and the rotated part scaled
+                by 0.1 ln(factor) + 1 (or by the mscale pair's ratio);
+    * longrope: each angle divided by its own entry of long_factor (of
+                short_factor when `factor` is at most 1), rotated part scaled
+                by sqrt(1 + ln(factor) / ln(original)).
+    """
+    import torch
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2")
+    inv = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    mult = 1.0
+    if scaling is not None:
+        kind = scaling.get("rope_type", scaling.get("type", "default"))
+        f = float(scaling.get("factor", 1.0))
+        old = float(scaling.get("original_max_position_embeddings", 8192))
+        if kind == "linear":
+            inv = inv / f
+        elif kind == "llama3":
+            lo, hi = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+            turns = old * inv / (2 * math.pi)
+            keep = ((turns - lo) / (hi - lo)).clamp(0, 1)
+            inv = inv * (keep + (1 - keep) / f)
+        elif kind == "yarn":
+            def dim_of(turns: float) -> float:  # the pair that makes `turns` turns over the original context
+                return rot_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base))
+            lo = max(math.floor(dim_of(float(scaling.get("beta_fast", 32.0)))), 0)
+            hi = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+            i = torch.arange(rot_dim // 2, dtype=torch.float64)
+            stretch = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+            inv = inv * (1 - stretch) + inv / f * stretch
+
+            def mscale(m: float) -> float:
+                return 0.1 * m * math.log(f) + 1.0 if f > 1 else 1.0
+            if "attention_factor" in scaling:
+                mult = float(scaling["attention_factor"])
+            elif scaling.get("mscale") and scaling.get("mscale_all_dim"):
+                mult = mscale(float(scaling["mscale"])) / mscale(float(scaling["mscale_all_dim"]))
+            else:
+                mult = mscale(1.0)
+        elif kind in ("longrope", "su"):
+            each = scaling["long_factor"] if f > 1 else scaling["short_factor"]
+            if len(each) != rot_dim // 2:
+                raise ValueError(f"expected {rot_dim // 2} factors, got {len(each)}")
+            inv = inv / torch.tensor(each, dtype=torch.float64)
+            mult = float(scaling.get("attention_factor",
+                                     math.sqrt(1 + math.log(f) / math.log(old)) if f > 1 else 1.0))
+        elif kind != "default":
+            raise ValueError(f"unknown rope scaling {kind!r}")
+    return inv.to(torch.float32).to(device), mult
+
+
+def rotary(q, k, positions, inv_freq, *, traditional: bool = False, factor: float = 1.0, q_norm=None, k_norm=None,
+           eps: float = 1e-6, q_out=None, k_out=None, stream=None):
+    """Rotary positions of queries and keys, with a per-head RMS norm before
+    them when q_norm / k_norm ([D] weights) are given, in one pass.
+
+    q, k: [tokens, heads, D] or [batch, heads, tokens, D] (any strides but the
+    last; either may be None); positions: int32 [tokens] or [batch, tokens].
+    inv_freq: fp32 [rot_dim / 2] (`rotary_frequencies`); the first rot_dim
+    elements of a head are rotated, in pairs (i, i + rot_dim / 2), or
+    neighbours when `traditional`. Returns (q_out, k_out), new contiguous
+    tensors unless given; a given one may be its input."""
+    import torch
+    ref = q if q is not None else k
+    if ref is None:
+        raise ValueError("q or k is required")
+    dev, dt, dim = _device(), ref.dtype, ref.shape[-1]
+    code = _dtype_code(dt)
+    handle, ctx = _handle(stream)
+    batch = tokens = 0
+    heads, rows, outs = [], [], []
+    for name, x, o in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            heads.append(0)
+            rows += [None, None]
+            outs.append(None)
+            continue
+        r, b, n, h = _rows(x, name, dt, dev, dim)
+        if x is not ref and (b, n) != (batch, tokens):
+            raise ValueError("q and k must have the same tokens")
+        batch, tokens = b, n
+        if o is None:
+            with ctx:
+                o = torch.empty(x.shape, dtype=dt, device=x.device)
+        elif o.shape != x.shape:
+            raise ValueError(f"{name}_out must have {name}'s shape")
+        heads.append(h)
+        rows += [r, _rows(o, name + "_out", dt, dev, dim)[0]]
+        outs.append(o)
+    want = (tokens,) if ref.dim() == 3 else (batch, tokens)
+    pos = _arg(positions, "positions", torch.int32, dev, want)
+    rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
+    _check(lib().sd_rotary(rot, code, dim, batch, tokens, pos, heads[0], rows[0], rows[1], heads[1], rows[2], rows[3],
+                           handle))
+    return outs[0], outs[1]
+
+
+class KVPages:
+    """The device arrays of a pool: k, v [n_pages, Hkv, page_size, D], or with
+    a leading n_layers dimension. 4/8-bit pools (`bits`): k, v int32 codes
+    [..., D * bits / 32] with scales and biases [..., D / 64] (the affine tuple
+    of a quantized cache)."""
+
+    def __init__(self, k, v, k_scales=None, k_biases=None, v_scales=None, v_biases=None, bits: int = 0):
+        import torch
+        dev = k.get_device()
+        if dev < 0:
+            raise ValueError("pool arrays must be CUDA tensors")
+        if k.dim() not in (4, 5):
+            raise ValueError("pool arrays must be [n_pages, Hkv, page_size, .] or [n_layers, n_pages, Hkv, page_size, .]")
+        *lead, n_pages, hkv, page = k.shape[:-1]
+        small = (k_scales, k_biases, v_scales, v_biases)
+        if bits:
+            if any(a is None for a in small):
+                raise ValueError("a quantized pool needs k/v scales and biases")
+            self.dtype = k_scales.dtype
+            dim = k.shape[-1] * 32 // bits
+            data = torch.int32
+        else:
+            if any(a is not None for a in small):
+                raise ValueError("scales and biases need bits")
+            self.dtype, dim, data = k.dtype, k.shape[-1], k.dtype
+        code = _dtype_code(self.dtype)
+        shape = k.shape
+        ptrs = [_arg(k, "k", data, dev), _arg(v, "v", data, dev, shape)]
+        ptrs += [_arg(a, n, self.dtype, dev, (*shape[:-1], dim // 64)) for n, a in
+                 zip(("k_scales", "k_biases", "v_scales", "v_biases"), small)]
+        self.k, self.v = k, v
+        self.k_scales, self.k_biases, self.v_scales, self.v_biases = small
+        self.bits, self.device = bits, dev
+        self.n_layers, self.n_pages = lead[0] if lead else 1, n_pages
+        self.n_kv_heads, self.page_size, self.head_dim = hkv, page, dim
+        self.struct = SDPages(*ptrs, n_pages, self.n_layers, hkv, dim, page, code, bits, 64 if bits else 0, 0)
+
+    def here(self) -> int:
+        """The current device, which must be the pool's."""
+        dev = _device()
+        if dev != self.device:
+            raise ValueError(f"the pool is on cuda:{self.device}, the current device is cuda:{dev}")
+        return dev
+
+
+def paged_append(pages: KVPages, k, v, tables, positions, *, seq=None, layer: int = 0, q=None, inv_freq=None,
+                 traditional: bool = False, factor: float = 1.0, q_norm=None, k_norm=None, eps: float = 1e-6,
+                 q_out=None, flags=None, stream=None):
+    """Store new tokens k, v [tokens, Hkv, D] into layer `layer` of the pool:
+    token n of sequence seq[n] (None: n) at positions[n] lands in page
+    tables[seq[n], position // page_size]; a negative position stores nothing.
+    With inv_freq or a norm the keys are normed and rotated on the way, and so
+    are queries q [tokens, Hq, D], which are returned (else None). Quantized
+    pools store codes of the rotated rows rounded to the pool's type.
+
+    tables [batch, width], positions [tokens], seq [tokens]: int32. flags: an
+    int32 tensor that receives bit 2 when an index is out of range (nothing is
+    stored for that token)."""
+    import torch
+    dev, dt, dim = pages.here(), pages.dtype, pages.head_dim
+    kr, b, n, h = _rows(k, "k", dt, dev, dim)
+    vr, vb, vn, vh = _rows(v, "v", dt, dev, dim)
+    if b != 1 or (vb, vn, vh) != (1, n, h) or h != pages.n_kv_heads:
+        raise ValueError(f"k and v must be [tokens, {pages.n_kv_heads}, {dim}]")
+    if tables.dim() != 2:
+        raise ValueError("tables must be [batch, width]")
+    handle, ctx = _handle(stream)
+    i32 = torch.int32
+    turns = inv_freq is not None or q_norm is not None or k_norm is not None
+    rot, qr, qo, hq = None, None, None, 0
+    if q is not None:
+        qr, qb, qn, hq = _rows(q, "q", dt, dev, dim)
+        if qb != 1 or qn != n:
+            raise ValueError("q must have k's tokens")
+        if q_out is None:
+            with ctx:
+                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+        elif q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
+        qo = _rows(q_out, "q_out", dt, dev, dim)[0]
+    if turns or q is not None:
+        rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
+    _check(lib().sd_paged_append(pages.struct, layer, n, kr, vr, _arg(tables, "tables", i32, dev), tables.shape[0],
+                                 tables.shape[1], _arg(positions, "positions", i32, dev, (n,)),
+                                 _arg(seq, "seq", i32, dev, (n,)), rot, hq, qr, qo, _arg(flags, "flags", i32, dev),
+                                 handle))
+    return q_out if q is not None else None
+
+
+def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
+    """Page dst[i] = page src[i] in every layer and array of the pool. src,
+    dst: int32 CUDA tensors, or sequences of ints (checked here). The dst
+    pages must be distinct and none of them a src."""
+    import torch
+    dev = pages.here()
+    handle, ctx = _handle(stream)
+    if not isinstance(src, torch.Tensor):
+        src, dst = [int(i) for i in src], [int(i) for i in dst]
+        if len(src) != len(dst):
+            raise ValueError("src and dst must have the same length")
+        if any(not 0 <= i < pages.n_pages for i in src + dst):
+            raise ValueError("page out of range")
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("dst pages must be distinct and none of them a src")
+        with ctx:
+            both = torch.tensor([src, dst], dtype=torch.int32).to(dev, non_blocking=True)
+        src, dst = both[0], both[1]
+    if src.dim() != 1:
+        raise ValueError("src and dst must be [n]")
+    _check(lib().sd_copy_pages(pages.struct, _arg(src, "src", torch.int32, dev),
+                               _arg(dst, "dst", torch.int32, dev, src.shape), src.shape[0],
+                               _arg(flags, "flags", torch.int32, dev), handle))
+
+
+def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = None, *, layer: int = 0, window: int = 0,
+                 sinks=None, out=None, flags=None, stream=None):
+    """Attention of one new token per sequence over its pages: q
+    [batch, Hq, D] -> [batch, Hq, D], softmax(scale q K^T) V over the last
+    `window` (0: all) of lengths[b] tokens. A length of 0 gives zeros.
+
+    tables [batch, width] and lengths [batch]: int32, read on the device only,
+    so a captured call serves growing sequences. sinks: fp32 [Hq] logits that
+    join the denominators. Hq / Hkv: 1 .. 16."""
+    import torch
+    dev, dt, dim = pages.here(), pages.dtype, pages.head_dim
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"q must be [batch, Hq, {dim}]")
+    batch, hq = q.shape[0], q.shape[1]
+    if tables.dim() != 2 or tables.shape[0] != batch:
+        raise ValueError("tables must be [batch, width]")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    handle, ctx = _handle(stream)
+    i32, L = torch.int32, lib()
+    need = ctypes.c_int64()
+    if batch:
+        _check(L.sd_paged_workspace(pages.struct, batch, hq, need))
+    with ctx:
+        if out is None:
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
+        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+    _check(L.sd_paged_decode(pages.struct, layer, _arg(q, "q", dt, dev), batch, hq, _arg(tables, "tables", i32, dev),
+                             tables.shape[1], _arg(lengths, "lengths", i32, dev, (batch,)), scale, window,
+                             _arg(sinks, "sinks", torch.float32, dev, (hq,)), _arg(out, "out", dt, dev, q.shape),
+                             work.data_ptr(), need.value, _arg(flags, "flags", i32, dev), handle))
+    return out
+
+
+class PagePool:
+    """A pool of KV pages for every layer of a model, and the sequences in it.
+
+    Sequences are named by the ids that `add` and `fork` return. Forking shares
+    every page; the first token that a sequence adds to a page it shares moves
+    it to a copy of its own (`extend` launches that copy). Pages are freed when
+    no sequence holds them."""
+
+    def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
+                 dtype: str = "bf16", kv_bits: int = 0):
+        import torch
+        if kv_bits not in (0, 4, 8):
+            raise ValueError("kv_bits must be 0, 4 or 8")
+        lead = (n_layers, n_pages, n_kv_heads, page_size)
+        tdt = _torch_dtype(dtype)
+        new = lambda last, dt: torch.zeros((*lead, last), dtype=dt, device="cuda")  # noqa: E731
+        if kv_bits:
+            data = [new(head_dim * kv_bits // 32, torch.int32) for _ in "kv"]
+            small = [new(head_dim // 64, tdt) for _ in range(4)]
+            self.pages = KVPages(*data, *small, bits=kv_bits)
+        else:
+            self.pages = KVPages(new(head_dim, tdt), new(head_dim, tdt))
+        self.flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+        h = ctypes.c_void_p()
+        _check(lib().sd_pagemap_create(n_pages, page_size, ctypes.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) is not None and self._h.value:
+            lib().sd_pagemap_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    # -- sequences -------------------------------------------------------------
+    def add(self) -> int:
+        s = ctypes.c_int64()
+        _check(lib().sd_pagemap_add(self._h, ctypes.byref(s)))
+        return s.value
+
+    def fork(self, seq: int) -> int:
+        s = ctypes.c_int64()
+        _check(lib().sd_pagemap_fork(self._h, seq, ctypes.byref(s)))
+        return s.value
+
+    def free(self, seq: int) -> None:
+        _check(lib().sd_pagemap_free(self._h, seq))
+
+    def trim(self, seq: int, n: int) -> int:
+        t = ctypes.c_int64()
+        _check(lib().sd_pagemap_trim(self._h, seq, n, ctypes.byref(t)))
+        return t.value
+
+    def length(self, seq: int) -> int:
+        t = ctypes.c_int64()
+        _check(lib().sd_pagemap_length(self._h, seq, ctypes.byref(t)))
+        return t.value
+
+    @property
+    def free_pages(self) -> int:
+        n = ctypes.c_int64()
+        _check(lib().sd_pagemap_free_pages(self._h, ctypes.byref(n)))
+        return n.value
+
+    def compact(self, stream=None) -> int:
+        """Move pages so that the used ones are the lowest; returns how many
+        moved. Batches made before are stale afterwards."""
+        n = ctypes.c_int32()
+        room = self.pages.n_pages // 2
+        src, dst = (ctypes.c_int32 * max(room, 1))(), (ctypes.c_int32 * max(room, 1))()
+        _check(lib().sd_pagemap_compact(self._h, src, dst, room, ctypes.byref(n)))
+        if n.value:
+            copy_pages(self.pages, src[:n.value], dst[:n.value], flags=self.flags, stream=stream)
+        return n.value
+
+    # -- steps -----------------------------------------------------------------
+    def extend(self, seqs: Sequence[int], n_tokens, stream=None) -> "PagedBatch":
+        """Make room for n_tokens (an int, or one per sequence) more tokens of
+        each sequence and return the batch that appends them. All or nothing:
+        when the pool has too few free pages, no sequence grows."""
+        each = [int(n_tokens)] * len(seqs) if isinstance(n_tokens, int) else [int(n) for n in n_tokens]
+        if len(each) != len(seqs):
+            raise ValueError("n_tokens must be an int or one per sequence")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence may be named once per batch")
+        src, dst, n = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
+        copies, grown = [], []
+        try:
+            for s, k in zip(seqs, each):
+                _check(lib().sd_pagemap_extend(self._h, s, k, ctypes.byref(src), ctypes.byref(dst), ctypes.byref(n)))
+                grown.append((s, k))
+                if n.value:
+                    copies.append((src.value, dst.value))
+        except SDError:
+            # the pages already copied-on-write stay with their sequences, so their contents must follow
+            for s, k in grown:
+                self.trim(s, k)
+            if copies:
+                copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
+            raise
+        if copies:
+            copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
+        return PagedBatch(self, list(seqs), each, stream)
+
+    def batch(self, seqs: Sequence[int], stream=None) -> "PagedBatch":
+        """The sequences as they are, with no new tokens."""
+        return PagedBatch(self, list(seqs), [0] * len(seqs), stream)
+
+    def check_device(self) -> int:
+        """Read and clear the device error bits (synchronises)."""
+        f = int(self.flags.item())
+        self.flags.zero_()
+        return f
+
+
+class PagedBatch:
+    """One step of some sequences of a pool: `tables` [batch, width] and
+    `lengths` [batch] with the step's new tokens counted in, and for the new
+    tokens, sequence by sequence, `positions` and `seq`. Built on the host and
+    copied to the device once, for every layer of the step."""
+
+    def __init__(self, pool: PagePool, seqs: list, new: list, stream=None):
+        import torch
+        self.pool, self.seqs, self.new = pool, seqs, new
+        n = len(seqs)
+        ids = (ctypes.c_int64 * max(n, 1))(*seqs)
+        width = ctypes.c_int32()
+        _check(lib().sd_pagemap_width(pool._h, ids, n, ctypes.byref(width)))
+        w = width.value
+        tokens = sum(new)
+        host = torch.empty(n * w + n + 2 * tokens, dtype=torch.int32, pin_memory=True)
+        i32p = ctypes.POINTER(ctypes.c_int32)
+        at = lambda k: ctypes.cast(host.data_ptr() + 4 * k, i32p)  # noqa: E731
+        _check(lib().sd_pagemap_tables(pool._h, ids, n, w, at(0), at(n * w)))
+        lengths = host[n * w:n * w + n].tolist()
+        pos = [p for t, k in zip(lengths, new) for p in range(t - k, t)]
+        seq = [b for b, k in enumerate(new) for _ in range(k)]
+        host[n * w + n:] = torch.tensor(pos + seq, dtype=torch.int32)
+        _, ctx = _handle(stream)
+        with ctx:
+            dev = host.to("cuda", non_blocking=True)
+        self.tables = dev[:n * w].view(n, w)
+        self.lengths = dev[n * w:n * w + n]
+        self.positions = dev[n * w + n:n * w + n + tokens]
+        self.seq = dev[n * w + n + tokens:]
+        self.host_lengths = lengths
+
+    def append(self, layer: int, k, v, q=None, **rotation):
+        """`paged_append` of this step's new tokens [tokens, heads, D]."""
+        return paged_append(self.pool.pages, k, v, self.tables, self.positions, seq=self.seq, layer=layer, q=q,
+                            flags=self.pool.flags, **rotation)
+
+    def decode(self, layer: int, q, scale: Optional[float] = None, **kw):
+        """`paged_decode` of one query token per sequence [batch, Hq, D]."""
+        return paged_decode(q, self.pool.pages, self.tables, self.lengths, scale, layer=layer, flags=self.pool.flags,
+                            **kw)
+
+    def layer(self, layer: int, **rotation) -> "PagedLayer":
+        """Layer `layer` of this step as a cache for attention_with_cache_update;
+        `rotation`: the keyword arguments of `paged_append` that norm and rotate
+        queries and keys (none: they come in rotated)."""
+        return PagedLayer(self, layer, rotation)
+
+
+class PagedLayer:
+    """What attention_with_cache_update needs of a paged step's layer."""
+
+    def __init__(self, batch: PagedBatch, layer: int, rotation: dict):
+        self.batch, self.index, self.rotation = batch, layer, rotation
+
+    @property
+    def offset(self):
+        """Tokens of each sequence before this step."""
+        return [t - n for t, n in zip(self.batch.host_lengths, self.batch.new)]
+
+    def attend(self, queries, keys, values, scale: float, mask=None, sinks=None):
+        """Append keys/values [B, Hkv, L, D] and attend with queries
+        [B, Hq, L, D]; every sequence has L new tokens. L == 1 takes the decode
+        kernel; longer prompts are attended densely, sequence by sequence."""
+        import torch
+        from .cache import _dense_attention
+        b = self.batch
+        B, Hq, L, D = queries.shape
+        if any(n != L for n in b.new) or len(b.new) != B:
+            raise ValueError(f"the step holds {b.new} new tokens, the queries {[L] * B}")
+        flat = lambda x: x.transpose(1, 2).reshape(B * L, x.shape[1], D)  # noqa: E731
+        q = flat(queries)
+        if self.rotation:
+            q = b.append(self.index, flat(keys), flat(values), q=q, **self.rotation)
+        else:
+            b.append(self.index, flat(keys), flat(values))
+        if L == 1:
+            if mask is not None:
+                raise ValueError("a single-token step takes no mask")
+            sinks = None if sinks is None else sinks.detach().float().contiguous()
+            return b.decode(self.index, q.contiguous(), scale, sinks=sinks).view(B, Hq, 1, D)
+        q = q.view(B, L, Hq, D).transpose(1, 2)
+        out = torch.empty_like(queries)
+        for i in range(B):
+            k, v = self.dense(i)
+            out[i] = _dense_attention(q[i:i + 1], k, v, scale, "causal" if mask is None else mask, sinks)[0]
+        return out
+
+    def dense(self, i: int):
+        """Keys and values of the batch's sequence i, [1, Hkv, tokens, D]."""
+        from .cache import _dequantize
+        b, p = self.batch, self.batch.pool.pages
+        n = b.host_lengths[i]
+        at = b.tables[i, :-(-n // p.page_size)].long()
+
+        def rows(x):
+            x = x[self.index, at]
+            return x.transpose(0, 1).flatten(1, 2)[None, :, :n]
+        if not p.bits:
+            return rows(p.k), rows(p.v)
+        return (_dequantize(rows(p.k), rows(p.k_scales), rows(p.k_biases), p.bits),
+                _dequantize(rows(p.v), rows(p.v_scales), rows(p.v_biases), p.bits))
