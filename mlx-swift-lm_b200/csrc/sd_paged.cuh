@@ -740,11 +740,21 @@ __device__ __forceinline__ int tiles_of(TokenRange r, int tile) {
   return r.end > r.begin ? (r.end + tile - 1) / tile - r.begin / tile : 0;
 }
 
-// CTAs that take part for U units: at least min_tiles tiles each.
-__device__ __forceinline__ int64_t active_ctas(const PagedParams& p, int64_t U) {
-  const int64_t n = (U + p.min_tiles - 1) / p.min_tiles;
-  return n < p.ncta ? n : p.ncta;
-}
+// The line of U units (tile, pair) in equal pieces for the CTAs that take
+// part, at least min_tiles each: the first `rem` pieces have base + 1 units.
+struct Pieces {
+  int n, base, rem;
+  __device__ __forceinline__ Pieces(const PagedParams& p, int U) {
+    n = min((U + p.min_tiles - 1) / p.min_tiles, p.ncta);
+    base = n ? U / n : 0;
+    rem = U - base * n;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, rem); }
+  __device__ __forceinline__ int of(int u) const {  // the piece that holds unit u
+    const int big = rem * (base + 1);
+    return u < big ? u / (base + 1) : rem + (u - big) / base;
+  }
+};
 
 struct Segment {
   int b, h;
@@ -753,27 +763,25 @@ struct Segment {
 
 struct Walk {
   const int* prefix;
-  int Hkv, b;
-  int64_t u, u1;
-  __device__ __forceinline__ Walk(const int* pre, int B, int hkv, int64_t begin, int64_t end)
+  int Hkv, b, u, u1;
+  __device__ __forceinline__ Walk(const int* pre, int B, int hkv, int begin, int end)
       : prefix(pre), Hkv(hkv), b(0), u(begin), u1(end) {
     int lo = 0, hi = B;  // the largest b with prefix[b] * Hkv <= u; a b without tiles is passed over
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (int64_t(prefix[mid]) * Hkv <= u) lo = mid; else hi = mid;
+      if (prefix[mid] * Hkv <= u) lo = mid; else hi = mid;
     }
     b = lo;
   }
   __device__ __forceinline__ bool next(Segment& s) {
     if (u >= u1) return false;
-    while (int64_t(prefix[b + 1]) * Hkv <= u) ++b;  // ends: u < prefix[B] * Hkv
+    while (prefix[b + 1] * Hkv <= u) ++b;  // ends: u < prefix[B] * Hkv
     s.b = b;
     s.nt = prefix[b + 1] - prefix[b];
-    const int64_t r = u - int64_t(prefix[b]) * Hkv;
-    s.h = int(r / s.nt);
-    s.i0 = int(r - int64_t(s.h) * s.nt);
-    const int64_t left = u1 - u;
-    s.i1 = left < s.nt - s.i0 ? s.i0 + int(left) : s.nt;
+    const int r = u - prefix[b] * Hkv;
+    s.h = r / s.nt;
+    s.i0 = r - s.h * s.nt;
+    s.i1 = min(s.nt, s.i0 + u1 - u);
     u += s.i1 - s.i0;
     return true;
   }
@@ -925,10 +933,9 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   }
   __syncthreads();
 
-  const int64_t U = int64_t(prefix[p.B]) * p.Hkv, N = active_ctas(p, U);
-  if (int64_t(blockIdx.x) >= N) return;
-  const int64_t u0 = blockIdx.x * U / N, u1 = (blockIdx.x + 1) * U / N;
-  Walk walk(prefix, p.B, p.Hkv, u0, u1);
+  const Pieces pieces(p, prefix[p.B] * p.Hkv);
+  if (int(blockIdx.x) >= pieces.n) return;
+  Walk walk(prefix, p.B, p.Hkv, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
 
   if (warp == kPagedWarps) {
     paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
@@ -1004,74 +1011,94 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     for (int k = max(0, it - p.stages); k < it; ++k) mbar_wait(full + k % p.stages, uint32_t(k / p.stages) & 1u, nullptr);
 }
 
-// Joins the segments of one query head (grid: B * Hq blocks of 128 threads)
-// in CTA order; a pair that one CTA did alone is already written, an empty
-// one is written here as zeros.
+// Joins the segments of one query head (grid: B * Hq blocks) in a fixed
+// order; a pair that one CTA did alone is already written, an empty one is
+// written here as zeros. Bound by the latency of its dependent loads, not by
+// their bytes (a few MB at most, from L2): warp w takes the segments w, w + 8,
+// ..., each lane first the (m, l) of one of them, and the o rows are loaded
+// eight at a time, the first eight before the weights are known.
 template <typename E, int D>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedParams p) {
-  __shared__ float wgt[2 * 256], red[4][D], tot[4], top[4];
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int NW = kMergeThreads / 32, V = D / 32, BATCH = 8;
+  __shared__ float red[NW][D], top[NW], tot[NW];
   griddep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int Hq = p.Hkv * p.G, b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, g = hq % p.G;
-  const int pre = p.prefix[b], nt = p.prefix[b + 1] - pre;
+  const int pre = p.prefix[b], nt = p.prefix[b + 1] - pre, all = p.prefix[p.B];
   E* out = static_cast<E*>(p.out) + int64_t(blockIdx.x) * D;
   if (nt == 0) {
-    for (int d = tid; d < D; d += 128) out[d] = Elt<E>::from_f32(0.0f);
+    for (int d = tid; d < D; d += kMergeThreads) out[d] = Elt<E>::from_f32(0.0f);
     return;
   }
-  const int64_t U = int64_t(p.prefix[p.B]) * p.Hkv, N = active_ctas(p, U);
-  const int64_t a = int64_t(pre) * p.Hkv + int64_t(h) * nt;
-  // the CTA whose piece [c U / N, (c + 1) U / N) holds unit x
-  const int c0 = int(((a + 1) * N - 1) / U), c1 = int(((a + nt) * N - 1) / U), ns = c1 - c0 + 1;
+  const Pieces pieces(p, all * p.Hkv);
+  const int a = pre * p.Hkv + h * nt;  // the pair's first unit
+  const int c0 = pieces.of(a), c1 = pieces.of(a + nt - 1), ns = c1 - c0 + 1;
   if (ns == 1) return;
   const int stride = paged_part_floats(p.G, D);
-  auto slot = [&](int c) {
-    return p.part + (int64_t(c) * 2 + (c * U / N >= a ? 0 : 1)) * stride;
-  };
-  float M = -INFINITY;
-  for (int i = tid; i < ns; i += 128) M = fmaxf(M, slot(c0 + i)[p.G * D + 2 * g]);
-  M = warp_max(M);
-  if (lane == 0) top[warp] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  float L = 0.0f;
-  for (int i = tid; i < ns; i += 128) {
-    const float* ml = slot(c0 + i) + p.G * D + 2 * g;
-    const float f = exp2_from(ml[0], M);
-    wgt[i] = f;
-    L = fmaf(f, ml[1], L);
-  }
-  L = warp_sum(L);
-  if (lane == 0) tot[warp] = L;
-  __syncthreads();
-  constexpr int V = D / 32;
-  float acc[V];
+  // a CTA leaves its first segment in slot 0: the pair is that for all but, perhaps, c0
+  const int skip = pieces.begin(c0) < a ? 1 : 0;
+  auto slot = [&](int i) { return p.part + (int64_t(c0 + i) * 2 + (i == 0 ? skip : 0)) * stride; };
+  float M = -INFINITY, L = 0.0f, acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-  for (int i = warp; i < ns; i += 4) {
-    const float f = wgt[i];
-    const float* o = slot(c0 + i) + g * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(o);
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]);
-      acc[3] = fmaf(f, x.w, acc[3]);
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(o);
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
+  for (int base = warp; base < ns; base += 32 * NW) {  // lane j: segment base + j * NW
+    const int n = min(32, (ns - base + NW - 1) / NW);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(slot(base + lane * NW) + p.G * D + 2 * g);
+    float x[BATCH][V];
+    auto load = [&](int j0) {
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        if (j0 + j < n) {
+          const float* o = slot(base + (j0 + j) * NW) + g * D + lane * V;
+          if constexpr (V == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(o);
+            x[j][0] = y.x, x[j][1] = y.y, x[j][2] = y.z, x[j][3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(o);
+            x[j][0] = y.x, x[j][1] = y.y;
+          }
+        }
+      }
+    };
+    load(0);
+    const float f0 = raise_max(M, warp_max(ml.x)), f = exp2_from(ml.x, M);
+    L = fmaf(L, f0, warp_sum(f * ml.y));
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] *= f0;
+    for (int j0 = 0; j0 < n; j0 += BATCH) {
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+        if (j0 + j < n) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[j][i], acc[i]);
+        }
+      }
+      load(j0 + BATCH);
     }
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) red[warp][lane * V + i] = acc[i];
+  if (lane == 0) {
+    top[warp] = M;
+    tot[warp] = L;
+  }
   __syncthreads();
-  L = tot[0] + tot[1] + tot[2] + tot[3];
+  if (tid >= D) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, top[w]);
+  float O = 0.0f;
+  L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float f = exp2_from(top[w], M);
+    L = fmaf(f, tot[w], L);
+    O = fmaf(f, red[w][tid], O);
+  }
   if (p.sinks) L += exp2f(fmaf(__ldg(p.sinks + hq), 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  for (int d = tid; d < D; d += 128)
-    out[d] = Elt<E>::from_f32((red[0][d] + red[1][d] + red[2][d] + red[3][d]) * inv);
+  out[tid] = Elt<E>::from_f32(L == 0.0f ? 0.0f : O / L);
 }
 
 }  // namespace sd

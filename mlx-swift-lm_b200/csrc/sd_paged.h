@@ -11,6 +11,7 @@ namespace sd {
 
 constexpr int kPagedWarps = 4;                          // warps that attend
 constexpr int kPagedThreads = (kPagedWarps + 1) * 32;   // + one producer warp
+constexpr int kMergeThreads = 256;
 constexpr int kPagedMaxBatch = 4096;                    // sequences per decode call
 constexpr int kPagedMaxStages = 16;
 // Two CTAs share an SM: half of its 228 KB each, less 1 KB that every CTA reserves.
@@ -77,6 +78,22 @@ PagedSet paged_e2_b8(int D, int nb);
 
 // ---------------------------------------------------------------------------
 
+// n / d for 0 <= n < 2^31 by a multiplication: a hardware division costs tens
+// of instructions, and the row kernels would make several per row.
+struct FastDiv {
+  uint32_t mul, shift;
+  int d;
+  void set(int div) {
+    d = div;
+    shift = 0;
+    while ((uint64_t(1) << shift) < uint64_t(div)) ++shift;
+    mul = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - uint64_t(div))) / uint64_t(div) + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const { return int((__umulhi(uint32_t(n), mul) + uint32_t(n)) >> shift); }
+#endif
+};
+
 // Rows [batch, tokens, heads, D] with D contiguous; strides in elements.
 struct Rows {
   void* data;
@@ -86,16 +103,25 @@ struct Rows {
 struct RotaryParams {
   Rows q, k, v, q_out, k_out;
   int Hq, Hkv, Hv;          // heads of q, k and v rows per token (0: none)
-  int R;                    // Hq + Hkv + Hv
   int D, rot2;              // head_dim, rotated pairs (0: no rotation)
-  int traditional;
-  int L;                    // tokens per batch entry
-  int64_t tasks;            // batch * L * R
+  float inv_dim;            // 1 / D
+  FastDiv L;                // tokens per batch entry
+  FastDiv pairs;            // rot2
+  int n_tokens;             // batch * L
+  // The warps of each kind of rows (queries, keys, values): a warp takes
+  // 2^tok_log tokens and makes `span` of the passes over their heads.
+  struct Kind {
+    int first;              // first warp
+    int tok_log;
+    int span;               // passes that one warp makes
+    FastDiv per;            // warps per group of tokens
+  } kind[3];
+  int units;                // warps in all
+  int ring_at;              // byte offset of the row ring in shared memory
   const int* positions;     // [batch * L]
   const float* inv_freq;    // [rot2]
   const void *q_norm, *k_norm;
   float eps, factor;
-  int span;                 // tokens whose rows one block may touch
   // append: where the k and v rows go (null tables: k_out)
   const int* tables;
   const int* seq;
@@ -106,20 +132,20 @@ struct RotaryParams {
 };
 
 constexpr int kRotThreads = 128;
-constexpr int kRotUnroll = 4;  // rows in flight per group of lanes
+constexpr int kRotDepth = 4;          // passes whose rows are under way
+constexpr int kRotPasses = 16;        // most passes that one warp makes
+constexpr int kRotFill = 2048;        // warps that fill the GPU
 // Lanes per row (log2): a power of two with a chunk pair of 2 * vec elements for each, at most a warp.
 __host__ __device__ constexpr int rotary_lanes_log(int D, int vec) {
   int l = 0;
   while (l < 5 && (1 << l) < D / (2 * vec)) ++l;
   return l;
 }
-// Shared floats before the staged rows: cos and sin of `span` tokens, two norms.
-__host__ __device__ constexpr int rotary_stage_at(int span, int rot2, int D) {
-  return (span * 2 * rot2 + 2 * D + 3) / 4 * 4;
-}
+// Floats of a cos (or sin) row in shared memory: whole 16-byte pieces.
+__host__ __device__ constexpr int rotary_pitch(int rot2) { return (rot2 + 7) / 8 * 8; }
 
 // vec: elements per access (1, 2, 4, 8 for 16-bit types; 1, 2, 4 for fp32); null if not instantiated.
-const void* rotary_kernel_for(int dtype, int bits, int vec);
+const void* rotary_kernel_for(int dtype, int bits, int vec, bool traditional);
 
 struct CopyParams {
   const int *src, *dst;

@@ -97,8 +97,8 @@ int32_t sm_count(int* n) {
   return SD_OK;
 }
 
-// CTAs of a decode launch: two per SM; paged_merge_kernel's weights hold 512.
-int decode_ctas(int sms) { return std::min(2 * sms, 512); }
+// CTAs of a decode launch: two per SM, all resident.
+int decode_ctas(int sms) { return 2 * sms; }
 
 // The launches here may begin while the kernel before them on the stream
 // ends (programmatic dependent launch); every kernel waits for it
@@ -147,7 +147,7 @@ void limit_vec(const sd::Rows& r, int heads, int esize, int* vec) {
   while (*vec > 1 && (misaligned(r.data, size_t(*vec) * esize) || r.batch % *vec || r.token % *vec || r.head % *vec)) *vec /= 2;
 }
 
-int32_t launch_rotary(sd::RotaryParams& p, int dtype, int bits, cudaStream_t st) {
+int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, int dtype, int bits, cudaStream_t st) {
   const int es = elt_size(dtype);
   int vec = 16 / es;
   limit_vec(p.q, p.Hq, es, &vec);
@@ -155,19 +155,39 @@ int32_t launch_rotary(sd::RotaryParams& p, int dtype, int bits, cudaStream_t st)
   limit_vec(p.k, p.Hkv, es, &vec);
   limit_vec(p.v, p.Hv, es, &vec);
   if (!p.tables) limit_vec(p.k_out, p.Hkv, es, &vec);
-  // chunk pairs must tile the head, and in the half layout the rotated halves
-  while (vec > 1 && (p.D % (2 * vec) || (!p.traditional && p.rot2 % vec))) vec /= 2;
-  const int lanes = 1 << sd::rotary_lanes_log(p.D, vec);
-  const int rows = sd::kRotThreads / lanes * sd::kRotUnroll;
-  p.R = p.Hq + p.Hkv + p.Hv;
-  if (p.tasks >= (int64_t(1) << 31) * rows) return fail(SD_ERR_SHAPE, "too many rows (%lld)", (long long)p.tasks);
-  p.span = (rows - 1) / p.R + 2;
-  if (p.span > rows) p.span = rows;
-  const size_t smem = size_t(sd::rotary_stage_at(p.span, p.rot2, p.D)) * 4 + (bits ? size_t(rows) * p.D * es : 0);
-  const void* fn = sd::rotary_kernel_for(dtype, bits, vec);
-  if (smem > 48 * 1024) SD_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  // chunk pairs must tile the head and its rotated part
+  while (vec > 1 && (p.D % (2 * vec) || p.rot2 % vec)) vec /= 2;
+  const int lg_log = sd::rotary_lanes_log(p.D, vec), groups = 32 >> lg_log, warps = sd::kRotThreads / 32;
+  // A warp's groups of lanes each take one row per pass. The more passes a
+  // warp makes, the more rows share its cos, sin and weights; the fewer, the
+  // more warps there are. So: as many as leave about kRotFill warps, at most
+  // kRotPasses, over more than one token where the heads are few.
+  const int heads[3] = {p.Hq, p.Hkv, p.Hv};
+  const int64_t passes = n_tokens * (p.Hq + p.Hkv + p.Hv) / groups;
+  const int span = int(std::min<int64_t>(sd::kRotPasses, std::max<int64_t>(1, passes / sd::kRotFill)));
+  int64_t units = 0;
+  for (int i = 0; i < 3; ++i) {
+    sd::RotaryParams::Kind& k = p.kind[i];
+    k.first = int(units);
+    k.tok_log = 0;
+    while ((2 << k.tok_log) <= groups && heads[i] * (2 << k.tok_log) <= span * groups) ++k.tok_log;
+    const int step = groups >> k.tok_log, per = ((heads[i] + step - 1) / step + span - 1) / span;
+    k.span = span;
+    k.per.set(std::max(per, 1));
+    units += ((n_tokens + (1 << k.tok_log) - 1) >> k.tok_log) * per;
+    if (units >= (int64_t(1) << 31) - warps - 64)
+      return fail(SD_ERR_SHAPE, "a call takes fewer than 2^31 rows (got %lld tokens)", (long long)n_tokens);
+  }
+  p.units = int(units);
+  p.n_tokens = int(n_tokens);
+  p.pairs.set(std::max(p.rot2, 1));
+  p.inv_dim = 1.0f / float(p.D);
+  p.ring_at = (warps * groups * (2 * sd::rotary_pitch(p.rot2) * 4 + (bits ? p.D * es : 0)) + 15) / 16 * 16;
+  const int per_lane = (vec >= 4 ? 1 : vec == 2 ? 2 : 4) * 2 * vec * es;
+  const size_t smem = size_t(p.ring_at) + size_t(warps) * sd::kRotDepth * 32 * per_lane;
+  const void* fn = sd::rotary_kernel_for(dtype, bits, vec, traditional);
   void* args[1] = {&p};
-  return launch(fn, dim3(unsigned((p.tasks + rows - 1) / rows)), sd::kRotThreads, smem, st, args);
+  return launch(fn, dim3(unsigned((p.units + warps - 1) / warps)), sd::kRotThreads, smem, st, args);
 }
 
 void set_rotation(sd::RotaryParams& p, const sd_rotation* rot) {
@@ -177,7 +197,6 @@ void set_rotation(sd::RotaryParams& p, const sd_rotation* rot) {
   p.eps = rot->eps;
   p.factor = rot->factor;
   p.rot2 = rot->rot_dim / 2;
-  p.traditional = rot->traditional ? 1 : 0;
 }
 
 }  // namespace
@@ -208,11 +227,10 @@ int32_t sd_rotary(const sd_rotation* rot, int32_t dtype, int32_t head_dim, int32
   p.Hq = n_q_heads;
   p.Hkv = n_kv_heads;
   p.D = head_dim;
-  p.L = tokens;
-  p.tasks = int64_t(batch) * tokens * (p.Hq + p.Hkv);
+  p.L.set(tokens);
   p.positions = positions;
   set_rotation(p, rot);
-  return launch_rotary(p, dtype, 0, static_cast<cudaStream_t>(stream));
+  return launch_rotary(p, int64_t(batch) * tokens, rot->traditional != 0, dtype, 0, static_cast<cudaStream_t>(stream));
 }
 
 int32_t sd_paged_append(const sd_pages* g, int32_t layer, int32_t n_tokens, const sd_rows* k, const sd_rows* v,
@@ -242,8 +260,7 @@ int32_t sd_paged_append(const sd_pages* g, int32_t layer, int32_t n_tokens, cons
   p.Hq = n_q_heads;
   p.Hkv = p.Hv = g->n_kv_heads;
   p.D = g->head_dim;
-  p.L = n_tokens;
-  p.tasks = int64_t(n_tokens) * (p.Hq + 2 * p.Hkv);
+  p.L.set(n_tokens);
   p.positions = positions;
   if (rot) set_rotation(p, rot);
   p.tables = tables;
@@ -263,7 +280,7 @@ int32_t sd_paged_append(const sd_pages* g, int32_t layer, int32_t n_tokens, cons
     p.v_biases = at(g->v_biases, rows * sb_bytes(g));
   }
   p.flags = device_flags;
-  return launch_rotary(p, g->dtype, g->kv_bits, static_cast<cudaStream_t>(stream));
+  return launch_rotary(p, n_tokens, rot && rot->traditional, g->dtype, g->kv_bits, static_cast<cudaStream_t>(stream));
 }
 
 int32_t sd_copy_pages(const sd_pages* g, const int32_t* src, const int32_t* dst, int32_t n, int32_t* device_flags,
@@ -344,7 +361,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   const sd::PagedSet ks = lookup(g->dtype, g->kv_bits, D, G <= 8 ? 1 : 2);
   if (!ks.decode) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   const int64_t max_tiles = (int64_t(table_width) * g->page_size + ks.tile - 1) / ks.tile;
-  if (max_tiles * batch >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "batch * table_width too large");
+  if (max_tiles * batch * g->n_kv_heads >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "batch * table_width too large");
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
   const int max_ctas = decode_ctas(sms);
@@ -405,7 +422,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   void* args[3] = {&p, &tmK, &tmV};
   if (int32_t rc = launch(ks.decode, dim3(unsigned(p.ncta)), sd::kPagedThreads, smem, st, args)) return rc;
   void* margs[1] = {&p};
-  return launch(ks.merge, dim3(unsigned(batch) * unsigned(n_q_heads)), 128, 0, st, margs);
+  return launch(ks.merge, dim3(unsigned(batch) * unsigned(n_q_heads)), sd::kMergeThreads, 0, st, margs);
 }
 
 }  // extern "C"

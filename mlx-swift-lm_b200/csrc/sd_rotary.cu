@@ -31,243 +31,283 @@ template <> struct Chunk<2> { using T = uint16_t; };
 template <typename E, int V> union Pack {
   typename Chunk<V * sizeof(E)>::T raw;
   E e[V];
+  uint32_t word[V * sizeof(E) / 4 ? V * sizeof(E) / 4 : 1];
   __device__ Pack() {}
+  __device__ __forceinline__ void zero() { memset(&raw, 0, sizeof(raw)); }
+  __device__ __forceinline__ void unpack(float* f) const {
+    if constexpr (sizeof(E) == 2 && V >= 2) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) unpack_word<E>(word[i], f + 2 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = Elt<E>::to_f32(e[i]);
+    }
+  }
+  __device__ __forceinline__ void pack(const float* f) {
+    if constexpr (sizeof(E) == 2 && V >= 2) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) word[i] = pack2<E>(f[2 * i], f[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = Elt<E>::from_f32(f[i]);
+    }
+  }
 };
 
+// Copy one chunk to shared memory, asynchronously where its size allows.
+template <int BYTES>
+__device__ __forceinline__ void copy_chunk(void* dst, const void* src) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  } else if constexpr (BYTES >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+  } else {
+    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+  }
+}
 
 }  // namespace
 
-// One group of lanes per row; a lane holds chunk pairs of V elements: pair j
-// is the elements [jV, jV + V) of the first rotated half and the same of the
-// second, or 2V neighbours (traditional layout, and past the rotated part).
-// So a lane always holds both elements of a rotation and needs no exchange.
-// A block takes kRotUnroll rows per group, consecutive in (token, head)
-// order, loads them all first, and while they are under way puts cos and sin
-// of its few tokens into shared memory: one sincos per token and pair instead
-// of one per row. BITS 4 / 8: k and v rows are rounded to E, staged in shared
-// memory and quantized from there a warp per row.
-template <typename E, int V, int BITS>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+// A warp takes rows of one kind (query, key or value) and of few tokens: a
+// group of lanes holds one row at a time and stays with one token, so what
+// depends on the position and the weights is computed once and stays in
+// registers. With the norm's weights w folded into cos and sin, a rotation is
+//   a' = inv * (a (w_a cos) - b (w_b sin)),  b' = inv * (b (w_b cos) + a (w_a sin)),
+// inv = the row's 1 / rms. A lane holds chunk pairs of V elements: pair j is
+// the elements [jV, jV + V) of the first rotated half and the same of the
+// second, or 2V neighbours (traditional layout, and past the rotated part), so
+// both elements of a rotation are in one lane. Rows are copied kRotDepth passes
+// ahead into shared memory (each lane its own chunks, so nothing waits for
+// another lane); while the first are under way the warp computes its tokens'
+// cos and sin, one pair per lane, and exchanges them through shared memory.
+// No barrier wider than a warp.
+// BITS 4 / 8: key and value rows are rounded to E, staged in shared memory and
+// quantized from there, a warp per row.
+template <typename E, int V, int BITS, bool TRAD>
+__global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int CPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // chunk pairs per lane for head_dim up to 256
   using P = Pack<E, V>;
-  extern __shared__ float smem[];
-  float* cs = smem;                                  // [span][2][rot2]
-  float* wn = cs + int64_t(p.span) * 2 * p.rot2;     // [2][D] norm weights
-  E* stage = reinterpret_cast<E*>(smem + rotary_stage_at(p.span, p.rot2, p.D));  // [rows per block][D] (BITS)
+  extern __shared__ __align__(16) float smem[];
   const int D = p.D, pairs = D / (2 * V), lg_log = rotary_lanes_log(D, V), lg = 1 << lg_log;
-  const int groups = kRotThreads >> lg_log, rows = groups * kRotUnroll;
-  const int tid = threadIdx.x, sub = tid & (lg - 1), grp = tid >> lg_log;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (lg - 1), grp = lane >> lg_log;
+  const int groups = 32 >> lg_log, pitch = rotary_pitch(p.rot2);
+  float* cs = smem + warp * groups * 2 * pitch;      // [tokens of this warp][cos, sin]
+  E* stage = reinterpret_cast<E*>(smem + kRotThreads / 32 * groups * 2 * pitch) + warp * groups * D;
   griddep_launch_dependents();
   griddep_wait();
 
-  const int64_t task0 = int64_t(blockIdx.x) * rows;
-  const int64_t n0 = task0 / p.R;
-  const int rem0 = int(task0 - n0 * p.R);
-  const int half = p.traditional ? 0 : p.rot2 / V;   // chunk pairs that straddle the two halves
-
+  const int unit = blockIdx.x * (kRotThreads / 32) + warp;
+  if (unit >= p.units) return;
+  const bool is_v = unit >= p.kind[2].first, is_q = unit < p.kind[1].first;
+  const RotaryParams::Kind& kd_ = p.kind[is_q ? 0 : is_v ? 2 : 1];
+  const Rows& in = is_q ? p.q : is_v ? p.v : p.k;
+  const int heads = is_q ? p.Hq : is_v ? p.Hv : p.Hkv;
+  const int chunk = kd_.per(unit - kd_.first), first_pass = (unit - kd_.first - chunk * kd_.per.d) * kd_.span;
+  // group g: token g mod 2^tok_log of the chunk, heads g / 2^tok_log, + step, ...
+  const int tl = kd_.tok_log, step = groups >> tl, n0 = chunk << tl;
+  const int n = n0 + (grp & ((1 << tl) - 1));
+  const bool here = n < p.n_tokens;
+  const int bt = p.L(n), tk = n - bt * p.L.d;
+  const int half = TRAD ? 0 : p.rot2 / V;            // chunk pairs that straddle the two halves
   // Element offset of chunk i (0, 1) of pair j.
   auto place = [&](int j, int i) { return j < half ? j * V + i * p.rot2 : 2 * j * V + i * V; };
+  const E* src = static_cast<const E*>(in.data) + bt * in.batch + tk * in.token;
 
-  P x[kRotUnroll][CPL][2];
+  // where key and value rows go: a page slot (the same for every head), or k_out
+  E* paged = nullptr;
+  int64_t slot = -1;  // row of head 0; head h is h * P rows on
+  bool store = here;
+  if (!is_q && p.tables) {
+    paged = static_cast<E*>(is_v ? p.v_data : p.k_data);
+    const int pos = here ? __ldg(p.positions + n) : -1, sq = here && p.seq ? __ldg(p.seq + n) : n;
+    store = pos >= 0;  // else padding
+    if (store) {
+      const int col = pos >> p.page_shift;
+      const int page = sq >= 0 && sq < p.B && col < p.W ? __ldg(p.tables + int64_t(sq) * p.W + col) : -1;
+      if (page >= 0 && page < p.n_pages) {
+        slot = int64_t(page) * p.Hkv * p.P + (pos & (p.P - 1));
+      } else {
+        store = false;
+        if (p.flags && sub == 0) atomicOr(p.flags, kErrBadIndex);
+      }
+    }
+  }
+  const Rows& outr = is_q ? p.q_out : p.k_out;
+  E* out = static_cast<E*>(outr.data) + bt * outr.batch + tk * outr.token;
+
+  const E* w = is_v ? nullptr : static_cast<const E*>(is_q ? p.q_norm : p.k_norm);
+  const int last = min(heads, (first_pass + kd_.span) * step);  // heads of this warp end here
+  int hd = first_pass * step + (grp >> tl);
+  // Rows under way: every lane copies its own chunks, kRotDepth passes ahead, and reads back only those.
+  constexpr int BYTES = V * int(sizeof(E)), PASS = CPL * 2 * 32 * BYTES;  // of one warp and pass
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem) + p.ring_at + warp * kRotDepth * PASS + lane * BYTES;
+  const E* from = src + hd * in.head;  // the row to load next
+  const int64_t from_step = step * in.head;
+  int ahead = hd;
+  auto fetch = [&](int st) {
+    if (here && ahead < last) {
 #pragma unroll
-  for (int u = 0; u < kRotUnroll; ++u) {
-    const int local = u * groups + grp;
-    if (task0 + local >= p.tasks) continue;
-    const int k = (rem0 + local) / p.R, r = rem0 + local - k * p.R;
-    const int64_t n = n0 + k;
-    const int64_t bt = n / p.L, t = n - bt * p.L;
-    const Rows& s = r < p.Hq ? p.q : r < p.Hq + p.Hkv ? p.k : p.v;
-    const int hd = r < p.Hq ? r : r < p.Hq + p.Hkv ? r - p.Hq : r - p.Hq - p.Hkv;
-    const E* src = static_cast<const E*>(s.data) + bt * s.batch + t * s.token + hd * s.head;
+      for (int c = 0; c < CPL; ++c) {
+        const int j = c * lg + sub;
+        if (j < pairs) {
+          copy_chunk<BYTES>(ring + st * PASS + (2 * c) * 32 * BYTES, from + place(j, 0));
+          copy_chunk<BYTES>(ring + st * PASS + (2 * c + 1) * 32 * BYTES, from + place(j, 1));
+        }
+      }
+    }
+    cp_async_commit();
+    from += from_step;
+    ahead += step;
+  };
+#pragma unroll
+  for (int st = 0; st < kRotDepth; ++st) fetch(st);
+  E* dst = BITS != 0 && paged ? stage + grp * D : paged ? paged + (slot + int64_t(hd) * p.P) * D : out + hd * outr.head;
+  const int64_t dst_step = BITS != 0 && paged ? 0 : paged ? int64_t(step) * p.P * D : step * outr.head;
+
+  // coefficients of this lane's pairs: wa cos, wb sin, wb cos, wa sin; wa and wb alone past the rotated part
+  float ka[CPL][V], kb[CPL][V], kc[CPL][V], kd[CPL][V];
+  bool turned[CPL];  // the host picks V so that a lane's V pairs are rotated all or none
+  if (!is_v) {
+    for (int i = lane; i < p.rot2 << tl; i += 32) {
+      const int t = p.pairs(i), f = i - t * p.rot2;
+      // turns of the angle, less whole turns
+      const double pos = n0 + t < p.n_tokens ? double(__ldg(p.positions + n0 + t)) : 0.0;
+      double turns = pos * (double(__ldg(p.inv_freq + f)) * 0.15915494309189535);
+      turns -= rint(turns);
+      float sn, c;
+      sincospif(2.0f * float(turns), &sn, &c);
+      cs[2 * t * pitch + f] = c * p.factor;
+      cs[(2 * t + 1) * pitch + f] = sn * p.factor;
+    }
+    __syncwarp();
+    const float* co_row = cs + 2 * (n - n0) * pitch;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       const int j = c * lg + sub;
-      if (j < pairs) {
-        x[u][c][0].raw = *reinterpret_cast<const decltype(P::raw)*>(src + place(j, 0));
-        x[u][c][1].raw = *reinterpret_cast<const decltype(P::raw)*>(src + place(j, 1));
+      turned[c] = j * V < p.rot2;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int ia = TRAD ? 2 * e : e, ib = TRAD ? 2 * e + 1 : V + e;  // within the two chunks
+        float wa = 1.0f, wb = 1.0f, co = 1.0f, si = 0.0f;
+        if (w && j < pairs) {
+          wa = Elt<E>::to_f32(w[place(j, ia / V) + ia % V]);
+          wb = Elt<E>::to_f32(w[place(j, ib / V) + ib % V]);
+        }
+        if (turned[c]) {
+          co = co_row[j * V + e];
+          si = co_row[pitch + j * V + e];
+        }
+        ka[c][e] = wa * co;
+        kb[c][e] = wb * si;
+        kc[c][e] = wb * co;
+        kd[c][e] = wa * si;
       }
     }
   }
 
-  if (p.rot2) {
-    const int64_t last = min(task0 + rows, p.tasks) - 1;
-    const int span = int(last / p.R - n0) + 1;
-    for (int i = tid; i < span * p.rot2; i += kRotThreads) {
-      const int k = i / p.rot2, f = i - k * p.rot2;
-      // turns of the angle, less whole turns
-      double turns = double(__ldg(p.positions + n0 + k)) * (double(__ldg(p.inv_freq + f)) * 0.15915494309189535);
-      turns -= rint(turns);
-      float sn, c;
-      sincospif(2.0f * float(turns), &sn, &c);
-      cs[(2 * k) * p.rot2 + f] = c * p.factor;
-      cs[(2 * k + 1) * p.rot2 + f] = sn * p.factor;
+  int st = 0;
+#pragma unroll 1
+  for (int pass = first_pass * step; pass < last; pass += step, hd += step, dst += dst_step) {
+    const bool live = store && hd < last;
+    cp_async_wait<kRotDepth - 1>();
+    P x[CPL][2];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      x[c][0].zero(), x[c][1].zero();
+      if (c * lg + sub < pairs) {
+        x[c][0].raw = *reinterpret_cast<const decltype(P::raw)*>(ring + st * PASS + (2 * c) * 32 * BYTES);
+        x[c][1].raw = *reinterpret_cast<const decltype(P::raw)*>(ring + st * PASS + (2 * c + 1) * 32 * BYTES);
+      }
     }
-  }
-  if (p.q_norm)
-    for (int i = tid; i < D; i += kRotThreads) wn[i] = Elt<E>::to_f32(static_cast<const E*>(p.q_norm)[i]);
-  if (p.k_norm)
-    for (int i = tid; i < D; i += kRotThreads) wn[D + i] = Elt<E>::to_f32(static_cast<const E*>(p.k_norm)[i]);
-  __syncthreads();
-
+    fetch(st);
+    st = st + 1 == kRotDepth ? 0 : st + 1;
+    float f[CPL][2 * V], inv = 1.0f;
 #pragma unroll
-  for (int u = 0; u < kRotUnroll; ++u) {
-    const int local = u * groups + grp;
-    const bool live = task0 + local < p.tasks;
-    const int k = (rem0 + local) / p.R, r = rem0 + local - k * p.R;
-    const int64_t n = n0 + k;
-    const bool is_q = r < p.Hq, is_v = r >= p.Hq + p.Hkv;
-    const int hd = is_q ? r : is_v ? r - p.Hq - p.Hkv : r - p.Hq;
-    float f[CPL][2][V];
-#pragma unroll
-    for (int c = 0; c < CPL; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[c][i][e] = live && c * lg + sub < pairs ? Elt<E>::to_f32(x[u][c][i].e[e]) : 0.0f;
-    if (p.q_norm || p.k_norm) {  // every lane of the warp takes part in the shuffles
+    for (int c = 0; c < CPL; ++c) {
+      x[c][0].unpack(f[c]);
+      x[c][1].unpack(f[c] + V);
+    }
+    if (w) {  // every lane of the warp takes part in the shuffles, each within its row's group
       float sq = 0.0f;
 #pragma unroll
       for (int c = 0; c < CPL; ++c)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < V; ++e) sq = fmaf(f[c][i][e], f[c][i][e], sq);
+        for (int e = 0; e < 2 * V; ++e) sq = fmaf(f[c][e], f[c][e], sq);
       for (int o = 1; o < lg; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-      if (!is_v && (is_q ? p.q_norm : p.k_norm)) {
-        const float inv = rsqrtf(sq / float(D) + p.eps);
-        const float* w = wn + (is_q ? 0 : D);
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const int j = c * lg + sub;
-          if (j < pairs) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int e = 0; e < V; ++e) f[c][i][e] *= inv * w[place(j, i) + e];
-          }
-        }
-      }
+      inv = rsqrtf(sq * p.inv_dim + p.eps);
     }
-    if (!live) continue;
-    if (!is_v && p.rot2) {
-      const float *co = cs + 2 * k * p.rot2, *si = co + p.rot2;
+    if (live) {
 #pragma unroll
       for (int c = 0; c < CPL; ++c) {
         const int j = c * lg + sub;
         if (j < pairs) {
-          if (p.traditional) {
-            // the 2V neighbours are V whole pairs
-            float z[2 * V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) z[e] = f[c][0][e], z[V + e] = f[c][1][e];
+          P y[2] = {x[c][0], x[c][1]};  // values are stored as they came
+          if (!is_v) {
+            float r[2 * V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const int i = j * V + e;
-              if (i < p.rot2) {
-                const float a = z[2 * e], b = z[2 * e + 1];
-                z[2 * e] = fmaf(a, co[i], -b * si[i]);
-                z[2 * e + 1] = fmaf(b, co[i], a * si[i]);
+              const int ia = TRAD ? 2 * e : e, ib = TRAD ? 2 * e + 1 : V + e;
+              const float a = f[c][ia] * inv, b = f[c][ib] * inv;
+              r[ia] = a * ka[c][e];
+              r[ib] = b * kc[c][e];
+              if (turned[c]) {  // not by zeros: 0 * inf would reach the other element
+                r[ia] = fmaf(-b, kb[c][e], r[ia]);
+                r[ib] = fmaf(a, kd[c][e], r[ib]);
               }
             }
-#pragma unroll
-            for (int e = 0; e < V; ++e) f[c][0][e] = z[e], f[c][1][e] = z[V + e];
-          } else if (j < half) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float a = f[c][0][e], b = f[c][1][e];
-              f[c][0][e] = fmaf(a, co[j * V + e], -b * si[j * V + e]);
-              f[c][1][e] = fmaf(b, co[j * V + e], a * si[j * V + e]);
-            }
+            y[0].pack(r);
+            y[1].pack(r + V);
           }
+          *reinterpret_cast<decltype(P::raw)*>(dst + place(j, 0)) = y[0].raw;
+          *reinterpret_cast<decltype(P::raw)*>(dst + place(j, 1)) = y[1].raw;
         }
       }
     }
-    // where the row goes
-    E* dst = nullptr;
-    if (is_q || !p.tables) {
-      const Rows& o = is_q ? p.q_out : p.k_out;
-      const int64_t bt = n / p.L, t = n - bt * p.L;
-      dst = static_cast<E*>(o.data) + bt * o.batch + t * o.token + hd * o.head;
-    } else if (BITS != 0) {
-      dst = stage + local * D;
-    } else {
-      const int pos = __ldg(p.positions + n), sq = p.seq ? __ldg(p.seq + n) : int(n);
-      if (pos >= 0) {
-        const int slot = pos >> p.page_shift;
-        const int page = sq >= 0 && sq < p.B && slot < p.W ? __ldg(p.tables + int64_t(sq) * p.W + slot) : -1;
-        if (page >= 0 && page < p.n_pages) {
-          dst = static_cast<E*>(is_v ? p.v_data : p.k_data) +
-                ((int64_t(page) * p.Hkv + hd) * p.P + (pos & (p.P - 1))) * D;
-        } else if (p.flags) {
-          atomicOr(p.flags, kErrBadIndex);
+    if constexpr (BITS != 0) {
+      if (paged) {
+        __syncwarp();
+        const int NG = D / 64, words = D * BITS / 32;
+        for (int g = 0; g < groups; ++g) {  // the row that group g staged
+          const int64_t s0 = __shfl_sync(0xffffffffu, live ? slot + int64_t(hd) * p.P : int64_t(-1), g << lg_log);
+          if (s0 < 0) continue;
+          uint32_t* wq = static_cast<uint32_t*>(is_v ? p.v_data : p.k_data) + s0 * words;
+          E* sc = static_cast<E*>(is_v ? p.v_scales : p.k_scales) + s0 * NG;
+          E* bi = static_cast<E*>(is_v ? p.v_biases : p.k_biases) + s0 * NG;
+          if (D == 128) quantize_row_warp<E, BITS, 128>(stage + g * D, wq, sc, bi, lane);
+          else quantize_row_warp<E, BITS, 64>(stage + g * D, wq, sc, bi, lane);
         }
-      }
-    }
-    if (dst) {
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const int j = c * lg + sub;
-        if (j < pairs) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            P y;
-#pragma unroll
-            for (int e = 0; e < V; ++e) y.e[e] = is_v ? x[u][c][i].e[e] : Elt<E>::from_f32(f[c][i][e]);
-            *reinterpret_cast<decltype(P::raw)*>(dst + place(j, i)) = y.raw;
-          }
-        }
+        __syncwarp();
       }
     }
   }
-
-  if constexpr (BITS != 0) {
-    __syncthreads();
-    const int warp = tid >> 5, lane = tid & 31, NG = D / 64, words = D * BITS / 32;
-    for (int local = warp; local < rows && task0 + local < p.tasks; local += kRotThreads / 32) {
-      const int k = (rem0 + local) / p.R, r = rem0 + local - k * p.R;
-      if (r < p.Hq) continue;
-      const int64_t n = n0 + k;
-      const int pos = __ldg(p.positions + n), sq = p.seq ? __ldg(p.seq + n) : int(n);
-      if (pos < 0) continue;
-      const int slot = pos >> p.page_shift;
-      const int page = sq >= 0 && sq < p.B && slot < p.W ? __ldg(p.tables + int64_t(sq) * p.W + slot) : -1;
-      if (page < 0 || page >= p.n_pages) {
-        if (p.flags && lane == 0) atomicOr(p.flags, kErrBadIndex);
-        continue;
-      }
-      const bool is_v = r >= p.Hq + p.Hkv;
-      const int hd = is_v ? r - p.Hq - p.Hkv : r - p.Hq;
-      const int64_t row = (int64_t(page) * p.Hkv + hd) * p.P + (pos & (p.P - 1));
-      uint32_t* wq = static_cast<uint32_t*>(is_v ? p.v_data : p.k_data) + row * words;
-      E* sc = static_cast<E*>(is_v ? p.v_scales : p.k_scales) + row * NG;
-      E* bi = static_cast<E*>(is_v ? p.v_biases : p.k_biases) + row * NG;
-      const E* src = stage + local * D;
-      if (D == 128) quantize_row_warp<E, BITS, 128>(src, wq, sc, bi, lane);
-      else quantize_row_warp<E, BITS, 64>(src, wq, sc, bi, lane);
-    }
-  }
+  cp_async_wait<0>();
 }
 
-template <typename E, int BITS>
+template <typename E, int BITS, bool TRAD>
 static const void* rotary_pick(int vec) {
   switch (vec) {
     case 8:
-      if constexpr (sizeof(E) == 2) return reinterpret_cast<const void*>(&rotary_kernel<E, 8, BITS>);
+      if constexpr (sizeof(E) == 2) return reinterpret_cast<const void*>(&rotary_kernel<E, 8, BITS, TRAD>);
       return nullptr;
-    case 4: return reinterpret_cast<const void*>(&rotary_kernel<E, 4, BITS>);
-    case 2: return reinterpret_cast<const void*>(&rotary_kernel<E, 2, BITS>);
-    case 1: return reinterpret_cast<const void*>(&rotary_kernel<E, 1, BITS>);
+    case 4: return reinterpret_cast<const void*>(&rotary_kernel<E, 4, BITS, TRAD>);
+    case 2: return reinterpret_cast<const void*>(&rotary_kernel<E, 2, BITS, TRAD>);
+    case 1: return reinterpret_cast<const void*>(&rotary_kernel<E, 1, BITS, TRAD>);
     default: return nullptr;
   }
 }
-template <typename E>
+template <typename E, bool TRAD>
 static const void* rotary_bits(int bits, int vec) {
-  return bits == 0 ? rotary_pick<E, 0>(vec) : bits == 4 ? rotary_pick<E, 4>(vec) : rotary_pick<E, 8>(vec);
+  return bits == 0 ? rotary_pick<E, 0, TRAD>(vec) : bits == 4 ? rotary_pick<E, 4, TRAD>(vec) : rotary_pick<E, 8, TRAD>(vec);
+}
+template <typename E>
+static const void* rotary_layout(int bits, int vec, bool trad) {
+  return trad ? rotary_bits<E, true>(bits, vec) : rotary_bits<E, false>(bits, vec);
 }
 
-const void* rotary_kernel_for(int dtype, int bits, int vec) {
-  return dtype == 0 ? rotary_bits<float>(bits, vec) : dtype == 1 ? rotary_bits<__half>(bits, vec)
-                                                                 : rotary_bits<__nv_bfloat16>(bits, vec);
+const void* rotary_kernel_for(int dtype, int bits, int vec, bool traditional) {
+  return dtype == 0   ? rotary_layout<float>(bits, vec, traditional)
+         : dtype == 1 ? rotary_layout<__half>(bits, vec, traditional)
+                      : rotary_layout<__nv_bfloat16>(bits, vec, traditional);
 }
 
 // Page dst[i] = page src[i] in every array and layer: a pure copy, bound by

@@ -21,28 +21,37 @@ caller, as for any torch operation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence
 
 from . import DTYPES, SDError, SDPages, SDRotation, SDRows, _check, _torch_dtype, lib
 
-_DTYPE_CODE: dict = {}
+# torch, its names used per call and the library, bound at the first call: the
+# calls here take a few microseconds on the GPU, so the host's share counts.
+torch = None
+_device = _raw_stream = None
+_CODE: dict = {}
+_I32 = _F32 = None
+_L: Optional[ctypes.CDLL] = None
+
+
+def _load() -> None:
+    global torch, _device, _raw_stream, _I32, _F32, _L
+    import torch as t
+    _L = lib()
+    t.cuda.init()
+    _device, _raw_stream = t.cuda.current_device, t._C._cuda_getCurrentRawStream
+    _I32, _F32 = t.int32, t.float32
+    _CODE.update({_torch_dtype(n): c for n, c in DTYPES.items()})
+    torch = t
 
 
 def _dtype_code(dtype) -> int:
-    if not _DTYPE_CODE:
-        _DTYPE_CODE.update({_torch_dtype(n): c for n, c in DTYPES.items()})
-    code = _DTYPE_CODE.get(dtype)
+    code = _CODE.get(dtype)
     if code is None:
         raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
     return code
-
-
-def _device() -> int:
-    import torch
-    return torch.cuda.current_device()
 
 
 def _arg(t, name: str, dtype, dev: int, shape=None) -> Optional[int]:
@@ -51,11 +60,11 @@ def _arg(t, name: str, dtype, dev: int, shape=None) -> Optional[int]:
         return None
     if t.get_device() != dev:
         raise ValueError(f"{name} must be a CUDA tensor on the current device")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
     return t.data_ptr()
 
@@ -65,40 +74,40 @@ def _rows(t, name: str, dtype, dev: int, dim: int) -> tuple:
     strides but the last, as (struct, batch, tokens, heads)."""
     if t.get_device() != dev:
         raise ValueError(f"{name} must be a CUDA tensor on the current device")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
     shape, st = t.shape, t.stride()
-    if len(shape) == 3:
-        n, h, d = shape
-        b, s = 1, (0, st[0], st[1])
-    elif len(shape) == 4:
-        b, h, n, d = shape
-        s = (st[0], st[2], st[1])
-    else:
-        raise ValueError(f"{name} must be [tokens, heads, D] or [batch, heads, tokens, D]")
-    if d != dim:
-        raise ValueError(f"{name} has head_dim {d}, expected {dim}")
-    if st[-1] != 1 and d != 1:
+    if shape[-1] != dim:
+        raise ValueError(f"{name} has head_dim {shape[-1]}, expected {dim}")
+    if st[-1] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    return SDRows(t.data_ptr(), *s), b, n, h
+    if len(shape) == 3:
+        return SDRows(t.data_ptr(), 0, st[0], st[1]), 1, shape[0], shape[1]
+    if len(shape) == 4:
+        return SDRows(t.data_ptr(), st[0], st[2], st[1]), shape[0], shape[2], shape[1]
+    raise ValueError(f"{name} must be [tokens, heads, D] or [batch, heads, tokens, D]")
 
 
-def _handle(stream):
-    """(cudaStream_t, context that allocates for it)."""
-    import torch
+def _like(x, stream):
+    """A new dense tensor of x's shape for work on `stream`."""
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream, contextlib.nullcontext()
-    return stream.cuda_stream, torch.cuda.stream(stream)
+        y = torch.empty_like(x)
+        return y if y.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with torch.cuda.stream(stream):
+        return _like(x, None)
+
+
+def _handle(stream, dev: int) -> int:
+    return _raw_stream(dev) if stream is None else stream.cuda_stream
 
 
 def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: int, dim: int) -> SDRotation:
-    import torch
     rot = 0
     if inv_freq is not None:
         if inv_freq.dim() != 1:
             raise ValueError("inv_freq must be [rot_dim / 2]")
         rot = 2 * inv_freq.shape[0]
-    return SDRotation(_arg(inv_freq, "inv_freq", torch.float32, dev), _arg(q_norm, "q_norm", dtype, dev, (dim,)),
+    return SDRotation(_arg(inv_freq, "inv_freq", _F32, dev), _arg(q_norm, "q_norm", dtype, dev, (dim,)),
                       _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
 
 
@@ -173,41 +182,39 @@ def rotary(q, k, positions, inv_freq, *, traditional: bool = False, factor: floa
     last; either may be None); positions: int32 [tokens] or [batch, tokens].
     inv_freq: fp32 [rot_dim / 2] (`rotary_frequencies`); the first rot_dim
     elements of a head are rotated, in pairs (i, i + rot_dim / 2), or
-    neighbours when `traditional`. Returns (q_out, k_out), new contiguous
-    tensors unless given; a given one may be its input."""
-    import torch
+    neighbours when `traditional`. Returns (q_out, k_out), new dense tensors
+    unless given; a given one may be its input."""
+    if torch is None:
+        _load()
     ref = q if q is not None else k
     if ref is None:
         raise ValueError("q or k is required")
     dev, dt, dim = _device(), ref.dtype, ref.shape[-1]
     code = _dtype_code(dt)
-    handle, ctx = _handle(stream)
-    batch = tokens = 0
-    heads, rows, outs = [], [], []
-    for name, x, o in (("q", q, q_out), ("k", k, k_out)):
-        if x is None:
-            heads.append(0)
-            rows += [None, None]
-            outs.append(None)
-            continue
-        r, b, n, h = _rows(x, name, dt, dev, dim)
-        if x is not ref and (b, n) != (batch, tokens):
+    qr = qo = kr = ko = None
+    hq = hk = 0
+    if q is not None:
+        qr, batch, tokens, hq = _rows(q, "q", dt, dev, dim)
+        if q_out is None:
+            q_out = _like(q, stream)
+        elif q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
+        qo = _rows(q_out, "q_out", dt, dev, dim)[0]
+    if k is not None:
+        kr, b, n, hk = _rows(k, "k", dt, dev, dim)
+        if q is None:
+            batch, tokens = b, n
+        elif b != batch or n != tokens or k.dim() != q.dim():
             raise ValueError("q and k must have the same tokens")
-        batch, tokens = b, n
-        if o is None:
-            with ctx:
-                o = torch.empty(x.shape, dtype=dt, device=x.device)
-        elif o.shape != x.shape:
-            raise ValueError(f"{name}_out must have {name}'s shape")
-        heads.append(h)
-        rows += [r, _rows(o, name + "_out", dt, dev, dim)[0]]
-        outs.append(o)
-    want = (tokens,) if ref.dim() == 3 else (batch, tokens)
-    pos = _arg(positions, "positions", torch.int32, dev, want)
+        if k_out is None:
+            k_out = _like(k, stream)
+        elif k_out.shape != k.shape:
+            raise ValueError("k_out must have k's shape")
+        ko = _rows(k_out, "k_out", dt, dev, dim)[0]
+    pos = _arg(positions, "positions", _I32, dev, (tokens,) if ref.dim() == 3 else (batch, tokens))
     rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
-    _check(lib().sd_rotary(rot, code, dim, batch, tokens, pos, heads[0], rows[0], rows[1], heads[1], rows[2], rows[3],
-                           handle))
-    return outs[0], outs[1]
+    _check(_L.sd_rotary(rot, code, dim, batch, tokens, pos, hq, qr, qo, hk, kr, ko, _handle(stream, dev)))
+    return (q_out if q is not None else None), (k_out if k is not None else None)
 
 
 class KVPages:
@@ -217,35 +224,36 @@ class KVPages:
     of a quantized cache)."""
 
     def __init__(self, k, v, k_scales=None, k_biases=None, v_scales=None, v_biases=None, bits: int = 0):
-        import torch
-        dev = k.get_device()
+        if torch is None:
+            _load()
+        dev, shape = k.get_device(), k.shape
         if dev < 0:
             raise ValueError("pool arrays must be CUDA tensors")
-        if k.dim() not in (4, 5):
+        if len(shape) == 4:
+            n_layers, (n_pages, hkv, page, dim) = 1, shape
+        elif len(shape) == 5:
+            n_layers, n_pages, hkv, page, dim = shape
+        else:
             raise ValueError("pool arrays must be [n_pages, Hkv, page_size, .] or [n_layers, n_pages, Hkv, page_size, .]")
-        *lead, n_pages, hkv, page = k.shape[:-1]
         small = (k_scales, k_biases, v_scales, v_biases)
         if bits:
             if any(a is None for a in small):
                 raise ValueError("a quantized pool needs k/v scales and biases")
-            self.dtype = k_scales.dtype
-            dim = k.shape[-1] * 32 // bits
-            data = torch.int32
+            dt, dim = k_scales.dtype, dim * 32 // bits
+            each = (*shape[:-1], dim // 64)
+            ptrs = [_arg(k, "k", _I32, dev), _arg(v, "v", _I32, dev, shape)]
+            ptrs += [_arg(a, n, dt, dev, each) for n, a in zip(("k_scales", "k_biases", "v_scales", "v_biases"), small)]
         else:
-            if any(a is not None for a in small):
+            if small != (None, None, None, None):
                 raise ValueError("scales and biases need bits")
-            self.dtype, dim, data = k.dtype, k.shape[-1], k.dtype
-        code = _dtype_code(self.dtype)
-        shape = k.shape
-        ptrs = [_arg(k, "k", data, dev), _arg(v, "v", data, dev, shape)]
-        ptrs += [_arg(a, n, self.dtype, dev, (*shape[:-1], dim // 64)) for n, a in
-                 zip(("k_scales", "k_biases", "v_scales", "v_biases"), small)]
+            dt = k.dtype
+            ptrs = (_arg(k, "k", dt, dev), _arg(v, "v", dt, dev, shape), None, None, None, None)
         self.k, self.v = k, v
         self.k_scales, self.k_biases, self.v_scales, self.v_biases = small
-        self.bits, self.device = bits, dev
-        self.n_layers, self.n_pages = lead[0] if lead else 1, n_pages
+        self.bits, self.device, self.dtype = bits, dev, dt
+        self.n_layers, self.n_pages = n_layers, n_pages
         self.n_kv_heads, self.page_size, self.head_dim = hkv, page, dim
-        self.struct = SDPages(*ptrs, n_pages, self.n_layers, hkv, dim, page, code, bits, 64 if bits else 0, 0)
+        self.struct = SDPages(*ptrs, n_pages, n_layers, hkv, dim, page, _dtype_code(dt), bits, 64 if bits else 0, 0)
 
     def here(self) -> int:
         """The current device, which must be the pool's."""
@@ -268,34 +276,30 @@ def paged_append(pages: KVPages, k, v, tables, positions, *, seq=None, layer: in
     tables [batch, width], positions [tokens], seq [tokens]: int32. flags: an
     int32 tensor that receives bit 2 when an index is out of range (nothing is
     stored for that token)."""
-    import torch
     dev, dt, dim = pages.here(), pages.dtype, pages.head_dim
     kr, b, n, h = _rows(k, "k", dt, dev, dim)
     vr, vb, vn, vh = _rows(v, "v", dt, dev, dim)
-    if b != 1 or (vb, vn, vh) != (1, n, h) or h != pages.n_kv_heads:
+    if k.dim() != 3 or v.dim() != 3 or vn != n or vh != h or h != pages.n_kv_heads:
         raise ValueError(f"k and v must be [tokens, {pages.n_kv_heads}, {dim}]")
     if tables.dim() != 2:
         raise ValueError("tables must be [batch, width]")
-    handle, ctx = _handle(stream)
-    i32 = torch.int32
-    turns = inv_freq is not None or q_norm is not None or k_norm is not None
-    rot, qr, qo, hq = None, None, None, 0
+    rot = qr = qo = None
+    hq = 0
     if q is not None:
         qr, qb, qn, hq = _rows(q, "q", dt, dev, dim)
-        if qb != 1 or qn != n:
+        if q.dim() != 3 or qn != n:
             raise ValueError("q must have k's tokens")
         if q_out is None:
-            with ctx:
-                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+            q_out = _like(q, stream)
         elif q_out.shape != q.shape:
             raise ValueError("q_out must have q's shape")
         qo = _rows(q_out, "q_out", dt, dev, dim)[0]
-    if turns or q is not None:
+    if q is not None or inv_freq is not None or q_norm is not None or k_norm is not None:
         rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
-    _check(lib().sd_paged_append(pages.struct, layer, n, kr, vr, _arg(tables, "tables", i32, dev), tables.shape[0],
-                                 tables.shape[1], _arg(positions, "positions", i32, dev, (n,)),
-                                 _arg(seq, "seq", i32, dev, (n,)), rot, hq, qr, qo, _arg(flags, "flags", i32, dev),
-                                 handle))
+    batch, width = tables.shape
+    _check(_L.sd_paged_append(pages.struct, layer, n, kr, vr, _arg(tables, "tables", _I32, dev), batch, width,
+                              _arg(positions, "positions", _I32, dev, (n,)), _arg(seq, "seq", _I32, dev, (n,)), rot, hq,
+                              qr, qo, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
     return q_out if q is not None else None
 
 
@@ -303,9 +307,7 @@ def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
     """Page dst[i] = page src[i] in every layer and array of the pool. src,
     dst: int32 CUDA tensors, or sequences of ints (checked here). The dst
     pages must be distinct and none of them a src."""
-    import torch
     dev = pages.here()
-    handle, ctx = _handle(stream)
     if not isinstance(src, torch.Tensor):
         src, dst = [int(i) for i in src], [int(i) for i in dst]
         if len(src) != len(dst):
@@ -314,14 +316,13 @@ def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
             raise ValueError("page out of range")
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             raise ValueError("dst pages must be distinct and none of them a src")
-        with ctx:
-            both = torch.tensor([src, dst], dtype=torch.int32).to(dev, non_blocking=True)
+        with torch.cuda.stream(stream):  # None: the current one
+            both = torch.tensor([src, dst], dtype=_I32).to(dev)
         src, dst = both[0], both[1]
     if src.dim() != 1:
         raise ValueError("src and dst must be [n]")
-    _check(lib().sd_copy_pages(pages.struct, _arg(src, "src", torch.int32, dev),
-                               _arg(dst, "dst", torch.int32, dev, src.shape), src.shape[0],
-                               _arg(flags, "flags", torch.int32, dev), handle))
+    _check(_L.sd_copy_pages(pages.struct, _arg(src, "src", _I32, dev), _arg(dst, "dst", _I32, dev, src.shape),
+                            src.shape[0], _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
 
 
 def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = None, *, layer: int = 0, window: int = 0,
@@ -333,28 +334,27 @@ def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = No
     tables [batch, width] and lengths [batch]: int32, read on the device only,
     so a captured call serves growing sequences. sinks: fp32 [Hq] logits that
     join the denominators. Hq / Hkv: 1 .. 16."""
-    import torch
     dev, dt, dim = pages.here(), pages.dtype, pages.head_dim
-    if q.dim() != 3 or q.shape[2] != dim:
-        raise ValueError(f"q must be [batch, Hq, {dim}]")
-    batch, hq = q.shape[0], q.shape[1]
-    if tables.dim() != 2 or tables.shape[0] != batch:
-        raise ValueError("tables must be [batch, width]")
+    shape, (batch, width) = q.shape, tables.shape
+    if len(shape) != 3 or shape[0] != batch or shape[2] != dim:
+        raise ValueError(f"q must be [batch, Hq, {dim}] and tables [batch, width]")
+    hq = shape[1]
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    handle, ctx = _handle(stream)
-    i32, L = torch.int32, lib()
     need = ctypes.c_int64()
     if batch:
-        _check(L.sd_paged_workspace(pages.struct, batch, hq, need))
-    with ctx:
-        if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=q.device)
+        _check(_L.sd_paged_workspace(pages.struct, batch, hq, need))
+    if out is None:
+        out = _like(q, stream)
+    if stream is None:
         work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    _check(L.sd_paged_decode(pages.struct, layer, _arg(q, "q", dt, dev), batch, hq, _arg(tables, "tables", i32, dev),
-                             tables.shape[1], _arg(lengths, "lengths", i32, dev, (batch,)), scale, window,
-                             _arg(sinks, "sinks", torch.float32, dev, (hq,)), _arg(out, "out", dt, dev, q.shape),
-                             work.data_ptr(), need.value, _arg(flags, "flags", i32, dev), handle))
+    else:
+        with torch.cuda.stream(stream):
+            work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+    _check(_L.sd_paged_decode(pages.struct, layer, _arg(q, "q", dt, dev), batch, hq, _arg(tables, "tables", _I32, dev),
+                              width, _arg(lengths, "lengths", _I32, dev, (batch,)), scale, window,
+                              _arg(sinks, "sinks", _F32, dev, (hq,)), _arg(out, "out", dt, dev, shape), work.data_ptr(),
+                              need.value, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
     return out
 
 
@@ -368,7 +368,8 @@ class PagePool:
 
     def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
                  dtype: str = "bf16", kv_bits: int = 0):
-        import torch
+        if torch is None:
+            _load()
         if kv_bits not in (0, 4, 8):
             raise ValueError("kv_bits must be 0, 4 or 8")
         lead = (n_layers, n_pages, n_kv_heads, page_size)
@@ -484,7 +485,6 @@ class PagedBatch:
     copied to the device once, for every layer of the step."""
 
     def __init__(self, pool: PagePool, seqs: list, new: list, stream=None):
-        import torch
         self.pool, self.seqs, self.new = pool, seqs, new
         n = len(seqs)
         ids = (ctypes.c_int64 * max(n, 1))(*seqs)
@@ -500,8 +500,7 @@ class PagedBatch:
         pos = [p for t, k in zip(lengths, new) for p in range(t - k, t)]
         seq = [b for b, k in enumerate(new) for _ in range(k)]
         host[n * w + n:] = torch.tensor(pos + seq, dtype=torch.int32)
-        _, ctx = _handle(stream)
-        with ctx:
+        with torch.cuda.stream(stream):  # None: the current one
             dev = host.to("cuda", non_blocking=True)
         self.tables = dev[:n * w].view(n, w)
         self.lengths = dev[n * w:n * w + n]
@@ -541,7 +540,6 @@ class PagedLayer:
         """Append keys/values [B, Hkv, L, D] and attend with queries
         [B, Hq, L, D]; every sequence has L new tokens. L == 1 takes the decode
         kernel; longer prompts are attended densely, sequence by sequence."""
-        import torch
         from .cache import _dense_attention
         b = self.batch
         B, Hq, L, D = queries.shape
