@@ -59,10 +59,29 @@ template <class F>
 struct TileAddr {
   uint32_t base;  // shared address of the K (or V) part
   int pb_log;     // log2 of the rows per box
+  // First byte of row `row` of the box columns.
+  __device__ __forceinline__ uint32_t row_at(int row) const {
+    return base + uint32_t(((row >> pb_log) << pb_log) * F::kRowBytes + (row & ((1 << pb_log) - 1)) * F::kBoxBytes);
+  }
   __device__ __forceinline__ uint32_t at(int row, int chunk) const {
     const int pb = 1 << pb_log;
     return base + uint32_t((row >> pb_log) * (pb * F::kRowBytes) + (chunk / F::kCpb) * (pb * F::kBoxBytes)) +
            swz(uint32_t((row & (pb - 1)) * F::kBoxBytes + (chunk % F::kCpb) * 16), F::kCpb);
+  }
+};
+// What a lane's ldmatrix address adds to row_at of its 16 rows, for row `r`
+// of them (boxes hold 16 rows at least) and chunk 2c + odd: the swizzle of a
+// row does not depend on which 16 rows it is in, and an even chunk number
+// joins the odd bit by xor.
+template <class F>
+struct LaneAddr {
+  uint32_t off, x;
+  __device__ __forceinline__ LaneAddr(int r, int odd) {
+    off = uint32_t(r * F::kBoxBytes);
+    x = (((off >> 7) & (F::kCpb - 1u)) << 4) ^ uint32_t(odd * 16);
+  }
+  __device__ __forceinline__ uint32_t at(uint32_t rows, int chunk, int pb_log) const {  // chunk: even
+    return rows + off + uint32_t((chunk / F::kCpb) << pb_log) * F::kBoxBytes + (x ^ uint32_t((chunk % F::kCpb) * 16));
   }
 };
 
@@ -82,12 +101,19 @@ struct WarpPart {
   }
 };
 
-__device__ __forceinline__ float exp2_from(float s, float m) { return exp2f(s - (m == -INFINITY ? 0.0f : m)); }
+// 2^x by the hardware's instruction (relative error 2^-22; results below
+// 2^-126 are zero, which a softmax weight may be).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_from(float s, float m) { return ex2(s - (m == -INFINITY ? 0.0f : m)); }
 
 // New running maximum and the factor for what was summed under the old one.
 __device__ __forceinline__ float raise_max(float& m, float mx) {
   const float mn = fmaxf(m, mx);
-  const float f = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+  const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
   m = mn;
   return f;
 }
@@ -135,7 +161,8 @@ struct DenseAttend {
     const int r0 = warp * TW;
     const int lo = t.lo - r0, hi = t.hi - r0;  // valid rows of this warp's 16
     if (hi <= 0 || lo >= TW) return;
-    const TileAddr<F> ka{smem_u32(t.stage), t.pb_log}, va{smem_u32(t.stage) + F::kKvBytes, t.pb_log};
+    const uint32_t krows = TileAddr<F>{smem_u32(t.stage), t.pb_log}.row_at(r0), vrows = krows + F::kKvBytes;
+    const LaneAddr<F> ka(8 * (mq & 1) + r8, mq >> 1), va(8 * (mq >> 1) + r8, mq & 1);
     float acc[2][NB][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -144,7 +171,7 @@ struct DenseAttend {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint32_t a0, a1, a2, a3;
-      ldsm_x4(ka.at(r0 + 8 * (mq & 1) + r8, 2 * c + (mq >> 1)), a0, a1, a2, a3);
+      ldsm_x4(ka.at(krows, 2 * c, t.pb_log), a0, a1, a2, a3);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) mma_full<E>(acc[c & 1][nb], a0, a1, a2, a3, qb[nb][c][0], qb[nb][c][1]);
     }
@@ -203,7 +230,7 @@ struct DenseAttend {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint32_t a0, a1, a2, a3;
-      ldsm_x4_t(va.at(r0 + 8 * (mq >> 1) + r8, 2 * c + (mq & 1)), a0, a1, a2, a3);
+      ldsm_x4_t(va.at(vrows, 2 * c, t.pb_log), a0, a1, a2, a3);
       if (!whole) {
         a0 &= m0;
         a1 &= m0;
@@ -245,27 +272,55 @@ struct DenseAttend {
   }
 };
 
-// Scales (or biases) of token t for every group, in fp32; zeros if !ok.
+// Codes as fp16 without removing the offset: two bytes of r as 1024 + c (sel
+// takes the low halves' bytes from r, the high ones, 0x64, from byte 1 of
+// `magic`); or the nibbles at bits [4 hi, 4 hi + 4) of r's halves as 1024 + c
+// (1024 + 16 c for hi). magic is 0x64006400, fp16 1024 twice, as a kernel
+// argument: as a literal it would make two instructions of each of these.
+__device__ __forceinline__ uint32_t raw_u8(uint32_t r, uint32_t sel, uint32_t magic) { return __byte_perm(r, magic, sel); }
+__device__ __forceinline__ uint32_t raw_u4(uint32_t r, int hi, uint32_t magic) {
+  return (r & (hi ? 0x00F000F0u : 0x000F000Fu)) | magic;
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Scales (or biases) of token t for every group, in fp32, from shared memory.
 template <typename E, int NG>
-__device__ __forceinline__ void load_groups(const E* a, int t, bool ok, float (&f)[NG]) {
+__device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
   if constexpr (NG == 2) {
-    unpack_word<E>(ok ? reinterpret_cast<const uint32_t*>(a)[t] : 0u, f);
+    unpack_word<E>(lds32(a + 4 * t), f);
   } else {
-    f[0] = ok ? Elt<E>::to_f32(a[t]) : 0.0f;
+    uint16_t w;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(a + 2 * t));
+    f[0] = Elt<E>::to_f32(__builtin_bit_cast(E, w));
   }
 }
 
 // ---------------------------------------------------------------------------
-// 4/8-bit codes with 16-bit scales, the same products. The codes enter as
-// exact fp16 integers (code_pair_u8 / code_pair_u4):
-//   q.k = s_k (q.c) + b_k sum(q)             per 64-dim group, in fp32
-//   p.v = (p s_v).c + sum_t p b_v
+// 4/8-bit codes with 16-bit scales, the same products, with the codes as exact
+// fp16 integers. What bounds this path is instructions, not bytes, so the
+// conversion is cut to the bone: one byte permute (or mask) puts codes into
+// the mantissas of 1024 + c, or 1024 + 16 c for the nibbles that lie 4 bits
+// higher.
+//   q.k = s_k (q.c) + b_k sum(q)  per 64-dim group, in fp32. For bf16 pools
+// the offset is left in: the accumulator starts at -1024 sum(q') (q' = q in
+// fp16, a 16th of it where the nibble's place counts 16), which costs 3 to 4
+// of fp32's bits over the 64 products of a group, scores off by some 3e-4 --
+// nothing next to bf16's rounding, but a good half of fp16's, so fp16 pools
+// subtract it.
+//   p.v = (p s_v).(c - z) + sum_t p (b_v + z s_v), z = the middle code. These
+// sums run over a whole segment, so their codes are centred by one packed
+// subtraction: no offset to cancel, and terms of both signs.
 // q is scaled by a power of two so that its largest element is in
 // [2^13, 2^14): bf16 values then keep all their bits in fp16 down to 2^-27 of
 // the largest. p s_v is scaled per group by a power of two kept across tiles
-// (vinv) so that the largest |s_v| so far maps near 2^6: hi + lo fp16 halves
-// hold it to about 22 bits, and values of any magnitude neither overflow nor
-// sink into fp16's subnormals.
+// (vinv) so that the largest |s_v| so far maps below 2^7 (with p up to
+// 2^kSlack, p s_v stays below 2^15): values of any magnitude neither overflow nor sink into fp16's subnormals, and split into
+// hi + lo halves (22 bits). One half alone was 13 bf16 ulp off where the terms
+// of an output nearly cancel, and no faster.
 // ---------------------------------------------------------------------------
 template <typename E, int BITS, int D, int NB>
 struct CodesAttend {
@@ -273,35 +328,37 @@ struct CodesAttend {
   static constexpr int NK = D / 16, NG = F::kGroups, NCH = F::kNChunk;
   static constexpr int KPC = NK / NCH;   // k-steps (and 16-dim output tiles) per 16-byte chunk: 1 or 2
   static constexpr int MT = F::kTile / kPagedWarps / 16;
+  static constexpr float MID = BITS == 8 ? 128.0f : 8.0f;
+  static constexpr bool kOffset = !__is_same(E, __half);
   uint32_t qb[NB][NK][2];
-  float qs[NB][2][NG], m[NB][2], l[NB][2], o[NB][NK][4], ob[NB][2][NG];
+  float qs[NB][2][NG], qoff[NB][2][NG], m[NB][2], l[NB][2], o[NB][NK][4], ob[NB][2][NG];
   float vinv[NG], vlim[NG], qfac;
-
-  // dims of k-slot pairs {2tq, 2tq + 1} and {2tq + 8, 2tq + 9} of k-step k
-  static __device__ __forceinline__ void dims(int k, int tq, int (&d)[4]) {
-    if constexpr (BITS == 8) {
-      const int d0 = 16 * k + 4 * tq;
-      d[0] = d0, d[1] = d0 + 1, d[2] = d0 + 2, d[3] = d0 + 3;
-    } else {
-      const int d0 = 32 * (k >> 1) + 8 * tq + 2 * (k & 1);
-      d[0] = d0, d[1] = d0 + 4, d[2] = d0 + 1, d[3] = d0 + 5;
-    }
-  }
 
   __device__ __forceinline__ void begin(const PagedParams& p, const float*, int b, int h, int, int lane) {
     const int g = lane >> 2, tq = lane & 3;
-    const E* q = static_cast<const E*>(p.q);
+    // this lane's elements of head g: four (8-bit) or eight (4-bit) neighbours of every chunk
+    constexpr int N = BITS == 8 ? 2 : 4;  // 32-bit words
+    uint32_t raw[NB][NCH][N];
     float qmax = 0.0f;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int hd = 8 * nb + g;
-      const E* row = q + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * D;
+      const E* row = static_cast<const E*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * D;
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        int d[4];
-        dims(k, tq, d);
+      for (int c = 0; c < NCH; ++c) {
+        if constexpr (BITS == 8) {
+          const uint2 w = hd < p.G ? __ldg(reinterpret_cast<const uint2*>(row + 16 * c + 4 * tq)) : make_uint2(0, 0);
+          raw[nb][c][0] = w.x, raw[nb][c][1] = w.y;
+        } else {
+          const uint4 w = hd < p.G ? __ldg(reinterpret_cast<const uint4*>(row + 32 * c + 8 * tq)) : make_uint4(0, 0, 0, 0);
+          raw[nb][c][0] = w.x, raw[nb][c][1] = w.y, raw[nb][c][2] = w.z, raw[nb][c][3] = w.w;
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qmax = fmaxf(qmax, hd < p.G ? fabsf(Elt<E>::to_f32(__ldg(row + d[i]))) : 0.0f);
+        for (int i = 0; i < N; ++i) {
+          float f[2];
+          unpack_word<E>(raw[nb][c][i], f);
+          qmax = fmaxf(qmax, fmaxf(fabsf(f[0]), fabsf(f[1])));
+        }
       }
     }
     qmax = warp_max(qmax);
@@ -310,33 +367,53 @@ struct CodesAttend {
     qfac = ldexpf(p.scale_log2, eq);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int hd = 8 * nb + g;
-      const E* row = q + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * D;
-      float sum[NG];
+      float sum[NG], off[NG];
 #pragma unroll
-      for (int r = 0; r < NG; ++r) sum[r] = 0.0f;
+      for (int r = 0; r < NG; ++r) sum[r] = off[r] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        int d[4];
-        dims(k, tq, d);
-        float f[4];
+      for (int c = 0; c < NCH; ++c) {
+        const int r = c * F::kEpc / 64;
+        float f[2 * N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f[i] = hd < p.G ? Elt<E>::to_f32(__ldg(row + d[i])) : 0.0f;
-          sum[k / 4] += f[i];
+        for (int i = 0; i < N; ++i) unpack_word<E>(raw[nb][c][i], f + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) {
+          sum[r] += f[i];
           f[i] *= up;
         }
-        qb[nb][k][0] = pack2<__half>(f[0], f[1]);
-        qb[nb][k][1] = pack2<__half>(f[2], f[3]);
-        o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.0f;
+        // k-slots {2tq, 2tq + 1} and {2tq + 8, 2tq + 9}, in the order in which the codes come out of a register
+        if constexpr (BITS == 8) {
+          qb[nb][c][0] = pack2<__half>(f[0], f[1]);
+          qb[nb][c][1] = pack2<__half>(f[2], f[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            qb[nb][2 * c + i][0] = pack2<__half>(f[2 * i], f[2 * i + 4]);
+            qb[nb][2 * c + i][1] = pack2<__half>(f[2 * i + 1] * 0.0625f, f[2 * i + 5] * 0.0625f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < KPC; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float g2[2];
+            unpack_word<__half>(qb[nb][KPC * c + i][j], g2);
+            off[r] += g2[0] + g2[1];
+          }
+        }
       }
+#pragma unroll
+      for (int k = 0; k < NK; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.0f;
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        off[r] += __shfl_xor_sync(0xffffffffu, off[r], 1);
+        off[r] += __shfl_xor_sync(0xffffffffu, off[r], 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           qs[nb][e][r] = p.scale_log2 * __shfl_sync(0xffffffffu, sum[r], 4 * (2 * tq + e));
+          qoff[nb][e][r] = kOffset ? -1024.0f * __shfl_sync(0xffffffffu, off[r], 4 * (2 * tq + e)) : 0.0f;
           ob[nb][e][r] = 0.0f;
         }
       }
@@ -350,29 +427,34 @@ struct CodesAttend {
     }
   }
 
-  __device__ __forceinline__ void tile(const PagedParams&, const float*, const TileView& t, int warp, int lane) {
+  __device__ __forceinline__ void tile(const PagedParams& p, const float*, const TileView& t, int warp, int lane) {
     constexpr int TW = 16 * MT;
     const int g = lane >> 2, mq = lane >> 3, r8 = lane & 7;
     const int r0 = warp * TW;
     const int lo = t.lo - r0, hi = t.hi - r0;
     if (hi <= 0 || lo >= TW) return;
-    const TileAddr<F> ka{smem_u32(t.stage), t.pb_log}, va{smem_u32(t.stage) + F::kKvBytes, t.pb_log};
-    const E* ksc = reinterpret_cast<const E*>(t.stage + 2 * F::kKvBytes) + r0 * NG;
-    const E *kbi = ksc + F::kTile * NG, *vsc = ksc + 2 * F::kTile * NG, *vbi = ksc + 3 * F::kTile * NG;
+    const TileAddr<F> rows{smem_u32(t.stage), t.pb_log};
+    const LaneAddr<F> la(8 * (mq & 1) + r8, mq >> 1);
+    const bool whole = lo <= 0 && hi >= TW;
+    const uint32_t magic = p.magic;
+    const uint32_t ksc = smem_u32(t.stage) + 2 * F::kKvBytes + r0 * NG * 2;  // K scales; K biases, V scales, V biases follow
+    const uint32_t kbi = ksc + F::kSbBytes, vsc = kbi + F::kSbBytes, vbi = vsc + F::kSbBytes;
     float s[MT][NB][4];
-    bool up = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float acc[NG][NB][4];
 #pragma unroll
       for (int r = 0; r < NG; ++r)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) acc[r][nb][0] = acc[r][nb][1] = acc[r][nb][2] = acc[r][nb][3] = 0.0f;
+        for (int nb = 0; nb < NB; ++nb) {
+          acc[r][nb][0] = acc[r][nb][2] = qoff[nb][0][r];
+          acc[r][nb][1] = acc[r][nb][3] = qoff[nb][1][r];
+        }
 #pragma unroll
       for (int c = 0; c < NCH; c += 2) {
         // matrices: tokens {0..7, 8..15} of chunks c and c + 1
         uint32_t a[4];
-        ldsm_x4(ka.at(r0 + 16 * mt + 8 * (mq & 1) + r8, c + (mq >> 1)), a[0], a[1], a[2], a[3]);
+        ldsm_x4(la.at(rows.row_at(r0 + 16 * mt), c, t.pb_log), a[0], a[1], a[2], a[3]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -381,11 +463,15 @@ struct CodesAttend {
             const uint32_t x0 = a[2 * j], x1 = a[2 * j + 1];
             uint32_t f0, f1, f2, f3;
             if constexpr (BITS == 8) {
-              f0 = code_pair_u8(x0, 0x4140u), f1 = code_pair_u8(x1, 0x4140u);
-              f2 = code_pair_u8(x0, 0x4342u), f3 = code_pair_u8(x1, 0x4342u);
-            } else {
-              f0 = code_pair_u4(x0, 2 * i), f1 = code_pair_u4(x1, 2 * i);
-              f2 = code_pair_u4(x0, 2 * i + 1), f3 = code_pair_u4(x1, 2 * i + 1);
+              f0 = raw_u8(x0, 0x5150u, magic), f1 = raw_u8(x1, 0x5150u, magic);
+              f2 = raw_u8(x0, 0x5352u, magic), f3 = raw_u8(x1, 0x5352u, magic);
+            } else {  // codes 2i, 2i + 4 (places 1) and 2i + 1, 2i + 5 (places 16) of the register
+              f0 = raw_u4(x0 >> (8 * i), 0, magic), f1 = raw_u4(x1 >> (8 * i), 0, magic);
+              f2 = raw_u4(x0 >> (8 * i), 1, magic), f3 = raw_u4(x1 >> (8 * i), 1, magic);
+            }
+            if constexpr (!kOffset) {
+              f0 = sub_f16x2(f0, 0x64006400u), f1 = sub_f16x2(f1, 0x64006400u);
+              f2 = sub_f16x2(f2, 0x64006400u), f3 = sub_f16x2(f3, 0x64006400u);
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -396,10 +482,11 @@ struct CodesAttend {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int tk = 16 * mt + g + 8 * e;
-        const bool ok = tk >= lo && tk < hi;
         float ks[NG], kb[NG];
-        load_groups<E, NG>(ksc, tk, ok, ks);
-        load_groups<E, NG>(kbi, tk, ok, kb);
+        load_groups<E, NG>(ksc, tk, ks);
+        load_groups<E, NG>(kbi, tk, kb);
+#pragma unroll
+        for (int r = 0; r < NG; ++r) ks[r] *= qfac;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -407,14 +494,29 @@ struct CodesAttend {
             float v = 0.0f;
 #pragma unroll
             for (int r = 0; r < NG; ++r)
-              v = fmaf(ks[r], acc[r][nb][2 * e + hh] * qfac, fmaf(kb[r], qs[nb][hh][r], v));
-            v = ok ? v : -INFINITY;
+              v = fmaf(ks[r], acc[r][nb][2 * e + hh], fmaf(kb[r], qs[nb][hh][r], v));
             s[mt][nb][2 * e + hh] = v;
-            up |= v > m[nb][hh] + kSlack;
           }
         }
       }
     }
+    if (!whole) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tk = 16 * mt + g + 8 * (i >> 1);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[mt][nb][i] = tk < lo || tk >= hi ? -INFINITY : s[mt][nb][i];
+        }
+    }
+    bool up = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) up |= s[mt][nb][i] > m[nb][i & 1] + kSlack;
     if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -438,30 +540,54 @@ struct CodesAttend {
         }
       }
     }
-    float vs[MT][2][NG];
+    float vs[MT][2][NG], vb[MT][2][NG];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        load_groups<E, NG>(vsc, 16 * mt + g + 8 * e, vs[mt][e]);
+        load_groups<E, NG>(vbi, 16 * mt + g + 8 * e, vb[mt][e]);
+      }
+    }
+    if (!whole) {  // anything may lie past the end
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tk = 16 * mt + g + 8 * e;
+#pragma unroll
+          for (int r = 0; r < NG; ++r) {
+            vs[mt][e][r] = tk < lo || tk >= hi ? 0.0f : vs[mt][e][r];
+            vb[mt][e][r] = tk < lo || tk >= hi ? 0.0f : vb[mt][e][r];
+          }
+        }
+    }
+    float mu[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) mu[nb][hh] = m[nb][hh] == -INFINITY ? 0.0f : m[nb][hh];
     bool big = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int tk = 16 * mt + g + 8 * e;
-        const bool ok = tk >= lo && tk < hi;
-        float vb[NG];
-        load_groups<E, NG>(vsc, tk, ok, vs[mt][e]);
-        load_groups<E, NG>(vbi, tk, ok, vb);
+#pragma unroll
+        for (int r = 0; r < NG; ++r) {
+          vb[mt][e][r] = fmaf(MID, vs[mt][e][r], vb[mt][e][r]);
+          big |= fabsf(vs[mt][e][r]) > vlim[r];
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            const float pr = exp2_from(s[mt][nb][2 * e + hh], m[nb][hh]);
+            const float pr = ex2(s[mt][nb][2 * e + hh] - mu[nb][hh]);
             s[mt][nb][2 * e + hh] = pr;
             l[nb][hh] += pr;
 #pragma unroll
-            for (int r = 0; r < NG; ++r) ob[nb][hh][r] = fmaf(pr, vb[r], ob[nb][hh][r]);
+            for (int r = 0; r < NG; ++r) ob[nb][hh][r] = fmaf(pr, vb[mt][e][r], ob[nb][hh][r]);
           }
         }
-#pragma unroll
-        for (int r = 0; r < NG; ++r) big |= fabsf(vs[mt][e][r]) > vlim[r];
       }
     }
     if (__any_sync(0xffffffffu, big)) {
@@ -473,10 +599,10 @@ struct CodesAttend {
         mx = warp_max(mx);
         if (mx > vlim[r] && mx < INFINITY) {
           const int e = max(ilogbf(mx), -100);
-          const float inv = ldexpf(1.0f, 6 - e);
+          const float inv = ldexpf(1.0f, 3 - e);
           const float f = vlim[r] > 0.0f ? inv / vinv[r] : 1.0f;  // o is still zero the first time
           vinv[r] = inv;
-          vlim[r] = ldexpf(1.0f, min(e + 8, 127));
+          vlim[r] = ldexpf(1.0f, min(e + 4, 127));
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -507,7 +633,7 @@ struct CodesAttend {
       for (int c = 0; c < NCH; c += 2) {
         // matrices (transposed): tokens {0..7, 8..15} of chunks c and c + 1
         uint32_t a[4];
-        ldsm_x4_t(va.at(r0 + 16 * mt + 8 * (mq & 1) + r8, c + (mq >> 1)), a[0], a[1], a[2], a[3]);
+        ldsm_x4_t(la.at(rows.row_at(r0 + 16 * mt) + F::kKvBytes, c, t.pb_log), a[0], a[1], a[2], a[3]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -515,12 +641,12 @@ struct CodesAttend {
             const int k = (c + j) * KPC + i, r = k / 4;
             const uint32_t x0 = a[2 * j], x1 = a[2 * j + 1];
             uint32_t f0, f1, f2, f3;
-            if constexpr (BITS == 8) {
-              f0 = code_pair_u8(x0, 0x4240u), f1 = code_pair_u8(x0, 0x4341u);
-              f2 = code_pair_u8(x1, 0x4240u), f3 = code_pair_u8(x1, 0x4341u);
-            } else {
-              f0 = code_pair_u4(x0, 2 * i), f1 = code_pair_u4(x0, 2 * i + 1);
-              f2 = code_pair_u4(x1, 2 * i), f3 = code_pair_u4(x1, 2 * i + 1);
+            if constexpr (BITS == 8) {  // less 1024 + 128
+              f0 = sub_f16x2(raw_u8(x0, 0x5250u, magic), 0x64806480u), f1 = sub_f16x2(raw_u8(x0, 0x5351u, magic), 0x64806480u);
+              f2 = sub_f16x2(raw_u8(x1, 0x5250u, magic), 0x64806480u), f3 = sub_f16x2(raw_u8(x1, 0x5351u, magic), 0x64806480u);
+            } else {  // less 1024 + 8, and 1024 + 16 * 8: rows g + 8 hold 16 (c - 8)
+              f0 = sub_f16x2(raw_u4(x0 >> (8 * i), 0, magic), 0x64086408u), f1 = sub_f16x2(raw_u4(x0 >> (8 * i), 1, magic), 0x64806480u);
+              f2 = sub_f16x2(raw_u4(x1 >> (8 * i), 0, magic), 0x64086408u), f3 = sub_f16x2(raw_u4(x1 >> (8 * i), 1, magic), 0x64806480u);
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -557,7 +683,7 @@ struct CodesAttend {
             const float back = 1.0f / vinv[k / 4];
             const int d = BITS == 8 ? 16 * k + 2 * g : 32 * (k >> 1) + 4 * g + 2 * (k & 1);
             w.o[hd * (D + 4) + d] = fmaf(o[nb][k][e], back, ob[nb][e][k / 4]);
-            w.o[hd * (D + 4) + d + 1] = fmaf(o[nb][k][2 + e], back, ob[nb][e][k / 4]);
+            w.o[hd * (D + 4) + d + 1] = fmaf(o[nb][k][2 + e], BITS == 8 ? back : back * 0.0625f, ob[nb][e][k / 4]);
           }
         }
       }
@@ -567,141 +693,140 @@ struct CodesAttend {
 
 // ---------------------------------------------------------------------------
 // fp32 pools (dense, or codes with fp32 scales) on the FMA pipes: the tensor
-// cores have no fp32 product. q.k: a lane holds one token and every
-// kParts-th 16-byte chunk of its row; p.v: a lane holds D / 32 dims and walks
-// the tokens, p broadcast by shuffles. q (times scale * log2 e) and, for
-// codes, its sum over each chunk lie in shared memory.
+// cores have no fp32 product. A warp has 8 tokens of a tile and takes the heads
+// four at a time. q.k: lane = (token, head), so a score needs no exchange and
+// no array over heads, which keeps the code short -- a small call spends more
+// on fetching instructions than on executing them. p.v: lane = (head, eighth
+// of the dims), p from the score's lane by one shuffle per token. q (times
+// scale * log2 e, rows padded against bank conflicts) and, for codes, its sum
+// over each 16-byte chunk lie in shared memory.
 // ---------------------------------------------------------------------------
 template <int BITS, int D, int NB>
 struct FmaAttend {
   using F = PagedFmt<4, BITS, D>;
-  static constexpr int GM = 8 * NB, NCH = F::kNChunk, EPC = F::kEpc, NG = F::kGroups;
-  static constexpr int TW = F::kTile / kPagedWarps, PARTS = 32 / TW, DPL = D / 32;
-  float m[GM], l[GM], o[GM][DPL];
+  static constexpr int HB = 2 * NB, NCH = F::kNChunk, EPC = F::kEpc, NG = F::kGroups;  // HB: blocks of four heads
+  static constexpr int TW = 8, DL = D / 8;
+  static_assert(F::kTile == TW * kPagedWarps, "eight tokens per warp");
+  float m[HB], l[HB], o[HB][DL];  // of head 4 hb + lane % 4 (m, l) and 4 hb + lane / 8 (o)
 
-  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[EPC]) {
+  // Four elements of a chunk, from element 4i on.
+  static __device__ __forceinline__ float4 four(const uint4& w, int i) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < EPC; ++i) {
-      if constexpr (BITS == 0) x[i] = __uint_as_float(u[i]);
-      else if constexpr (BITS == 8) x[i] = float((u[i / 4] >> (8 * (i % 4))) & 255u);
-      else x[i] = float((u[i / 8] >> (4 * (i % 8))) & 15u);
+    if constexpr (BITS == 0) {
+      return make_float4(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3]));
+    } else if constexpr (BITS == 8) {
+      return make_float4(code_u8(u[i], 0), code_u8(u[i], 1), code_u8(u[i], 2), code_u8(u[i], 3));
+    } else {
+      const int h = 4 * (i & 1);
+      return make_float4(code_u4(u[i / 2], h), code_u4(u[i / 2], h + 1), code_u4(u[i / 2], h + 2), code_u4(u[i / 2], h + 3));
     }
   }
 
-  // every consumer thread calls; qf: [G][D] then [G][NCH] chunk sums
+  // every consumer thread calls; qf: [G][D + 4], then [G][NCH] chunk sums
   __device__ __forceinline__ void begin(const PagedParams& p, float* qf, int b, int h, int warp, int lane) {
     const float* q = static_cast<const float*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G) * D;
     const int t = warp * 32 + lane;
-    for (int i = t; i < p.G * D; i += 32 * kPagedWarps) qf[i] = __ldg(q + i) * p.scale_log2;
+#pragma unroll 1
+    for (int i = t; i < p.G * D; i += 32 * kPagedWarps) qf[i / D * (D + 4) + i % D] = __ldg(q + i) * p.scale_log2;
     if constexpr (BITS != 0) {
+#pragma unroll 1
       for (int i = t; i < p.G * NCH; i += 32 * kPagedWarps) {
         float sum = 0.0f;
         for (int d = 0; d < EPC; ++d) sum += __ldg(q + (i / NCH) * D + (i % NCH) * EPC + d);
-        qf[p.G * D + i] = sum * p.scale_log2;
+        qf[p.G * (D + 4) + i] = sum * p.scale_log2;
       }
     }
     named_barrier(1, 32 * kPagedWarps);
 #pragma unroll
-    for (int g = 0; g < GM; ++g) {
-      m[g] = -INFINITY;
-      l[g] = 0.0f;
+    for (int hb = 0; hb < HB; ++hb) {
+      m[hb] = -INFINITY;
+      l[hb] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < DPL; ++i) o[g][i] = 0.0f;
+      for (int i = 0; i < DL; ++i) o[hb][i] = 0.0f;
     }
   }
 
   __device__ __forceinline__ void tile(const PagedParams& p, const float* qf, const TileView& t, int warp, int lane) {
-    const int tok = lane % TW, part = lane / TW, r0 = warp * TW;
+    const int r0 = warp * TW;
     const int lo = max(t.lo - r0, 0), hi = min(t.hi - r0, TW);
     if (hi <= lo) return;
     const TileAddr<F> ka{smem_u32(t.stage), t.pb_log}, va{smem_u32(t.stage) + F::kKvBytes, t.pb_log};
     const float* ksc = reinterpret_cast<const float*>(t.stage + 2 * F::kKvBytes) + r0 * NG;
     const float *kbi = ksc + F::kTile * NG, *vsc = ksc + 2 * F::kTile * NG, *vbi = ksc + 3 * F::kTile * NG;
+    const int tok = lane >> 2, vh = lane >> 3, d0 = (lane & 7) * DL;  // q.k: (tok, lane % 4); p.v: (vh, d0 ..)
     const bool ok = tok >= lo && tok < hi;
-    float s[GM];
 #pragma unroll
-    for (int g = 0; g < GM; ++g) s[g] = 0.0f;
-#pragma unroll 2
-    for (int c = part; c < NCH; c += PARTS) {
-      float x[EPC];
-      unpack(lds128(ka.at(r0 + tok, c)), x);
-      float sc = 1.0f, bi = 0.0f;
-      if constexpr (BITS != 0) {
-        sc = ksc[tok * NG + c * EPC / 64];
-        bi = kbi[tok * NG + c * EPC / 64];
-      }
+    for (int hb = 0; hb < HB; ++hb) {
+      if (4 * hb >= p.G) break;
+      const int hd = min(4 * hb + (lane & 3), p.G - 1);  // a head past the last repeats it
+      const float* qrow = qf + hd * (D + 4);
+      float s = 0.0f;
+#pragma unroll 4
+      for (int c = 0; c < NCH; ++c) {
+        const uint4 w = lds128(ka.at(r0 + tok, c));
+        float a = 0.0f;
 #pragma unroll
-      for (int g = 0; g < GM; ++g) {
-        if (g < p.G) {
-          const float4* qv = reinterpret_cast<const float4*>(qf + g * D + c * EPC);
-          float a = 0.0f;
-#pragma unroll
-          for (int i = 0; i < EPC; i += 4) {
-            const float4 w = qv[i / 4];
-            a = fmaf(w.x, x[i], a);
-            a = fmaf(w.y, x[i + 1], a);
-            a = fmaf(w.z, x[i + 2], a);
-            a = fmaf(w.w, x[i + 3], a);
-          }
-          if constexpr (BITS != 0) s[g] = fmaf(sc, a, fmaf(bi, qf[p.G * D + g * NCH + c], s[g]));
-          else s[g] += a;
+        for (int i = 0; i < EPC / 4; ++i) {
+          const float4 x = four(w, i), y = *reinterpret_cast<const float4*>(qrow + c * EPC + 4 * i);
+          a = fmaf(x.x, y.x, a);
+          a = fmaf(x.y, y.y, a);
+          a = fmaf(x.z, y.z, a);
+          a = fmaf(x.w, y.w, a);
         }
-      }
-    }
-    bool up = false;
-#pragma unroll
-    for (int g = 0; g < GM; ++g) {
-      if (g < p.G) {
-#pragma unroll
-        for (int x = TW; x < 32; x <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], x);
-        s[g] = ok ? s[g] : -INFINITY;
-        up |= s[g] > m[g] + kSlack;
-      }
-    }
-    if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-      for (int g = 0; g < GM; ++g) {
-        if (g < p.G) {
-          const float f = raise_max(m[g], warp_max(s[g]));
-          l[g] *= f;
-#pragma unroll
-          for (int i = 0; i < DPL; ++i) o[g][i] *= f;
-        }
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < GM; ++g) {
-      if (g < p.G) {
-        s[g] = exp2_from(s[g], m[g]);
-        if (part == 0) l[g] += s[g];
-      }
-    }
-#pragma unroll 2
-    for (int tk = lo; tk < hi; ++tk) {
-      float v[DPL];
-      constexpr int BPL = F::kRowBytes / 32;  // bytes of a row that a lane owns
-      const uint32_t a = va.at(r0 + tk, lane * BPL / 16) + (lane * BPL) % 16;
-      if constexpr (BITS == 0) {
-        if constexpr (DPL == 4) {
-          const float4 f = lds_f4(a);
-          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        if constexpr (BITS != 0) {
+          const int r = tok * NG + c * EPC / 64;
+          s = fmaf(ksc[r], a, fmaf(kbi[r], qf[p.G * (D + 4) + hd * NCH + c], s));
         } else {
-          const uint2 f = lds64(a);
-          v[0] = __uint_as_float(f.x), v[1] = __uint_as_float(f.y);
+          s += a;
         }
-      } else {
-        const uint32_t w = lds32(a & ~3u) >> (8 * (a & 3u));
-        const float sc = vsc[tk * NG + lane * DPL / 64], bi = vbi[tk * NG + lane * DPL / 64];
-#pragma unroll
-        for (int i = 0; i < DPL; ++i) v[i] = fmaf(sc, float((w >> (BITS * i)) & ((1u << BITS) - 1u)), bi);
       }
+      s = ok ? s : -INFINITY;
+      float f = 1.0f;
+      if (__any_sync(0xffffffffu, s > m[hb] + kSlack)) {
+        float mx = s;
+        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        f = raise_max(m[hb], mx);
+        l[hb] *= f;
+        f = __shfl_sync(0xffffffffu, f, vh);  // lane vh holds head vh's
 #pragma unroll
-      for (int g = 0; g < GM; ++g) {
-        if (g < p.G) {
-          const float pr = __shfl_sync(0xffffffffu, s[g], tk);
+        for (int i = 0; i < DL; ++i) o[hb][i] *= f;
+      }
+      s = exp2_from(s, m[hb]);
+      l[hb] += s;
+#pragma unroll 2
+      for (int tk = lo; tk < hi; ++tk) {
+        const float pr = __shfl_sync(0xffffffffu, s, 4 * tk + vh);
+        float sc = 1.0f, bi = 0.0f;
+        if constexpr (BITS != 0) {
+          sc = vsc[tk * NG + d0 / 64];
+          bi = vbi[tk * NG + d0 / 64];
+        }
+        // this lane's DL elements of the row: whole chunks, or a part of one
+        constexpr int PART = DL < EPC ? DL : EPC;
 #pragma unroll
-          for (int i = 0; i < DPL; ++i) o[g][i] = fmaf(pr, v[i], o[g][i]);
+        for (int c = 0; c < DL / PART; ++c) {
+          const int e = d0 + c * PART;
+          const uint4 w = lds128(va.at(r0 + tk, e / EPC));
+#pragma unroll
+          for (int i = 0; i < PART / 4; ++i) {
+            float4 x;
+            if constexpr (PART == EPC) {
+              x = four(w, i);
+            } else {  // the part begins at element e % EPC of the chunk
+              uint4 v = w;
+              const int word = (e % EPC) * BITS / 32;
+              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+              v.x = word == 0 ? u[0] : word == 1 ? u[1] : word == 2 ? u[2] : u[3];
+              v.y = word == 0 ? u[1] : u[3];
+              x = four(v, i);
+            }
+            if constexpr (BITS != 0) x = make_float4(fmaf(sc, x.x, bi), fmaf(sc, x.y, bi), fmaf(sc, x.z, bi), fmaf(sc, x.w, bi));
+            float* oo = o[hb] + c * PART + 4 * i;
+            oo[0] = fmaf(pr, x.x, oo[0]);
+            oo[1] = fmaf(pr, x.y, oo[1]);
+            oo[2] = fmaf(pr, x.z, oo[2]);
+            oo[3] = fmaf(pr, x.w, oo[3]);
+          }
         }
       }
     }
@@ -709,15 +834,19 @@ struct FmaAttend {
 
   __device__ __forceinline__ void end(const PagedParams& p, const WarpPart<D>& w, int lane) {
 #pragma unroll
-    for (int g = 0; g < GM; ++g) {
-      if (g < p.G) {
-        const float ls = warp_sum(l[g]);
-        if (lane == 0) {
-          w.ml[2 * g] = m[g];
-          w.ml[2 * g + 1] = ls;
-        }
+    for (int hb = 0; hb < HB; ++hb) {
+      float ls = l[hb];
+      for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+      const int hd = 4 * hb + (lane & 3), vh = 4 * hb + (lane >> 3);
+      if (lane < 4 && hd < p.G) {
+        w.ml[2 * hd] = m[hb];
+        w.ml[2 * hd + 1] = ls;
+      }
+      if (vh < p.G) {
 #pragma unroll
-        for (int i = 0; i < DPL; ++i) w.o[g * (D + 4) + lane * DPL + i] = o[g][i];
+        for (int i = 0; i < DL; i += 4)
+          *reinterpret_cast<float4*>(w.o + vh * (D + 4) + (lane & 7) * DL + i) =
+              make_float4(o[hb][i], o[hb][i + 1], o[hb][i + 2], o[hb][i + 3]);
       }
     }
   }
@@ -736,16 +865,18 @@ __device__ __forceinline__ TokenRange token_range(const PagedParams& p, int b) {
   const int len = raw < 0 ? 0 : raw > cap ? int(cap) : raw;
   return {p.window > 0 && len > p.window ? len - p.window : 0, len};
 }
-__device__ __forceinline__ int tiles_of(TokenRange r, int tile) {
-  return r.end > r.begin ? (r.end + tile - 1) / tile - r.begin / tile : 0;
+// Units of one pair on the line: kSegmentUnits for beginning and ending its
+// segment, then one per tile; none if it has no tokens.
+__device__ __forceinline__ int units_of(TokenRange r, int tile) {
+  return r.end > r.begin ? (r.end + tile - 1) / tile - r.begin / tile + kSegmentUnits : 0;
 }
 
-// The line of U units (tile, pair) in equal pieces for the CTAs that take
-// part, at least min_tiles each: the first `rem` pieces have base + 1 units.
+// The line of U units in equal pieces for the CTAs that take part: the first
+// `rem` pieces have base + 1 units.
 struct Pieces {
   int n, base, rem;
   __device__ __forceinline__ Pieces(const PagedParams& p, int U) {
-    n = min((U + p.min_tiles - 1) / p.min_tiles, p.ncta);
+    n = min(U, p.ncta);
     base = n ? U / n : 0;
     rem = U - base * n;
   }
@@ -774,16 +905,19 @@ struct Walk {
     b = lo;
   }
   __device__ __forceinline__ bool next(Segment& s) {
-    if (u >= u1) return false;
-    while (prefix[b + 1] * Hkv <= u) ++b;  // ends: u < prefix[B] * Hkv
-    s.b = b;
-    s.nt = prefix[b + 1] - prefix[b];
-    const int r = u - prefix[b] * Hkv;
-    s.h = r / s.nt;
-    s.i0 = r - s.h * s.nt;
-    s.i1 = min(s.nt, s.i0 + u1 - u);
-    u += s.i1 - s.i0;
-    return true;
+    while (u < u1) {
+      while (prefix[b + 1] * Hkv <= u) ++b;  // ends: u < prefix[B] * Hkv
+      const int nu = prefix[b + 1] - prefix[b], r = u - prefix[b] * Hkv;
+      s.b = b;
+      s.h = r / nu;
+      s.nt = nu - kSegmentUnits;
+      const int first = r - s.h * nu, last = min(nu, first + u1 - u);
+      u += last - first;
+      s.i0 = max(first - kSegmentUnits, 0);
+      s.i1 = last - kSegmentUnits;
+      if (s.i1 > s.i0) return true;
+    }
+    return false;
   }
 };
 
@@ -796,6 +930,12 @@ struct PickAttend<E, BITS, D, NB, true> { using type = CodesAttend<E, BITS, D, N
 template <typename E, int BITS, int D, int NB>
 struct PickAttend<E, BITS, D, NB, false> { using type = FmaAttend<BITS, D, NB>; };
 
+// After a wait that expired: wait, with the limit, for the copies of the last
+// `stages` of `it` uses, which still land in this CTA's shared memory.
+static __device__ __noinline__ void drain(uint64_t* full, int it, int stages) {
+  for (int k = max(0, it - stages); k < it; ++k) mbar_wait(full + k % stages, uint32_t(k / stages) & 1u, nullptr);
+}
+
 // The producer warp: this CTA's tiles into the ring, stage by stage.
 template <typename E, int BITS, int D>
 __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV,
@@ -805,7 +945,8 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
   const int pb = min(p.P, F::kTile), nb = F::kTile / pb;   // rows per box, boxes per tile
   const int p_log = __ffs(p.P) - 1, pb_log = __ffs(pb) - 1;
   const int oob_row = int(p.n_pages * p.Hkv * p.P);  // past the tensor: TMA fills zeros
-  int it = 0;
+  int it = 0, st = 0;
+  uint32_t round = 0;  // parity of the stages' current use
   Segment s;
   while (walk.next(s)) {
     const TokenRange r = token_range(p, s.b);
@@ -816,7 +957,7 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
     int base = ((t0 + s.i0) * F::kTile) >> p_log;
     int cur = load(base + lane), nxt = load(base + 32 + lane);
     for (int i = s.i0; i < s.i1; ++i, ++it) {
-      const int st = it % p.stages, tok = (t0 + i) * F::kTile;
+      const int tok = (t0 + i) * F::kTile;
       if ((tok >> p_log) - base >= 32) {
         base += 32;
         cur = nxt;
@@ -835,9 +976,9 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
       }
       const int n_box = __popc(__ballot_sync(0xffffffffu, need));
       const int64_t krow = (int64_t(page) * p.Hkv + s.h) * p.P + (tj & (p.P - 1));
-      if (it >= p.stages && !mbar_wait(empty + st, uint32_t(it / p.stages - 1) & 1u, p.flags)) {
+      if (it >= p.stages && !mbar_wait(empty + st, round ^ 1u, p.flags)) {
         // the consumers gave up: no more copies, but those under way must land before this CTA may end
-        for (int k = max(0, it - p.stages); k < it; ++k) mbar_wait(full + k % p.stages, uint32_t(k / p.stages) & 1u, nullptr);
+        drain(full, it, p.stages);
         return;
       }
       uint8_t* stage = ring + st * F::kStageBytes;
@@ -871,6 +1012,10 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
         }
         cp_async_arrive(full + st);
       }
+      if (++st == p.stages) {
+        st = 0;
+        round ^= 1u;
+      }
     }
   }
 }
@@ -902,12 +1047,12 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   griddep_launch_dependents();
   griddep_wait();
 
-  // tiles before each sequence
+  // units of the line before each sequence (of one kv head)
   const int per = (p.B + kPagedThreads - 1) / kPagedThreads;
   int mine = 0;
   for (int k = 0; k < per; ++k) {
     const int b = tid * per + k;
-    if (b < p.B) mine += tiles_of(token_range(p, b), F::kTile);
+    if (b < p.B) mine += units_of(token_range(p, b), F::kTile);
   }
   int incl = mine;
 #pragma unroll
@@ -924,7 +1069,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     if (b < p.B) {
       prefix[b] = run;
       if (blockIdx.x == 0) p.prefix[b] = run;
-      run += tiles_of(token_range(p, b), F::kTile);
+      run += units_of(token_range(p, b), F::kTile);
       if (b == p.B - 1) {
         prefix[p.B] = run;
         if (blockIdx.x == 0) p.prefix[p.B] = run;
@@ -945,19 +1090,24 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
   A att;
   Segment s;
-  int it = 0;
+  int it = 0, st = 0;
+  uint32_t round = 0;
   bool dead = false, first = true;
   while (walk.next(s)) {
     const TokenRange r = token_range(p, s.b);
     const int t0 = r.begin / F::kTile;
     att.begin(p, qf, s.b, s.h, warp, lane);
     for (int i = s.i0; i < s.i1; ++i, ++it) {
-      const int st = it % p.stages, tok = (t0 + i) * F::kTile;
-      if (!dead) dead = !mbar_wait(full + st, uint32_t(it / p.stages) & 1u, p.flags);
+      const int tok = (t0 + i) * F::kTile;
+      if (!dead) dead = !mbar_wait(full + st, round, p.flags);
       if (!dead) {
         att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, r.begin - tok, r.end - tok}, warp, lane);
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + st);
+      }
+      if (++st == p.stages) {
+        st = 0;
+        round ^= 1u;
       }
     }
     att.end(p, WarpPart<D>(buf, p.G, warp), lane);
@@ -1006,9 +1156,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     named_barrier(1, 32 * kPagedWarps);
     first = false;
   }
-  // after a wait that expired: copies under way still land in this CTA's memory
-  if (dead)
-    for (int k = max(0, it - p.stages); k < it; ++k) mbar_wait(full + k % p.stages, uint32_t(k / p.stages) & 1u, nullptr);
+  if (dead) drain(full, it, p.stages);
 }
 
 // Joins the segments of one query head (grid: B * Hq blocks) in a fixed
@@ -1024,15 +1172,15 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   griddep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int Hq = p.Hkv * p.G, b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, g = hq % p.G;
-  const int pre = p.prefix[b], nt = p.prefix[b + 1] - pre, all = p.prefix[p.B];
+  const int pre = p.prefix[b], nu = p.prefix[b + 1] - pre, all = p.prefix[p.B];
   E* out = static_cast<E*>(p.out) + int64_t(blockIdx.x) * D;
-  if (nt == 0) {
+  if (nu == 0) {
     for (int d = tid; d < D; d += kMergeThreads) out[d] = Elt<E>::from_f32(0.0f);
     return;
   }
   const Pieces pieces(p, all * p.Hkv);
-  const int a = pre * p.Hkv + h * nt;  // the pair's first unit
-  const int c0 = pieces.of(a), c1 = pieces.of(a + nt - 1), ns = c1 - c0 + 1;
+  const int a = pre * p.Hkv + h * nu;  // the pair's first unit
+  const int c0 = pieces.of(a + kSegmentUnits), c1 = pieces.of(a + nu - 1), ns = c1 - c0 + 1;  // with tiles of it
   if (ns == 1) return;
   const int stride = paged_part_floats(p.G, D);
   // a CTA leaves its first segment in slot 0: the pair is that for all but, perhaps, c0

@@ -14,6 +14,7 @@ constexpr int kPagedThreads = (kPagedWarps + 1) * 32;   // + one producer warp
 constexpr int kMergeThreads = 256;
 constexpr int kPagedMaxBatch = 4096;                    // sequences per decode call
 constexpr int kPagedMaxStages = 16;
+constexpr int kSegmentUnits = 2;                        // a segment costs about as much as two tiles, beside its tiles
 // Two CTAs share an SM: half of its 228 KB each, less 1 KB that every CTA reserves.
 constexpr int kPagedSmem = 115712;
 
@@ -30,7 +31,7 @@ struct PagedFmt {
   static constexpr int kEpc = BITS ? 128 / BITS : 16 / ESIZE;  // elements per chunk
   static constexpr int kGroups = BITS ? D / 64 : 1;
   // Tokens of one stage: about 16 to 32 KB for K and V together.
-  static constexpr int kTile = BITS ? 128 : ESIZE == 2 ? 64 : 32;
+  static constexpr int kTile = ESIZE == 4 ? 32 : BITS ? 128 : 64;
   static constexpr int kKvBytes = kTile * kRowBytes;    // K (or V) of a stage
   static constexpr int kSbBytes = BITS ? kTile * kGroups * ESIZE : 0;  // each of the four scale/bias pieces
   static constexpr int kStageBytes = (2 * kKvBytes + 4 * kSbBytes + 1023) / 1024 * 1024;
@@ -47,16 +48,17 @@ struct PagedParams {
   const void* q;          // [B, Hkv * G, D]
   void* out;              // [B, Hkv * G, D]
   float* part;            // [grid][2][paged_part_floats]: o [G][D], then (m, l) [G]
-  int* prefix;            // [B + 1] tiles of the sequences before b
+  int* prefix;            // [B + 1] units of the sequences before b, per kv head
   const int* tables;      // [B, W]
   const int* lengths;     // [B]
   const float* sinks;     // [Hkv * G] or null
   const void *k_scales, *k_biases, *v_scales, *v_biases;  // of this layer
   int64_t n_pages;
   int B, Hkv, G, P, W, window;
-  int stages, ncta, min_tiles;
+  int stages, ncta;
   int q_off, buf_off, prefix_off, bar_off;  // shared-memory layout
   float scale_log2;
+  uint32_t magic;         // 0x64006400, see raw_u8
   int* flags;
 };
 

@@ -360,7 +360,8 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   const int D = g->head_dim, G = n_q_heads / g->n_kv_heads;
   const sd::PagedSet ks = lookup(g->dtype, g->kv_bits, D, G <= 8 ? 1 : 2);
   if (!ks.decode) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
-  const int64_t max_tiles = (int64_t(table_width) * g->page_size + ks.tile - 1) / ks.tile;
+  // most units (tiles and segment ends) of one sequence and kv head
+  const int64_t max_tiles = (int64_t(table_width) * g->page_size + ks.tile - 1) / ks.tile + sd::kSegmentUnits;
   if (max_tiles * batch * g->n_kv_heads >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "batch * table_width too large");
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
@@ -398,12 +399,12 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   p.W = table_width;
   p.window = window;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.magic = 0x64006400u;
   p.flags = device_flags;
-  p.min_tiles = 1;
 
   // shared memory: as many stages as fit beside the fixed parts
   const int buf = sd::kPagedWarps * sd::paged_warp_floats(G, D) * 4;
-  const int qf = g->dtype == SD_F32 ? (G * D + G * (rb / 16)) * 4 : 0;
+  const int qf = g->dtype == SD_F32 ? G * (D + 4 + rb / 16) * 4 : 0;
   const int pre = (batch + 1) * 4, bars = 2 * sd::kPagedMaxStages * 8;
   auto up = [](int x) { return (x + 127) / 128 * 128; };
   const int fixed = up(qf) + up(buf) + up(pre) + bars + 1024;

@@ -66,6 +66,52 @@ __device__ __forceinline__ void copy_chunk(void* dst, const void* src) {
   }
 }
 
+// Quantize elements [sub * EL, sub * EL + EL) of a row of E whose lanes hold EL
+// elements each, with the affine group-64 rule and the fp32 operations of
+// quantize_row_regs; every lane of the warp calls, `live` ones store.
+template <typename E, int BITS, int EL>
+__device__ __forceinline__ void quantize_part(const E* row, uint8_t* wq, E* sc, E* bi, int sub, bool live) {
+  constexpr int LPG = 64 / EL;  // lanes per quantization group
+  const float n_bins = float((1 << BITS) - 1);
+  float w[EL];
+#pragma unroll
+  for (int e = 0; e < EL; ++e) w[e] = Elt<E>::to_f32(row[sub * EL + e]);
+  float wmax = w[0], wmin = w[0];
+#pragma unroll
+  for (int e = 1; e < EL; ++e) wmax = fmaxf(wmax, w[e]), wmin = fminf(wmin, w[e]);
+#pragma unroll
+  for (int o = 1; o < LPG; o <<= 1) {
+    wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, o));
+    wmin = fminf(wmin, __shfl_xor_sync(0xffffffffu, wmin, o));
+  }
+  float scale = fmaxf(__fdiv_rn(__fsub_rn(wmax, wmin), n_bins), 1e-7f);
+  const bool low = fabsf(wmin) > fabsf(wmax);
+  if (!low) scale = -scale;
+  const float edge = low ? wmin : wmax;
+  const float q0 = rintf(__fdiv_rn(edge, scale));
+  if (q0 != 0.0f) scale = __fdiv_rn(edge, q0);
+  const float bias = q0 == 0.0f ? 0.0f : edge;
+  constexpr int BYTES = EL * BITS / 8;
+  uint32_t words[(BYTES + 3) / 4] = {};
+#pragma unroll
+  for (int e = 0; e < EL; ++e) {
+    float c = rintf(__fdiv_rn(__fsub_rn(w[e], bias), scale));
+    c = fminf(fmaxf(c, 0.0f), n_bins);
+    words[e * BITS / 32] |= uint32_t(c) << (e * BITS % 32);
+  }
+  if (!live) return;
+  uint8_t* d = wq + sub * BYTES;
+  if constexpr (BYTES == 16) *reinterpret_cast<uint4*>(d) = make_uint4(words[0], words[1], words[2], words[3]);
+  else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(d) = make_uint2(words[0], words[1]);
+  else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(d) = words[0];
+  else if constexpr (BYTES == 2) *reinterpret_cast<uint16_t*>(d) = uint16_t(words[0]);
+  else *d = uint8_t(words[0]);
+  if (sub % LPG == 0) {
+    sc[sub / LPG] = Elt<E>::from_f32(scale);
+    bi[sub / LPG] = Elt<E>::from_f32(bias);
+  }
+}
+
 }  // namespace
 
 // A warp takes rows of one kind (query, key or value) and of few tokens: a
@@ -82,7 +128,7 @@ __device__ __forceinline__ void copy_chunk(void* dst, const void* src) {
 // cos and sin, one pair per lane, and exchanges them through shared memory.
 // No barrier wider than a warp.
 // BITS 4 / 8: key and value rows are rounded to E, staged in shared memory and
-// quantized from there, a warp per row.
+// quantized from there by the group of lanes that holds the row.
 template <typename E, int V, int BITS, bool TRAD>
 __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int CPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // chunk pairs per lane for head_dim up to 256
@@ -266,16 +312,13 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
     if constexpr (BITS != 0) {
       if (paged) {
         __syncwarp();
-        const int NG = D / 64, words = D * BITS / 32;
-        for (int g = 0; g < groups; ++g) {  // the row that group g staged
-          const int64_t s0 = __shfl_sync(0xffffffffu, live ? slot + int64_t(hd) * p.P : int64_t(-1), g << lg_log);
-          if (s0 < 0) continue;
-          uint32_t* wq = static_cast<uint32_t*>(is_v ? p.v_data : p.k_data) + s0 * words;
-          E* sc = static_cast<E*>(is_v ? p.v_scales : p.k_scales) + s0 * NG;
-          E* bi = static_cast<E*>(is_v ? p.v_biases : p.k_biases) + s0 * NG;
-          if (D == 128) quantize_row_warp<E, BITS, 128>(stage + g * D, wq, sc, bi, lane);
-          else quantize_row_warp<E, BITS, 64>(stage + g * D, wq, sc, bi, lane);
-        }
+        const int64_t row = slot + int64_t(hd) * p.P;
+        uint8_t* wq = static_cast<uint8_t*>(is_v ? p.v_data : p.k_data) + row * (D * BITS / 8);
+        E* sc = static_cast<E*>(is_v ? p.v_scales : p.k_scales) + row * (D / 64);
+        E* bi = static_cast<E*>(is_v ? p.v_biases : p.k_biases) + row * (D / 64);
+        // head_dim 64 and 128: a lane has 2V neighbours, or 4 where 2V would need more than a warp
+        if (V == 1 && D == 128) quantize_part<E, BITS, 4>(stage + grp * D, wq, sc, bi, sub, live);
+        else quantize_part<E, BITS, 2 * V>(stage + grp * D, wq, sc, bi, sub, live);
         __syncwarp();
       }
     }

@@ -347,6 +347,37 @@ def test_decode_scales_that_grow_along_the_sequence(cuda):
     assert_close(out.double().cpu().numpy().reshape(-1, 128), ref.cpu().numpy().reshape(-1, 128), "bf16")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_scales_that_jump_while_the_maximum_lags(cuda, dtype, bits):
+    """The running maximum may lag the true one by 8 (log2 units): p up to 256 meets value scales that jump 2^7-fold
+    between tiles, so p times the scaled s_v comes near fp16's largest number."""
+    import torch
+    import sparse_decode as sd
+    d, page, n = 128, 64, 64 * 12
+    pool = Pool(torch, sd, dtype, bits, 1, d, page, 13, 15)
+    tables = tables_of(torch, [n], page, 13, 16)
+    # every key of page j: codes equal, so that the score is a constant of the page, rising by 7.5 after page 3
+    q = torch.ones(1, 4, d, device="cuda", dtype=tdt(torch, dtype))
+    kc, ks, kb = pool.arrays[0]
+    kc.zero_(), ks.fill_(1.0)
+    vs, vb = pool.arrays[1][1:]
+    vs.abs_(), vb.copy_(-vs)
+    for j in range(12):
+        pg = int(tables[0, j])
+        kb[pg] = 0.0 if j < 4 else 7.5 * math.log(2) / math.sqrt(d)
+        for r in range(2):
+            vs[pg, ..., r] *= 2.0 ** -7 if j < 8 - 4 * r else 1.0
+        vb[pg] = -vs[pg]
+    words = pool.arrays[1][0].long() & 0xFFFFFFFF
+    codes = torch.stack([(words >> (bits * j)) & ((1 << bits) - 1) for j in range(32 // bits)], -1).flatten(-2).double()
+    grow = lambda t: t.double().repeat_interleave(64, -1)  # noqa: E731
+    pool.values = [grow(kb), codes * grow(vs) + grow(vb)]
+    out = sd.paged_decode(q, pool.pages, tables, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    ref = decode64(q, pool, tables, [n], 1 / math.sqrt(d))
+    assert_close(out.double().cpu().numpy().reshape(-1, d), ref.cpu().numpy().reshape(-1, d), dtype)
+
+
 @pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("bf16", 8), ("f32", 0)])
 def test_decode_nan_in_a_valid_token_reaches_its_heads_only(cuda, dtype, bits):
     import torch
