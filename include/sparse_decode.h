@@ -350,8 +350,9 @@ int32_t sd_copy_pages(const sd_pages* pages, const int32_t* src, const int32_t* 
  * token is the new one, stored before the call). sinks: [n_q_heads] fp32 as
  * in sd_set_sinks, or NULL. A length of 0 gives zeros. Query heads per kv
  * head: 1 .. 16. Lengths and tables are read on the device only. The
- * workspace (sd_paged_workspace bytes, 16-byte aligned, contents do not
- * matter) must not be shared by calls that may overlap. Pages past a
+ * workspace (sd_paged_workspace bytes -- they depend on n_q_heads, the pool and
+ * the GPU, not on the batch -- 16-byte aligned, contents do not matter) must
+ * not be shared by calls that may overlap. Pages past a
  * sequence's length, or before its window, are not read. An index or length
  * out of range sets bit 2 of *device_flags; rows of such a page read as 0. */
 int32_t sd_paged_workspace(const sd_pages* pages, int32_t batch, int32_t n_q_heads, int64_t* bytes);

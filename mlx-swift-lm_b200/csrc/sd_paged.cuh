@@ -1044,39 +1044,49 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     prefetch_tensormap(&tmK);
     prefetch_tensormap(&tmV);
   }
-  griddep_launch_dependents();
+  // The merge may start from here on: what ran before this kernel is complete then, so that it may read the lengths.
   griddep_wait();
+  griddep_launch_dependents();
 
   // units of the line before each sequence (of one kv head)
-  const int per = (p.B + kPagedThreads - 1) / kPagedThreads;
-  int mine = 0;
-  for (int k = 0; k < per; ++k) {
-    const int b = tid * per + k;
-    if (b < p.B) mine += units_of(token_range(p, b), F::kTile);
-  }
-  int incl = mine;
+  if (p.B < 32) {  // every warp for itself: no barrier on the way to the first copy
+    prefix += warp * 32;
+    int incl = lane < p.B ? units_of(token_range(p, lane), F::kTile) : 0;
 #pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, x);
-    if (lane >= x) incl += v;
-  }
-  if (lane == 31) warp_tot[warp] = incl;
-  __syncthreads();
-  int run = incl - mine;
-  for (int w = 0; w < warp; ++w) run += warp_tot[w];
-  for (int k = 0; k < per; ++k) {
-    const int b = tid * per + k;
-    if (b < p.B) {
-      prefix[b] = run;
-      if (blockIdx.x == 0) p.prefix[b] = run;
-      run += units_of(token_range(p, b), F::kTile);
-      if (b == p.B - 1) {
-        prefix[p.B] = run;
-        if (blockIdx.x == 0) p.prefix[p.B] = run;
+    for (int x = 1; x < 32; x <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += v;
+    }
+    const int before = __shfl_up_sync(0xffffffffu, incl, 1);
+    prefix[lane] = lane ? before : 0;  // B + 1 entries matter
+    __syncthreads();                   // the barriers of the ring are set up, too
+  } else {
+    const int per = (p.B + kPagedThreads - 1) / kPagedThreads;
+    int mine = 0;
+    for (int k = 0; k < per; ++k) {
+      const int b = tid * per + k;
+      if (b < p.B) mine += units_of(token_range(p, b), F::kTile);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += v;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    int run = incl - mine;
+    for (int w = 0; w < warp; ++w) run += warp_tot[w];
+    for (int k = 0; k < per; ++k) {
+      const int b = tid * per + k;
+      if (b < p.B) {
+        prefix[b] = run;
+        run += units_of(token_range(p, b), F::kTile);
+        if (b == p.B - 1) prefix[p.B] = run;
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
 
   const Pieces pieces(p, prefix[p.B] * p.Hkv);
   if (int(blockIdx.x) >= pieces.n) return;
@@ -1165,14 +1175,29 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
 // their bytes (a few MB at most, from L2): warp w takes the segments w, w + 8,
 // ..., each lane first the (m, l) of one of them, and the o rows are loaded
 // eight at a time, the first eight before the weights are known.
-template <typename E, int D>
+template <typename E, int D, int TILE>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedParams p) {
   constexpr int NW = kMergeThreads / 32, V = D / 32, BATCH = 8;
   __shared__ float red[NW][D], top[NW], tot[NW];
-  griddep_wait();
+  __shared__ int sums[NW][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int Hq = p.Hkv * p.G, b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, g = hq % p.G;
-  const int pre = p.prefix[b], nu = p.prefix[b + 1] - pre, all = p.prefix[p.B];
+  // The pair's place on the line, from the lengths, while the segments are still being worked on.
+  int pre = 0, all = 0;
+  for (int i = tid; i < p.B; i += kMergeThreads) {
+    const int n = units_of(token_range(p, i), TILE);
+    all += n;
+    pre += i < b ? n : 0;
+  }
+  pre = __reduce_add_sync(0xffffffffu, pre);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (lane == 0) sums[warp][0] = pre, sums[warp][1] = all;
+  __syncthreads();
+  pre = all = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) pre += sums[w][0], all += sums[w][1];
+  const int nu = units_of(token_range(p, b), TILE);
+  griddep_wait();
   E* out = static_cast<E*>(p.out) + int64_t(blockIdx.x) * D;
   if (nu == 0) {
     for (int d = tid; d < D; d += kMergeThreads) out[d] = Elt<E>::from_f32(0.0f);
@@ -1233,7 +1258,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
     tot[warp] = L;
   }
   __syncthreads();
-  if (tid >= D) return;
+  if (tid >= D) return;  // D <= kMergeThreads
   M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < NW; ++w) M = fmaxf(M, top[w]);

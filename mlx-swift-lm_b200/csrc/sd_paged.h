@@ -48,7 +48,6 @@ struct PagedParams {
   const void* q;          // [B, Hkv * G, D]
   void* out;              // [B, Hkv * G, D]
   float* part;            // [grid][2][paged_part_floats]: o [G][D], then (m, l) [G]
-  int* prefix;            // [B + 1] units of the sequences before b, per kv head
   const int* tables;      // [B, W]
   const int* lengths;     // [B]
   const float* sinks;     // [Hkv * G] or null
@@ -64,7 +63,7 @@ struct PagedParams {
 
 struct PagedSet {
   const void* decode;  // paged_decode_kernel<E, BITS, D, NB>(PagedParams, CUtensorMap, CUtensorMap)
-  const void* merge;   // paged_merge_kernel<E, D>(PagedParams, int tile)
+  const void* merge;   // paged_merge_kernel<E, D, tile>(PagedParams)
   int tile, stage_bytes, row_bytes, groups;
 };
 // nb: blocks of 8 query heads per kv head (1 or 2). Null members without an instantiation.

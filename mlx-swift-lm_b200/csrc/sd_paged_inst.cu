@@ -24,7 +24,7 @@ static PagedSet make_paged() {
   using F = PagedFmt<sizeof(ET), SD_BITS, D>;
   PagedSet s;
   s.decode = reinterpret_cast<const void*>(&paged_decode_kernel<ET, SD_BITS, D, NB>);
-  s.merge = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D>);
+  s.merge = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D, F::kTile>);
   s.tile = F::kTile;
   s.stage_bytes = F::kStageBytes;
   s.row_bytes = F::kRowBytes;

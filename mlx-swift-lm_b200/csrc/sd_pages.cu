@@ -314,10 +314,9 @@ int32_t sd_copy_pages(const sd_pages* g, const int32_t* src, const int32_t* dst,
                 sd::kCopyThreads, 0, static_cast<cudaStream_t>(stream), args);
 }
 
-// prefix [batch + 1] ints, then two segments (o, m, l) per CTA
-static int64_t workspace_bytes_of(const sd_pages* g, int32_t batch, int32_t n_q_heads, int ctas) {
-  return (int64_t(batch + 1) * 4 + 255) / 256 * 256 +
-         int64_t(ctas) * 2 * sd::paged_part_floats(n_q_heads / g->n_kv_heads, g->head_dim) * 4;
+// two segments (o, m, l) per CTA
+static int64_t workspace_bytes_of(const sd_pages* g, int32_t n_q_heads, int ctas) {
+  return int64_t(ctas) * 2 * sd::paged_part_floats(n_q_heads / g->n_kv_heads, g->head_dim) * 4;
 }
 
 static int32_t check_heads(const sd_pages* g, int32_t batch, int32_t n_q_heads) {
@@ -335,7 +334,7 @@ int32_t sd_paged_workspace(const sd_pages* g, int32_t batch, int32_t n_q_heads, 
   if (int32_t rc = check_heads(g, batch, n_q_heads)) return rc;
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
-  *bytes = workspace_bytes_of(g, batch, n_q_heads, decode_ctas(sms));
+  *bytes = workspace_bytes_of(g, n_q_heads, decode_ctas(sms));
   return SD_OK;
 }
 
@@ -366,9 +365,9 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
   const int max_ctas = decode_ctas(sms);
-  if (workspace_bytes < workspace_bytes_of(g, batch, n_q_heads, max_ctas))
+  if (workspace_bytes < workspace_bytes_of(g, n_q_heads, max_ctas))
     return fail(SD_ERR_CAPACITY, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                (long long)workspace_bytes_of(g, batch, n_q_heads, max_ctas));
+                (long long)workspace_bytes_of(g, n_q_heads, max_ctas));
 
   const int64_t rows = layer_rows(g);
   const int rb = row_bytes(g), box = std::min(g->page_size, ks.tile);
@@ -379,8 +378,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   sd::PagedParams p{};
   p.q = q;
   p.out = out;
-  p.prefix = static_cast<int*>(workspace);
-  p.part = static_cast<float*>(at(workspace, (int64_t(batch + 1) * 4 + 255) / 256 * 256));
+  p.part = static_cast<float*>(workspace);
   p.tables = tables;
   p.lengths = lengths;
   p.sinks = sinks;
@@ -405,7 +403,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   // shared memory: as many stages as fit beside the fixed parts
   const int buf = sd::kPagedWarps * sd::paged_warp_floats(G, D) * 4;
   const int qf = g->dtype == SD_F32 ? G * (D + 4 + rb / 16) * 4 : 0;
-  const int pre = (batch + 1) * 4, bars = 2 * sd::kPagedMaxStages * 8;
+  const int pre = (batch < 32 ? 32 * (sd::kPagedWarps + 1) : batch + 1) * 4, bars = 2 * sd::kPagedMaxStages * 8;
   auto up = [](int x) { return (x + 127) / 128 * 128; };
   const int fixed = up(qf) + up(buf) + up(pre) + bars + 1024;
   p.stages = std::min((sd::kPagedSmem - fixed) / ks.stage_bytes, sd::kPagedMaxStages);

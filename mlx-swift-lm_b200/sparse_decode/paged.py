@@ -32,17 +32,17 @@ from . import DTYPES, SDError, SDPages, SDRotation, SDRows, _check, _torch_dtype
 torch = None
 _device = _raw_stream = None
 _CODE: dict = {}
-_I32 = _F32 = None
+_I32 = _F32 = _U8 = None
 _L: Optional[ctypes.CDLL] = None
 
 
 def _load() -> None:
-    global torch, _device, _raw_stream, _I32, _F32, _L
+    global torch, _device, _raw_stream, _I32, _F32, _U8, _L
     import torch as t
     _L = lib()
     t.cuda.init()
     _device, _raw_stream = t.cuda.current_device, t._C._cuda_getCurrentRawStream
-    _I32, _F32 = t.int32, t.float32
+    _I32, _F32, _U8 = t.int32, t.float32, t.uint8
     _CODE.update({_torch_dtype(n): c for n, c in DTYPES.items()})
     torch = t
 
@@ -95,6 +95,19 @@ def _like(x, stream):
         return y if y.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with torch.cuda.stream(stream):
         return _like(x, None)
+
+
+def _out(x, out, name: str, dtype, dev: int, dim: int, stream) -> tuple:
+    """The output for x's rows -- `out`, or a new tensor -- and its sd_rows."""
+    if out is not None:
+        if out.shape != x.shape:
+            raise ValueError(f"{name} must have its input's shape")
+        return out, _rows(out, name, dtype, dev, dim)[0]
+    out = _like(x, stream)
+    st = out.stride()
+    if len(st) == 3:
+        return out, SDRows(out.data_ptr(), 0, st[0], st[1])
+    return out, SDRows(out.data_ptr(), st[0], st[2], st[1])
 
 
 def _handle(stream, dev: int) -> int:
@@ -195,22 +208,14 @@ def rotary(q, k, positions, inv_freq, *, traditional: bool = False, factor: floa
     hq = hk = 0
     if q is not None:
         qr, batch, tokens, hq = _rows(q, "q", dt, dev, dim)
-        if q_out is None:
-            q_out = _like(q, stream)
-        elif q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
-        qo = _rows(q_out, "q_out", dt, dev, dim)[0]
+        q_out, qo = _out(q, q_out, "q_out", dt, dev, dim, stream)
     if k is not None:
         kr, b, n, hk = _rows(k, "k", dt, dev, dim)
         if q is None:
             batch, tokens = b, n
         elif b != batch or n != tokens or k.dim() != q.dim():
             raise ValueError("q and k must have the same tokens")
-        if k_out is None:
-            k_out = _like(k, stream)
-        elif k_out.shape != k.shape:
-            raise ValueError("k_out must have k's shape")
-        ko = _rows(k_out, "k_out", dt, dev, dim)[0]
+        k_out, ko = _out(k, k_out, "k_out", dt, dev, dim, stream)
     pos = _arg(positions, "positions", _I32, dev, (tokens,) if ref.dim() == 3 else (batch, tokens))
     rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
     _check(_L.sd_rotary(rot, code, dim, batch, tokens, pos, hq, qr, qo, hk, kr, ko, _handle(stream, dev)))
@@ -250,7 +255,8 @@ class KVPages:
             ptrs = (_arg(k, "k", dt, dev), _arg(v, "v", dt, dev, shape), None, None, None, None)
         self.k, self.v = k, v
         self.k_scales, self.k_biases, self.v_scales, self.v_biases = small
-        self.bits, self.device, self.dtype = bits, dev, dt
+        self.bits, self.device, self.torch_device, self.dtype = bits, dev, k.device, dt
+        self.workspace: dict = {}  # bytes of paged_decode's workspace by query heads
         self.n_layers, self.n_pages = n_layers, n_pages
         self.n_kv_heads, self.page_size, self.head_dim = hkv, page, dim
         self.struct = SDPages(*ptrs, n_pages, n_layers, hkv, dim, page, _dtype_code(dt), bits, 64 if bits else 0, 0)
@@ -289,11 +295,7 @@ def paged_append(pages: KVPages, k, v, tables, positions, *, seq=None, layer: in
         qr, qb, qn, hq = _rows(q, "q", dt, dev, dim)
         if q.dim() != 3 or qn != n:
             raise ValueError("q must have k's tokens")
-        if q_out is None:
-            q_out = _like(q, stream)
-        elif q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
-        qo = _rows(q_out, "q_out", dt, dev, dim)[0]
+        q_out, qo = _out(q, q_out, "q_out", dt, dev, dim, stream)
     if q is not None or inv_freq is not None or q_norm is not None or k_norm is not None:
         rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
     batch, width = tables.shape
@@ -341,20 +343,22 @@ def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = No
     hq = shape[1]
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    need = ctypes.c_int64()
-    if batch:
-        _check(_L.sd_paged_workspace(pages.struct, batch, hq, need))
+    need = pages.workspace.get(hq)
+    if need is None:  # the bytes depend on the pool's heads and hq alone
+        n = ctypes.c_int64()
+        _check(_L.sd_paged_workspace(pages.struct, 1, hq, n))
+        need = pages.workspace[hq] = n.value
     if out is None:
         out = _like(q, stream)
     if stream is None:
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        work = torch.empty(need, dtype=_U8, device=pages.torch_device)
     else:
         with torch.cuda.stream(stream):
-            work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            work = torch.empty(need, dtype=_U8, device=pages.torch_device)
     _check(_L.sd_paged_decode(pages.struct, layer, _arg(q, "q", dt, dev), batch, hq, _arg(tables, "tables", _I32, dev),
                               width, _arg(lengths, "lengths", _I32, dev, (batch,)), scale, window,
                               _arg(sinks, "sinks", _F32, dev, (hq,)), _arg(out, "out", dt, dev, shape), work.data_ptr(),
-                              need.value, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
+                              need, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
     return out
 
 
