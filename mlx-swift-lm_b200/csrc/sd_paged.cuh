@@ -693,21 +693,27 @@ struct CodesAttend {
 
 // ---------------------------------------------------------------------------
 // fp32 pools (dense, or codes with fp32 scales) on the FMA pipes: the tensor
-// cores have no fp32 product. A warp has 8 tokens of a tile and takes the heads
-// four at a time. q.k: lane = (token, head), so a score needs no exchange and
+// cores have no fp32 product. A warp has 8 tokens of a tile and HB blocks of
+// four heads. q.k: lane = (token, head), so a score needs no exchange and
 // no array over heads, which keeps the code short -- a small call spends more
 // on fetching instructions than on executing them. p.v: lane = (head, eighth
 // of the dims), p from the score's lane by one shuffle per token. q (times
 // scale * log2 e, rows padded against bank conflicts) and, for codes, its sum
 // over each 16-byte chunk lie in shared memory.
 // ---------------------------------------------------------------------------
-template <int BITS, int D, int NB>
+template <int BITS, int D, int HB>
 struct FmaAttend {
   using F = PagedFmt<4, BITS, D>;
-  static constexpr int HB = 2 * NB, NCH = F::kNChunk, EPC = F::kEpc, NG = F::kGroups;  // HB: blocks of four heads
+  static constexpr int NCH = F::kNChunk, EPC = F::kEpc, NG = F::kGroups;
   static constexpr int TW = 8, DL = D / 8;
   static_assert(F::kTile == TW * kPagedWarps, "eight tokens per warp");
   float m[HB], l[HB], o[HB][DL];  // of head 4 hb + lane % 4 (m, l) and 4 hb + lane / 8 (o)
+
+  // Element i of a lane's dims: every eighth chunk of a dense row, so that the
+  // eight lanes of a head read all banks; neighbours of a row of codes.
+  static __device__ __forceinline__ int dim(int lane, int i) {
+    return BITS == 0 ? 4 * (8 * (i / 4) + (lane & 7)) + i % 4 : (lane & 7) * DL + i;
+  }
 
   // Four elements of a chunk, from element 4i on.
   static __device__ __forceinline__ float4 four(const uint4& w, int i) {
@@ -753,81 +759,99 @@ struct FmaAttend {
     const TileAddr<F> ka{smem_u32(t.stage), t.pb_log}, va{smem_u32(t.stage) + F::kKvBytes, t.pb_log};
     const float* ksc = reinterpret_cast<const float*>(t.stage + 2 * F::kKvBytes) + r0 * NG;
     const float *kbi = ksc + F::kTile * NG, *vsc = ksc + 2 * F::kTile * NG, *vbi = ksc + 3 * F::kTile * NG;
-    const int tok = lane >> 2, vh = lane >> 3, d0 = (lane & 7) * DL;  // q.k: (tok, lane % 4); p.v: (vh, d0 ..)
+    const int tok = lane >> 2, vh = lane >> 3, d0 = (lane & 7) * DL;  // q.k: (tok, lane % 4); p.v: (vh, dims)
     const bool ok = tok >= lo && tok < hi;
+    // dense rows: chunk c of row r of the eight lies at rows + (c / 8) box + 128 r + 16 ((c % 8) ^ r)
+    const uint32_t krow = ka.row_at(r0) + tok * F::kBoxBytes, vrows = krow - tok * F::kBoxBytes + F::kKvBytes;
+    const uint32_t box = uint32_t(F::kBoxBytes) << t.pb_log;
+    const float* qrow[HB];
+    float s[HB];
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-      if (4 * hb >= p.G) break;
-      const int hd = min(4 * hb + (lane & 3), p.G - 1);  // a head past the last repeats it
-      const float* qrow = qf + hd * (D + 4);
-      float s = 0.0f;
+      qrow[hb] = qf + min(4 * hb + (lane & 3), p.G - 1) * (D + 4);  // a head past the last repeats it
+      s[hb] = 0.0f;
+    }
 #pragma unroll 4
-      for (int c = 0; c < NCH; ++c) {
-        const uint4 w = lds128(ka.at(r0 + tok, c));
+    for (int c = 0; c < NCH; ++c) {
+      const uint4 w = lds128(BITS == 0 ? krow + (c / 8) * box + (((c % 8) ^ tok) << 4) : ka.at(r0 + tok, c));
+      float4 x[EPC / 4];
+#pragma unroll
+      for (int i = 0; i < EPC / 4; ++i) x[i] = four(w, i);
+      float sc = 1.0f, bi = 0.0f;
+      if constexpr (BITS != 0) {
+        sc = ksc[tok * NG + c * EPC / 64];
+        bi = kbi[tok * NG + c * EPC / 64];
+      }
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb) {
         float a = 0.0f;
 #pragma unroll
         for (int i = 0; i < EPC / 4; ++i) {
-          const float4 x = four(w, i), y = *reinterpret_cast<const float4*>(qrow + c * EPC + 4 * i);
-          a = fmaf(x.x, y.x, a);
-          a = fmaf(x.y, y.y, a);
-          a = fmaf(x.z, y.z, a);
-          a = fmaf(x.w, y.w, a);
+          const float4 y = *reinterpret_cast<const float4*>(qrow[hb] + c * EPC + 4 * i);
+          a = fmaf(x[i].x, y.x, a);
+          a = fmaf(x[i].y, y.y, a);
+          a = fmaf(x[i].z, y.z, a);
+          a = fmaf(x[i].w, y.w, a);
         }
         if constexpr (BITS != 0) {
-          const int r = tok * NG + c * EPC / 64;
-          s = fmaf(ksc[r], a, fmaf(kbi[r], qf[p.G * (D + 4) + hd * NCH + c], s));
+          const int hd = min(4 * hb + (lane & 3), p.G - 1);
+          s[hb] = fmaf(sc, a, fmaf(bi, qf[p.G * (D + 4) + hd * NCH + c], s[hb]));
         } else {
-          s += a;
+          s[hb] += a;
         }
       }
-      s = ok ? s : -INFINITY;
-      float f = 1.0f;
-      if (__any_sync(0xffffffffu, s > m[hb] + kSlack)) {
-        float mx = s;
+    }
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb) {
+      s[hb] = ok ? s[hb] : -INFINITY;
+      if (__any_sync(0xffffffffu, s[hb] > m[hb] + kSlack)) {
+        float mx = s[hb];
         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        f = raise_max(m[hb], mx);
+        float f = raise_max(m[hb], mx);
         l[hb] *= f;
         f = __shfl_sync(0xffffffffu, f, vh);  // lane vh holds head vh's
 #pragma unroll
         for (int i = 0; i < DL; ++i) o[hb][i] *= f;
       }
-      s = exp2_from(s, m[hb]);
-      l[hb] += s;
+      s[hb] = exp2_from(s[hb], m[hb]);
+      l[hb] += s[hb];
+    }
 #pragma unroll 2
-      for (int tk = lo; tk < hi; ++tk) {
-        const float pr = __shfl_sync(0xffffffffu, s, 4 * tk + vh);
-        float sc = 1.0f, bi = 0.0f;
-        if constexpr (BITS != 0) {
-          sc = vsc[tk * NG + d0 / 64];
-          bi = vbi[tk * NG + d0 / 64];
+    for (int tk = lo; tk < hi; ++tk) {
+      float v[DL];
+      if constexpr (BITS == 0) {
+        const uint32_t at = vrows + tk * F::kBoxBytes + (((lane & 7) ^ tk) << 4);
+#pragma unroll
+        for (int c = 0; c < DL / 4; ++c) {
+          const float4 x = lds_f4(at + c * box);
+          v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
         }
-        // this lane's DL elements of the row: whole chunks, or a part of one
+      } else {  // this lane's DL elements: whole chunks, or a part of one
         constexpr int PART = DL < EPC ? DL : EPC;
+        const float sc = vsc[tk * NG + d0 / 64], bi = vbi[tk * NG + d0 / 64];
 #pragma unroll
         for (int c = 0; c < DL / PART; ++c) {
           const int e = d0 + c * PART;
-          const uint4 w = lds128(va.at(r0 + tk, e / EPC));
+          uint4 w = lds128(va.at(r0 + tk, e / EPC));
+          if constexpr (PART < EPC) {  // the part begins at element e % EPC of the chunk
+            const int word = (e % EPC) * BITS / 32;
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            w.x = word == 0 ? u[0] : word == 1 ? u[1] : word == 2 ? u[2] : u[3];
+            w.y = word == 0 ? u[1] : u[3];
+          }
 #pragma unroll
           for (int i = 0; i < PART / 4; ++i) {
-            float4 x;
-            if constexpr (PART == EPC) {
-              x = four(w, i);
-            } else {  // the part begins at element e % EPC of the chunk
-              uint4 v = w;
-              const int word = (e % EPC) * BITS / 32;
-              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-              v.x = word == 0 ? u[0] : word == 1 ? u[1] : word == 2 ? u[2] : u[3];
-              v.y = word == 0 ? u[1] : u[3];
-              x = four(v, i);
-            }
-            if constexpr (BITS != 0) x = make_float4(fmaf(sc, x.x, bi), fmaf(sc, x.y, bi), fmaf(sc, x.z, bi), fmaf(sc, x.w, bi));
-            float* oo = o[hb] + c * PART + 4 * i;
-            oo[0] = fmaf(pr, x.x, oo[0]);
-            oo[1] = fmaf(pr, x.y, oo[1]);
-            oo[2] = fmaf(pr, x.z, oo[2]);
-            oo[3] = fmaf(pr, x.w, oo[3]);
+            const float4 x = four(w, i);
+            float* vv = v + c * PART + 4 * i;
+            vv[0] = fmaf(sc, x.x, bi), vv[1] = fmaf(sc, x.y, bi), vv[2] = fmaf(sc, x.z, bi), vv[3] = fmaf(sc, x.w, bi);
           }
         }
+      }
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb) {
+        const float pr = __shfl_sync(0xffffffffu, s[hb], 4 * tk + vh);
+#pragma unroll
+        for (int i = 0; i < DL; ++i) o[hb][i] = fmaf(pr, v[i], o[hb][i]);
       }
     }
   }
@@ -845,7 +869,7 @@ struct FmaAttend {
       if (vh < p.G) {
 #pragma unroll
         for (int i = 0; i < DL; i += 4)
-          *reinterpret_cast<float4*>(w.o + vh * (D + 4) + (lane & 7) * DL + i) =
+          *reinterpret_cast<float4*>(w.o + vh * (D + 4) + dim(lane, i)) =
               make_float4(o[hb][i], o[hb][i + 1], o[hb][i + 2], o[hb][i + 3]);
       }
     }

@@ -62,20 +62,20 @@ struct PagedParams {
 };
 
 struct PagedSet {
-  const void* decode;  // paged_decode_kernel<E, BITS, D, NB>(PagedParams, CUtensorMap, CUtensorMap)
+  const void* decode;  // paged_decode_kernel<E, BITS, D, blocks of heads>(PagedParams, CUtensorMap, CUtensorMap)
   const void* merge;   // paged_merge_kernel<E, D, tile>(PagedParams)
   int tile, stage_bytes, row_bytes, groups;
 };
-// nb: blocks of 8 query heads per kv head (1 or 2). Null members without an instantiation.
-PagedSet paged_e0_b0(int D, int nb);
-PagedSet paged_e1_b0(int D, int nb);
-PagedSet paged_e2_b0(int D, int nb);
-PagedSet paged_e0_b4(int D, int nb);
-PagedSet paged_e1_b4(int D, int nb);
-PagedSet paged_e2_b4(int D, int nb);
-PagedSet paged_e0_b8(int D, int nb);
-PagedSet paged_e1_b8(int D, int nb);
-PagedSet paged_e2_b8(int D, int nb);
+// For G query heads per kv head; null members without an instantiation.
+PagedSet paged_e0_b0(int D, int G);
+PagedSet paged_e1_b0(int D, int G);
+PagedSet paged_e2_b0(int D, int G);
+PagedSet paged_e0_b4(int D, int G);
+PagedSet paged_e1_b4(int D, int G);
+PagedSet paged_e2_b4(int D, int G);
+PagedSet paged_e0_b8(int D, int G);
+PagedSet paged_e1_b8(int D, int G);
+PagedSet paged_e2_b8(int D, int G);
 
 // ---------------------------------------------------------------------------
 

@@ -32,10 +32,17 @@ static PagedSet make_paged() {
   return s;
 }
 
-PagedSet SD_NAME(SD_E, SD_BITS)(int D, int nb) {
-  if (D == 64) return nb == 1 ? make_paged<64, 1>() : make_paged<64, 2>();
-  if (D == 128) return nb == 1 ? make_paged<128, 1>() : make_paged<128, 2>();
-  return PagedSet{nullptr, nullptr, 0, 0, 0, 0};
+template <int D>
+static PagedSet pick_heads(int G) {
+#if SD_E == 0
+  return G <= 4 ? make_paged<D, 1>() : G <= 8 ? make_paged<D, 2>() : make_paged<D, 4>();  // blocks of 4 heads
+#else
+  return G <= 8 ? make_paged<D, 1>() : make_paged<D, 2>();  // blocks of 8
+#endif
+}
+
+PagedSet SD_NAME(SD_E, SD_BITS)(int D, int G) {
+  return D == 64 ? pick_heads<64>(G) : D == 128 ? pick_heads<128>(G) : PagedSet{nullptr, nullptr, 0, 0, 0, 0};
 }
 
 }  // namespace sd

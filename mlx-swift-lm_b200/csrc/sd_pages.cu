@@ -27,17 +27,17 @@ int log2_of(int x) {
   return l;
 }
 
-sd::PagedSet lookup(int dtype, int bits, int D, int nb) {
+sd::PagedSet lookup(int dtype, int bits, int D, int G) {
   switch (dtype * 16 + bits) {
-    case 0 * 16 + 0: return sd::paged_e0_b0(D, nb);
-    case 1 * 16 + 0: return sd::paged_e1_b0(D, nb);
-    case 2 * 16 + 0: return sd::paged_e2_b0(D, nb);
-    case 0 * 16 + 4: return sd::paged_e0_b4(D, nb);
-    case 1 * 16 + 4: return sd::paged_e1_b4(D, nb);
-    case 2 * 16 + 4: return sd::paged_e2_b4(D, nb);
-    case 0 * 16 + 8: return sd::paged_e0_b8(D, nb);
-    case 1 * 16 + 8: return sd::paged_e1_b8(D, nb);
-    case 2 * 16 + 8: return sd::paged_e2_b8(D, nb);
+    case 0 * 16 + 0: return sd::paged_e0_b0(D, G);
+    case 1 * 16 + 0: return sd::paged_e1_b0(D, G);
+    case 2 * 16 + 0: return sd::paged_e2_b0(D, G);
+    case 0 * 16 + 4: return sd::paged_e0_b4(D, G);
+    case 1 * 16 + 4: return sd::paged_e1_b4(D, G);
+    case 2 * 16 + 4: return sd::paged_e2_b4(D, G);
+    case 0 * 16 + 8: return sd::paged_e0_b8(D, G);
+    case 1 * 16 + 8: return sd::paged_e1_b8(D, G);
+    case 2 * 16 + 8: return sd::paged_e2_b8(D, G);
     default: return sd::PagedSet{nullptr, nullptr, 0, 0, 0, 0};
   }
 }
@@ -357,7 +357,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   if (misaligned(tables, 4) || misaligned(lengths, 4) || misaligned(sinks, 4) || misaligned(device_flags, 4))
     return fail(SD_ERR_INVALID_ARG, "an int32 or fp32 array is misaligned");
   const int D = g->head_dim, G = n_q_heads / g->n_kv_heads;
-  const sd::PagedSet ks = lookup(g->dtype, g->kv_bits, D, G <= 8 ? 1 : 2);
+  const sd::PagedSet ks = lookup(g->dtype, g->kv_bits, D, G);
   if (!ks.decode) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   // most units (tiles and segment ends) of one sequence and kv head
   const int64_t max_tiles = (int64_t(table_width) * g->page_size + ks.tile - 1) / ks.tile + sd::kSegmentUnits;
