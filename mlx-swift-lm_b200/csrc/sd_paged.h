@@ -157,10 +157,9 @@ struct CopyParams {
   int64_t bytes[6];   // of one page in each array
   int pieces[6];      // kCopyPiece pieces of one page
   int per_pair;       // pieces of one page pair in one layer
-  int64_t total;      // n * n_layers * per_pair
   int* flags;
 };
-constexpr int kCopyPiece = 16384;
+constexpr int kCopyPiece = 32768;
 constexpr int kCopyThreads = 256;
 const void* copy_pages_kernel_ptr();
 

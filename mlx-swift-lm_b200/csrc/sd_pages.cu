@@ -305,12 +305,11 @@ int32_t sd_copy_pages(const sd_pages* g, const int32_t* src, const int32_t* dst,
     p.pieces[i] = int((p.bytes[i] + sd::kCopyPiece - 1) / sd::kCopyPiece);
     p.per_pair += p.pieces[i];
   }
-  p.total = int64_t(n) * p.n_layers * p.per_pair;
   p.flags = device_flags;
-  int sms = 0;
-  if (int32_t rc = sm_count(&sms)) return rc;
+  const int64_t pieces = int64_t(n) * p.n_layers * p.per_pair;
+  if (pieces >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "too many pages at once (%d)", n);
   void* args[1] = {&p};
-  return launch(sd::copy_pages_kernel_ptr(), dim3(unsigned(std::min<int64_t>(p.total, int64_t(sms) * 8))),
+  return launch(sd::copy_pages_kernel_ptr(), dim3(unsigned(pieces)),
                 sd::kCopyThreads, 0, static_cast<cudaStream_t>(stream), args);
 }
 

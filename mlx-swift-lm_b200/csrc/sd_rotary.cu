@@ -355,39 +355,38 @@ const void* rotary_kernel_for(int dtype, int bits, int vec, bool traditional) {
 
 // Page dst[i] = page src[i] in every array and layer: a pure copy, bound by
 // HBM (every byte read once and written once). Pages are contiguous in each
-// array, so the work is cut into pieces of at most kCopyPiece bytes; a block
-// moves one piece with four 16-byte loads per thread in flight.
+// array; a block moves one piece of at most kCopyPiece bytes, eight 16-byte
+// loads per thread in flight. One block per piece rather than a few that walk
+// over many: with a third of the pieces small (the scales and biases of
+// quantized pools) the scheduler fills the gaps better, 4.0 GB of pages moved
+// in 597 us (6.7 TB/s) against 616 to 700 for 64 down to 8 blocks per SM.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
   griddep_launch_dependents();
   griddep_wait();
-  for (int64_t w = blockIdx.x; w < p.total; w += gridDim.x) {
-    const int64_t unit = w / p.per_pair;           // (layer, pair)
-    int piece = int(w - unit * p.per_pair);
-    const int64_t layer = unit / p.n;
-    const int i = int(unit - layer * p.n);
-    const int src = __ldg(p.src + i), dst = __ldg(p.dst + i);
-    if (src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages) {
-      if (p.flags && threadIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
-      continue;
-    }
-    int a = 0;
-    while (piece >= p.pieces[a]) piece -= p.pieces[a++];
-    const int64_t page = p.bytes[a], at = int64_t(piece) * kCopyPiece;
-    const int n16 = int(min(int64_t(kCopyPiece), page - at) / 16);
-    const uint4* s = reinterpret_cast<const uint4*>(p.array[a] + (layer * p.n_pages + src) * page + at);
-    uint4* d = reinterpret_cast<uint4*>(p.array[a] + (layer * p.n_pages + dst) * page + at);
-    constexpr int K = kCopyPiece / 16 / kCopyThreads;
-    uint4 v[K];
+  const int unit = blockIdx.x / p.per_pair;  // (layer, pair)
+  int piece = blockIdx.x - unit * p.per_pair, a = 0;
+  const int layer = unit / p.n, i = unit - layer * p.n;
+  const int src = __ldg(p.src + i), dst = __ldg(p.dst + i);
+  if (src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages) {
+    if (p.flags && threadIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
+    return;
+  }
+  while (piece >= p.pieces[a]) piece -= p.pieces[a++];
+  const int64_t page = p.bytes[a], at = int64_t(piece) * kCopyPiece;
+  const int n16 = int(min(int64_t(kCopyPiece), page - at) / 16);
+  const uint4* s = reinterpret_cast<const uint4*>(p.array[a] + (layer * p.n_pages + src) * page + at);
+  uint4* d = reinterpret_cast<uint4*>(p.array[a] + (layer * p.n_pages + dst) * page + at);
+  constexpr int K = kCopyPiece / 16 / kCopyThreads;
+  uint4 v[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int x = k * kCopyThreads + threadIdx.x;
-      if (x < n16) v[k] = __ldcs(s + x);
-    }
+  for (int k = 0; k < K; ++k) {
+    const int x = k * kCopyThreads + threadIdx.x;
+    if (x < n16) v[k] = __ldg(s + x);
+  }
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int x = k * kCopyThreads + threadIdx.x;
-      if (x < n16) __stcs(d + x, v[k]);
-    }
+  for (int k = 0; k < K; ++k) {
+    const int x = k * kCopyThreads + threadIdx.x;
+    if (x < n16) d[x] = v[k];
   }
 }
 
