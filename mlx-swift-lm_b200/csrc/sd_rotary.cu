@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   const int groups = 32 >> lg_log, pitch = rotary_pitch(p.rot2);
   float* cs = smem + warp * groups * 2 * pitch;      // [tokens of this warp][cos, sin]
   E* stage = reinterpret_cast<E*>(smem + kRotThreads / 32 * groups * 2 * pitch) + warp * groups * D;
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
 
   const int unit = blockIdx.x * (kRotThreads / 32) + warp;
   if (unit >= p.units) return;
@@ -361,8 +361,8 @@ const void* rotary_kernel_for(int dtype, int bits, int vec, bool traditional) {
 // quantized pools) the scheduler fills the gaps better, 4.0 GB of pages moved
 // in 597 us (6.7 TB/s) against 616 to 700 for 64 down to 8 blocks per SM.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   const int unit = blockIdx.x / p.per_pair;  // (layer, pair)
   int piece = blockIdx.x - unit * p.per_pair, a = 0;
   const int layer = unit / p.n, i = unit - layer * p.n;

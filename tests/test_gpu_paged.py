@@ -675,3 +675,115 @@ def test_python_refusals(cuda):
             bad()
     assert sd.paged_decode(q[:0], p, t[:0], ln[:0]).shape == (0, 8, 128)
     assert sd.rotary(q[:0], None, ln[:0], torch.ones(64, device="cuda"))[0].shape == (0, 8, 128)
+
+
+# ---------------------------------------------------------------------------
+# the pool, the router, the example
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+def test_pool_lifecycle_keeps_every_sequence(cuda, bits):
+    """Random adds, forks, extends, trims, frees and compactions; every sequence's pages hold its own tokens' rows in
+    both layers all along (checked by decoding against a contiguous copy)."""
+    import torch
+    import sparse_decode as sd
+    rng = np.random.default_rng(bits + 1)
+    g = gen(torch, 90 + bits)
+    layers, hkv, hq, d = 2, 2, 4, 64
+    pool = sd.PagePool(layers, 40, hkv, d, 16, "bf16", bits)
+    rows: dict = {}   # sequence -> per layer (k, v) [tokens, Hkv, D]
+    empty = lambda: [(torch.empty(0, hkv, d, device="cuda").bfloat16(),) * 2 for _ in range(layers)]  # noqa: E731
+
+    def check(seqs):
+        if not seqs:
+            return
+        batch = pool.batch(seqs)
+        q = torch.randn(len(seqs), hq, d, generator=g, device="cuda").bfloat16()
+        for layer in range(layers):
+            out = batch.decode(layer, q)
+            for i, s in enumerate(seqs):
+                k, v = rows[s][layer]
+                if len(k) == 0:
+                    assert not out[i].any()
+                    continue
+                one = sd.PagePool(1, -(-len(k) // 16), hkv, d, 16, "bf16", bits)
+                alone = one.extend([one.add()], len(k))
+                alone.append(0, k, v)
+                assert torch.allclose(out[i].float(), alone.decode(0, q[i:i + 1])[0].float(), rtol=2e-2, atol=2e-3)
+    for move in range(60):
+        r = rng.random()
+        seqs = list(rows)
+        if r < 0.15 or not seqs:
+            rows[pool.add()] = empty()
+        elif r < 0.3:
+            s = int(rng.choice(seqs))
+            rows[pool.fork(s)] = list(rows[s])
+        elif r < 0.75:
+            some = [int(s) for s in rng.permutation(seqs)[:rng.integers(1, 4)]]
+            each = [int(n) for n in rng.integers(1, 40, len(some))]
+            try:
+                batch = pool.extend(some, each)
+            except sd.SDError:
+                check(seqs)
+                continue
+            for layer in range(layers):
+                k, v = (torch.randn(sum(each), hkv, d, generator=g, device="cuda").bfloat16() for _ in "kv")
+                batch.append(layer, k, v)
+                at = 0
+                for s, n in zip(some, each):
+                    a, b = rows[s][layer]
+                    rows[s] = list(rows[s])
+                    rows[s][layer] = (torch.cat((a, k[at:at + n])), torch.cat((b, v[at:at + n])))
+                    at += n
+        elif r < 0.85:
+            s = int(rng.choice(seqs))
+            n = pool.trim(s, int(rng.integers(0, 30)))
+            keep = [(a[:len(a) - n], b[:len(b) - n]) for a, b in rows[s]]
+            rows[s] = keep
+        elif r < 0.93:
+            s = int(rng.choice(seqs))
+            pool.free(s)
+            del rows[s]
+        else:
+            pool.compact()
+        for s in rows:
+            assert pool.length(s) == len(rows[s][0][0])
+        if move % 6 == 5:
+            check(list(rows))
+    check(list(rows))
+    assert pool.check_device() == 0
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+def test_router_takes_paged_layers(cuda, bits):
+    """Prefill and decode through attention_with_cache_update equal its own dense attention over the same tokens."""
+    import torch
+    import sparse_decode as sd
+    g = gen(torch, 95)
+    B, hq, hkv, d, n = 2, 8, 2, 128, 37
+    pool = sd.PagePool(1, 16, hkv, d, 16, "bf16", bits)
+    seqs = [pool.add() for _ in range(B)]
+    t = lambda h, L: torch.randn(B, h, L, d, generator=g, device="cuda").bfloat16()  # noqa: E731
+    q, k, v = t(hq, n), t(hkv, n), t(hkv, n)
+    sinks = torch.randn(hq, generator=g, device="cuda")
+    out = sd.attention_with_cache_update(q, k, v, pool.extend(seqs, n).layer(0), d ** -0.5, "causal", sinks)
+    want = sd.attention_with_cache_update(q, k, v, None, d ** -0.5, "causal", sinks)
+    assert torch.allclose(out.float(), want.float(), rtol=5e-2, atol=5e-2 if bits else 1e-2)
+    q1, k1, v1 = t(hq, 1), t(hkv, 1), t(hkv, 1)
+    layer = pool.extend(seqs, 1).layer(0)
+    assert layer.offset == [n, n]
+    out = sd.attention_with_cache_update(q1, k1, v1, layer, d ** -0.5, None, sinks)
+    want = sd.attention_with_cache_update(q1, torch.cat((k, k1), 2), torch.cat((v, v1), 2), None, d ** -0.5, None, sinks)
+    assert out.shape == q1.shape and torch.allclose(out.float(), want.float(), rtol=5e-2, atol=5e-2 if bits else 1e-2)
+    with pytest.raises(ValueError):
+        sd.attention_with_cache_update(q, k, v, layer, d ** -0.5)   # the step holds one new token each
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+def test_example_runs(cuda, bits):
+    from sparse_decode import paged_example
+    pool, seqs, outs, worst = paged_example.run(kv_bits=bits, check=True)
+    assert [pool.length(s) for s in seqs] == [110, 110]  # the prompt of 70 and its fork, 40 steps on
+    # normwise against 64 bits over what the pool stores: bf16's own rounding (2^-8 sqrt(1/12) per element) and
+    # _dequantize's rounding of the stored values to bf16
+    assert worst < 4e-3
