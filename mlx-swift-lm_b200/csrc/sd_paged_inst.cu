@@ -27,8 +27,6 @@ static PagedSet make_paged() {
   s.merge = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D, F::kTile>);
   s.tile = F::kTile;
   s.stage_bytes = F::kStageBytes;
-  s.row_bytes = F::kRowBytes;
-  s.groups = F::kGroups;
   return s;
 }
 
@@ -42,7 +40,7 @@ static PagedSet pick_heads(int G) {
 }
 
 PagedSet SD_NAME(SD_E, SD_BITS)(int D, int G) {
-  return D == 64 ? pick_heads<64>(G) : D == 128 ? pick_heads<128>(G) : PagedSet{nullptr, nullptr, 0, 0, 0, 0};
+  return D == 64 ? pick_heads<64>(G) : D == 128 ? pick_heads<128>(G) : PagedSet{nullptr, nullptr, 0, 0};
 }
 
 }  // namespace sd

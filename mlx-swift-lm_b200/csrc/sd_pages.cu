@@ -38,7 +38,7 @@ sd::PagedSet lookup(int dtype, int bits, int D, int G) {
     case 0 * 16 + 8: return sd::paged_e0_b8(D, G);
     case 1 * 16 + 8: return sd::paged_e1_b8(D, G);
     case 2 * 16 + 8: return sd::paged_e2_b8(D, G);
-    default: return sd::PagedSet{nullptr, nullptr, 0, 0, 0, 0};
+    default: return sd::PagedSet{nullptr, nullptr, 0, 0};
   }
 }
 
@@ -302,17 +302,15 @@ int32_t sd_copy_pages(const sd_pages* g, const int32_t* src, const int32_t* dst,
   p.dst = dst;
   p.n = n;
   p.n_pages = g->n_pages;
-  p.n_layers = g->n_layers;
-  p.n_arrays = g->kv_bits ? 6 : 2;
   void* a[6] = {g->k_data, g->v_data, g->k_scales, g->k_biases, g->v_scales, g->v_biases};
-  for (int i = 0; i < p.n_arrays; ++i) {
+  for (int i = 0; i < (g->kv_bits ? 6 : 2); ++i) {
     p.array[i] = static_cast<uint8_t*>(a[i]);
     p.bytes[i] = int64_t(g->n_kv_heads) * g->page_size * (i < 2 ? row_bytes(g) : sb_bytes(g));
     p.pieces[i] = int((p.bytes[i] + sd::kCopyPiece - 1) / sd::kCopyPiece);
     p.per_pair += p.pieces[i];
   }
   p.flags = device_flags;
-  const int64_t pieces = int64_t(n) * p.n_layers * p.per_pair;
+  const int64_t pieces = int64_t(n) * g->n_layers * p.per_pair;
   if (pieces >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "too many pages at once (%d)", n);
   void* args[1] = {&p};
   return launch(sd::copy_pages_kernel_ptr(), dim3(unsigned(pieces)),

@@ -313,6 +313,14 @@ def test_decode_many_short_sequences(cuda, dtype, bits):
     run_case(torch, dtype, bits, 64, hkv=2, G=2, page=16, lengths=lengths, seed=9)
 
 
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("bf16", 8), ("f32", 0)])
+def test_decode_largest_batch_and_group(cuda, dtype, bits):
+    """4096 sequences and 16 heads per kv head leave the fewest stages of shared memory."""
+    import torch
+    rng = np.random.default_rng(5)
+    run_case(torch, dtype, bits, 128, hkv=1, G=16, page=16, lengths=[int(x) for x in rng.integers(0, 24, 4096)], seed=3)
+
+
 @pytest.mark.parametrize("scale", [1e-4, 1e3])
 @pytest.mark.parametrize("bits", [0, 4, 8])
 def test_decode_small_and_large_values(cuda, scale, bits):
