@@ -73,11 +73,6 @@ struct TileAddr {
   __device__ __forceinline__ uint32_t row_at(int row) const {
     return base + uint32_t(((row >> pb_log) << pb_log) * F::kRowBytes + (row & ((1 << pb_log) - 1)) * F::kBoxBytes);
   }
-  __device__ __forceinline__ uint32_t at(int row, int chunk) const {
-    const int pb = 1 << pb_log;
-    return base + uint32_t((row >> pb_log) * (pb * F::kRowBytes) + (chunk / F::kCpb) * (pb * F::kBoxBytes)) +
-           swz(uint32_t((row & (pb - 1)) * F::kBoxBytes + (chunk % F::kCpb) * 16), F::kCpb);
-  }
 };
 // What a lane's ldmatrix address adds to row_at of its 16 rows, for row `r`
 // of them (boxes hold 16 rows at least) and chunk 2c + odd: the swizzle of a
@@ -301,7 +296,12 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
 // Scales (or biases) of token t for every group, in fp32, from shared memory.
 template <typename E, int NG>
 __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
-  if constexpr (NG == 2) {
+  if constexpr (sizeof(E) == 4 && NG == 2) {
+    const uint2 w = lds64(a + 8 * t);
+    f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y);
+  } else if constexpr (sizeof(E) == 4) {
+    f[0] = __uint_as_float(lds32(a + 4 * t));
+  } else if constexpr (NG == 2) {
     unpack_word<E>(lds32(a + 4 * t), f);
   } else {
     uint16_t w;
@@ -311,8 +311,7 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 }
 
 // ---------------------------------------------------------------------------
-// 4/8-bit codes with 16-bit scales, the same products, with the codes as exact
-// fp16 integers. What bounds this path is instructions, not bytes, so the
+// 4/8-bit codes, the same products, with the codes as exact fp16 integers. What bounds this path is instructions, not bytes, so the
 // conversion is cut to the bone: one byte permute (or mask) puts codes into
 // the mantissas of 1024 + c, or 1024 + 16 c for the nibbles that lie 4 bits
 // higher.
@@ -320,8 +319,8 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 // the offset is left in: the accumulator starts at -1024 sum(q') (q' = q in
 // fp16, a 16th of it where the nibble's place counts 16), which costs 3 to 4
 // of fp32's bits over the 64 products of a group, scores off by some 3e-4 --
-// nothing next to bf16's rounding, but a good half of fp16's, so fp16 pools
-// subtract it.
+// nothing next to bf16's rounding, but a good half of fp16's, so other pools
+// subtract it. fp32 pools take q as hi + lo halves, 22 bits.
 //   p.v = (p s_v).(c - z) + sum_t p (b_v + z s_v), z = the middle code. These
 // sums run over a whole segment, so their codes are centred by one packed
 // subtraction: no offset to cancel, and terms of both signs.
@@ -335,21 +334,29 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 // ---------------------------------------------------------------------------
 template <typename E, int BITS, int D, int NB>
 struct CodesAttend {
-  using F = PagedFmt<2, BITS, D>;
+  using F = PagedFmt<sizeof(E), BITS, D>;
   static constexpr int NK = D / 16, NG = F::kGroups, NCH = F::kNChunk;
   static constexpr int KPC = NK / NCH;   // k-steps (and 16-dim output tiles) per 16-byte chunk: 1 or 2
   static constexpr int MT = F::kTile / kPagedWarps / 16;
   static constexpr float MID = BITS == 8 ? 128.0f : 8.0f;
-  static constexpr bool kOffset = !__is_same(E, __half);
-  uint32_t qb[NB][NK][2];
+  static constexpr bool kOffset = __is_same(E, __nv_bfloat16);
+  static constexpr int QT = sizeof(E) == 4 ? 2 : 1;  // fp16 terms of q
+  uint32_t qb[QT][NB][NK][2];
   float qs[NB][2][NG], qoff[NB][2][NG], m[NB][2], l[NB][2], o[NB][NK][4], ob[NB][2][NG];
   float vinv[NG], vlim[NG], qfac;
 
   __device__ __forceinline__ void begin(const PagedParams& p, const float*, int b, int h, int, int lane) {
     const int g = lane >> 2, tq = lane & 3;
     // this lane's elements of head g: four (8-bit) or eight (4-bit) neighbours of every chunk
-    constexpr int N = BITS == 8 ? 2 : 4;  // 32-bit words
-    uint32_t raw[NB][NCH][N];
+    constexpr int N = BITS == 8 ? 4 : 8, W = N * int(sizeof(E)) / 4;  // elements, 32-bit words
+    uint32_t raw[NB][NCH][W];
+    auto elements = [&](const uint32_t (&w)[W], float (&f)[N]) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if constexpr (sizeof(E) == 4) f[i] = __uint_as_float(w[i]);
+        else unpack_word<E>(w[i], f + 2 * i);
+      }
+    };
     float qmax = 0.0f;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -357,19 +364,21 @@ struct CodesAttend {
       const E* row = static_cast<const E*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * D;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        if constexpr (BITS == 8) {
-          const uint2 w = hd < p.G ? __ldg(reinterpret_cast<const uint2*>(row + 16 * c + 4 * tq)) : make_uint2(0, 0);
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(row + F::kEpc * c + N * tq);
+        if constexpr (W == 2) {
+          const uint2 w = hd < p.G ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
           raw[nb][c][0] = w.x, raw[nb][c][1] = w.y;
         } else {
-          const uint4 w = hd < p.G ? __ldg(reinterpret_cast<const uint4*>(row + 32 * c + 8 * tq)) : make_uint4(0, 0, 0, 0);
-          raw[nb][c][0] = w.x, raw[nb][c][1] = w.y, raw[nb][c][2] = w.z, raw[nb][c][3] = w.w;
-        }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          float f[2];
-          unpack_word<E>(raw[nb][c][i], f);
-          qmax = fmaxf(qmax, fmaxf(fabsf(f[0]), fabsf(f[1])));
+          for (int i = 0; i < W; i += 4) {
+            const uint4 w = hd < p.G ? __ldg(reinterpret_cast<const uint4*>(at + i)) : make_uint4(0, 0, 0, 0);
+            raw[nb][c][i] = w.x, raw[nb][c][i + 1] = w.y, raw[nb][c][i + 2] = w.z, raw[nb][c][i + 3] = w.w;
+          }
         }
+        float f[N];
+        elements(raw[nb][c], f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) qmax = fmaxf(qmax, fabsf(f[i]));
       }
     }
     qmax = warp_max(qmax);
@@ -384,32 +393,33 @@ struct CodesAttend {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int r = c * F::kEpc / 64;
-        float f[2 * N];
+        float f[N];
+        elements(raw[nb][c], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) unpack_word<E>(raw[nb][c][i], f + 2 * i);
-#pragma unroll
-        for (int i = 0; i < 2 * N; ++i) {
+        for (int i = 0; i < N; ++i) {
           sum[r] += f[i];
           f[i] *= up;
         }
         // k-slots {2tq, 2tq + 1} and {2tq + 8, 2tq + 9}, in the order in which the codes come out of a register
-        if constexpr (BITS == 8) {
-          qb[nb][c][0] = pack2<__half>(f[0], f[1]);
-          qb[nb][c][1] = pack2<__half>(f[2], f[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            qb[nb][2 * c + i][0] = pack2<__half>(f[2 * i], f[2 * i + 4]);
-            qb[nb][2 * c + i][1] = pack2<__half>(f[2 * i + 1] * 0.0625f, f[2 * i + 5] * 0.0625f);
-          }
-        }
 #pragma unroll
         for (int i = 0; i < KPC; ++i) {
+          float x[2][2];
+          if constexpr (BITS == 8) {
+            x[0][0] = f[0], x[0][1] = f[1], x[1][0] = f[2], x[1][1] = f[3];
+          } else {
+            x[0][0] = f[2 * i], x[0][1] = f[2 * i + 4];
+            x[1][0] = f[2 * i + 1] * 0.0625f, x[1][1] = f[2 * i + 5] * 0.0625f;
+          }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float g2[2];
-            unpack_word<__half>(qb[nb][KPC * c + i][j], g2);
-            off[r] += g2[0] + g2[1];
+            if constexpr (QT == 2) {
+              split2<__half>(x[j][0], x[j][1], qb[0][nb][KPC * c + i][j], qb[QT - 1][nb][KPC * c + i][j]);
+            } else {
+              qb[0][nb][KPC * c + i][j] = pack2<__half>(x[j][0], x[j][1]);
+              float g2[2];
+              unpack_word<__half>(qb[0][nb][KPC * c + i][j], g2);
+              off[r] += g2[0] + g2[1];
+            }
           }
         }
       }
@@ -448,7 +458,7 @@ struct CodesAttend {
     const LaneAddr<F> la(8 * (mq & 1) + r8, mq >> 1);
     const bool whole = lo <= 0 && hi >= TW;
     const uint32_t magic = p.magic;
-    const uint32_t ksc = smem_u32(t.stage) + 2 * F::kKvBytes + r0 * NG * 2;  // K scales; K biases, V scales, V biases follow
+    const uint32_t ksc = smem_u32(t.stage) + 2 * F::kKvBytes + r0 * NG * int(sizeof(E));  // K scales; K biases, V scales, V biases follow
     const uint32_t kbi = ksc + F::kSbBytes, vsc = kbi + F::kSbBytes, vbi = vsc + F::kSbBytes;
     float s[MT][NB][4];
 #pragma unroll
@@ -486,7 +496,9 @@ struct CodesAttend {
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              mma16816_f16(acc[k / 4][nb], f0, f1, f2, f3, qb[nb][k][0], qb[nb][k][1]);
+#pragma unroll
+              for (int t2 = 0; t2 < QT; ++t2)
+                mma16816_f16(acc[k / 4][nb], f0, f1, f2, f3, qb[t2][nb][k][0], qb[t2][nb][k][1]);
           }
         }
       }
@@ -703,56 +715,31 @@ struct CodesAttend {
 };
 
 // ---------------------------------------------------------------------------
-// fp32 pools (dense, or codes with fp32 scales) on the FMA pipes: the tensor
-// cores have no fp32 product. A warp has 8 tokens of a tile and HB blocks of
-// four heads. q.k: lane = (token, head), so a score needs no exchange and
-// no array over heads, which keeps the code short -- a small call spends more
-// on fetching instructions than on executing them. p.v: lane = (head, eighth
-// of the dims), p from the score's lane by one shuffle per token. q (times
-// scale * log2 e, rows padded against bank conflicts) and, for codes, its sum
-// over each 16-byte chunk lie in shared memory.
+// Dense fp32 pools on the FMA pipes: the tensor cores have no fp32 product. A
+// warp has 8 tokens of a tile and HB blocks of four heads. q.k: lane = (token,
+// head), so a score needs no exchange and no array over heads, which keeps the
+// code short -- a small call spends more on fetching instructions than on
+// executing them. p.v: lane = (head, every eighth chunk of the row), p from the
+// score's lane by one shuffle per token. Keys and values are read once for all
+// heads. q (times scale * log2 e, rows padded against bank conflicts) lies in
+// shared memory.
 // ---------------------------------------------------------------------------
-template <int BITS, int D, int HB>
+template <int D, int HB>
 struct FmaAttend {
-  using F = PagedFmt<4, BITS, D>;
-  static constexpr int NCH = F::kNChunk, EPC = F::kEpc, NG = F::kGroups;
-  static constexpr int TW = 8, DL = D / 8;
-  static_assert(F::kTile == TW * kPagedWarps, "eight tokens per warp");
+  using F = PagedFmt<4, 0, D>;
+  static constexpr int NCH = F::kNChunk, TW = 8, DL = D / 8;
+  static_assert(F::kTile == TW * kPagedWarps && F::kBoxBytes == 128, "eight tokens per warp, whole swizzle rows");
   float m[HB], l[HB], o[HB][DL];  // of head 4 hb + lane % 4 (m, l) and 4 hb + lane / 8 (o)
 
-  // Element i of a lane's dims: every eighth chunk of a dense row, so that the
-  // eight lanes of a head read all banks; neighbours of a row of codes.
-  static __device__ __forceinline__ int dim(int lane, int i) {
-    return BITS == 0 ? 4 * (8 * (i / 4) + (lane & 7)) + i % 4 : (lane & 7) * DL + i;
-  }
+  // Where a lane's dims lie in the row: every eighth chunk, so that the eight lanes of a head read all banks.
+  static __device__ __forceinline__ int dim(int lane, int i) { return 4 * (8 * (i / 4) + (lane & 7)) + i % 4; }
 
-  // Four elements of a chunk, from element 4i on.
-  static __device__ __forceinline__ float4 four(const uint4& w, int i) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    if constexpr (BITS == 0) {
-      return make_float4(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3]));
-    } else if constexpr (BITS == 8) {
-      return make_float4(code_u8(u[i], 0), code_u8(u[i], 1), code_u8(u[i], 2), code_u8(u[i], 3));
-    } else {
-      const int h = 4 * (i & 1);
-      return make_float4(code_u4(u[i / 2], h), code_u4(u[i / 2], h + 1), code_u4(u[i / 2], h + 2), code_u4(u[i / 2], h + 3));
-    }
-  }
-
-  // every consumer thread calls; qf: [G][D + 4], then [G][NCH] chunk sums
+  // every consumer thread calls; qf: [G][D + 4]
   __device__ __forceinline__ void begin(const PagedParams& p, float* qf, int b, int h, int warp, int lane) {
     const float* q = static_cast<const float*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G) * D;
-    const int t = warp * 32 + lane;
 #pragma unroll 1
-    for (int i = t; i < p.G * D; i += 32 * kPagedWarps) qf[i / D * (D + 4) + i % D] = __ldg(q + i) * p.scale_log2;
-    if constexpr (BITS != 0) {
-#pragma unroll 1
-      for (int i = t; i < p.G * NCH; i += 32 * kPagedWarps) {
-        float sum = 0.0f;
-        for (int d = 0; d < EPC; ++d) sum += __ldg(q + (i / NCH) * D + (i % NCH) * EPC + d);
-        qf[p.G * (D + 4) + i] = sum * p.scale_log2;
-      }
-    }
+    for (int i = warp * 32 + lane; i < p.G * D; i += 32 * kPagedWarps)
+      qf[i / D * (D + 4) + i % D] = __ldg(q + i) * p.scale_log2;
     named_barrier(1, 32 * kPagedWarps);
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
@@ -767,14 +754,11 @@ struct FmaAttend {
     const int r0 = warp * TW;
     const int lo = max(t.lo - r0, 0), hi = min(t.hi - r0, TW);
     if (hi <= lo) return;
-    const TileAddr<F> ka{smem_u32(t.stage), t.pb_log}, va{smem_u32(t.stage) + F::kKvBytes, t.pb_log};
-    const float* ksc = reinterpret_cast<const float*>(t.stage + 2 * F::kKvBytes) + r0 * NG;
-    const float *kbi = ksc + F::kTile * NG, *vsc = ksc + 2 * F::kTile * NG, *vbi = ksc + 3 * F::kTile * NG;
-    const int tok = lane >> 2, vh = lane >> 3, d0 = (lane & 7) * DL;  // q.k: (tok, lane % 4); p.v: (vh, dims)
+    const int tok = lane >> 2, vh = lane >> 3;  // q.k: (tok, lane % 4); p.v: (vh, dims)
     const bool ok = tok >= lo && tok < hi;
-    // dense rows: chunk c of row r of the eight lies at rows + (c / 8) box + 128 r + 16 ((c % 8) ^ r)
-    const uint32_t krow = ka.row_at(r0) + tok * F::kBoxBytes, vrows = krow - tok * F::kBoxBytes + F::kKvBytes;
-    const uint32_t box = uint32_t(F::kBoxBytes) << t.pb_log;
+    // chunk c of row r of the eight lies at rows + (c / 8) box + 128 r + 16 ((c % 8) ^ r)
+    const uint32_t rows = TileAddr<F>{smem_u32(t.stage), t.pb_log}.row_at(r0), box = 128u << t.pb_log;
+    const uint32_t krow = rows + tok * 128, vrows = rows + F::kKvBytes;
     const float* qrow[HB];
     float s[HB];
 #pragma unroll
@@ -784,32 +768,11 @@ struct FmaAttend {
     }
 #pragma unroll 4
     for (int c = 0; c < NCH; ++c) {
-      const uint4 w = lds128(BITS == 0 ? krow + (c / 8) * box + (((c % 8) ^ tok) << 4) : ka.at(r0 + tok, c));
-      float4 x[EPC / 4];
-#pragma unroll
-      for (int i = 0; i < EPC / 4; ++i) x[i] = four(w, i);
-      float sc = 1.0f, bi = 0.0f;
-      if constexpr (BITS != 0) {
-        sc = ksc[tok * NG + c * EPC / 64];
-        bi = kbi[tok * NG + c * EPC / 64];
-      }
+      const float4 x = lds_f4(krow + (c / 8) * box + (((c % 8) ^ tok) << 4));
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb) {
-        float a = 0.0f;
-#pragma unroll
-        for (int i = 0; i < EPC / 4; ++i) {
-          const float4 y = *reinterpret_cast<const float4*>(qrow[hb] + c * EPC + 4 * i);
-          a = fmaf(x[i].x, y.x, a);
-          a = fmaf(x[i].y, y.y, a);
-          a = fmaf(x[i].z, y.z, a);
-          a = fmaf(x[i].w, y.w, a);
-        }
-        if constexpr (BITS != 0) {
-          const int hd = min(4 * hb + (lane & 3), p.G - 1);
-          s[hb] = fmaf(sc, a, fmaf(bi, qf[p.G * (D + 4) + hd * NCH + c], s[hb]));
-        } else {
-          s[hb] += a;
-        }
+        const float4 y = *reinterpret_cast<const float4*>(qrow[hb] + 4 * c);
+        s[hb] += fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, x.x * y.x)));
       }
     }
 #pragma unroll
@@ -830,33 +793,11 @@ struct FmaAttend {
 #pragma unroll 2
     for (int tk = lo; tk < hi; ++tk) {
       float v[DL];
-      if constexpr (BITS == 0) {
-        const uint32_t at = vrows + tk * F::kBoxBytes + (((lane & 7) ^ tk) << 4);
+      const uint32_t at = vrows + tk * 128 + (((lane & 7) ^ tk) << 4);
 #pragma unroll
-        for (int c = 0; c < DL / 4; ++c) {
-          const float4 x = lds_f4(at + c * box);
-          v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
-        }
-      } else {  // this lane's DL elements: whole chunks, or a part of one
-        constexpr int PART = DL < EPC ? DL : EPC;
-        const float sc = vsc[tk * NG + d0 / 64], bi = vbi[tk * NG + d0 / 64];
-#pragma unroll
-        for (int c = 0; c < DL / PART; ++c) {
-          const int e = d0 + c * PART;
-          uint4 w = lds128(va.at(r0 + tk, e / EPC));
-          if constexpr (PART < EPC) {  // the part begins at element e % EPC of the chunk
-            const int word = (e % EPC) * BITS / 32;
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-            w.x = word == 0 ? u[0] : word == 1 ? u[1] : word == 2 ? u[2] : u[3];
-            w.y = word == 0 ? u[1] : u[3];
-          }
-#pragma unroll
-          for (int i = 0; i < PART / 4; ++i) {
-            const float4 x = four(w, i);
-            float* vv = v + c * PART + 4 * i;
-            vv[0] = fmaf(sc, x.x, bi), vv[1] = fmaf(sc, x.y, bi), vv[2] = fmaf(sc, x.z, bi), vv[3] = fmaf(sc, x.w, bi);
-          }
-        }
+      for (int c = 0; c < DL / 4; ++c) {
+        const float4 x = lds_f4(at + c * box);
+        v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
       }
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb) {
@@ -956,14 +897,13 @@ struct Walk {
   }
 };
 
-template <typename E, int BITS, int D, int NB, bool kTensor>
-struct PickAttend;
+// NB: blocks of heads, of four for dense fp32 pools, else of eight.
+template <typename E, int BITS, int D, int NB>
+struct PickAttend { using type = CodesAttend<E, BITS, D, NB>; };
 template <typename E, int D, int NB>
-struct PickAttend<E, 0, D, NB, true> { using type = DenseAttend<E, D, NB>; };
-template <typename E, int BITS, int D, int NB>
-struct PickAttend<E, BITS, D, NB, true> { using type = CodesAttend<E, BITS, D, NB>; };
-template <typename E, int BITS, int D, int NB>
-struct PickAttend<E, BITS, D, NB, false> { using type = FmaAttend<BITS, D, NB>; };
+struct PickAttend<E, 0, D, NB> { using type = DenseAttend<E, D, NB>; };
+template <int D, int NB>
+struct PickAttend<float, 0, D, NB> { using type = FmaAttend<D, NB>; };
 
 // After a wait that expired: wait, with the limit, for the copies of the last
 // `stages` of `it` uses, which still land in this CTA's shared memory.
@@ -1131,7 +1071,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
     return;
   }
-  using A = typename PickAttend<E, BITS, D, NB, F::kTensor>::type;
+  using A = typename PickAttend<E, BITS, D, NB>::type;
   const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
   A att;
   Segment s;

@@ -25,7 +25,6 @@ constexpr int kPagedSmem = 115712;
 // the scales and biases), BITS = 0 / 4 / 8.
 template <int ESIZE, int BITS, int D>
 struct PagedFmt {
-  static constexpr bool kTensor = ESIZE == 2;           // 16-bit formats go through the tensor cores
   static constexpr int kRowBytes = BITS ? D * BITS / 8 : D * ESIZE;
   static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;
   static constexpr int kNBox = kRowBytes / kBoxBytes;
@@ -36,8 +35,8 @@ struct PagedFmt {
   // Tokens of one stage. Codes take 32 tokens per warp (two m-tiles), so that
   // what a tile costs beside its tokens weighs less: 4 x 128K tokens in 8 bits
   // 178 us, 218 us with 64 tokens per tile. 16-bit rows are bound by the loads
-  // with 16 per warp already; fp32 warps hold 8 tokens.
-  static constexpr int kTile = ESIZE == 4 ? 32 : BITS ? 128 : 64;
+  // with 16 per warp already; dense fp32 warps hold 8 tokens.
+  static constexpr int kTile = ESIZE == 4 ? (BITS ? 64 : 32) : BITS ? 128 : 64;
   static constexpr int kKvBytes = kTile * kRowBytes;    // K (or V) of a stage
   static constexpr int kSbBytes = BITS ? kTile * kGroups * ESIZE : 0;  // each of the four scale/bias pieces
   static constexpr int kStageBytes = (2 * kKvBytes + 4 * kSbBytes + 1023) / 1024 * 1024;

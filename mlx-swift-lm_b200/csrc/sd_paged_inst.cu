@@ -32,7 +32,7 @@ static PagedSet make_paged() {
 
 template <int D>
 static PagedSet pick_heads(int G) {
-#if SD_E == 0
+#if SD_E == 0 && SD_BITS == 0
   return G <= 4 ? make_paged<D, 1>() : G <= 8 ? make_paged<D, 2>() : make_paged<D, 4>();  // blocks of 4 heads
 #else
   return G <= 8 ? make_paged<D, 1>() : make_paged<D, 2>();  // blocks of 8

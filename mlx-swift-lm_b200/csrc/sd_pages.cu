@@ -405,7 +405,7 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
 
   // shared memory: as many stages as fit beside the fixed parts
   const int buf = sd::kPagedWarps * sd::paged_warp_floats(G, D) * 4;
-  const int qf = g->dtype == SD_F32 ? G * (D + 4 + rb / 16) * 4 : 0;
+  const int qf = g->dtype == SD_F32 && !g->kv_bits ? G * (D + 4) * 4 : 0;  // q of a dense fp32 call
   const int pre = (batch < 32 ? 32 * (sd::kPagedWarps + 1) : batch + 1) * 4, bars = 2 * sd::kPagedMaxStages * 8;
   auto up = [](int x) { return (x + 127) / 128 * 128; };
   const int fixed = up(qf) + up(buf) + up(pre) + bars + 1024;

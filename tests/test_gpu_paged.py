@@ -305,6 +305,34 @@ def test_decode_long_split_over_all_ctas(cuda, dtype, bits):
     run_case(torch, dtype, bits, 64, hkv=2, G=2, page=64, lengths=[20000, 3, 0, 0, 9000, 1], seed=2)
 
 
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("bf16", 8), ("f16", 0), ("f16", 4), ("f32", 0), ("f32", 4), ("f32", 8)])
+def test_decode_sums_stay_exact_over_long_segments(cuda, dtype, bits):
+    """40 sequences over the same 100K tokens: as many (sequence, head) pairs as CTAs, so every pair is summed by one
+    CTA from end to end. Small queries spread the probabilities over all tokens and the values' mean is not zero, so
+    that errors that add up along the sums would show."""
+    import torch
+    import sparse_decode as sd
+    B, hkv, G, d, page, n = 40, 8, 1, 128, 256, 100000
+    n_pages = -(-n // page)
+    pool = Pool(torch, sd, dtype, bits, hkv, d, page, n_pages, 61)
+    v = pool.arrays[1]
+    v[-1] += 2.0   # the biases of codes, or the values themselves
+    if bits:
+        words = v[0].long() & 0xFFFFFFFF
+        codes = torch.stack([(words >> (bits * j)) & ((1 << bits) - 1) for j in range(32 // bits)], -1).flatten(-2)
+        grow = lambda t: t.double().repeat_interleave(64, -1)  # noqa: E731
+        pool.values[1] = codes.double() * grow(v[1]) + grow(v[2])
+    else:
+        pool.values[1] = v[0].double()
+    tables = tables_of(torch, [n], page, n_pages, 62).repeat(B, 1).contiguous()
+    q = (0.05 * torch.randn(B, hkv * G, d, generator=gen(torch, 63), device="cuda")).to(tdt(torch, dtype))
+    ln = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    out = sd.paged_decode(q, pool.pages, tables, ln)
+    some = [0, 13, 39]
+    ref = decode64(q[some], pool, tables[some], [n] * 3, 1 / math.sqrt(d))
+    assert_close(out[some].double().cpu().numpy().reshape(-1, d), ref.cpu().numpy().reshape(-1, d), dtype)
+
+
 @pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 4), ("f32", 0)])
 def test_decode_many_short_sequences(cuda, dtype, bits):
     import torch
