@@ -363,9 +363,12 @@ int32_t sd_paged_decode(const sd_pages* pages, int32_t layer, const void* q, int
 
 /* Which sequence holds which page: host bookkeeping of one pool, with pages
  * shared between forked sequences by reference counts. No call touches the
- * GPU; those that need page copies return the pairs for sd_copy_pages, to be
- * copied before the next append (extend) or decode (compact). One map is used
- * by one host thread at a time. Sequence ids are never reused. */
+ * GPU; those that need page copies return the pairs for sd_copy_pages. The
+ * pairs of any number of sd_pagemap_extend calls in a row may go into one
+ * copy, which must come before the appends they are for, and before the next
+ * sd_pagemap_free, _trim or _compact; those of a sd_pagemap_compact before
+ * the next use of the pool. One map is used by one host thread at a time.
+ * Sequence ids are never reused. */
 typedef struct sd_pagemap sd_pagemap; /* opaque */
 int32_t sd_pagemap_create(int64_t n_pages, int32_t page_size, sd_pagemap** out);
 int32_t sd_pagemap_destroy(sd_pagemap* map);

@@ -446,7 +446,9 @@ class PagePool:
     def extend(self, seqs: Sequence[int], n_tokens, stream=None) -> "PagedBatch":
         """Make room for n_tokens (an int, or one per sequence) more tokens of
         each sequence and return the batch that appends them. All or nothing:
-        when the pool has too few free pages, no sequence grows."""
+        when the pool has too few free pages, no sequence grows. Page copies
+        and the batch's tables are issued on `stream`, on which the step's
+        calls must then run or wait."""
         each = [int(n_tokens)] * len(seqs) if isinstance(n_tokens, int) else [int(n) for n in n_tokens]
         if len(each) != len(seqs):
             raise ValueError("n_tokens must be an int or one per sequence")
@@ -462,10 +464,10 @@ class PagePool:
                     copies.append((src.value, dst.value))
         except SDError:
             # the pages already copied-on-write stay with their sequences, so their contents must follow
-            for s, k in grown:
-                self.trim(s, k)
             if copies:
                 copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
+            for s, k in grown:
+                self.trim(s, k)
             raise
         if copies:
             copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
