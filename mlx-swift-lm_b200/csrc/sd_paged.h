@@ -152,8 +152,9 @@ __host__ __device__ constexpr int rotary_lanes_log(int D, int vec) {
 // Floats of a cos (or sin) row in shared memory: whole 16-byte pieces.
 __host__ __device__ constexpr int rotary_pitch(int rot2) { return (rot2 + 7) / 8 * 8; }
 
-// vec: elements per access (1, 2, 4, 8 for 16-bit types; 1, 2, 4 for fp32); null if not instantiated.
-const void* rotary_kernel_for(int dtype, int bits, int vec, bool traditional);
+// vec: elements per access (1, 2, 4, and 8 for 16-bit types); wide: head_dim
+// above 128; rows: whole rows through shared memory (vec 1).
+const void* rotary_kernel_for(int dtype, int bits, int vec, bool wide, bool rows, bool traditional);
 
 struct CopyParams {
   const int *src, *dst;

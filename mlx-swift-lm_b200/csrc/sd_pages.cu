@@ -157,6 +157,7 @@ int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, i
   limit_vec(p.k, p.Hkv, es, &vec);
   limit_vec(p.v, p.Hv, es, &vec);
   if (!p.tables) limit_vec(p.k_out, p.Hkv, es, &vec);
+  const bool aligned = vec * es == 16 && p.D * es % 16 == 0;  // every row is whole 16-byte pieces
   // chunk pairs must tile the head and its rotated part
   while (vec > 1 && (p.D % (2 * vec) || p.rot2 % vec)) vec /= 2;
   // Quantizing makes a small call wait for a lane's divisions: half the
@@ -189,9 +190,10 @@ int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, i
   p.pairs.set(std::max(p.rot2, 1));
   p.inv_dim = 1.0f / float(p.D);
   p.ring_at = (warps * groups * (2 * sd::rotary_pitch(p.rot2) * 4 + (bits ? p.D * es : 0)) + 15) / 16 * 16;
-  const int per_lane = (vec >= 4 ? 1 : vec == 2 ? 2 : 4) * 2 * vec * es;
-  const size_t smem = size_t(p.ring_at) + size_t(warps) * sd::kRotDepth * 32 * per_lane;
-  const void* fn = sd::rotary_kernel_for(dtype, bits, vec, traditional);
+  const bool wide = p.D > 128, by_rows = vec == 1 && aligned && groups == 1;
+  const int pass = by_rows ? p.D * es : 32 * (vec >= 4 ? 1 : (wide ? 2 : 1) * (2 / vec)) * 2 * vec * es;
+  const size_t smem = size_t(p.ring_at) + size_t(warps) * sd::kRotDepth * pass;
+  const void* fn = sd::rotary_kernel_for(dtype, bits, vec, wide, by_rows, traditional);
   void* args[1] = {&p};
   return launch(fn, dim3(unsigned((p.units + warps - 1) / warps)), sd::kRotThreads, smem, st, args);
 }
