@@ -151,8 +151,8 @@ struct DenseAttend {
       const int64_t row = (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * (D / 2);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        qb[nb][c][0] = hd < p.G ? __ldg(q + row + 8 * c + tq) : 0u;
-        qb[nb][c][1] = hd < p.G ? __ldg(q + row + 8 * c + 4 + tq) : 0u;
+        qb[nb][c][0] = hd < p.G ? q[row + 8 * c + tq] : 0u;
+        qb[nb][c][1] = hd < p.G ? q[row + 8 * c + 4 + tq] : 0u;
         o[nb][c][0] = o[nb][c][1] = o[nb][c][2] = o[nb][c][3] = 0.0f;
       }
       m[nb][0] = m[nb][1] = -INFINITY;
@@ -311,10 +311,10 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 }
 
 // ---------------------------------------------------------------------------
-// 4/8-bit codes, the same products, with the codes as exact fp16 integers. What bounds this path is instructions, not bytes, so the
-// conversion is cut to the bone: one byte permute (or mask) puts codes into
-// the mantissas of 1024 + c, or 1024 + 16 c for the nibbles that lie 4 bits
-// higher.
+// 4/8-bit codes, the same products, with the codes as exact fp16 integers.
+// What bounds this path is instructions as much as bytes, so the conversion is
+// short: one byte permute (or mask) puts codes into the mantissas of 1024 + c,
+// or 1024 + 16 c for the nibbles that lie 4 bits higher.
 //   q.k = s_k (q.c) + b_k sum(q)  per 64-dim group, in fp32. For bf16 pools
 // the offset is left in: the accumulator starts at -1024 sum(q') (q' = q in
 // fp16, a 16th of it where the nibble's place counts 16), which costs 3 to 4
@@ -366,12 +366,12 @@ struct CodesAttend {
       for (int c = 0; c < NCH; ++c) {
         const uint32_t* at = reinterpret_cast<const uint32_t*>(row + F::kEpc * c + N * tq);
         if constexpr (W == 2) {
-          const uint2 w = hd < p.G ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+          const uint2 w = hd < p.G ? *reinterpret_cast<const uint2*>(at) : make_uint2(0, 0);
           raw[nb][c][0] = w.x, raw[nb][c][1] = w.y;
         } else {
 #pragma unroll
           for (int i = 0; i < W; i += 4) {
-            const uint4 w = hd < p.G ? __ldg(reinterpret_cast<const uint4*>(at + i)) : make_uint4(0, 0, 0, 0);
+            const uint4 w = hd < p.G ? *reinterpret_cast<const uint4*>(at + i) : make_uint4(0, 0, 0, 0);
             raw[nb][c][i] = w.x, raw[nb][c][i + 1] = w.y, raw[nb][c][i + 2] = w.z, raw[nb][c][i + 3] = w.w;
           }
         }
@@ -739,7 +739,7 @@ struct FmaAttend {
     const float* q = static_cast<const float*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G) * D;
 #pragma unroll 1
     for (int i = warp * 32 + lane; i < p.G * D; i += 32 * kPagedWarps)
-      qf[i / D * (D + 4) + i % D] = __ldg(q + i) * p.scale_log2;
+      qf[i / D * (D + 4) + i % D] = q[i] * p.scale_log2;
     named_barrier(1, 32 * kPagedWarps);
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
@@ -836,7 +836,7 @@ struct FmaAttend {
 struct TokenRange { int begin, end; };
 __device__ __forceinline__ TokenRange token_range(const PagedParams& p, int b) {
   const int64_t cap = int64_t(p.W) * p.P;
-  const int raw = __ldg(p.lengths + b);
+  const int raw = __ldcg(p.lengths + b);  // from L2: the merge reads it before its wait
   if ((raw < 0 || raw > cap) && p.flags && blockIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
   const int len = raw < 0 ? 0 : raw > cap ? int(cap) : raw;
   return {p.window > 0 && len > p.window ? len - p.window : 0, len};
@@ -848,11 +848,13 @@ __device__ __forceinline__ int units_of(TokenRange r, int tile) {
 }
 
 // The line of U units in equal pieces for the CTAs that take part: the first
-// `rem` pieces have base + 1 units.
+// `rem` pieces have base + 1 units. Small calls give every CTA two units
+// rather than one: half as many segments to join (one bf16 sequence of 2K
+// tokens 8.4 -> 7.6 us; with three or four 7.9, 8.3).
 struct Pieces {
   int n, base, rem;
   __device__ __forceinline__ Pieces(const PagedParams& p, int U) {
-    n = min(U, p.ncta);
+    n = min((U + 1) / 2, p.ncta);
     base = n ? U / n : 0;
     rem = U - base * n;
   }
@@ -928,7 +930,7 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
     const int* row = p.tables + int64_t(s.b) * p.W;
     const int t0 = r.begin / F::kTile;
     const int last_slot = (r.end - 1) >> p_log, first_slot = r.begin >> p_log;
-    auto load = [&](int slot) { return slot >= first_slot && slot <= last_slot ? __ldg(row + slot) : -1; };
+    auto load = [&](int slot) { return slot >= first_slot && slot <= last_slot ? row[slot] : -1; };
     int base = ((t0 + s.i0) * F::kTile) >> p_log;
     int cur = load(base + lane), nxt = load(base + 32 + lane);
     for (int i = s.i0; i < s.i1; ++i, ++it) {
@@ -1122,7 +1124,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
       }
       if (whole) {
         const int hq = s.h * p.G + g;
-        if (p.sinks) L += exp2f(fmaf(__ldg(p.sinks + hq), 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
+        if (p.sinks) L += exp2f(fmaf(p.sinks[hq], 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         E* out = static_cast<E*>(p.out) + (int64_t(s.b) * p.Hkv * p.G + hq) * D + d;
         if constexpr (sizeof(E) == 4) {
@@ -1245,7 +1247,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
     L = fmaf(f, tot[w], L);
     O = fmaf(f, red[w][tid], O);
   }
-  if (p.sinks) L += exp2f(fmaf(__ldg(p.sinks + hq), 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
+  if (p.sinks) L += exp2f(fmaf(p.sinks[hq], 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
   out[tid] = Elt<E>::from_f32(L == 0.0f ? 0.0f : O / L);
 }
 

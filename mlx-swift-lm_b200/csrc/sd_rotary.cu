@@ -171,11 +171,11 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   bool store = here;
   if (!is_q && p.tables) {
     paged = static_cast<E*>(is_v ? p.v_data : p.k_data);
-    const int pos = here ? __ldg(p.positions + n) : -1, sq = here && p.seq ? __ldg(p.seq + n) : n;
+    const int pos = here ? p.positions[n] : -1, sq = here && p.seq ? p.seq[n] : n;
     store = pos >= 0;  // else padding
     if (store) {
       const int col = pos >> p.page_shift;
-      const int page = sq >= 0 && sq < p.B && col < p.W ? __ldg(p.tables + int64_t(sq) * p.W + col) : -1;
+      const int page = sq >= 0 && sq < p.B && col < p.W ? p.tables[int64_t(sq) * p.W + col] : -1;
       if (page >= 0 && page < p.n_pages) {
         slot = int64_t(page) * p.Hkv * p.P + (pos & (p.P - 1));
       } else {
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
     for (int i = lane; i < p.rot2 << tl; i += 32) {
       const int t = p.pairs(i), f = i - t * p.rot2;
       // turns of the angle, less whole turns
-      const double pos = n0 + t < p.n_tokens ? double(__ldg(p.positions + n0 + t)) : 0.0;
-      double turns = pos * (double(__ldg(p.inv_freq + f)) * 0.15915494309189535);
+      const double pos = n0 + t < p.n_tokens ? double(p.positions[n0 + t]) : 0.0;
+      double turns = pos * (double(p.inv_freq[f]) * 0.15915494309189535);
       turns -= rint(turns);
       float sn, c;
       sincospif(2.0f * float(turns), &sn, &c);
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
   const int unit = blockIdx.x / p.per_pair;  // (layer, pair)
   int piece = blockIdx.x - unit * p.per_pair, a = 0;
   const int layer = unit / p.n, i = unit - layer * p.n;
-  const int src = __ldg(p.src + i), dst = __ldg(p.dst + i);
+  const int src = p.src[i], dst = p.dst[i];
   if (src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages) {
     if (p.flags && threadIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
     return;
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int x = k * kCopyThreads + threadIdx.x;
-    if (x < n16) v[k] = __ldg(s + x);
+    if (x < n16) v[k] = s[x];
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
