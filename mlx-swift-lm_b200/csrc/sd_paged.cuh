@@ -337,7 +337,8 @@ struct CodesAttend {
   using F = PagedFmt<sizeof(E), BITS, D>;
   static constexpr int NK = D / 16, NG = F::kGroups, NCH = F::kNChunk;
   static constexpr int KPC = NK / NCH;   // k-steps (and 16-dim output tiles) per 16-byte chunk: 1 or 2
-  static constexpr int MT = F::kTile / kPagedWarps / 16;
+  // Two blocks of heads take their tokens 16 at a time: with 32 they spilled (register limit 168).
+  static constexpr int MT = NB == 1 ? F::kTile / kPagedWarps / 16 : 1, PARTS = F::kTile / kPagedWarps / 16 / MT;
   static constexpr float MID = BITS == 8 ? 128.0f : 8.0f;
   static constexpr bool kOffset = __is_same(E, __nv_bfloat16);
   static constexpr int QT = sizeof(E) == 4 ? 2 : 1;  // fp16 terms of q
@@ -449,9 +450,14 @@ struct CodesAttend {
   }
 
   __device__ __forceinline__ void tile(const PagedParams& p, const float*, const TileView& t, int warp, int lane) {
+#pragma unroll 1
+    for (int i = 0; i < PARTS; ++i) part(p, t, (warp * PARTS + i) * 16 * MT, lane);
+  }
+
+  // Rows r0 .. r0 + 16 MT of the tile.
+  __device__ __forceinline__ void part(const PagedParams& p, const TileView& t, int r0, int lane) {
     constexpr int TW = 16 * MT;
     const int g = lane >> 2, mq = lane >> 3, r8 = lane & 7;
-    const int r0 = warp * TW;
     const int lo = t.lo - r0, hi = t.hi - r0;
     if (hi <= 0 || lo >= TW) return;
     const TileAddr<F> rows{smem_u32(t.stage), t.pb_log};
@@ -705,8 +711,9 @@ struct CodesAttend {
           for (int k = 0; k < NK; ++k) {
             const float back = 1.0f / vinv[k / 4];
             const int d = BITS == 8 ? 16 * k + 2 * g : 32 * (k >> 1) + 4 * g + 2 * (k & 1);
-            w.o[hd * (D + 4) + d] = fmaf(o[nb][k][e], back, ob[nb][e][k / 4]);
-            w.o[hd * (D + 4) + d + 1] = fmaf(o[nb][k][2 + e], BITS == 8 ? back : back * 0.0625f, ob[nb][e][k / 4]);
+            *reinterpret_cast<float2*>(w.o + hd * (D + 4) + d) =
+                make_float2(fmaf(o[nb][k][e], back, ob[nb][e][k / 4]),
+                            fmaf(o[nb][k][2 + e], BITS == 8 ? back : back * 0.0625f, ob[nb][e][k / 4]));
           }
         }
       }
@@ -1146,20 +1153,24 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   if (dead) drain(full, it, p.stages);
 }
 
-// Joins the segments of one query head (grid: B * Hq blocks) in a fixed
-// order; a pair that one CTA did alone is already written, an empty one is
-// written here as zeros. Bound by the latency of its dependent loads, not by
-// their bytes (a few MB at most, from L2): warp w takes the segments w, w + 8,
-// ..., each lane first the (m, l) of one of them, and the o rows are loaded
-// eight at a time, the first eight before the weights are known.
-template <typename E, int D, int TILE>
+// Joins the segments of HB query heads of one sequence (grid: B * ceil(Hq / HB)
+// blocks) in a fixed order; a pair that one CTA did alone is already written,
+// an empty one is written here as zeros. Bound by the latency of its dependent
+// loads, not by their bytes (a few MB at most, from L2): a lane takes the
+// (m, l) of one segment each, and the o rows are loaded eight at a time, the
+// first eight before the weights are known. Warps share a head's segments
+// (warp w: w, w + 8, ...), except that with HB = 8 they take a head each where
+// no pair has more than 32 segments.
+template <typename E, int D, int TILE, int HB>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedParams p) {
   constexpr int NW = kMergeThreads / 32, V = D / 32, BATCH = 8;
+  static_assert(HB == 1 || HB == NW, "a warp per head, or all for one");
   __shared__ float red[NW][D], top[NW], tot[NW];
   __shared__ int sums[NW][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int Hq = p.Hkv * p.G, b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, g = hq % p.G;
-  // The pair's place on the line, from the lengths, while the segments are still being worked on.
+  const int Hq = p.Hkv * p.G, per = (Hq + HB - 1) / HB, b = blockIdx.x / per;
+  const int h0 = (blockIdx.x - b * per) * HB, h1 = min(h0 + HB, Hq);  // query heads
+  // The sequence's place on the line, from the lengths, while the segments are still being worked on.
   int pre = 0, all = 0;
   for (int i = tid; i < p.B; i += kMergeThreads) {
     const int n = units_of(token_range(p, i), TILE);
@@ -1174,81 +1185,123 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 #pragma unroll
   for (int w = 0; w < NW; ++w) pre += sums[w][0], all += sums[w][1];
   const int nu = units_of(token_range(p, b), TILE);
+  const Pieces pieces(p, all * p.Hkv);
+  struct Place { int g, c0, ns, skip; };  // head of its pair; the pair's first CTA, its segments, the slot of the first
+  auto place = [&](int hq) {
+    const int h = hq / p.G, a = pre * p.Hkv + h * nu;  // the pair's first unit
+    const int c0 = pieces.of(a + kSegmentUnits), c1 = pieces.of(a + nu - 1);  // with tiles of it
+    // a CTA leaves its first segment in slot 0: the pair is that for all but, perhaps, c0
+    return Place{hq - h * p.G, c0, c1 - c0 + 1, pieces.begin(c0) < a ? 1 : 0};
+  };
+  const int mine = HB > 1 ? min(h0 + warp, h1 - 1) : h0;
+  Place at = {};
+  if (nu != 0) at = place(mine);
   griddep_wait();
-  E* out = static_cast<E*>(p.out) + int64_t(blockIdx.x) * D;
+  E* out = static_cast<E*>(p.out) + int64_t(b) * Hq * D;
   if (nu == 0) {
-    for (int d = tid; d < D; d += kMergeThreads) out[d] = Elt<E>::from_f32(0.0f);
+    for (int d = h0 * D + tid; d < h1 * D; d += kMergeThreads) out[d] = Elt<E>::from_f32(0.0f);
     return;
   }
-  const Pieces pieces(p, all * p.Hkv);
-  const int a = pre * p.Hkv + h * nu;  // the pair's first unit
-  const int c0 = pieces.of(a + kSegmentUnits), c1 = pieces.of(a + nu - 1), ns = c1 - c0 + 1;  // with tiles of it
-  if (ns == 1) return;
   const int stride = paged_part_floats(p.G, D);
-  // a CTA leaves its first segment in slot 0: the pair is that for all but, perhaps, c0
-  const int skip = pieces.begin(c0) < a ? 1 : 0;
-  auto slot = [&](int i) { return p.part + (int64_t(c0 + i) * 2 + (i == 0 ? skip : 0)) * stride; };
-  float M = -INFINITY, L = 0.0f, acc[V];
+
+  // Segments first, first + step, ... of the head at `at` joined into M, L, acc
+  // (o of elements lane * V ...); false: its pair has one segment.
+  auto join = [&](const Place& at, int first, int step, float& M, float& L, float (&acc)[V]) {
+    const int g = at.g, ns = at.ns;
+    if (ns == 1) return false;
+    auto slot = [&](int i) { return p.part + (int64_t(at.c0 + i) * 2 + (i == 0 ? at.skip : 0)) * stride; };
+    M = -INFINITY, L = 0.0f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-  for (int base = warp; base < ns; base += 32 * NW) {  // lane j: segment base + j * NW
-    const int n = min(32, (ns - base + NW - 1) / NW);
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < n) ml = *reinterpret_cast<const float2*>(slot(base + lane * NW) + p.G * D + 2 * g);
-    float x[BATCH][V];
-    auto load = [&](int j0) {
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    for (int base = first; base < ns; base += 32 * step) {  // lane j: segment base + j * step
+      const int n = min(32, (ns - base + step - 1) / step);
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (lane < n) ml = *reinterpret_cast<const float2*>(slot(base + lane * step) + p.G * D + 2 * g);
+      float x[BATCH][V];
+      auto load = [&](int j0) {
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        if (j0 + j < n) {
-          const float* o = slot(base + (j0 + j) * NW) + g * D + lane * V;
-          if constexpr (V == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(o);
-            x[j][0] = y.x, x[j][1] = y.y, x[j][2] = y.z, x[j][3] = y.w;
-          } else {
-            const float2 y = *reinterpret_cast<const float2*>(o);
-            x[j][0] = y.x, x[j][1] = y.y;
+        for (int j = 0; j < BATCH; ++j) {
+          if (j0 + j < n) {
+            const float* o = slot(base + (j0 + j) * step) + g * D + lane * V;
+            if constexpr (V == 4) {
+              const float4 y = *reinterpret_cast<const float4*>(o);
+              x[j][0] = y.x, x[j][1] = y.y, x[j][2] = y.z, x[j][3] = y.w;
+            } else {
+              const float2 y = *reinterpret_cast<const float2*>(o);
+              x[j][0] = y.x, x[j][1] = y.y;
+            }
           }
         }
-      }
-    };
-    load(0);
-    const float f0 = raise_max(M, warp_max(ml.x)), f = exp2_from(ml.x, M);
-    L = fmaf(L, f0, warp_sum(f * ml.y));
+      };
+      load(0);
+      const float f0 = raise_max(M, warp_max(ml.x)), f = exp2_from(ml.x, M);
+      L = fmaf(L, f0, warp_sum(f * ml.y));
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= f0;
-    for (int j0 = 0; j0 < n; j0 += BATCH) {
+      for (int i = 0; i < V; ++i) acc[i] *= f0;
+      for (int j0 = 0; j0 < n; j0 += BATCH) {
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-        if (j0 + j < n) {
+        for (int j = 0; j < BATCH; ++j) {
+          const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+          if (j0 + j < n) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[j][i], acc[i]);
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[j][i], acc[i]);
+          }
         }
+        load(j0 + BATCH);
       }
-      load(j0 + BATCH);
     }
-  }
+    return true;
+  };
+  auto sink = [&](int hq, float M) {
+    return p.sinks ? exp2f(fmaf(p.sinks[hq], 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M))) : 0.0f;
+  };
+
+  float M, L, acc[V];
+  if (HB > 1 && nu / pieces.base + 2 <= 32) {  // at least the segments of a pair of nu units
+    const int hq = h0 + warp;
+    if (hq >= h1 || !join(at, 0, 1, M, L, acc)) return;
+    L += sink(hq, M);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-  for (int i = 0; i < V; ++i) red[warp][lane * V + i] = acc[i];
-  if (lane == 0) {
-    top[warp] = M;
-    tot[warp] = L;
-  }
-  __syncthreads();
-  if (tid >= D) return;  // D <= kMergeThreads
-  M = -INFINITY;
+    for (int i = 0; i < V; ++i) acc[i] *= inv;
+    E* row = out + hq * D + lane * V;
+    if constexpr (sizeof(E) == 4) {
 #pragma unroll
-  for (int w = 0; w < NW; ++w) M = fmaxf(M, top[w]);
-  float O = 0.0f;
-  L = 0.0f;
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(row + i) = make_float2(acc[i], acc[i + 1]);
+    } else {
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const float f = exp2_from(top[w], M);
-    L = fmaf(f, tot[w], L);
-    O = fmaf(f, red[w][tid], O);
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(row + i) = pack2<E>(acc[i], acc[i + 1]);
+    }
+    return;
   }
-  if (p.sinks) L += exp2f(fmaf(p.sinks[hq], 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
-  out[tid] = Elt<E>::from_f32(L == 0.0f ? 0.0f : O / L);
+#pragma unroll 1
+  for (int hq = h0; hq < h1; ++hq) {
+    if (HB > 1) at = place(hq);
+    if (!join(at, warp, NW, M, L, acc)) continue;  // alike for all threads
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[warp][lane * V + i] = acc[i];
+    if (lane == 0) {
+      top[warp] = M;
+      tot[warp] = L;
+    }
+    __syncthreads();
+    if (tid < D) {  // D <= kMergeThreads
+      M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, top[w]);
+      float O = 0.0f;
+      L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = exp2_from(top[w], M);
+        L = fmaf(f, tot[w], L);
+        O = fmaf(f, red[w][tid], O);
+      }
+      L += sink(hq, M);
+      out[hq * D + tid] = Elt<E>::from_f32(L == 0.0f ? 0.0f : O / L);
+    }
+    if (HB > 1) __syncthreads();
+  }
 }
 
 }  // namespace sd

@@ -12,6 +12,13 @@ namespace sd {
 constexpr int kPagedWarps = 4;                          // warps that attend
 constexpr int kPagedThreads = (kPagedWarps + 1) * 32;   // + one producer warp
 constexpr int kMergeThreads = 256;
+// Query heads of one merge block in calls of more than kMergeMany (sequence,
+// query head) pairs, which come in several waves as blocks of one head each:
+// 39 ragged sequences to 2.6K tokens, 128 heads on 4-bit codes 71 -> 49 us, 16
+// sequences of 2K, 32 heads in bf16 29.5 -> 27.4; at 256 pairs and below blocks
+// of one head are as fast, or faster where a sequence has many segments (4
+// ragged sequences to 60K, 32 heads 67.5, 69.2 by eight).
+constexpr int kMergeHeads = 8, kMergeMany = 256;
 constexpr int kPagedMaxBatch = 4096;                    // sequences per decode call
 constexpr int kPagedMaxStages = 16;
 // Beginning and ending a segment costs about as much as two tiles. With 16
@@ -68,7 +75,7 @@ struct PagedParams {
 
 struct PagedSet {
   const void* decode;  // paged_decode_kernel<E, BITS, D, blocks of heads>(PagedParams, CUtensorMap, CUtensorMap)
-  const void* merge;   // paged_merge_kernel<E, D, tile>(PagedParams)
+  const void *merge, *merge_many;  // paged_merge_kernel<E, D, tile, 1 or kMergeHeads>(PagedParams)
   int tile, stage_bytes;
 };
 // For G query heads per kv head; null members without an instantiation.

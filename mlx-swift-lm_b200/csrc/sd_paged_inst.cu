@@ -24,7 +24,8 @@ static PagedSet make_paged() {
   using F = PagedFmt<sizeof(ET), SD_BITS, D>;
   PagedSet s;
   s.decode = reinterpret_cast<const void*>(&paged_decode_kernel<ET, SD_BITS, D, NB>);
-  s.merge = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D, F::kTile>);
+  s.merge = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D, F::kTile, 1>);
+  s.merge_many = reinterpret_cast<const void*>(&paged_merge_kernel<ET, D, F::kTile, kMergeHeads>);
   s.tile = F::kTile;
   s.stage_bytes = F::kStageBytes;
   return s;
@@ -40,7 +41,7 @@ static PagedSet pick_heads(int G) {
 }
 
 PagedSet SD_NAME(SD_E, SD_BITS)(int D, int G) {
-  return D == 64 ? pick_heads<64>(G) : D == 128 ? pick_heads<128>(G) : PagedSet{nullptr, nullptr, 0, 0};
+  return D == 64 ? pick_heads<64>(G) : D == 128 ? pick_heads<128>(G) : PagedSet{};
 }
 
 }  // namespace sd

@@ -427,6 +427,10 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   void* args[3] = {&p, &tmK, &tmV};
   if (int32_t rc = launch(ks.decode, dim3(unsigned(p.ncta)), sd::kPagedThreads, smem, st, args)) return rc;
   void* margs[1] = {&p};
+  if (int64_t(batch) * n_q_heads > sd::kMergeMany) {
+    const unsigned per = unsigned(n_q_heads + sd::kMergeHeads - 1) / sd::kMergeHeads;
+    return launch(ks.merge_many, dim3(unsigned(batch) * per), sd::kMergeThreads, 0, st, margs);
+  }
   return launch(ks.merge, dim3(unsigned(batch) * unsigned(n_q_heads)), sd::kMergeThreads, 0, st, margs);
 }
 

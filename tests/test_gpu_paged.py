@@ -349,6 +349,19 @@ def test_decode_largest_batch_and_group(cuda, dtype, bits):
     run_case(torch, dtype, bits, 128, hkv=1, G=16, page=16, lengths=[int(x) for x in rng.integers(0, 24, 4096)], seed=3)
 
 
+@pytest.mark.parametrize("dtype,bits,d,hkv,G", [("bf16", 0, 128, 3, 7), ("f16", 4, 64, 2, 16), ("bf16", 8, 128, 8, 3), ("f32", 0, 64, 5, 5)])
+@pytest.mark.parametrize("long", [700, 21000])
+def test_decode_many_heads_beside_a_long_sequence(cuda, dtype, bits, d, hkv, G, long):
+    """More query heads than one wave of blocks joins one by one; the long sequence has many segments, the others one or
+    two, some none, and the heads of a sequence do not divide by eight."""
+    import torch
+    rng = np.random.default_rng(long + G)
+    lengths = [int(x) for x in rng.integers(0, 200, 44)]
+    lengths[5] = lengths[43] = 0
+    lengths[17] = long
+    run_case(torch, dtype, bits, d, hkv=hkv, G=G, page=32, lengths=lengths, sinks=True, seed=G)
+
+
 @pytest.mark.parametrize("scale", [1e-4, 1e3])
 @pytest.mark.parametrize("bits", [0, 4, 8])
 def test_decode_small_and_large_values(cuda, scale, bits):
