@@ -383,7 +383,7 @@ struct CodesAttend {
       }
     }
     qmax = warp_max(qmax);
-    const int eq = qmax > 0.0f && qmax < INFINITY ? ilogbf(qmax) - 13 : 0;
+    const int eq = qmax > 0.0f && qmax < INFINITY ? max(ilogbf(qmax) - 13, -126) : 0;
     const float up = exp2f(float(-eq));
     qfac = ldexpf(p.scale_log2, eq);
 #pragma unroll

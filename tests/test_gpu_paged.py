@@ -362,6 +362,22 @@ def test_decode_many_heads_beside_a_long_sequence(cuda, dtype, bits, d, hkv, G, 
     run_case(torch, dtype, bits, d, hkv=hkv, G=G, page=32, lengths=lengths, sinks=True, seed=G)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_queries_below_every_power_of_two(cuda, dtype, bits):
+    """Queries of 2^-130, subnormal: every score is zero to all digits, the output is the mean of the values."""
+    import torch
+    import sparse_decode as sd
+    pool = Pool(torch, sd, dtype, bits, 2, 128, 64, 6, 21)
+    lengths = [200, 3]
+    tables = tables_of(torch, lengths, 64, 6, 22)
+    q = (torch.ones(2, 8, 128, device="cuda", dtype=torch.float64) * 2.0 ** -130).to(tdt(torch, dtype))
+    assert float(q.double().abs().min()) == 2.0 ** -130
+    out = sd.paged_decode(q, pool.pages, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    ref = decode64(q, pool, tables, lengths, 1 / math.sqrt(128))
+    assert_close(out.double().cpu().numpy().reshape(-1, 128), ref.cpu().numpy().reshape(-1, 128), dtype)
+
+
 @pytest.mark.parametrize("scale", [1e-4, 1e3])
 @pytest.mark.parametrize("bits", [0, 4, 8])
 def test_decode_small_and_large_values(cuda, scale, bits):
