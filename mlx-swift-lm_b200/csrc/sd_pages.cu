@@ -158,9 +158,17 @@ int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, i
   limit_vec(p.k, p.Hkv, es, &vec);
   limit_vec(p.v, p.Hv, es, &vec);
   if (!p.tables) limit_vec(p.k_out, p.Hkv, es, &vec);
-  const bool aligned = vec * es == 16 && p.D * es % 16 == 0;  // every row is whole 16-byte pieces
-  // chunk pairs must tile the head and its rotated part
-  while (vec > 1 && (p.D % (2 * vec) || p.rot2 % vec)) vec /= 2;
+  while (vec > 1 && p.D % (2 * vec)) vec /= 2;  // chunk pairs must tile the head
+  // In the half layout each rotated half must be whole chunks too, down to two
+  // elements; with an odd number of rotations the kernel fetches the other
+  // elements one by one from shared memory instead, four to a chunk (6023
+  // tokens of 48 heads of 128 in bf16: 61 rotations 61 us so, 107 with
+  // one-element chunks; 62 and 60 rotations 62 and 62 us so, 57 and 40 with
+  // chunks of two and four).
+  int even = vec;
+  while (even > 1 && p.rot2 % even) even /= 2;
+  const bool shifted = !traditional && vec >= 4 && even == 1 && p.rot2 > 0;
+  if (!traditional) vec = shifted ? 4 : even;
   // Quantizing makes a small call wait for a lane's divisions: half the
   // elements per lane then, 16 users' appends to an 8-bit pool 4.7 -> 3.9 us.
   const int64_t rows = n_tokens * (p.Hq + p.Hkv + p.Hv);
@@ -191,10 +199,10 @@ int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, i
   p.pairs.set(std::max(p.rot2, 1));
   p.inv_dim = 1.0f / float(p.D);
   p.ring_at = (warps * groups * (2 * sd::rotary_pitch(p.rot2) * 4 + (bits ? p.D * es : 0)) + 15) / 16 * 16;
-  const bool wide = p.D > 128, by_rows = vec == 1 && aligned && groups == 1;
-  const int pass = by_rows ? p.D * es : 32 * (vec >= 4 ? 1 : (wide ? 2 : 1) * (2 / vec)) * 2 * vec * es;
+  const bool wide = p.D > 128;
+  const int pass = 32 * (vec >= 4 ? 1 : (wide ? 2 : 1) * (2 / vec)) * 2 * vec * es;
   const size_t smem = size_t(p.ring_at) + size_t(warps) * sd::kRotDepth * pass;
-  const void* fn = sd::rotary_kernel_for(dtype, bits, vec, wide, by_rows, traditional);
+  const void* fn = sd::rotary_kernel_for(dtype, bits, vec, wide, shifted, traditional);
   void* args[1] = {&p};
   return launch(fn, dim3(unsigned((p.units + warps - 1) / warps)), sd::kRotThreads, smem, st, args);
 }

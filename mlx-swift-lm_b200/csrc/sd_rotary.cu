@@ -114,30 +114,32 @@ __device__ __forceinline__ void quantize_part(const E* row, uint8_t* wq, E* sc, 
 
 }  // namespace
 
+// Which elements a lane holds, and where it finds the other one of a rotation.
+enum RotaryForm {
+  kHalves,   // chunk pair j: [jV, jV + V) of both rotated halves, so every rotation is within a lane
+  kNearby,   // traditional layout: two chunks that are half a row apart, each of whole rotations
+  kShifted,  // halves that are no whole number of chunks: as kNearby, the other elements from shared memory
+};
+
 // A warp takes rows of one kind (query, key or value) and of few tokens: a
 // group of lanes holds one row at a time and stays with one token, so what
 // depends on the position and the weights is computed once and stays in
 // registers. With the norm's weights w folded into cos and sin, a rotation is
 //   a' = inv * (a (w_a cos) - b (w_b sin)),  b' = inv * (b (w_b cos) + a (w_a sin)),
-// inv = the row's 1 / rms. A lane holds chunk pairs of V elements: pair j is
-// the elements [jV, jV + V) of the first rotated half and the same of the
-// second, or 2V neighbours (traditional layout, and past the rotated part), so
-// both elements of a rotation are in one lane. Rows are copied kRotDepth passes
-// ahead into shared memory (each lane its own chunks, so nothing waits for
-// another lane); while the first are under way the warp computes its tokens'
-// cos and sin, one pair per lane, and exchanges them through shared memory.
-// No barrier wider than a warp.
+// inv = the row's 1 / rms. A lane holds chunk pairs of V elements (RotaryForm);
+// the lanes' first chunks lie side by side, and so do their second ones, as an
+// access that skips every other 16 bytes moves half as much (traditional
+// layout with neighbouring chunks 38 us instead of 27 at 6023 tokens of 48
+// heads). Rows are copied kRotDepth passes ahead into shared memory (each lane
+// its own chunks, so nothing waits for another lane but in kShifted); while the
+// first are under way the warp computes its tokens' cos and sin, one pair per
+// lane, and exchanges them through shared memory. No barrier wider than a warp.
 // BITS 4 / 8: key and value rows are rounded to E, staged in shared memory and
 // quantized from there by the group of lanes that holds the row.
-// ROWS (V = 1, an odd number of rotated pairs): rows that begin on 16-byte
-// boundaries are copied whole, 16 bytes at a time, rotated in shared memory and
-// copied out whole; only the accesses there are of single elements (4096
-// tokens of 40 heads, 61 pairs: 55 us against 68 with single-element accesses
-// to global memory, 16 with 64 pairs).
 // CPL: chunk pairs per lane.
-template <typename E, int V, int CPL, bool ROWS, int BITS, bool TRAD>
+template <typename E, int V, int CPL, int BITS, RotaryForm FORM>
 __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  static_assert(!ROWS || V == 1, "whole rows are for single-element chunks");
+  static_assert(FORM != kShifted || CPL == 1, "one chunk pair per lane");
   using P = Pack<E, V>;
   extern __shared__ __align__(16) float smem[];
   const int D = p.D, pairs = D / (2 * V), lg_log = rotary_lanes_log(D, V), lg = 1 << lg_log;
@@ -160,9 +162,16 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   const int n = n0 + (grp & ((1 << tl) - 1));
   const bool here = n < p.n_tokens;
   const int bt = p.L(n), tk = n - bt * p.L.d;
-  const int half = TRAD ? 0 : p.rot2 / V;            // chunk pairs that straddle the two halves
+  const int half = FORM == kHalves ? p.rot2 / V : 0;  // chunk pairs of the two rotated halves
   // Element offset of chunk i (0, 1) of pair j.
-  auto place = [&](int j, int i) { return j < half ? j * V + i * p.rot2 : 2 * j * V + i * V; };
+  auto place = [&](int j, int i) {
+    if constexpr (FORM == kHalves) return j < half ? j * V + i * p.rot2 : 2 * p.rot2 + (j - half) * V + i * (D / 2 - p.rot2);
+    else if constexpr (V == 1) return 2 * j + i;
+    else return j * V + i * (D / 2);
+  };
+  int at[CPL][2];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) at[c][0] = place(c * lg + sub, 0), at[c][1] = place(c * lg + sub, 1);
   const E* src = static_cast<const E*>(in.data) + bt * in.batch + tk * in.token;
 
   // where key and value rows go: a page slot (the same for every head), or k_out
@@ -190,28 +199,24 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   const E* w = is_v ? nullptr : static_cast<const E*>(is_q ? p.q_norm : p.k_norm);
   const int last = min(heads, (first_pass + kd_.span) * step);  // heads of this warp end here
   int hd = first_pass * step + (grp >> tl);
-  // Rows under way, kRotDepth passes ahead: every lane copies its own chunks and reads back only those, or (ROWS) the
-  // warp, which is then one group, copies its row.
+  // Rows under way, kRotDepth passes ahead. A lane's chunks lie together with the other lanes' (kShifted: as the row).
   constexpr int BYTES = V * int(sizeof(E)), PASS = CPL * 2 * 32 * BYTES;  // of one warp and pass
-  const int pieces = D * int(sizeof(E)) / 16;                             // of a whole row
-  uint8_t* ring = reinterpret_cast<uint8_t*>(smem) + p.ring_at + warp * kRotDepth * (ROWS ? pieces * 16 : PASS) +
-                  (ROWS ? 0 : lane * BYTES);
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem) + p.ring_at + warp * kRotDepth * PASS +
+                  (FORM == kShifted ? grp * D * int(sizeof(E)) : lane * BYTES);
+  auto slot_of = [&](int st, int c, int i) {
+    return ring + st * PASS + (FORM == kShifted ? at[c][i] * int(sizeof(E)) : (2 * c + i) * 32 * BYTES);
+  };
   const E* from = src + hd * in.head;  // the row to load next
   const int64_t from_step = step * in.head;
   int ahead = hd;
   auto fetch = [&](int st) {
     if (here && ahead < last) {
-      if constexpr (ROWS) {
-        for (int i = lane; i < pieces; i += 32)
-          copy_chunk<16>(ring + (st * pieces + i) * 16, reinterpret_cast<const uint8_t*>(from) + i * 16);
-      } else {
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const int j = c * lg + sub;
-          if (j < pairs) {
-            copy_chunk<BYTES>(ring + st * PASS + (2 * c) * 32 * BYTES, from + place(j, 0));
-            copy_chunk<BYTES>(ring + st * PASS + (2 * c + 1) * 32 * BYTES, from + place(j, 1));
-          }
+      for (int c = 0; c < CPL; ++c) {
+        const int j = c * lg + sub;
+        if (j < pairs) {
+          copy_chunk<BYTES>(slot_of(st, c, 0), from + at[c][0]);
+          copy_chunk<BYTES>(slot_of(st, c, 1), from + at[c][1]);
         }
       }
     }
@@ -224,9 +229,10 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   E* dst = BITS != 0 && paged ? stage + grp * D : paged ? paged + (slot + int64_t(hd) * p.P) * D : out + hd * outr.head;
   const int64_t dst_step = BITS != 0 && paged ? 0 : paged ? int64_t(step) * p.P * D : step * outr.head;
 
-  // coefficients of this lane's pairs: wa cos, wb sin, wb cos, wa sin; wa and wb alone past the rotated part
-  float ka[CPL][V], kb[CPL][V], kc[CPL][V], kd[CPL][V];
-  bool turned[CPL];  // the host picks V so that a lane's V pairs are rotated all or none
+  // This lane's elements: own * k1 + other * k2, k1 = w_own cos, k2 = -w_other sin (first of a rotation) or w_other sin
+  // (second). Bit e of `turned`: rotation e (kShifted: element e) is one; in kHalves a chunk pair is rotated all or not at all.
+  float k1[CPL][2 * V], k2[CPL][2 * V];
+  uint32_t turned[CPL], far[V];  // far: byte offsets within the row of the other elements, two to a word (kShifted)
   if (!is_v) {
     for (int i = lane; i < p.rot2 << tl; i += 32) {
       const int t = p.pairs(i), f = i - t * p.rot2;
@@ -244,23 +250,41 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       const int j = c * lg + sub;
-      turned[c] = j * V < p.rot2;
+      turned[c] = 0;
+      float wt[2 * V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int ia = TRAD ? 2 * e : e, ib = TRAD ? 2 * e + 1 : V + e;  // within the two chunks
-        float wa = 1.0f, wb = 1.0f, co = 1.0f, si = 0.0f;
-        if (w && j < pairs) {
-          wa = Elt<E>::to_f32(w[place(j, ia / V) + ia % V]);
-          wb = Elt<E>::to_f32(w[place(j, ib / V) + ib % V]);
+      for (int e = 0; e < 2 * V; ++e) wt[e] = 1.0f;
+      if (w && j < pairs) {
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) wt[e] = Elt<E>::to_f32(w[at[c][e / V] + e % V]);
+      }
+      if constexpr (FORM != kShifted) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int a = FORM == kNearby ? 2 * e : e, b = FORM == kNearby ? 2 * e + 1 : V + e;
+          const int f = FORM == kNearby ? (at[c][a / V] + a % V) / 2 : j * V + e;
+          const bool turn = FORM == kHalves ? j < half : j < pairs && f < p.rot2;
+          const float co = turn ? co_row[f] : 1.0f, si = turn ? co_row[pitch + f] : 0.0f;
+          k1[c][a] = wt[a] * co;
+          k1[c][b] = wt[b] * co;
+          k2[c][a] = -(wt[b] * si);
+          k2[c][b] = wt[a] * si;
+          turned[c] |= uint32_t(turn) << e;
         }
-        if (turned[c]) {
-          co = co_row[j * V + e];
-          si = co_row[pitch + j * V + e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) {
+          const int x = at[c][e / V] + e % V, f = x < p.rot2 ? x : x - p.rot2;
+          const bool turn = j < pairs && f < p.rot2;
+          const int y = !turn ? 0 : x < p.rot2 ? x + p.rot2 : f;
+          const float co = turn ? co_row[f] : 1.0f, si = turn ? co_row[pitch + f] : 0.0f;
+          const float other = w && turn ? Elt<E>::to_f32(w[y]) : 1.0f;
+          k1[c][e] = wt[e] * co;
+          k2[c][e] = other * (x < p.rot2 ? -si : si);
+          turned[c] |= uint32_t(turn) << e;
+          const uint32_t at = uint32_t(y * int(sizeof(E)));
+          far[e / 2] = e % 2 ? far[e / 2] | at << 16 : at;
         }
-        ka[c][e] = wa * co;
-        kb[c][e] = wb * si;
-        kc[c][e] = wb * co;
-        kd[c][e] = wa * si;
       }
     }
   }
@@ -270,27 +294,28 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
   for (int pass = first_pass * step; pass < last; pass += step, hd += step, dst += dst_step) {
     const bool live = store && hd < last;
     cp_async_wait<kRotDepth - 1>();
-    E* row = reinterpret_cast<E*>(ring + st * pieces * 16);  // ROWS
-    if constexpr (ROWS) __syncwarp();
+    if constexpr (FORM == kShifted) __syncwarp();
     P x[CPL][2];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       const int j = c * lg + sub;
       x[c][0].zero(), x[c][1].zero();
       if (j < pairs) {
-        if constexpr (ROWS) {
-          x[c][0].e[0] = row[place(j, 0)];
-          x[c][1].e[0] = row[place(j, 1)];
-        } else {
-          x[c][0].raw = *reinterpret_cast<const decltype(P::raw)*>(ring + st * PASS + (2 * c) * 32 * BYTES);
-          x[c][1].raw = *reinterpret_cast<const decltype(P::raw)*>(ring + st * PASS + (2 * c + 1) * 32 * BYTES);
-        }
+        x[c][0].raw = *reinterpret_cast<const decltype(P::raw)*>(slot_of(st, c, 0));
+        x[c][1].raw = *reinterpret_cast<const decltype(P::raw)*>(slot_of(st, c, 1));
       }
     }
-    if constexpr (!ROWS) {
-      fetch(st);
-      st = st + 1 == kRotDepth ? 0 : st + 1;
+    E others[FORM == kShifted ? 2 * V : 1];
+    if constexpr (FORM == kShifted) {
+      if (!is_v) {
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e)
+          others[e] = *reinterpret_cast<const E*>(ring + st * PASS + (e % 2 ? far[e / 2] >> 16 : far[e / 2] & 0xffffu));
+      }
+      __syncwarp();  // every lane has read before the next rows may land here
     }
+    fetch(st);
+    st = st + 1 == kRotDepth ? 0 : st + 1;
     float f[CPL][2 * V], inv = 1.0f;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
@@ -314,36 +339,38 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
           P y[2] = {x[c][0], x[c][1]};  // values are stored as they came
           if (!is_v) {
             float r[2 * V];
+            // a rotation is left out by a branch, not by zeros: 0 * inf would reach the other element
+            if constexpr (FORM != kShifted) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const int ia = TRAD ? 2 * e : e, ib = TRAD ? 2 * e + 1 : V + e;
-              const float a = f[c][ia] * inv, b = f[c][ib] * inv;
-              r[ia] = a * ka[c][e];
-              r[ib] = b * kc[c][e];
-              if (turned[c]) {  // not by zeros: 0 * inf would reach the other element
-                r[ia] = fmaf(-b, kb[c][e], r[ia]);
-                r[ib] = fmaf(a, kd[c][e], r[ib]);
+              for (int e = 0; e < V; ++e) {
+                const int ia = FORM == kNearby ? 2 * e : e, ib = FORM == kNearby ? 2 * e + 1 : V + e;
+                const float a = f[c][ia] * inv, b = f[c][ib] * inv;
+                r[ia] = a * k1[c][ia];
+                r[ib] = b * k1[c][ib];
+                if (FORM == kNearby ? (turned[c] >> e & 1) != 0 : turned[c] != 0) {
+                  r[ia] = fmaf(b, k2[c][ia], r[ia]);
+                  r[ib] = fmaf(a, k2[c][ib], r[ib]);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2 * V; ++e) {
+                r[e] = f[c][e] * inv * k1[c][e];
+                if (turned[c] >> e & 1) r[e] = fmaf(Elt<E>::to_f32(others[e]) * inv, k2[c][e], r[e]);
               }
             }
             y[0].pack(r);
             y[1].pack(r + V);
           }
-          E* to = ROWS ? row : dst;
-          *reinterpret_cast<decltype(P::raw)*>(to + place(j, 0)) = y[0].raw;
-          *reinterpret_cast<decltype(P::raw)*>(to + place(j, 1)) = y[1].raw;
+          *reinterpret_cast<decltype(P::raw)*>(dst + at[c][0]) = y[0].raw;
+          *reinterpret_cast<decltype(P::raw)*>(dst + at[c][1]) = y[1].raw;
         }
       }
-    }
-    if constexpr (ROWS) {
-      __syncwarp();
-      if (live && !(BITS != 0 && paged))
-        for (int i = lane; i < pieces; i += 32)
-          reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(row)[i];
     }
     if constexpr (BITS != 0) {
       if (paged) {
         __syncwarp();
-        const E* staged = ROWS ? row : stage + grp * D;
+        const E* staged = stage + grp * D;
         const int64_t at = slot + int64_t(hd) * p.P;
         uint8_t* wq = static_cast<uint8_t*>(is_v ? p.v_data : p.k_data) + at * (D * BITS / 8);
         E* sc = static_cast<E*>(is_v ? p.v_scales : p.k_scales) + at * (D / 64);
@@ -354,43 +381,36 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_con
         __syncwarp();
       }
     }
-    if constexpr (ROWS) {
-      __syncwarp();  // every lane is done with the row
-      fetch(st);
-      st = st + 1 == kRotDepth ? 0 : st + 1;
-    }
   }
   cp_async_wait<0>();
 }
 
-template <typename E, int V, int CPL, bool ROWS, int BITS>
+template <typename E, int V, int CPL, int BITS>
 static const void* rotary_entry(bool trad) {
-  return trad ? reinterpret_cast<const void*>(&rotary_kernel<E, V, CPL, ROWS, BITS, true>)
-              : reinterpret_cast<const void*>(&rotary_kernel<E, V, CPL, ROWS, BITS, false>);
+  return trad ? reinterpret_cast<const void*>(&rotary_kernel<E, V, CPL, BITS, kNearby>)
+              : reinterpret_cast<const void*>(&rotary_kernel<E, V, CPL, BITS, kHalves>);
 }
 template <typename E, int BITS>
-static const void* rotary_pick(int vec, bool wide, bool rows, bool trad) {
+static const void* rotary_pick(int vec, bool wide, bool shifted, bool trad) {
   if constexpr (sizeof(E) == 2)
-    if (vec == 8) return rotary_entry<E, 8, 1, false, BITS>(trad);
-  if (vec == 4) return rotary_entry<E, 4, 1, false, BITS>(trad);
+    if (vec == 8) return shifted ? reinterpret_cast<const void*>(&rotary_kernel<E, 8, 1, BITS, kShifted>) : rotary_entry<E, 8, 1, BITS>(trad);
+  if (vec == 4) return shifted ? reinterpret_cast<const void*>(&rotary_kernel<E, 4, 1, BITS, kShifted>) : rotary_entry<E, 4, 1, BITS>(trad);
   if constexpr (BITS == 0) {  // quantized pools have head_dim 64 and 128
-    if (wide && vec == 2) return rotary_entry<E, 2, 2, false, BITS>(trad);
-    if (wide) return rows ? rotary_entry<E, 1, 4, true, BITS>(trad) : rotary_entry<E, 1, 4, false, BITS>(trad);
+    if (wide) return vec == 2 ? rotary_entry<E, 2, 2, BITS>(trad) : rotary_entry<E, 1, 4, BITS>(trad);
   }
-  if (vec == 2) return rotary_entry<E, 2, 1, false, BITS>(trad);
-  return rows ? rotary_entry<E, 1, 2, true, BITS>(trad) : rotary_entry<E, 1, 2, false, BITS>(trad);
+  return vec == 2 ? rotary_entry<E, 2, 1, BITS>(trad) : rotary_entry<E, 1, 2, BITS>(trad);
 }
 template <typename E>
-static const void* rotary_bits(int bits, int vec, bool wide, bool rows, bool trad) {
-  return bits == 0   ? rotary_pick<E, 0>(vec, wide, rows, trad)
-         : bits == 4 ? rotary_pick<E, 4>(vec, wide, rows, trad)
-                     : rotary_pick<E, 8>(vec, wide, rows, trad);
+static const void* rotary_bits(int bits, int vec, bool wide, bool shifted, bool trad) {
+  return bits == 0   ? rotary_pick<E, 0>(vec, wide, shifted, trad)
+         : bits == 4 ? rotary_pick<E, 4>(vec, wide, shifted, trad)
+                     : rotary_pick<E, 8>(vec, wide, shifted, trad);
 }
 
-const void* rotary_kernel_for(int dtype, int bits, int vec, bool wide, bool rows, bool traditional) {
-  return dtype == 0   ? rotary_bits<float>(bits, vec, wide, rows, traditional)
-         : dtype == 1 ? rotary_bits<__half>(bits, vec, wide, rows, traditional)
-                      : rotary_bits<__nv_bfloat16>(bits, vec, wide, rows, traditional);
+const void* rotary_kernel_for(int dtype, int bits, int vec, bool wide, bool shifted, bool traditional) {
+  return dtype == 0   ? rotary_bits<float>(bits, vec, wide, shifted, traditional)
+         : dtype == 1 ? rotary_bits<__half>(bits, vec, wide, shifted, traditional)
+                      : rotary_bits<__nv_bfloat16>(bits, vec, wide, shifted, traditional);
 }
 
 // Page dst[i] = page src[i] in every array and layer: a pure copy, bound by

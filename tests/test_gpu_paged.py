@@ -147,6 +147,47 @@ def test_rotary_rotates_gradients_back(cuda):
     assert abs(float(a - b)) < 1e-5 * float(x.double().norm() * y.double().norm())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("trad", [False, True])
+@pytest.mark.parametrize("d,rot", [(128, 122), (128, 2), (96, 62), (72, 70), (40, 6), (256, 250), (64, 36), (128, 120), (200, 100)])
+def test_rotary_parts_that_end_inside_an_access(cuda, d, rot, trad, dtype):
+    """Rotated halves and parts that are no whole number of 16-byte accesses, at lengths that fill the GPU and not."""
+    import torch
+    import sparse_decode as sd
+    dt, inv = tdt(torch, dtype), sd.rotary_frequencies(rot, 1e5)[0]
+    for n, hq in ((3, 2), (450, 9)):
+        g = gen(torch, d + rot + n)
+        q = torch.randn(n, hq, d, generator=g, device="cuda").to(dt)
+        k = torch.randn(n, 1, d, generator=g, device="cuda").to(dt)
+        w = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(dt)
+        pos = torch.randint(0, 1 << 20, (n,), generator=g, device="cuda", dtype=torch.int32)
+        want = [rotary64(q, pos, inv, trad, 1.25, w, 1e-5), rotary64(k, pos, inv, trad, 1.25, None, 0)]
+        got = sd.rotary(q, k, pos, inv, traditional=trad, factor=1.25, q_norm=w, eps=1e-5, q_out=q, k_out=k)  # in place
+        for o, (ref, size) in zip(got, want):
+            check_rows(torch, o, ref, size, dtype)
+
+
+@pytest.mark.parametrize("d,rot", [(128, 128), (128, 122), (64, 32), (96, 62)])
+@pytest.mark.parametrize("trad", [False, True])
+def test_rotary_infinities_reach_their_partner_only(cuda, d, rot, trad):
+    import torch
+    import sparse_decode as sd
+    x = torch.randn(2 * d, 3, d, generator=gen(torch, d + rot), device="cuda").bfloat16()
+    at = torch.arange(2 * d, device="cuda")
+    x[at, 1, at % d] = float("inf")
+    pos = (1 + at).int()
+    out = sd.rotary(x, None, pos, sd.rotary_frequencies(rot)[0], traditional=trad)[0]
+    i = at % d
+    if trad:
+        j = i ^ 1
+    else:
+        j = torch.where(i < rot // 2, i + rot // 2, i - rot // 2)
+    j = torch.where(i < rot, j, i)
+    hit = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    hit[at, 1, i] = hit[at, 1, j] = True
+    assert torch.equal(~torch.isfinite(out), hit)
+
+
 def test_rotary_nan_and_inf_stay_in_their_row(cuda):
     import torch
     import sparse_decode as sd
