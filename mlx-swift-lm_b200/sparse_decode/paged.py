@@ -34,6 +34,7 @@ _device = _raw_stream = None
 _CODE: dict = {}
 _I32 = _F32 = _U8 = None
 _L: Optional[ctypes.CDLL] = None
+_WORKSPACE: dict = {}  # bytes of paged_decode's workspace, which depend on the device and the heads alone
 
 
 def _load() -> None:
@@ -242,12 +243,15 @@ class KVPages:
             raise ValueError("pool arrays must be [n_pages, Hkv, page_size, .] or [n_layers, n_pages, Hkv, page_size, .]")
         small = (k_scales, k_biases, v_scales, v_biases)
         if bits:
-            if any(a is None for a in small):
+            if k_scales is None or k_biases is None or v_scales is None or v_biases is None:
                 raise ValueError("a quantized pool needs k/v scales and biases")
             dt, dim = k_scales.dtype, dim * 32 // bits
-            each = (*shape[:-1], dim // 64)
-            ptrs = [_arg(k, "k", _I32, dev), _arg(v, "v", _I32, dev, shape)]
-            ptrs += [_arg(a, n, dt, dev, each) for n, a in zip(("k_scales", "k_biases", "v_scales", "v_biases"), small)]
+            each = k_scales.shape
+            if each[:-1] != shape[:-1] or each[-1] != dim // 64:
+                raise ValueError(f"k_scales must have shape {(*shape[:-1], dim // 64)} (got {tuple(each)})")
+            ptrs = (_arg(k, "k", _I32, dev), _arg(v, "v", _I32, dev, shape), _arg(k_scales, "k_scales", dt, dev),
+                    _arg(k_biases, "k_biases", dt, dev, each), _arg(v_scales, "v_scales", dt, dev, each),
+                    _arg(v_biases, "v_biases", dt, dev, each))
         else:
             if small != (None, None, None, None):
                 raise ValueError("scales and biases need bits")
@@ -256,7 +260,6 @@ class KVPages:
         self.k, self.v = k, v
         self.k_scales, self.k_biases, self.v_scales, self.v_biases = small
         self.bits, self.device, self.torch_device, self.dtype = bits, dev, k.device, dt
-        self.workspace: dict = {}  # bytes of paged_decode's workspace by query heads
         self.n_layers, self.n_pages = n_layers, n_pages
         self.n_kv_heads, self.page_size, self.head_dim = hkv, page, dim
         self.struct = SDPages(*ptrs, n_pages, n_layers, hkv, dim, page, _dtype_code(dt), bits, 64 if bits else 0, 0)
@@ -343,11 +346,11 @@ def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = No
     hq = shape[1]
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    need = pages.workspace.get(hq)
-    if need is None:  # the bytes depend on the pool's heads and hq alone
+    need = _WORKSPACE.get((dev, pages.n_kv_heads, dim, hq))
+    if need is None:
         n = ctypes.c_int64()
         _check(_L.sd_paged_workspace(pages.struct, 1, hq, n))
-        need = pages.workspace[hq] = n.value
+        need = _WORKSPACE[dev, pages.n_kv_heads, dim, hq] = n.value
     if out is None:
         out = _like(q, stream)
     if stream is None:
