@@ -148,8 +148,8 @@ constexpr int kRotThreads = 128;
 // Measured on a 32K-token prompt of 32 + 8 heads of 128 (671 MB, floor 102 us)
 // and, for kRotFill, on 1000 tokens of it:
 constexpr int kRotDepth = 4;          // passes whose rows are under way: 107 us; 3: 114, 6: 112
-constexpr int kRotPasses = 16;        // most passes that one warp makes: 107 us; 8: 109, 32: 110
-constexpr int kRotFill = 2048;        // warps that fill the GPU: 5.9 us; 1024: 8.6, 4096: 6.9
+constexpr int kRotPasses = 16;        // most passes that one warp makes: 107.5 us; 8: 108.2, 32: 110.5
+constexpr int kRotFill = 2048;        // warps that fill the GPU: 6.2 us; 1024: 7.3, 4096: 7.4
 // Lanes per row (log2): a power of two with a chunk pair of 2 * vec elements for each, at most a warp.
 __host__ __device__ constexpr int rotary_lanes_log(int D, int vec) {
   int l = 0;

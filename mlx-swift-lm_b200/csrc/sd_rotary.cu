@@ -137,6 +137,9 @@ enum RotaryForm {
 // BITS 4 / 8: key and value rows are rounded to E, staged in shared memory and
 // quantized from there by the group of lanes that holds the row.
 // CPL: chunk pairs per lane.
+// Measured, bf16 rows of 128 with norms: 32K tokens of 40 heads (671 MB) 107.5
+// us, 6.2 TB/s; 6023 tokens of 48 heads (148 MB, floor 22.6 us) 27.5 us in the
+// half layout, 27.6 traditional, 62 in kShifted.
 template <typename E, int V, int CPL, int BITS, RotaryForm FORM>
 __global__ void __launch_bounds__(kRotThreads, 5) rotary_kernel(const __grid_constant__ RotaryParams p) {
   static_assert(FORM != kShifted || CPL == 1, "one chunk pair per lane");
