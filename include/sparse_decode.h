@@ -319,7 +319,7 @@ typedef struct {
 /* q_out / k_out = rotated q / k for batch x tokens tokens at
  * positions[batch * tokens] (int32). k (with n_kv_heads 0) or q (with
  * n_q_heads 0) may be absent; an output may be its own input. head_dim: even,
- * 2 .. 256. */
+ * 2 .. 256; batch * tokens (here, and n_tokens below): less than 2^31 - 64. */
 int32_t sd_rotary(const sd_rotation* rot, int32_t dtype, int32_t head_dim, int32_t batch, int32_t tokens,
                   const int32_t* positions, int32_t n_q_heads, const sd_rows* q, const sd_rows* q_out,
                   int32_t n_kv_heads, const sd_rows* k, const sd_rows* k_out, sd_stream stream);

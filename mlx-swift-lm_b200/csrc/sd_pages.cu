@@ -151,6 +151,9 @@ void limit_vec(const sd::Rows& r, int heads, int esize, int* vec) {
 }
 
 int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, int dtype, int bits, cudaStream_t st) {
+  // a warp's last group of tokens may reach 31 past the end, in 32-bit indexes
+  if (n_tokens >= (int64_t(1) << 31) - 64)
+    return fail(SD_ERR_SHAPE, "a call takes fewer than 2^31 - 64 tokens (got %lld)", (long long)n_tokens);
   const int es = elt_size(dtype);
   int vec = 16 / es;
   limit_vec(p.q, p.Hq, es, &vec);
@@ -192,7 +195,7 @@ int32_t launch_rotary(sd::RotaryParams& p, int64_t n_tokens, bool traditional, i
     k.per.set(std::max(per, 1));
     units += ((n_tokens + (1 << k.tok_log) - 1) >> k.tok_log) * per;
     if (units >= (int64_t(1) << 31) - warps - 64)
-      return fail(SD_ERR_SHAPE, "a call takes fewer than 2^31 rows (got %lld tokens)", (long long)n_tokens);
+      return fail(SD_ERR_SHAPE, "too many rows at once (%lld tokens)", (long long)n_tokens);
   }
   p.units = int(units);
   p.n_tokens = int(n_tokens);
