@@ -349,7 +349,7 @@ int32_t sd_copy_pages(const sd_pages* pages, const int32_t* src, const int32_t* 
  * [max(0, lengths[b] - window), lengths[b]) (window 0: all of them; the last
  * token is the new one, stored before the call). sinks: [n_q_heads] fp32 as
  * in sd_set_sinks, or NULL. A length of 0 gives zeros. Query heads per kv
- * head: 1 .. 16. Lengths and tables are read on the device only. The
+ * head: 1 .. 16; 65536 at most in all. Lengths and tables are read on the device only. The
  * workspace (sd_paged_workspace bytes -- they depend on n_q_heads, the pool and
  * the GPU, not on the batch -- 16-byte aligned, contents do not matter) must
  * not be shared by calls that may overlap. Pages past a

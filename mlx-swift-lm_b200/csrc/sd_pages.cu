@@ -340,6 +340,7 @@ static int32_t check_heads(const sd_pages* g, int32_t batch, int32_t n_q_heads) 
   if (batch < 1 || batch > sd::kPagedMaxBatch) return fail(SD_ERR_SHAPE, "batch must be in [1, %d] (got %d)", sd::kPagedMaxBatch, batch);
   if (n_q_heads < 1 || n_q_heads % g->n_kv_heads)
     return fail(SD_ERR_SHAPE, "n_q_heads (%d) is not a positive multiple of n_kv_heads (%d)", n_q_heads, g->n_kv_heads);
+  if (n_q_heads > 65536) return fail(SD_ERR_SHAPE, "too many heads");  // the kernels index head * D in 32 bits
   if (n_q_heads / g->n_kv_heads > 16) return fail(SD_ERR_SHAPE, "at most 16 query heads per kv head (got %d)", n_q_heads / g->n_kv_heads);
   return SD_OK;
 }
