@@ -70,6 +70,13 @@ def _arg(t, name: str, dtype, dev: int, shape=None) -> Optional[int]:
     return t.data_ptr()
 
 
+def _count(n: int, name: str) -> int:
+    """A number that goes into a 32-bit argument: ctypes would keep its low bits."""
+    if not -(1 << 31) <= n < 1 << 31:
+        raise ValueError(f"{name} must be below 2^31 (got {n})")
+    return n
+
+
 def _rows(t, name: str, dtype, dev: int, dim: int) -> tuple:
     """sd_rows of [tokens, heads, D] or [batch, heads, tokens, D] with any
     strides but the last, as (struct, batch, tokens, heads)."""
@@ -82,6 +89,8 @@ def _rows(t, name: str, dtype, dev: int, dim: int) -> tuple:
         raise ValueError(f"{name} has head_dim {shape[-1]}, expected {dim}")
     if st[-1] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
+    if max(shape) >= 1 << 31:
+        raise ValueError(f"{name} must have fewer than 2^31 tokens and heads (got {tuple(shape)})")
     if len(shape) == 3:
         return SDRows(t.data_ptr(), 0, st[0], st[1]), 1, shape[0], shape[1]
     if len(shape) == 4:
@@ -120,7 +129,7 @@ def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: in
     if inv_freq is not None:
         if inv_freq.dim() != 1:
             raise ValueError("inv_freq must be [rot_dim / 2]")
-        rot = 2 * inv_freq.shape[0]
+        rot = _count(2 * inv_freq.shape[0], "rot_dim")
     return SDRotation(_arg(inv_freq, "inv_freq", _F32, dev), _arg(q_norm, "q_norm", dtype, dev, (dim,)),
                       _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
 
@@ -301,10 +310,10 @@ def paged_append(pages: KVPages, k, v, tables, positions, *, seq=None, layer: in
         q_out, qo = _out(q, q_out, "q_out", dt, dev, dim, stream)
     if q is not None or inv_freq is not None or q_norm is not None or k_norm is not None:
         rot = _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dt, dev, dim)
-    batch, width = tables.shape
-    _check(_L.sd_paged_append(pages.struct, layer, n, kr, vr, _arg(tables, "tables", _I32, dev), batch, width,
-                              _arg(positions, "positions", _I32, dev, (n,)), _arg(seq, "seq", _I32, dev, (n,)), rot, hq,
-                              qr, qo, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
+    batch, width = _count(tables.shape[0], "batch"), _count(tables.shape[1], "width")
+    _check(_L.sd_paged_append(pages.struct, _count(layer, "layer"), n, kr, vr, _arg(tables, "tables", _I32, dev), batch,
+                              width, _arg(positions, "positions", _I32, dev, (n,)), _arg(seq, "seq", _I32, dev, (n,)),
+                              rot, hq, qr, qo, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
     return q_out if q is not None else None
 
 
@@ -327,7 +336,7 @@ def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
     if src.dim() != 1:
         raise ValueError("src and dst must be [n]")
     _check(_L.sd_copy_pages(pages.struct, _arg(src, "src", _I32, dev), _arg(dst, "dst", _I32, dev, src.shape),
-                            src.shape[0], _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
+                            _count(src.shape[0], "n"), _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
 
 
 def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = None, *, layer: int = 0, window: int = 0,
@@ -358,8 +367,9 @@ def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = No
     else:
         with torch.cuda.stream(stream):
             work = torch.empty(need, dtype=_U8, device=pages.torch_device)
-    _check(_L.sd_paged_decode(pages.struct, layer, _arg(q, "q", dt, dev), batch, hq, _arg(tables, "tables", _I32, dev),
-                              width, _arg(lengths, "lengths", _I32, dev, (batch,)), scale, window,
+    _check(_L.sd_paged_decode(pages.struct, _count(layer, "layer"), _arg(q, "q", dt, dev), batch, hq,
+                              _arg(tables, "tables", _I32, dev), _count(width, "width"),
+                              _arg(lengths, "lengths", _I32, dev, (batch,)), scale, _count(window, "window"),
                               _arg(sinks, "sinks", _F32, dev, (hq,)), _arg(out, "out", dt, dev, shape), work.data_ptr(),
                               need, _arg(flags, "flags", _I32, dev), _handle(stream, dev)))
     return out

@@ -37,3 +37,39 @@ def test_decode_refuses_heads_past_its_32_bit_rows(native, kv, G):  # noqa: F811
     assert _decode(native, g=g, heads=kv * G, batch=1, width=1) == "SD_ERR_SHAPE"
     n = ctypes.c_int64()
     assert sdp.STATUS[native.sd_paged_workspace(g, 1, kv * G, ctypes.byref(n))] == "SD_ERR_SHAPE"
+
+
+def test_rows_of_more_tokens_than_32_bits_are_refused():
+    """A ctypes argument keeps the low 32 bits of a larger number, so the calls refuse it first."""
+    import torch
+    x = torch.zeros(2)
+    for n in ((1 << 32) + 5, 1 << 31):
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged._rows(x.as_strided((n, 1, 2), (0, 0, 1)), "q", x.dtype, -1, 2)
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged._rows(x.as_strided((n, 1, 1, 2), (0, 0, 0, 1)), "q", x.dtype, -1, 2)
+    assert paged._rows(x.as_strided(((1 << 31) - 1, 1, 2), (0, 0, 1)), "q", x.dtype, -1, 2)[2] == (1 << 31) - 1
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 16, 1 << 62, -(1 << 32) + 5])
+def test_counts_past_32_bits_are_refused(n):
+    with pytest.raises(ValueError, match="window"):
+        paged._count(n, "window")
+
+
+@pytest.mark.parametrize("n", [0, -1, 7, (1 << 31) - 1, -(1 << 31)])
+def test_counts_of_32_bits_pass(n):
+    assert paged._count(n, "window") == n
+
+
+@pytest.mark.gpu
+def test_calls_refuse_layers_and_windows_past_32_bits(cuda):
+    import torch
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    p, i32 = sdp.KVPages(z(2, 1, 16, 64), z(2, 1, 16, 64)), torch.int32
+    q, k, t, n = z(1, 4, 64), z(1, 1, 64), z(1, 1, dt=i32), torch.ones(1, dtype=i32, device="cuda")
+    far = 1 << 32
+    for bad in (lambda: sdp.paged_decode(q, p, t, n, window=far + 16), lambda: sdp.paged_decode(q, p, t, n, layer=far),
+                lambda: sdp.paged_append(p, k, k, t, n - 1, layer=far)):
+        with pytest.raises(ValueError):
+            bad()
