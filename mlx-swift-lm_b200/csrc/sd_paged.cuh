@@ -1016,7 +1016,6 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   int* prefix = reinterpret_cast<int*>(sm + p.prefix_off);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
   uint64_t* empty = full + kPagedMaxStages;
-  __shared__ int warp_tot[kPagedThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -1045,6 +1044,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     prefix[lane] = lane ? before : 0;  // B + 1 entries matter
     __syncthreads();                   // the barriers of the ring are set up, too
   } else {
+    int* warp_tot = prefix + p.B + 1;
     const int per = (p.B + kPagedThreads - 1) / kPagedThreads;
     int mine = 0;
     for (int k = 0; k < per; ++k) {

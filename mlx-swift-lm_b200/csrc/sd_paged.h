@@ -25,7 +25,11 @@ constexpr int kPagedMaxStages = 16;
 // ragged users of up to 4096 tokens in 8 bits, a decode took 25.2 us when cut
 // by tiles alone, 19.9 / 19.3 / 20.2 us with 1 / 2 / 3.
 constexpr int kSegmentUnits = 2;
-// Two CTAs share an SM: half of its 228 KB each, less 1 KB that every CTA reserves.
+// Two CTAs share an SM: half of its 228 KB each, less 1 KB that every CTA
+// reserves. All of it is dynamic: 32 static bytes beside a full dynamic share
+// left room for one CTA only, and the second half of the grid ran after the
+// first (11 heads of 64 per kv head on 4-bit codes, 4 x 32K tokens: 66.2 us,
+// 44.3 without them; 224 bf16 sequences of 2K, 28 heads: 150.8, 147.2).
 constexpr int kPagedSmem = 115712;
 
 // Stored rows of one pool format: E of ESIZE bytes (dense element, or type of
@@ -55,6 +59,31 @@ struct PagedFmt {
 // 16-byte accesses.
 __host__ __device__ constexpr int paged_warp_floats(int G, int D) { return (G * (D + 6) + 3) / 4 * 4; }
 __host__ __device__ constexpr int paged_part_floats(int G, int D) { return (G * (D + 2) + 3) / 4 * 4; }
+
+// Where the parts of a decode CTA's shared memory lie, from a 1 KB boundary:
+// the ring, q of dense fp32 calls, the warps' combine buffer, the units before
+// each sequence (and the warps' totals of them), the ring's barriers.
+struct PagedLayout {
+  int stages;  // as many as fit beside the fixed parts; below 1: the call does not fit
+  int q_off, buf_off, prefix_off, bar_off;
+  int bytes;   // of the launch, the way to the boundary included
+};
+constexpr PagedLayout paged_layout(int batch, int G, int D, bool dense_f32, int stage_bytes) {
+  const int qf = dense_f32 ? G * (D + 4) * 4 : 0, buf = kPagedWarps * paged_warp_floats(G, D) * 4;
+  // below 32 sequences every warp has its own row of 32
+  const int pre = (batch < 32 ? 32 * (kPagedWarps + 1) : batch + 1 + kPagedThreads / 32) * 4;
+  const int bars = 2 * kPagedMaxStages * 8;
+  const int q128 = (qf + 127) / 128 * 128, buf128 = (buf + 127) / 128 * 128, pre128 = (pre + 127) / 128 * 128;
+  const int room = (kPagedSmem - (q128 + buf128 + pre128 + bars + 1024)) / stage_bytes;
+  PagedLayout l{};
+  l.stages = room < kPagedMaxStages ? room : kPagedMaxStages;
+  l.q_off = l.stages * stage_bytes;
+  l.buf_off = l.q_off + q128;
+  l.prefix_off = l.buf_off + buf128;
+  l.bar_off = l.prefix_off + pre128;
+  l.bytes = l.bar_off + bars + 1024;
+  return l;
+}
 
 struct PagedParams {
   const void* q;          // [B, Hkv * G, D]

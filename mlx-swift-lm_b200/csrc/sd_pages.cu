@@ -418,26 +418,20 @@ int32_t sd_paged_decode(const sd_pages* g, int32_t layer, const void* q, int32_t
   p.magic = 0x64006400u;
   p.flags = device_flags;
 
-  // shared memory: as many stages as fit beside the fixed parts
-  const int buf = sd::kPagedWarps * sd::paged_warp_floats(G, D) * 4;
-  const int qf = g->dtype == SD_F32 && !g->kv_bits ? G * (D + 4) * 4 : 0;  // q of a dense fp32 call
-  const int pre = (batch < 32 ? 32 * (sd::kPagedWarps + 1) : batch + 1) * 4, bars = 2 * sd::kPagedMaxStages * 8;
-  auto up = [](int x) { return (x + 127) / 128 * 128; };
-  const int fixed = up(qf) + up(buf) + up(pre) + bars + 1024;
-  p.stages = std::min((sd::kPagedSmem - fixed) / ks.stage_bytes, sd::kPagedMaxStages);
-  if (p.stages < 1) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
-  p.q_off = p.stages * ks.stage_bytes;
-  p.buf_off = p.q_off + up(qf);
-  p.prefix_off = p.buf_off + up(buf);
-  p.bar_off = p.prefix_off + up(pre);
-  const size_t smem = size_t(p.bar_off + bars) + 1024;
+  const sd::PagedLayout lay = sd::paged_layout(batch, G, D, g->dtype == SD_F32 && !g->kv_bits, ks.stage_bytes);
+  if (lay.stages < 1) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
+  p.stages = lay.stages;
+  p.q_off = lay.q_off;
+  p.buf_off = lay.buf_off;
+  p.prefix_off = lay.prefix_off;
+  p.bar_off = lay.bar_off;
   SD_CUDA(cudaFuncSetAttribute(ks.decode, cudaFuncAttributeMaxDynamicSharedMemorySize, sd::kPagedSmem));
 
   const int64_t max_units = max_tiles * batch * g->n_kv_heads;
   p.ncta = int(std::min<int64_t>(max_ctas, max_units));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   void* args[3] = {&p, &tmK, &tmV};
-  if (int32_t rc = launch(ks.decode, dim3(unsigned(p.ncta)), sd::kPagedThreads, smem, st, args)) return rc;
+  if (int32_t rc = launch(ks.decode, dim3(unsigned(p.ncta)), sd::kPagedThreads, size_t(lay.bytes), st, args)) return rc;
   void* margs[1] = {&p};
   if (int64_t(batch) * n_q_heads > sd::kMergeMany) {
     const unsigned per = unsigned(n_q_heads + sd::kMergeHeads - 1) / sd::kMergeHeads;

@@ -2,12 +2,51 @@
 answer here comes before a launch."""
 from __future__ import annotations
 
+import subprocess
+
 import pytest
 
 import sparse_decode as sdp
 from sparse_decode import paged
 
 from test_paged import _decode, _pages, _rotary, native  # noqa: F401
+
+
+# -- residency ------------------------------------------------------------------
+
+def test_two_decode_ctas_fit_an_sm(tmp_path):
+    """For every format, head count and batch, from the layout that the launch uses: an SM has 228 KB and keeps 1 KB of
+    it per CTA. Static shared memory would come on top; the decode kernel has none."""
+    src = tmp_path / "layout.cpp"
+    src.write_text("""#include <cuda_runtime.h>
+#include <cstdio>
+#include "sd_paged.h"
+using namespace sd;
+int bad = 0, full = 0;
+template <int ESIZE, int BITS, int D> void all() {
+  using F = PagedFmt<ESIZE, BITS, D>;
+  for (int G = 1; G <= 16; ++G)
+    for (int b = 1; b <= kPagedMaxBatch; ++b) {
+      const PagedLayout l = paged_layout(b, G, D, ESIZE == 4 && BITS == 0, F::kStageBytes);
+      const int parts = l.q_off <= l.buf_off && l.buf_off + 4 * kPagedWarps * paged_warp_floats(G, D) <= l.prefix_off &&
+                        l.prefix_off + 4 * (b < 32 ? 160 : b + 1 + 5) <= l.bar_off && l.bar_off + 2 * 8 * l.stages + 1024 <= l.bytes;
+      if (l.stages < 1 || !parts || 2 * (l.bytes + 1024) > 228 * 1024) ++bad;
+      full += l.bytes == kPagedSmem;
+    }
+}
+int main() {
+  all<2, 0, 64>(); all<2, 0, 128>(); all<4, 0, 64>(); all<4, 0, 128>();
+  all<2, 4, 64>(); all<2, 4, 128>(); all<4, 4, 64>(); all<4, 4, 128>();
+  all<2, 8, 64>(); all<2, 8, 128>(); all<4, 8, 64>(); all<4, 8, 128>();
+  std::printf("%d %d", bad, full);
+}
+""")
+    exe = tmp_path / "layout"
+    csrc = sdp.LIB_PATH.parent / "csrc"
+    subprocess.run(["g++", "-std=c++17", f"-I{csrc}", "-I/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
+    bad, full = map(int, subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
+    assert bad == 0
+    assert full > 0  # some calls fill their share to the last byte: nothing may be added to it
 
 
 # -- counts ---------------------------------------------------------------------
