@@ -145,8 +145,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 low_freq_factor are divided, those below .../high_freq_factor
                 are kept, a linear blend between;
     * yarn:     the same blend by the number of turns over the original
-                context (beta_fast, beta_slow), and the rotated part scaled
-                by 0.1 ln(factor) + 1 (or by the mscale pair's ratio);
+                context (beta_fast, beta_slow; between whole pairs unless
+                `truncate` is false), and the rotated part scaled by
+                0.1 ln(factor) + 1 (or by the mscale pair's ratio);
     * longrope: each angle divided by its own entry of long_factor (of
                 short_factor when `factor` is at most 1), rotated part scaled
                 by sqrt(1 + ln(factor) / ln(original)).
@@ -170,8 +171,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
         elif kind == "yarn":
             def dim_of(turns: float) -> float:  # the pair that makes `turns` turns over the original context
                 return rot_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base))
-            lo = max(math.floor(dim_of(float(scaling.get("beta_fast", 32.0)))), 0)
-            hi = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+            lo, hi = dim_of(float(scaling.get("beta_fast", 32.0))), dim_of(float(scaling.get("beta_slow", 1.0)))
+            if scaling.get("truncate", True):
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(lo, 0), min(hi, rot_dim - 1)
             i = torch.arange(rot_dim // 2, dtype=torch.float64)
             stretch = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
             inv = inv * (1 - stretch) + inv / f * stretch
