@@ -134,7 +134,9 @@ def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: in
                       _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
 
 
-def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda"):
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda", *,
+                       max_position_embeddings: Optional[int] = None,
+                       original_max_position_embeddings: Optional[int] = None):
     """(inv_freq [rot_dim / 2] fp32 on `device`, factor) for `rotary` and
     `paged_append`: base^(-2i / rot_dim), computed in 64 bits, with the
     positions stretched for long contexts by `scaling`, a model
@@ -150,7 +152,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 0.1 ln(factor) + 1 (or by the mscale pair's ratio);
     * longrope: each angle divided by its own entry of long_factor (of
                 short_factor when `factor` is at most 1), rotated part scaled
-                by sqrt(1 + ln(factor) / ln(original)).
+                by sqrt(1 + ln(factor) / ln(original)) or attention_factor.
+                Where the dict has no `factor`, it is max_position_embeddings
+                / original_max_position_embeddings, which such configurations
+                keep outside of it: pass them here.
     """
     import torch
     if rot_dim < 2 or rot_dim % 2:
@@ -188,12 +193,22 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
             else:
                 mult = mscale(1.0)
         elif kind in ("longrope", "su"):
-            each = scaling["long_factor"] if f > 1 else scaling["short_factor"]
-            if len(each) != rot_dim // 2:
-                raise ValueError(f"expected {rot_dim // 2} factors, got {len(each)}")
+            known = scaling.get("original_max_position_embeddings", original_max_position_embeddings)
+            if "factor" not in scaling:
+                if known is None or max_position_embeddings is None:
+                    raise ValueError("longrope needs factor, or max_ and original_max_position_embeddings")
+                f = max_position_embeddings / known
+            name = "long_factor" if f > 1 else "short_factor"
+            each = scaling.get(name)
+            if each is None or len(each) != rot_dim // 2:
+                raise ValueError(f"longrope needs {rot_dim // 2} numbers in {name}")
             inv = inv / torch.tensor(each, dtype=torch.float64)
-            mult = float(scaling.get("attention_factor",
-                                     math.sqrt(1 + math.log(f) / math.log(old)) if f > 1 else 1.0))
+            if "attention_factor" in scaling:
+                mult = float(scaling["attention_factor"])
+            elif f > 1:
+                if known is None:
+                    raise ValueError("longrope needs original_max_position_embeddings or attention_factor")
+                mult = math.sqrt(1 + math.log(f) / math.log(known))
         elif kind != "default":
             raise ValueError(f"unknown rope scaling {kind!r}")
     return inv.to(torch.float32).to(device), mult

@@ -36,3 +36,45 @@ def test_yarn_bounds_are_whole_pairs_unless_told_otherwise(more, truncate):
     got, mult = freq(64, 150000.0, s)
     assert got == pytest.approx(yarn(64, 150000.0, 32.0, 4096, truncate=truncate), rel=1e-6)
     assert mult == pytest.approx(0.1 * math.log(32) + 1)
+
+
+LONG, SHORT = [1.0 + 0.5 * i for i in range(48)], [1.0 + 0.01 * i for i in range(48)]
+PUBLISHED = {"type": "longrope", "long_factor": LONG, "short_factor": SHORT}  # the lengths stand outside the dict
+
+
+def longrope(each):
+    return [10000.0 ** (-2 * i / 96) / f for i, f in enumerate(each)]
+
+
+def test_longrope_takes_the_lengths_that_stand_outside_the_dict():
+    got, mult = freq(96, 10000.0, PUBLISHED, max_position_embeddings=131072, original_max_position_embeddings=4096)
+    assert got == pytest.approx(longrope(LONG), rel=1e-6)
+    assert mult == pytest.approx(math.sqrt(1 + math.log(32) / math.log(4096))) == pytest.approx(1.19, abs=1e-2)
+    got, mult = freq(96, 10000.0, PUBLISHED, max_position_embeddings=4096, original_max_position_embeddings=4096)
+    assert got == pytest.approx(longrope(SHORT), rel=1e-6) and mult == 1.0
+    # what the dict says itself comes first
+    s = {**PUBLISHED, "factor": 8.0, "original_max_position_embeddings": 16384}
+    got, mult = freq(96, 10000.0, s, max_position_embeddings=131072, original_max_position_embeddings=4096)
+    assert got == pytest.approx(longrope(LONG), rel=1e-6)
+    assert mult == pytest.approx(math.sqrt(1 + math.log(8) / math.log(16384)))
+
+
+@pytest.mark.parametrize("more", [{}, {"max_position_embeddings": 131072}, {"original_max_position_embeddings": 4096}])
+def test_longrope_without_its_lengths_is_refused(more):
+    with pytest.raises(ValueError):
+        freq(96, 10000.0, PUBLISHED, **more)
+
+
+@pytest.mark.parametrize("missing", ["long_factor", "short_factor"])
+def test_longrope_without_its_factors_is_refused(missing):
+    s = {k: v for k, v in PUBLISHED.items() if k != missing}
+    with pytest.raises(ValueError):
+        freq(96, 10000.0, s, max_position_embeddings=131072 if missing == "long_factor" else 4096,
+             original_max_position_embeddings=4096)
+
+
+def test_longrope_without_an_original_length_to_scale_by_is_refused():
+    with pytest.raises(ValueError):
+        freq(96, 10000.0, {**PUBLISHED, "factor": 32.0})
+    got, mult = freq(96, 10000.0, {**PUBLISHED, "factor": 32.0, "attention_factor": 1.25})  # needs none
+    assert got == pytest.approx(longrope(LONG), rel=1e-6) and mult == 1.25
