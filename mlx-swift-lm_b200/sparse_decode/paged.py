@@ -134,6 +134,20 @@ def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: in
                       _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
 
 
+# The keys of a rope_scaling dict that each kind's formula has, and those that say nothing about the angles (rope_theta
+# is checked against the base).
+_SCALING_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"),
+    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "attention_factor",
+             "mscale", "mscale_all_dim"),
+    "longrope": ("factor", "original_max_position_embeddings", "long_factor", "short_factor", "attention_factor"),
+}
+_SCALING_KEYS["su"] = _SCALING_KEYS["longrope"]
+_SILENT_KEYS = ("type", "rope_type", "rope_theta", "partial_rotary_factor", "finetuned")
+
+
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda", *,
                        max_position_embeddings: Optional[int] = None,
                        original_max_position_embeddings: Optional[int] = None):
@@ -156,6 +170,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 Where the dict has no `factor`, it is max_position_embeddings
                 / original_max_position_embeddings, which such configurations
                 keep outside of it: pass them here.
+
+    A missing `factor` or original length is refused, and so is a key that the
+    formula does not have; low_ and high_freq_factor are 1 and 4, beta_fast
+    and beta_slow 32 and 1 where they are not given. What the dict says comes
+    before the parameters; None counts as not given.
     """
     import torch
     if rot_dim < 2 or rot_dim % 2:
@@ -163,13 +182,28 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
     inv = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
     mult = 1.0
     if scaling is not None:
+        scaling = {k: v for k, v in scaling.items() if v is not None}
         kind = scaling.get("rope_type", scaling.get("type", "default"))
+        if kind not in _SCALING_KEYS:
+            raise ValueError(f"unknown rope scaling {kind!r}")
+        other = [k for k in scaling if k not in _SCALING_KEYS[kind] and k not in _SILENT_KEYS]
+        if other:
+            raise ValueError(f"{kind} rope scaling does not have {', '.join(other)}")
+        if float(scaling.get("rope_theta", base)) != float(base):
+            raise ValueError(f"rope_theta is {scaling['rope_theta']}, the base {base}")
         f = float(scaling.get("factor", 1.0))
-        old = float(scaling.get("original_max_position_embeddings", 8192))
+        known = scaling.get("original_max_position_embeddings", original_max_position_embeddings)
+        if kind in ("linear", "llama3", "yarn") and "factor" not in scaling:
+            raise ValueError(f"{kind} rope scaling needs factor")
+        if kind in ("llama3", "yarn") and known is None:
+            raise ValueError(f"{kind} rope scaling needs original_max_position_embeddings")
+        old = float(known or 0)
         if kind == "linear":
             inv = inv / f
         elif kind == "llama3":
             lo, hi = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+            if hi <= lo:
+                raise ValueError("high_freq_factor must be above low_freq_factor")
             turns = old * inv / (2 * math.pi)
             keep = ((turns - lo) / (hi - lo)).clamp(0, 1)
             inv = inv * (keep + (1 - keep) / f)
@@ -188,12 +222,13 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 return 0.1 * m * math.log(f) + 1.0 if f > 1 else 1.0
             if "attention_factor" in scaling:
                 mult = float(scaling["attention_factor"])
+            elif ("mscale" in scaling) != ("mscale_all_dim" in scaling):
+                raise ValueError("mscale and mscale_all_dim come together")
             elif scaling.get("mscale") and scaling.get("mscale_all_dim"):
                 mult = mscale(float(scaling["mscale"])) / mscale(float(scaling["mscale_all_dim"]))
             else:
                 mult = mscale(1.0)
         elif kind in ("longrope", "su"):
-            known = scaling.get("original_max_position_embeddings", original_max_position_embeddings)
             if "factor" not in scaling:
                 if known is None or max_position_embeddings is None:
                     raise ValueError("longrope needs factor, or max_ and original_max_position_embeddings")
@@ -209,8 +244,6 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 if known is None:
                     raise ValueError("longrope needs original_max_position_embeddings or attention_factor")
                 mult = math.sqrt(1 + math.log(f) / math.log(known))
-        elif kind != "default":
-            raise ValueError(f"unknown rope scaling {kind!r}")
     return inv.to(torch.float32).to(device), mult
 
 

@@ -78,3 +78,50 @@ def test_longrope_without_an_original_length_to_scale_by_is_refused():
         freq(96, 10000.0, {**PUBLISHED, "factor": 32.0})
     got, mult = freq(96, 10000.0, {**PUBLISHED, "factor": 32.0, "attention_factor": 1.25})  # needs none
     assert got == pytest.approx(longrope(LONG), rel=1e-6) and mult == 1.25
+
+
+COMPLETE = {
+    "linear": {"rope_type": "linear", "factor": 4.0},
+    "llama3": {"rope_type": "llama3", "factor": 8.0, "original_max_position_embeddings": 8192},
+    "yarn": {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768},
+}
+
+
+@pytest.mark.parametrize("kind,key", [(k, key) for k, s in COMPLETE.items() for key in s if key != "rope_type"])
+def test_a_missing_key_is_refused_and_not_guessed(kind, key):
+    s = COMPLETE[kind]
+    freq(64, 10000.0, s)
+    for without in ({k: v for k, v in s.items() if k != key}, {**s, key: None}):
+        with pytest.raises(ValueError, match=key):
+            freq(64, 10000.0, without)
+
+
+@pytest.mark.parametrize("kind", ["llama3", "yarn"])
+def test_the_original_length_may_stand_outside_the_dict(kind):
+    s = dict(COMPLETE[kind])
+    old = s.pop("original_max_position_embeddings")
+    assert freq(64, 10000.0, s, original_max_position_embeddings=old) == freq(64, 10000.0, COMPLETE[kind])
+    # and the dict's own comes first
+    assert freq(64, 10000.0, COMPLETE[kind], original_max_position_embeddings=77) == freq(64, 10000.0, COMPLETE[kind])
+
+
+@pytest.mark.parametrize("s", [
+    {**COMPLETE["yarn"], "long_mscale": 1.2}, {**COMPLETE["linear"], "beta_fast": 32.0},
+    {**COMPLETE["llama3"], "attention_factor": 1.1}, {"rope_type": "default", "factor": 4.0},
+    {"type": "default", "mrope_section": [16, 24, 24]}, {**COMPLETE["yarn"], "mscale": 0.7},
+    {**COMPLETE["yarn"], "mscale_all_dim": 0.7}, {**COMPLETE["linear"], "rope_theta": 5e5},
+    {**COMPLETE["llama3"], "low_freq_factor": 4.0}])
+def test_what_is_not_honoured_is_refused(s):
+    """Keys that would change the angles and that the kind's formula does not have; half of a pair; another base."""
+    with pytest.raises(ValueError):
+        freq(64, 10000.0, s)
+
+
+def test_keys_that_change_nothing_pass():
+    for kind, s in COMPLETE.items():
+        more = {**s, "type": kind, "rope_theta": 10000, "partial_rotary_factor": 0.5, "attention_factor": None}
+        assert freq(64, 10000.0, more) == freq(64, 10000.0, s)
+    assert freq(64, 10000.0, {**COMPLETE["yarn"], "finetuned": True}) == freq(64, 10000.0, COMPLETE["yarn"])
+    assert freq(64, 10000.0, {**COMPLETE["yarn"], "truncate": None}) == freq(64, 10000.0, COMPLETE["yarn"])
+    assert freq(64, 10000.0, {**COMPLETE["yarn"], "mscale": 1.0, "mscale_all_dim": 1.0})[1] == 1.0
+    assert freq(64, 10000.0, {}) == freq(64, 10000.0)
