@@ -609,7 +609,9 @@ class PagedLayer:
     def attend(self, queries, keys, values, scale: float, mask=None, sinks=None):
         """Append keys/values [B, Hkv, L, D] and attend with queries
         [B, Hq, L, D]; every sequence has L new tokens. L == 1 takes the decode
-        kernel; longer prompts are attended densely, sequence by sequence."""
+        kernel; longer prompts are attended densely, sequence by sequence, with
+        `mask` as for the other caches: None hides nothing, "causal" the tokens
+        after each one."""
         from .cache import _dense_attention
         b = self.batch
         B, Hq, L, D = queries.shape
@@ -630,7 +632,7 @@ class PagedLayer:
         out = torch.empty_like(queries)
         for i in range(B):
             k, v = self.dense(i)
-            out[i] = _dense_attention(q[i:i + 1], k, v, scale, "causal" if mask is None else mask, sinks)[0]
+            out[i] = _dense_attention(q[i:i + 1], k, v, scale, mask, sinks)[0]
         return out
 
     def dense(self, i: int):

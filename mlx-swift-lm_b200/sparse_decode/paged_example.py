@@ -37,7 +37,7 @@ def run(layers: int = 4, kv_bits: int = 0, prompts=(70, 33), steps: int = 20, pa
         for i in range(layers):
             q, k, v = (x @ project[i]).unflatten(-1, (-1, d)).split((hq, hkv, hkv), dim=2)
             out = attention_with_cache_update(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
-                                              batch.layer(i, **turn), d ** -0.5)
+                                              batch.layer(i, **turn), d ** -0.5, "causal" if x.shape[1] > 1 else None)
             outs.append(out[:, :, -1])
             x = (x + out.transpose(1, 2).flatten(2)[..., :hidden]).bfloat16()
         return outs

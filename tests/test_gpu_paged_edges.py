@@ -1,0 +1,71 @@
+"""The paged cache on the GPU where its answers are easy to lose: weights far
+below the largest, scores that tie, masks of the router, steps that fail.
+
+Bounds are stated at each test, from the kernels' arithmetic; the references
+are computed in 64 bits.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+from test_gpu_paged import gen, tdt
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# the router
+# ---------------------------------------------------------------------------
+
+def prompt(torch, bits=0, lengths=(37, 37), new=None, hq=8, hkv=2, d=128, seed=0):
+    """A pool with sequences of these lengths, all but the last `new` tokens (None: none of them) stored, and the
+    step's q, k, v [B, heads, new, d]."""
+    import sparse_decode as sd
+    g = gen(torch, seed)
+    B, new = len(lengths), min(lengths) if new is None else new
+    pool = sd.PagePool(1, 40, hkv, d, 16, "bf16", bits)
+    seqs = [pool.add() for _ in lengths]
+    rows = [[torch.randn(hkv, n, d, generator=g, device="cuda").bfloat16() for n in lengths] for _ in "kv"]
+    for i, n in enumerate(lengths):
+        if n > new:
+            step = pool.extend(seqs[i:i + 1], n - new)
+            step.append(0, *(x[i][:, :n - new].transpose(0, 1) for x in rows))
+    q = torch.randn(B, hq, new, d, generator=g, device="cuda").bfloat16()
+    k, v = (torch.stack([y[:, -new:] for y in x]) for x in rows)
+    return pool, seqs, rows, q, k, v
+
+
+def attend64(q, k, v, scale, keep, sinks=None):
+    """One sequence: q [Hq, L, D], k, v [Hkv, T, D], keep [.., L, T] (bool, or numbers to add)."""
+    import torch
+    k, v = (x.double().repeat_interleave(q.shape[0] // x.shape[0], 0) for x in (k, v))
+    s = q.double() @ k.transpose(1, 2) * scale
+    s = s.masked_fill(~keep, -math.inf) if keep.dtype == torch.bool else s + keep.double()
+    if sinks is not None:
+        s = torch.cat((s, sinks.double().view(-1, 1, 1).expand(-1, s.shape[1], 1)), -1)
+    return torch.softmax(s, -1)[..., :k.shape[1]] @ v
+
+
+def close(out, ref):
+    """Dense attention in bf16: its probabilities and sums may be rounded to bf16, 2^-8, once or twice."""
+    assert float((out.double() - ref).norm() / ref.norm()) < 2e-2
+
+
+@pytest.mark.parametrize("mask", [None, "causal"])
+@pytest.mark.parametrize("with_sinks", [False, True])
+def test_router_without_a_mask_hides_nothing(cuda, mask, with_sinks):
+    """None and "causal" mean for a paged layer what they mean for the other caches."""
+    import torch
+    import sparse_decode as sd
+    pool, seqs, rows, q, k, v = prompt(torch, seed=1)
+    sinks = torch.randn(8, generator=gen(torch, 2), device="cuda") if with_sinks else None
+    out = sd.attention_with_cache_update(q, k, v, pool.extend(seqs, 37).layer(0), 0.1, mask, sinks)
+    same = sd.attention_with_cache_update(q, k, v, None, 0.1, mask, sinks)
+    keep = torch.ones(37, 37, dtype=torch.bool, device="cuda")
+    keep = keep.tril() if mask else keep
+    for b in range(2):
+        ref = attend64(q[b], k[b], v[b], 0.1, keep, sinks)
+        close(out[b], ref)
+        close(same[b], ref)
