@@ -611,12 +611,17 @@ class PagedLayer:
         [B, Hq, L, D]; every sequence has L new tokens. L == 1 takes the decode
         kernel; longer prompts are attended densely, sequence by sequence, with
         `mask` as for the other caches: None hides nothing, "causal" the tokens
-        after each one."""
+        after each one; a tensor (bool, or numbers to add) is broadcast to
+        [B, Hq, L, T], T the longest sequence's tokens, and column t is token t
+        of every sequence."""
         from .cache import _dense_attention
         b = self.batch
         B, Hq, L, D = queries.shape
         if any(n != L for n in b.new) or len(b.new) != B:
             raise ValueError(f"the step holds {b.new} new tokens, the queries {[L] * B}")
+        if L == 1 and mask is not None:
+            raise ValueError("a single-token step takes no mask")
+        masks = self._masks(mask, B, Hq, L)
         flat = lambda x: x.transpose(1, 2).reshape(B * L, x.shape[1], D)  # noqa: E731
         q = flat(queries)
         if self.rotation:
@@ -624,16 +629,27 @@ class PagedLayer:
         else:
             b.append(self.index, flat(keys), flat(values))
         if L == 1:
-            if mask is not None:
-                raise ValueError("a single-token step takes no mask")
             sinks = None if sinks is None else sinks.detach().float().contiguous()
             return b.decode(self.index, q.contiguous(), scale, sinks=sinks).view(B, Hq, 1, D)
         q = q.view(B, L, Hq, D).transpose(1, 2)
         out = torch.empty_like(queries)
         for i in range(B):
             k, v = self.dense(i)
-            out[i] = _dense_attention(q[i:i + 1], k, v, scale, mask, sinks)[0]
+            out[i] = _dense_attention(q[i:i + 1], k, v, scale, masks[i], sinks)[0]
         return out
+
+    def _masks(self, mask, B: int, Hq: int, L: int) -> list:
+        """The mask of each sequence."""
+        if mask is None or isinstance(mask, str):
+            if mask not in (None, "causal"):
+                raise ValueError(f"unknown mask {mask!r}")
+            return [mask] * B
+        lengths = self.batch.host_lengths
+        shape = (B, Hq, L, max(lengths))
+        if not 2 <= mask.dim() <= 4 or any(n not in (1, m) for n, m in zip(reversed(mask.shape), reversed(shape))):
+            raise ValueError(f"mask must broadcast to {shape} (got {tuple(mask.shape)})")
+        mask = mask.expand(shape)
+        return [mask[i:i + 1, ..., :n] for i, n in enumerate(lengths)]
 
     def dense(self, i: int):
         """Keys and values of the batch's sequence i, [1, Hkv, tokens, D]."""

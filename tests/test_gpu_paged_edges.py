@@ -69,3 +69,38 @@ def test_router_without_a_mask_hides_nothing(cuda, mask, with_sinks):
         ref = attend64(q[b], k[b], v[b], 0.1, keep, sinks)
         close(out[b], ref)
         close(same[b], ref)
+
+
+@pytest.mark.parametrize("with_sinks", [False, True])
+@pytest.mark.parametrize("kind", ["bool", "add", "heads", "shared", "2d", "3d"])
+def test_router_takes_each_sequence_its_mask(cuda, kind, with_sinks):
+    """Masks with a batch dimension, for sequences of different lengths: column t is token t, and the columns past a
+    sequence's end are not its own."""
+    import torch
+    import sparse_decode as sd
+    lengths, L, B, hq = [70, 37, 51], 20, 3, 8
+    pool, seqs, rows, q, k, v = prompt(torch, lengths=lengths, new=L, seed=3)
+    g = gen(torch, 4)
+    T = max(lengths)
+    shape = {"shared": (1, 1, L, T), "heads": (B, hq, L, T), "2d": (L, T), "3d": (hq, L, T)}.get(kind, (B, 1, L, T))
+    mask = torch.rand(shape, generator=g, device="cuda") < 0.5
+    mask[..., 0] = True
+    if kind == "add":
+        mask = torch.where(mask, torch.randn(shape, generator=g, device="cuda"), -math.inf).bfloat16()
+    sinks = torch.randn(hq, generator=g, device="cuda") if with_sinks else None
+    out = sd.attention_with_cache_update(q, k, v, pool.extend(seqs, L).layer(0), 0.1, mask, sinks)
+    full = mask.expand(B, hq, L, T)
+    for b, n in enumerate(lengths):
+        close(out[b], attend64(q[b], rows[0][b], rows[1][b], 0.1, full[b][..., :n], sinks))
+
+
+def test_router_refuses_masks_that_do_not_fit(cuda):
+    import torch
+    import sparse_decode as sd
+    pool, seqs, rows, q, k, v = prompt(torch, lengths=[40, 30], new=10, seed=5)
+    layer = pool.extend(seqs, 10).layer(0)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bool, device="cuda")  # noqa: E731
+    for bad in (z(3, 1, 10, 40), z(2, 3, 10, 40), z(2, 1, 9, 40), z(2, 1, 10, 39), z(2, 1, 10, 41), z(10), z(1, 2, 1, 10, 40),
+                "full"):
+        with pytest.raises(ValueError):
+            sd.attention_with_cache_update(q, k, v, layer, 0.1, bad)
