@@ -619,8 +619,8 @@ class PagedLayer:
         B, Hq, L, D = queries.shape
         if any(n != L for n in b.new) or len(b.new) != B:
             raise ValueError(f"the step holds {b.new} new tokens, the queries {[L] * B}")
-        if L == 1 and mask is not None:
-            raise ValueError("a single-token step takes no mask")
+        if L == 1 and mask is not None and not isinstance(mask, str):
+            raise ValueError("a single-token step takes no mask but \"causal\", which hides nothing there")
         masks = self._masks(mask, B, Hq, L)
         flat = lambda x: x.transpose(1, 2).reshape(B * L, x.shape[1], D)  # noqa: E731
         q = flat(queries)

@@ -104,3 +104,17 @@ def test_router_refuses_masks_that_do_not_fit(cuda):
                 "full"):
         with pytest.raises(ValueError):
             sd.attention_with_cache_update(q, k, v, layer, 0.1, bad)
+
+
+def test_router_takes_causal_for_a_single_token(cuda):
+    """The newest token sees all of its sequence: "causal" hides nothing."""
+    import torch
+    import sparse_decode as sd
+    pool, seqs, rows, q, k, v = prompt(torch, lengths=[40, 30], new=1, seed=6)
+    layer = pool.extend(seqs, 1).layer(0)
+    a = sd.attention_with_cache_update(q, k, v, layer, 0.1, None)
+    b = sd.attention_with_cache_update(q, k, v, layer, 0.1, "causal")
+    assert torch.equal(a, b)
+    for bad in (torch.ones(2, 1, 1, 40, dtype=torch.bool, device="cuda"), "full"):
+        with pytest.raises(ValueError):
+            sd.attention_with_cache_update(q, k, v, layer, 0.1, bad)
