@@ -588,18 +588,21 @@ class PagedBatch:
         return paged_decode(q, self.pool.pages, self.tables, self.lengths, scale, layer=layer, flags=self.pool.flags,
                             **kw)
 
-    def layer(self, layer: int, **rotation) -> "PagedLayer":
+    def layer(self, layer: int, *, window: int = 0, **rotation) -> "PagedLayer":
         """Layer `layer` of this step as a cache for attention_with_cache_update;
-        `rotation`: the keyword arguments of `paged_append` that norm and rotate
-        queries and keys (none: they come in rotated)."""
-        return PagedLayer(self, layer, rotation)
+        `window`: each new token sees the last `window` tokens up to itself
+        (0: all); `rotation`: the keyword arguments of `paged_append` that norm
+        and rotate queries and keys (none: they come in rotated)."""
+        return PagedLayer(self, layer, rotation, window)
 
 
 class PagedLayer:
     """What attention_with_cache_update needs of a paged step's layer."""
 
-    def __init__(self, batch: PagedBatch, layer: int, rotation: dict):
-        self.batch, self.index, self.rotation = batch, layer, rotation
+    def __init__(self, batch: PagedBatch, layer: int, rotation: dict, window: int = 0):
+        if window < 0:
+            raise ValueError("window must not be negative")
+        self.batch, self.index, self.rotation, self.window = batch, layer, rotation, window
 
     @property
     def offset(self):
@@ -613,7 +616,8 @@ class PagedLayer:
         `mask` as for the other caches: None hides nothing, "causal" the tokens
         after each one; a tensor (bool, or numbers to add) is broadcast to
         [B, Hq, L, T], T the longest sequence's tokens, and column t is token t
-        of every sequence."""
+        of every sequence. A layer with a window takes several tokens with
+        "causal" only."""
         from .cache import _dense_attention
         b = self.batch
         B, Hq, L, D = queries.shape
@@ -630,7 +634,7 @@ class PagedLayer:
             b.append(self.index, flat(keys), flat(values))
         if L == 1:
             sinks = None if sinks is None else sinks.detach().float().contiguous()
-            return b.decode(self.index, q.contiguous(), scale, sinks=sinks).view(B, Hq, 1, D)
+            return b.decode(self.index, q.contiguous(), scale, window=self.window, sinks=sinks).view(B, Hq, 1, D)
         q = q.view(B, L, Hq, D).transpose(1, 2)
         out = torch.empty_like(queries)
         for i in range(B):
@@ -640,11 +644,18 @@ class PagedLayer:
 
     def _masks(self, mask, B: int, Hq: int, L: int) -> list:
         """The mask of each sequence."""
+        lengths = self.batch.host_lengths
         if mask is None or isinstance(mask, str):
             if mask not in (None, "causal"):
                 raise ValueError(f"unknown mask {mask!r}")
-            return [mask] * B
-        lengths = self.batch.host_lengths
+            if not self.window or L == 1:  # a single token's window is the kernel's
+                return [mask] * B
+        if self.window and not isinstance(mask, str):
+            raise ValueError("a layer with a window takes several tokens with mask \"causal\"")
+        if self.window:
+            dev = self.batch.tables.device
+            back = [torch.arange(n - L, n, device=dev)[:, None] - torch.arange(n, device=dev) for n in lengths]
+            return [(x >= 0) & (x < self.window) for x in back]
         shape = (B, Hq, L, max(lengths))
         if not 2 <= mask.dim() <= 4 or any(n not in (1, m) for n, m in zip(reversed(mask.shape), reversed(shape))):
             raise ValueError(f"mask must broadcast to {shape} (got {tuple(mask.shape)})")

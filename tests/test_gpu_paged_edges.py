@@ -118,3 +118,27 @@ def test_router_takes_causal_for_a_single_token(cuda):
     for bad in (torch.ones(2, 1, 1, 40, dtype=torch.bool, device="cuda"), "full"):
         with pytest.raises(ValueError):
             sd.attention_with_cache_update(q, k, v, layer, 0.1, bad)
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("window", [1, 7, 16, 30, 1000])
+def test_router_windows(cuda, window, new, bits):
+    """A layer with a window: every token sees the last `window` tokens up to itself, whichever path its step takes."""
+    import torch
+    import sparse_decode as sd
+    lengths = [70, 37, 20]
+    pool, seqs, rows, q, k, v = prompt(torch, bits, lengths, new, seed=7)
+    step = pool.extend(seqs, new)
+    sinks = torch.randn(8, generator=gen(torch, 8), device="cuda")
+    out = sd.attention_with_cache_update(q, k, v, step.layer(0, window=window), 0.1, "causal", sinks)
+    for b, n in enumerate(lengths):
+        kk, vv = step.layer(0).dense(b)
+        back = torch.arange(n - new, n, device="cuda")[:, None] - torch.arange(n, device="cuda")
+        close(out[b], attend64(q[b], kk[0], vv[0], 0.1, (back >= 0) & (back < window), sinks))
+    if new > 1:  # a window and another mask than "causal" say two things
+        for mask in (None, torch.ones(new, 70, dtype=torch.bool, device="cuda")):
+            with pytest.raises(ValueError):
+                sd.attention_with_cache_update(q, k, v, step.layer(0, window=window), 0.1, mask)
+    with pytest.raises(ValueError):
+        step.layer(0, window=-1)
