@@ -31,7 +31,8 @@
 //
 // The running maximum m is a lower bound of the true one by at most kSlack
 // (log2 units): it moves, and l and o are rescaled, only when a score passes
-// m + kSlack, which one vote per tile finds; p stays below 2^kSlack.
+// m + kSlack, which one vote per tile finds; p stays below 2^kSlack (for dense
+// fp16 m stands lower still, see there).
 #pragma once
 
 #include "sd_device.cuh"
@@ -133,12 +134,17 @@ __device__ __forceinline__ float raise_max(float& m, float mx) {
 // of a head lies where its outputs are. P^T gets its operand layout from
 // movmatrix. p is used as hi + lo halves of the element type (about 16 bits
 // of it for bf16): a single bf16 p would cost as much accuracy as the final
-// rounding does, and the extra mma is free next to the loads.
+// rounding does, and the extra mma is free next to the loads. fp16 has no
+// halves below 2^-24, so there m stands 2^kUp below the maximum: p goes up to
+// 2^(kUp + kSlack) = 2^15, and a weight keeps its bits down to 2^-(24 + kUp) of
+// the maximum's. At a kUp of 0 the many small weights beside an attention sink
+// (each below 2^-25) were lost to o, though not to l.
 // ---------------------------------------------------------------------------
 template <typename E, int D, int NB>
 struct DenseAttend {
   using F = PagedFmt<2, 0, D>;
   static constexpr int NC = D / 16;
+  static constexpr float kUp = __is_same(E, __half) ? 7.0f : 0.0f;
   uint32_t qb[NB][NC][2];
   float m[NB][2], l[NB][2], o[NB][NC][4];
 
@@ -190,7 +196,7 @@ struct DenseAttend {
       for (int i = 0; i < 4; ++i) {
         const float v = (acc[0][nb][i] + acc[1][nb][i]) * p.scale_log2;
         s[nb][i] = (i < 2 ? ok0 : ok1) ? v : -INFINITY;
-        up |= s[nb][i] > m[nb][i & 1] + kSlack;
+        up |= s[nb][i] > m[nb][i & 1] + (kSlack + kUp);
       }
     }
     if (__any_sync(0xffffffffu, up)) {
@@ -202,7 +208,7 @@ struct DenseAttend {
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float f = raise_max(m[nb][e], mx);
+          const float f = raise_max(m[nb][e], mx - kUp);
           l[nb][e] *= f;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {

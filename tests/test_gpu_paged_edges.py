@@ -16,6 +16,45 @@ pytestmark = pytest.mark.gpu
 
 
 # ---------------------------------------------------------------------------
+# decode: accuracy
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_decode_keeps_weights_far_below_the_largest(cuda, d, dtype):
+    """One token of each sequence has nearly all the weight and a value of zero, as an attention sink has, so that the
+    output is what the 16383 others add up to, each with a weight of e^-17.5 .. e^-19.5 of the largest. 300 sequences
+    over the same pages: segments of a whole sequence.
+
+    Bound: a weight of at most 2^8 times the running maximum's is held as two halves of the element type. In fp16 they
+    reach down to half of 2^-24 at a scale of 2^7: 2^-32 of the maximum's weight at most for each token. bf16's two
+    halves lose 2^-16 of a weight; the weights and their sums in fp32 2^-20 of them, and the
+    rounding of the output, or of a subnormal one."""
+    import torch
+    import sparse_decode as sd
+    dt, g = tdt(torch, dtype), gen(torch, d)
+    B, page, n = 300, 256, 16384
+    k = torch.zeros(n // page, 1, page, d, device="cuda")
+    score = -17.5 - 2 * torch.rand(n, generator=g, device="cuda")
+    score[9000] = 0.0
+    k[..., 0] = score.view(n // page, 1, page)
+    v = torch.rand(n, d, generator=g, device="cuda") + 0.5
+    v[9000] = 0.0
+    k, v = k.to(dt), v.view(n // page, page, d)[:, None].to(dt).contiguous()
+    q = torch.zeros(B, 1, d, device="cuda", dtype=dt)
+    q[..., 0] = 1.0
+    tables = torch.arange(n // page, dtype=torch.int32, device="cuda").repeat(B, 1)
+    out = sd.paged_decode(q, sd.KVPages(k, v), tables, torch.full((B,), n, dtype=torch.int32, device="cuda"), 1.0)
+    p = torch.softmax(k[..., 0].double().flatten(), 0)
+    ref = p @ v.double().view(n, d)
+    each = {"f16": n * 2.0 ** -32 * 1.5, "bf16": 0.0}[dtype]
+    rel = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8 + 2.0 ** -16}[dtype] + 2.0 ** -20 + 2.0 ** -22
+    bound = each + rel * ref + (2.0 ** -25 if dtype == "f16" else 0.0)
+    worst = ((out[:, 0].double() - ref).abs() / bound).max()
+    assert float(worst) <= 1.0, float(worst)
+
+
+# ---------------------------------------------------------------------------
 # the router
 # ---------------------------------------------------------------------------
 
