@@ -24,7 +24,7 @@
 // tiles, whose M of 64 or more would be mostly padding. Measured, 32 query and
 // 8 kv heads of 128, inputs beyond L2: 16 ragged bf16 sequences of up to 128K
 // tokens (4.2 GB) 609 us, 6.9 TB/s; 4 x 128K in 8 bits (1.1 GB) 182 us, 6.3
-// TB/s; the same in 4 bits (0.6 GB) 148 us, 4.1 TB/s, bound by instructions; 4
+// TB/s; the same in 4 bits (0.6 GB) 152 us, 4.0 TB/s, bound by instructions; 4
 // x 32K in fp32 (1.1 GB) 175 us, 6.1 TB/s; one bf16 sequence of 32K (134 MB)
 // 27 us, of which 20 are the bytes and the rest start (first tile 3 us after
 // the launch) and merge (2.5 us).
@@ -321,12 +321,16 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 // What bounds this path is instructions as much as bytes, so the conversion is
 // short: one byte permute (or mask) puts codes into the mantissas of 1024 + c,
 // or 1024 + 16 c for the nibbles that lie 4 bits higher.
-//   q.k = s_k (q.c) + b_k sum(q)  per 64-dim group, in fp32. For bf16 pools
-// the offset is left in: the accumulator starts at -1024 sum(q') (q' = q in
-// fp16, a 16th of it where the nibble's place counts 16), which costs 3 to 4
-// of fp32's bits over the 64 products of a group, scores off by some 3e-4 --
-// nothing next to bf16's rounding, but a good half of fp16's, so other pools
-// subtract it. fp32 pools take q as hi + lo halves, 22 bits.
+//   q.k = s_k (q.c) + b_k sum(q)  per 64-dim group, in fp32. bf16 pools leave
+// the offset in where it is at most four times the codes' range -- 1024 for 8
+// bits, 1024 / 16 = 64 for a nibble whose place counts 16: the accumulator
+// starts at -1024 sum(q') (q' = q in fp16, a 16th of it at those places). That
+// costs fp32 3 bits at most; a score is off by at most 2^-20 (four mma, two
+// units of the largest partial sum each) of scale s_k sum((c + offset) |q|) per
+// group. The low nibble's 1024 would be 68 times the range, 6 bits, and scores
+// of wide keys (a range of 240) under queries of one sign off by up to 3e-2, so
+// it is subtracted there (4 x 128K tokens 148.6 -> 151.6 us), as it is in fp16
+// and fp32 pools throughout. fp32 pools take q as hi + lo halves, 22 bits.
 //   p.v = (p s_v).(c - z) + sum_t p (b_v + z s_v), z = the middle code. These
 // sums run over a whole segment, so their codes are centred by one packed
 // subtraction: no offset to cancel, and terms of both signs.
@@ -346,7 +350,7 @@ struct CodesAttend {
   // Two blocks of heads take their tokens 16 at a time: with 32 they spilled (register limit 168).
   static constexpr int MT = NB == 1 ? F::kTile / kPagedWarps / 16 : 1, PARTS = F::kTile / kPagedWarps / 16 / MT;
   static constexpr float MID = BITS == 8 ? 128.0f : 8.0f;
-  static constexpr bool kOffset = __is_same(E, __nv_bfloat16);
+  static constexpr bool kOffset = __is_same(E, __nv_bfloat16), kOffsetLow = kOffset && BITS == 8;
   static constexpr int QT = sizeof(E) == 4 ? 2 : 1;  // fp16 terms of q
   uint32_t qb[QT][NB][NK][2];
   float qs[NB][2][NG], qoff[NB][2][NG], m[NB][2], l[NB][2], o[NB][NK][4], ob[NB][2][NG];
@@ -423,9 +427,11 @@ struct CodesAttend {
               split2<__half>(x[j][0], x[j][1], qb[0][nb][KPC * c + i][j], qb[QT - 1][nb][KPC * c + i][j]);
             } else {
               qb[0][nb][KPC * c + i][j] = pack2<__half>(x[j][0], x[j][1]);
-              float g2[2];
-              unpack_word<__half>(qb[0][nb][KPC * c + i][j], g2);
-              off[r] += g2[0] + g2[1];
+              if (BITS == 8 || j == 1) {
+                float g2[2];
+                unpack_word<__half>(qb[0][nb][KPC * c + i][j], g2);
+                off[r] += g2[0] + g2[1];
+              }
             }
           }
         }
@@ -502,10 +508,8 @@ struct CodesAttend {
               f0 = raw_u4(x0 >> (8 * i), 0, magic), f1 = raw_u4(x1 >> (8 * i), 0, magic);
               f2 = raw_u4(x0 >> (8 * i), 1, magic), f3 = raw_u4(x1 >> (8 * i), 1, magic);
             }
-            if constexpr (!kOffset) {
-              f0 = sub_f16x2(f0, 0x64006400u), f1 = sub_f16x2(f1, 0x64006400u);
-              f2 = sub_f16x2(f2, 0x64006400u), f3 = sub_f16x2(f3, 0x64006400u);
-            }
+            if constexpr (!kOffsetLow) f0 = sub_f16x2(f0, 0x64006400u), f1 = sub_f16x2(f1, 0x64006400u);
+            if constexpr (!kOffset) f2 = sub_f16x2(f2, 0x64006400u), f3 = sub_f16x2(f3, 0x64006400u);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll

@@ -54,6 +54,56 @@ def test_decode_keeps_weights_far_below_the_largest(cuda, d, dtype):
     assert float(worst) <= 1.0, float(worst)
 
 
+@pytest.mark.parametrize("dtype,bits", [("bf16", 4), ("bf16", 8), ("f16", 4), ("f32", 4)])
+@pytest.mark.parametrize("dims", ["even", "odd", "all"])
+def test_decode_ties_of_wide_keys_and_queries_of_one_sign(cuda, dtype, bits, dims):
+    """Two tokens per sequence with the same score to all digits: the second one's codes are the first one's in another
+    order, between dims where the query is the same. Their values are +1 and -1, so the output is tanh of half the
+    difference that rounding makes between the scores, and 0 without it.
+
+    Bound, for a group of 64 dims: four mma steps, each off by at most two units (2^-23) of the largest partial sum A,
+    which is sum(c |q|) plus what is left in of the offset that makes codes fp16 numbers: 1024 |q| for 8-bit codes of
+    bf16 pools, 64 |q| for the odd dims of 4-bit ones, none for other pools; in fp32 pools q is cut to two halves, 2^-22
+    of sum(c |q|) more. Times scale and the key's scale for either token; the difference is halved by the mean and
+    doubled by there being two. Then four fp32 operations on the score and its bias part, for either token."""
+    import torch
+    import sparse_decode as sd
+    dt, g = tdt(torch, dtype), gen(torch, bits)
+    B, hkv, G, d, page, top = 256, 2, 4, 128, 16, (1 << bits) - 1
+    each = 2.0 ** (7 * torch.rand(B, hkv, 1, 2, 16, generator=g, device="cuda") - 3)
+    each[..., 1::2] *= dims != "even"
+    each[..., 0::2] *= dims != "odd"
+    f = 1 + torch.rand(B, hkv, G, 1, 1, generator=g, device="cuda")  # another query for each head
+    q = (each * f).to(dt)[..., None, :].expand(B, hkv, G, 2, 4, 16).reshape(B, hkv * G, d).contiguous()
+    one = torch.randint(0, top + 1, (B, hkv, 2, 4, 16), generator=g, device="cuda")
+    other = one.gather(3, torch.rand(one.shape, generator=g, device="cuda").argsort(3))
+    codes = torch.zeros(B, hkv, page, d, dtype=torch.int64, device="cuda")
+    codes[:, :, 0], codes[:, :, 1] = one.flatten(2), other.flatten(2)
+    per = 32 // bits
+    words = (codes.unflatten(-1, (-1, per)) << (torch.arange(per, device="cuda") * bits)).sum(-1)
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    s, b = 240.0 / top, -100.0
+    small = torch.full((B, hkv, page, d // 64), s, device="cuda").to(dt)
+    s = float(small[0, 0, 0, 0])
+    vb = torch.zeros_like(small)
+    vb[:, :, 0], vb[:, :, 1] = 1.0, -1.0
+    pages = sd.KVPages(words, torch.zeros_like(words), small, torch.full_like(small, b), torch.ones_like(small), vb,
+                       bits=bits)
+    tables = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+    scale = d ** -0.5
+    out = sd.paged_decode(q, pages, tables, torch.full((B,), 2, dtype=torch.int32, device="cuda"), scale)
+    x = q.double().view(B, hkv, G, d).abs()
+    c = torch.maximum(codes[:, :, 0], codes[:, :, 1]).double()[:, :, None]
+    cq = (x * c).sum(-1)
+    left = {("bf16", 8): 1024 * x.sum(-1), ("bf16", 4): 64 * x[..., 1::2].sum(-1)}.get((dtype, bits), 0.0)
+    bound = 4 * 2 * 2.0 ** -23 * (cq + left) * s * scale
+    if dtype == "f32":
+        bound = bound + 2.0 ** -22 * cq * s * scale
+    bound = bound + 2 * 4 * 2.0 ** -24 * scale * (s * cq + abs(b) * x.sum(-1)) + 1e-6
+    worst = (out.double().view(B, hkv, G, d).abs().amax(-1) / bound).max()
+    assert float(worst) <= 1.0, float(worst)
+
+
 # ---------------------------------------------------------------------------
 # the router
 # ---------------------------------------------------------------------------
