@@ -120,6 +120,15 @@ def _out(x, out, name: str, dtype, dev: int, dim: int, stream) -> tuple:
     return out, SDRows(out.data_ptr(), st[0], st[2], st[1])
 
 
+def _upload(host, stream):
+    """Pinned host tensor -> device, queued on `stream` (None: the current one) without waiting; the allocator keeps
+    the host memory until it is copied. A graph would read it again at every replay, when it holds something else."""
+    with torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("host lists cannot be copied in a captured graph: pass device tensors")
+        return host.to("cuda", non_blocking=True)
+
+
 def _handle(stream, dev: int) -> int:
     return _raw_stream(dev) if stream is None else stream.cuda_stream
 
@@ -381,8 +390,7 @@ def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
             raise ValueError("page out of range")
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             raise ValueError("dst pages must be distinct and none of them a src")
-        with torch.cuda.stream(stream):  # None: the current one
-            both = torch.tensor([src, dst], dtype=_I32).to(dev)
+        both = _upload(torch.tensor([src, dst], dtype=_I32, pin_memory=True), stream)
         src, dst = both[0], both[1]
     if src.dim() != 1:
         raise ValueError("src and dst must be [n]")

@@ -231,3 +231,44 @@ def test_router_windows(cuda, window, new, bits):
                 sd.attention_with_cache_update(q, k, v, step.layer(0, window=window), 0.1, mask)
     with pytest.raises(ValueError):
         step.layer(0, window=-1)
+
+
+# ---------------------------------------------------------------------------
+# steps
+# ---------------------------------------------------------------------------
+
+def test_page_copies_of_a_step_do_not_stop_the_host(cuda):
+    """Copy-on-write, compaction and copies of host lists are queued like the rest of a step."""
+    import torch
+    import sparse_decode as sd
+    pool = sd.PagePool(2, 12, 2, 64, 16)
+    a = pool.add()
+    step = pool.extend([a], 40)
+    x = torch.randn(40, 2, 64, device="cuda").bfloat16()
+    for layer in range(2):
+        step.append(layer, x, -x)
+    b = pool.fork(a)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        step = pool.extend([b], 1)                 # leaves the shared page
+        sd.copy_pages(pool.pages, [0, 1], [10, 11])
+        pool.free(a)
+        assert pool.compact() == 1
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    k, v = pool.batch([b]).layer(1).dense(0)
+    assert torch.equal(k[0, :, :40], x.transpose(0, 1)) and torch.equal(v[0, :, :40], -x.transpose(0, 1))
+    assert torch.equal(pool.pages.k[:, 10:], pool.pages.k[:, :2])
+
+
+def test_host_lists_are_refused_in_a_captured_graph(cuda):
+    """A replay would copy whatever the host memory holds by then."""
+    import torch
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 12, 2, 64, 16)
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            sd.copy_pages(pool.pages, [0], [1])
+    torch.cuda.synchronize()
+    sd.copy_pages(pool.pages, [0], [1])
