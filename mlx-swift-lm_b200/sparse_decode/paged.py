@@ -120,12 +120,17 @@ def _out(x, out, name: str, dtype, dev: int, dim: int, stream) -> tuple:
     return out, SDRows(out.data_ptr(), st[0], st[2], st[1])
 
 
+def _refuse_capture(stream) -> None:
+    with torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("host lists and tables cannot be copied in a captured graph")
+
+
 def _upload(host, stream):
     """Pinned host tensor -> device, queued on `stream` (None: the current one) without waiting; the allocator keeps
     the host memory until it is copied. A graph would read it again at every replay, when it holds something else."""
+    _refuse_capture(stream)
     with torch.cuda.stream(stream):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("host lists cannot be copied in a captured graph: pass device tensors")
         return host.to("cuda", non_blocking=True)
 
 
@@ -506,6 +511,7 @@ class PagePool:
     def compact(self, stream=None) -> int:
         """Move pages so that the used ones are the lowest; returns how many
         moved. Batches made before are stale afterwards."""
+        _refuse_capture(stream)
         n = ctypes.c_int32()
         room = self.pages.n_pages // 2
         src, dst = (ctypes.c_int32 * max(room, 1))(), (ctypes.c_int32 * max(room, 1))()
@@ -526,6 +532,7 @@ class PagePool:
             raise ValueError("n_tokens must be an int or one per sequence")
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence may be named once per batch")
+        _refuse_capture(stream)
         src, dst, n = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
         copies, grown = [], []
         try:
@@ -578,8 +585,7 @@ class PagedBatch:
         pos = [p for t, k in zip(lengths, new) for p in range(t - k, t)]
         seq = [b for b, k in enumerate(new) for _ in range(k)]
         host[n * w + n:] = torch.tensor(pos + seq, dtype=torch.int32)
-        with torch.cuda.stream(stream):  # None: the current one
-            dev = host.to("cuda", non_blocking=True)
+        dev = _upload(host, stream)
         self.tables = dev[:n * w].view(n, w)
         self.lengths = dev[n * w:n * w + n]
         self.positions = dev[n * w + n:n * w + n + tokens]

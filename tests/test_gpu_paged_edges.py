@@ -272,3 +272,18 @@ def test_host_lists_are_refused_in_a_captured_graph(cuda):
             sd.copy_pages(pool.pages, [0], [1])
     torch.cuda.synchronize()
     sd.copy_pages(pool.pages, [0], [1])
+
+
+def test_a_step_cannot_be_made_in_a_captured_graph(cuda):
+    """Its tables come from the host; the step's calls are what a graph may hold. No sequence grows."""
+    import torch
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 12, 2, 64, 16)
+    a = pool.add()
+    pool.extend([a], 5)
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            pool.extend([a], 1)
+    torch.cuda.synchronize()
+    assert pool.length(a) == 5
+    assert pool.batch([a]).lengths.tolist() == [5]
