@@ -524,14 +524,16 @@ class PagePool:
     def extend(self, seqs: Sequence[int], n_tokens, stream=None) -> "PagedBatch":
         """Make room for n_tokens (an int, or one per sequence) more tokens of
         each sequence and return the batch that appends them. All or nothing:
-        when the pool has too few free pages, no sequence grows. Page copies
-        and the batch's tables are issued on `stream`, on which the step's
-        calls must then run or wait."""
+        when the pool has too few free pages, or anything else is refused, no
+        sequence grows. Page copies and the batch's tables are issued on
+        `stream`, on which the step's calls must then run or wait."""
         each = [int(n_tokens)] * len(seqs) if isinstance(n_tokens, int) else [int(n) for n in n_tokens]
         if len(each) != len(seqs):
             raise ValueError("n_tokens must be an int or one per sequence")
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence may be named once per batch")
+        if any(not -(1 << 63) <= i < 1 << 63 for i in [*seqs, *each]):  # what ctypes would keep the low bits of
+            raise ValueError("a sequence or its number of tokens does not fit 64 bits")
         _refuse_capture(stream)
         src, dst, n = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
         copies, grown = [], []
@@ -541,16 +543,18 @@ class PagePool:
                 grown.append((s, k))
                 if n.value:
                     copies.append((src.value, dst.value))
-        except SDError:
-            # the pages already copied-on-write stay with their sequences, so their contents must follow
-            if copies:
-                copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
-            for s, k in grown:
-                self.trim(s, k)
+            batch = PagedBatch(self, list(seqs), each, stream)
+        except BaseException:
+            try:  # the pages already copied-on-write stay with their sequences, so their contents must follow
+                if copies:
+                    copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
+            finally:
+                for s, k in grown:
+                    self.trim(s, k)
             raise
         if copies:
             copy_pages(self.pages, *zip(*copies), flags=self.flags, stream=stream)
-        return PagedBatch(self, list(seqs), each, stream)
+        return batch
 
     def batch(self, seqs: Sequence[int], stream=None) -> "PagedBatch":
         """The sequences as they are, with no new tokens."""

@@ -287,3 +287,15 @@ def test_a_step_cannot_be_made_in_a_captured_graph(cuda):
     torch.cuda.synchronize()
     assert pool.length(a) == 5
     assert pool.batch([a]).lengths.tolist() == [5]
+
+
+@pytest.mark.parametrize("bad", [([0, "x"], 3), ([0, 1], [3, "x"]), ([0, 1], [3, 1 << 70]), ([0, 1 << 70], 3), ([0, 9], 3)])
+def test_a_step_that_fails_leaves_every_sequence_as_it_was(cuda, bad):
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 12, 2, 64, 16)
+    a, b = pool.add(), pool.add()
+    assert (a, b) == (0, 1)
+    pool.extend([a, b], 5)
+    with pytest.raises(Exception):
+        pool.extend(*bad)
+    assert (pool.length(a), pool.length(b)) == (5, 5)
