@@ -190,7 +190,7 @@ __host__ __device__ constexpr int rotary_pitch(int rot2) { return (rot2 + 7) / 8
 
 // vec: elements per access (1, 2, 4, and 8 for 16-bit types); wide: head_dim
 // above 128; shifted: rotated halves that are no whole number of accesses (vec
-// 4 and 8).
+// is 4 then).
 const void* rotary_kernel_for(int dtype, int bits, int vec, bool wide, bool shifted, bool traditional);
 
 struct CopyParams {

@@ -396,7 +396,7 @@ static const void* rotary_entry(bool trad) {
 template <typename E, int BITS>
 static const void* rotary_pick(int vec, bool wide, bool shifted, bool trad) {
   if constexpr (sizeof(E) == 2)
-    if (vec == 8) return shifted ? reinterpret_cast<const void*>(&rotary_kernel<E, 8, 1, BITS, kShifted>) : rotary_entry<E, 8, 1, BITS>(trad);
+    if (vec == 8) return rotary_entry<E, 8, 1, BITS>(trad);
   if (vec == 4) return shifted ? reinterpret_cast<const void*>(&rotary_kernel<E, 4, 1, BITS, kShifted>) : rotary_entry<E, 4, 1, BITS>(trad);
   if constexpr (BITS == 0) {  // quantized pools have head_dim 64 and 128
     if (wide) return vec == 2 ? rotary_entry<E, 2, 2, BITS>(trad) : rotary_entry<E, 1, 4, BITS>(trad);
