@@ -20,6 +20,7 @@ import math
 from typing import Optional
 
 from . import SparseIndex, _torch_dtype
+from .paged import PagedLayer
 
 
 class SparseKVCache:
@@ -262,7 +263,6 @@ def attention_with_cache_update(queries, keys, values, cache, scale: float, mask
     MiMoV2Flash.swift:14-56). queries [B, Hq, L, D]; keys/values
     [B, Hkv, L, D]; sinks [Hq] or None. Returns [B, Hq, L, D]. `cache`: None, a
     SparseKVCache, or a layer of a paged step (PagedBatch.layer)."""
-    from .paged import PagedLayer
     if cache is None:
         return _dense_attention(queries, keys, values, scale, mask, sinks)
     if isinstance(cache, SparseKVCache):

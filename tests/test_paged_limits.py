@@ -112,3 +112,17 @@ def test_calls_refuse_layers_and_windows_past_32_bits(cuda):
                 lambda: sdp.paged_append(p, k, k, t, n - 1, layer=far)):
         with pytest.raises(ValueError):
             bad()
+
+
+# -- the router -------------------------------------------------------------------
+
+def test_router_looks_up_nothing_per_call(monkeypatch):
+    """A layer's call takes microseconds: the router's import of the paged layers is made once, not in each of them."""
+    import sys
+
+    import torch
+    monkeypatch.setitem(sys.modules, "sparse_decode.paged", None)  # an import now fails
+    x = torch.randn(1, 2, 3, 64)
+    assert sdp.attention_with_cache_update(x, x, x, None, 0.1).shape == x.shape
+    with pytest.raises(TypeError):
+        sdp.attention_with_cache_update(x, x, x, object(), 0.1)
