@@ -446,6 +446,19 @@ __device__ __forceinline__ void consume_tiles_mma(const DecodeParams& p, const T
 // ldmatrix.trans, and p' = p * s_v (per token and group, as hi + lo fp16) is
 // the A operand; the bias part sum_t p * b_v is accumulated on the side. q is scaled by 2^-eq
 // so that its fp16 form cannot overflow; eq is undone on the product.
+__device__ __forceinline__ uint32_t code_pair_u8(uint32_t r, uint32_t sel) {
+  const uint32_t h = __byte_perm(r, 0x6464u, sel);  // fp16 1024 + c in each half
+  uint32_t out;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(out) : "r"(h), "r"(0x64006400u));
+  return out;
+}
+__device__ __forceinline__ uint32_t code_pair_u4(uint32_t r, int j) {
+  const uint32_t h = ((r >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
+  uint32_t out;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(out) : "r"(h), "r"(0x64006400u));
+  return out;
+}
+
 template <typename E, int BITS, int D, int G>
 __device__ __forceinline__ void consume_tiles_qmma(const DecodeParams& p, const TileWalk& tw, const E* qg,
                                                    const float* qs, int warp, int lane) {

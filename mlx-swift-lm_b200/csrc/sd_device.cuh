@@ -443,21 +443,6 @@ template <typename E> __device__ __forceinline__ void split2(float x, float y, u
   unpack_word<E>(hi, hx);
   lo = pack2<E>(x - hx[0], y - hx[1]);
 }
-// Two 8-bit (4-bit) codes of r as an exact fp16 pair: a byte permute (shift and
-// mask) puts each code c in the mantissa of 1024 + c, and a packed subtraction
-// leaves c.
-__device__ __forceinline__ uint32_t code_pair_u8(uint32_t r, uint32_t sel) {
-  const uint32_t h = __byte_perm(r, 0x6464u, sel);  // fp16 1024 + c in each half
-  uint32_t out;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(out) : "r"(h), "r"(0x64006400u));
-  return out;
-}
-__device__ __forceinline__ uint32_t code_pair_u4(uint32_t r, int j) {
-  const uint32_t h = ((r >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
-  uint32_t out;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(out) : "r"(h), "r"(0x64006400u));
-  return out;
-}
 __device__ __forceinline__ void named_barrier(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
