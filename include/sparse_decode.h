@@ -352,7 +352,9 @@ int32_t sd_copy_pages(const sd_pages* pages, const int32_t* src, const int32_t* 
  * head: 1 .. 16; 65536 at most in all. Lengths and tables are read on the device only. The
  * workspace (sd_paged_workspace bytes -- they depend on n_q_heads, the pool and
  * the GPU, not on the batch -- 16-byte aligned, contents do not matter) must
- * not be shared by calls that may overlap. Pages past a
+ * not be shared by calls that may overlap. Equal calls give equal bits; a
+ * sequence's last bits may differ where the other lengths of its batch do, as
+ * they say where the work is cut. Pages past a
  * sequence's length, or before its window, are not read. An index or length
  * out of range sets bit 2 of *device_flags; rows of such a page read as 0. */
 int32_t sd_paged_workspace(const sd_pages* pages, int32_t batch, int32_t n_q_heads, int64_t* bytes);

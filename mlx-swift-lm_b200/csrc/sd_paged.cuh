@@ -16,18 +16,20 @@
 // between warps until a segment (the CTA's share of one pair) ends. A segment
 // that is a whole pair is written out; the others leave (m, l, o) in the
 // workspace and paged_merge_kernel joins them in CTA order, so results do not
-// depend on timing. The lengths are read on the device only, so a captured
-// graph serves growing sequences.
+// depend on timing (the last bits of a sequence do depend on the other lengths
+// of the batch, which say where it is cut). The lengths are read on the device
+// only, so a captured graph serves growing sequences.
 //
 // The products have at most 16 query heads on one side, so they run on
 // register-level mma (16-bit rows and codes) or FMA (fp32), not on tcgen05
 // tiles, whose M of 64 or more would be mostly padding. Measured, 32 query and
 // 8 kv heads of 128, inputs beyond L2: 16 ragged bf16 sequences of up to 128K
 // tokens (4.2 GB) 609 us, 6.9 TB/s; 4 x 128K in 8 bits (1.1 GB) 182 us, 6.3
-// TB/s; the same in 4 bits (0.6 GB) 152 us, 4.0 TB/s, bound by instructions; 4
-// x 32K in fp32 (1.1 GB) 175 us, 6.1 TB/s; one bf16 sequence of 32K (134 MB)
-// 27 us, of which 20 are the bytes and the rest start (first tile 3 us after
-// the launch) and merge (2.5 us).
+// TB/s; the same in 4 bits (0.6 GB) 152 us, 4.0 TB/s, bound by the latency of a
+// tile's chain of instructions (56% of the issue slots used); 4 x 32K in fp32
+// (1.1 GB) 175 us, 6.1 TB/s; one bf16 sequence of 32K (134 MB) 27 us, of which
+// 20 are the bytes and the rest start (first tile 3 us after the launch) and
+// merge (2.5 us).
 //
 // The running maximum m is a lower bound of the true one by at most kSlack
 // (log2 units): it moves, and l and o are rescaled, only when a score passes
@@ -318,8 +320,8 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 
 // ---------------------------------------------------------------------------
 // 4/8-bit codes, the same products, with the codes as exact fp16 integers.
-// What bounds this path is instructions as much as bytes, so the conversion is
-// short: one byte permute (or mask) puts codes into the mantissas of 1024 + c,
+// The chain of instructions bounds this path as much as bytes do, so the
+// conversion is short: one byte permute (or mask) puts codes into the mantissas of 1024 + c,
 // or 1024 + 16 c for the nibbles that lie 4 bits higher.
 //   q.k = s_k (q.c) + b_k sum(q)  per 64-dim group, in fp32. bf16 pools leave
 // the offset in where it is at most four times the codes' range -- 1024 for 8
@@ -338,16 +340,19 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 // [2^13, 2^14): bf16 values then keep all their bits in fp16 down to 2^-27 of
 // the largest. p s_v is scaled per group by a power of two kept across tiles
 // (vinv) so that the largest |s_v| so far maps below 2^7 (with p up to
-// 2^kSlack, p s_v stays below 2^15): values of any magnitude neither overflow nor sink into fp16's subnormals, and split into
-// hi + lo halves (22 bits). One half alone was 13 bf16 ulp off where the terms
-// of an output nearly cancel, and no faster.
+// 2^kSlack, p s_v stays below 2^15) and at 2^3 or above: scales of
+// any magnitude neither overflow nor sink into fp16's subnormals. Split into hi
+// + lo halves, a p s_v has 22 bits down to 2^-5 of the largest |s_v|, and below
+// that an error of at most 2^-28 of it. One half alone was 13 bf16 ulp off where
+// the terms of an output nearly cancel, and no faster.
 // ---------------------------------------------------------------------------
 template <typename E, int BITS, int D, int NB>
 struct CodesAttend {
   using F = PagedFmt<sizeof(E), BITS, D>;
   static constexpr int NK = D / 16, NG = F::kGroups, NCH = F::kNChunk;
   static constexpr int KPC = NK / NCH;   // k-steps (and 16-dim output tiles) per 16-byte chunk: 1 or 2
-  // Two blocks of heads take their tokens 16 at a time: with 32 they spilled (register limit 168).
+  // Two blocks of heads take their tokens 16 at a time: with 32 they spill more at the register limit of 168 (heads of
+  // 128 still do: bf16 176 bytes stored and 216 loaded), 4 x 128K in 8 bits 349 -> 303 us.
   static constexpr int MT = NB == 1 ? F::kTile / kPagedWarps / 16 : 1, PARTS = F::kTile / kPagedWarps / 16 / MT;
   static constexpr float MID = BITS == 8 ? 128.0f : 8.0f;
   static constexpr bool kOffset = __is_same(E, __nv_bfloat16), kOffsetLow = kOffset && BITS == 8;

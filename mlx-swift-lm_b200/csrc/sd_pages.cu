@@ -104,7 +104,9 @@ int decode_ctas(int sms) { return 2 * sms; }
 // ends (programmatic dependent launch); every kernel waits for it
 // (griddepcontrol.wait) before its first access to memory, and lets its own
 // successor begin only after that, so that whatever begins early finds all
-// work before its predecessor complete. Since a kernel's inputs may be written
+// work before its predecessor complete. One access comes before the wait: the
+// merge reads the lengths, which no decode kernel writes and whatever did is
+// complete. Since a kernel's inputs may be written
 // while it already waits, none is read through the non-coherent path.
 int32_t launch(const void* fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void** args) {
   cudaLaunchConfig_t cfg{};

@@ -406,7 +406,7 @@ def copy_pages(pages: KVPages, src, dst, *, flags=None, stream=None) -> None:
 def paged_decode(q, pages: KVPages, tables, lengths, scale: Optional[float] = None, *, layer: int = 0, window: int = 0,
                  sinks=None, out=None, flags=None, stream=None):
     """Attention of one new token per sequence over its pages: q
-    [batch, Hq, D] -> [batch, Hq, D], softmax(scale q K^T) V over the last
+    [batch, Hq, D] (contiguous, on a 16-byte boundary) -> [batch, Hq, D], softmax(scale q K^T) V over the last
     `window` (0: all) of lengths[b] tokens. A length of 0 gives zeros.
 
     tables [batch, width] and lengths [batch]: int32, read on the device only,
