@@ -148,18 +148,18 @@ def _rotation(inv_freq, traditional, factor, q_norm, k_norm, eps, dtype, dev: in
                       _arg(k_norm, "k_norm", dtype, dev, (dim,)), eps, factor, rot, 1 if traditional else 0)
 
 
-# The keys of a rope_scaling dict that each kind's formula has, and those that say nothing about the angles (rope_theta
-# is checked against the base).
+# The keys of a rope_scaling dict that each kind's formula has, and those that every kind's dict may have: the lengths,
+# which some formulas read, and what says nothing about the angles (rope_theta is checked against the base).
 _SCALING_KEYS = {
     "default": (),
     "linear": ("factor",),
-    "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"),
-    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "attention_factor",
-             "mscale", "mscale_all_dim"),
-    "longrope": ("factor", "original_max_position_embeddings", "long_factor", "short_factor", "attention_factor"),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+    "yarn": ("factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"),
+    "longrope": ("factor", "long_factor", "short_factor", "attention_factor"),
 }
 _SCALING_KEYS["su"] = _SCALING_KEYS["longrope"]
-_SILENT_KEYS = ("type", "rope_type", "rope_theta", "partial_rotary_factor", "finetuned")
+_COMMON_KEYS = ("type", "rope_type", "rope_theta", "partial_rotary_factor", "finetuned", "max_position_embeddings",
+                "original_max_position_embeddings")
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda", *,
@@ -200,13 +200,14 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
         kind = scaling.get("rope_type", scaling.get("type", "default"))
         if kind not in _SCALING_KEYS:
             raise ValueError(f"unknown rope scaling {kind!r}")
-        other = [k for k in scaling if k not in _SCALING_KEYS[kind] and k not in _SILENT_KEYS]
+        other = [k for k in scaling if k not in _SCALING_KEYS[kind] and k not in _COMMON_KEYS]
         if other:
             raise ValueError(f"{kind} rope scaling does not have {', '.join(other)}")
         if float(scaling.get("rope_theta", base)) != float(base):
             raise ValueError(f"rope_theta is {scaling['rope_theta']}, the base {base}")
         f = float(scaling.get("factor", 1.0))
         known = scaling.get("original_max_position_embeddings", original_max_position_embeddings)
+        most = scaling.get("max_position_embeddings", max_position_embeddings)
         if kind in ("linear", "llama3", "yarn") and "factor" not in scaling:
             raise ValueError(f"{kind} rope scaling needs factor")
         if kind in ("llama3", "yarn") and known is None:
@@ -244,9 +245,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[di
                 mult = mscale(1.0)
         elif kind in ("longrope", "su"):
             if "factor" not in scaling:
-                if known is None or max_position_embeddings is None:
+                if known is None or most is None:
                     raise ValueError("longrope needs factor, or max_ and original_max_position_embeddings")
-                f = max_position_embeddings / known
+                f = most / known
             name = "long_factor" if f > 1 else "short_factor"
             each = scaling.get(name)
             if each is None or len(each) != rot_dim // 2:

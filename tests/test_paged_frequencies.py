@@ -125,3 +125,12 @@ def test_keys_that_change_nothing_pass():
     assert freq(64, 10000.0, {**COMPLETE["yarn"], "truncate": None}) == freq(64, 10000.0, COMPLETE["yarn"])
     assert freq(64, 10000.0, {**COMPLETE["yarn"], "mscale": 1.0, "mscale_all_dim": 1.0})[1] == 1.0
     assert freq(64, 10000.0, {}) == freq(64, 10000.0)
+
+
+def test_lengths_in_the_dict_of_a_kind_without_them_pass():
+    """A context's lengths do not change the angles of these kinds; longrope reads them in the dict as well."""
+    lengths = {"original_max_position_embeddings": 4096, "max_position_embeddings": 131072}
+    for s in (COMPLETE["linear"], {"rope_type": "default"}):
+        assert freq(64, 10000.0, {**s, **lengths}) == freq(64, 10000.0, s)
+    assert freq(64, 10000.0, {**COMPLETE["yarn"], "max_position_embeddings": 131072}) == freq(64, 10000.0, COMPLETE["yarn"])
+    assert freq(96, 10000.0, {**PUBLISHED, **lengths}) == freq(96, 10000.0, PUBLISHED, **lengths)
