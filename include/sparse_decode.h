@@ -363,6 +363,95 @@ int32_t sd_paged_decode(const sd_pages* pages, int32_t layer, const void* q, int
                         int32_t window, const float* sinks, void* out, void* workspace, int64_t workspace_bytes,
                         int32_t* device_flags, sd_stream stream);
 
+/* ---------------------------------------------------------------------------
+ * Several new tokens per sequence: drafted tokens, in a chain or a tree, that
+ * one step checks (speculative decoding). The plan says where they go, the
+ * attention lets each see the cached tokens and its own ancestors, and the
+ * rows of those that are accepted move to where they stay.
+ *
+ * The new tokens of a step are rows of packed arrays, sequence by sequence:
+ * those of sequence b are rows first[b] .. first[b + 1], its node i the i-th
+ * of them. Node i is stored at position held + i of its sequence (held: the
+ * tokens before the step), whatever its place in the tree. No counterpart in
+ * the reference (its speculative decoding checks one sequence's chain of
+ * drafted tokens through the model's prompt path and trims the cache:
+ * Libraries/MLXLMCommon/Evaluate.swift).
+ * ------------------------------------------------------------------------- */
+#define SD_MAX_NODES 64
+
+/* All arrays are device arrays; the plan is made on the device alone, so it
+ * can be captured in a graph together with the step. */
+typedef struct {
+  const int32_t* lengths;     /* [batch] tokens that each sequence has */
+  const int32_t* added;       /* [batch] new tokens of each */
+  int32_t* tables;            /* [batch, table_width] pages, in order */
+  int32_t batch;              /* 0 .. 4096 */
+  int32_t table_width;
+  int32_t page_size;          /* 16, 32, 64, 128 or 256 */
+  int32_t n_rows;             /* rows of the outputs below */
+  /* Pages to take, or NULL (all four): the tables are complete. Sequence b has
+   * held[b] pages; those that its new tokens need beyond them are
+   * free_pages[*taken], free_pages[*taken + 1], ..., in the order of the
+   * sequences, and are written into tables, held and *taken. */
+  int32_t* held;              /* [batch] */
+  const int32_t* free_pages;  /* [n_free] */
+  int32_t* taken;             /* [1] */
+  int32_t n_free;
+  /* Trees, or NULL: chains. Node i's parent, a node before it or -1 (the last
+   * token of those held); below -1: there is no such node, nor any below it. */
+  int32_t nodes;              /* most new tokens of a sequence, at most SD_MAX_NODES */
+  const int32_t* parents;     /* [batch, nodes] with rows parents_stride apart; stride 0: one tree for all */
+  int64_t parents_stride;
+  /* outputs */
+  int32_t* first;             /* [batch + 1] rows before each sequence */
+  int32_t* ends;              /* [batch] lengths + new tokens */
+  int32_t* seq;               /* [n_rows] sequence of each row; -1 behind the last */
+  int32_t* positions;         /* [n_rows] where the token is stored; -1: nowhere (sd_paged_append skips it) */
+  int64_t* slots;             /* [n_rows] or NULL: page * page_size + slot in the page, or -1 */
+  int32_t* places;            /* [n_rows] or NULL: position of the token for the rotation, held + depth in the tree; or -1 */
+  int64_t* masks;             /* [n_rows] or NULL: bit j: the token sees node j (itself and its ancestors) */
+} sd_plan;
+
+/* What does not fit -- the tables, the free pages, the tree, n_rows -- is cut
+ * from the new tokens (first and ends say what is left) and sets bit 2 of
+ * *device_flags (nullable); so do negative numbers, which count as 0, and a
+ * parent that does not come before its node, which counts as absent. */
+int32_t sd_paged_plan(const sd_plan* plan, int32_t* device_flags, sd_stream stream);
+
+/* Attention of the new tokens of a step: q, out [n_rows, n_q_heads, D];
+ * lengths [batch] count the new tokens, which are stored before the call.
+ * Row n of sequence b sees the tokens before the step and, of the new ones,
+ * those whose bits masks[n] has (NULL: the ones up to itself). With a window
+ * it sees the tokens whose place is above its own less the window; places
+ * [n_rows], at least the tokens before the step; NULL: where they are stored.
+ * sinks as in sd_paged_decode. A row that sees nothing gives zeros; nodes that
+ * a row does not see are not read for it; rows from first[batch] on are left
+ * as they are. At most SD_MAX_NODES new tokens per sequence, 16 query heads
+ * per kv head, batch <= 4096. A sequence whose numbers cannot be (rows outside
+ * n_rows, more nodes, fewer tokens than nodes, more than the table holds) gives
+ * zeros and sets bit 2 of *device_flags, and so does a page out of range,
+ * whose tokens read as 0. Equal calls give equal bits. The workspace
+ * (sd_paged_tree_workspace bytes, 16-byte aligned, contents do not matter)
+ * must not be shared by calls that may overlap. q, out: 16-byte aligned. */
+int32_t sd_paged_tree_workspace(const sd_pages* pages, int32_t batch, int32_t n_rows, int32_t n_q_heads, int64_t* bytes);
+int32_t sd_paged_tree_decode(const sd_pages* pages, int32_t layer, const void* q, int32_t n_rows, int32_t batch,
+                             int32_t n_q_heads, const int32_t* tables, int32_t table_width, const int32_t* lengths,
+                             const int32_t* first, const int64_t* masks, const int32_t* places, float scale,
+                             int32_t window, const float* sinks, void* out, void* workspace, int64_t workspace_bytes,
+                             int32_t* device_flags, sd_stream stream);
+
+/* Keep kept[b] of the new tokens of each sequence, nodes path[b, 0] < path[b, 1]
+ * < ... (path [batch, path_width], path_width <= SD_MAX_NODES): their rows move
+ * to positions held, held + 1, ..., in every layer and array of the pool, and
+ * new_lengths[b] = held + kept[b], held = ends[b] - (first[b + 1] - first[b]).
+ * Pages of two sequences must not be the same where rows move. An entry that
+ * is no node or does not rise, or a page out of range, ends its sequence's
+ * path there and sets bit 2 of *device_flags. new_lengths must be none of the
+ * inputs here (it may be the lengths that the plan was made from). */
+int32_t sd_paged_keep(const sd_pages* pages, const int32_t* tables, int32_t batch, int32_t table_width,
+                      const int32_t* ends, const int32_t* first, const int32_t* path, int32_t path_width,
+                      const int32_t* kept, int32_t* new_lengths, int32_t* device_flags, sd_stream stream);
+
 /* Which sequence holds which page: host bookkeeping of one pool, with pages
  * shared between forked sequences by reference counts. No call touches the
  * GPU; those that need page copies return the pairs for sd_copy_pages. The

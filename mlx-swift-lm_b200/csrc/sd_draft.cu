@@ -1,0 +1,289 @@
+// sd_draft.cu -- the plan of a step of new tokens, and the rows that stay of
+// them.
+#include "sd_device.cuh"
+#include "sd_draft.h"
+
+namespace sd {
+
+namespace {
+
+// Exclusive sum of v over the block's threads in order; *total: of all.
+__device__ __forceinline__ int64_t block_before(int64_t v, int64_t* sums, int64_t* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  int64_t incl = v;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, x);
+    if (lane >= x) incl += y;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int w = 0; w < nw; ++w) {
+    before += w < warp ? sums[w] : 0;
+    all += sums[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + incl - v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* at, int64_t row, int n, const T (&v)[kPlanRows], bool wide) {
+  if (wide && n == kPlanRows) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<int4*>(at + row) = make_int4(v[0], v[1], v[2], v[3]);
+    } else {
+      *reinterpret_cast<longlong2*>(at + row) = make_longlong2(v[0], v[1]);
+      *reinterpret_cast<longlong2*>(at + row + 2) = make_longlong2(v[2], v[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPlanRows; ++i)
+      if (i < n) at[row + i] = v[i];
+  }
+}
+
+}  // namespace
+
+// Sequence b has len[b] tokens and gets n[b] more. With c[b] pages held,
+//   need[b] = max(0, ceil((len + n) / P) - c), from free[taken + sum_{a < b} need[a]] on,
+// rows first[b] = sum_{a < b} n[a] on are its new tokens: row first[b] + i lies at
+// position len[b] + i, slot table[position / P] * P + position % P. Of a tree,
+// node i's mask has its own bit and those of its parent's mask, its place is
+// one past its parent's (the sequence's length for a root). What does not fit
+// (the table, the free pages, the tree, the rows) is cut, with an error bit,
+// so that what is planned can always be done.
+//
+// Bound by latency up to some ten thousand rows (a launch, the lengths, the
+// table), then by its stores: 16 bytes a row, 28 with a tree. Every CTA works out all sequences'
+// sums for itself (at most 4096) and then takes blocks of rows; a thread
+// finds its first row's sequence by bisection and goes on from there. A mask
+// is a walk up the tree, one cached load per ancestor. The pages taken are
+// written by the same launch where its CTAs can wait until all have read what
+// is held (one cluster of at most 8), and by a second one otherwise.
+// Measured as whole calls: see the table of the operators.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int sm[];
+  __shared__ int64_t sums[kPlanThreads / 32];
+  int *first = sm, *len = first + p.B + 1, *have = len + p.B, *base = have + p.B;
+  const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int per = (p.B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  const int taken = p.held ? max(0, min(__ldcg(p.taken), p.n_free)) : 0;
+  bool bad = p.held && taken != __ldcg(p.taken);
+  // first[b + 1]: the new tokens of b, as far as the table and the tree hold them
+  int64_t need = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int raw = __ldcg(p.lengths + b), add = __ldcg(p.added + b);
+    const int l = max(raw, 0), c = p.held ? __ldcg(p.held + b) : p.W, h = max(0, min(c, p.W));
+    int n = int(max(int64_t(0), min(int64_t(max(add, 0)), min(int64_t(p.W) * p.P - l, int64_t(p.N)))));
+    if (p.parents) n = min(n, p.T);
+    bad = bad || raw < 0 || n != add || h != c;
+    len[b] = l;
+    have[b] = h;
+    first[b + 1] = n;
+    base[b] = max(0, int((int64_t(l) + n + p.P - 1) >> p.page_shift) - h);
+    if (!p.held) base[b] = 0;
+    need += base[b];
+  }
+  int64_t all, run = block_before(need, sums, &all);
+  need = 0;  // from here on: rows
+  for (int b = b0; b < b1; ++b) {
+    const int want = base[b], got = int(max(int64_t(0), min(int64_t(want), p.n_free - taken - run)));
+    base[b] = int(min(run, int64_t(p.n_free - taken))) + taken;
+    run += want;
+    if (got < want) {
+      bad = true;
+      first[b + 1] = int(max(int64_t(0), min(int64_t(first[b + 1]), (int64_t(have[b]) + got) * p.P - len[b])));
+    }
+    need += first[b + 1];
+  }
+  const int pages_end = int(min(all, int64_t(p.n_free - taken))) + taken;
+  run = block_before(need, sums, &all);
+  for (int b = b0; b < b1; ++b) {
+    const int n = first[b + 1];
+    bad = bad || run + n > p.N;
+    run += n;
+    first[b + 1] = int(min(run, int64_t(p.N)));
+  }
+  if (tid == 0) first[0] = 0;
+  __syncthreads();
+  const int total = first[p.B];
+  if (bad && p.flags && blockIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
+
+  if (p.rows) {
+    for (int b = blockIdx.x * kPlanThreads + tid; b <= p.B; b += gridDim.x * kPlanThreads) {
+      p.first[b] = first[b];
+      if (b < p.B) p.ends[b] = len[b] + first[b + 1] - first[b];
+    }
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.seq) | reinterpret_cast<uintptr_t>(p.positions) |
+                        reinterpret_cast<uintptr_t>(p.places) | reinterpret_cast<uintptr_t>(p.slots) |
+                        reinterpret_cast<uintptr_t>(p.masks)) & 15) == 0;
+    bool odd = false;  // a parent that does not come before its node
+    const int64_t step = int64_t(gridDim.x) * kPlanThreads * kPlanRows;
+    for (int64_t r0 = (int64_t(blockIdx.x) * kPlanThreads + tid) * kPlanRows; r0 < p.N; r0 += step) {
+      const int cnt = int(min(int64_t(kPlanRows), p.N - r0));
+      int seq[kPlanRows], pos[kPlanRows], place[kPlanRows];
+      int64_t slot[kPlanRows], mask[kPlanRows];
+      int b = 0;
+      if (r0 < total) {  // the last b with first[b] <= r0: it has rows
+        int hi = p.B;
+        while (hi - b > 1) {
+          const int mid = (b + hi) >> 1;
+          if (first[mid] <= r0) b = mid; else hi = mid;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kPlanRows; ++i) {
+        const int r = int(r0) + i;
+        seq[i] = pos[i] = place[i] = -1;
+        slot[i] = -1;
+        mask[i] = 0;
+        if (i >= cnt || r >= total) continue;
+        while (r >= first[b + 1]) ++b;  // ends: r < total
+        seq[i] = b;
+        const int node = r - first[b], at = len[b] + node;
+        if (p.parents) {
+          const int* up = p.parents + b * p.parents_stride;
+          uint64_t m = 0;
+          int a = node, d = -1;
+          while (a >= 0) {  // ends: every parent taken lies before its node
+            m |= uint64_t(1) << a;
+            ++d;
+            const int next = __ldcg(up + a);
+            if (next >= a) odd = true;
+            a = next >= a ? -2 : next;
+          }
+          if (a != -1) continue;  // absent, or below an absent node
+          mask[i] = int64_t(m);
+          place[i] = len[b] + d;
+        } else {
+          place[i] = at;
+          mask[i] = int64_t((uint64_t(2) << min(node, kMaxNodes - 1)) - 1);
+        }
+        pos[i] = at;
+        const int col = at >> p.page_shift;
+        const int page = col < have[b] ? __ldcg(p.tables + int64_t(b) * p.W + col) : __ldcg(p.free_pages + base[b] + col - have[b]);
+        slot[i] = page < 0 ? -1 : int64_t(page) * p.P + (at & (p.P - 1));
+      }
+      store4(p.seq, r0, cnt, seq, wide);
+      store4(p.positions, r0, cnt, pos, wide);
+      if (p.slots) store4(p.slots, r0, cnt, slot, wide);
+      if (p.places) store4(p.places, r0, cnt, place, wide);
+      if (p.masks) store4(p.masks, r0, cnt, mask, wide);
+    }
+    if (odd && p.flags) atomicOr(p.flags, kErrBadIndex);
+  }
+  if (!p.commit) return;
+  if (gridDim.x > 1) cluster_sync();  // every CTA has read what is held
+  for (int b = blockIdx.x * kPlanThreads + tid; b < p.B; b += gridDim.x * kPlanThreads) {
+    const int got = (b + 1 < p.B ? base[b + 1] : pages_end) - base[b];
+    for (int i = 0; i < got; ++i) p.tables[int64_t(b) * p.W + have[b] + i] = __ldcg(p.free_pages + base[b] + i);
+    if (got > 0) p.held[b] = have[b] + got;
+  }
+  if (blockIdx.x == 0 && tid == 0) *p.taken = pages_end;
+}
+
+const void* plan_kernel_ptr() { return reinterpret_cast<const void*>(&plan_kernel); }
+
+namespace {
+
+// Rows src[i] -> dst[i] (row numbers of head 0, -1: stays), i < n, of one column of an array: W bytes at `at`.
+template <typename W>
+__device__ __forceinline__ void keep_rows(uint8_t* at, int row, const int* src, const int* dst, int n) {
+  for (int i0 = 0; i0 < n; i0 += kKeepBatch) {
+    W x[kKeepBatch];
+#pragma unroll
+    for (int i = 0; i < kKeepBatch; ++i)
+      if (i0 + i < n && src[i0 + i] >= 0) x[i] = *reinterpret_cast<const W*>(at + int64_t(src[i0 + i]) * row);
+#pragma unroll
+    for (int i = 0; i < kKeepBatch; ++i)
+      if (i0 + i < n && src[i0 + i] >= 0) *reinterpret_cast<W*>(at + int64_t(dst[i0 + i]) * row) = x[i];
+  }
+}
+
+}  // namespace
+
+// Row h + i of a sequence becomes its row h + path[i], i < kept, in every layer,
+// K and V (h: its tokens before the step), and its length h + kept. path rises,
+// so path[i] >= i: a row is overwritten only when it has been read, if rows are
+// taken in order -- a thread does so with its own 16 bytes of a (head, row),
+// eight rows under way at a time, and no thread waits for another. One block
+// per (layer, sequence). Bound by HBM for many users, by latency (path, table,
+// rows: three loads one after the other) for few.
+__global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constant__ KeepParams p) {
+  __shared__ int src[kMaxNodes], dst[kMaxNodes], count;
+  const int tid = threadIdx.x, b = blockIdx.x % p.B, layer = blockIdx.x / p.B;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (tid < 32) {
+    const int f0 = __ldcg(p.first + b), f1 = __ldcg(p.first + b + 1), end = __ldcg(p.ends + b), k0 = __ldcg(p.kept + b);
+    int64_t nodes = int64_t(f1) - f0, held = int64_t(end) - nodes;
+    bool bad = false;
+    if (nodes < 0 || held < 0 || end > int64_t(p.W) * p.P) {
+      bad = true;
+      nodes = 0;
+      held = max(int64_t(0), min(int64_t(end), int64_t(p.W) * p.P));
+    }
+    int k = int(max(int64_t(0), min(int64_t(k0), min(int64_t(p.T), nodes))));
+    bad = bad || k != k0;
+    int stop = k;  // the first entry that cannot be done
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int i = half * 32 + tid;
+      bool wrong = false;
+      if (i < k) {
+        const int* path = p.path + int64_t(b) * p.T;
+        const int j = __ldcg(path + i), before = i ? __ldcg(path + i - 1) : -1;
+        wrong = j <= before || j >= nodes;
+        int from = -1, to = -1;
+        if (!wrong && j != i) {
+          const int a = int(held) + j, c = int(held) + i;
+          const int pa = __ldcg(p.tables + int64_t(b) * p.W + (a >> p.page_shift));
+          const int pc = __ldcg(p.tables + int64_t(b) * p.W + (c >> p.page_shift));
+          wrong = pa < 0 || pa >= p.n_pages || pc < 0 || pc >= p.n_pages;
+          if (!wrong) {
+            from = pa * p.Hkv * p.P + (a & (p.P - 1));
+            to = pc * p.Hkv * p.P + (c & (p.P - 1));
+          }
+        }
+        src[i] = from;
+        dst[i] = to;
+      }
+      const unsigned w = __ballot_sync(0xffffffffu, wrong);
+      if (w) stop = min(stop, half * 32 + __ffs(w) - 1);
+    }
+    if (stop < k) bad = true;
+    if (tid == 0) {
+      count = stop;
+      if (layer == 0) {
+        p.lengths[b] = int(held) + stop;
+        if (bad && p.flags) atomicOr(p.flags, kErrBadIndex);
+      }
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  for (int c = tid; c < p.all_columns && n > 0; c += kKeepThreads) {
+    int a = 0, x = c;
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+      if (a == i && x >= p.columns[i]) x -= p.columns[i], ++a;
+    const int row = p.row[a], width = min(row, 16), per = row / width;
+    const int h = x / per;
+    uint8_t* at = p.array[a] + p.layer[a] * layer + int64_t(h) * p.P * row + (x - h * per) * width;
+    switch (width) {
+      case 16: keep_rows<uint4>(at, row, src, dst, n); break;
+      case 8: keep_rows<uint2>(at, row, src, dst, n); break;
+      case 4: keep_rows<uint32_t>(at, row, src, dst, n); break;
+      default: keep_rows<uint16_t>(at, row, src, dst, n);
+    }
+  }
+}
+
+const void* keep_kernel_ptr() { return reinterpret_cast<const void*>(&keep_kernel); }
+
+}  // namespace sd

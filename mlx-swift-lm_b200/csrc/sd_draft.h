@@ -1,0 +1,97 @@
+// sd_draft.h -- parameters and kernels of the operators around drafted tokens:
+// the plan of a step, the rows that are kept, attention over trees. Included by
+// host and device code.
+#pragma once
+
+#include "sd_paged.h"
+
+namespace sd {
+
+constexpr int kMaxNodes = 64;  // new tokens of one sequence in a tree: the bits of a mask
+
+// ---------------------------------------------------------------------------
+// The plan of a step and the rows that are kept
+// ---------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanRows = 4;      // rows that a thread takes at a time: 16-byte stores
+constexpr int kPlanCluster = 8;   // CTAs that may wait for one another
+
+struct PlanParams {
+  const int *lengths, *added;  // [B]
+  int* tables;                 // [B, W]
+  int* held;                   // [B] or null: no pages are taken
+  const int* free_pages;
+  int* taken;
+  const int* parents;          // [B or 1, T] or null
+  int64_t parents_stride;      // of a sequence; 0: one tree for all
+  int n_free, T;
+  int B, W, P, page_shift, N;
+  int *first, *ends, *seq, *positions, *places;
+  int64_t *slots, *masks;
+  int* flags;
+  bool rows, commit;           // what this launch does: the rows, the pages taken
+};
+// Dynamic shared memory of a plan launch: rows before, lengths, held pages and pages before each sequence.
+constexpr int plan_smem(int B) { return (4 * B + 1) * 4; }
+const void* plan_kernel_ptr();
+
+struct KeepParams {
+  const int *tables, *ends, *first, *path, *kept;
+  int* lengths;
+  int B, W, P, page_shift, N, T, Hkv;
+  int64_t n_pages;
+  uint8_t* array[6];
+  int row[6];                 // bytes of a row (token and head) in each array
+  int64_t layer[6];           // bytes of a layer
+  int columns[6];             // accesses that make one token's rows of each array: heads * row / width
+  int all_columns;
+  int* flags;
+};
+constexpr int kKeepThreads = 256;
+constexpr int kKeepBatch = 8;  // rows that a thread has under way
+const void* keep_kernel_ptr();
+
+// ---------------------------------------------------------------------------
+// Attention over trees
+// ---------------------------------------------------------------------------
+
+// lengths: tokens of each sequence, its new ones counted in; G, q and out: of packed rows [N, Hq, D].
+struct TreeParams : PagedParams {
+  const int* first;        // [B + 1]
+  const int64_t* masks;    // [N] or null: a node sees those up to itself
+  const int* places;       // [N] or null: the position of each node, for windows
+  const uint8_t *k_data, *v_data;  // of this layer
+  int* line;               // [2][B + 1]: units and pairs before each sequence
+  int N, Hq;
+  int RT;                  // columns (node, query head) of a pair
+  int halves;              // segments of one pair and CTA
+  int part_floats;         // of one segment in the workspace
+  int row_floats, dim_floats;  // from one column to the next there, and from four dims to the next four
+};
+
+struct TreeSet {
+  const void* attend;  // tree_attend_kernel<E, BITS, D, blocks of columns>(TreeParams, CUtensorMap, CUtensorMap)
+  const void* merge;   // tree_merge_kernel<E, BITS, D>(TreeParams)
+  int tile, stage_bytes, columns;
+};
+// For at most `columns` columns a pair, or as many as there are.
+TreeSet tree_e0_b0(int D, int columns);
+TreeSet tree_e1_b0(int D, int columns);
+TreeSet tree_e2_b0(int D, int columns);
+TreeSet tree_e0_b4(int D, int columns);
+TreeSet tree_e1_b4(int D, int columns);
+TreeSet tree_e2_b4(int D, int columns);
+TreeSet tree_e0_b8(int D, int columns);
+TreeSet tree_e1_b8(int D, int columns);
+TreeSet tree_e2_b8(int D, int columns);
+
+constexpr int kTreeMergeThreads = 256;
+constexpr int kTreeHeads = 4;  // query heads of one merge warp
+
+// Shared memory of an attend CTA: as a decode's, with two numbers per sequence and the columns' first tokens.
+constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
+  return paged_layout_of((2 * (batch + 1) + 2 * (kPagedThreads / 32) + 16) * 4, columns, D, dense_f32, stage_bytes);
+}
+
+}  // namespace sd

@@ -96,7 +96,20 @@ struct LaneAddr {
 struct TileView {
   const uint8_t* stage;
   int pb_log;
-  int lo, hi;  // valid token rows of the tile
+  int lo, hi;      // valid token rows of the tile
+  const int* low;  // drafted tokens: the first token that each column sees, where that may lie in the tile; else null
+  int tok;         // the tile's first token, with low
+};
+
+// The columns of a decode's products: the query heads of one kv head. Those of
+// drafted tokens are NodeCols (sd_tree.cuh).
+struct HeadCols {
+  static constexpr bool kLow = false;  // all see the same tokens
+  int n;
+  int64_t row0;
+  __device__ __forceinline__ HeadCols(const PagedParams& p, int b, int h)
+      : n(p.G), row0(int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G) {}
+  __device__ __forceinline__ int64_t row(int i) const { return row0 + i; }
 };
 
 // (m, l) and o of one warp in the combine buffer.
@@ -142,7 +155,7 @@ __device__ __forceinline__ float raise_max(float& m, float mx) {
 // the maximum's. At a kUp of 0 the many small weights beside an attention sink
 // (each below 2^-25) were lost to o, though not to l.
 // ---------------------------------------------------------------------------
-template <typename E, int D, int NB>
+template <typename E, int D, int NB, class Cols>
 struct DenseAttend {
   using F = PagedFmt<2, 0, D>;
   static constexpr int NC = D / 16;
@@ -150,17 +163,17 @@ struct DenseAttend {
   uint32_t qb[NB][NC][2];
   float m[NB][2], l[NB][2], o[NB][NC][4];
 
-  __device__ __forceinline__ void begin(const PagedParams& p, const float*, int b, int h, int, int lane) {
+  __device__ __forceinline__ void begin(const PagedParams& p, const float*, const Cols& cols, int, int lane) {
     const int g = lane >> 2, tq = lane & 3;
     const uint32_t* q = static_cast<const uint32_t*>(p.q);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int hd = 8 * nb + g;
-      const int64_t row = (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * (D / 2);
+      const int64_t row = cols.row(hd) * (D / 2);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        qb[nb][c][0] = hd < p.G ? q[row + 8 * c + tq] : 0u;
-        qb[nb][c][1] = hd < p.G ? q[row + 8 * c + 4 + tq] : 0u;
+        qb[nb][c][0] = hd < cols.n ? q[row + 8 * c + tq] : 0u;
+        qb[nb][c][1] = hd < cols.n ? q[row + 8 * c + 4 + tq] : 0u;
         o[nb][c][0] = o[nb][c][1] = o[nb][c][2] = o[nb][c][3] = 0.0f;
       }
       m[nb][0] = m[nb][1] = -INFINITY;
@@ -197,7 +210,9 @@ struct DenseAttend {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float v = (acc[0][nb][i] + acc[1][nb][i]) * p.scale_log2;
-        s[nb][i] = (i < 2 ? ok0 : ok1) ? v : -INFINITY;
+        bool ok = i < 2 ? ok0 : ok1;
+        if (Cols::kLow && t.low) ok = ok && t.tok + r0 + g + 8 * (i >> 1) >= t.low[8 * nb + 2 * tq + (i & 1)];
+        s[nb][i] = ok ? v : -INFINITY;
         up |= s[nb][i] > m[nb][i & 1] + (kSlack + kUp);
       }
     }
@@ -259,7 +274,7 @@ struct DenseAttend {
     }
   }
 
-  __device__ __forceinline__ void end(const PagedParams& p, const WarpPart<D>& w, int lane) {
+  __device__ __forceinline__ void end(int n, const WarpPart<D>& w, int lane) {
     const int g = lane >> 2, tq = lane & 3;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -270,7 +285,7 @@ struct DenseAttend {
         ls += __shfl_xor_sync(0xffffffffu, ls, 8);
         ls += __shfl_xor_sync(0xffffffffu, ls, 16);
         const int hd = 8 * nb + 2 * tq + e;
-        if (hd < p.G) {
+        if (hd < n) {
           if (g == 0) {
             w.ml[2 * hd] = m[nb][e];
             w.ml[2 * hd + 1] = ls;
@@ -346,7 +361,7 @@ __device__ __forceinline__ void load_groups(uint32_t a, int t, float (&f)[NG]) {
 // that an error of at most 2^-28 of it. One half alone was 13 bf16 ulp off where
 // the terms of an output nearly cancel, and no faster.
 // ---------------------------------------------------------------------------
-template <typename E, int BITS, int D, int NB>
+template <typename E, int BITS, int D, int NB, class Cols>
 struct CodesAttend {
   using F = PagedFmt<sizeof(E), BITS, D>;
   static constexpr int NK = D / 16, NG = F::kGroups, NCH = F::kNChunk;
@@ -361,7 +376,7 @@ struct CodesAttend {
   float qs[NB][2][NG], qoff[NB][2][NG], m[NB][2], l[NB][2], o[NB][NK][4], ob[NB][2][NG];
   float vinv[NG], vlim[NG], qfac;
 
-  __device__ __forceinline__ void begin(const PagedParams& p, const float*, int b, int h, int, int lane) {
+  __device__ __forceinline__ void begin(const PagedParams& p, const float*, const Cols& cols, int, int lane) {
     const int g = lane >> 2, tq = lane & 3;
     // this lane's elements of head g: four (8-bit) or eight (4-bit) neighbours of every chunk
     constexpr int N = BITS == 8 ? 4 : 8, W = N * int(sizeof(E)) / 4;  // elements, 32-bit words
@@ -377,17 +392,17 @@ struct CodesAttend {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int hd = 8 * nb + g;
-      const E* row = static_cast<const E*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G + hd) * D;
+      const E* row = static_cast<const E*>(p.q) + cols.row(hd) * D;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const uint32_t* at = reinterpret_cast<const uint32_t*>(row + F::kEpc * c + N * tq);
         if constexpr (W == 2) {
-          const uint2 w = hd < p.G ? *reinterpret_cast<const uint2*>(at) : make_uint2(0, 0);
+          const uint2 w = hd < cols.n ? *reinterpret_cast<const uint2*>(at) : make_uint2(0, 0);
           raw[nb][c][0] = w.x, raw[nb][c][1] = w.y;
         } else {
 #pragma unroll
           for (int i = 0; i < W; i += 4) {
-            const uint4 w = hd < p.G ? *reinterpret_cast<const uint4*>(at + i) : make_uint4(0, 0, 0, 0);
+            const uint4 w = hd < cols.n ? *reinterpret_cast<const uint4*>(at + i) : make_uint4(0, 0, 0, 0);
             raw[nb][c][i] = w.x, raw[nb][c][i + 1] = w.y, raw[nb][c][i + 2] = w.z, raw[nb][c][i + 3] = w.w;
           }
         }
@@ -554,6 +569,15 @@ struct CodesAttend {
           for (int nb = 0; nb < NB; ++nb) s[mt][nb][i] = tk < lo || tk >= hi ? -INFINITY : s[mt][nb][i];
         }
     }
+    if (Cols::kLow && t.low) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            if (t.tok + r0 + 16 * mt + g + 8 * (i >> 1) < t.low[8 * nb + 2 * (lane & 3) + (i & 1)]) s[mt][nb][i] = -INFINITY;
+    }
     bool up = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -703,7 +727,7 @@ struct CodesAttend {
     }
   }
 
-  __device__ __forceinline__ void end(const PagedParams& p, const WarpPart<D>& w, int lane) {
+  __device__ __forceinline__ void end(int n, const WarpPart<D>& w, int lane) {
     const int g = lane >> 2, tq = lane & 3;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -717,7 +741,7 @@ struct CodesAttend {
           for (int r = 0; r < NG; ++r) ob[nb][e][r] += __shfl_xor_sync(0xffffffffu, ob[nb][e][r], x);
         }
         const int hd = 8 * nb + 2 * tq + e;
-        if (hd < p.G) {
+        if (hd < n) {
           if (g == 0) {
             w.ml[2 * hd] = m[nb][e];
             w.ml[2 * hd + 1] = ls;
@@ -746,7 +770,7 @@ struct CodesAttend {
 // heads. q (times scale * log2 e, rows padded against bank conflicts) lies in
 // shared memory.
 // ---------------------------------------------------------------------------
-template <int D, int HB>
+template <int D, int HB, class Cols>
 struct FmaAttend {
   using F = PagedFmt<4, 0, D>;
   static constexpr int NCH = F::kNChunk, TW = 8, DL = D / 8;
@@ -756,12 +780,15 @@ struct FmaAttend {
   // Where a lane's dims lie in the row: every eighth chunk, so that the eight lanes of a head read all banks.
   static __device__ __forceinline__ int dim(int lane, int i) { return 4 * (8 * (i / 4) + (lane & 7)) + i % 4; }
 
-  // every consumer thread calls; qf: [G][D + 4]
-  __device__ __forceinline__ void begin(const PagedParams& p, float* qf, int b, int h, int warp, int lane) {
-    const float* q = static_cast<const float*>(p.q) + (int64_t(b) * p.Hkv * p.G + int64_t(h) * p.G) * D;
+  int last;  // column, of drafted tokens
+
+  // every consumer thread calls; qf: [columns][D + 4]
+  __device__ __forceinline__ void begin(const PagedParams& p, float* qf, const Cols& cols, int warp, int lane) {
+    const float* q = static_cast<const float*>(p.q) + cols.row0 * D;
+    last = cols.n - 1;
 #pragma unroll 1
-    for (int i = warp * 32 + lane; i < p.G * D; i += 32 * kPagedWarps)
-      qf[i / D * (D + 4) + i % D] = q[i] * p.scale_log2;
+    for (int i = warp * 32 + lane; i < cols.n * D; i += 32 * kPagedWarps)
+      qf[i / D * (D + 4) + i % D] = q[Cols::kLow ? (cols.row(i / D) - cols.row0) * D + i % D : i] * p.scale_log2;
     named_barrier(1, 32 * kPagedWarps);
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
@@ -785,7 +812,7 @@ struct FmaAttend {
     float s[HB];
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-      qrow[hb] = qf + min(4 * hb + (lane & 3), p.G - 1) * (D + 4);  // a head past the last repeats it
+      qrow[hb] = qf + min(4 * hb + (lane & 3), Cols::kLow ? last : p.G - 1) * (D + 4);  // past the last: it again
       s[hb] = 0.0f;
     }
 #pragma unroll 4
@@ -799,7 +826,7 @@ struct FmaAttend {
     }
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-      s[hb] = ok ? s[hb] : -INFINITY;
+      s[hb] = ok && !(Cols::kLow && t.low && t.tok + r0 + tok < t.low[4 * hb + (lane & 3)]) ? s[hb] : -INFINITY;
       if (__any_sync(0xffffffffu, s[hb] > m[hb] + kSlack)) {
         float mx = s[hb];
         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
@@ -830,17 +857,17 @@ struct FmaAttend {
     }
   }
 
-  __device__ __forceinline__ void end(const PagedParams& p, const WarpPart<D>& w, int lane) {
+  __device__ __forceinline__ void end(int n, const WarpPart<D>& w, int lane) {
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
       float ls = l[hb];
       for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
       const int hd = 4 * hb + (lane & 3), vh = 4 * hb + (lane >> 3);
-      if (lane < 4 && hd < p.G) {
+      if (lane < 4 && hd < n) {
         w.ml[2 * hd] = m[hb];
         w.ml[2 * hd + 1] = ls;
       }
-      if (vh < p.G) {
+      if (vh < n) {
 #pragma unroll
         for (int i = 0; i < DL; i += 4)
           *reinterpret_cast<float4*>(w.o + vh * (D + 4) + dim(lane, i)) =
@@ -893,6 +920,7 @@ struct Segment {
 };
 
 struct Walk {
+  using Seg = Segment;
   const int* prefix;
   int Hkv, b, u, u1;
   __device__ __forceinline__ Walk(const int* pre, int B, int hkv, int begin, int end)
@@ -922,12 +950,12 @@ struct Walk {
 };
 
 // NB: blocks of heads, of four for dense fp32 pools, else of eight.
-template <typename E, int BITS, int D, int NB>
-struct PickAttend { using type = CodesAttend<E, BITS, D, NB>; };
-template <typename E, int D, int NB>
-struct PickAttend<E, 0, D, NB> { using type = DenseAttend<E, D, NB>; };
-template <int D, int NB>
-struct PickAttend<float, 0, D, NB> { using type = FmaAttend<D, NB>; };
+template <typename E, int BITS, int D, int NB, class Cols>
+struct PickAttend { using type = CodesAttend<E, BITS, D, NB, Cols>; };
+template <typename E, int D, int NB, class Cols>
+struct PickAttend<E, 0, D, NB, Cols> { using type = DenseAttend<E, D, NB, Cols>; };
+template <int D, int NB, class Cols>
+struct PickAttend<float, 0, D, NB, Cols> { using type = FmaAttend<D, NB, Cols>; };
 
 // After a wait that expired: wait, with the limit, for the copies of the last
 // `stages` of `it` uses, which still land in this CTA's shared memory.
@@ -936,9 +964,9 @@ static __device__ __noinline__ void drain(uint64_t* full, int it, int stages) {
 }
 
 // The producer warp: this CTA's tiles into the ring, stage by stage.
-template <typename E, int BITS, int D>
-__device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV,
-                                              uint8_t* ring, uint64_t* full, uint64_t* empty, Walk walk, int lane) {
+template <typename E, int BITS, int D, class Params, class Line>
+__device__ __forceinline__ void paged_produce(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV,
+                                              uint8_t* ring, uint64_t* full, uint64_t* empty, Line walk, int lane) {
   using F = PagedFmt<sizeof(E), BITS, D>;
   const uint64_t pol = stream_policy(false);
   const int pb = min(p.P, F::kTile), nb = F::kTile / pb;   // rows per box, boxes per tile
@@ -946,7 +974,7 @@ __device__ __forceinline__ void paged_produce(const PagedParams& p, const CUtens
   const int oob_row = int(p.n_pages * p.Hkv * p.P);  // past the tensor: TMA fills zeros
   int it = 0, st = 0;
   uint32_t round = 0;  // parity of the stages' current use
-  Segment s;
+  typename Line::Seg s;
   while (walk.next(s)) {
     const TokenRange r = token_range(p, s.b);
     const int* row = p.tables + int64_t(s.b) * p.W;
@@ -1095,7 +1123,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
     paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
     return;
   }
-  using A = typename PickAttend<E, BITS, D, NB>::type;
+  using A = typename PickAttend<E, BITS, D, NB, HeadCols>::type;
   const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
   A att;
   Segment s;
@@ -1105,12 +1133,12 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
   while (walk.next(s)) {
     const TokenRange r = token_range(p, s.b);
     const int t0 = r.begin / F::kTile;
-    att.begin(p, qf, s.b, s.h, warp, lane);
+    att.begin(p, qf, HeadCols(p, s.b, s.h), warp, lane);
     for (int i = s.i0; i < s.i1; ++i, ++it) {
       const int tok = (t0 + i) * F::kTile;
       if (!dead) dead = !mbar_wait(full + st, round, p.flags);
       if (!dead) {
-        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, r.begin - tok, r.end - tok}, warp, lane);
+        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, r.begin - tok, r.end - tok, nullptr, 0}, warp, lane);
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + st);
       }
@@ -1119,7 +1147,7 @@ paged_decode_kernel(const __grid_constant__ PagedParams p, const __grid_constant
         round ^= 1u;
       }
     }
-    att.end(p, WarpPart<D>(buf, p.G, warp), lane);
+    att.end(p.G, WarpPart<D>(buf, p.G, warp), lane);
     named_barrier(1, 32 * kPagedWarps);
     // the four warps' parts, in warp order
     const bool whole = s.i0 == 0 && s.i1 == s.nt;

@@ -68,10 +68,8 @@ struct PagedLayout {
   int q_off, buf_off, prefix_off, bar_off;
   int bytes;   // of the launch, the way to the boundary included
 };
-constexpr PagedLayout paged_layout(int batch, int G, int D, bool dense_f32, int stage_bytes) {
+constexpr PagedLayout paged_layout_of(int pre, int G, int D, bool dense_f32, int stage_bytes) {  // pre: bytes
   const int qf = dense_f32 ? G * (D + 4) * 4 : 0, buf = kPagedWarps * paged_warp_floats(G, D) * 4;
-  // below 32 sequences every warp has its own row of 32
-  const int pre = (batch < 32 ? 32 * (kPagedWarps + 1) : batch + 1 + kPagedThreads / 32) * 4;
   const int bars = 2 * kPagedMaxStages * 8;
   const int q128 = (qf + 127) / 128 * 128, buf128 = (buf + 127) / 128 * 128, pre128 = (pre + 127) / 128 * 128;
   const int room = (kPagedSmem - (q128 + buf128 + pre128 + bars + 1024)) / stage_bytes;
@@ -83,6 +81,11 @@ constexpr PagedLayout paged_layout(int batch, int G, int D, bool dense_f32, int 
   l.bar_off = l.prefix_off + pre128;
   l.bytes = l.bar_off + bars + 1024;
   return l;
+}
+constexpr PagedLayout paged_layout(int batch, int G, int D, bool dense_f32, int stage_bytes) {
+  // below 32 sequences every warp has its own row of 32
+  const int pre = (batch < 32 ? 32 * (kPagedWarps + 1) : batch + 1 + kPagedThreads / 32) * 4;
+  return paged_layout_of(pre, G, D, dense_f32, stage_bytes);
 }
 
 struct PagedParams {

@@ -1,0 +1,536 @@
+// sd_tree.cuh -- attention of the drafted tokens of each sequence, a tree of at
+// most 64 nodes, over a paged KV pool.
+//
+// Sequence b has held = lengths[b] - n tokens before its n nodes, which are rows
+// first[b] .. first[b + 1] of q and out. Node i sees the held tokens and the
+// nodes j whose bit its mask has; with a window those alone whose place is above
+// its own less the window (token t's place is t). For its query head hq,
+//   out = sum_t e^(s_t) v_t / (sum_t e^(s_t) + e^(sink)),  s_t = scale q.k_t;
+// a row that sees nothing gives zeros.
+//
+// The held tokens are the same for all nodes (but for the low end of a window),
+// the nodes are few and differ from row to row. So the work is in two parts that
+// know nothing of each other:
+//   * tree_attend_kernel (or the tile kernel, sd_tree_tile.cu) attends to the
+//     held tokens with no mask at all. The (node, query head) columns of a kv
+//     head are cut into pairs of at most RT columns, and the pairs' tiles are one
+//     line that CTAs share equally, as in a decode (sd_paged.cuh). Every segment
+//     leaves (o, m, l) in the workspace.
+//   * tree_merge_kernel takes a row and four query heads per warp: it attends to
+//     the visible nodes one by one, reading no other node's rows -- what lies
+//     there, not-a-numbers included, does not reach it -- while the segments
+//     are still being worked on, and then joins those in CTA order.
+// Results depend on no timing. Lengths, rows and tables are read on the device
+// only, so a captured graph serves growing sequences.
+#pragma once
+
+#include "sd_draft.h"
+#include "sd_paged.cuh"
+
+namespace sd {
+
+// What one sequence has of a call. A sequence whose numbers cannot be is taken
+// for one without tokens, and its rows give zeros.
+struct TreeSeq {
+  int row0, n, held, begin;  // first row, nodes, tokens before them, first of those that any node sees
+  bool bad;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
+  const int f0 = __ldcg(p.first + b), f1 = __ldcg(p.first + b + 1), len = __ldcg(p.lengths + b);
+  const int64_t n = int64_t(f1) - f0;
+  TreeSeq s;
+  s.bad = f0 < 0 || f1 > p.N || n < 0 || n > kMaxNodes || len < n || len > int64_t(p.W) * p.P;
+  s.row0 = f0;
+  s.n = s.bad ? 0 : int(n);
+  s.held = s.n ? len - s.n : 0;
+  s.begin = p.window > 0 && s.held >= p.window ? s.held - p.window + 1 : 0;
+  return s;
+}
+// The held tokens of sequence b, for the producer.
+__device__ __forceinline__ TokenRange token_range(const TreeParams& p, int b) {
+  const TreeSeq s = tree_seq(p, b);
+  return {s.begin, s.held};
+}
+__device__ __forceinline__ int tree_pairs(const TreeParams& p, const TreeSeq& s) {
+  return (s.n * p.G + p.RT - 1) / p.RT * p.Hkv;
+}
+// The first token that node i sees: `place` is its position.
+__device__ __forceinline__ int tree_low(const TreeParams& p, const TreeSeq& s, int node) {
+  const int place = p.places ? __ldcg(p.places + s.row0 + node) : s.held + node;
+  return p.window > 0 ? max(0, int(min(int64_t(place) + 1 - p.window, int64_t(s.held)))) : 0;
+}
+
+// Units and pairs before each sequence, by all NT threads of the block; tmp: [2 * NT / 32].
+template <int NT>
+__device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* units, int* pairs, int* tmp) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (p.B + NT - 1) / NT, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  int u = 0, k = 0;
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const TreeSeq s = tree_seq(p, b);
+    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.held}, tile);
+    bad = bad || s.bad;
+    k += np;
+    u += np * nu;
+  }
+  if (bad && p.flags && blockIdx.x == 0) atomicOr(p.flags, kErrBadIndex);
+  int iu = u, ik = k;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int yu = __shfl_up_sync(0xffffffffu, iu, x), yk = __shfl_up_sync(0xffffffffu, ik, x);
+    if (lane >= x) iu += yu, ik += yk;
+  }
+  if (lane == 31) tmp[2 * warp] = iu, tmp[2 * warp + 1] = ik;
+  __syncthreads();
+  u = iu - u, k = ik - k;
+  for (int w = 0; w < warp; ++w) u += tmp[2 * w], k += tmp[2 * w + 1];
+  if (tid == 0) units[0] = pairs[0] = 0;
+  for (int b = b0; b < b1; ++b) {
+    const TreeSeq s = tree_seq(p, b);
+    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.held}, tile);
+    units[b + 1] = u += np * nu;
+    pairs[b + 1] = k += np;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {  // for the merge
+    for (int b = tid; b <= p.B; b += NT) {
+      p.line[b] = units[b];
+      p.line[p.B + 1 + b] = pairs[b];
+    }
+  }
+}
+
+struct TreeSegment {
+  int b, h, c, pair;   // kv head, which RT columns of it, number of the pair
+  int i0, i1;          // tiles
+};
+
+// A CTA's way along the line. Pairs of a sequence: kv head by kv head, its columns' pairs side by side, which share
+// their tiles in L2.
+struct TreeWalk {
+  using Seg = TreeSegment;
+  const int *units, *pairs;
+  int Hkv, b, u, u1;
+  __device__ __forceinline__ TreeWalk(const int* un, const int* pr, int B, int hkv, int begin, int end)
+      : units(un), pairs(pr), Hkv(hkv), b(0), u(begin), u1(end) {
+    int hi = B;  // the largest b with units[b] <= u
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (units[mid] <= u) b = mid; else hi = mid;
+    }
+  }
+  __device__ __forceinline__ bool next(TreeSegment& s) {
+    while (u < u1) {
+      while (units[b + 1] <= u) ++b;  // ends: u < units[B]
+      const int np = pairs[b + 1] - pairs[b], nu = (units[b + 1] - units[b]) / np, r = u - units[b], k = r / nu;
+      const int per = np / Hkv, first = r - k * nu, last = min(nu, first + u1 - u);
+      s.b = b;
+      s.h = k / per;
+      s.c = k - s.h * per;
+      s.pair = pairs[b] + k;
+      u += last - first;
+      s.i0 = max(first - kSegmentUnits, 0);
+      s.i1 = last - kSegmentUnits;
+      if (s.i1 > s.i0) return true;
+    }
+    return false;
+  }
+};
+
+// The columns of a pair: x0 + i is (node, query head of the kv head) number x0 + i of the sequence.
+struct NodeCols {
+  static constexpr bool kLow = true;
+  int n, x0, G, Hq;
+  int64_t row0;  // of column x0
+  __device__ __forceinline__ NodeCols(const TreeParams& p, const TreeSeq& s, int h, int c)
+      : n(min(p.RT, s.n * p.G - c * p.RT)), x0(c * p.RT), G(p.G), Hq(p.Hq) {
+    base = int64_t(s.row0) * p.Hq + int64_t(h) * p.G;
+    row0 = row(0);
+  }
+  __device__ __forceinline__ int node(int i) const { return (x0 + i) / G; }
+  __device__ __forceinline__ int64_t row(int i) const {
+    const int nd = node(i);
+    return base + int64_t(nd) * Hq + (x0 + i - nd * G);
+  }
+ private:
+  int64_t base;
+};
+
+// Where segment `k` (pair + CTA: both rise along the line, so no two segments share it) lies in the workspace.
+__device__ __forceinline__ float* tree_part(const TreeParams& p, int k) { return p.part + int64_t(k) * p.part_floats; }
+
+// The consumers of a decode (sd_paged.cuh) with columns for heads.
+template <typename E, int BITS, int D, int NB>
+__global__ void __launch_bounds__(kPagedThreads, 2)
+tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV) {
+  using F = PagedFmt<sizeof(E), BITS, D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* qf = reinterpret_cast<float*>(sm + p.q_off);
+  float* buf = reinterpret_cast<float*>(sm + p.buf_off);
+  int* units = reinterpret_cast<int*>(sm + p.prefix_off);
+  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kPagedThreads / 32);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
+  uint64_t* empty = full + kPagedMaxStages;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(full + i, BITS ? 33 : 1);
+      mbar_init(empty + i, kPagedWarps);
+    }
+    fence_mbar_init();
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  tree_line<kPagedThreads>(p, F::kTile, units, pairs, tmp);
+
+  const Pieces pieces(p, units[p.B]);
+  if (int(blockIdx.x) >= pieces.n) return;
+  TreeWalk walk(units, pairs, p.B, p.Hkv, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
+
+  if (warp == kPagedWarps) {
+    paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
+    return;
+  }
+  using A = typename PickAttend<E, BITS, D, NB, NodeCols>::type;
+  const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
+  A att;
+  TreeSegment s;
+  int it = 0, st = 0;
+  uint32_t round = 0;
+  bool dead = false;
+  while (walk.next(s)) {
+    const TreeSeq sq = tree_seq(p, s.b);
+    const NodeCols cols(p, sq, s.h, s.c);
+    const int t0 = sq.begin / F::kTile;
+    int edge = 0;  // tokens below it are not seen by every column
+    if (p.window) {
+      if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
+      named_barrier(1, 32 * kPagedWarps);
+      edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
+    }
+    att.begin(p, qf, cols, warp, lane);
+    for (int i = s.i0; i < s.i1; ++i, ++it) {
+      const int tok = (t0 + i) * F::kTile;
+      if (!dead) dead = !mbar_wait(full + st, round, p.flags);
+      if (!dead) {
+        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, sq.begin - tok, sq.held - tok, tok < edge ? low : nullptr, tok},
+                 warp, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + st);
+      }
+      if (++st == p.stages) {
+        st = 0;
+        round ^= 1u;
+      }
+    }
+    att.end(cols.n, WarpPart<D>(buf, p.RT, warp), lane);
+    named_barrier(1, 32 * kPagedWarps);
+    // the four warps' parts, in warp order
+    float* part = tree_part(p, s.pair + blockIdx.x);
+    for (int k = tid; k < cols.n * (D / 4); k += 32 * kPagedWarps) {
+      const int g = k / (D / 4), d4 = k % (D / 4);
+      float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        mw[w] = WarpPart<D>(buf, p.RT, w).ml[2 * g];
+        M = fmaxf(M, mw[w]);
+      }
+      float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        const WarpPart<D> wp(buf, p.RT, w);
+        const float f = exp2_from(mw[w], M);
+        const float4 x = *reinterpret_cast<const float4*>(wp.o + g * (D + 4) + 4 * d4);
+        L = fmaf(f, wp.ml[2 * g + 1], L);
+        O.x = fmaf(f, x.x, O.x);
+        O.y = fmaf(f, x.y, O.y);
+        O.z = fmaf(f, x.z, O.z);
+        O.w = fmaf(f, x.w, O.w);
+      }
+      *reinterpret_cast<float4*>(part + g * p.row_floats + d4 * p.dim_floats) = O;
+      if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
+    }
+    named_barrier(1, 32 * kPagedWarps);
+  }
+  if (dead) drain(full, it, p.stages);
+}
+
+// ---------------------------------------------------------------------------
+// The nodes, and the join
+// ---------------------------------------------------------------------------
+
+// V neighbouring elements of a row, E each, in fp32.
+template <typename E, int V>
+__device__ __forceinline__ void load_elements(const E* at, float (&f)[V]) {
+  if constexpr (sizeof(E) == 4) {
+    if constexpr (V == 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(at));
+      f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+    } else {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(at));
+      f[0] = x.x, f[1] = x.y;
+    }
+  } else if constexpr (V == 4) {
+    const uint2 x = __ldcg(reinterpret_cast<const uint2*>(at));
+    unpack_word<E>(x.x, f);
+    unpack_word<E>(x.y, f + 2);
+  } else {
+    unpack_word<E>(__ldcg(reinterpret_cast<const unsigned int*>(at)), f);
+  }
+}
+
+// One lane's V elements of a stored row, as loaded (the loads of several tokens are under way together) and as values.
+template <typename E, int BITS, int V>
+struct StoredPiece {
+  uint32_t code;
+  E scale, bias;
+  __device__ __forceinline__ void load(const uint8_t* data, const void* scales, const void* biases, int64_t row, int lane) {
+    constexpr int D = 32 * V, ROW = D * BITS / 8, W = V * BITS / 8;
+    const uint8_t* at = data + row * ROW + lane * W;
+    if constexpr (W == 4) code = __ldcg(reinterpret_cast<const unsigned int*>(at));
+    else if constexpr (W == 2) code = __ldcg(reinterpret_cast<const unsigned short*>(at));
+    else code = __ldcg(at);
+    const int64_t g = row * (D / 64) + lane * V / 64;
+    scale = static_cast<const E*>(scales)[g];
+    bias = static_cast<const E*>(biases)[g];
+  }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+    const float s = Elt<E>::to_f32(scale), b = Elt<E>::to_f32(bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = fmaf(float((code >> (BITS * i)) & ((1u << BITS) - 1)), s, b);
+  }
+};
+template <typename E, int V>
+struct StoredPiece<E, 0, V> {
+  float x[V];
+  __device__ __forceinline__ void load(const uint8_t* data, const void*, const void*, int64_t row, int lane) {
+    load_elements<E, V>(reinterpret_cast<const E*>(data) + row * (32 * V) + lane * V, x);
+  }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = x[i];
+  }
+};
+
+// A warp per (row, up to four query heads of one kv head). Lane l holds
+// dimensions [l V, l V + V) of q, o and the rows; scores are summed over the
+// lanes by a butterfly that ends with head l / 8's in lane l, so that lane l
+// keeps token l % 8's of the eight that are taken at a time. Bound by latency:
+// a row sees some ten nodes, and their loads, eight together, hide behind the
+// attend kernel, as does everything before griddep_wait.
+template <typename E, int BITS, int D>
+__global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int V = D / 32, HB = kTreeHeads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups;
+  const int64_t item = int64_t(blockIdx.x) * (kTreeMergeThreads / 32) + warp;
+  const int n = int(item / per);
+  int b = -1;
+  if (n < p.N && n < __ldcg(p.first + p.B)) {  // the last b with first[b] <= n: it has rows
+    b = 0;
+    int hi = p.B;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (__ldcg(p.first + mid) <= n) b = mid; else hi = mid;
+    }
+  }
+  if (b < 0) {  // rows behind the last sequence stay as they are
+    griddep_wait();
+    return;
+  }
+  const TreeSeq s = tree_seq(p, b);
+  const int hg = int(item - int64_t(n) * per), h = hg / groups, g0 = (hg - h * groups) * HB, heads = min(HB, p.G - g0);
+  const int node = n - s.row0;
+  const int64_t row0 = int64_t(n) * p.Hq + int64_t(h) * p.G + g0;  // of q and out
+  E* out = static_cast<E*>(p.out);
+  const bool mine = !s.bad && node >= 0 && node < s.n;
+
+  float q[HB][V], o[HB][V], m[HB], l[HB];
+#pragma unroll
+  for (int g = 0; g < HB; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[g][i] = o[g][i] = 0.0f;
+    if (mine && g < heads) load_elements<E, V>(static_cast<const E*>(p.q) + (row0 + g) * D + lane * V, q[g]);
+  }
+  if (mine) {
+    uint64_t seen = p.masks ? uint64_t(__ldcg(reinterpret_cast<const long long*>(p.masks) + n)) : (uint64_t(2) << node) - 1;
+    if (s.n < 64) seen &= (uint64_t(1) << s.n) - 1;
+    // lane j: rows of nodes j and j + 32
+    int at[2];
+    const int64_t place = p.window ? (p.places ? int64_t(__ldcg(p.places + n)) : int64_t(s.held) + node) - p.window : 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = lane + 32 * e;
+      bool see = (seen >> j) & 1;
+      if (see && p.window) see = (p.places ? __ldcg(p.places + s.row0 + j) : s.held + j) > place;
+      at[e] = -1;
+      if (see) {
+        const int t = s.held + j, page = __ldcg(p.tables + int64_t(b) * p.W + t / p.P);
+        if (page >= 0 && page < p.n_pages) at[e] = (page * p.Hkv + h) * p.P + (t & (p.P - 1));
+        else if (p.flags) atomicOr(p.flags, kErrBadIndex);
+      }
+      const unsigned v = __ballot_sync(0xffffffffu, see);
+      seen = e ? (seen & 0xffffffffull) | (uint64_t(v) << 32) : (seen & ~0xffffffffull) | v;
+    }
+#pragma unroll 1
+    while (seen) {
+      StoredPiece<E, BITS, V> kp[8], vp[8];
+      bool ok[8];  // alike for all lanes; a page out of range reads as zeros
+      int cnt = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        ok[t] = false;
+        if (seen) {
+          const int j = __ffsll(seen) - 1;
+          seen &= seen - 1;
+          const int row = __shfl_sync(0xffffffffu, j < 32 ? at[0] : at[1], j & 31);
+          ok[t] = row >= 0;
+          cnt = t + 1;
+          if (ok[t]) {
+            kp[t].load(p.k_data, p.k_scales, p.k_biases, row, lane);
+            vp[t].load(p.v_data, p.v_scales, p.v_biases, row, lane);
+          }
+        }
+      }
+      float sc = -INFINITY;  // of head lane / 8 and token lane % 8
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        float a[HB] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (ok[t]) {
+          float f[V];
+          kp[t].get(f);
+#pragma unroll
+          for (int g = 0; g < HB; ++g)
+#pragma unroll
+            for (int i = 0; i < V; ++i) a[g] = fmaf(q[g][i], f[i], a[g]);
+        }
+        const bool b4 = lane & 16, b3 = lane & 8;
+        float x0 = b4 ? a[2] : a[0], x1 = b4 ? a[3] : a[1];
+        x0 += __shfl_xor_sync(0xffffffffu, b4 ? a[0] : a[2], 16);
+        x1 += __shfl_xor_sync(0xffffffffu, b4 ? a[1] : a[3], 16);
+        float x = b3 ? x1 : x0;
+        x += __shfl_xor_sync(0xffffffffu, b3 ? x0 : x1, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        if (t < cnt && (lane & 7) == t) sc = x * p.scale_log2;
+      }
+      float mx = sc;
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      float w = 0.0f;
+#pragma unroll
+      for (int g = 0; g < HB; ++g) {
+        const float f = raise_max(m[g], __shfl_sync(0xffffffffu, mx, 8 * g));
+        l[g] *= f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[g][i] *= f;
+        if (lane >> 3 == g) w = exp2_from(sc, m[g]);
+      }
+      if ((lane & 7) >= cnt) w = 0.0f;
+      float sum = w;
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+#pragma unroll
+      for (int g = 0; g < HB; ++g) l[g] += __shfl_sync(0xffffffffu, sum, 8 * g);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        float f[V] = {};
+        if (ok[t]) vp[t].get(f);
+#pragma unroll
+        for (int g = 0; g < HB; ++g) {
+          const float pr = __shfl_sync(0xffffffffu, w, 8 * g + t);
+          if (ok[t]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[g][i] = fmaf(pr, f[i], o[g][i]);
+          }
+        }
+      }
+    }
+  }
+
+  griddep_wait();
+  if (mine && s.held > s.begin) {
+    const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
+    const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
+    const int rt = np / p.Hkv, nu = (u1 - up) / np;
+    const Pieces pieces(p, all);
+    int at[HB], c0[HB], ns[HB], most = 0;  // column of its pair; pair + first CTA; segments
+    float2 ml[HB];
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      const int x = node * p.G + g0 + min(g, heads - 1), c = x / p.RT, k = h * rt + c;
+      at[g] = x - c * p.RT;
+      const int a = up + k * nu, first = pieces.of(a + kSegmentUnits), last = pieces.of(a + nu - 1);
+      c0[g] = pp + k + first;
+      ns[g] = (last - first + 1) * p.halves;
+      most = max(most, ns[g]);
+      c0[g] *= p.halves;
+    }
+    for (int base = 0; base < most; base += 32) {
+#pragma unroll
+      for (int g = 0; g < HB; ++g) {
+        ml[g] = make_float2(-INFINITY, 0.0f);
+        if (base + lane < ns[g])
+          ml[g] = __ldcg(reinterpret_cast<const float2*>(tree_part(p, c0[g] + base + lane) + p.RT * D + 2 * at[g]));
+      }
+      float f[HB];
+#pragma unroll
+      for (int g = 0; g < HB; ++g) {
+        const float f0 = raise_max(m[g], warp_max(ml[g].x));
+        f[g] = exp2_from(ml[g].x, m[g]);
+        l[g] = fmaf(l[g], f0, warp_sum(f[g] * ml[g].y));
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[g][i] *= f0;
+      }
+#pragma unroll 4
+      for (int j = 0; j < min(32, most - base); ++j) {
+#pragma unroll
+        for (int g = 0; g < HB; ++g) {
+          const float w = __shfl_sync(0xffffffffu, f[g], j);
+          if (base + j < ns[g]) {
+            const float* x = tree_part(p, c0[g] + base + j) + at[g] * p.row_floats + lane * V / 4 * p.dim_floats + lane * V % 4;
+            if constexpr (V == 4) {
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(x));
+              o[g][0] = fmaf(w, y.x, o[g][0]);
+              o[g][1] = fmaf(w, y.y, o[g][1]);
+              o[g][2] = fmaf(w, y.z, o[g][2]);
+              o[g][3] = fmaf(w, y.w, o[g][3]);
+            } else {
+              const float2 y = __ldcg(reinterpret_cast<const float2*>(x));
+              o[g][0] = fmaf(w, y.x, o[g][0]);
+              o[g][1] = fmaf(w, y.y, o[g][1]);
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < HB; ++g) {
+    if (g < heads) {
+      float L = l[g];
+      if (p.sinks) L += exp2f(fmaf(__ldcg(p.sinks + h * p.G + g0 + g), 1.4426950408889634f, -(m[g] == -INFINITY ? 0.0f : m[g])));
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      E* at = out + (row0 + g) * D + lane * V;
+      if constexpr (sizeof(E) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(at + i) = make_float2(o[g][i] * inv, o[g][i + 1] * inv);
+      } else if constexpr (V == 4) {
+        *reinterpret_cast<uint2*>(at) = make_uint2(pack2<E>(o[g][0] * inv, o[g][1] * inv), pack2<E>(o[g][2] * inv, o[g][3] * inv));
+      } else {
+        *reinterpret_cast<uint32_t*>(at) = pack2<E>(o[g][0] * inv, o[g][1] * inv);
+      }
+    }
+  }
+}
+
+}  // namespace sd

@@ -45,7 +45,8 @@ EXPORTED = ["sd_abi_version", "sd_status_string", "sd_last_error", "sd_index_cre
             "sd_shard_decode", "sd_set_sinks", "sd_rotary", "sd_paged_append", "sd_copy_pages", "sd_paged_workspace",
             "sd_paged_decode", "sd_pagemap_create", "sd_pagemap_destroy", "sd_pagemap_add", "sd_pagemap_fork",
             "sd_pagemap_free", "sd_pagemap_extend", "sd_pagemap_trim", "sd_pagemap_length", "sd_pagemap_tables",
-            "sd_pagemap_width", "sd_pagemap_free_pages", "sd_pagemap_compact"]
+            "sd_pagemap_width", "sd_pagemap_free_pages", "sd_pagemap_compact", "sd_paged_plan",
+            "sd_paged_tree_workspace", "sd_paged_tree_decode", "sd_paged_keep"]
 COMM_HANDLE_BYTES = 128
 
 
@@ -86,6 +87,15 @@ class SDRotation(ctypes.Structure):
     _fields_ = [("inv_freq", ctypes.c_void_p), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
                 ("eps", ctypes.c_float), ("factor", ctypes.c_float), ("rot_dim", ctypes.c_int32),
                 ("traditional", ctypes.c_int32), ("reserved", ctypes.c_int32 * 2)]
+
+
+class SDPlan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("lengths", "added", "tables")] + [
+        (n, ctypes.c_int32) for n in ("batch", "table_width", "page_size", "n_rows")] + [
+        (n, ctypes.c_void_p) for n in ("held", "free_pages", "taken")] + [
+        ("n_free", ctypes.c_int32), ("nodes", ctypes.c_int32), ("parents", ctypes.c_void_p),
+        ("parents_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("first", "ends", "seq", "positions", "slots", "places", "masks")]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -151,6 +161,11 @@ def lib() -> ctypes.CDLL:
             "sd_pagemap_width": ([vp, pi64, i32, pi32], i32),
             "sd_pagemap_free_pages": ([vp, pi64], i32),
             "sd_pagemap_compact": ([vp, pi32, pi32, i32, pi32], i32),
+            "sd_paged_plan": ([ctypes.POINTER(SDPlan), vp, vp], i32),
+            "sd_paged_tree_workspace": ([pg, i32, i32, i32, pi64], i32),
+            "sd_paged_tree_decode": ([pg, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, vp, f32, i32, vp, vp, vp, i64, vp,
+                                      vp], i32),
+            "sd_paged_keep": ([pg, vp, i32, i32, vp, vp, vp, i32, vp, vp, vp, vp], i32),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
@@ -485,3 +500,4 @@ from .persist import (load_prompt_cache, make_prompt_cache, maybe_quantize_kv_ca
                       save_prompt_cache)
 from .paged import (KVPages, PagedBatch, PagedLayer, PagePool, copy_pages, paged_append, paged_decode,  # noqa: E402,F401
                     rotary, rotary_frequencies)
+from .drafts import MAX_NODES, TokenPlan, paged_keep, paged_plan, paged_tree_decode  # noqa: E402,F401

@@ -1,9 +1,10 @@
 """Build libsparse_decode.so (sm_100a) in-tree with nvcc.
 
 The library is compiled from mlx-swift-lm_b200/csrc: one object per storage
-format (sd_inst.cu and, for the paged cache, sd_paged_inst.cu, with
-SD_E/SD_BITS), the rotary and page-copy kernels (sd_rotary.cu), plus the C ABI
-(sd_api.cu, sd_pages.cu). The CUDA runtime is linked statically, so the .so
+format (sd_inst.cu and, for the paged cache, sd_paged_inst.cu and sd_tree_inst.cu,
+with SD_E/SD_BITS), the rotary and page-copy kernels (sd_rotary.cu), the plan
+and row kernels of drafted tokens (sd_draft.cu), plus the C ABI (sd_api.cu,
+sd_pages.cu, sd_steps.cu). The CUDA runtime is linked statically, so the .so
 only needs the driver at run time.
 
 `build(phase_timing=True)` makes a second library, libsparse_decode_phases.so,
@@ -42,12 +43,12 @@ def _kernel_sources(name: str, skip: set) -> list[Path]:
     """What a kernel object depends on: its source and csrc's headers, less
     those of host code and of the other kernels."""
     return [CSRC / name] + [h for h in sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
-                            if h.name not in skip | {"sd_host.h"}]
+                            if h.name not in skip | {"sd_host.h", "sd_pages_host.h"}]
 
 
 def _host_sources(name: str) -> list[Path]:
-    return [CSRC / n for n in (name, "sd_format.h", "sd_params.h", "sd_kernels.h", "sd_host.h", "sd_paged.h")] + [
-        INCLUDE / "sparse_decode.h"]
+    return [CSRC / n for n in (name, "sd_format.h", "sd_params.h", "sd_kernels.h", "sd_host.h", "sd_paged.h",
+                               "sd_pages_host.h", "sd_draft.h")] + [INCLUDE / "sparse_decode.h"]
 
 
 def _stale(target: Path, sources: list[Path] | None = None) -> bool:
@@ -71,12 +72,17 @@ def build(force: bool = False, verbose: bool = False, phase_timing: bool = False
     bdir.mkdir(exist_ok=True)
     # (object, source, extra flags, files it depends on)
     units = []
+    tree = {"sd_tree.cuh", "sd_draft.h"}
     for e, b in FORMATS:
         fmt = [f"-DSD_E={e}", f"-DSD_BITS={b}"]
-        units.append((f"sd_inst_e{e}_b{b}.o", "sd_inst.cu", fmt, _kernel_sources("sd_inst.cu", {"sd_paged.cuh", "sd_paged.h"})))
-        units.append((f"sd_paged_e{e}_b{b}.o", "sd_paged_inst.cu", fmt, _kernel_sources("sd_paged_inst.cu", {"sd_decode.cuh"})))
-    units.append(("sd_rotary.o", "sd_rotary.cu", [], _kernel_sources("sd_rotary.cu", {"sd_decode.cuh", "sd_paged.cuh"})))
-    units += [(f"{n}.o", f"{n}.cu", [], _host_sources(f"{n}.cu")) for n in ("sd_api", "sd_pages")]
+        units.append((f"sd_inst_e{e}_b{b}.o", "sd_inst.cu", fmt, _kernel_sources("sd_inst.cu", tree | {"sd_paged.cuh", "sd_paged.h"})))
+        units.append((f"sd_paged_e{e}_b{b}.o", "sd_paged_inst.cu", fmt, _kernel_sources("sd_paged_inst.cu", tree | {"sd_decode.cuh"})))
+        units.append((f"sd_tree_e{e}_b{b}.o", "sd_tree_inst.cu", fmt, _kernel_sources("sd_tree_inst.cu", {"sd_decode.cuh"})))
+    units.append(("sd_rotary.o", "sd_rotary.cu", [],
+                  _kernel_sources("sd_rotary.cu", tree | {"sd_decode.cuh", "sd_paged.cuh"})))
+    units.append(("sd_draft.o", "sd_draft.cu", [],
+                  _kernel_sources("sd_draft.cu", {"sd_tree.cuh", "sd_decode.cuh", "sd_paged.cuh"})))
+    units += [(f"{n}.o", f"{n}.cu", [], _host_sources(f"{n}.cu")) for n in ("sd_api", "sd_pages", "sd_steps")]
     jobs = []
     for obj, src, extra, deps in units:
         if force or _stale(bdir / obj, deps):

@@ -1,0 +1,498 @@
+"""Drafted tokens over the paged cache on the GPU against plain computations:
+plans and moved rows bit for bit against a host model, tree attention against
+64 bits.
+
+Tolerance of the attention: the framework's (_util.assert_close) where weights
+keep 16 bits or more. Where many columns share the tile kernel (16-bit pools,
+more than 16 columns a sequence) a weight p is rounded to the pool's type once,
+by at most u = eps / 2 of it, and the sum that it is divided by is made of the
+rounded ones. With A = sum p |v| / sum p, out is then off by at most
+u A + u |out| (numerator and denominator) before its own rounding of u |out|;
+scores in fp32 add less than 1e-4 of A, as do fp16 weights below 2^-14 of
+2^-7 (at most 2^-24 a token each, against a largest of 2^7).
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+
+from _util import assert_close
+from test_gpu_paged import Pool, gen, tables_of, tdt
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(torch, values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def random_parents(rng, n, chain=False, absent=0.0):
+    p = []
+    for i in range(n):
+        if i and rng.random() < absent:
+            p.append(-2)
+        else:
+            p.append(i - 1 if chain else rng.randint(max(-1, i - 6), i - 1))
+    return p
+
+
+def lineage(parents):
+    """(mask, depth) of each node; mask 0 and depth None for an absent one."""
+    got = []
+    for i, up in enumerate(parents):
+        if up < -1 or up >= i:
+            got.append((0, None))
+        elif up < 0:
+            got.append((1 << i, 0))
+        else:
+            m, d = got[up]
+            got.append((m | 1 << i, d + 1) if m else (0, None))
+    return got
+
+
+def signed(mask):
+    return mask - (1 << 64) if mask >> 63 else mask
+
+
+# ---------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------
+
+def plan_model(lengths, new, tables, page, n_rows, parents=None, held=None, free=None, taken=0):
+    """What paged_plan makes of host lists: dict of lists, and whether anything was cut."""
+    B, W = len(lengths), len(tables[0])
+    tables, held_out, bad = [list(r) for r in tables], list(held) if held else None, False
+    seq, pos, slots, places, masks, first, ends = [], [], [], [], [], [0], []
+    for b in range(B):
+        n, ln = max(0, new[b]), max(0, lengths[b])
+        n = min(n, max(0, W * page - ln))
+        if parents is not None:
+            n = min(n, len(parents[b]))
+        n = min(n, n_rows) if n > n_rows else n
+        bad |= n != new[b] or ln != lengths[b]
+        if held:
+            need = max(0, -(-(ln + n) // page) - held[b])
+            got = min(need, len(free) - taken)
+            tables[b][held[b]:held[b] + got] = free[taken:taken + got]
+            taken += got
+            held_out[b] = held[b] + got
+            if got < need:
+                bad, n = True, max(0, min(n, (held[b] + got) * page - ln))
+        if first[-1] + n > n_rows:
+            bad, n = True, n_rows - first[-1]
+        lines = lineage(parents[b][:n]) if parents is not None else [((2 << min(i, 63)) - 1, i) for i in range(n)]
+        if parents is not None:
+            bad |= any(up >= i for i, up in enumerate(parents[b][:n]))
+        for i, (m, d) in enumerate(lines):
+            at = ln + i
+            seq.append(b)
+            pos.append(at if m else -1)
+            pg = tables[b][at // page]
+            slots.append(pg * page + at % page if m and pg >= 0 else -1)
+            places.append(ln + d if m else -1)
+            masks.append(signed(m))
+        first.append(first[-1] + n)
+        ends.append(ln + n)
+    pad = n_rows - first[-1]
+    return dict(first=first, ends=ends, seq=seq + [-1] * pad, positions=pos + [-1] * pad, slots=slots + [-1] * pad,
+                places=places + [-1] * pad, masks=masks + [0] * pad, tables=tables, held=held_out, taken=taken), bad
+
+
+def check_plan(torch, lengths, new, tables, page, n_rows, parents=None, held=None, free=None, taken=0, shared=False):
+    import sparse_decode as sd
+    want, bad = plan_model(lengths, new, tables, page, n_rows, parents, held, free, taken)
+    flags, t = i32(torch, [0]), i32(torch, tables)
+    grow = dict(held=i32(torch, held), free=i32(torch, free), taken=i32(torch, [taken])) if held else {}
+    up = None if parents is None else i32(torch, parents[0] if shared else parents)
+    p = sd.paged_plan(i32(torch, lengths), i32(torch, new), t, page, n_rows, parents=up, flags=flags, **grow)
+    for name in ("first", "ends", "seq", "positions", "slots"):
+        assert getattr(p, name).tolist() == want[name], name
+    if parents is None:
+        assert p.places is p.positions and p.masks is None
+    else:
+        assert p.places.tolist() == want["places"] and p.masks.tolist() == want["masks"]
+    assert t.tolist() == want["tables"]
+    if held:
+        assert grow["held"].tolist() == want["held"] and grow["taken"].tolist() == [want["taken"]]
+    assert bool(int(flags) & 2) == bad and int(flags) in (0, 2)
+
+
+def plan_case(rng, B, page, most, ctx, nodes=0, spare=4):
+    lengths = [rng.choice([0, page, rng.randint(0, ctx)]) for _ in range(B)]
+    new = [rng.choice([0, 1, rng.randint(0, most)]) for _ in range(B)]
+    held = [-(-n // page) + rng.choice([0, 0, 1]) for n in lengths]  # one page from an earlier draft, perhaps
+    W = max(max(h, -(-(n + k) // page)) for h, n, k in zip(held, lengths, new)) + 1
+    ids = list(range(sum(held) + spare + sum(-(-(n + k) // page) for n, k in zip(lengths, new))))
+    rng.shuffle(ids)
+    tables = []
+    for h in held:
+        tables.append(ids[:h] + [-1] * (W - h))
+        del ids[:h]
+    parents = [random_parents(rng, nodes, absent=0.1) for _ in range(B)] if nodes else None
+    return lengths, new, tables, held, ids, parents
+
+
+@pytest.mark.parametrize("B,page,most,ctx", [(1, 64, 1, 200), (1, 16, 5000, 30), (7, 32, 90, 500), (40, 16, 700, 90),
+                                             (300, 64, 3, 5000), (4096, 16, 9, 100), (2, 256, 70000, 300)])
+def test_plan_takes_pages(cuda, B, page, most, ctx):
+    rng = random.Random(B + page)
+    lengths, new, tables, held, free, _ = plan_case(rng, B, page, most, ctx)
+    for extra in (0, 5):
+        check_plan(cuda, lengths, new, tables, page, sum(new) + extra, held=held, free=free)
+    check_plan(cuda, lengths, new, tables, page, sum(new) + 3, held=held, free=[9, 8, 7] + free, taken=3)
+
+
+@pytest.mark.parametrize("B,nodes,page", [(1, 1, 64), (1, 64, 16), (5, 33, 32), (64, 16, 64), (513, 7, 16)])
+@pytest.mark.parametrize("grow", [False, True])
+def test_plan_of_trees(cuda, B, nodes, page, grow):
+    rng = random.Random(nodes)
+    lengths, new, tables, held, free, parents = plan_case(rng, B, page, nodes, 300, nodes)
+    if grow:
+        check_plan(cuda, lengths, new, tables, page, B * nodes, parents, held, free)
+        return
+    whole, _ = plan_model(lengths, new, tables, page, B * nodes, None, held, free)
+    check_plan(cuda, lengths, new, whole["tables"], page, B * nodes, parents)
+    check_plan(cuda, lengths, new, whole["tables"], page, B * nodes, [parents[0]] * B, shared=True)
+
+
+def test_plan_of_a_long_chain_of_parents(cuda):
+    check_plan(cuda, [5, 0], [64, 64], [[0, 1], [2, 3]], 64, 130, [list(range(-1, 63))] * 2, shared=True)
+
+
+def test_plan_cuts_what_does_not_fit(cuda):
+    t = [[0, 1, -1, -1], [2, -1, -1, -1], [3, -1, -1, -1]]
+    free = [7, 8, 9]
+    # more tokens than the table holds; fewer free pages than needed; more rows than there are; none free at all
+    check_plan(cuda, [20, 3, 0], [100, 4, 2], t, 16, 200, held=[2, 1, 1], free=free)
+    check_plan(cuda, [20, 3, 0], [40, 40, 40], t, 16, 200, held=[2, 1, 1], free=free)
+    check_plan(cuda, [20, 3, 0], [40, 40, 40], t, 16, 30, held=[2, 1, 1], free=free * 3)
+    check_plan(cuda, [32, 3, 0], [1, 1, 17], t, 16, 30, held=[2, 1, 1], free=free, taken=3)
+    # negative numbers; a tree that is smaller than its tokens; parents that do not come before their nodes
+    check_plan(cuda, [-4, 3, 0], [2, -1, 5], t, 16, 20, held=[2, 1, 1], free=free)
+    check_plan(cuda, [20, 3, 0], [3, 5, 2], t, 16, 20, [[-1, 0, 0]] * 3, held=[2, 1, 1], free=free)
+    check_plan(cuda, [1, 3, 0], [4, 4, 4], t, 16, 20, [[-1, 1, 0, 2], [0, -1, 7, 2], [-1, -1, 0, -3]], held=[2, 1, 1], free=free)
+
+
+def test_plan_marks_positions_without_a_page(cuda):
+    check_plan(cuda, [14, 3], [4, 2], [[0, -1], [2, -1]], 16, 8)
+
+
+def test_plan_without_rows_or_sequences(cuda):
+    import sparse_decode as sd
+    p = sd.paged_plan(i32(cuda, []), i32(cuda, []), cuda.empty((0, 3), dtype=cuda.int32, device="cuda"), 16, 5)
+    assert p.first.tolist() == [0] and p.positions.tolist() == [-1] * 5 and p.seq.tolist() == [-1] * 5
+    p = sd.paged_plan(i32(cuda, [4]), i32(cuda, [0]), i32(cuda, [[1]]), 16, 0)
+    assert p.first.tolist() == [0, 0] and p.ends.tolist() == [4]
+
+
+def test_plan_outputs_that_start_between_wide_accesses(cuda):
+    """One tree for all read through a strided view is refused; outputs of odd sizes are written to the last row."""
+    import sparse_decode as sd
+    for n in (1, 2, 3, 5, 7):
+        check_plan(cuda, [3], [n], [[0, 1]], 16, n)
+    with pytest.raises(ValueError):
+        sd.paged_plan(i32(cuda, [3]), i32(cuda, [1]), i32(cuda, [[0]]), 16, 1, parents=i32(cuda, [[-1, 0]] * 2)[:, 0])
+
+
+# ---------------------------------------------------------------------------
+# keep
+# ---------------------------------------------------------------------------
+
+def check_keep(torch, sd, arrays, bits, tables, page, ends, counts, paths, want_paths=None, flag=0, lengths=None):
+    first = [0]
+    for n in counts:
+        first.append(first[-1] + n)
+    want = [[a.clone() for a in half] for half in arrays]
+    for half in want:
+        for a in half:
+            x = a if a.dim() == 5 else a[None]
+            for b, path in enumerate(want_paths if want_paths is not None else paths):
+                h = ends[b] - counts[b]
+                for i, j in enumerate(path):
+                    (tp, ts), (fp, fs) = divmod(h + i, page), divmod(h + j, page)
+                    x[:, tables[b][tp], :, ts] = x[:, tables[b][fp], :, fs].clone()
+    (k, *ks), (v, *vs) = arrays
+    T = max(map(len, paths))
+    flags = i32(torch, [0])
+    path = torch.tensor([p[:T] + [-9] * (T - len(p)) for p in paths], dtype=torch.int32, device="cuda").view(len(paths), T)
+    got = sd.paged_keep(sd.KVPages(k, v, *ks, *vs, bits=bits), i32(torch, tables), i32(torch, ends), i32(torch, first),
+                        path, i32(torch, [len(p) for p in paths]), flags=flags)
+    assert int(flags) == flag
+    done = want_paths if want_paths is not None else paths
+    assert got.tolist() == (lengths or [e - n + len(p) for e, n, p in zip(ends, counts, done)])
+    for a, b in zip(arrays, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def random_arrays(torch, seed, dtype, bits, layers, n_pages, hkv, page, d):
+    g = gen(torch, seed)
+    lead = (layers, n_pages, hkv, page) if layers else (n_pages, hkv, page)
+    raw = lambda last, dt: torch.randint(0, 256, (*lead, last * dt.itemsize), generator=g, device="cuda",  # noqa: E731
+                                         dtype=torch.uint8).view(dt)
+    if bits:
+        return [[raw(d * bits // 32, torch.int32), raw(d // 64, tdt(torch, dtype)), raw(d // 64, tdt(torch, dtype))]
+                for _ in "kv"]
+    return [[raw(d, tdt(torch, dtype))] for _ in "kv"]
+
+
+@pytest.mark.parametrize("dtype,bits,hkv,d,page,layers", [
+    ("bf16", 0, 8, 128, 64, 3), ("f16", 0, 3, 64, 16, 1), ("f32", 0, 2, 128, 32, 0), ("bf16", 8, 8, 128, 128, 2),
+    ("f16", 4, 5, 64, 16, 2), ("f32", 8, 1, 64, 256, 0), ("f32", 4, 40, 128, 16, 1), ("bf16", 4, 2, 64, 64, 5)])
+def test_keep_moves_the_accepted_rows(cuda, dtype, bits, hkv, d, page, layers):
+    import sparse_decode as sd
+    rng = random.Random(d + page)
+    counts = [1, 64, 17, 5, 33, 2, 64]
+    held = [0, page - 3, 100, page, 3 * page - 1, 0, 7]
+    paths = [[0], list(range(64)), sorted(rng.sample(range(17), 9)), [], sorted(rng.sample(range(33), 20)), [1],
+             sorted(rng.sample(range(64), 40))]
+    ends = [h + n for h, n in zip(held, counts)]
+    n_pages = sum(-(-e // page) for e in ends) + 2
+    tables = tables_of(cuda, ends, page, n_pages, 5).tolist()
+    arrays = random_arrays(cuda, 3, dtype, bits, layers, n_pages, hkv, page, d)
+    check_keep(cuda, sd, arrays, bits, tables, page, ends, counts, paths)
+
+
+def test_keep_ends_a_path_that_cannot_be(cuda):
+    import sparse_decode as sd
+    arrays = random_arrays(cuda, 4, "bf16", 0, 2, 20, 2, 16, 64)
+    tables = [[1, 2, 3], [4, 5, 99], [7, -1, 9], [10, 11, 12], [13, 14, 15], [16, 17, 18]]
+    ends, counts = [30, 40, 40, 20, 47, 49], [10, 20, 20, 5, 4, 4]
+    paths = [[1, 3, 3, 4], [0, 9, 14], [1, 2], [2, 4, 5], [3, 2], [0, 1]]
+    # an entry that does not rise; a page past the pool; no page; past the nodes; falling; more tokens than the table,
+    # which keeps what the table holds
+    done = [[1, 3], [0, 9], [], [2, 4], [3], []]
+    want = [22, 22, 20, 17, 44, 48]
+    check_keep(cuda, sd, arrays, 0, tables, 16, ends, counts, paths, done, flag=2, lengths=want)
+
+
+def test_keep_refuses_lengths_that_are_inputs(cuda):
+    import sparse_decode as sd
+    (k,), (v,) = random_arrays(cuda, 4, "bf16", 0, 1, 4, 2, 16, 64)
+    pages, one = sd.KVPages(k, v), i32(cuda, [[0]])
+    ends, first, kept = i32(cuda, [4]), i32(cuda, [0, 2]), i32(cuda, [1])
+    for bad in (ends, kept, first[:1], first[1:], one[0]):
+        with pytest.raises(sd.SDError):
+            sd.paged_keep(pages, one, ends, first, one, kept, lengths=bad)
+    lengths = i32(cuda, [2])
+    assert sd.paged_keep(pages, one, ends, first, one, kept, lengths=lengths) is lengths
+    assert lengths.tolist() == [3]
+
+
+# ---------------------------------------------------------------------------
+# tree attention
+# ---------------------------------------------------------------------------
+
+def tree64(q, pool, tables, held, lines, scale, window=0, sinks=None):
+    """(out, sum p |v| / sum p) in fp64; lines: [[(mask, place)] per node] per sequence, rows in order."""
+    import torch
+    k, v = pool.values
+    hkv, D = k.shape[1], k.shape[-1]
+    out, size = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    row = 0
+    for b, (h, nodes) in enumerate(zip(held, lines)):
+        n = len(nodes)
+        if not n:
+            continue
+        at = tables[b, :-(-(h + n) // pool.page)].long()
+        kk, vv = (x[at].permute(1, 0, 2, 3).flatten(1, 2)[:, :h + n] for x in (k, v))
+        place = torch.tensor(list(range(h)) + [p for _, p in nodes])
+        seen = torch.zeros(n, h + n, dtype=torch.bool)
+        for i, (m, p) in enumerate(nodes):
+            seen[i, :h] = True
+            for j in range(n):
+                seen[i, h + j] = bool(m >> j & 1)
+            if window:
+                seen[i] &= place > p - window
+        seen = seen.cuda()
+        s = torch.einsum("nhgd,htd->hngt", q[row:row + n].double().view(n, hkv, -1, D), kk) * scale
+        s = torch.where(seen[None, :, None], s, -math.inf)  # also not-a-numbers that are not seen
+        if sinks is not None:
+            s = torch.cat((s, sinks.double().view(hkv, 1, -1, 1).expand(hkv, n, -1, 1)), -1)
+        top = s.amax(-1, keepdim=True).clamp(min=-1e300)
+        p = torch.exp(s - top)
+        p = (p / p.sum(-1, keepdim=True).clamp(min=1e-300))[..., :h + n]
+        vz = torch.where(seen.any(0)[None, :, None], vv, 0.0)
+        out[row:row + n] = torch.einsum("hngt,htd->nhgd", p, vz).reshape(n, -1, D)
+        size[row:row + n] = torch.einsum("hngt,htd->nhgd", p, vz.abs()).reshape(n, -1, D)
+        row += n
+    return out, size
+
+
+def check_tree(torch, out, ref, size, dtype, tile):
+    assert torch.isfinite(out).all()
+    if tile:
+        u = torch.finfo(out.dtype).eps / 2
+        off = (out.double() - ref).abs()
+        bound = u * (size + 2 * ref.abs()) * 1.01 + 1e-4 * size + (2.0 ** -24 if dtype == "f16" else 0.0)
+        assert (off <= bound).all(), f"{int((off > bound).sum())} of {off.numel()} off, worst {float((off / bound).max()):.3g}"
+        rel = (off.pow(2).sum() / ref.pow(2).sum().clamp(min=1e-300)).sqrt()
+        assert rel <= u, float(rel)  # the worst case everywhere is more than what adds up in squares
+    else:
+        live = ref.abs().sum(-1) > 0
+        if live.any():
+            d = ref.shape[-1]
+            assert_close(out[live].double().cpu().numpy().reshape(-1, d), ref[live].cpu().numpy().reshape(-1, d), dtype)
+        assert not out[~live].any()
+
+
+def uses_tiles(dtype, bits, counts, G):
+    return dtype != "f32" and not bits and -(-sum(counts) // len(counts)) * G > 16
+
+
+def run_tree(torch, dtype, bits, d, hkv, G, page, held, counts, window=0, sinks=False, seed=0, scale=1.0, chain=False,
+             absent=0.0, causal=False, tail=0):
+    import sparse_decode as sd
+    rng = random.Random(seed)
+    ends = [h + n for h, n in zip(held, counts)]
+    n_pages = sum(-(-t // page) for t in ends) + 3
+    pool = Pool(torch, sd, dtype, bits, hkv, d, page, n_pages, seed + 1, scale)
+    tables = tables_of(torch, ends, page, n_pages, seed + 2)
+    lines, first = [], [0]
+    for h, n in zip(held, counts):
+        nodes = [((2 << i) - 1, i) for i in range(n)] if causal else lineage(random_parents(rng, n, chain, absent))
+        lines.append([(m, h + (x or 0)) for m, x in nodes])
+        first.append(first[-1] + n)
+    # what no row sees holds not-a-numbers
+    keep = torch.zeros(n_pages, page, dtype=torch.bool)
+    for b, (h, nodes) in enumerate(zip(held, lines)):
+        lo = max(0, min((p for _, p in nodes), default=0) + 1 - window) if window else 0
+        for t in range(lo, h if nodes else 0):
+            keep[int(tables[b, t // page]), t % page] = True
+        for j in range(len(nodes)):
+            if any(m >> j & 1 for m, _ in nodes):
+                keep[int(tables[b, (h + j) // page]), (h + j) % page] = True
+    pool.spoil(keep.cuda())
+    N = first[-1] + tail
+    q = (2 * torch.randn(N, hkv * G, d, generator=gen(torch, seed + 3), device="cuda")).to(tdt(torch, dtype))
+    sk = torch.randn(hkv * G, generator=gen(torch, seed + 4), device="cuda") * 3 if sinks else None
+    masks = torch.tensor([signed(m) for x in lines for m, _ in x] + [0] * tail, dtype=torch.int64, device="cuda")
+    places = i32(torch, [p for x in lines for _, p in x] + [-1] * tail)
+    flags = i32(torch, [0])
+    call = lambda: sd.paged_tree_decode(  # noqa: E731
+        q, pool.pages, tables, i32(torch, ends), i32(torch, first), None if causal else masks,
+        places=None if causal else places, window=window, sinks=sk, flags=flags, out=torch.full_like(q, 7.0))
+    out, again = call(), call()
+    assert int(flags) == 0
+    assert torch.equal(out, again)
+    n = first[-1]
+    assert (out[n:] == 7.0).all()
+    ref, size = tree64(q[:n], pool, tables, held, lines, 1 / math.sqrt(d), window, sk)
+    check_tree(torch, out[:n], ref, size, dtype, uses_tiles(dtype, bits, counts, G))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tree_formats(cuda, dtype, bits, d):
+    run_tree(cuda, dtype, bits, d, 2, 4, 64, [300, 5, 0, 1000], [4, 2, 3, 1], seed=d + bits)
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("f32", 8)])
+@pytest.mark.parametrize("G", [1, 3, 5, 8, 16])
+def test_tree_head_groups(cuda, dtype, bits, G):
+    run_tree(cuda, dtype, bits, 128, 3, G, 32, [70, 259, 31], [7, 1, 13], seed=G)
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8), ("bf16", 4)])
+@pytest.mark.parametrize("nodes", [1, 2, 31, 32, 33, 63, 64])
+def test_tree_sizes(cuda, dtype, bits, nodes):
+    run_tree(cuda, dtype, bits, 64, 2, 4, 64, [513, 64, 0], [nodes, max(1, nodes // 2), nodes], seed=nodes)
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8)])
+def test_tree_of_a_chain_and_without_masks(cuda, dtype, bits):
+    run_tree(cuda, dtype, bits, 128, 2, 4, 64, [500, 0, 63], [9, 64, 20], chain=True, seed=3)
+    run_tree(cuda, dtype, bits, 128, 2, 4, 64, [500, 0, 63], [9, 64, 20], causal=True, seed=4)
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 4)])
+@pytest.mark.parametrize("window", [1, 2, 16, 64, 65, 200])
+def test_tree_windows_and_sinks(cuda, dtype, bits, window):
+    run_tree(cuda, dtype, bits, 64, 2, 4, 16, [400, 3, 150, 64, 0], [20, 12, 1, 64, 30], window=window,
+             sinks=window % 2 == 0, seed=window)
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("bf16", 8)])
+def test_tree_absent_nodes_and_rows_behind_the_last(cuda, dtype, bits):
+    run_tree(cuda, dtype, bits, 128, 2, 3, 64, [200, 0, 77], [30, 25, 40], absent=0.2, tail=5, seed=9)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dtype,bits,d", [("bf16", 0, 128), ("f16", 0, 64), ("bf16", 8, 128), ("f32", 0, 64), ("f16", 4, 64)])
+def test_tree_page_sizes(cuda, page, dtype, bits, d):
+    run_tree(cuda, dtype, bits, d, 2, 4, page, [page, 3 * page - 1, 700, 1], [16, 5, 33, 9], seed=page)
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 8), ("f32", 0)])
+def test_tree_long_split_over_all_ctas(cuda, dtype, bits):
+    run_tree(cuda, dtype, bits, 128, 2, 4, 64, [20000, 37], [33, 60], seed=1)
+    run_tree(cuda, dtype, bits, 128, 1, 8, 64, [9000], [12], seed=2)
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 4), ("f32", 0)])
+def test_tree_many_short_sequences(cuda, dtype, bits):
+    rng = random.Random(5)
+    run_tree(cuda, dtype, bits, 64, 2, 2, 16, [rng.randint(0, 90) for _ in range(300)], [rng.randint(0, 12) for _ in range(300)], seed=6)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("scale", [1e-3, 30.0])
+def test_tree_small_and_large_values(cuda, dtype, scale):
+    run_tree(cuda, dtype, 0, 128, 2, 4, 64, [700, 90], [33, 20], scale=scale, seed=7)
+
+
+def test_tree_hidden_nodes_do_not_reach_their_siblings(cuda):
+    """Two branches from one root: infinities and not-a-numbers in one branch's keys and values leave the other alone."""
+    import sparse_decode as sd
+    torch = cuda
+    for dtype in ("f32", "f16"):
+        pool = Pool(torch, sd, dtype, 0, 2, 64, 16, 8, 3)
+        tables, held = i32(torch, [[1, 4, 6, 2]]), 37
+        parents = [-1, 0, 0, 1, 2, 3]
+        masks = torch.tensor([m for m, _ in lineage(parents)], dtype=torch.int64, device="cuda")
+        q = torch.randn(6, 8, 64, generator=gen(torch, 4), device="cuda").to(tdt(torch, dtype))
+        call = lambda: sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [43]), i32(torch, [0, 6]), masks)  # noqa: E731
+        clean = call()
+        for a, x in zip(pool.arrays, (float("nan"), float("inf"))):
+            for node in (2, 4):
+                t = held + node
+                a[0][int(tables[0, t // 16]), :, t % 16, 5] = x
+        out = call()
+        for node in (0, 1, 3, 5):
+            assert torch.equal(out[node], clean[node])
+        assert not torch.isfinite(out[2]).any() and not torch.isfinite(out[4]).any()
+
+
+def test_tree_reports_sequences_that_cannot_be(cuda):
+    import sparse_decode as sd
+    torch = cuda
+    pool = Pool(torch, sd, "bf16", 0, 2, 64, 16, 40, 3)
+    good = tables_of(torch, [40, 40, 40, 40], 16, 40, 4)
+    q = torch.randn(200, 8, 64, generator=gen(torch, 4), device="cuda").bfloat16()
+    flags = i32(torch, [0])
+
+    def call(tables, lengths, first):
+        flags.zero_()
+        out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, lengths), i32(torch, first), flags=flags,
+                                   out=torch.full_like(q, 7.0))
+        return out, int(flags)
+    want, f = call(good, [40, 40, 40, 40], [0, 6, 12, 18, 24])
+    assert f == 0 and (want[24:] == 7).all()
+    # fewer tokens than nodes, more tokens than the table, more nodes than a mask has bits, rows outside the call
+    for lengths, first in (([40, 5, 40, 40], [0, 6, 12, 18, 24]), ([40, 49, 40, 40], [0, 6, 12, 18, 24]),
+                           ([40, -3, 40, 40], [0, 6, 12, 18, 24])):
+        out, f = call(good, lengths, first)
+        assert f == 2 and not out[6:12].any() and torch.equal(out[:6], want[:6]) and torch.equal(out[12:], want[12:])
+    out, f = call(good, [40, 47, 40, 40], [0, 6, 77, 78, 84])
+    assert f == 2 and not out[6:77].any() and torch.equal(out[:6], want[:6]) and (out[84:] == 7).all()
+    out, f = call(good, [40, 40, 40, 40], [0, 6, 12, 18, 300])
+    assert f == 2 and not out[18:].any() and torch.equal(out[:18], want[:18])
+    # pages out of range read as zeros
+    bad = good.clone()
+    bad[1, 1], bad[2, 2] = 99, -1
+    out, f = call(bad, [40, 40, 40, 40], [0, 6, 12, 18, 24])
+    assert f == 2 and torch.isfinite(out).all()
+    assert torch.equal(out[:6], want[:6]) and torch.equal(out[18:], want[18:])
