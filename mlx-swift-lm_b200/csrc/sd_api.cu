@@ -54,7 +54,7 @@ EncodeTiledFn encode_fn() {
 // its boxes, landing as [box][row][box bytes] in shared memory. One TMA
 // operation per tile rather than one per box: the SM's TMA unit spends a fixed
 // time on each operation, which dominates copies of a few KB.
-int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows) {
+int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const int box_bytes = std::min(row_bytes, 128);
@@ -64,7 +64,7 @@ int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, in
                                             : CU_TENSOR_MAP_SWIZZLE_32B;
   cuuint64_t dims[3] = {cuuint64_t(box_bytes), cuuint64_t(rows), cuuint64_t(nbox)};
   cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(box_bytes)};
-  cuuint32_t box[3] = {cuuint32_t(box_bytes), cuuint32_t(box_rows), cuuint32_t(nbox)};
+  cuuint32_t box[3] = {cuuint32_t(box_bytes), cuuint32_t(box_rows), cuuint32_t(whole ? nbox : 1)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -94,4 +94,25 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
   return paged_layout_of((2 * (batch + 1) + 2 * (kPagedThreads / 32) + 16) * 4, columns, D, dense_f32, stage_bytes);
 }
 
+// The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
+// of four warps, a loading warp and one that issues products.
+constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
+constexpr int kTreeTileThreads = 320;
+constexpr int kTreeTileTokens = 128;
+constexpr int kTreeTileStages = 16, kTreeTileLeast = 4;  // a step's K and V, and the next one's K beside them
+constexpr int kTreeTileBarBytes = 512;
+constexpr int kTreeTileSmem = 232448;
+// For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
+const void* tree_tile_kernel_for(int dtype, int D, bool shared);
+constexpr PagedLayout tree_tile_layout(int batch, int D) {
+  const int stage = 128 * D * 2, pre = (2 * (batch + 1) + 2 * (kTreeTileThreads / 32)) * 4, pre128 = (pre + 127) / 128 * 128;
+  const int room = (kTreeTileSmem - 1024 - 2 * stage - pre128 - kTreeTileBarBytes) / stage;
+  PagedLayout l{};
+  l.stages = room < kTreeTileStages ? room : kTreeTileStages;
+  l.prefix_off = (2 + l.stages) * stage;
+  l.bar_off = l.prefix_off + pre128;
+  l.bytes = l.bar_off + kTreeTileBarBytes + 1024;
+  return l;
+}
+
 }  // namespace sd

@@ -15,8 +15,9 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_fn();
 
-// Tensor map of `rows` rows of row_bytes at `base`, copied box_rows rows at a time.
-int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows);
+// Tensor map of `rows` rows of row_bytes at `base`, copied box_rows rows at a
+// time: whole rows, or 128 bytes of each.
+int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole = true);
 
 }  // namespace sd
 

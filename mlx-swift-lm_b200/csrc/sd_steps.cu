@@ -41,9 +41,14 @@ bool any_misaligned4(std::initializer_list<const void*> list) {
 
 // How a call is cut: by the rows of an average sequence, as the host knows no more.
 struct TreeShape {
-  TreeSet set;
+  const void* attend;
+  const void* merge;
+  int threads, smem_most;  // of attend
+  PagedLayout lay;
+  int tile, columns;  // tokens of a tile, columns of a pair
+  bool tiles;         // the tile kernel
   int ctas, halves;
-  int64_t pairs;  // at most
+  int64_t pairs;      // at most
   int part_floats;
   int64_t line_bytes, bytes;
 };
@@ -51,16 +56,36 @@ struct TreeShape {
 int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q_heads, TreeShape* s) {
   const int G = n_q_heads / g->n_kv_heads, D = g->head_dim;
   const int64_t columns = (int64_t(n_rows) + batch - 1) / batch * G;
-  s->set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
-  if (!s->set.attend) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
-  s->ctas = 2 * sms;
-  s->halves = 1;
-  const int RT = s->set.columns;
+  const TreeSet set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
+  if (!set.attend) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
+  s->merge = set.merge;
+  s->tiles = g->kv_bits == 0 && g->dtype != SD_F32 && columns > kTreeColumns;
+  if (s->tiles) {
+    const bool shared = columns > 128;
+    s->attend = tree_tile_kernel_for(g->dtype, D, shared);
+    s->threads = kTreeTileThreads;
+    s->smem_most = kTreeTileSmem;
+    s->lay = tree_tile_layout(batch, D);
+    s->tile = kTreeTileTokens;
+    s->columns = shared ? 256 : 128;
+    s->ctas = sms;
+    s->halves = shared ? 1 : 2;
+  } else {
+    s->attend = set.attend;
+    s->threads = kPagedThreads;
+    s->smem_most = kPagedSmem;
+    s->lay = tree_layout(batch, set.columns, D, g->dtype == SD_F32 && !g->kv_bits, set.stage_bytes);
+    s->tile = set.tile;
+    s->columns = set.columns;
+    s->ctas = 2 * sms;
+    s->halves = 1;
+  }
+  if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
   // a sequence's last pair may be almost empty; no more pairs than columns
-  s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / RT + batch);
-  s->part_floats = paged_part_floats(RT, D);
+  s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / s->columns + batch);
+  s->part_floats = paged_part_floats(s->columns, D);
   s->line_bytes = (int64_t(2) * (batch + 1) * 4 + 127) / 128 * 128;
   s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->halves * s->part_floats * 4;
   if (s->pairs + s->ctas >= (int64_t(1) << 30)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
@@ -182,21 +207,21 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   if (int32_t rc = tree_shape(g, batch, n_rows, n_q_heads, &s)) return rc;
   if (workspace_bytes < s.bytes)
     return fail(SD_ERR_CAPACITY, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)s.bytes);
-  const int D = g->head_dim, G = n_q_heads / g->n_kv_heads, RT = s.set.columns;
-  const int64_t max_tiles = (int64_t(table_width) * g->page_size + s.set.tile - 1) / s.set.tile + kSegmentUnits;
+  const int D = g->head_dim, G = n_q_heads / g->n_kv_heads;
+  const int64_t max_tiles = (int64_t(table_width) * g->page_size + s.tile - 1) / s.tile + kSegmentUnits;
   if (max_tiles * s.pairs >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "rows * table_width too large");
   const int64_t merge_warps = int64_t(n_rows) * g->n_kv_heads * ((G + kTreeHeads - 1) / kTreeHeads);
   const int per_block = kTreeMergeThreads / 32;
   if (merge_warps >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
 
   const int64_t rows = layer_rows(g) * layer;
-  const int rb = row_bytes(g), box = std::min(g->page_size, s.set.tile);
+  const int rb = row_bytes(g), box = std::min(g->page_size, s.tile);
   TreeParams p{};
   p.k_data = static_cast<uint8_t*>(at(g->k_data, rows * rb));
   p.v_data = static_cast<uint8_t*>(at(g->v_data, rows * rb));
   CUtensorMap tmK, tmV;
-  if (int32_t rc = encode_map(&tmK, const_cast<uint8_t*>(p.k_data), rb, layer_rows(g), box)) return rc;
-  if (int32_t rc = encode_map(&tmV, const_cast<uint8_t*>(p.v_data), rb, layer_rows(g), box)) return rc;
+  if (int32_t rc = encode_map(&tmK, const_cast<uint8_t*>(p.k_data), rb, layer_rows(g), box, !s.tiles)) return rc;
+  if (int32_t rc = encode_map(&tmV, const_cast<uint8_t*>(p.v_data), rb, layer_rows(g), box, !s.tiles)) return rc;
   p.q = q;
   p.out = out;
   p.line = static_cast<int*>(workspace);
@@ -223,28 +248,27 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.W = table_width;
   p.N = n_rows;
   p.window = window;
-  p.RT = RT;
+  p.RT = s.columns;
   p.halves = s.halves;
   p.part_floats = s.part_floats;
-  p.row_floats = D;
-  p.dim_floats = 4;
+  // a thread of the tile kernel holds a column: side by side, its warp's stores are whole lines
+  p.row_floats = s.tiles ? 4 : D;
+  p.dim_floats = s.tiles ? 4 * s.columns : 4;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.magic = 0x64006400u;
   p.flags = device_flags;
-  const PagedLayout lay = tree_layout(batch, RT, D, g->dtype == SD_F32 && !g->kv_bits, s.set.stage_bytes);
-  if (lay.stages < 1) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
-  p.stages = lay.stages;
-  p.q_off = lay.q_off;
-  p.buf_off = lay.buf_off;
-  p.prefix_off = lay.prefix_off;
-  p.bar_off = lay.bar_off;
+  p.stages = s.lay.stages;
+  p.q_off = s.lay.q_off;
+  p.buf_off = s.lay.buf_off;
+  p.prefix_off = s.lay.prefix_off;
+  p.bar_off = s.lay.bar_off;
   // no more CTAs than the line can have pieces of two units
   p.ncta = int(std::min<int64_t>(s.ctas, std::max<int64_t>(1, (max_tiles * s.pairs + 1) / 2)));
-  SD_CUDA(cudaFuncSetAttribute(s.set.attend, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem));
+  SD_CUDA(cudaFuncSetAttribute(s.attend, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem_most));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   void* args[3] = {&p, &tmK, &tmV};
-  if (int32_t rc = launch(s.set.attend, dim3(unsigned(p.ncta)), kPagedThreads, size_t(lay.bytes), st, args)) return rc;
-  return launch(s.set.merge, dim3(unsigned((merge_warps + per_block - 1) / per_block)), kTreeMergeThreads, 0, st, args);
+  if (int32_t rc = launch(s.attend, dim3(unsigned(p.ncta)), s.threads, size_t(s.lay.bytes), st, args)) return rc;
+  return launch(s.merge, dim3(unsigned((merge_warps + per_block - 1) / per_block)), kTreeMergeThreads, 0, st, args);
 }
 
 int32_t sd_paged_keep(const sd_pages* g, const int32_t* tables, int32_t batch, int32_t table_width,

@@ -3,7 +3,8 @@
 The library is compiled from mlx-swift-lm_b200/csrc: one object per storage
 format (sd_inst.cu and, for the paged cache, sd_paged_inst.cu and sd_tree_inst.cu,
 with SD_E/SD_BITS), the rotary and page-copy kernels (sd_rotary.cu), the plan
-and row kernels of drafted tokens (sd_draft.cu), plus the C ABI (sd_api.cu,
+and row kernels of drafted tokens (sd_draft.cu) and their attention's tile
+kernel (sd_tree_tile.cu), plus the C ABI (sd_api.cu,
 sd_pages.cu, sd_steps.cu). The CUDA runtime is linked statically, so the .so
 only needs the driver at run time.
 
@@ -82,6 +83,7 @@ def build(force: bool = False, verbose: bool = False, phase_timing: bool = False
                   _kernel_sources("sd_rotary.cu", tree | {"sd_decode.cuh", "sd_paged.cuh"})))
     units.append(("sd_draft.o", "sd_draft.cu", [],
                   _kernel_sources("sd_draft.cu", {"sd_tree.cuh", "sd_decode.cuh", "sd_paged.cuh"})))
+    units.append(("sd_tree_tile.o", "sd_tree_tile.cu", [], _kernel_sources("sd_tree_tile.cu", {"sd_decode.cuh"})))
     units += [(f"{n}.o", f"{n}.cu", [], _host_sources(f"{n}.cu")) for n in ("sd_api", "sd_pages", "sd_steps")]
     jobs = []
     for obj, src, extra, deps in units:
