@@ -202,7 +202,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     if (wait.dead) drain(bars->full, use, p.stages);  // what is under way lands in this CTA's shared memory
   } else if (warp == 9) {  // ---- products ----
-    uint32_t seg = 0, k[2] = {0, 0};  // segments; steps of each group, whose parities are those of its barriers
+    uint32_t seg[2] = {0, 0}, k[2] = {0, 0};  // segments and steps of each group: the parities of its barriers
     const uint32_t ring_a = smem_u32(ring);
     const uint32_t first_lane = lane == 0;
     while (walk.next(s)) {
@@ -224,10 +224,10 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
         __syncwarp();
       };
-      // both groups load their rows of Q in every segment, and have read what they need of the last one's S and O then
-      if (wait(bars->q_full, seg & 1u)) wait(bars->q_full + 1, seg & 1u);
-      scores(0);
-      if (n > 1) scores(1);
+      // A group with steps loads its rows of Q first, and has read what it needs of its last S and O then. One without
+      // (a segment of one tile) does not take part: it could run ahead of this wait by more than a phase.
+      for (int w = 0; w < min(n, 2); ++w, ++seg[w - 1])
+        if (wait(bars->q_full + w, seg[w] & 1u)) scores(w);
       for (int step = 0; step < n && !wait.dead; ++step) {
         const int w = step & 1, u = stage_of(step, 1);
         if (!wait(bars->p_full + w, k[w] & 1u) || !landed(u)) break;
@@ -249,7 +249,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         ++k[w];
       }
       it0 += nt;
-      ++seg;
     }
     if (first_lane) mma_commit(&bars->done);  // no product may read shared memory that is no longer this CTA's
     __syncwarp();
@@ -268,7 +267,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       const int t0 = sq.begin / kTileT;
       const int low = p.window && x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
       const int edge = __reduce_max_sync(0xffffffffu, low);
-      {  // Q: 16 bytes at a time, a row's chunks side by side
+      if (SHARED || s.i0 + w < s.i1) {  // Q: 16 bytes at a time, a row's chunks side by side
         constexpr int CPR = D / 8;
         const uint32_t q = smem_u32(qs) + w * kStage;
 #pragma unroll 4

@@ -439,6 +439,16 @@ def test_tree_many_short_sequences(cuda, dtype, bits):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("G,d", [(2, 64), (8, 128)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_tree_many_segments_per_cta(cuda, dtype, G, d, window):
+    """Short sequences, some of a single tile, several of them for every CTA."""
+    rng = random.Random(8)
+    run_tree(cuda, dtype, 0, d, 8, G, 32, [rng.choice([0, 20, 129, rng.randint(0, 700)]) for _ in range(120)],
+             [rng.randint(10, 40) for _ in range(120)], window=window, seed=9)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("scale", [1e-3, 30.0])
 def test_tree_small_and_large_values(cuda, dtype, scale):
     run_tree(cuda, dtype, 0, 128, 2, 4, 64, [700, 90], [33, 20], scale=scale, seed=7)
