@@ -65,9 +65,7 @@ struct TreeParams : PagedParams {
   int* line;               // [2][B + 1]: units and pairs before each sequence
   int N, Hq;
   int RT;                  // columns (node, query head) of a pair
-  int halves;              // segments of one pair and CTA
-  int part_floats;         // of one segment in the workspace
-  int row_floats, dim_floats;  // from one column to the next there, and from four dims to the next four
+  int part_floats;         // of one segment in the workspace: o [D / 4][RT][4], then (m, l) [RT]
 };
 
 struct TreeSet {
@@ -86,8 +84,8 @@ TreeSet tree_e0_b8(int D, int columns);
 TreeSet tree_e1_b8(int D, int columns);
 TreeSet tree_e2_b8(int D, int columns);
 
-constexpr int kTreeMergeThreads = 256;
-constexpr int kTreeHeads = 4;  // query heads of one merge warp
+constexpr int kTreeHeads = 4;    // query heads of one merge warp's share of the nodes
+constexpr int kTreeMergeCols = 8;  // columns of a merge block
 
 // Shared memory of an attend CTA: as a decode's, with two numbers per sequence and the columns' first tokens.
 constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
@@ -101,7 +99,7 @@ constexpr int kTreeTileThreads = 320;
 constexpr int kTreeTileTokens = 128;
 constexpr int kTreeTileStages = 16, kTreeTileLeast = 4;  // a step's K and V, and the next one's K beside them
 constexpr int kTreeTileBarBytes = 512;
-constexpr int kTreeTileSmem = 232448;
+constexpr int kTreeTileSmem = 232448 - 1024;  // beside 1 KB of static shared memory
 // For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
 const void* tree_tile_kernel_for(int dtype, int D, bool shared);
 constexpr PagedLayout tree_tile_layout(int batch, int D) {

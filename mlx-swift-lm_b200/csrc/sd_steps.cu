@@ -47,7 +47,7 @@ struct TreeShape {
   PagedLayout lay;
   int tile, columns;  // tokens of a tile, columns of a pair
   bool tiles;         // the tile kernel
-  int ctas, halves;
+  int ctas;
   int64_t pairs;      // at most
   int part_floats;
   int64_t line_bytes, bytes;
@@ -71,7 +71,6 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->tile = kTreeTileTokens;
     s->columns = shared ? 256 : 128;
     s->ctas = sms;
-    s->halves = shared ? 1 : 2;
   } else {
     s->attend = set.attend;
     s->threads = kPagedThreads;
@@ -80,14 +79,13 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->tile = set.tile;
     s->columns = set.columns;
     s->ctas = 2 * sms;
-    s->halves = 1;
   }
   if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
   // a sequence's last pair may be almost empty; no more pairs than columns
   s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / s->columns + batch);
   s->part_floats = paged_part_floats(s->columns, D);
   s->line_bytes = (int64_t(2) * (batch + 1) * 4 + 127) / 128 * 128;
-  s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->halves * s->part_floats * 4;
+  s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->part_floats * 4;
   if (s->pairs + s->ctas >= (int64_t(1) << 30)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
   return SD_OK;
 }
@@ -210,9 +208,9 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   const int D = g->head_dim, G = n_q_heads / g->n_kv_heads;
   const int64_t max_tiles = (int64_t(table_width) * g->page_size + s.tile - 1) / s.tile + kSegmentUnits;
   if (max_tiles * s.pairs >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "rows * table_width too large");
-  const int64_t merge_warps = int64_t(n_rows) * g->n_kv_heads * ((G + kTreeHeads - 1) / kTreeHeads);
-  const int per_block = kTreeMergeThreads / 32;
-  if (merge_warps >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
+  const int64_t columns = int64_t(n_rows) * G, blocks = (columns + kTreeMergeCols - 1) / kTreeMergeCols * g->n_kv_heads;
+  if (columns >= (int64_t(1) << 31) - kTreeMergeCols || blocks >= (int64_t(1) << 31))
+    return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
 
   const int64_t rows = layer_rows(g) * layer;
   const int rb = row_bytes(g), box = std::min(g->page_size, s.tile);
@@ -249,11 +247,7 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.N = n_rows;
   p.window = window;
   p.RT = s.columns;
-  p.halves = s.halves;
   p.part_floats = s.part_floats;
-  // a thread of the tile kernel holds a column: side by side, its warp's stores are whole lines
-  p.row_floats = s.tiles ? 4 : D;
-  p.dim_floats = s.tiles ? 4 * s.columns : 4;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.magic = 0x64006400u;
   p.flags = device_flags;
@@ -268,7 +262,7 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   void* args[3] = {&p, &tmK, &tmV};
   if (int32_t rc = launch(s.attend, dim3(unsigned(p.ncta)), s.threads, size_t(s.lay.bytes), st, args)) return rc;
-  return launch(s.merge, dim3(unsigned((merge_warps + per_block - 1) / per_block)), kTreeMergeThreads, 0, st, args);
+  return launch(s.merge, dim3(unsigned(blocks)), kTreeMergeCols * D / 4, 0, st, args);
 }
 
 int32_t sd_paged_keep(const sd_pages* g, const int32_t* tables, int32_t batch, int32_t table_width,

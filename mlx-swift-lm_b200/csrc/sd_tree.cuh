@@ -16,8 +16,8 @@
 //     head are cut into pairs of at most RT columns, and the pairs' tiles are one
 //     line that CTAs share equally, as in a decode (sd_paged.cuh). Every segment
 //     leaves (o, m, l) in the workspace.
-//   * tree_merge_kernel takes a row and four query heads per warp: it attends to
-//     the visible nodes one by one, reading no other node's rows -- what lies
+//   * tree_merge_kernel takes eight columns per block: it attends to their
+//     visible nodes one by one, reading no other node's rows -- what lies
 //     there, not-a-numbers included, does not reach it -- while the segments
 //     are still being worked on, and then joins those in CTA order.
 // Results depend on no timing. Lengths, rows and tables are read on the device
@@ -233,8 +233,9 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
     named_barrier(1, 32 * kPagedWarps);
     // the four warps' parts, in warp order
     float* part = tree_part(p, s.pair + blockIdx.x);
-    for (int k = tid; k < cols.n * (D / 4); k += 32 * kPagedWarps) {
-      const int g = k / (D / 4), d4 = k % (D / 4);
+    for (int k = tid; k < p.RT * (D / 4); k += 32 * kPagedWarps) {
+      const int d4 = k / p.RT, g = k - d4 * p.RT;
+      if (g >= cols.n) continue;
       float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
 #pragma unroll
       for (int w = 0; w < kPagedWarps; ++w) {
@@ -253,7 +254,7 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
         O.z = fmaf(f, x.z, O.z);
         O.w = fmaf(f, x.w, O.w);
       }
-      *reinterpret_cast<float4*>(part + g * p.row_floats + d4 * p.dim_floats) = O;
+      reinterpret_cast<float4*>(part)[k] = O;
       if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
     }
     named_barrier(1, 32 * kPagedWarps);
@@ -318,67 +319,75 @@ struct StoredPiece<E, 0, V> {
   }
 };
 
-// A warp per (row, up to four query heads of one kv head). Lane l holds
-// dimensions [l V, l V + V) of q, o and the rows; scores are summed over the
-// lanes by a butterfly that ends with head l / 8's in lane l, so that lane l
-// keeps token l % 8's of the eight that are taken at a time. Bound by latency:
-// a row sees some ten nodes, and their loads, eight together, hide behind the
-// attend kernel, as does everything before griddep_wait.
+// Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per
+// block. First the nodes: a warp takes up to four of the columns that are heads
+// of one row. Lane l holds dimensions [l V, l V + V) of q, o and the rows; scores
+// are summed over the lanes by a butterfly that ends with head l / 8's in lane
+// l, so that lane l keeps token l % 8's of the eight that are taken at a time.
+// Then, when the attend kernel is done, the segments: a thread has one column
+// and four dimensions, and eight segments' loads under way. Bound by latency.
 template <typename E, int BITS, int D>
-__global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const __grid_constant__ TreeParams p) {
-  constexpr int V = D / 32, HB = kTreeHeads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups;
-  const int64_t item = int64_t(blockIdx.x) * (kTreeMergeThreads / 32) + warp;
-  const int n = int(item / per);
-  int b = -1;
-  if (n < p.N && n < __ldcg(p.first + p.B)) {  // the last b with first[b] <= n: it has rows
-    b = 0;
-    int hi = p.B;
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if (__ldcg(p.first + mid) <= n) b = mid; else hi = mid;
-    }
-  }
-  if (b < 0) {  // rows behind the last sequence stay as they are
-    griddep_wait();
-    return;
-  }
-  const TreeSeq s = tree_seq(p, b);
-  const int hg = int(item - int64_t(n) * per), h = hg / groups, g0 = (hg - h * groups) * HB, heads = min(HB, p.G - g0);
-  const int node = n - s.row0;
-  const int64_t row0 = int64_t(n) * p.Hq + int64_t(h) * p.G + g0;  // of q and out
-  E* out = static_cast<E*>(p.out);
-  const bool mine = !s.bad && node >= 0 && node < s.n;
+__global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int V = D / 32, HB = kTreeHeads, NC = kTreeMergeCols, NW = NC * D / 128;
+  static_assert(NC == 8 && HB == 4, "at most eight rows in a block, one per warp of a head of 128");
+  __shared__ float4 node_o[D / 4][NC];
+  __shared__ float2 node_ml[NC];
+  __shared__ int seq_of[NC];  // of each column; -1: behind the last, -2: gives zeros
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int blocks = (p.N * p.G + NC - 1) / NC, h = blockIdx.x / blocks, x0 = (blockIdx.x - h * blocks) * NC;
+  const int x1 = min(x0 + NC, p.N * p.G);
+  const E* qp = static_cast<const E*>(p.q);
+  const int rows_end = __ldcg(p.first + p.B);
 
-  float q[HB][V], o[HB][V], m[HB], l[HB];
-#pragma unroll
-  for (int g = 0; g < HB; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) q[g][i] = o[g][i] = 0.0f;
-    if (mine && g < heads) load_elements<E, V>(static_cast<const E*>(p.q) + (row0 + g) * D + lane * V, q[g]);
-  }
-  if (mine) {
-    uint64_t seen = p.masks ? uint64_t(__ldcg(reinterpret_cast<const long long*>(p.masks) + n)) : (uint64_t(2) << node) - 1;
-    if (s.n < 64) seen &= (uint64_t(1) << s.n) - 1;
-    // lane j: rows of nodes j and j + 32
-    int at[2];
-    const int64_t place = p.window ? (p.places ? int64_t(__ldcg(p.places + n)) : int64_t(s.held) + node) - p.window : 0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int j = lane + 32 * e;
-      bool see = (seen >> j) & 1;
-      if (see && p.window) see = (p.places ? __ldcg(p.places + s.row0 + j) : s.held + j) > place;
-      at[e] = -1;
-      if (see) {
-        const int t = s.held + j, page = __ldcg(p.tables + int64_t(b) * p.W + t / p.P);
-        if (page >= 0 && page < p.n_pages) at[e] = (page * p.Hkv + h) * p.P + (t & (p.P - 1));
-        else if (p.flags) atomicOr(p.flags, kErrBadIndex);
+  // items: the rows of [x0, x1), up to HB of their heads each; at most NC of them
+  int item = 0;
+  for (int a = x0; a < x1; ++item) {
+    const int n = a / p.G, g0 = a - n * p.G, heads = min(min(HB, p.G - g0), x1 - a), c0 = a - x0;
+    a += heads;
+    if (item % NW != warp) continue;
+    int b = -1;
+    if (n < rows_end) {  // the last b with first[b] <= n: it has rows
+      b = 0;
+      int hi = p.B;
+      while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (__ldcg(p.first + mid) <= n) b = mid; else hi = mid;
       }
-      const unsigned v = __ballot_sync(0xffffffffu, see);
-      seen = e ? (seen & 0xffffffffull) | (uint64_t(v) << 32) : (seen & ~0xffffffffull) | v;
+    }
+    TreeSeq s{};
+    if (b >= 0) s = tree_seq(p, b);
+    const int node = n - s.row0;
+    const bool mine = b >= 0 && !s.bad && node >= 0 && node < s.n;
+    if (lane < heads) seq_of[c0 + lane] = b < 0 ? -1 : mine ? b : -2;
+    float q[HB][V], o[HB][V], m[HB], l[HB];
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) q[g][i] = o[g][i] = 0.0f;
+      if (mine && g < heads)
+        load_elements<E, V>(qp + (int64_t(n) * p.Hq + int64_t(h) * p.G + g0 + g) * D + lane * V, q[g]);
+    }
+    uint64_t seen = 0;
+    int at[2] = {-1, -1};  // rows of nodes lane and lane + 32
+    if (mine) {
+      seen = p.masks ? uint64_t(__ldcg(reinterpret_cast<const long long*>(p.masks) + n)) : (uint64_t(2) << node) - 1;
+      if (s.n < 64) seen &= (uint64_t(1) << s.n) - 1;
+      const int64_t place = p.window ? (p.places ? int64_t(__ldcg(p.places + n)) : int64_t(s.held) + node) - p.window : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = lane + 32 * e;
+        bool see = (seen >> j) & 1;
+        if (see && p.window) see = (p.places ? __ldcg(p.places + s.row0 + j) : s.held + j) > place;
+        if (see) {
+          const int t = s.held + j, page = __ldcg(p.tables + int64_t(b) * p.W + t / p.P);
+          if (page >= 0 && page < p.n_pages) at[e] = (page * p.Hkv + h) * p.P + (t & (p.P - 1));
+          else if (p.flags) atomicOr(p.flags, kErrBadIndex);
+        }
+        const unsigned v = __ballot_sync(0xffffffffu, see);
+        seen = e ? (seen & 0xffffffffull) | (uint64_t(v) << 32) : (seen & ~0xffffffffull) | v;
+      }
     }
 #pragma unroll 1
     while (seen) {
@@ -403,29 +412,29 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const __g
       float sc = -INFINITY;  // of head lane / 8 and token lane % 8
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        float a[HB] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float a4[HB] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (ok[t]) {
           float f[V];
           kp[t].get(f);
 #pragma unroll
           for (int g = 0; g < HB; ++g)
 #pragma unroll
-            for (int i = 0; i < V; ++i) a[g] = fmaf(q[g][i], f[i], a[g]);
+            for (int i = 0; i < V; ++i) a4[g] = fmaf(q[g][i], f[i], a4[g]);
         }
         const bool b4 = lane & 16, b3 = lane & 8;
-        float x0 = b4 ? a[2] : a[0], x1 = b4 ? a[3] : a[1];
-        x0 += __shfl_xor_sync(0xffffffffu, b4 ? a[0] : a[2], 16);
-        x1 += __shfl_xor_sync(0xffffffffu, b4 ? a[1] : a[3], 16);
-        float x = b3 ? x1 : x0;
-        x += __shfl_xor_sync(0xffffffffu, b3 ? x0 : x1, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 4);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        if (t < cnt && (lane & 7) == t) sc = x * p.scale_log2;
+        float y0 = b4 ? a4[2] : a4[0], y1 = b4 ? a4[3] : a4[1];
+        y0 += __shfl_xor_sync(0xffffffffu, b4 ? a4[0] : a4[2], 16);
+        y1 += __shfl_xor_sync(0xffffffffu, b4 ? a4[1] : a4[3], 16);
+        float y = b3 ? y1 : y0;
+        y += __shfl_xor_sync(0xffffffffu, b3 ? y0 : y1, 8);
+        y += __shfl_xor_sync(0xffffffffu, y, 4);
+        y += __shfl_xor_sync(0xffffffffu, y, 2);
+        y += __shfl_xor_sync(0xffffffffu, y, 1);
+        if (t < cnt && (lane & 7) == t) sc = y * p.scale_log2;
       }
       float mx = sc;
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      for (int i = 1; i < 8; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
       float w = 0.0f;
 #pragma unroll
       for (int g = 0; g < HB; ++g) {
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const __g
       if ((lane & 7) >= cnt) w = 0.0f;
       float sum = w;
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      for (int i = 1; i < 8; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
 #pragma unroll
       for (int g = 0; g < HB; ++g) l[g] += __shfl_sync(0xffffffffu, sum, 8 * g);
 #pragma unroll
@@ -455,82 +464,70 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const __g
         }
       }
     }
-  }
-
-  griddep_wait();
-  if (mine && s.held > s.begin) {
-    const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
-    const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
-    const int rt = np / p.Hkv, nu = (u1 - up) / np;
-    const Pieces pieces(p, all);
-    int at[HB], c0[HB], ns[HB], most = 0;  // column of its pair; pair + first CTA; segments
-    float2 ml[HB];
 #pragma unroll
     for (int g = 0; g < HB; ++g) {
-      const int x = node * p.G + g0 + min(g, heads - 1), c = x / p.RT, k = h * rt + c;
-      at[g] = x - c * p.RT;
-      const int a = up + k * nu, first = pieces.of(a + kSegmentUnits), last = pieces.of(a + nu - 1);
-      c0[g] = pp + k + first;
-      ns[g] = (last - first + 1) * p.halves;
-      most = max(most, ns[g]);
-      c0[g] *= p.halves;
+      if (g < heads) {
+        float* to = reinterpret_cast<float*>(&node_o[lane * V / 4][c0 + g]) + lane * V % 4;
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = o[g][i];
+        if (lane == 0) node_ml[c0 + g] = make_float2(m[g], l[g]);
+      }
     }
-    for (int base = 0; base < most; base += 32) {
+  }
+  __syncthreads();
+  const int col = tid % NC, d4 = tid / NC, x = x0 + col;
+  const int b = x < x1 ? seq_of[col] : -1;
+  griddep_wait();
+  if (b == -1) return;  // rows behind the last sequence stay as they are
+  float M = -INFINITY, L = 0.0f;
+  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int n = x / p.G, g = x - n * p.G;
+  if (b >= 0) {
+    M = node_ml[col].x, L = node_ml[col].y, O = node_o[d4][col];
+    const TreeSeq s = tree_seq(p, b);
+    if (s.held > s.begin) {
+      const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
+      const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
+      const int nu = (u1 - up) / np, y = (n - s.row0) * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;
+      const Pieces pieces(p, all);
+      const int a = up + k * nu, cta = pieces.of(a + kSegmentUnits), ns = pieces.of(a + nu - 1) - cta + 1;
+      const float* part = tree_part(p, pp + k + cta);
+#pragma unroll 1
+      for (int j0 = 0; j0 < ns; j0 += 8) {
+        float2 ml[8];
+        float4 v[8];
 #pragma unroll
-      for (int g = 0; g < HB; ++g) {
-        ml[g] = make_float2(-INFINITY, 0.0f);
-        if (base + lane < ns[g])
-          ml[g] = __ldcg(reinterpret_cast<const float2*>(tree_part(p, c0[g] + base + lane) + p.RT * D + 2 * at[g]));
-      }
-      float f[HB];
-#pragma unroll
-      for (int g = 0; g < HB; ++g) {
-        const float f0 = raise_max(m[g], warp_max(ml[g].x));
-        f[g] = exp2_from(ml[g].x, m[g]);
-        l[g] = fmaf(l[g], f0, warp_sum(f[g] * ml[g].y));
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[g][i] *= f0;
-      }
-#pragma unroll 4
-      for (int j = 0; j < min(32, most - base); ++j) {
-#pragma unroll
-        for (int g = 0; g < HB; ++g) {
-          const float w = __shfl_sync(0xffffffffu, f[g], j);
-          if (base + j < ns[g]) {
-            const float* x = tree_part(p, c0[g] + base + j) + at[g] * p.row_floats + lane * V / 4 * p.dim_floats + lane * V % 4;
-            if constexpr (V == 4) {
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(x));
-              o[g][0] = fmaf(w, y.x, o[g][0]);
-              o[g][1] = fmaf(w, y.y, o[g][1]);
-              o[g][2] = fmaf(w, y.z, o[g][2]);
-              o[g][3] = fmaf(w, y.w, o[g][3]);
-            } else {
-              const float2 y = __ldcg(reinterpret_cast<const float2*>(x));
-              o[g][0] = fmaf(w, y.x, o[g][0]);
-              o[g][1] = fmaf(w, y.y, o[g][1]);
-            }
+        for (int j = 0; j < 8; ++j) {
+          ml[j] = make_float2(-INFINITY, 0.0f);
+          v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (j0 + j < ns) {
+            const float* from = part + int64_t(j0 + j) * p.part_floats;
+            ml[j] = __ldcg(reinterpret_cast<const float2*>(from + p.RT * D) + at);
+            v[j] = __ldcg(reinterpret_cast<const float4*>(from) + d4 * p.RT + at);
           }
+        }
+        float top = ml[0].x;
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, ml[j].x);
+        const float f = raise_max(M, top);
+        L *= f;
+        O.x *= f, O.y *= f, O.z *= f, O.w *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = exp2_from(ml[j].x, M);
+          L = fmaf(w, ml[j].y, L);
+          O.x = fmaf(w, v[j].x, O.x), O.y = fmaf(w, v[j].y, O.y);
+          O.z = fmaf(w, v[j].z, O.z), O.w = fmaf(w, v[j].w, O.w);
         }
       }
     }
   }
-#pragma unroll
-  for (int g = 0; g < HB; ++g) {
-    if (g < heads) {
-      float L = l[g];
-      if (p.sinks) L += exp2f(fmaf(__ldcg(p.sinks + h * p.G + g0 + g), 1.4426950408889634f, -(m[g] == -INFINITY ? 0.0f : m[g])));
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      E* at = out + (row0 + g) * D + lane * V;
-      if constexpr (sizeof(E) == 4) {
-#pragma unroll
-        for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(at + i) = make_float2(o[g][i] * inv, o[g][i + 1] * inv);
-      } else if constexpr (V == 4) {
-        *reinterpret_cast<uint2*>(at) = make_uint2(pack2<E>(o[g][0] * inv, o[g][1] * inv), pack2<E>(o[g][2] * inv, o[g][3] * inv));
-      } else {
-        *reinterpret_cast<uint32_t*>(at) = pack2<E>(o[g][0] * inv, o[g][1] * inv);
-      }
-    }
-  }
+  const int64_t row = int64_t(n) * p.Hq + int64_t(h) * p.G + g;
+  if (p.sinks) L += exp2f(fmaf(__ldcg(p.sinks + h * p.G + g), 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  E* out = static_cast<E*>(p.out) + row * D + 4 * d4;
+  if constexpr (sizeof(E) == 4) *reinterpret_cast<float4*>(out) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<E>(O.x * inv, O.y * inv), pack2<E>(O.z * inv, O.w * inv));
 }
 
 }  // namespace sd

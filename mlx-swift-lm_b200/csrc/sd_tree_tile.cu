@@ -12,7 +12,7 @@
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
-//     groups in turn (each leaves a segment of its own in the workspace).
+//     groups in turn, whose parts are joined at a segment's end.
 // P is one value of the element type: 128 x 128 products cost as much as their
 // exponentials, and a second half would cost as much again (SHARED). The sum
 // that O is divided by is made of the rounded values, so their errors cancel
@@ -63,7 +63,6 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define SD_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
@@ -75,6 +74,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
       "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : SD_R8(v, 0), SD_R8(v, 8), SD_R8(v, 16), SD_R8(v, 24)
       : "r"(addr));
+}
+// The loads before are done; the operands keep what uses v behind it.
+#define SD_U8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tmem_wait(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : SD_U8(v, 0), SD_U8(v, 8), SD_U8(v, 16), SD_U8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+               SD_W8(v, 0), SD_W8(v, 8)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
   asm volatile(
@@ -115,6 +124,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   TileBars* bars = reinterpret_cast<TileBars*>(sm + p.bar_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
+  __shared__ float2 other[SHARED ? 1 : 128];  // (m, l) of the second group
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -200,7 +210,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
       }
     }
-    if (wait.dead) drain(bars->full, use, p.stages);  // what is under way lands in this CTA's shared memory
+    if (wait.dead)  // what is under way lands in this CTA's shared memory
+      for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
   } else if (warp == 9) {  // ---- products ----
     uint32_t seg[2] = {0, 0}, k[2] = {0, 0};  // segments and steps of each group: the parities of its barriers
     const uint32_t ring_a = smem_u32(ring);
@@ -288,24 +299,43 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.held - tok;
         if (!wait(bars->s_full + w, k & 1u)) continue;
         tc_fence_after();
-        uint32_t v[128];
+        // The row's scores, 32 at a time, twice: for the maximum and for the weights. All 128 in registers would spill.
+        const bool some = lo > 0 || hi < kTileT || tok < edge;  // some may not be seen
+        const int from = max(lo, low - tok);
+        auto as_seen = [&](uint32_t (&v)[32], int c) {
+          if (neg) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, v + 32 * c);
-        tc_wait_ld();
-        float* f = reinterpret_cast<float*>(v);
-        if (neg) {
+            for (int j = 0; j < 32; ++j) v[j] ^= 0x80000000u;
+          }
+          if (some) {
 #pragma unroll
-          for (int j = 0; j < 128; ++j) f[j] = -f[j];
-        }
-        if (lo > 0 || hi < kTileT || tok < edge) {
-          const int from = max(lo, low - tok);
+            for (int j = 0; j < 32; ++j) v[j] = 32 * c + j < from || 32 * c + j >= hi ? 0xff800000u : v[j];
+          }
+        };
+        uint32_t va[32], vb[32];
+        float mx[2] = {-INFINITY, -INFINITY};
+        auto most = [&](uint32_t (&v)[32], int c) {
+          as_seen(v, c);
 #pragma unroll
-          for (int j = 0; j < 128; ++j) f[j] = j < from || j >= hi ? -INFINITY : f[j];
-        }
-        float mx[4] = {f[0], f[1], f[2], f[3]};
-#pragma unroll
-        for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+          for (int j = 0; j < 32; j += 2) {
+            mx[0] = fmaxf(mx[0], __uint_as_float(v[j]));
+            mx[1] = fmaxf(mx[1], __uint_as_float(v[j + 1]));
+          }
+        };
+        tmem_ld32(ts, va);
+        tmem_wait(va);
+        tmem_ld32(ts + 32, vb);
+        most(va, 0);
+        tmem_wait(vb);
+        tmem_ld32(ts + 64, va);
+        most(vb, 1);
+        tmem_wait(va);
+        tmem_ld32(ts + 96, vb);
+        most(va, 2);
+        tmem_wait(vb);
+        tmem_ld32(ts, va);
+        most(vb, 3);
+        const float top = fmaxf(mx[0], mx[1]) * sc;
         if (steps == 0) {
           m = top - kUp;
         } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
@@ -315,29 +345,41 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(to + 32 * c, o);
-              tc_wait_ld();
+              tmem_ld32(to + 32 * c, vb);
+              tmem_wait(vb);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fac);
-              tmem_st32(to + 32 * c, o);
+              for (int j = 0; j < 32; ++j) vb[j] = __float_as_uint(__uint_as_float(vb[j]) * fac);
+              tmem_st32(to + 32 * c, vb);
             }
           }
         }
         const float mm = m == -INFINITY ? 0.0f : m;
         float sum[2] = {0.0f, 0.0f};
+        auto weigh = [&](uint32_t (&v)[32], int c) {  // P takes the place of scores that have been read
+          as_seen(v, c);
+          uint32_t two[16];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          const uint32_t two = pack2<E>(ex2(fmaf(f[2 * j], sc, -mm)), ex2(fmaf(f[2 * j + 1], sc, -mm)));
-          float g[2];
-          unpack_word<E>(two, g);
-          sum[0] += g[0];
-          sum[1] += g[1];
-          v[j] = two;
-        }
+          for (int j = 0; j < 16; ++j) {
+            two[j] = pack2<E>(ex2(fmaf(__uint_as_float(v[2 * j]), sc, -mm)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), sc, -mm)));
+            float g[2];
+            unpack_word<E>(two[j], g);
+            sum[0] += g[0];
+            sum[1] += g[1];
+          }
+          tmem_st16(ts + 16 * c, two);
+        };
+        tmem_wait(va);
+        tmem_ld32(ts + 32, vb);
+        weigh(va, 0);
+        tmem_wait(vb);
+        tmem_ld32(ts + 64, va);
+        weigh(vb, 1);
+        tmem_wait(va);
+        tmem_ld32(ts + 96, vb);
+        weigh(va, 2);
+        tmem_wait(vb);
+        weigh(vb, 3);
         l += sum[0] + sum[1];
-        tmem_st32(ts, v);
-        tmem_st32(ts + 32, v + 32);
         if ((lo > 0 || hi < kTileT) && (!SHARED || w == 0)) {
           const int u = 2 * (it0 + i - s.i0) + 1;
           if (wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
@@ -356,26 +398,65 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
-      float* part = tree_part(p, (s.pair + int(blockIdx.x)) * (SHARED ? 1 : 2) + (SHARED ? 0 : w));
+      float* part = tree_part(p, s.pair + int(blockIdx.x));
       if (steps > 0 && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();
+      const bool has = steps > 0 && !wait.dead;
+      float4* swap = reinterpret_cast<float4*>(qs);  // [D / 4][128]: no score of this segment is still to come
+      float f0 = 1.0f, f1 = 0.0f;
+      if constexpr (!SHARED) {
+        // the second group's part goes to the first through shared memory
+        named_barrier(1, 256);
+        if (w == 1) {
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (steps > 0 && !wait.dead) {
-          tmem_ld32(to + 32 * c, o);
-          tc_wait_ld();
-        } else {
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (has) {
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait(o);
+            }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0;
+            for (int j = 0; j < 8; ++j)
+              swap[(8 * c + j) * 128 + r] = has ? make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                                              __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]))
+                                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          other[r] = make_float2(m, l);
         }
-        if (x < cols.n) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(part + (8 * c + j) * p.dim_floats + x * p.row_floats) =
-                make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        named_barrier(1, 256);
+        if (w == 0) {
+          const float2 ml = other[r];
+          const float top = fmaxf(m, ml.x);
+          f0 = exp2_from(m, top), f1 = exp2_from(ml.x, top);
+          m = top;
+          l = fmaf(f1, ml.y, l * f0);
         }
       }
-      if (x < cols.n) *reinterpret_cast<float2*>(part + p.RT * D + 2 * x) = make_float2(m, l);
+      if (SHARED || w == 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (has) {
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait(o);
+          }
+          if (x < cols.n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float4 y = has ? make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                           __uint_as_float(o[4 * j + 3]))
+                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if constexpr (!SHARED) {
+                const float4 z = swap[(8 * c + j) * 128 + r];
+                y.x = fmaf(f1, z.x, f0 * y.x), y.y = fmaf(f1, z.y, f0 * y.y);
+                y.z = fmaf(f1, z.z, f0 * y.z), y.w = fmaf(f1, z.w, f0 * y.w);
+              }
+              reinterpret_cast<float4*>(part)[(8 * c + j) * p.RT + x] = y;
+            }
+          }
+        }
+        if (x < cols.n) *reinterpret_cast<float2*>(part + p.RT * D + 2 * x) = make_float2(m, l);
+      }
+      if constexpr (!SHARED) named_barrier(1, 256);  // before the next rows of Q
     }
     tc_fence_before();
   }
