@@ -3,6 +3,8 @@
 // host and device code.
 #pragma once
 
+#include <cuda_runtime.h>
+
 #include "sd_paged.h"
 
 namespace sd {
@@ -66,11 +68,14 @@ struct TreeParams : PagedParams {
   int N, Hq;
   int RT;                  // columns (node, query head) of a pair
   int part_floats;         // of one segment in the workspace: o [D / 4][RT][4], then (m, l) [RT]
+  float* node_o;           // [N * Hq][D], of the nodes alone
+  float2* node_ml;         // [N * Hq]
+  FastDiv by_g;            // G
 };
 
 struct TreeSet {
   const void* attend;  // tree_attend_kernel<E, BITS, D, blocks of columns>(TreeParams, CUtensorMap, CUtensorMap)
-  const void* merge;   // tree_merge_kernel<E, BITS, D>(TreeParams)
+  const void* merge;   // tree_merge_kernel<E, D>(TreeParams)
   int tile, stage_bytes, columns;
 };
 // For at most `columns` columns a pair, or as many as there are.
@@ -84,22 +89,23 @@ TreeSet tree_e0_b8(int D, int columns);
 TreeSet tree_e1_b8(int D, int columns);
 TreeSet tree_e2_b8(int D, int columns);
 
-constexpr int kTreeHeads = 4;    // query heads of one merge warp's share of the nodes
+constexpr int kTreeHeads = 4;      // query heads that a warp takes to the nodes at once
+constexpr int kTreeAttendThreads = kPagedThreads + 32;  // a decode's, and a warp for the nodes
 constexpr int kTreeMergeCols = 8;  // columns of a merge block
 
 // Shared memory of an attend CTA: as a decode's, with two numbers per sequence and the columns' first tokens.
 constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
-  return paged_layout_of((2 * (batch + 1) + 2 * (kPagedThreads / 32) + 16) * 4, columns, D, dense_f32, stage_bytes);
+  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 16) * 4, columns, D, dense_f32, stage_bytes);
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
-// of four warps, a loading warp and one that issues products.
+// of four warps, a loading warp, one that issues products and two for the nodes.
 constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
-constexpr int kTreeTileThreads = 320;
+constexpr int kTreeTileThreads = 384;
 constexpr int kTreeTileTokens = 128;
 constexpr int kTreeTileStages = 16, kTreeTileLeast = 4;  // a step's K and V, and the next one's K beside them
 constexpr int kTreeTileBarBytes = 512;
-constexpr int kTreeTileSmem = 232448 - 1024;  // beside 1 KB of static shared memory
+constexpr int kTreeTileSmem = 232448 - 2048;  // beside 2 KB of static shared memory
 // For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
 const void* tree_tile_kernel_for(int dtype, int D, bool shared);
 constexpr PagedLayout tree_tile_layout(int batch, int D) {

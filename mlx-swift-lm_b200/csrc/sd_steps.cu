@@ -50,7 +50,7 @@ struct TreeShape {
   int ctas;
   int64_t pairs;      // at most
   int part_floats;
-  int64_t line_bytes, bytes;
+  int64_t line_bytes, node_bytes, bytes;  // of the workspace: line, segments, the nodes' (m, l) and o
 };
 
 int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q_heads, TreeShape* s) {
@@ -73,7 +73,7 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->ctas = sms;
   } else {
     s->attend = set.attend;
-    s->threads = kPagedThreads;
+    s->threads = kTreeAttendThreads;
     s->smem_most = kPagedSmem;
     s->lay = tree_layout(batch, set.columns, D, g->dtype == SD_F32 && !g->kv_bits, set.stage_bytes);
     s->tile = set.tile;
@@ -85,7 +85,9 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / s->columns + batch);
   s->part_floats = paged_part_floats(s->columns, D);
   s->line_bytes = (int64_t(2) * (batch + 1) * 4 + 127) / 128 * 128;
-  s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->part_floats * 4;
+  const int64_t all = int64_t(n_rows) * n_q_heads;
+  s->node_bytes = (all * 8 + 127) / 128 * 128 + all * D * 4;
+  s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->part_floats * 4 + s->node_bytes;
   if (s->pairs + s->ctas >= (int64_t(1) << 30)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
   return SD_OK;
 }
@@ -224,6 +226,9 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.out = out;
   p.line = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.line_bytes);
+  p.node_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.bytes - s.node_bytes);
+  p.node_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.bytes - int64_t(n_rows) * n_q_heads * D * 4);
+  p.by_g.set(G);
   p.tables = tables;
   p.lengths = lengths;
   p.first = first;
@@ -256,8 +261,7 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.buf_off = s.lay.buf_off;
   p.prefix_off = s.lay.prefix_off;
   p.bar_off = s.lay.bar_off;
-  // no more CTAs than the line can have pieces of two units
-  p.ncta = int(std::min<int64_t>(s.ctas, std::max<int64_t>(1, (max_tiles * s.pairs + 1) / 2)));
+  p.ncta = s.ctas;
   SD_CUDA(cudaFuncSetAttribute(s.attend, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem_most));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   void* args[3] = {&p, &tmK, &tmV};

@@ -11,15 +11,16 @@
 // The held tokens are the same for all nodes (but for the low end of a window),
 // the nodes are few and differ from row to row. So the work is in two parts that
 // know nothing of each other:
-//   * tree_attend_kernel (or the tile kernel, sd_tree_tile.cu) attends to the
-//     held tokens with no mask at all. The (node, query head) columns of a kv
-//     head are cut into pairs of at most RT columns, and the pairs' tiles are one
-//     line that CTAs share equally, as in a decode (sd_paged.cuh). Every segment
-//     leaves (o, m, l) in the workspace.
-//   * tree_merge_kernel takes eight columns per block: it attends to their
-//     visible nodes one by one, reading no other node's rows -- what lies
-//     there, not-a-numbers included, does not reach it -- while the segments
-//     are still being worked on, and then joins those in CTA order.
+//   * The held tokens: the (node, query head) columns of a kv head are cut into
+//     pairs of at most RT columns, and the pairs' tiles are one line that CTAs
+//     share equally, as in a decode (sd_paged.cuh). Every segment leaves (o, m, l)
+//     in the workspace. No mask at all.
+//   * The nodes: a warp that a CTA has for it takes a row and up to four query
+//     heads at a time and attends to the visible nodes alone, reading no other
+//     node's rows -- what lies there, not-a-numbers included, does not reach it.
+//     It runs beside the tiles' warps, whose time hides its chain of loads.
+// tree_attend_kernel and the tile kernel (sd_tree_tile.cu) do both, and
+// tree_merge_kernel joins a column's nodes and segments in CTA order.
 // Results depend on no timing. Lengths, rows and tables are read on the device
 // only, so a captured graph serves growing sequences.
 #pragma once
@@ -46,6 +47,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
   s.begin = p.window > 0 && s.held >= p.window ? s.held - p.window + 1 : 0;
   return s;
 }
+// The sequence of row n < first[B]: the last b with first[b] <= n, which has rows.
+__device__ __forceinline__ int tree_find(const TreeParams& p, int n) {
+  int b = 0, hi = p.B;
+  while (hi - b > 1) {
+    const int mid = (b + hi) >> 1;
+    if (__ldcg(p.first + mid) <= n) b = mid; else hi = mid;
+  }
+  return b;
+}
 // The held tokens of sequence b, for the producer.
 __device__ __forceinline__ TokenRange token_range(const TreeParams& p, int b) {
   const TreeSeq s = tree_seq(p, b);
@@ -71,6 +81,8 @@ __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* un
     const TreeSeq s = tree_seq(p, b);
     const int np = tree_pairs(p, s), nu = units_of({s.begin, s.held}, tile);
     bad = bad || s.bad;
+    units[b + 1] = np * nu;  // of the sequence, for now
+    pairs[b + 1] = np;
     k += np;
     u += np * nu;
   }
@@ -87,18 +99,12 @@ __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* un
   for (int w = 0; w < warp; ++w) u += tmp[2 * w], k += tmp[2 * w + 1];
   if (tid == 0) units[0] = pairs[0] = 0;
   for (int b = b0; b < b1; ++b) {
-    const TreeSeq s = tree_seq(p, b);
-    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.held}, tile);
-    units[b + 1] = u += np * nu;
-    pairs[b + 1] = k += np;
+    u += units[b + 1], k += pairs[b + 1];
+    units[b + 1] = u, pairs[b + 1] = k;
+    if (blockIdx.x == 0) p.line[b + 1] = u, p.line[p.B + 2 + b] = k;  // for the merge
   }
+  if (blockIdx.x == 0 && tid == 0) p.line[0] = p.line[p.B + 1] = 0;
   __syncthreads();
-  if (blockIdx.x == 0) {  // for the merge
-    for (int b = tid; b <= p.B; b += NT) {
-      p.line[b] = units[b];
-      p.line[p.B + 1 + b] = pairs[b];
-    }
-  }
 }
 
 struct TreeSegment {
@@ -141,129 +147,26 @@ struct TreeWalk {
 // The columns of a pair: x0 + i is (node, query head of the kv head) number x0 + i of the sequence.
 struct NodeCols {
   static constexpr bool kLow = true;
-  int n, x0, G, Hq;
-  int64_t row0;  // of column x0
+  int n, x0, Hq;
+  int64_t base, row0;  // of the sequence's first column, of column x0
+  FastDiv by_g;
   __device__ __forceinline__ NodeCols(const TreeParams& p, const TreeSeq& s, int h, int c)
-      : n(min(p.RT, s.n * p.G - c * p.RT)), x0(c * p.RT), G(p.G), Hq(p.Hq) {
+      : n(min(p.RT, s.n * p.G - c * p.RT)), x0(c * p.RT), Hq(p.Hq), by_g(p.by_g) {
     base = int64_t(s.row0) * p.Hq + int64_t(h) * p.G;
     row0 = row(0);
   }
-  __device__ __forceinline__ int node(int i) const { return (x0 + i) / G; }
+  __device__ __forceinline__ int node(int i) const { return by_g(x0 + i); }
   __device__ __forceinline__ int64_t row(int i) const {
     const int nd = node(i);
-    return base + int64_t(nd) * Hq + (x0 + i - nd * G);
+    return base + int64_t(nd) * Hq + (x0 + i - nd * by_g.d);
   }
- private:
-  int64_t base;
 };
 
 // Where segment `k` (pair + CTA: both rise along the line, so no two segments share it) lies in the workspace.
 __device__ __forceinline__ float* tree_part(const TreeParams& p, int k) { return p.part + int64_t(k) * p.part_floats; }
 
-// The consumers of a decode (sd_paged.cuh) with columns for heads.
-template <typename E, int BITS, int D, int NB>
-__global__ void __launch_bounds__(kPagedThreads, 2)
-tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
-                   const __grid_constant__ CUtensorMap tmV) {
-  using F = PagedFmt<sizeof(E), BITS, D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* qf = reinterpret_cast<float*>(sm + p.q_off);
-  float* buf = reinterpret_cast<float*>(sm + p.buf_off);
-  int* units = reinterpret_cast<int*>(sm + p.prefix_off);
-  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kPagedThreads / 32);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
-  uint64_t* empty = full + kPagedMaxStages;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  if (tid == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      mbar_init(full + i, BITS ? 33 : 1);
-      mbar_init(empty + i, kPagedWarps);
-    }
-    fence_mbar_init();
-    prefetch_tensormap(&tmK);
-    prefetch_tensormap(&tmV);
-  }
-  griddep_wait();
-  griddep_launch_dependents();
-  tree_line<kPagedThreads>(p, F::kTile, units, pairs, tmp);
-
-  const Pieces pieces(p, units[p.B]);
-  if (int(blockIdx.x) >= pieces.n) return;
-  TreeWalk walk(units, pairs, p.B, p.Hkv, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
-
-  if (warp == kPagedWarps) {
-    paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
-    return;
-  }
-  using A = typename PickAttend<E, BITS, D, NB, NodeCols>::type;
-  const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
-  A att;
-  TreeSegment s;
-  int it = 0, st = 0;
-  uint32_t round = 0;
-  bool dead = false;
-  while (walk.next(s)) {
-    const TreeSeq sq = tree_seq(p, s.b);
-    const NodeCols cols(p, sq, s.h, s.c);
-    const int t0 = sq.begin / F::kTile;
-    int edge = 0;  // tokens below it are not seen by every column
-    if (p.window) {
-      if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
-      named_barrier(1, 32 * kPagedWarps);
-      edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
-    }
-    att.begin(p, qf, cols, warp, lane);
-    for (int i = s.i0; i < s.i1; ++i, ++it) {
-      const int tok = (t0 + i) * F::kTile;
-      if (!dead) dead = !mbar_wait(full + st, round, p.flags);
-      if (!dead) {
-        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, sq.begin - tok, sq.held - tok, tok < edge ? low : nullptr, tok},
-                 warp, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + st);
-      }
-      if (++st == p.stages) {
-        st = 0;
-        round ^= 1u;
-      }
-    }
-    att.end(cols.n, WarpPart<D>(buf, p.RT, warp), lane);
-    named_barrier(1, 32 * kPagedWarps);
-    // the four warps' parts, in warp order
-    float* part = tree_part(p, s.pair + blockIdx.x);
-    for (int k = tid; k < p.RT * (D / 4); k += 32 * kPagedWarps) {
-      const int d4 = k / p.RT, g = k - d4 * p.RT;
-      if (g >= cols.n) continue;
-      float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        mw[w] = WarpPart<D>(buf, p.RT, w).ml[2 * g];
-        M = fmaxf(M, mw[w]);
-      }
-      float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const WarpPart<D> wp(buf, p.RT, w);
-        const float f = exp2_from(mw[w], M);
-        const float4 x = *reinterpret_cast<const float4*>(wp.o + g * (D + 4) + 4 * d4);
-        L = fmaf(f, wp.ml[2 * g + 1], L);
-        O.x = fmaf(f, x.x, O.x);
-        O.y = fmaf(f, x.y, O.y);
-        O.z = fmaf(f, x.z, O.z);
-        O.w = fmaf(f, x.w, O.w);
-      }
-      reinterpret_cast<float4*>(part)[k] = O;
-      if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
-    }
-    named_barrier(1, 32 * kPagedWarps);
-  }
-  if (dead) drain(full, it, p.stages);
-}
-
 // ---------------------------------------------------------------------------
-// The nodes, and the join
+// The nodes
 // ---------------------------------------------------------------------------
 
 // V neighbouring elements of a row, E each, in fp32.
@@ -319,46 +222,23 @@ struct StoredPiece<E, 0, V> {
   }
 };
 
-// Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per
-// block. First the nodes: a warp takes up to four of the columns that are heads
-// of one row. Lane l holds dimensions [l V, l V + V) of q, o and the rows; scores
-// are summed over the lanes by a butterfly that ends with head l / 8's in lane
-// l, so that lane l keeps token l % 8's of the eight that are taken at a time.
-// Then, when the attend kernel is done, the segments: a thread has one column
-// and four dimensions, and eight segments' loads under way. Bound by latency.
+// Rows and up to four query heads of one kv head at a time, number `first` and
+// every `step`-th after it; a warp calls. Lane l holds dimensions [l V, l V + V)
+// of q, o and the rows; scores are summed over the lanes by a butterfly that ends
+// with head l / 8's in lane l, so that lane l keeps token l % 8's of the eight
+// that are taken at a time.
 template <typename E, int BITS, int D>
-__global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(const __grid_constant__ TreeParams p) {
-  constexpr int V = D / 32, HB = kTreeHeads, NC = kTreeMergeCols, NW = NC * D / 128;
-  static_assert(NC == 8 && HB == 4, "at most eight rows in a block, one per warp of a head of 128");
-  __shared__ float4 node_o[D / 4][NC];
-  __shared__ float2 node_ml[NC];
-  __shared__ int seq_of[NC];  // of each column; -1: behind the last, -2: gives zeros
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int blocks = (p.N * p.G + NC - 1) / NC, h = blockIdx.x / blocks, x0 = (blockIdx.x - h * blocks) * NC;
-  const int x1 = min(x0 + NC, p.N * p.G);
-  const E* qp = static_cast<const E*>(p.q);
-  const int rows_end = __ldcg(p.first + p.B);
-
-  // items: the rows of [x0, x1), up to HB of their heads each; at most NC of them
-  int item = 0;
-  for (int a = x0; a < x1; ++item) {
-    const int n = a / p.G, g0 = a - n * p.G, heads = min(min(HB, p.G - g0), x1 - a), c0 = a - x0;
-    a += heads;
-    if (item % NW != warp) continue;
-    int b = -1;
-    if (n < rows_end) {  // the last b with first[b] <= n: it has rows
-      b = 0;
-      int hi = p.B;
-      while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (__ldcg(p.first + mid) <= n) b = mid; else hi = mid;
-      }
-    }
-    TreeSeq s{};
-    if (b >= 0) s = tree_seq(p, b);
+__device__ __forceinline__ void tree_nodes(const TreeParams& p, int first, int step) {
+  constexpr int V = D / 32, HB = kTreeHeads;
+  const int lane = threadIdx.x & 31;
+  const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups, rows_end = min(__ldcg(p.first + p.B), p.N);
+  for (int64_t item = first; item < int64_t(rows_end) * per; item += step) {
+    const int n = int(item / per), hg = int(item - int64_t(n) * per), h = hg / groups, g0 = (hg - h * groups) * HB;
+    const int heads = min(HB, p.G - g0), b = tree_find(p, n);
+    const TreeSeq s = tree_seq(p, b);
     const int node = n - s.row0;
-    const bool mine = b >= 0 && !s.bad && node >= 0 && node < s.n;
-    if (lane < heads) seq_of[c0 + lane] = b < 0 ? -1 : mine ? b : -2;
+    const bool mine = !s.bad && node >= 0 && node < s.n;
+    const int64_t col0 = int64_t(n) * p.Hq + int64_t(h) * p.G + g0;  // of q, out and the nodes' parts
     float q[HB][V], o[HB][V], m[HB], l[HB];
 #pragma unroll
     for (int g = 0; g < HB; ++g) {
@@ -367,7 +247,7 @@ __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(cons
 #pragma unroll
       for (int i = 0; i < V; ++i) q[g][i] = o[g][i] = 0.0f;
       if (mine && g < heads)
-        load_elements<E, V>(qp + (int64_t(n) * p.Hq + int64_t(h) * p.G + g0 + g) * D + lane * V, q[g]);
+        load_elements<E, V>(static_cast<const E*>(p.q) + (col0 + g) * D + lane * V, q[g]);
     }
     uint64_t seen = 0;
     int at[2] = {-1, -1};  // rows of nodes lane and lane + 32
@@ -467,62 +347,184 @@ __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(cons
 #pragma unroll
     for (int g = 0; g < HB; ++g) {
       if (g < heads) {
-        float* to = reinterpret_cast<float*>(&node_o[lane * V / 4][c0 + g]) + lane * V % 4;
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = o[g][i];
-        if (lane == 0) node_ml[c0 + g] = make_float2(m[g], l[g]);
+        float* to = p.node_o + (col0 + g) * D + lane * V;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(to) = make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
+        else *reinterpret_cast<float2*>(to) = make_float2(o[g][0], o[g][1]);
+        if (lane == 0) p.node_ml[col0 + g] = make_float2(m[g], l[g]);
       }
     }
   }
-  __syncthreads();
-  const int col = tid % NC, d4 = tid / NC, x = x0 + col;
-  const int b = x < x1 ? seq_of[col] : -1;
+}
+
+// ---------------------------------------------------------------------------
+// The held tokens
+// ---------------------------------------------------------------------------
+
+// The warps of a decode (sd_paged.cuh) with columns for heads, and one for the nodes.
+template <typename E, int BITS, int D, int NB>
+__global__ void __launch_bounds__(kTreeAttendThreads, 2)
+tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV) {
+  using F = PagedFmt<sizeof(E), BITS, D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* qf = reinterpret_cast<float*>(sm + p.q_off);
+  float* buf = reinterpret_cast<float*>(sm + p.buf_off);
+  int* units = reinterpret_cast<int*>(sm + p.prefix_off);
+  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kTreeAttendThreads / 32);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
+  uint64_t* empty = full + kPagedMaxStages;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(full + i, BITS ? 33 : 1);
+      mbar_init(empty + i, kPagedWarps);
+    }
+    fence_mbar_init();
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+  }
   griddep_wait();
-  if (b == -1) return;  // rows behind the last sequence stay as they are
-  float M = -INFINITY, L = 0.0f;
-  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const int n = x / p.G, g = x - n * p.G;
-  if (b >= 0) {
-    M = node_ml[col].x, L = node_ml[col].y, O = node_o[d4][col];
-    const TreeSeq s = tree_seq(p, b);
-    if (s.held > s.begin) {
-      const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
-      const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
-      const int nu = (u1 - up) / np, y = (n - s.row0) * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;
-      const Pieces pieces(p, all);
-      const int a = up + k * nu, cta = pieces.of(a + kSegmentUnits), ns = pieces.of(a + nu - 1) - cta + 1;
-      const float* part = tree_part(p, pp + k + cta);
+  griddep_launch_dependents();
+  tree_line<kTreeAttendThreads>(p, F::kTile, units, pairs, tmp);
+
+  if (warp == kPagedWarps + 1) {
+    tree_nodes<E, BITS, D>(p, blockIdx.x, gridDim.x);
+    return;
+  }
+  const Pieces pieces(p, units[p.B]);
+  if (int(blockIdx.x) >= pieces.n) return;
+  TreeWalk walk(units, pairs, p.B, p.Hkv, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
+
+  if (warp == kPagedWarps) {
+    paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
+    return;
+  }
+  using A = typename PickAttend<E, BITS, D, NB, NodeCols>::type;
+  const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
+  A att;
+  TreeSegment s;
+  int it = 0, st = 0;
+  uint32_t round = 0;
+  bool dead = false;
+  while (walk.next(s)) {
+    const TreeSeq sq = tree_seq(p, s.b);
+    const NodeCols cols(p, sq, s.h, s.c);
+    const int t0 = sq.begin / F::kTile;
+    int edge = 0;  // tokens below it are not seen by every column
+    if (p.window) {
+      if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
+      named_barrier(1, 32 * kPagedWarps);
+      edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
+    }
+    att.begin(p, qf, cols, warp, lane);
+    for (int i = s.i0; i < s.i1; ++i, ++it) {
+      const int tok = (t0 + i) * F::kTile;
+      if (!dead) dead = !mbar_wait(full + st, round, p.flags);
+      if (!dead) {
+        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, sq.begin - tok, sq.held - tok, tok < edge ? low : nullptr, tok},
+                 warp, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + st);
+      }
+      if (++st == p.stages) {
+        st = 0;
+        round ^= 1u;
+      }
+    }
+    att.end(cols.n, WarpPart<D>(buf, p.RT, warp), lane);
+    named_barrier(1, 32 * kPagedWarps);
+    // the four warps' parts, in warp order
+    float* part = tree_part(p, s.pair + blockIdx.x);
+    for (int k = tid; k < p.RT * (D / 4); k += 32 * kPagedWarps) {
+      const int d4 = k / p.RT, g = k - d4 * p.RT;
+      if (g >= cols.n) continue;
+      float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        mw[w] = WarpPart<D>(buf, p.RT, w).ml[2 * g];
+        M = fmaxf(M, mw[w]);
+      }
+      float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        const WarpPart<D> wp(buf, p.RT, w);
+        const float f = exp2_from(mw[w], M);
+        const float4 x = *reinterpret_cast<const float4*>(wp.o + g * (D + 4) + 4 * d4);
+        L = fmaf(f, wp.ml[2 * g + 1], L);
+        O.x = fmaf(f, x.x, O.x);
+        O.y = fmaf(f, x.y, O.y);
+        O.z = fmaf(f, x.z, O.z);
+        O.w = fmaf(f, x.w, O.w);
+      }
+      reinterpret_cast<float4*>(part)[k] = O;
+      if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
+    }
+    named_barrier(1, 32 * kPagedWarps);
+  }
+  if (dead) drain(full, it, p.stages);
+}
+
+// Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per
+// block: a thread has one column and four dimensions, and eight segments' loads
+// under way. Bound by latency: the line, the segments' places, their loads.
+template <typename E, int D>
+__global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int NC = kTreeMergeCols;
+  const int columns = p.N * p.G, blocks = (columns + NC - 1) / NC, h = blockIdx.x / blocks;
+  const int col = threadIdx.x % NC, d4 = threadIdx.x / NC, x = (blockIdx.x - h * blocks) * NC + col;
+  const int n = p.by_g(min(x, columns - 1)), g = x - n * p.G;
+  const bool live = x < columns && n < __ldcg(p.first + p.B);  // rows behind the last sequence stay as they are
+  int b = 0;
+  TreeSeq s{};
+  if (live) {
+    b = tree_find(p, n);
+    s = tree_seq(p, b);
+  }
+  griddep_wait();
+  if (!live) return;
+  const int64_t row = int64_t(n) * p.Hq + int64_t(h) * p.G + g;
+  const float2 node = __ldcg(p.node_ml + row);
+  float4 O = __ldcg(reinterpret_cast<const float4*>(p.node_o + row * D) + d4);
+  float M = node.x, L = node.y;
+  const int i = n - s.row0;
+  if (i >= 0 && i < s.n && s.held > s.begin) {
+    const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
+    const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
+    const int nu = (u1 - up) / np, y = i * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;
+    const Pieces pieces(p, all);
+    const int a = up + k * nu, cta = pieces.of(a + kSegmentUnits), ns = pieces.of(a + nu - 1) - cta + 1;
+    const float* part = tree_part(p, pp + k + cta);
 #pragma unroll 1
-      for (int j0 = 0; j0 < ns; j0 += 8) {
-        float2 ml[8];
-        float4 v[8];
+    for (int j0 = 0; j0 < ns; j0 += 8) {
+      float2 ml[8];
+      float4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ml[j] = make_float2(-INFINITY, 0.0f);
-          v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (j0 + j < ns) {
-            const float* from = part + int64_t(j0 + j) * p.part_floats;
-            ml[j] = __ldcg(reinterpret_cast<const float2*>(from + p.RT * D) + at);
-            v[j] = __ldcg(reinterpret_cast<const float4*>(from) + d4 * p.RT + at);
-          }
+      for (int j = 0; j < 8; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.0f);
+        v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j0 + j < ns) {
+          const float* from = part + int64_t(j0 + j) * p.part_floats;
+          ml[j] = __ldcg(reinterpret_cast<const float2*>(from + p.RT * D) + at);
+          v[j] = __ldcg(reinterpret_cast<const float4*>(from) + d4 * p.RT + at);
         }
-        float top = ml[0].x;
+      }
+      float top = ml[0].x;
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, ml[j].x);
-        const float f = raise_max(M, top);
-        L *= f;
-        O.x *= f, O.y *= f, O.z *= f, O.w *= f;
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, ml[j].x);
+      const float f = raise_max(M, top);
+      L *= f;
+      O.x *= f, O.y *= f, O.z *= f, O.w *= f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = exp2_from(ml[j].x, M);
-          L = fmaf(w, ml[j].y, L);
-          O.x = fmaf(w, v[j].x, O.x), O.y = fmaf(w, v[j].y, O.y);
-          O.z = fmaf(w, v[j].z, O.z), O.w = fmaf(w, v[j].w, O.w);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float w = exp2_from(ml[j].x, M);
+        L = fmaf(w, ml[j].y, L);
+        O.x = fmaf(w, v[j].x, O.x), O.y = fmaf(w, v[j].y, O.y);
+        O.z = fmaf(w, v[j].z, O.z), O.w = fmaf(w, v[j].w, O.w);
       }
     }
   }
-  const int64_t row = int64_t(n) * p.Hq + int64_t(h) * p.G + g;
   if (p.sinks) L += exp2f(fmaf(__ldcg(p.sinks + h * p.G + g), 1.4426950408889634f, -(M == -INFINITY ? 0.0f : M)));
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   E* out = static_cast<E*>(p.out) + row * D + 4 * d4;

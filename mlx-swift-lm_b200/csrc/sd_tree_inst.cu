@@ -24,7 +24,7 @@ static TreeSet make_tree() {
   using F = PagedFmt<sizeof(ET), SD_BITS, D>;
   TreeSet s;
   s.attend = reinterpret_cast<const void*>(&tree_attend_kernel<ET, SD_BITS, D, NB>);
-  s.merge = reinterpret_cast<const void*>(&tree_merge_kernel<ET, SD_BITS, D>);
+  s.merge = reinterpret_cast<const void*>(&tree_merge_kernel<ET, D>);
   s.tile = F::kTile;
   s.stage_bytes = F::kStageBytes;
   s.columns = NB * (SD_E == 0 && SD_BITS == 0 ? 4 : 8);

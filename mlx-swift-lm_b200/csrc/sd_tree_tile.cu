@@ -6,13 +6,16 @@
 // 128 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes
 // S's place there as the next product's left operand, Q, K and V are 128B-
 // swizzled tiles in shared memory (TMA, one box per page and 64 dimensions).
-// One warp loads, one thread issues the products, and two groups of four warps
-// hold a row per thread and make P, each with its own S and O, so that the
-// products of one group run while the other makes its P:
+// One warp loads, one thread issues the products, two groups of four warps hold
+// a row per thread and make P, each with its own S and O, and two warps see to
+// the nodes:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
 //     groups in turn, whose parts are joined at a segment's end.
+// A tile of 128 tokens is two halves. A group's S has a buffer for each, so that
+// it weighs one half while the products of the other run: O += P V, and then,
+// when that has read P, the scores of the next half in P's place.
 // P is one value of the element type: 128 x 128 products cost as much as their
 // exponentials, and a second half would cost as much again (SHARED). The sum
 // that O is divided by is made of the rounded values, so their errors cancel
@@ -28,7 +31,7 @@ namespace sd {
 
 namespace {
 
-constexpr int kTileT = kTreeTileTokens;
+constexpr int kTileT = kTreeTileTokens, kHalfT = kTileT / 2;
 constexpr int kTmemCols = 512;
 constexpr int kSCol = 0, kOCol = 256;  // tensor memory columns of the first group's S and O; the second's 128 on
 
@@ -80,11 +83,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
 __device__ __forceinline__ void tmem_wait(uint32_t* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : SD_U8(v, 0), SD_U8(v, 8), SD_U8(v, 16), SD_U8(v, 24)::"memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-               SD_W8(v, 0), SD_W8(v, 8)
-               : "memory");
-}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -105,7 +103,7 @@ struct Waiter {
 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+  uint64_t q_full[2], o_full[2], s_full[2][2], p_full[2][2], done;  // of a group; of a group's buffer
   uint32_t tmem;
 };
 static_assert(sizeof(TileBars) <= kTreeTileBarBytes, "room in the layout");
@@ -124,7 +122,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   TileBars* bars = reinterpret_cast<TileBars*>(sm + p.bar_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
-  __shared__ float2 other[SHARED ? 1 : 128];  // (m, l) of the second group
+  __shared__ float2 ml_of[2][SHARED ? 1 : 128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -134,9 +132,11 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(bars->q_full + w, 128);
-      mbar_init(bars->s_full + w, 1);
-      mbar_init(bars->p_full + w, 128);
       mbar_init(bars->o_full + w, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars->s_full[w][i], 1);
+        mbar_init(&bars->p_full[w][i], 128);
+      }
     }
     mbar_init(&bars->done, 1);
     fence_mbar_init();
@@ -213,129 +213,143 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     if (wait.dead)  // what is under way lands in this CTA's shared memory
       for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
   } else if (warp == 9) {  // ---- products ----
-    uint32_t seg[2] = {0, 0}, k[2] = {0, 0};  // segments and steps of each group: the parities of its barriers
-    const uint32_t ring_a = smem_u32(ring);
-    const uint32_t first_lane = lane == 0;
+    // Segments of each group that it took part in, and its halves: the parities of its barriers.
+    uint32_t seg[2] = {0, 0}, k[2] = {0, 0};
+    const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(qs);
+    const bool issue = lane == 0;
     while (walk.next(s)) {
-      const int nt = s.i1 - s.i0, n = SHARED ? 2 * nt : nt;
-      auto stage_of = [&](int step, int kv) { return 2 * (it0 + (SHARED ? step >> 1 : step)) + kv; };
+      const int nt = s.i1 - s.i0;
+      // halves of a group; half i of group w is half i & 1 of tile_of(w, i)
+      auto halves = [&](int w) { return SHARED ? 2 * nt : 2 * ((nt + 1 - w) / 2); };
+      auto tile_of = [&](int w, int i) { return it0 + (SHARED ? i >> 1 : 2 * (i >> 1) + w); };
       auto landed = [&](int u) { return wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u); };
-      auto scores = [&](int step) {  // S of a step
-        const int w = step & 1, u = stage_of(step, 0);
+      auto scores = [&](int w, int i) {  // half i of group w
+        const int u = 2 * tile_of(w, i), h = i & 1;
         if (!landed(u)) return;
         tc_fence_after();
-        if (first_lane) {
-          const uint32_t q = smem_u32(qs) + w * kStage, kk = ring_a + (u % p.stages) * kStage;
+        if (issue) {
+          const uint32_t q = q_a + w * kStage, kk = ring_a + (u % p.stages) * kStage + h * kHalfT * 128;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c)
-            mma_ss(tmem + kSCol + w * 128, operand_desc(q + (c / 4) * kHalf + (c % 4) * 32, 16, 1024),
-                   operand_desc(kk + (c / 4) * kHalf + (c % 4) * 32, 16, 1024), product_desc<E>(kTileT, false), c > 0);
-          mma_commit(bars->s_full + w);
-          if (!SHARED || w == 1) mma_commit(bars->empty + u % p.stages);
+            mma_ss(tmem + kSCol + w * 128 + h * kHalfT, operand_desc(q + (c / 4) * kHalf + (c % 4) * 32, 16, 1024),
+                   operand_desc(kk + (c / 4) * kHalf + (c % 4) * 32, 16, 1024), product_desc<E>(kHalfT, false), c > 0);
+          mma_commit(&bars->s_full[w][h]);
+          if (h == 1 && (!SHARED || w == 1)) mma_commit(bars->empty + u % p.stages);
         }
         __syncwarp();
       };
-      // A group with steps loads its rows of Q first, and has read what it needs of its last S and O then. One without
-      // (a segment of one tile) does not take part: it could run ahead of this wait by more than a phase.
-      for (int w = 0; w < min(n, 2); ++w, ++seg[w - 1])
-        if (wait(bars->q_full + w, seg[w] & 1u)) scores(w);
-      for (int step = 0; step < n && !wait.dead; ++step) {
-        const int w = step & 1, u = stage_of(step, 1);
-        if (!wait(bars->p_full + w, k[w] & 1u) || !landed(u)) break;
+      auto values = [&](int w, int i) {
+        const int u = 2 * tile_of(w, i) + 1, h = i & 1;
+        if (!wait(&bars->p_full[w][h], ((k[w] + i) >> 1) & 1u) || !landed(u)) return;
         tc_fence_after();
-        if (first_lane) {
-          const uint32_t v = ring_a + (u % p.stages) * kStage;
+        if (issue) {
+          const uint32_t v = ring_a + (u % p.stages) * kStage + h * kHalfT * 128;
 #pragma unroll
-          for (int c = 0; c < kTileT / 16; ++c)
-            mma_ts(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + c * 8, operand_desc(v + c * 2048, kHalf, 1024),
-                   product_desc<E>(D, true), step > 1 || c > 0);
+          for (int c = 0; c < kHalfT / 16; ++c)
+            mma_ts(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + h * kHalfT + c * 8, operand_desc(v + c * 2048, kHalf, 1024),
+                   product_desc<E>(D, true), i > 0 || c > 0);
           mma_commit(bars->o_full + w);
-          if (!SHARED || w == 1) mma_commit(bars->empty + u % p.stages);
+          if (h == 1 && (!SHARED || w == 1)) mma_commit(bars->empty + u % p.stages);
         }
         __syncwarp();
-        if (step + 2 < n) {
-          if (!wait(bars->o_full + w, k[w] & 1u)) break;  // P lies where the next S goes
-          scores(step + 2);
+      };
+      const int n0 = halves(0), n1 = halves(1);
+      // A group with tiles loads its rows of Q first, and has read what it needs of its last S and O then. One without
+      // (a segment of one tile) does not take part: it could run ahead of this wait by more than a phase.
+      if (wait(bars->q_full, seg[0]++ & 1u)) scores(0, 0), scores(0, 1);
+      if (n1 > 0 && wait(bars->q_full + 1, seg[1]++ & 1u)) scores(1, 0);
+      for (int i = 0; i < n0 && !wait.dead; ++i) {
+        values(0, i);
+        if (i + 1 < n1) {  // P of half i - 1 lies where these scores go
+          if (i > 0) wait(bars->o_full + 1, (k[1] + i - 1) & 1u);
+          if (!wait.dead) scores(1, i + 1);
         }
-        ++k[w];
+        if (i < n1 && !wait.dead) values(1, i);
+        if (i + 2 < n0) {
+          wait(bars->o_full, (k[0] + i) & 1u);
+          if (!wait.dead) scores(0, i + 2);
+        }
       }
+      k[0] += n0, k[1] += n1;
       it0 += nt;
     }
-    if (first_lane) mma_commit(&bars->done);  // no product may read shared memory that is no longer this CTA's
+    if (issue) mma_commit(&bars->done);  // no product may read shared memory that is no longer this CTA's
     __syncwarp();
     mbar_wait(&bars->done, 0, p.flags);
+  } else if (warp >= 10) {
+    tree_nodes<E, 0, D>(p, 2 * blockIdx.x + warp - 10, 2 * gridDim.x);
   } else {  // ---- weights: a row per thread ----
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
     const uint32_t ts = tmem + lanes + kSCol + w * 128, to = tmem + lanes + kOCol + w * 128;
     const bool neg = p.scale_log2 < 0.0f;
     const float sc = fmaxf(fabsf(p.scale_log2), 1.1754944e-38f);  // -inf times it stays -inf
-    uint32_t k = 0;  // steps of this group
+    uint32_t k = 0;  // halves of this group
     while (walk.next(s)) {
       const TreeSeq sq = tree_seq(p, s.b);
       const NodeCols cols(p, sq, s.h, s.c);
       const int x = SHARED ? w * 128 + r : r;  // column of the pair
       const int t0 = sq.begin / kTileT;
-      const int low = p.window && x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
-      const int edge = __reduce_max_sync(0xffffffffu, low);
-      if (SHARED || s.i0 + w < s.i1) {  // Q: 16 bytes at a time, a row's chunks side by side
-        constexpr int CPR = D / 8;
+      if (SHARED || s.i0 + w < s.i1) {  // Q: a thread has one 16-byte chunk of every eighth (or sixteenth) row
+        constexpr int CPR = D / 8, RPT = 128 / CPR, N = 128 / RPT;
         const uint32_t q = smem_u32(qs) + w * kStage;
-#pragma unroll 4
-        for (int c = r; c < 128 * CPR; c += 128) {
-          const int row = c / CPR, ch = c % CPR, xx = (SHARED ? w * 128 : 0) + row;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (xx < cols.n) v = __ldcg(reinterpret_cast<const uint4*>(static_cast<const E*>(p.q) + cols.row(xx) * D) + ch);
+        const int ch = r % CPR;
+        uint4 v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int xx = (SHARED ? w * 128 : 0) + r / CPR + RPT * i;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (xx < cols.n) v[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const E*>(p.q) + cols.row(xx) * D) + ch);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int row = r / CPR + RPT * i;
           const uint32_t at = q + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
         }
         fence_proxy_async_shared();
         tc_fence_before();
         mbar_arrive(bars->q_full + w);
       }
+      const int low = p.window && x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
+      const int edge = __reduce_max_sync(0xffffffffu, low);
       float m = -INFINITY, l = 0.0f;
       int steps = 0;
-      for (int i = s.i0 + (SHARED ? 0 : w); i < s.i1; i += SHARED ? 1 : 2, ++steps, ++k) {
-        const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.held - tok;
-        if (!wait(bars->s_full + w, k & 1u)) continue;
+      const int each = SHARED ? 1 : 2, n = 2 * ((s.i1 - s.i0 + (SHARED ? 0 : 1 - w)) / each);
+#pragma unroll 1
+      for (; steps < n; ++steps, ++k) {
+        const int h = steps & 1, tile = (steps >> 1) * each + (SHARED ? 0 : w);  // of the segment
+        const int tok = (t0 + s.i0 + tile) * kTileT + h * kHalfT, lo = sq.begin - tok, hi = sq.held - tok;
+        const uint32_t sh = ts + h * kHalfT;
+        if (!wait(&bars->s_full[w][h], (k >> 1) & 1u)) continue;
         tc_fence_after();
-        // The row's scores, 32 at a time, twice: for the maximum and for the weights. All 128 in registers would spill.
-        const bool some = lo > 0 || hi < kTileT || tok < edge;  // some may not be seen
-        const int from = max(lo, low - tok);
-        auto as_seen = [&](uint32_t (&v)[32], int c) {
-          if (neg) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] ^= 0x80000000u;
-          }
-          if (some) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 32 * c + j < from || 32 * c + j >= hi ? 0xff800000u : v[j];
-          }
-        };
         uint32_t va[32], vb[32];
-        float mx[2] = {-INFINITY, -INFINITY};
-        auto most = [&](uint32_t (&v)[32], int c) {
-          as_seen(v, c);
+        tmem_ld32(sh, va);
+        tmem_ld32(sh + 32, vb);
+        tmem_wait(va);
+        tmem_wait(vb);
+        if (neg) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            mx[0] = fmaxf(mx[0], __uint_as_float(v[j]));
-            mx[1] = fmaxf(mx[1], __uint_as_float(v[j + 1]));
+          for (int j = 0; j < 32; ++j) va[j] ^= 0x80000000u, vb[j] ^= 0x80000000u;
+        }
+        const bool ends = lo > 0 || hi < kHalfT;
+        if (ends || tok < edge) {  // some are not seen
+          const int from = max(lo, low - tok);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            va[j] = j < from || j >= hi ? 0xff800000u : va[j];
+            vb[j] = j + 32 < from || j + 32 >= hi ? 0xff800000u : vb[j];
           }
-        };
-        tmem_ld32(ts, va);
-        tmem_wait(va);
-        tmem_ld32(ts + 32, vb);
-        most(va, 0);
-        tmem_wait(vb);
-        tmem_ld32(ts + 64, va);
-        most(vb, 1);
-        tmem_wait(va);
-        tmem_ld32(ts + 96, vb);
-        most(va, 2);
-        tmem_wait(vb);
-        tmem_ld32(ts, va);
-        most(vb, 3);
-        const float top = fmaxf(mx[0], mx[1]) * sc;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          mx[0] = fmaxf(mx[0], __uint_as_float(va[j]));
+          mx[1] = fmaxf(mx[1], __uint_as_float(va[j + 1]));
+          mx[2] = fmaxf(mx[2], __uint_as_float(vb[j]));
+          mx[3] = fmaxf(mx[3], __uint_as_float(vb[j + 1]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         if (steps == 0) {
           m = top - kUp;
         } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
@@ -343,120 +357,116 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           l *= fac;
           if (wait(bars->o_full + w, (k - 1) & 1u)) {
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              tmem_ld32(to + 32 * c, vb);
-              tmem_wait(vb);
+              uint32_t o[32];
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait(o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) vb[j] = __float_as_uint(__uint_as_float(vb[j]) * fac);
-              tmem_st32(to + 32 * c, vb);
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fac);
+              tmem_st32(to + 32 * c, o);
             }
           }
         }
         const float mm = m == -INFINITY ? 0.0f : m;
-        float sum[2] = {0.0f, 0.0f};
-        auto weigh = [&](uint32_t (&v)[32], int c) {  // P takes the place of scores that have been read
-          as_seen(v, c);
-          uint32_t two[16];
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t two[32];
+        auto weigh = [&](const uint32_t (&v)[32], int c) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            two[j] = pack2<E>(ex2(fmaf(__uint_as_float(v[2 * j]), sc, -mm)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), sc, -mm)));
+            two[16 * c + j] = pack2<E>(ex2(fmaf(__uint_as_float(v[2 * j]), sc, -mm)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), sc, -mm)));
             float g[2];
-            unpack_word<E>(two[j], g);
-            sum[0] += g[0];
-            sum[1] += g[1];
+            unpack_word<E>(two[16 * c + j], g);
+            sum[2 * (j & 1)] += g[0];
+            sum[2 * (j & 1) + 1] += g[1];
           }
-          tmem_st16(ts + 16 * c, two);
         };
-        tmem_wait(va);
-        tmem_ld32(ts + 32, vb);
         weigh(va, 0);
-        tmem_wait(vb);
-        tmem_ld32(ts + 64, va);
         weigh(vb, 1);
-        tmem_wait(va);
-        tmem_ld32(ts + 96, vb);
-        weigh(va, 2);
-        tmem_wait(vb);
-        weigh(vb, 3);
-        l += sum[0] + sum[1];
-        if ((lo > 0 || hi < kTileT) && (!SHARED || w == 0)) {
-          const int u = 2 * (it0 + i - s.i0) + 1;
+        tmem_st32(sh, two);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (ends && (!SHARED || w == 0)) {
+          const int u = 2 * (it0 + tile) + 1;
           if (wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
-            if (r < lo || r >= hi) {
-              const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + r * 128;
+            const int row = r >> 1;  // of the half; a thread zeroes half of it
+            if (row < lo || row >= hi) {
+              const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
 #pragma unroll
-              for (int c = 0; c < NH * 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + (c / 8) * kHalf + (c % 8) * 16), "r"(0) : "memory");
+              for (int c = 0; c < NH * 4; ++c) {
+                const int cc = (r & 1) * NH * 4 + c;
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + (cc / 8) * kHalf + (cc % 8) * 16), "r"(0) : "memory");
+              }
             }
             fence_proxy_async_shared();
           }
         }
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(bars->p_full + w);
+        mbar_arrive(&bars->p_full[w][h]);
       }
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
       float* part = tree_part(p, s.pair + int(blockIdx.x));
-      if (steps > 0 && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();
+      // both of the last products may be under way, and a wait for a phase takes the one before the last for it
+      if (steps > 0 && wait(bars->o_full + w, k & 1u) && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();
       const bool has = steps > 0 && !wait.dead;
-      float4* swap = reinterpret_cast<float4*>(qs);  // [D / 4][128]: no score of this segment is still to come
-      float f0 = 1.0f, f1 = 0.0f;
-      if constexpr (!SHARED) {
-        // the second group's part goes to the first through shared memory
-        named_barrier(1, 256);
-        if (w == 1) {
+      auto load = [&](int c, uint32_t (&o)[32]) {  // dimensions 32 c ..
+        if (has) {
+          tmem_ld32(to + 32 * c, o);
+          tmem_wait(o);
+        } else {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            if (has) {
-              tmem_ld32(to + 32 * c, o);
-              tmem_wait(o);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              swap[(8 * c + j) * 128 + r] = has ? make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                                              __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]))
-                                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          }
-          other[r] = make_float2(m, l);
+          for (int j = 0; j < 32; ++j) o[j] = 0;
         }
-        named_barrier(1, 256);
-        if (w == 0) {
-          const float2 ml = other[r];
-          const float top = fmaxf(m, ml.x);
-          f0 = exp2_from(m, top), f1 = exp2_from(ml.x, top);
-          m = top;
-          l = fmaf(f1, ml.y, l * f0);
-        }
-      }
-      if (SHARED || w == 0) {
-#pragma unroll
+      };
+      if constexpr (SHARED) {
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          if (has) {
-            tmem_ld32(to + 32 * c, o);
-            tmem_wait(o);
+          load(c, o);
+          if (x < cols.n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              reinterpret_cast<uint4*>(part)[(8 * c + j) * 256 + x] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
+        }
+      } else {
+        // each group finishes half of the dimensions and hands the other half over, in the place of Q: no score of this
+        // segment is still to come
+        uint4* swap = reinterpret_cast<uint4*>(qs + w * kStage);  // [D / 8][128]
+        const uint4* from = reinterpret_cast<const uint4*>(qs + (1 - w) * kStage);
+        named_barrier(1, 256);
+        ml_of[w][r] = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[32];
+          load((1 - w) * (D / 64) + c, o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            swap[(8 * c + j) * 128 + r] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+        named_barrier(1, 256);
+        const float2 ml = ml_of[1 - w][r];
+        const float most = fmaxf(m, ml.x), f0 = exp2_from(m, most), f1 = exp2_from(ml.x, most);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[32];
+          load(w * (D / 64) + c, o);
           if (x < cols.n) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              float4 y = has ? make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
-                                           __uint_as_float(o[4 * j + 3]))
-                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if constexpr (!SHARED) {
-                const float4 z = swap[(8 * c + j) * 128 + r];
-                y.x = fmaf(f1, z.x, f0 * y.x), y.y = fmaf(f1, z.y, f0 * y.y);
-                y.z = fmaf(f1, z.z, f0 * y.z), y.w = fmaf(f1, z.w, f0 * y.w);
-              }
-              reinterpret_cast<float4*>(part)[(8 * c + j) * p.RT + x] = y;
+              const uint4 z = from[(8 * c + j) * 128 + r];
+              auto join = [&](uint32_t a, uint32_t b) { return fmaf(f1, __uint_as_float(b), f0 * __uint_as_float(a)); };
+              reinterpret_cast<float4*>(part)[(w * (D / 8) + 8 * c + j) * 128 + x] =
+                  make_float4(join(o[4 * j], z.x), join(o[4 * j + 1], z.y), join(o[4 * j + 2], z.z), join(o[4 * j + 3], z.w));
             }
           }
         }
-        if (x < cols.n) *reinterpret_cast<float2*>(part + p.RT * D + 2 * x) = make_float2(m, l);
+        m = most;
+        l = w == 0 ? fmaf(f1, ml.y, l * f0) : fmaf(f0, l, ml.y * f1);
+        named_barrier(1, 256);  // before the next rows of Q
       }
-      if constexpr (!SHARED) named_barrier(1, 256);  // before the next rows of Q
+      if (x < cols.n && (SHARED || w == 0)) *reinterpret_cast<float2*>(part + p.RT * D + 2 * x) = make_float2(m, l);
     }
     tc_fence_before();
   }
