@@ -25,6 +25,8 @@
 // group rescales O in tensor memory. Rows of V outside the range may hold
 // anything and are zeroed in shared memory (0 * NaN is NaN); scores there are
 // replaced.
+#include <type_traits>
+
 #include "sd_tree.cuh"
 
 namespace sd {
@@ -48,21 +50,26 @@ __host__ __device__ constexpr uint32_t product_desc(int n, bool b_mn) {
   constexpr uint32_t fmt = __is_same(E, __half) ? 0u : 1u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
+// A whole warp calls these and one thread of it, always the same, issues: what the products' operands are computed
+// from stays uniform.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(int(add))
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(int(add))
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(int(add))
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(int(add))
       : "memory");
 }
-// The barrier gets one arrival when the products issued so far by this thread are done.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The barrier gets one arrival when the products issued so far are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -213,68 +220,93 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     if (wait.dead)  // what is under way lands in this CTA's shared memory
       for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
   } else if (warp == 9) {  // ---- products ----
-    // Segments of each group that it took part in, and its halves: the parities of its barriers.
-    uint32_t seg[2] = {0, 0}, k[2] = {0, 0};
-    const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(qs);
-    const bool issue = lane == 0;
+    // Per group: segments that it took part in and halves, whose parities are those of its barriers; the stages of its
+    // next K and V, and their parities.
+    uint32_t seg0 = 0, seg1 = 0, k0 = 0, k1 = 0;
+    struct Ring {
+      int st, par, n;
+      __device__ __forceinline__ void go(int by) {  // by: at most n
+        st += by;
+        if (st >= n) st -= n, par ^= 1;
+      }
+    };
+    Ring rk[2], rv[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) rk[w].n = rv[w].n = p.stages;
+    const uint64_t desc0 = operand_desc(0, 16, 1024), vdesc0 = operand_desc(0, kHalf, 1024);
+    const uint32_t ring_a = smem_u32(ring) >> 4, q_a = smem_u32(qs) >> 4;
+    const uint32_t empty = smem_u32(bars->empty), s_full = smem_u32(bars->s_full), o_full = smem_u32(bars->o_full);
+    // scores of a half (h) of group w's next K; products with its weights
+    auto scores = [&](auto w_, int h) {
+      constexpr int w = decltype(w_)::value;
+      Ring& g = rk[w];
+      if (!wait(bars->full + g.st, uint32_t(g.par))) return;
+      tc_fence_after();
+      const uint64_t q = desc0 + q_a + w * (kStage >> 4);
+      const uint64_t kk = desc0 + ring_a + g.st * (kStage >> 4) + h * (kHalfT * 128 >> 4);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        constexpr uint32_t idesc = product_desc<E>(kHalfT, false);
+        const int off = (c / 4) * (kHalf >> 4) + (c % 4) * 2;
+        mma_ss(tmem + kSCol + w * 128 + h * kHalfT, q + off, kk + off, idesc, c > 0);
+      }
+      mma_commit(s_full + (2 * w + h) * 8);
+      if (h == 1) {
+        if (!SHARED || w == 1) mma_commit(empty + g.st * 8);
+        g.go(SHARED ? 2 : 4);
+      }
+    };
+    auto values = [&](auto w_, int h, uint32_t half, bool add) {  // half: its number, over all segments
+      constexpr int w = decltype(w_)::value;
+      Ring& g = rv[w];
+      if (!wait(&bars->p_full[w][h], (half >> 1) & 1u) || !wait(bars->full + g.st, uint32_t(g.par))) return;
+      tc_fence_after();
+      const uint64_t v = vdesc0 + ring_a + g.st * (kStage >> 4) + h * (kHalfT * 128 >> 4);
+#pragma unroll
+      for (int c = 0; c < kHalfT / 16; ++c) {
+        constexpr uint32_t idesc = product_desc<E>(D, true);
+        mma_ts(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + h * kHalfT + c * 8, v + c * (2048 >> 4), idesc, add || c > 0);
+      }
+      mma_commit(o_full + w * 8);
+      if (h == 1) {
+        if (!SHARED || w == 1) mma_commit(empty + g.st * 8);
+        g.go(SHARED ? 2 : 4);
+      }
+    };
+    using W0 = std::integral_constant<int, 0>;
+    using W1 = std::integral_constant<int, 1>;
     while (walk.next(s)) {
-      const int nt = s.i1 - s.i0;
-      // halves of a group; half i of group w is half i & 1 of tile_of(w, i)
-      auto halves = [&](int w) { return SHARED ? 2 * nt : 2 * ((nt + 1 - w) / 2); };
-      auto tile_of = [&](int w, int i) { return it0 + (SHARED ? i >> 1 : 2 * (i >> 1) + w); };
-      auto landed = [&](int u) { return wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u); };
-      auto scores = [&](int w, int i) {  // half i of group w
-        const int u = 2 * tile_of(w, i), h = i & 1;
-        if (!landed(u)) return;
-        tc_fence_after();
-        if (issue) {
-          const uint32_t q = q_a + w * kStage, kk = ring_a + (u % p.stages) * kStage + h * kHalfT * 128;
+      const int nt = s.i1 - s.i0, n0 = SHARED ? 2 * nt : 2 * ((nt + 1) / 2), n1 = SHARED ? n0 : 2 * (nt / 2);
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-            mma_ss(tmem + kSCol + w * 128 + h * kHalfT, operand_desc(q + (c / 4) * kHalf + (c % 4) * 32, 16, 1024),
-                   operand_desc(kk + (c / 4) * kHalf + (c % 4) * 32, 16, 1024), product_desc<E>(kHalfT, false), c > 0);
-          mma_commit(&bars->s_full[w][h]);
-          if (h == 1 && (!SHARED || w == 1)) mma_commit(bars->empty + u % p.stages);
+      for (int w = 0; w < 2; ++w) {
+        const int u = 2 * (it0 + (SHARED ? 0 : w));
+        rk[w].st = u % p.stages, rk[w].par = (u / p.stages) & 1;
+        rv[w].st = (u + 1) % p.stages, rv[w].par = ((u + 1) / p.stages) & 1;
+      }
+      // In turn: P V of half i of the first group, the scores of half i + 1 of the second, P V of its half i, the scores
+      // of half i + 2 of the first. Scores go where P of two halves before lies, whose product has to be done; the first
+      // ones of a segment want the group's rows of Q instead, and with those it has read what it needs of its last S
+      // and O. A group without tiles (a segment of one) loads no rows: it could run ahead by more than a phase.
+#pragma unroll 1
+      for (int i = -2; i < n0 && !wait.dead; ++i) {
+        const int h = i & 1;
+        if (i >= 0) values(W0{}, h, k0 + i, i > 0);
+        if (i + 1 >= 0 && i + 1 < n1) {
+          if (i < 0) wait(bars->q_full + 1, seg1++ & 1u);
+          else if (i > 0) wait(bars->o_full + 1, (k1 + i - 1) & 1u);
+          if (!wait.dead) scores(W1{}, h ^ 1);
         }
-        __syncwarp();
-      };
-      auto values = [&](int w, int i) {
-        const int u = 2 * tile_of(w, i) + 1, h = i & 1;
-        if (!wait(&bars->p_full[w][h], ((k[w] + i) >> 1) & 1u) || !landed(u)) return;
-        tc_fence_after();
-        if (issue) {
-          const uint32_t v = ring_a + (u % p.stages) * kStage + h * kHalfT * 128;
-#pragma unroll
-          for (int c = 0; c < kHalfT / 16; ++c)
-            mma_ts(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + h * kHalfT + c * 8, operand_desc(v + c * 2048, kHalf, 1024),
-                   product_desc<E>(D, true), i > 0 || c > 0);
-          mma_commit(bars->o_full + w);
-          if (h == 1 && (!SHARED || w == 1)) mma_commit(bars->empty + u % p.stages);
-        }
-        __syncwarp();
-      };
-      const int n0 = halves(0), n1 = halves(1);
-      // A group with tiles loads its rows of Q first, and has read what it needs of its last S and O then. One without
-      // (a segment of one tile) does not take part: it could run ahead of this wait by more than a phase.
-      if (wait(bars->q_full, seg[0]++ & 1u)) scores(0, 0), scores(0, 1);
-      if (n1 > 0 && wait(bars->q_full + 1, seg[1]++ & 1u)) scores(1, 0);
-      for (int i = 0; i < n0 && !wait.dead; ++i) {
-        values(0, i);
-        if (i + 1 < n1) {  // P of half i - 1 lies where these scores go
-          if (i > 0) wait(bars->o_full + 1, (k[1] + i - 1) & 1u);
-          if (!wait.dead) scores(1, i + 1);
-        }
-        if (i < n1 && !wait.dead) values(1, i);
+        if (i >= 0 && i < n1 && !wait.dead) values(W1{}, h, k1 + i, i > 0);
         if (i + 2 < n0) {
-          wait(bars->o_full, (k[0] + i) & 1u);
-          if (!wait.dead) scores(0, i + 2);
+          if (i == -2) wait(bars->q_full, seg0++ & 1u);
+          else if (i >= 0) wait(bars->o_full, (k0 + i) & 1u);
+          if (!wait.dead) scores(W0{}, h);
         }
       }
-      k[0] += n0, k[1] += n1;
+      k0 += n0, k1 += n1;
       it0 += nt;
     }
-    if (issue) mma_commit(&bars->done);  // no product may read shared memory that is no longer this CTA's
-    __syncwarp();
+    mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
     mbar_wait(&bars->done, 0, p.flags);
   } else if (warp >= 10) {
     tree_nodes<E, 0, D>(p, 2 * blockIdx.x + warp - 10, 2 * gridDim.x);
