@@ -99,7 +99,8 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
-// of four warps, a loading warp, one that issues products and two for the nodes.
+// of four warps, a warp that issues products for each, a loading warp and one
+// for the nodes.
 constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
 constexpr int kTreeTileThreads = 384;
 constexpr int kTreeTileTokens = 128;

@@ -6,9 +6,9 @@
 // 128 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes
 // S's place there as the next product's left operand, Q, K and V are 128B-
 // swizzled tiles in shared memory (TMA, one box per page and 64 dimensions).
-// One warp loads, one thread issues the products, two groups of four warps hold
-// a row per thread and make P, each with its own S and O, and two warps see to
-// the nodes:
+// One warp loads, two groups of four warps hold a row per thread and make P,
+// each with its own S and O and a warp that issues its products, and one warp
+// sees to the nodes:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
@@ -25,8 +25,6 @@
 // group rescales O in tensor memory. Rows of V outside the range may hold
 // anything and are zeroed in shared memory (0 * NaN is NaN); scores there are
 // replaced.
-#include <type_traits>
-
 #include "sd_tree.cuh"
 
 namespace sd {
@@ -108,9 +106,11 @@ struct Waiter {
   }
 };
 
+// A wait names a phase by its parity: right as long as the phase before it is done and the one after it is not. So
+// what a group's products signal has a barrier per buffer, whose next use waits for what the group makes of this one.
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
-  uint64_t q_full[2], o_full[2], s_full[2][2], p_full[2][2], done;  // of a group; of a group's buffer
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2], done;  // of a group; of a group's buffer
   uint32_t tmem;
 };
 static_assert(sizeof(TileBars) <= kTreeTileBarBytes, "room in the layout");
@@ -135,17 +135,17 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   if (tid == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(bars->full + i, 1);
-      mbar_init(bars->empty + i, 1);
+      mbar_init(bars->empty + i, SHARED ? 2 : 1);  // groups that use the tile
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(bars->q_full + w, 128);
-      mbar_init(bars->o_full + w, 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->s_full[w][i], 1);
+        mbar_init(&bars->o_full[w][i], 1);
         mbar_init(&bars->p_full[w][i], 128);
       }
     }
-    mbar_init(&bars->done, 1);
+    mbar_init(&bars->done, 2);
     fence_mbar_init();
     prefetch_tensormap(&tmK);
     prefetch_tensormap(&tmV);
@@ -219,97 +219,64 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     if (wait.dead)  // what is under way lands in this CTA's shared memory
       for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
-  } else if (warp == 9) {  // ---- products ----
-    // Per group: segments that it took part in and halves, whose parities are those of its barriers; the stages of its
-    // next K and V, and their parities.
-    uint32_t seg0 = 0, seg1 = 0, k0 = 0, k1 = 0;
-    struct Ring {
-      int st, par, n;
-      __device__ __forceinline__ void go(int by) {  // by: at most n
-        st += by;
-        if (st >= n) st -= n, par ^= 1;
-      }
-    };
-    Ring rk[2], rv[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) rk[w].n = rv[w].n = p.stages;
-    const uint64_t desc0 = operand_desc(0, 16, 1024), vdesc0 = operand_desc(0, kHalf, 1024);
-    const uint32_t ring_a = smem_u32(ring) >> 4, q_a = smem_u32(qs) >> 4;
-    const uint32_t empty = smem_u32(bars->empty), s_full = smem_u32(bars->s_full), o_full = smem_u32(bars->o_full);
-    // scores of a half (h) of group w's next K; products with its weights
-    auto scores = [&](auto w_, int h) {
-      constexpr int w = decltype(w_)::value;
-      Ring& g = rk[w];
-      if (!wait(bars->full + g.st, uint32_t(g.par))) return;
-      tc_fence_after();
-      const uint64_t q = desc0 + q_a + w * (kStage >> 4);
-      const uint64_t kk = desc0 + ring_a + g.st * (kStage >> 4) + h * (kHalfT * 128 >> 4);
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        constexpr uint32_t idesc = product_desc<E>(kHalfT, false);
-        const int off = (c / 4) * (kHalf >> 4) + (c % 4) * 2;
-        mma_ss(tmem + kSCol + w * 128 + h * kHalfT, q + off, kk + off, idesc, c > 0);
-      }
-      mma_commit(s_full + (2 * w + h) * 8);
-      if (h == 1) {
-        if (!SHARED || w == 1) mma_commit(empty + g.st * 8);
-        g.go(SHARED ? 2 : 4);
-      }
-    };
-    auto values = [&](auto w_, int h, uint32_t half, bool add) {  // half: its number, over all segments
-      constexpr int w = decltype(w_)::value;
-      Ring& g = rv[w];
-      if (!wait(&bars->p_full[w][h], (half >> 1) & 1u) || !wait(bars->full + g.st, uint32_t(g.par))) return;
-      tc_fence_after();
-      const uint64_t v = vdesc0 + ring_a + g.st * (kStage >> 4) + h * (kHalfT * 128 >> 4);
-#pragma unroll
-      for (int c = 0; c < kHalfT / 16; ++c) {
-        constexpr uint32_t idesc = product_desc<E>(D, true);
-        mma_ts(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + h * kHalfT + c * 8, v + c * (2048 >> 4), idesc, add || c > 0);
-      }
-      mma_commit(o_full + w * 8);
-      if (h == 1) {
-        if (!SHARED || w == 1) mma_commit(empty + g.st * 8);
-        g.go(SHARED ? 2 : 4);
-      }
-    };
-    using W0 = std::integral_constant<int, 0>;
-    using W1 = std::integral_constant<int, 1>;
+  } else if (warp == 9 || warp == 10) {  // ---- products of a group ----
+    const int w = warp - 9;
+    uint32_t seg = 0, k = 0;  // segments that the group took part in and halves: the parities of its barriers
+    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + w * kStage) >> 4);
+    const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
+    const uint32_t ds = tmem + kSCol + w * 128, dO = tmem + kOCol + w * 128;
+    const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full[w]);
     while (walk.next(s)) {
-      const int nt = s.i1 - s.i0, n0 = SHARED ? 2 * nt : 2 * ((nt + 1) / 2), n1 = SHARED ? n0 : 2 * (nt / 2);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int u = 2 * (it0 + (SHARED ? 0 : w));
-        rk[w].st = u % p.stages, rk[w].par = (u / p.stages) & 1;
-        rv[w].st = (u + 1) % p.stages, rv[w].par = ((u + 1) / p.stages) & 1;
-      }
-      // In turn: P V of half i of the first group, the scores of half i + 1 of the second, P V of its half i, the scores
-      // of half i + 2 of the first. Scores go where P of two halves before lies, whose product has to be done; the first
-      // ones of a segment want the group's rows of Q instead, and with those it has read what it needs of its last S
-      // and O. A group without tiles (a segment of one) loads no rows: it could run ahead by more than a phase.
+      const int nt = s.i1 - s.i0, n = SHARED ? 2 * nt : 2 * ((nt + 1 - w) / 2);
+      // A group without tiles (a segment of one) loads no rows of Q: it could run ahead by more than a phase.
+      if (n > 0) wait(bars->q_full + w, seg++ & 1u);
+      const int u = 2 * (it0 + (SHARED ? 0 : w));
+      int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
+      // P V of half i, then the scores of half i + 2 in the place of its P. The first ones follow the rows of Q: with
+      // those the group has read what it needs of its last S and O.
 #pragma unroll 1
-      for (int i = -2; i < n0 && !wait.dead; ++i) {
+      for (int i = -2; i < n && !wait.dead; ++i) {
         const int h = i & 1;
-        if (i >= 0) values(W0{}, h, k0 + i, i > 0);
-        if (i + 1 >= 0 && i + 1 < n1) {
-          if (i < 0) wait(bars->q_full + 1, seg1++ & 1u);
-          else if (i > 0) wait(bars->o_full + 1, (k1 + i - 1) & 1u);
-          if (!wait.dead) scores(W1{}, h ^ 1);
+        if (i >= 0) {
+          if (!wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u) || !wait(bars->full + vs, uint32_t(vp))) break;
+          tc_fence_after();
+          const uint64_t v = vd0 + vs * (kStage >> 4) + h * (kHalfT * 128 >> 4);
+          const uint32_t pp = ds + h * kHalfT;
+#pragma unroll
+          for (int c = 0; c < kHalfT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
+          mma_commit(o_full + h * 8);
+          if (h == 1) {
+            mma_commit(empty + vs * 8);
+            vs += SHARED ? 2 : 4;
+            if (vs >= p.stages) vs -= p.stages, vp ^= 1;
+          }
         }
-        if (i >= 0 && i < n1 && !wait.dead) values(W1{}, h, k1 + i, i > 0);
-        if (i + 2 < n0) {
-          if (i == -2) wait(bars->q_full, seg0++ & 1u);
-          else if (i >= 0) wait(bars->o_full, (k0 + i) & 1u);
-          if (!wait.dead) scores(W0{}, h);
+        if (i + 2 < n) {
+          if (i >= 0 && !wait(&bars->o_full[w][h], ((k + i) >> 1) & 1u)) break;
+          if (!wait(bars->full + ks, uint32_t(kp))) break;
+          tc_fence_after();
+          const uint64_t kd = kd0 + ks * (kStage >> 4) + h * (kHalfT * 128 >> 4);
+          const uint32_t d = ds + h * kHalfT;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            const int off = (c / 4) * (kHalf >> 4) + (c % 4) * 2;
+            mma_ss(d, q + off, kd + off, product_desc<E>(kHalfT, false), c > 0);
+          }
+          mma_commit(s_full + h * 8);
+          if (h == 1) {
+            mma_commit(empty + ks * 8);
+            ks += SHARED ? 2 : 4;
+            if (ks >= p.stages) ks -= p.stages, kp ^= 1;
+          }
         }
       }
-      k0 += n0, k1 += n1;
+      k += n;
       it0 += nt;
     }
     mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
     mbar_wait(&bars->done, 0, p.flags);
-  } else if (warp >= 10) {
-    tree_nodes<E, 0, D>(p, 2 * blockIdx.x + warp - 10, 2 * gridDim.x);
+  } else if (warp == 11) {
+    tree_nodes<E, 0, D>(p, blockIdx.x, gridDim.x);
   } else {  // ---- weights: a row per thread ----
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
@@ -353,7 +320,25 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const int h = steps & 1, tile = (steps >> 1) * each + (SHARED ? 0 : w);  // of the segment
         const int tok = (t0 + s.i0 + tile) * kTileT + h * kHalfT, lo = sq.begin - tok, hi = sq.held - tok;
         const uint32_t sh = ts + h * kHalfT;
-        if (!wait(&bars->s_full[w][h], (k >> 1) & 1u)) continue;
+        const bool ends = lo > 0 || hi < kHalfT;
+        const bool here = wait(&bars->s_full[w][h], (k >> 1) & 1u);
+        if (ends && here && (!SHARED || w == 0)) {
+          const int u = 2 * (it0 + tile) + 1;
+          if (wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
+            const int row = r >> 1;  // of the half; a thread zeroes half of it
+            if (row < lo || row >= hi) {
+              const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
+#pragma unroll
+              for (int c = 0; c < NH * 4; ++c) {
+                const int cc = (r & 1) * NH * 4 + c;
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + (cc / 8) * kHalf + (cc % 8) * 16), "r"(0) : "memory");
+              }
+            }
+            fence_proxy_async_shared();
+          }
+        }
+        if (SHARED && ends) named_barrier(1, 256);  // the second group's product reads the rows, too
+        if (!here) continue;
         tc_fence_after();
         uint32_t va[32], vb[32];
         tmem_ld32(sh, va);
@@ -364,7 +349,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
           for (int j = 0; j < 32; ++j) va[j] ^= 0x80000000u, vb[j] ^= 0x80000000u;
         }
-        const bool ends = lo > 0 || hi < kHalfT;
         if (ends || tok < edge) {  // some are not seen
           const int from = max(lo, low - tok);
 #pragma unroll
@@ -387,7 +371,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
           const float fac = raise_max(m, top - kUp);
           l *= fac;
-          if (wait(bars->o_full + w, (k - 1) & 1u)) {
+          if (wait(&bars->o_full[w][h ^ 1], ((k - 1) >> 1) & 1u)) {
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -417,21 +401,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         weigh(vb, 1);
         tmem_st32(sh, two);
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (ends && (!SHARED || w == 0)) {
-          const int u = 2 * (it0 + tile) + 1;
-          if (wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
-            const int row = r >> 1;  // of the half; a thread zeroes half of it
-            if (row < lo || row >= hi) {
-              const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
-#pragma unroll
-              for (int c = 0; c < NH * 4; ++c) {
-                const int cc = (r & 1) * NH * 4 + c;
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + (cc / 8) * kHalf + (cc % 8) * 16), "r"(0) : "memory");
-              }
-            }
-            fence_proxy_async_shared();
-          }
-        }
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(&bars->p_full[w][h]);
@@ -439,8 +408,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
       float* part = tree_part(p, s.pair + int(blockIdx.x));
-      // both of the last products may be under way, and a wait for a phase takes the one before the last for it
-      if (steps > 0 && wait(bars->o_full + w, k & 1u) && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();
+      if (steps > 0 && wait(&bars->o_full[w][0], ((k - 1) >> 1) & 1u) && wait(&bars->o_full[w][1], ((k - 1) >> 1) & 1u)) tc_fence_after();
       const bool has = steps > 0 && !wait.dead;
       auto load = [&](int c, uint32_t (&o)[32]) {  // dimensions 32 c ..
         if (has) {
