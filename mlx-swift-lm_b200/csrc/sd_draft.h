@@ -69,7 +69,7 @@ struct TreeParams : PagedParams {
   int RT;                  // columns (node, query head) of a pair
   int part_floats;         // of one segment in the workspace: o [D / 4][RT][4], then (m, l) [RT]
   float* node_o;           // [N * Hq][D], of the nodes alone
-  float2* node_ml;         // [N * Hq]
+  float2* node_ml;         // [N * Hq]; null: the nodes are on the line
   FastDiv by_g;            // G
 };
 
@@ -99,10 +99,9 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
-// of four warps, a warp that issues products for each, a loading warp and one
-// for the nodes.
+// of four warps, a warp that issues products for each and a loading warp.
 constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
-constexpr int kTreeTileThreads = 384;
+constexpr int kTreeTileThreads = 352;
 constexpr int kTreeTileTokens = 128;
 constexpr int kTreeTileStages = 16, kTreeTileLeast = 4;  // a step's K and V, and the next one's K beside them
 constexpr int kTreeTileBarBytes = 512;

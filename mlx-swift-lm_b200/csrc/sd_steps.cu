@@ -86,7 +86,7 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   s->part_floats = paged_part_floats(s->columns, D);
   s->line_bytes = (int64_t(2) * (batch + 1) * 4 + 127) / 128 * 128;
   const int64_t all = int64_t(n_rows) * n_q_heads;
-  s->node_bytes = (all * 8 + 127) / 128 * 128 + all * D * 4;
+  s->node_bytes = s->tiles ? 0 : (all * 8 + 127) / 128 * 128 + all * D * 4;
   s->bytes = s->line_bytes + (s->pairs + s->ctas) * s->part_floats * 4 + s->node_bytes;
   if (s->pairs + s->ctas >= (int64_t(1) << 30)) return fail(SD_ERR_SHAPE, "too many rows at once (%d)", n_rows);
   return SD_OK;
@@ -226,8 +226,10 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.out = out;
   p.line = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.line_bytes);
-  p.node_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.bytes - s.node_bytes);
-  p.node_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.bytes - int64_t(n_rows) * n_q_heads * D * 4);
+  if (s.node_bytes) {
+    p.node_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.bytes - s.node_bytes);
+    p.node_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.bytes - int64_t(n_rows) * n_q_heads * D * 4);
+  }
   p.by_g.set(G);
   p.tables = tables;
   p.lengths = lengths;

@@ -11,16 +11,17 @@
 // The held tokens are the same for all nodes (but for the low end of a window),
 // the nodes are few and differ from row to row. So the work is in two parts that
 // know nothing of each other:
-//   * The held tokens: the (node, query head) columns of a kv head are cut into
-//     pairs of at most RT columns, and the pairs' tiles are one line that CTAs
-//     share equally, as in a decode (sd_paged.cuh). Every segment leaves (o, m, l)
-//     in the workspace. No mask at all.
+//   * The (node, query head) columns of a kv head are cut into pairs of at most
+//     RT columns, and the pairs' tiles of held tokens are one line that CTAs share
+//     equally, as in a decode (sd_paged.cuh). Every segment leaves (o, m, l) in
+//     the workspace. No mask at all.
 //   * The nodes: a warp that a CTA has for it takes a row and up to four query
 //     heads at a time and attends to the visible nodes alone, reading no other
 //     node's rows -- what lies there, not-a-numbers included, does not reach it.
 //     It runs beside the tiles' warps, whose time hides its chain of loads.
-// tree_attend_kernel and the tile kernel (sd_tree_tile.cu) do both, and
-// tree_merge_kernel joins a column's nodes and segments in CTA order.
+// tree_attend_kernel does both, and tree_merge_kernel joins a column's nodes and
+// segments in CTA order. The tile kernel of 16-bit pools (sd_tree_tile.cu) has
+// the nodes on the line, as a sequence's last tokens.
 // Results depend on no timing. Lengths, rows and tables are read on the device
 // only, so a captured graph serves growing sequences.
 #pragma once
@@ -33,7 +34,8 @@ namespace sd {
 // What one sequence has of a call. A sequence whose numbers cannot be is taken
 // for one without tokens, and its rows give zeros.
 struct TreeSeq {
-  int row0, n, held, begin;  // first row, nodes, tokens before them, first of those that any node sees
+  int row0, n, held;  // first row, nodes, tokens before them
+  int begin, end;     // the tokens on the line: from the first that any node sees, and up to the nodes or with them
   bool bad;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
@@ -45,6 +47,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
   s.n = s.bad ? 0 : int(n);
   s.held = s.n ? len - s.n : 0;
   s.begin = p.window > 0 && s.held >= p.window ? s.held - p.window + 1 : 0;
+  s.end = s.held + (p.node_ml ? 0 : s.n);
   return s;
 }
 // The sequence of row n < first[B]: the last b with first[b] <= n, which has rows.
@@ -56,10 +59,10 @@ __device__ __forceinline__ int tree_find(const TreeParams& p, int n) {
   }
   return b;
 }
-// The held tokens of sequence b, for the producer.
+// The tokens of sequence b on the line, for the producer.
 __device__ __forceinline__ TokenRange token_range(const TreeParams& p, int b) {
   const TreeSeq s = tree_seq(p, b);
-  return {s.begin, s.held};
+  return {s.begin, s.end};
 }
 __device__ __forceinline__ int tree_pairs(const TreeParams& p, const TreeSeq& s) {
   return (s.n * p.G + p.RT - 1) / p.RT * p.Hkv;
@@ -68,6 +71,21 @@ __device__ __forceinline__ int tree_pairs(const TreeParams& p, const TreeSeq& s)
 __device__ __forceinline__ int tree_low(const TreeParams& p, const TreeSeq& s, int node) {
   const int place = p.places ? __ldcg(p.places + s.row0 + node) : s.held + node;
   return p.window > 0 ? max(0, int(min(int64_t(place) + 1 - p.window, int64_t(s.held)))) : 0;
+}
+
+// The nodes that node i sees.
+__device__ __forceinline__ uint64_t tree_seen(const TreeParams& p, const TreeSeq& s, int node) {
+  uint64_t m = p.masks ? uint64_t(__ldcg(reinterpret_cast<const long long*>(p.masks) + s.row0 + node)) : (uint64_t(2) << node) - 1;
+  if (s.n < 64) m &= (uint64_t(1) << s.n) - 1;
+  if (p.window) {
+    const int64_t least = (p.places ? int64_t(__ldcg(p.places + s.row0 + node)) : int64_t(s.held) + node) - p.window;
+    if (least >= s.held)  // places are no lower than that
+      for (uint64_t left = m; left; left &= left - 1) {
+        const int j = __ffsll(left) - 1;
+        if ((p.places ? __ldcg(p.places + s.row0 + j) : s.held + j) <= least) m &= ~(uint64_t(1) << j);
+      }
+  }
+  return m;
 }
 
 // Units and pairs before each sequence, by all NT threads of the block; tmp: [2 * NT / 32].
@@ -79,7 +97,7 @@ __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* un
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
     const TreeSeq s = tree_seq(p, b);
-    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.held}, tile);
+    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.end}, tile);
     bad = bad || s.bad;
     units[b + 1] = np * nu;  // of the sequence, for now
     pairs[b + 1] = np;
@@ -485,11 +503,15 @@ __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(cons
   griddep_wait();
   if (!live) return;
   const int64_t row = int64_t(n) * p.Hq + int64_t(h) * p.G + g;
-  const float2 node = __ldcg(p.node_ml + row);
-  float4 O = __ldcg(reinterpret_cast<const float4*>(p.node_o + row * D) + d4);
-  float M = node.x, L = node.y;
+  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float M = -INFINITY, L = 0.0f;
+  if (p.node_ml) {
+    const float2 ml = __ldcg(p.node_ml + row);
+    M = ml.x, L = ml.y;
+    O = __ldcg(reinterpret_cast<const float4*>(p.node_o + row * D) + d4);
+  }
   const int i = n - s.row0;
-  if (i >= 0 && i < s.n && s.held > s.begin) {
+  if (i >= 0 && i < s.n && s.end > s.begin) {
     const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
     const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
     const int nu = (u1 - up) / np, y = i * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;

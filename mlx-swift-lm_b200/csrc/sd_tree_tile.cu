@@ -1,14 +1,13 @@
 // sd_tree_tile.cu -- attention of many (node, query head) columns per sequence
-// to the held tokens of 16-bit pools, on the fifth-generation tensor cores.
-// See sd_tree.cuh for what it is a part of.
+// of 16-bit pools, on the fifth-generation tensor cores. See sd_tree.cuh for what
+// it is a part of.
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
 // 128 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes
 // S's place there as the next product's left operand, Q, K and V are 128B-
 // swizzled tiles in shared memory (TMA, one box per page and 64 dimensions).
 // One warp loads, two groups of four warps hold a row per thread and make P,
-// each with its own S and O and a warp that issues its products, and one warp
-// sees to the nodes:
+// each with its own S and O and a warp that issues its products:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
@@ -22,9 +21,12 @@
 // where few tokens have the weight.
 //
 // The running maximum lags by up to kSlack, as in a decode; when it moves, its
-// group rescales O in tensor memory. Rows of V outside the range may hold
-// anything and are zeroed in shared memory (0 * NaN is NaN); scores there are
-// replaced.
+// group rescales O in tensor memory. The nodes are the sequence's last tokens: a
+// row's bits of them and the first token that it sees make 64 bits for a half,
+// and scores without theirs are replaced. But 0 * NaN is NaN: rows of V outside
+// the range may hold anything and are zeroed in shared memory, and so are
+// infinities and not-a-numbers in a node's row, which a row that does see the
+// node gets back at the end.
 #include "sd_tree.cuh"
 
 namespace sd {
@@ -108,6 +110,25 @@ struct Waiter {
 
 // A wait names a phase by its parity: right as long as the phase before it is done and the one after it is not. So
 // what a group's products signal has a barrier per buffer, whose next use waits for what the group makes of this one.
+
+// Whether one of the threads says so: a barrier of n threads.
+__device__ __forceinline__ bool barrier_or(int id, int n, bool p) {
+  int any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+      : "=r"(any) : "r"(int(p)), "r"(id), "r"(n) : "memory");
+  return any != 0;
+}
+// Makes zeros of those of a word's two values that are not finite; true if there was one.
+template <typename E>
+__device__ __forceinline__ bool finite2(uint32_t& w) {
+  constexpr uint32_t top = __is_same(E, __half) ? 0x7c00u : 0x7f80u;
+  const bool a = (w & top) == top, b = (w & (top << 16)) == (top << 16);
+  if (a) w &= 0xffff0000u;
+  if (b) w &= 0x0000ffffu;
+  return a || b;
+}
+
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2], done;  // of a group; of a group's buffer
@@ -177,7 +198,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     while (walk.next(s)) {
       const TreeSeq sq = tree_seq(p, s.b);
       const int* row = p.tables + int64_t(s.b) * p.W;
-      const int t0 = sq.begin / kTileT, last_slot = (sq.held - 1) >> p_log, first_slot = sq.begin >> p_log;
+      const int t0 = sq.begin / kTileT, last_slot = (sq.end - 1) >> p_log, first_slot = sq.begin >> p_log;
       auto load = [&](int slot) { return slot >= first_slot && slot <= last_slot ? row[slot] : -1; };
       int base = ((t0 + s.i0) * kTileT) >> p_log;
       int cur = load(base + lane), nxt = load(base + 32 + lane);
@@ -191,7 +212,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const int tj = tok + (lane < nb ? lane : 0) * pb, off = (tj >> p_log) - base;
         const int a = __shfl_sync(0xffffffffu, cur, off & 31), c = __shfl_sync(0xffffffffu, nxt, off & 31);
         const int page = off < 32 ? a : c;
-        const bool need = lane < nb && tj < sq.held && tj + pb > sq.begin;
+        const bool need = lane < nb && tj < sq.end && tj + pb > sq.begin;
         int y = oob_row;
         if (need) {
           if (page >= 0 && page < p.n_pages) y = int((int64_t(page) * p.Hkv + s.h) * p.P + (tj & (p.P - 1)));
@@ -275,8 +296,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
     mbar_wait(&bars->done, 0, p.flags);
-  } else if (warp == 11) {
-    tree_nodes<E, 0, D>(p, blockIdx.x, gridDim.x);
   } else {  // ---- weights: a row per thread ----
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
@@ -310,34 +329,43 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         tc_fence_before();
         mbar_arrive(bars->q_full + w);
       }
-      const int low = p.window && x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
+      const int low = x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
+      const uint64_t seen = x < cols.n ? tree_seen(p, sq, cols.node(x)) : 0;
       const int edge = __reduce_max_sync(0xffffffffu, low);
       float m = -INFINITY, l = 0.0f;
       int steps = 0;
+      bool odd = false;  // a node has a value that is not finite
       const int each = SHARED ? 1 : 2, n = 2 * ((s.i1 - s.i0 + (SHARED ? 0 : 1 - w)) / each);
 #pragma unroll 1
       for (; steps < n; ++steps, ++k) {
         const int h = steps & 1, tile = (steps >> 1) * each + (SHARED ? 0 : w);  // of the segment
-        const int tok = (t0 + s.i0 + tile) * kTileT + h * kHalfT, lo = sq.begin - tok, hi = sq.held - tok;
+        const int tok = (t0 + s.i0 + tile) * kTileT + h * kHalfT, lo = sq.begin - tok, hi = sq.end - tok;
         const uint32_t sh = ts + h * kHalfT;
-        const bool ends = lo > 0 || hi < kHalfT;
+        const int old = sq.held - tok;  // rows of the half before the nodes'
+        const bool ends = lo > 0 || old < kHalfT;
         const bool here = wait(&bars->s_full[w][h], (k >> 1) & 1u);
-        if (ends && here && (!SHARED || w == 0)) {
+        if (ends) {
+          bool mine = false;
           const int u = 2 * (it0 + tile) + 1;
-          if (wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
-            const int row = r >> 1;  // of the half; a thread zeroes half of it
-            if (row < lo || row >= hi) {
-              const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
-#pragma unroll
+          if (here && (!SHARED || w == 0) && wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
+            const int row = r >> 1;  // of the half; a thread has half of it
+            const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
+            if (row < lo || row >= old) {
+#pragma unroll 2
               for (int c = 0; c < NH * 4; ++c) {
                 const int cc = (r & 1) * NH * 4 + c;
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + (cc / 8) * kHalf + (cc % 8) * 16), "r"(0) : "memory");
+                const uint32_t a = at + (cc / 8) * kHalf + (cc % 8) * 16;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row >= old && row < hi) v = lds128(a);
+                mine |= finite2<E>(v.x) | finite2<E>(v.y) | finite2<E>(v.z) | finite2<E>(v.w);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
               }
             }
             fence_proxy_async_shared();
           }
+          // every group that uses the tile waits for the rows, dead or not
+          odd |= SHARED ? barrier_or(1, 256, mine) : barrier_or(2 + w, 128, mine);
         }
-        if (SHARED && ends) named_barrier(1, 256);  // the second group's product reads the rows, too
         if (!here) continue;
         tc_fence_after();
         uint32_t va[32], vb[32];
@@ -350,11 +378,14 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           for (int j = 0; j < 32; ++j) va[j] ^= 0x80000000u, vb[j] ^= 0x80000000u;
         }
         if (ends || tok < edge) {  // some are not seen
-          const int from = max(lo, low - tok);
+          auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };  // the first n rows
+          const uint64_t nodes = old >= 64 || old <= -64 ? 0 : old >= 0 ? seen << old : seen >> -old;
+          const uint64_t vis = (below(old) & ~below(max(lo, low - tok))) | nodes;
+          const uint32_t v0 = uint32_t(vis), v1 = uint32_t(vis >> 32);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            va[j] = j < from || j >= hi ? 0xff800000u : va[j];
-            vb[j] = j + 32 < from || j + 32 >= hi ? 0xff800000u : vb[j];
+            va[j] = v0 & (1u << j) ? va[j] : 0xff800000u;
+            vb[j] = v1 & (1u << j) ? vb[j] : 0xff800000u;
           }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -410,6 +441,23 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       float* part = tree_part(p, s.pair + int(blockIdx.x));
       if (steps > 0 && wait(&bars->o_full[w][0], ((k - 1) >> 1) & 1u) && wait(&bars->o_full[w][1], ((k - 1) >> 1) & 1u)) tc_fence_after();
       const bool has = steps > 0 && !wait.dead;
+      // A node's value that is not finite counts in the rows that see it.
+      auto add_odd = [&](int c, uint32_t (&o)[32]) {
+#pragma unroll 1
+        for (uint64_t left = x < cols.n ? seen : 0; left; left &= left - 1) {
+          const int t = sq.held + __ffsll(left) - 1, page = __ldcg(p.tables + int64_t(s.b) * p.W + t / p.P);
+          if (page < 0 || page >= p.n_pages) continue;
+          const int64_t row = (int64_t(page) * p.Hkv + s.h) * p.P + (t & (p.P - 1));
+          const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data) + row * (D / 2) + 16 * c;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float f[2];
+            unpack_word<E>(__ldcg(v + j), f);
+            if (!(fabsf(f[0]) < INFINITY)) o[2 * j] = __float_as_uint(__uint_as_float(o[2 * j]) + f[0]);
+            if (!(fabsf(f[1]) < INFINITY)) o[2 * j + 1] = __float_as_uint(__uint_as_float(o[2 * j + 1]) + f[1]);
+          }
+        }
+      };
       auto load = [&](int c, uint32_t (&o)[32]) {  // dimensions 32 c ..
         if (has) {
           tmem_ld32(to + 32 * c, o);
@@ -418,6 +466,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0;
         }
+        if (odd) add_odd(c, o);
       };
       if constexpr (SHARED) {
 #pragma unroll 1
