@@ -66,6 +66,7 @@ struct TreeParams : PagedParams {
   const uint8_t *k_data, *v_data;  // of this layer
   int* line;               // [2][B + 1]: units and pairs before each sequence
   int N, Hq;
+  int seg_units;           // see tree_units
   int RT;                  // columns (node, query head) of a pair
   int part_floats;         // of one segment in the workspace: o [D / 4][RT][4], then (m, l) [RT]
   float* node_o;           // [N * Hq][D], of the nodes alone
@@ -102,18 +103,22 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 // of four warps, a warp that issues products for each and a loading warp.
 constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
 constexpr int kTreeTileThreads = 352;
-constexpr int kTreeTileTokens = 128;
-constexpr int kTreeTileStages = 16, kTreeTileLeast = 4;  // a step's K and V, and the next one's K beside them
-constexpr int kTreeTileBarBytes = 512;
+constexpr int kTreeTileTokens = 64;
+constexpr int kTreeTileUnits = 8;  // beginning and ending a segment, in tiles
+constexpr int kTreeTileStages = 24, kTreeTileLeast = 4;
+constexpr int kTreeTileBarBytes = 640;
 constexpr int kTreeTileSmem = 232448 - 2048;  // beside 2 KB of static shared memory
 // For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
 const void* tree_tile_kernel_for(int dtype, int D, bool shared);
-constexpr PagedLayout tree_tile_layout(int batch, int D) {
-  const int stage = 128 * D * 2, pre = (2 * (batch + 1) + 2 * (kTreeTileThreads / 32)) * 4, pre128 = (pre + 127) / 128 * 128;
-  const int room = (kTreeTileSmem - 1024 - 2 * stage - pre128 - kTreeTileBarBytes) / stage;
+constexpr PagedLayout tree_tile_layout(int batch, int D, bool shared) {
+  const int stage = kTreeTileTokens * D * 2, q = 2 * 128 * D * 2, pre = (2 * (batch + 1) + 2 * (kTreeTileThreads / 32)) * 4, pre128 = (pre + 127) / 128 * 128;
+  const int room = (kTreeTileSmem - 1024 - q - pre128 - kTreeTileBarBytes) / stage;
   PagedLayout l{};
   l.stages = room < kTreeTileStages ? room : kTreeTileStages;
-  l.prefix_off = (2 + l.stages) * stage;
+  // Where the groups take tiles in turn, a stage stays with the K, or the V, of one of them: a wait for a stage names
+  // its phase by the parity, so whoever waits has to know that the phase before is done.
+  if (!shared) l.stages = l.stages / 4 * 4;
+  l.prefix_off = q + l.stages * stage;
   l.bar_off = l.prefix_off + pre128;
   l.bytes = l.bar_off + kTreeTileBarBytes + 1024;
   return l;

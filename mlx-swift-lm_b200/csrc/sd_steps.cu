@@ -47,7 +47,7 @@ struct TreeShape {
   PagedLayout lay;
   int tile, columns;  // tokens of a tile, columns of a pair
   bool tiles;         // the tile kernel
-  int ctas;
+  int ctas, seg_units;
   int64_t pairs;      // at most
   int part_floats;
   int64_t line_bytes, node_bytes, bytes;  // of the workspace: line, segments, the nodes' (m, l) and o
@@ -67,10 +67,11 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->attend = tree_tile_kernel_for(g->dtype, D, shared);
     s->threads = kTreeTileThreads;
     s->smem_most = kTreeTileSmem;
-    s->lay = tree_tile_layout(batch, D);
+    s->lay = tree_tile_layout(batch, D, shared);
     s->tile = kTreeTileTokens;
     s->columns = shared ? 256 : 128;
     s->ctas = sms;
+    s->seg_units = kTreeTileUnits;
   } else {
     s->attend = set.attend;
     s->threads = kTreeAttendThreads;
@@ -79,6 +80,7 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->tile = set.tile;
     s->columns = set.columns;
     s->ctas = 2 * sms;
+    s->seg_units = kSegmentUnits;
   }
   if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
   // a sequence's last pair may be almost empty; no more pairs than columns
@@ -208,7 +210,7 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   if (workspace_bytes < s.bytes)
     return fail(SD_ERR_CAPACITY, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)s.bytes);
   const int D = g->head_dim, G = n_q_heads / g->n_kv_heads;
-  const int64_t max_tiles = (int64_t(table_width) * g->page_size + s.tile - 1) / s.tile + kSegmentUnits;
+  const int64_t max_tiles = (int64_t(table_width) * g->page_size + s.tile - 1) / s.tile + s.seg_units;
   if (max_tiles * s.pairs >= (int64_t(1) << 31)) return fail(SD_ERR_SHAPE, "rows * table_width too large");
   const int64_t columns = int64_t(n_rows) * G, blocks = (columns + kTreeMergeCols - 1) / kTreeMergeCols * g->n_kv_heads;
   if (columns >= (int64_t(1) << 31) - kTreeMergeCols || blocks >= (int64_t(1) << 31))
@@ -254,6 +256,7 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.N = n_rows;
   p.window = window;
   p.RT = s.columns;
+  p.seg_units = s.seg_units;
   p.part_floats = s.part_floats;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.magic = 0x64006400u;

@@ -67,6 +67,10 @@ __device__ __forceinline__ TokenRange token_range(const TreeParams& p, int b) {
 __device__ __forceinline__ int tree_pairs(const TreeParams& p, const TreeSeq& s) {
   return (s.n * p.G + p.RT - 1) / p.RT * p.Hkv;
 }
+// Units of one pair on the line: what beginning and ending its segment costs, in tiles, and its tiles.
+__device__ __forceinline__ int tree_units(const TreeParams& p, const TreeSeq& s, int tile) {
+  return s.end > s.begin ? (s.end + tile - 1) / tile - s.begin / tile + p.seg_units : 0;
+}
 // The first token that node i sees: `place` is its position.
 __device__ __forceinline__ int tree_low(const TreeParams& p, const TreeSeq& s, int node) {
   const int place = p.places ? __ldcg(p.places + s.row0 + node) : s.held + node;
@@ -97,7 +101,7 @@ __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* un
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
     const TreeSeq s = tree_seq(p, b);
-    const int np = tree_pairs(p, s), nu = units_of({s.begin, s.end}, tile);
+    const int np = tree_pairs(p, s), nu = tree_units(p, s, tile);
     bad = bad || s.bad;
     units[b + 1] = np * nu;  // of the sequence, for now
     pairs[b + 1] = np;
@@ -135,10 +139,10 @@ struct TreeSegment {
 struct TreeWalk {
   using Seg = TreeSegment;
   const int *units, *pairs;
-  int Hkv, b, u, u1;
-  __device__ __forceinline__ TreeWalk(const int* un, const int* pr, int B, int hkv, int begin, int end)
-      : units(un), pairs(pr), Hkv(hkv), b(0), u(begin), u1(end) {
-    int hi = B;  // the largest b with units[b] <= u
+  int Hkv, seg_units, b, u, u1;
+  __device__ __forceinline__ TreeWalk(const TreeParams& p, const int* un, const int* pr, int begin, int end)
+      : units(un), pairs(pr), Hkv(p.Hkv), seg_units(p.seg_units), b(0), u(begin), u1(end) {
+    int hi = p.B;  // the largest b with units[b] <= u
     while (hi - b > 1) {
       const int mid = (b + hi) >> 1;
       if (units[mid] <= u) b = mid; else hi = mid;
@@ -154,8 +158,8 @@ struct TreeWalk {
       s.c = k - s.h * per;
       s.pair = pairs[b] + k;
       u += last - first;
-      s.i0 = max(first - kSegmentUnits, 0);
-      s.i1 = last - kSegmentUnits;
+      s.i0 = max(first - seg_units, 0);
+      s.i1 = last - seg_units;
       if (s.i1 > s.i0) return true;
     }
     return false;
@@ -413,7 +417,7 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   }
   const Pieces pieces(p, units[p.B]);
   if (int(blockIdx.x) >= pieces.n) return;
-  TreeWalk walk(units, pairs, p.B, p.Hkv, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
+  TreeWalk walk(p, units, pairs, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
 
   if (warp == kPagedWarps) {
     paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
@@ -516,7 +520,7 @@ __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(cons
     const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
     const int nu = (u1 - up) / np, y = i * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;
     const Pieces pieces(p, all);
-    const int a = up + k * nu, cta = pieces.of(a + kSegmentUnits), ns = pieces.of(a + nu - 1) - cta + 1;
+    const int a = up + k * nu, cta = pieces.of(a + p.seg_units), ns = pieces.of(a + nu - 1) - cta + 1;
     const float* part = tree_part(p, pp + k + cta);
 #pragma unroll 1
     for (int j0 = 0; j0 < ns; j0 += 8) {

@@ -3,22 +3,21 @@
 // it is a part of.
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
-// 128 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes
-// S's place there as the next product's left operand, Q, K and V are 128B-
-// swizzled tiles in shared memory (TMA, one box per page and 64 dimensions).
-// One warp loads, two groups of four warps hold a row per thread and make P,
-// each with its own S and O and a warp that issues its products:
+// 64 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes S's
+// place there as the next product's left operand, Q, K and V are 128B-swizzled
+// tiles in shared memory (TMA, one box per page and 64 dimensions). One warp
+// loads, two groups of four warps hold a row per thread and make P, each with its
+// own S and O and a warp that issues its products:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
 //     groups in turn, whose parts are joined at a segment's end.
-// A tile of 128 tokens is two halves. A group's S has a buffer for each, so that
-// it weighs one half while the products of the other run: O += P V, and then,
-// when that has read P, the scores of the next half in P's place.
-// P is one value of the element type: 128 x 128 products cost as much as their
-// exponentials, and a second half would cost as much again (SHARED). The sum
-// that O is divided by is made of the rounded values, so their errors cancel
-// where few tokens have the weight.
+// A group's S has two buffers, so that it weighs one tile while the products of
+// the other run: O += P V, and then, when that has read P, the scores of the next
+// tile but one in P's place. With tiles of 128 tokens and one buffer a group
+// waited longer for its products than it weighed.
+// P is one value of the element type: its products cost as much as its
+// exponentials, and a second half of it would cost as much again.
 //
 // The running maximum lags by up to kSlack, as in a decode; when it moves, its
 // group rescales O in tensor memory. The nodes are the sequence's last tokens: a
@@ -33,7 +32,8 @@ namespace sd {
 
 namespace {
 
-constexpr int kTileT = kTreeTileTokens, kHalfT = kTileT / 2;
+constexpr int kTileT = kTreeTileTokens;
+static_assert(kTileT == 64, "a row's bits of a tile are a mask's");
 constexpr int kTmemCols = 512;
 constexpr int kSCol = 0, kOCol = 256;  // tensor memory columns of the first group's S and O; the second's 128 on
 
@@ -111,6 +111,20 @@ struct Waiter {
 // A wait names a phase by its parity: right as long as the phase before it is done and the one after it is not. So
 // what a group's products signal has a barrier per buffer, whose next use waits for what the group makes of this one.
 
+// Two products and sums in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 // Whether one of the threads says so: a barrier of n threads.
 __device__ __forceinline__ bool barrier_or(int id, int n, bool p) {
   int any;
@@ -131,7 +145,8 @@ __device__ __forceinline__ bool finite2(uint32_t& w) {
 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2], done;  // of a group; of a group's buffer
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer
+  uint64_t started, done;
   uint32_t tmem;
 };
 static_assert(sizeof(TileBars) <= kTreeTileBarBytes, "room in the layout");
@@ -142,11 +157,12 @@ template <typename E, int D, bool SHARED>
 __global__ void __launch_bounds__(kTreeTileThreads, 1)
 tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV) {
-  constexpr int NH = D / 64, kHalf = 128 * 128, kStage = NH * kHalf;  // bytes: 128 rows x 64 elements; a tile of K or V
+  constexpr int NH = D / 64, kQHalf = 128 * 128, kHalf = kTileT * 128;  // bytes of 64 dimensions of Q, of a tile
+  constexpr int kQ = NH * kQHalf, kStage = NH * kHalf;
   constexpr float kUp = __is_same(E, __half) ? 7.0f : 0.0f;  // as in a decode: fp16 weights up to 2^(kUp + kSlack)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *qs = sm, *ring = sm + 2 * kStage;
+  uint8_t *qs = sm, *ring = sm + 2 * kQ;
   TileBars* bars = reinterpret_cast<TileBars*>(sm + p.bar_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
@@ -166,6 +182,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         mbar_init(&bars->p_full[w][i], 128);
       }
     }
+    mbar_init(&bars->started, 128);
     mbar_init(&bars->done, 2);
     fence_mbar_init();
     prefetch_tensormap(&tmK);
@@ -183,7 +200,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   const uint32_t tmem = bars->tmem;
   const Pieces pieces(p, units[p.B]);
   const bool work = int(blockIdx.x) < pieces.n;
-  TreeWalk walk(units, pairs, p.B, p.Hkv, work ? pieces.begin(blockIdx.x) : 0, work ? pieces.begin(blockIdx.x + 1) : 0);
+  TreeWalk walk(p, units, pairs, work ? pieces.begin(blockIdx.x) : 0, work ? pieces.begin(blockIdx.x + 1) : 0);
   TreeSegment s;
   int it0 = 0;  // tiles of the segments before
   Waiter wait{p.flags, false};
@@ -242,53 +259,52 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
   } else if (warp == 9 || warp == 10) {  // ---- products of a group ----
     const int w = warp - 9;
-    uint32_t seg = 0, k = 0;  // segments that the group took part in and halves: the parities of its barriers
-    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + w * kStage) >> 4);
+    uint32_t seg = 0, k = 0;  // segments that the group took part in and tiles: the parities of its barriers
+    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + w * kQ) >> 4);
     const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
     const uint32_t ds = tmem + kSCol + w * 128, dO = tmem + kOCol + w * 128;
     const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full[w]);
     while (walk.next(s)) {
-      const int nt = s.i1 - s.i0, n = SHARED ? 2 * nt : 2 * ((nt + 1 - w) / 2);
-      // A group without tiles (a segment of one) loads no rows of Q: it could run ahead by more than a phase.
-      if (n > 0) wait(bars->q_full + w, seg++ & 1u);
+      const int nt = s.i1 - s.i0, n = SHARED ? nt : (nt + 1 - w) / 2;
+      if (n > 0) {
+        // A group without tiles (a segment of one) loads no rows of Q: it could run ahead by more than a phase. The
+        // second group begins when the first has weighed its first tile: out of step, one's exponentials overlap the
+        // other's loads, maxima and stores.
+        if (w == 1 && k == 0) wait(&bars->started, 0);
+        wait(bars->q_full + w, seg++ & 1u);
+      }
       const int u = 2 * (it0 + (SHARED ? 0 : w));
       int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
-      // P V of half i, then the scores of half i + 2 in the place of its P. The first ones follow the rows of Q: with
+      // P V of tile i, then the scores of tile i + 2 in the place of its P. The first ones follow the rows of Q: with
       // those the group has read what it needs of its last S and O.
 #pragma unroll 1
       for (int i = -2; i < n && !wait.dead; ++i) {
-        const int h = i & 1;
+        const uint32_t h = (k + i) & 1u, use = (k + i) >> 1;  // buffer, and how often it was used (of i >= 0)
         if (i >= 0) {
-          if (!wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u) || !wait(bars->full + vs, uint32_t(vp))) break;
+          if (!wait(&bars->p_full[w][h], use & 1u) || !wait(bars->full + vs, uint32_t(vp))) break;
           tc_fence_after();
-          const uint64_t v = vd0 + vs * (kStage >> 4) + h * (kHalfT * 128 >> 4);
-          const uint32_t pp = ds + h * kHalfT;
+          const uint64_t v = vd0 + vs * (kStage >> 4);
+          const uint32_t pp = ds + h * kTileT;
 #pragma unroll
-          for (int c = 0; c < kHalfT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
+          for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
           mma_commit(o_full + h * 8);
-          if (h == 1) {
-            mma_commit(empty + vs * 8);
-            vs += SHARED ? 2 : 4;
-            if (vs >= p.stages) vs -= p.stages, vp ^= 1;
-          }
+          mma_commit(empty + vs * 8);
+          vs += SHARED ? 2 : 4;
+          if (vs >= p.stages) vs -= p.stages, vp ^= 1;
         }
         if (i + 2 < n) {
-          if (i >= 0 && !wait(&bars->o_full[w][h], ((k + i) >> 1) & 1u)) break;
+          if (i >= 0 && !wait(&bars->o_full[w][h], use & 1u)) break;
           if (!wait(bars->full + ks, uint32_t(kp))) break;
           tc_fence_after();
-          const uint64_t kd = kd0 + ks * (kStage >> 4) + h * (kHalfT * 128 >> 4);
-          const uint32_t d = ds + h * kHalfT;
+          const uint64_t kd = kd0 + ks * (kStage >> 4);
+          const uint32_t d = ds + h * kTileT;
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const int off = (c / 4) * (kHalf >> 4) + (c % 4) * 2;
-            mma_ss(d, q + off, kd + off, product_desc<E>(kHalfT, false), c > 0);
-          }
+          for (int c = 0; c < D / 16; ++c)
+            mma_ss(d, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<E>(kTileT, false), c > 0);
           mma_commit(s_full + h * 8);
-          if (h == 1) {
-            mma_commit(empty + ks * 8);
-            ks += SHARED ? 2 : 4;
-            if (ks >= p.stages) ks -= p.stages, kp ^= 1;
-          }
+          mma_commit(empty + ks * 8);
+          ks += SHARED ? 2 : 4;
+          if (ks >= p.stages) ks -= p.stages, kp ^= 1;
         }
       }
       k += n;
@@ -302,7 +318,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     const uint32_t ts = tmem + lanes + kSCol + w * 128, to = tmem + lanes + kOCol + w * 128;
     const bool neg = p.scale_log2 < 0.0f;
     const float sc = fmaxf(fabsf(p.scale_log2), 1.1754944e-38f);  // -inf times it stays -inf
-    uint32_t k = 0;  // halves of this group
+    uint32_t k = 0;  // tiles of this group
     while (walk.next(s)) {
       const TreeSeq sq = tree_seq(p, s.b);
       const NodeCols cols(p, sq, s.h, s.c);
@@ -310,7 +326,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       const int t0 = sq.begin / kTileT;
       if (SHARED || s.i0 + w < s.i1) {  // Q: a thread has one 16-byte chunk of every eighth (or sixteenth) row
         constexpr int CPR = D / 8, RPT = 128 / CPR, N = 128 / RPT;
-        const uint32_t q = smem_u32(qs) + w * kStage;
+        const uint32_t q = smem_u32(qs) + w * kQ;
         const int ch = r % CPR;
         uint4 v[N];
 #pragma unroll
@@ -322,7 +338,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int row = r / CPR + RPT * i;
-          const uint32_t at = q + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+          const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
         }
         fence_proxy_async_shared();
@@ -335,21 +351,24 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       float m = -INFINITY, l = 0.0f;
       int steps = 0;
       bool odd = false;  // a node has a value that is not finite
-      const int each = SHARED ? 1 : 2, n = 2 * ((s.i1 - s.i0 + (SHARED ? 0 : 1 - w)) / each);
+      const int n = SHARED ? s.i1 - s.i0 : (s.i1 - s.i0 + 1 - w) / 2;
 #pragma unroll 1
       for (; steps < n; ++steps, ++k) {
-        const int h = steps & 1, tile = (steps >> 1) * each + (SHARED ? 0 : w);  // of the segment
-        const int tok = (t0 + s.i0 + tile) * kTileT + h * kHalfT, lo = sq.begin - tok, hi = sq.end - tok;
-        const uint32_t sh = ts + h * kHalfT;
-        const int old = sq.held - tok;  // rows of the half before the nodes'
-        const bool ends = lo > 0 || old < kHalfT;
-        const bool here = wait(&bars->s_full[w][h], (k >> 1) & 1u);
-        if (ends) {
+        const int tile = SHARED ? steps : 2 * steps + w;  // of the segment
+        const int tok = (t0 + s.i0 + tile) * kTileT, lo = sq.begin - tok, hi = sq.end - tok;
+        const uint32_t h = k & 1u, use = k >> 1, sh = ts + h * kTileT;
+        const int old = sq.held - tok;  // rows of the tile before the nodes'
+        const bool ends = lo > 0 || old < kTileT;
+        // Every group that uses the tile waits for its rows, dead or not; the second one before its own scores, which may
+        // wait for the first.
+        if (SHARED && ends && w == 1) odd |= barrier_or(1, 256, false);
+        const bool here = wait(&bars->s_full[w][h], use & 1u);
+        if (ends && (!SHARED || w == 0)) {
           bool mine = false;
           const int u = 2 * (it0 + tile) + 1;
-          if (here && (!SHARED || w == 0) && wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
-            const int row = r >> 1;  // of the half; a thread has half of it
-            const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + (h * kHalfT + row) * 128;
+          if (here && wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
+            const int row = r >> 1;  // a thread has half of it
+            const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + row * 128;
             if (row < lo || row >= old) {
 #pragma unroll 2
               for (int c = 0; c < NH * 4; ++c) {
@@ -363,7 +382,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             }
             fence_proxy_async_shared();
           }
-          // every group that uses the tile waits for the rows, dead or not
           odd |= SHARED ? barrier_or(1, 256, mine) : barrier_or(2 + w, 128, mine);
         }
         if (!here) continue;
@@ -390,11 +408,11 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          mx[0] = fmaxf(mx[0], __uint_as_float(va[j]));
-          mx[1] = fmaxf(mx[1], __uint_as_float(va[j + 1]));
-          mx[2] = fmaxf(mx[2], __uint_as_float(vb[j]));
-          mx[3] = fmaxf(mx[3], __uint_as_float(vb[j + 1]));
+        for (int j = 0; j < 32; j += 4) {  // maxima of three
+          mx[0] = fmaxf(fmaxf(mx[0], __uint_as_float(va[j])), __uint_as_float(va[j + 1]));
+          mx[1] = fmaxf(fmaxf(mx[1], __uint_as_float(va[j + 2])), __uint_as_float(va[j + 3]));
+          mx[2] = fmaxf(fmaxf(mx[2], __uint_as_float(vb[j])), __uint_as_float(vb[j + 1]));
+          mx[3] = fmaxf(fmaxf(mx[3], __uint_as_float(vb[j + 2])), __uint_as_float(vb[j + 3]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         if (steps == 0) {
@@ -402,7 +420,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
           const float fac = raise_max(m, top - kUp);
           l *= fac;
-          if (wait(&bars->o_full[w][h ^ 1], ((k - 1) >> 1) & 1u)) {
+          if (wait(&bars->o_full[w][h ^ 1], ((k - 1) >> 1) & 1u)) {  // the last product
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -415,31 +433,32 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             }
           }
         }
-        const float mm = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m, -m), sc2 = make_float2(sc, sc);
+        float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         uint32_t two[32];
         auto weigh = [&](const uint32_t (&v)[32], int c) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            two[16 * c + j] = pack2<E>(ex2(fmaf(__uint_as_float(v[2 * j]), sc, -mm)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), sc, -mm)));
-            float g[2];
-            unpack_word<E>(two[16 * c + j], g);
-            sum[2 * (j & 1)] += g[0];
-            sum[2 * (j & 1) + 1] += g[1];
+            float2 e = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc2, mm);
+            e.x = ex2(e.x), e.y = ex2(e.y);
+            two[16 * c + j] = pack2<E>(e.x, e.y);
+            sum[j & 1] = add2(sum[j & 1], e);
           }
         };
         weigh(va, 0);
         weigh(vb, 1);
         tmem_st32(sh, two);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(&bars->p_full[w][h]);
+        if (w == 0 && k == 0) mbar_arrive(&bars->started);
       }
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
       float* part = tree_part(p, s.pair + int(blockIdx.x));
-      if (steps > 0 && wait(&bars->o_full[w][0], ((k - 1) >> 1) & 1u) && wait(&bars->o_full[w][1], ((k - 1) >> 1) & 1u)) tc_fence_after();
+      if (steps > 1) wait(&bars->o_full[w][k & 1u], ((k - 2) >> 1) & 1u);
+      if (steps > 0 && wait(&bars->o_full[w][(k - 1) & 1u], ((k - 1) >> 1) & 1u)) tc_fence_after();
       const bool has = steps > 0 && !wait.dead;
       // A node's value that is not finite counts in the rows that see it.
       auto add_odd = [&](int c, uint32_t (&o)[32]) {
@@ -482,8 +501,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       } else {
         // each group finishes half of the dimensions and hands the other half over, in the place of Q: no score of this
         // segment is still to come
-        uint4* swap = reinterpret_cast<uint4*>(qs + w * kStage);  // [D / 8][128]
-        const uint4* from = reinterpret_cast<const uint4*>(qs + (1 - w) * kStage);
+        uint4* swap = reinterpret_cast<uint4*>(qs + w * kQ);  // [D / 8][128]
+        const uint4* from = reinterpret_cast<const uint4*>(qs + (1 - w) * kQ);
         named_barrier(1, 256);
         ml_of[w][r] = make_float2(m, l);
 #pragma unroll 1
