@@ -3,19 +3,17 @@
 // it is a part of.
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
-// 64 tokens), P = 2^(S - m), O += P V. S and O live in tensor memory, P takes S's
-// place there as the next product's left operand, Q, K and V are 128B-swizzled
-// tiles in shared memory (TMA, one box per page and 64 dimensions). One warp
+// 64 tokens), P = 2^(S - m), O += P V. S, P -- the second product's left operand --
+// and O live in tensor memory, Q, K and V are 128B-swizzled tiles in shared memory (TMA, one box per page and 64 dimensions). One warp
 // loads, two groups of four warps hold a row per thread and make P, each with its
 // own S and O and a warp that issues its products:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
 //     groups in turn, whose parts are joined at a segment's end.
-// A group's S has two buffers, so that it weighs one tile while the products of
-// the other run: O += P V, and then, when that has read P, the scores of the next
-// tile but one in P's place. With tiles of 128 tokens and one buffer a group
-// waited longer for its products than it weighed.
+// P has two buffers beside S, so that the scores of the next tile are made as
+// soon as this one's have been read, and P V while the next is weighed: no
+// product waits for another one to end.
 // P is one value of the element type: its products cost as much as its
 // exponentials, and a second half of it would cost as much again.
 //
@@ -35,7 +33,8 @@ namespace {
 constexpr int kTileT = kTreeTileTokens;
 static_assert(kTileT == 64, "a row's bits of a tile are a mask's");
 constexpr int kTmemCols = 512;
-constexpr int kSCol = 0, kOCol = 256;  // tensor memory columns of the first group's S and O; the second's 128 on
+// Tensor memory columns of the first group's S, its P's two buffers, and its O; the second's are 128 on.
+constexpr int kSCol = 0, kPCol = 64, kOCol = 256;
 
 // --- tensor core pieces -----------------------------------------------------
 
@@ -99,17 +98,28 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
 }
 
 // --- waits: bounded; the answer is the warp's, as the tensor memory accesses are ---
+// A wait that has to go on is out of line: every instruction in the loops here is fetched again for each tile.
+static __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* flags) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
+}
 struct Waiter {
   int* flags;
   bool dead;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) {
-    if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
+    if (!dead && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) dead = !wait_on(bar, parity, flags);
     return !dead;
   }
 };
 
+// One arrival for a warp, after what its lanes did: a barrier takes some three cycles for each, and 128 of them made
+// every signal between the warps 430 cycles late.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(smem_u32(bar))
+               : "memory");
+}
 // A wait names a phase by its parity: right as long as the phase before it is done and the one after it is not. So
-// what a group's products signal has a barrier per buffer, whose next use waits for what the group makes of this one.
+// what goes with P has a barrier per buffer, as the other buffer's may be a phase ahead.
 
 // Two products and sums in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -145,7 +155,7 @@ __device__ __forceinline__ bool finite2(uint32_t& w) {
 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer
+  uint64_t q_full[2], s_full[2], s_free[2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer of P
   uint64_t started, done;
   uint32_t tmem;
 };
@@ -175,14 +185,15 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       mbar_init(bars->empty + i, SHARED ? 2 : 1);  // groups that use the tile
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(bars->q_full + w, 128);
+      mbar_init(bars->q_full + w, 4);
+      mbar_init(bars->s_full + w, 1);
+      mbar_init(bars->s_free + w, 4);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars->s_full[w][i], 1);
         mbar_init(&bars->o_full[w][i], 1);
-        mbar_init(&bars->p_full[w][i], 128);
+        mbar_init(&bars->p_full[w][i], 4);
       }
     }
-    mbar_init(&bars->started, 128);
+    mbar_init(&bars->started, 4);
     mbar_init(&bars->done, 2);
     fence_mbar_init();
     prefetch_tensormap(&tmK);
@@ -262,8 +273,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     uint32_t seg = 0, k = 0;  // segments that the group took part in and tiles: the parities of its barriers
     const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + w * kQ) >> 4);
     const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
-    const uint32_t ds = tmem + kSCol + w * 128, dO = tmem + kOCol + w * 128;
-    const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full[w]);
+    const uint32_t ds = tmem + kSCol + w * 128, dp = tmem + kPCol + w * 128, dO = tmem + kOCol + w * 128;
+    const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full + w);
     while (walk.next(s)) {
       const int nt = s.i1 - s.i0, n = SHARED ? nt : (nt + 1 - w) / 2;
       if (n > 0) {
@@ -275,36 +286,34 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
       const int u = 2 * (it0 + (SHARED ? 0 : w));
       int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
-      // P V of tile i, then the scores of tile i + 2 in the place of its P. The first ones follow the rows of Q: with
-      // those the group has read what it needs of its last S and O.
+      // The scores of tile i + 1, then P V of tile i. The first scores follow the rows of Q: with those the group has
+      // read what it needs of its last S and O.
 #pragma unroll 1
-      for (int i = -2; i < n && !wait.dead; ++i) {
-        const uint32_t h = (k + i) & 1u, use = (k + i) >> 1;  // buffer, and how often it was used (of i >= 0)
+      for (int i = -1; i < n && !wait.dead; ++i) {
+        if (i + 1 < n) {
+          if (!wait(bars->full + ks, uint32_t(kp)) || (i >= 0 && !wait(bars->s_free + w, (k + i) & 1u))) break;
+          tc_fence_after();
+          const uint64_t kd = kd0 + ks * (kStage >> 4);
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c)
+            mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<E>(kTileT, false), c > 0);
+          mma_commit(s_full);
+          mma_commit(empty + ks * 8);
+          ks += SHARED ? 2 : 4;
+          if (ks >= p.stages) ks -= p.stages, kp ^= 1;
+        }
         if (i >= 0) {
-          if (!wait(&bars->p_full[w][h], use & 1u) || !wait(bars->full + vs, uint32_t(vp))) break;
+          const uint32_t h = (k + i) & 1u;  // buffer of P
+          if (!wait(bars->full + vs, uint32_t(vp)) || !wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u)) break;
           tc_fence_after();
           const uint64_t v = vd0 + vs * (kStage >> 4);
-          const uint32_t pp = ds + h * kTileT;
+          const uint32_t pp = dp + h * (kTileT / 2);
 #pragma unroll
           for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
           mma_commit(o_full + h * 8);
           mma_commit(empty + vs * 8);
           vs += SHARED ? 2 : 4;
           if (vs >= p.stages) vs -= p.stages, vp ^= 1;
-        }
-        if (i + 2 < n) {
-          if (i >= 0 && !wait(&bars->o_full[w][h], use & 1u)) break;
-          if (!wait(bars->full + ks, uint32_t(kp))) break;
-          tc_fence_after();
-          const uint64_t kd = kd0 + ks * (kStage >> 4);
-          const uint32_t d = ds + h * kTileT;
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-            mma_ss(d, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<E>(kTileT, false), c > 0);
-          mma_commit(s_full + h * 8);
-          mma_commit(empty + ks * 8);
-          ks += SHARED ? 2 : 4;
-          if (ks >= p.stages) ks -= p.stages, kp ^= 1;
         }
       }
       k += n;
@@ -315,7 +324,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   } else {  // ---- weights: a row per thread ----
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
-    const uint32_t ts = tmem + lanes + kSCol + w * 128, to = tmem + lanes + kOCol + w * 128;
+    const uint32_t ts = tmem + lanes + kSCol + w * 128, tp = tmem + lanes + kPCol + w * 128, to = tmem + lanes + kOCol + w * 128;
     const bool neg = p.scale_log2 < 0.0f;
     const float sc = fmaxf(fabsf(p.scale_log2), 1.1754944e-38f);  // -inf times it stays -inf
     uint32_t k = 0;  // tiles of this group
@@ -343,7 +352,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
         fence_proxy_async_shared();
         tc_fence_before();
-        mbar_arrive(bars->q_full + w);
+        warp_arrive(bars->q_full + w);
       }
       const int low = x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
       const uint64_t seen = x < cols.n ? tree_seen(p, sq, cols.node(x)) : 0;
@@ -356,13 +365,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       for (; steps < n; ++steps, ++k) {
         const int tile = SHARED ? steps : 2 * steps + w;  // of the segment
         const int tok = (t0 + s.i0 + tile) * kTileT, lo = sq.begin - tok, hi = sq.end - tok;
-        const uint32_t h = k & 1u, use = k >> 1, sh = ts + h * kTileT;
+        const uint32_t h = k & 1u;  // buffer of P
         const int old = sq.held - tok;  // rows of the tile before the nodes'
         const bool ends = lo > 0 || old < kTileT;
         // Every group that uses the tile waits for its rows, dead or not; the second one before its own scores, which may
         // wait for the first.
         if (SHARED && ends && w == 1) odd |= barrier_or(1, 256, false);
-        const bool here = wait(&bars->s_full[w][h], use & 1u);
+        const bool here = wait(bars->s_full + w, k & 1u);
         if (ends && (!SHARED || w == 0)) {
           bool mine = false;
           const int u = 2 * (it0 + tile) + 1;
@@ -387,10 +396,12 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         if (!here) continue;
         tc_fence_after();
         uint32_t va[32], vb[32];
-        tmem_ld32(sh, va);
-        tmem_ld32(sh + 32, vb);
+        tmem_ld32(ts, va);
+        tmem_ld32(ts + 32, vb);
         tmem_wait(va);
         tmem_wait(vb);
+        tc_fence_before();
+        warp_arrive(bars->s_free + w);
         if (neg) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) va[j] ^= 0x80000000u, vb[j] ^= 0x80000000u;
@@ -447,12 +458,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         };
         weigh(va, 0);
         weigh(vb, 1);
-        tmem_st32(sh, two);
+        // the buffer's last product is done, too: what signalled these scores was issued after it and waits for both
+        tmem_st32(tp + h * (kTileT / 2), two);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(&bars->p_full[w][h]);
-        if (w == 0 && k == 0) mbar_arrive(&bars->started);
+        warp_arrive(&bars->p_full[w][h]);
+        if (w == 0 && k == 0) warp_arrive(&bars->started);
       }
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
