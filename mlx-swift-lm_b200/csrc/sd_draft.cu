@@ -58,8 +58,10 @@ __device__ __forceinline__ void store4(T* at, int64_t row, int n, const T (&v)[k
 // Bound by latency up to some ten thousand rows (a launch, the lengths, the
 // table), then by its stores: 16 bytes a row, 28 with a tree. Every CTA works out all sequences'
 // sums for itself (at most 4096) and then takes blocks of rows; a thread
-// finds its first row's sequence by bisection and goes on from there. A mask
-// is a walk up the tree, one cached load per ancestor. The pages taken are
+// finds its first row's sequence by bisection and goes on from there. Of trees a
+// warp takes a whole one: lane l has nodes l and l + 32, and six exchanges, each
+// of which doubles how far up a node has looked, make every mask (a walk up by
+// one load per ancestor took 50 us for 64 trees of 32). The pages taken are
 // written by the same launch where its CTAs can wait until all have read what
 // is held (one cluster of at most 8), and by a second one otherwise.
 // Measured as whole calls: see the table of the operators.
@@ -122,9 +124,67 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     const bool wide = ((reinterpret_cast<uintptr_t>(p.seq) | reinterpret_cast<uintptr_t>(p.positions) |
                         reinterpret_cast<uintptr_t>(p.places) | reinterpret_cast<uintptr_t>(p.slots) |
                         reinterpret_cast<uintptr_t>(p.masks)) & 15) == 0;
-    bool odd = false;  // a parent that does not come before its node
+    // page and slot of position `at` of sequence b
+    auto slot_of = [&](int b, int at) {
+      const int col = at >> p.page_shift;
+      const int page = col < have[b] ? __ldcg(p.tables + int64_t(b) * p.W + col) : __ldcg(p.free_pages + base[b] + col - have[b]);
+      return page < 0 ? int64_t(-1) : int64_t(page) * p.P + (at & (p.P - 1));
+    };
+    if (p.parents) {
+      const int lane = tid & 31, warps = gridDim.x * (kPlanThreads / 32);
+      bool odd = false;  // a parent that does not come before its node
+      for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < p.B; b += warps) {
+        const int n = first[b + 1] - first[b];
+        const int* up = p.parents + b * p.parents_stride;
+        uint32_t lo[2], hi[2];  // the masks' words
+        int next[2];            // the ancestor to look at from; -1: none, -2: there is no such node
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int node = lane + 32 * e;
+          next[e] = node < n ? __ldcg(up + node) : -2;
+          odd |= node < n && next[e] >= node;
+          if (next[e] < -1 || next[e] >= node) next[e] = -2;
+          lo[e] = e ? 0u : 1u << lane, hi[e] = e ? 1u << lane : 0u;
+        }
+        while (__any_sync(0xffffffffu, next[0] >= 0 || next[1] >= 0)) {  // six times at most
+          uint32_t l2[2], h2[2];
+          int n2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int from = max(next[e], 0), at = from & 31;
+            const bool far = from >= 32;
+            const uint32_t a = __shfl_sync(0xffffffffu, lo[0], at), c = __shfl_sync(0xffffffffu, lo[1], at);
+            const uint32_t d = __shfl_sync(0xffffffffu, hi[0], at), f = __shfl_sync(0xffffffffu, hi[1], at);
+            const int g = __shfl_sync(0xffffffffu, next[0], at), k = __shfl_sync(0xffffffffu, next[1], at);
+            l2[e] = far ? c : a, h2[e] = far ? f : d, n2[e] = far ? k : g;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (next[e] >= 0) lo[e] |= l2[e], hi[e] |= h2[e], next[e] = n2[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int node = lane + 32 * e;
+          if (node >= n) continue;
+          const int64_t r = first[b] + node;
+          const bool there = next[e] == -1;
+          p.seq[r] = b;
+          p.positions[r] = there ? len[b] + node : -1;
+          if (p.slots) p.slots[r] = there ? slot_of(b, len[b] + node) : -1;
+          if (p.places) p.places[r] = there ? len[b] + __popc(lo[e]) + __popc(hi[e]) - 1 : -1;
+          if (p.masks) p.masks[r] = there ? int64_t(uint64_t(hi[e]) << 32 | lo[e]) : 0;
+        }
+      }
+      for (int64_t r = int64_t(total) + blockIdx.x * kPlanThreads + tid; r < p.N; r += int64_t(gridDim.x) * kPlanThreads) {
+        p.seq[r] = p.positions[r] = -1;
+        if (p.slots) p.slots[r] = -1;
+        if (p.places) p.places[r] = -1;
+        if (p.masks) p.masks[r] = 0;
+      }
+      if (odd && p.flags) atomicOr(p.flags, kErrBadIndex);
+    }
     const int64_t step = int64_t(gridDim.x) * kPlanThreads * kPlanRows;
-    for (int64_t r0 = (int64_t(blockIdx.x) * kPlanThreads + tid) * kPlanRows; r0 < p.N; r0 += step) {
+    for (int64_t r0 = (int64_t(blockIdx.x) * kPlanThreads + tid) * kPlanRows; r0 < p.N && !p.parents; r0 += step) {
       const int cnt = int(min(int64_t(kPlanRows), p.N - r0));
       int seq[kPlanRows], pos[kPlanRows], place[kPlanRows];
       int64_t slot[kPlanRows], mask[kPlanRows];
@@ -144,30 +204,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         mask[i] = 0;
         if (i >= cnt || r >= total) continue;
         while (r >= first[b + 1]) ++b;  // ends: r < total
-        seq[i] = b;
         const int node = r - first[b], at = len[b] + node;
-        if (p.parents) {
-          const int* up = p.parents + b * p.parents_stride;
-          uint64_t m = 0;
-          int a = node, d = -1;
-          while (a >= 0) {  // ends: every parent taken lies before its node
-            m |= uint64_t(1) << a;
-            ++d;
-            const int next = __ldcg(up + a);
-            if (next >= a) odd = true;
-            a = next >= a ? -2 : next;
-          }
-          if (a != -1) continue;  // absent, or below an absent node
-          mask[i] = int64_t(m);
-          place[i] = len[b] + d;
-        } else {
-          place[i] = at;
-          mask[i] = int64_t((uint64_t(2) << min(node, kMaxNodes - 1)) - 1);
-        }
-        pos[i] = at;
-        const int col = at >> p.page_shift;
-        const int page = col < have[b] ? __ldcg(p.tables + int64_t(b) * p.W + col) : __ldcg(p.free_pages + base[b] + col - have[b]);
-        slot[i] = page < 0 ? -1 : int64_t(page) * p.P + (at & (p.P - 1));
+        seq[i] = b;
+        pos[i] = place[i] = at;
+        mask[i] = int64_t((uint64_t(2) << min(node, kMaxNodes - 1)) - 1);
+        slot[i] = slot_of(b, at);
       }
       store4(p.seq, r0, cnt, seq, wide);
       store4(p.positions, r0, cnt, pos, wide);
@@ -175,7 +216,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
       if (p.places) store4(p.places, r0, cnt, place, wide);
       if (p.masks) store4(p.masks, r0, cnt, mask, wide);
     }
-    if (odd && p.flags) atomicOr(p.flags, kErrBadIndex);
   }
   if (!p.commit) return;
   if (gridDim.x > 1) cluster_sync();  // every CTA has read what is held

@@ -158,7 +158,8 @@ int32_t sd_paged_plan(const sd_plan* g, int32_t* device_flags, sd_stream stream)
   p.slots = g->slots;
   p.masks = g->masks;
   p.flags = device_flags;
-  const int64_t threads = (int64_t(g->n_rows) + kPlanRows - 1) / kPlanRows;
+  // a thread per few rows, or a warp per tree
+  const int64_t threads = g->parents ? int64_t(g->batch) * 32 : (int64_t(g->n_rows) + kPlanRows - 1) / kPlanRows;
   const int grid = int(std::max<int64_t>(1, std::min<int64_t>((threads + kPlanThreads - 1) / kPlanThreads, 2 * sms)));
   const size_t smem = plan_smem(g->batch);
   const void* fn = plan_kernel_ptr();

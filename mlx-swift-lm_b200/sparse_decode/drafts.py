@@ -66,8 +66,8 @@ def paged_plan(lengths, new, tables, page_size: int, n_rows: int, *, parents=Non
         _p._load()
     torch, dev = _p.torch, _p._device()
     i32 = _p._I32
-    if tables.dim() != 2:
-        raise ValueError("tables must be [batch, width]")
+    if tables.dim() != 2 or tables.dtype is not i32:
+        raise ValueError("tables must be int32 [batch, width]")
     batch, width = tables.shape
     n_rows = _count(n_rows, "n_rows")
     if n_rows < 0:
@@ -88,9 +88,9 @@ def paged_plan(lengths, new, tables, page_size: int, n_rows: int, *, parents=Non
         n_free = _count(free.shape[0], "free")
     if stream is not None:
         with _on(stream):
-            p = _new_plan(torch, batch, n_rows, parents is not None, tables.device)
+            p = _new_plan(torch, batch, n_rows, parents is not None, tables)
     else:
-        p = _new_plan(torch, batch, n_rows, parents is not None, tables.device)
+        p = _new_plan(torch, batch, n_rows, parents is not None, tables)
     tree = parents is not None
     g = SDPlan(_arg(lengths, "lengths", i32, dev, (batch,)), _arg(new, "new", i32, dev, (batch,)),
                _arg(tables, "tables", i32, dev), _count(batch, "batch"), _count(width, "width"), page_size, n_rows,
@@ -102,13 +102,11 @@ def paged_plan(lengths, new, tables, page_size: int, n_rows: int, *, parents=Non
     return p
 
 
-def _new_plan(torch, batch: int, n_rows: int, tree: bool, device) -> TokenPlan:
-    p = TokenPlan()
-    new = lambda n, dt: torch.empty(n, dtype=dt, device=device)  # noqa: E731
-    i32, i64 = torch.int32, torch.int64
-    p.first, p.ends = new(batch + 1, i32), new(batch, i32)
-    p.seq, p.positions, p.slots = new(n_rows, i32), new(n_rows, i32), new(n_rows, i64)
-    p.places, p.masks = (new(n_rows, i32), new(n_rows, i64)) if tree else (p.positions, None)
+def _new_plan(torch, batch: int, n_rows: int, tree: bool, like) -> TokenPlan:
+    p, new, i64 = TokenPlan(), like.new_empty, torch.int64  # an allocation each: cutting one up costs the host more
+    p.first, p.ends, p.seq, p.positions = new(batch + 1), new(batch), new(n_rows), new(n_rows)
+    p.slots = new(n_rows, dtype=i64)
+    p.places, p.masks = (new(n_rows), new(n_rows, dtype=i64)) if tree else (p.positions, None)
     return p
 
 
