@@ -452,6 +452,7 @@ class PagePool:
                  dtype: str = "bf16", kv_bits: int = 0):
         if torch is None:
             _load()
+        self._forks: dict = {}  # how often each sequence was forked
         if kv_bits not in (0, 4, 8):
             raise ValueError("kv_bits must be 0, 4 or 8")
         lead = (n_layers, n_pages, n_kv_heads, page_size)
@@ -488,10 +489,12 @@ class PagePool:
     def fork(self, seq: int) -> int:
         s = ctypes.c_int64()
         _check(lib().sd_pagemap_fork(self._h, seq, ctypes.byref(s)))
+        self._forks[seq] = self._forks.get(seq, 0) + 1
         return s.value
 
     def free(self, seq: int) -> None:
         _check(lib().sd_pagemap_free(self._h, seq))
+        self._forks.pop(seq, None)
 
     def trim(self, seq: int, n: int) -> int:
         t = ctypes.c_int64()
@@ -568,11 +571,19 @@ class PagePool:
         return f
 
 
+# New tokens from which on a step's positions are made on the device: on the host 250 of them cost as much as the plan's
+# call and launch, a prompt of 32K tokens 7 ms.
+_PLAN_TOKENS = 256
+
+
 class PagedBatch:
     """One step of some sequences of a pool: `tables` [batch, width] and
     `lengths` [batch] with the step's new tokens counted in, and for the new
-    tokens, sequence by sequence, `positions` and `seq`. Built on the host and
-    copied to the device once, for every layer of the step."""
+    tokens, sequence by sequence, `positions` and `seq`. Built once, for every
+    layer of the step. `tree` makes drafted tokens of the new ones, and `keep`
+    ends such a step."""
+
+    plan = None  # of `tree`
 
     def __init__(self, pool: PagePool, seqs: list, new: list, stream=None):
         self.pool, self.seqs, self.new = pool, seqs, new
@@ -582,20 +593,101 @@ class PagedBatch:
         _check(lib().sd_pagemap_width(pool._h, ids, n, ctypes.byref(width)))
         w = width.value
         tokens = sum(new)
-        host = torch.empty(n * w + n + 2 * tokens, dtype=torch.int32, pin_memory=True)
+        planned = tokens >= _PLAN_TOKENS and n <= 4096
+        more = 2 * n if planned else 2 * tokens
+        host = torch.empty(n * w + n + more, dtype=torch.int32, pin_memory=True)
         i32p = ctypes.POINTER(ctypes.c_int32)
         at = lambda k: ctypes.cast(host.data_ptr() + 4 * k, i32p)  # noqa: E731
         _check(lib().sd_pagemap_tables(pool._h, ids, n, w, at(0), at(n * w)))
         lengths = host[n * w:n * w + n].tolist()
-        pos = [p for t, k in zip(lengths, new) for p in range(t - k, t)]
-        seq = [b for b, k in enumerate(new) for _ in range(k)]
-        host[n * w + n:] = torch.tensor(pos + seq, dtype=torch.int32)
+        if planned:
+            extra = [t - k for t, k in zip(lengths, new)] + new
+        else:
+            extra = [p for t, k in zip(lengths, new) for p in range(t - k, t)] + [b for b, k in enumerate(new) for _ in range(k)]
+        host[n * w + n:] = torch.tensor(extra, dtype=torch.int32)
         dev = _upload(host, stream)
         self.tables = dev[:n * w].view(n, w)
         self.lengths = dev[n * w:n * w + n]
-        self.positions = dev[n * w + n:n * w + n + tokens]
-        self.seq = dev[n * w + n + tokens:]
+        rest = dev[n * w + n:]
+        if planned:
+            from .drafts import paged_plan
+            p = paged_plan(rest[:n], rest[n:], self.tables, pool.pages.page_size, tokens, flags=pool.flags, stream=stream)
+            self.positions, self.seq = p.positions, p.seq
+        else:
+            self.positions, self.seq = rest[:tokens], rest[tokens:]
         self.host_lengths = lengths
+        self._forks = [pool._forks.get(s, 0) for s in seqs]
+
+    def tree(self, parents=None, stream=None) -> "PagedBatch":
+        """Make drafted tokens of the step's new ones: node i of a sequence has
+        the parent parents[i] (or parents[b][i]), a node before it or -1, the
+        last token of the ones before the step; below -1: there is no such
+        node. None: a chain. parents: lists, or an int32 tensor [nodes] or
+        [batch, nodes]. The layers of the step then rotate by places in the
+        tree and attend to ancestors; `positions` leaves out absent nodes.
+        Returns the batch."""
+        from .drafts import MAX_NODES, paged_plan
+        n, new = len(self.seqs), self.new
+        if max(new, default=0) > MAX_NODES:
+            raise ValueError(f"a tree has at most {MAX_NODES} nodes (got {max(new)})")
+        if parents is None:
+            parents = list(range(-1, max(new, default=0) - 1))
+        host = [t - k for t, k in zip(self.host_lengths, new)] + list(new)
+        if not isinstance(parents, torch.Tensor):
+            rows = parents if parents and not isinstance(parents[0], int) else [parents] * n
+            if len(rows) != n or any(len(r) < k for r, k in zip(rows, new)):
+                raise ValueError("parents must name one for every new token")
+            if any(p >= i for r, k in zip(rows, new) for i, p in enumerate(r[:k])):
+                raise ValueError("a parent comes before its node")
+            wide = max(1, max(new, default=0))
+            host += [p for r, k in zip(rows, new) for p in [*r[:k], *[-2] * (wide - k)]]
+            parents = None
+        elif parents.shape[-1] < max(new, default=0):
+            raise ValueError("parents must name one for every new token")
+        dev = _upload(torch.tensor(host, dtype=torch.int32).pin_memory(), stream)
+        if parents is None:
+            parents = dev[2 * n:].view(n, wide)
+        self.plan = paged_plan(dev[:n], dev[n:2 * n], self.tables, self.pool.pages.page_size, sum(new), parents=parents,
+                               flags=self.pool.flags, stream=stream)
+        self.positions, self.seq = self.plan.positions, self.plan.seq
+        return self
+
+    def attend_tree(self, layer: int, q, scale: Optional[float] = None, **kw):
+        """`paged_tree_decode` of the step's new tokens [tokens, Hq, D]."""
+        from .drafts import paged_tree_decode
+        p = self.plan
+        if p is None:
+            raise ValueError("the step has no tree")
+        return paged_tree_decode(q, self.pool.pages, self.tables, p.ends, p.first, p.masks, scale, places=p.places,
+                                 layer=layer, flags=self.pool.flags, **kw)
+
+    def keep(self, paths: Sequence[Sequence[int]], stream=None) -> None:
+        """End a tree's step: of sequence i the nodes paths[i], rising, are kept
+        and become its next tokens, in every layer, the others are dropped. The
+        step's calls must be on `stream` or waited for by it; the batch is
+        stale afterwards. Refused when a sequence has changed since the step
+        was made: a fork of it shares the pages that would be written."""
+        from .drafts import paged_keep
+        pool, p, n = self.pool, self.plan, len(self.seqs)
+        if p is None:
+            raise ValueError("the step has no tree")
+        paths = [[int(i) for i in x] for x in paths]
+        if len(paths) != n:
+            raise ValueError("one path per sequence")
+        for x, k in zip(paths, self.new):
+            if any(not 0 <= i < k for i in x) or any(a >= b for a, b in zip(x, x[1:])):
+                raise ValueError("a path names nodes in rising order")
+        if [pool._forks.get(s, 0) for s in self.seqs] != self._forks or \
+                [pool.length(s) for s in self.seqs] != self.host_lengths:
+            raise ValueError("a sequence of the step was forked, trimmed or extended since")
+        wide = max(1, max(map(len, paths), default=0))
+        host = [i for x in paths for i in [*x, *[-1] * (wide - len(x))]] + [len(x) for x in paths]
+        dev = _upload(torch.tensor(host, dtype=torch.int32).pin_memory(), stream)
+        paged_keep(pool.pages, self.tables, p.ends, p.first, dev[:n * wide].view(n, wide), dev[n * wide:],
+                   flags=pool.flags, stream=stream)
+        for s, x, k in zip(self.seqs, paths, self.new):
+            pool.trim(s, k - len(x))
+        self.plan = None
 
     def append(self, layer: int, k, v, q=None, **rotation):
         """`paged_append` of this step's new tokens [tokens, heads, D]."""
@@ -630,7 +722,8 @@ class PagedLayer:
 
     def attend(self, queries, keys, values, scale: float, mask=None, sinks=None):
         """Append keys/values [B, Hkv, L, D] and attend with queries
-        [B, Hq, L, D]; every sequence has L new tokens. L == 1 takes the decode
+        [B, Hq, L, D]; every sequence has L new tokens. A tree's step takes the
+        tree kernels, with mask None or "causal". L == 1 takes the decode
         kernel; longer prompts are attended densely, sequence by sequence, with
         `mask` as for the other caches: None hides nothing, "causal" the tokens
         after each one; a tensor (bool, or numbers to add) is broadcast to
@@ -642,6 +735,8 @@ class PagedLayer:
         B, Hq, L, D = queries.shape
         if any(n != L for n in b.new) or len(b.new) != B:
             raise ValueError(f"the step holds {b.new} new tokens, the queries {[L] * B}")
+        if b.plan is not None:
+            return self._attend_tree(queries, keys, values, scale, mask, sinks)
         if L == 1 and mask is not None and not isinstance(mask, str):
             raise ValueError("a single-token step takes no mask but \"causal\", which hides nothing there")
         masks = self._masks(mask, B, Hq, L)
@@ -660,6 +755,21 @@ class PagedLayer:
             k, v = self.dense(i)
             out[i] = _dense_attention(q[i:i + 1], k, v, scale, masks[i], sinks)[0]
         return out
+
+    def _attend_tree(self, queries, keys, values, scale: float, mask, sinks):
+        """A step of drafted tokens: rotated by their places in the tree, stored, and attended to their ancestors."""
+        if mask is not None and not (isinstance(mask, str) and mask == "causal"):
+            raise ValueError("the tree is the mask of a step of drafted tokens: pass none, or \"causal\"")
+        b = self.batch
+        B, Hq, L, D = queries.shape
+        flat = lambda x: x.transpose(1, 2).reshape(B * L, x.shape[1], D)  # noqa: E731
+        q, k = flat(queries), flat(keys)
+        if self.rotation:
+            q, k = rotary(q, k, b.plan.places, **{"inv_freq": None, **self.rotation})
+        b.append(self.index, k, flat(values))
+        sinks = None if sinks is None else sinks.detach().float().contiguous()
+        out = b.attend_tree(self.index, q.contiguous(), scale, window=self.window, sinks=sinks)
+        return out.view(B, L, Hq, D).transpose(1, 2)
 
     def _masks(self, mask, B: int, Hq: int, L: int) -> list:
         """The mask of each sequence."""

@@ -3,7 +3,8 @@
 Two prompts of different lengths go into a paged cache; one of them is forked
 (shared pages, copied when written); the three sequences decode together, each
 step rotating, storing and attending in every layer; then one is freed, the
-pool is compacted, and the rest decode on. Random weights stand in for a
+pool is compacted, and the rest decode on, in `drafts` rounds by trees of
+drafted tokens of which a path is kept. Random weights stand in for a
 model: what is shown is how the calls fit together. With --check, the last
 step's attention is compared with a plain computation over each sequence's
 own tokens.
@@ -14,7 +15,7 @@ import argparse
 
 
 def run(layers: int = 4, kv_bits: int = 0, prompts=(70, 33), steps: int = 20, page_size: int = 16, check: bool = False,
-        seed: int = 0):
+        seed: int = 0, drafts: int = 0):
     """Returns (pool, sequence ids, last outputs [sequences, Hq, D] per layer, largest error or None)."""
     import torch
 
@@ -51,6 +52,11 @@ def run(layers: int = 4, kv_bits: int = 0, prompts=(70, 33), steps: int = 20, pa
         step(pool.extend(seqs, 1), rand(len(seqs), 1, hidden))
     pool.free(seqs.pop(1))
     pool.compact()
+    parents = [-1, 0, 0, 1, 1, 2]  # two drafted tokens after the root, three after those
+    for i in range(drafts):
+        batch = pool.extend(seqs, len(parents)).tree(parents)
+        step(batch, rand(len(seqs), len(parents), hidden))
+        batch.keep([[0, 2, 5], [0, 1, 4]][i % 2:] + [[0]] * (len(seqs) - 2 + i % 2))  # what a sampler accepts
     last = {}
     for _ in range(steps):
         batch = pool.extend(seqs, 1)
@@ -76,9 +82,10 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--kv-bits", type=int, default=0, choices=(0, 4, 8))
     ap.add_argument("--steps", type=int, default=20)
+    ap.add_argument("--drafts", type=int, default=4)
     ap.add_argument("--check", action="store_true")
     a = ap.parse_args()
-    pool, seqs, outs, worst = run(kv_bits=a.kv_bits, steps=a.steps, check=a.check)
+    pool, seqs, outs, worst = run(kv_bits=a.kv_bits, steps=a.steps, check=a.check, drafts=a.drafts)
     print(f"sequences {[pool.length(s) for s in seqs]} tokens, {pool.free_pages} of {pool.pages.n_pages} pages free, "
           f"{len(outs)} layers" + (f", relative error {worst:.1e}" if worst is not None else ""))
 

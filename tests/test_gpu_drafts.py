@@ -506,3 +506,315 @@ def test_tree_reports_sequences_that_cannot_be(cuda):
     out, f = call(bad, [40, 40, 40, 40], [0, 6, 12, 18, 24])
     assert f == 2 and torch.isfinite(out).all()
     assert torch.equal(out[:6], want[:6]) and torch.equal(out[18:], want[18:])
+
+
+# ---------------------------------------------------------------------------
+# rounds
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 8), ("f32", 0)])
+def test_a_captured_round_serves_growing_sequences(cuda, dtype, bits):
+    """plan + append + attend + keep in one CUDA graph: lengths, pages and what is kept advance on the device."""
+    import sparse_decode as sd
+    torch = cuda
+    B, hkv, G, d, page, nodes, W = 3, 2, 4, 64, 16, 7, 12
+    n_pages = B * W
+    pool = Pool(torch, sd, dtype, bits, hkv, d, page, n_pages, 3)
+    lengths = i32(torch, [5, 31, 60])
+    held, taken = i32(torch, [1, 2, 4]), i32(torch, [0])
+    order = torch.randperm(n_pages, generator=gen(torch, 4), device="cuda").to(torch.int32)
+    tables = torch.full((B, W), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, h in enumerate([1, 2, 4]):
+        tables[b, :h] = order[at:at + h]
+        at += h
+    free = order[at:].clone()
+    parents = i32(torch, [-1, 0, 0, 1, 2, 2, 4])
+    new, path, kept = i32(torch, [7, 5, 6]), i32(torch, [[0, 2, 4, 6]] * B), i32(torch, [4, 3, 1])
+    x = torch.randn(B * nodes, (G + 2) * hkv, d, generator=gen(torch, 5), device="cuda").to(tdt(torch, dtype))
+    q, k, v = x[:, :G * hkv].contiguous(), x[:, G * hkv:(G + 1) * hkv], x[:, (G + 1) * hkv:]
+    flags = i32(torch, [0])
+    inv = (10000.0 ** (-torch.arange(0, d, 2, device="cuda") / d)).float()
+
+    def step():
+        p = sd.paged_plan(lengths, new, tables, page, B * nodes, parents=parents, held=held, free=free, taken=taken, flags=flags)
+        q2, k2 = sd.rotary(q, k, p.places, inv)
+        sd.paged_append(pool.pages, k2, v, tables, p.positions, seq=p.seq, flags=flags)
+        out = sd.paged_tree_decode(q2, pool.pages, tables, p.ends, p.first, p.masks, places=p.places, flags=flags)
+        sd.paged_keep(pool.pages, tables, p.ends, p.first, path, kept, lengths=lengths, flags=flags)
+        return p, q2, out
+    saved = [t.clone() for t in (lengths, tables, held, taken)]
+    step()
+    for t, old in zip((lengths, tables, held, taken), saved):
+        t.copy_(old)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p, q2, out = step()
+    now = [5, 31, 60]
+    lines = [lineage([-1, 0, 0, 1, 2, 2, 4][:n]) for n in (7, 5, 6)]
+    for rnd in range(4):
+        x.copy_(torch.randn(x.shape, generator=gen(torch, 10 + rnd), device="cuda"))
+        q.copy_(x[:, :G * hkv])
+        before = [stored(torch, pool, tables, b, n) for b, n in enumerate(now)]
+        g.replay()
+        torch.cuda.synchronize()
+        assert int(flags) == 0
+        assert p.first.tolist() == [0, 7, 12, 18] and p.positions.tolist()[18:] == [-1] * 3
+        assert p.ends.tolist() == [t + n for t, n in zip(now, (7, 5, 6))]
+        now = [t + n for t, n in zip(now, (4, 3, 1))]
+        assert lengths.tolist() == now
+        for b, n in enumerate(now):
+            after = stored(torch, pool, tables, b, n)
+            for x0, x1 in zip(before[b], after):
+                assert torch.equal(x0, x1[:, :x0.shape[1]])
+        # the round's attention, from the tokens before it and the drafted ones that were stored
+        row = 0
+        for b, n in enumerate((7, 5, 6)):
+            h = now[b] - (4, 3, 1)[b]
+            keys, vals = (t[:, :h] for t in stored(torch, pool, tables, b, now[b]))
+            for i in range(n):
+                seen = [j for j in range(n) if lines[b][i][0] >> j & 1]
+                if any(j not in (0, 2, 4, 6)[:(4, 3, 1)[b]] for j in seen):
+                    continue  # a node that was dropped is overwritten by now
+                new_at = [(0, 2, 4, 6).index(j) for j in seen]
+                both = [torch.cat((t, s[:, [h + j for j in new_at]]), 1) for t, s in
+                        zip((keys, vals), stored(torch, pool, tables, b, now[b]))]
+                s = torch.einsum("hgd,htd->hgt", q2[row + i].double().view(hkv, G, d), both[0]) / math.sqrt(d)
+                ref = torch.einsum("hgt,htd->hgd", torch.softmax(s, -1), both[1]).reshape(-1, d)
+                tol = {"bf16": 2e-2, "f16": 3e-3, "f32": 2e-5}[dtype]
+                assert float((out[row + i].double() - ref).norm() / ref.norm()) < tol
+            row += n
+
+
+def stored(torch, pool, tables, b, n):
+    """Keys and values of a sequence's first n tokens, [Hkv, n, D] in fp64, from the pool's arrays as they are now."""
+    at = tables[b, :-(-n // pool.page)].long()
+    got = []
+    for a in pool.arrays:
+        if pool.bits:
+            w = a[0][at].long() & 0xFFFFFFFF
+            c = torch.stack([(w >> (pool.bits * j)) & ((1 << pool.bits) - 1) for j in range(32 // pool.bits)], -1).flatten(-2)
+            x = c.double() * a[1][at].double().repeat_interleave(64, -1) + a[2][at].double().repeat_interleave(64, -1)
+        else:
+            x = a[0][at].double()
+        got.append(x.permute(1, 0, 2, 3).flatten(1, 2)[:, :n])
+    return got
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+def test_pool_keeps_the_accepted_tokens(cuda, bits):
+    """Tree steps through the router: outputs against single steps of the accepted path, and the pool afterwards."""
+    import sparse_decode as sd
+    from sparse_decode import attention_with_cache_update
+    torch = cuda
+    hq, hkv, d, page, layers = 8, 2, 64, 16, 2
+    inv, factor = sd.rotary_frequencies(d, 1e4)
+    turn = dict(inv_freq=inv, factor=factor)
+    g = gen(torch, 1)
+    rand = lambda n, h, m: torch.randn(n, h, m, d, generator=g, device="cuda").bfloat16()  # noqa: E731
+    pools = [sd.PagePool(layers, 60, hkv, d, page, "bf16", bits) for _ in range(2)]
+    seqs = [[p.add(), p.add()] for p in pools]
+    prompt = [(rand(1, hq, n), rand(1, hkv, n), rand(1, hkv, n)) for n in (300, 29)]
+    for p, ss in zip(pools, seqs):
+        for s, (q, k, v) in zip(ss, prompt):
+            step = p.extend([s], q.shape[2])
+            assert step.positions.tolist() == list(range(q.shape[2]))
+            for i in range(layers):
+                attention_with_cache_update(q, k, v, step.layer(i, **turn), d ** -0.5, "causal")
+    parents, paths = [-1, 0, 0, 1, 2, 4], [[0, 2, 4, 5], [0, 1]]
+    q, k, v = (rand(2, h, 6) for h in (hq, hkv, hkv))
+    step = pools[0].extend(seqs[0], 6).tree(parents)
+    got = [attention_with_cache_update(q, k, v, step.layer(i, window=40 * i, **turn), d ** -0.5) for i in range(layers)]
+    step.keep(paths)
+    assert [pools[0].length(s) for s in seqs[0]] == [304, 31]
+    for b, path in enumerate(paths):
+        for node in path:
+            one = pools[1].extend([seqs[1][b]], 1)
+            for i in range(layers):
+                ref = attention_with_cache_update(*(x[b:b + 1, :, node:node + 1] for x in (q, k, v)),
+                                                  one.layer(i, window=40 * i, **turn), d ** -0.5)
+                a, c = got[i][b, :, node].double(), ref[0, :, 0].double()
+                # two roundings of the output and one of the weights
+                assert float((a - c).abs().max()) <= 3 * 2.0 ** -8 * float(c.abs().max())
+    for p in pools:
+        assert p.check_device() == 0
+    for b in range(2):
+        views = [p.batch([ss[b]]).layer(1).dense(0) for p, ss in zip(pools, seqs)]
+        for x, y in zip(*views):
+            assert torch.equal(x, y)
+
+
+def test_pool_refuses_what_a_tree_cannot_be(cuda):
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 20, 2, 64, 16)
+    a, b = pool.add(), pool.add()
+    step = pool.extend([a, b], [3, 2])
+    for bad in ([0, 0, 1], [[-1, 0, 0], [-1]], [[-1, 0, 2], [-1, 0]], [-1, 0]):
+        with pytest.raises(ValueError):
+            step.tree(bad)
+    with pytest.raises(ValueError):
+        step.keep([[0], [0]])
+    with pytest.raises(ValueError):
+        step.attend_tree(0, cuda.zeros(5, 4, 64, device="cuda").bfloat16())
+    step.tree([[-1, -1, 1], [-1, 0]])
+    assert step.plan.masks.tolist() == [1, 2, 6, 1, 3] and step.plan.places.tolist() == [0, 0, 1, 0, 1]
+    for bad in ([[0]], [[0], [2]], [[1, 0], [0]], [[0, 0], []], [[-1], []]):
+        with pytest.raises(ValueError):
+            step.keep(bad)
+    with pytest.raises(ValueError):
+        sd.PagedLayer(step, 0, {}).attend(cuda.zeros(2, 4, 3, 64, device="cuda"), None, None, 1.0)  # ragged new tokens
+    c = pool.fork(a)
+    with pytest.raises(ValueError, match="forked"):
+        step.keep([[0], [0]])
+    pool.free(c)
+    step = pool.extend([b], 65)
+    with pytest.raises(ValueError):
+        step.tree()
+    pool.trim(b, 65)
+    step = pool.extend([b], 2).tree()
+    assert step.plan.masks.tolist() == [1, 3]
+    q = cuda.zeros(1, 4, 2, 64, device="cuda").bfloat16()
+    with pytest.raises(ValueError, match="mask"):
+        step.layer(0).attend(q, q[:, :2], q[:, :2], 1.0, mask=cuda.ones(2, 4, dtype=cuda.bool, device="cuda"))
+    step.layer(0).attend(q, q[:, :2], q[:, :2], 1.0, mask="causal")
+    step.keep([[]])
+    assert pool.length(b) == 2 and pool.check_device() == 0
+
+
+def test_a_plan_on_the_device_gives_the_positions_of_the_host(cuda):
+    import sparse_decode as sd
+    from sparse_decode import paged
+    pool = sd.PagePool(1, 200, 1, 64, 16)
+    seqs = [pool.add() for _ in range(3)]
+    pool.extend(seqs, [5, 0, 40])
+    step = pool.extend(seqs, [400, 1, 0])
+    assert sum(step.new) >= paged._PLAN_TOKENS
+    assert step.positions.tolist() == [*range(5, 405), 0] and step.seq.tolist() == [0] * 400 + [1]
+    assert step.lengths.tolist() == [405, 1, 40]
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+def test_example_drafts(cuda, bits):
+    from sparse_decode import paged_example
+    pool, seqs, outs, worst = paged_example.run(layers=2, kv_bits=bits, steps=3, drafts=4, check=True)
+    # prompts of 70, steps, drafts that keep three and three, or three and one, and steps again
+    assert [pool.length(s) for s in seqs] == [70 + 3 + 4 * 3 + 3, 70 + 3 + 2 * (3 + 1) + 3]
+    assert worst < 5e-3
+
+
+# ---------------------------------------------------------------------------
+# limits and refusals
+# ---------------------------------------------------------------------------
+
+def test_calls_on_two_streams_share_nothing(cuda):
+    import sparse_decode as sd
+    torch = cuda
+    rng = random.Random(3)
+    cases = []
+    for i, (dtype, bits, counts) in enumerate([("bf16", 0, [30, 9, 64]), ("bf16", 8, [4, 3, 1]), ("f16", 0, [64, 64, 64])]):
+        held = [2000, 31, 600]
+        ends = [h + n for h, n in zip(held, counts)]
+        pool = Pool(torch, sd, dtype, bits, 2, 128, 64, 60, 50 + i)
+        tables = tables_of(torch, ends, 64, 60, 52 + i)
+        first = [0, counts[0], counts[0] + counts[1], sum(counts)]
+        masks = [signed(m) for n in counts for m, _ in lineage(random_parents(rng, n))]
+        q = torch.randn(sum(counts), 8, 128, generator=gen(torch, 54 + i), device="cuda").to(tdt(torch, dtype))
+        args = (q, pool.pages, tables, i32(torch, ends), i32(torch, first), torch.tensor(masks, device="cuda"))
+        cases.append((args, sd.paged_tree_decode(*args), pool))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in cases], [[] for _ in cases]
+    for _ in range(6):
+        for i, (args, _, _) in enumerate(cases):
+            outs[i].append(sd.paged_tree_decode(*args, stream=streams[i]))
+    torch.cuda.synchronize()
+    for i, (_, want, _) in enumerate(cases):
+        assert all(torch.equal(o, want) for o in outs[i])
+
+
+def test_tree_offsets_past_32_bits(cuda):
+    """A pool of 9 GB: the last pages' rows lie past 2^32 bytes."""
+    import sparse_decode as sd
+    torch = cuda
+    n_pages, hkv, page, d = 70000, 4, 64, 128
+    k, v = (torch.zeros(n_pages, hkv, page, d, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    pages = sd.KVPages(k, v)
+    for counts, G in (([3], 4), ([40], 4)):
+        n = counts[0]
+        held = 100
+        tables = i32(torch, [[n_pages - 1, n_pages - 3, n_pages - 7]])
+        rows = torch.randn(held + n, hkv, 2 * d, generator=gen(torch, 3), device="cuda").bfloat16()
+        pos = torch.arange(held + n, device="cuda", dtype=torch.int32)
+        sd.paged_append(pages, rows[..., :d], rows[..., d:], tables, pos, seq=torch.zeros_like(pos))
+        q = torch.randn(n, hkv * G, d, generator=gen(torch, 4), device="cuda").bfloat16()
+        out = sd.paged_tree_decode(q, pages, tables, i32(torch, [held + n]), i32(torch, [0, n]))
+        kk, vv = (x.double().transpose(0, 1) for x in (rows[..., :d], rows[..., d:]))
+        s = torch.einsum("nhgd,htd->hngt", q.double().view(n, hkv, G, d), kk) / math.sqrt(d)
+        s = s.masked_fill(pos[None, None, None] > (held + torch.arange(n, device="cuda"))[None, :, None, None], -math.inf)
+        ref = torch.einsum("hngt,htd->nhgd", torch.softmax(s, -1), vv).reshape(n, -1, d)
+        assert float((out.double() - ref).norm() / ref.norm()) < 2.0 ** -8
+        kept = i32(torch, [2])
+        got = sd.paged_keep(pages, tables, i32(torch, [held + n]), i32(torch, [0, n]), i32(torch, [[0, n - 1]]), kept)
+        assert got.tolist() == [held + 2]
+        t = held + 1
+        assert torch.equal(k[int(tables[0, t // page]), :, t % page], rows[held + n - 1, :, :d])
+
+
+@pytest.mark.parametrize("dtype,bits,G", [("bf16", 0, 16), ("bf16", 8, 16), ("f32", 0, 4)])
+def test_tree_largest_batch(cuda, dtype, bits, G):
+    rng = random.Random(7)
+    run_tree(cuda, dtype, bits, 64, 1, G, 16, [rng.randint(0, 20) for _ in range(4096)], [rng.choice([0, 1, 3]) for _ in range(4096)], seed=5)
+
+
+def test_tree_scales_of_either_sign_and_none(cuda):
+    """Negative and zero scales reach both kernels."""
+    import sparse_decode as sd
+    torch = cuda
+    for n in (2, 20):
+        pool = Pool(torch, sd, "bf16", 0, 2, 64, 16, 30, 3)
+        tables = tables_of(torch, [300 + n], 16, 30, 4)
+        q = torch.randn(n, 8, 64, generator=gen(torch, 4), device="cuda").bfloat16()
+        for scale in (-0.2, 0.0):
+            out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [300 + n]), i32(torch, [0, n]), None, scale)
+            lines = [[((2 << i) - 1, 300 + i) for i in range(n)]]
+            ref, size = tree64(q, pool, tables, [300], lines, scale)
+            check_tree(torch, out, ref, size, "bf16", n * 4 > 16)
+
+
+def test_python_refusals(cuda):
+    import sparse_decode as sd
+    torch = cuda
+    pool = Pool(torch, sd, "bf16", 0, 2, 64, 16, 8, 3)
+    q, t = torch.zeros(4, 8, 64, device="cuda").bfloat16(), i32(torch, [[0, 1]])
+    ends, first = i32(torch, [20]), i32(torch, [0, 4])
+    masks = torch.ones(4, dtype=torch.int64, device="cuda")
+    tree = sd.paged_tree_decode
+    tree(q, pool.pages, t, ends, first, masks)
+    for args in ((q.float(), pool.pages, t, ends, first), (q.cpu(), pool.pages, t, ends, first), (q[..., :32], pool.pages, t, ends, first),
+                 (q.transpose(0, 1), pool.pages, t, ends, first), (q, pool.pages, t.long(), ends, first),
+                 (q, pool.pages, t, ends, first[:1]), (q, pool.pages, t, first, first), (q, pool.pages, t, ends, first, masks[:3]),
+                 (q, pool.pages, t, ends, first, masks.int())):
+        with pytest.raises((TypeError, ValueError)):
+            tree(*args)
+    for kw in (dict(window=-1), dict(layer=1), dict(scale=float("nan"))):
+        with pytest.raises(sd.SDError):
+            tree(q, pool.pages, t, ends, first, masks, **kw)
+    for kw in (dict(places=ends), dict(sinks=torch.zeros(7, device="cuda")), dict(out=q.float()), dict(window=1 << 31)):
+        with pytest.raises((TypeError, ValueError)):
+            tree(q, pool.pages, t, ends, first, masks, **kw)
+    with pytest.raises(sd.SDError):  # 17 query heads per kv head
+        tree(torch.zeros(1, 34, 64, device="cuda").bfloat16(), pool.pages, t, ends, i32(torch, [0, 1]))
+    plan = sd.paged_plan
+    for args, kw in (((ends, ends, t[0], 16, 4), {}), ((ends, ends, t, 16, 1 << 31), {}), ((ends, first, t, 16, 4), {}),
+                     ((ends, ends, t, 16, -1), {}), ((ends, ends, t, 16, 4), dict(held=ends)),
+                     ((ends, ends, t, 16, 4), dict(parents=t[None])), ((ends.cpu(), ends, t, 16, 4), {}),
+                     ((ends, ends, t.long(), 16, 4), {})):
+        with pytest.raises((TypeError, ValueError)):
+            plan(*args, **kw)
+    for page, kw in ((48, {}), (16, dict(parents=i32(torch, [-1] * 65)))):
+        with pytest.raises(sd.SDError):
+            plan(ends, ends, t, page, 4, **kw)
+    with pytest.raises(ValueError):
+        sd.paged_keep(pool.pages, t, ends, first, ends, ends)
+    with pytest.raises(sd.SDError):
+        sd.paged_keep(pool.pages, t, ends, first, i32(torch, [[0] * 65]), ends)
