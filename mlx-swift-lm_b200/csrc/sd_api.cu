@@ -54,7 +54,7 @@ EncodeTiledFn encode_fn() {
 // its boxes, landing as [box][row][box bytes] in shared memory. One TMA
 // operation per tile rather than one per box: the SM's TMA unit spends a fixed
 // time on each operation, which dominates copies of a few KB.
-int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole) {
+int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole, bool swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SD_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const int box_bytes = std::min(row_bytes, 128);
@@ -62,6 +62,7 @@ int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, in
   CUtensorMapSwizzle sw = box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                           : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                             : CU_TENSOR_MAP_SWIZZLE_32B;
+  if (!swizzle) sw = CU_TENSOR_MAP_SWIZZLE_NONE;
   cuuint64_t dims[3] = {cuuint64_t(box_bytes), cuuint64_t(rows), cuuint64_t(nbox)};
   cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(box_bytes)};
   cuuint32_t box[3] = {cuuint32_t(box_bytes), cuuint32_t(box_rows), cuuint32_t(whole ? nbox : 1)};

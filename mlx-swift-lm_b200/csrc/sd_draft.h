@@ -67,6 +67,7 @@ struct TreeParams : PagedParams {
   int* line;               // [2][B + 1]: units and pairs before each sequence
   int N, Hq;
   int seg_units;           // see tree_units
+  int raw_stages;          // of the tile kernel for codes
   int RT;                  // columns (node, query head) of a pair
   int part_floats;         // of one segment in the workspace: o [D / 4][RT][4], then (m, l) [RT]
   float* node_o;           // [N * Hq][D], of the nodes alone
@@ -106,19 +107,51 @@ constexpr int kTreeTileThreads = 352;
 constexpr int kTreeTileTokens = 64;
 constexpr int kTreeTileUnits = 8;  // beginning and ending a segment, in tiles
 constexpr int kTreeTileStages = 24, kTreeTileLeast = 4;
-constexpr int kTreeTileBarBytes = 640;
-constexpr int kTreeTileSmem = 232448 - 2048;  // beside 2 KB of static shared memory
+constexpr int kTreeTileBarBytes = 768;
+// For codes four more warps make tiles of fp16 values of them.
+constexpr int kTreeCodeThreads = 512;
+constexpr int kTreeRawStages = 8;
+constexpr int kTreePows = 32;  // tiles whose powers are kept: more than stages hold
+static_assert(kTreePows > kTreeTileStages / 2 + 1, "a tile's powers are read while later ones are written");
+__host__ __device__ constexpr int tree_tile_queries(int D, int bits, bool shared) { return bits && !shared && D == 128 ? 1 : 2; }
+// Codes of K and V of a tile and their scales and biases.
+__host__ __device__ constexpr int tree_raw_stage(int D, int bits) {
+  return bits ? 2 * kTreeTileTokens * D * bits / 8 + 4 * kTreeTileTokens * (D / 64) * 2 : 0;
+}
+constexpr int kTreeTileSmem = 232448 - 4096;  // beside 4 KB of static shared memory
 // For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
-const void* tree_tile_kernel_for(int dtype, int D, bool shared);
-constexpr PagedLayout tree_tile_layout(int batch, int D, bool shared) {
-  const int stage = kTreeTileTokens * D * 2, q = 2 * 128 * D * 2, pre = (2 * (batch + 1) + 2 * (kTreeTileThreads / 32)) * 4, pre128 = (pre + 127) / 128 * 128;
-  const int room = (kTreeTileSmem - 1024 - q - pre128 - kTreeTileBarBytes) / stage;
-  PagedLayout l{};
-  l.stages = room < kTreeTileStages ? room : kTreeTileStages;
+const void* tree_tile_e1_b0(int D, bool shared);
+const void* tree_tile_e2_b0(int D, bool shared);
+const void* tree_tile_e1_b4(int D, bool shared);
+const void* tree_tile_e2_b4(int D, bool shared);
+const void* tree_tile_e1_b8(int D, bool shared);
+const void* tree_tile_e2_b8(int D, bool shared);
+
+struct TileLayout {
+  int stages, raw_stages;
+  int raw_off, prefix_off, bar_off, bytes;
+};
+constexpr TileLayout tree_tile_layout(int batch, int D, int bits, bool shared) {
+  const int stage = kTreeTileTokens * D * 2, q = tree_tile_queries(D, bits, shared) * 128 * D * 2, raw = tree_raw_stage(D, bits);
+  const int pre = (2 * (batch + 1) + 2 * (kTreeCodeThreads / 32)) * 4, pre128 = (pre + 127) / 128 * 128;
+  int room = kTreeTileSmem - 1024 - q - pre128 - kTreeTileBarBytes;
+  TileLayout l{};
   // Where the groups take tiles in turn, a stage stays with the K, or the V, of one of them: a wait for a stage names
   // its phase by the parity, so whoever waits has to know that the phase before is done.
-  if (!shared) l.stages = l.stages / 4 * 4;
-  l.prefix_off = q + l.stages * stage;
+  // (Of codes, with one of the two pairs of warps that make the tiles, too.)
+  const int by = shared && !bits ? 1 : 4;
+  if (bits) {  // four tiles of values, or two, and the rest for codes, but two stages at least
+    const int fit = (room - 2 * raw) / stage;
+    l.stages = (fit < 8 ? fit : 8) / by * by;
+    l.raw_stages = (room - l.stages * stage) / raw / 2 * 2;
+    if (l.raw_stages > kTreeRawStages) l.raw_stages = kTreeRawStages;
+  } else {
+    l.stages = room / stage;
+    if (l.stages > kTreeTileStages) l.stages = kTreeTileStages;
+    l.stages = l.stages / by * by;
+  }
+  l.raw_off = q + l.stages * stage;
+  l.prefix_off = (l.raw_off + l.raw_stages * raw + 127) / 128 * 128;
   l.bar_off = l.prefix_off + pre128;
   l.bytes = l.bar_off + kTreeTileBarBytes + 1024;
   return l;

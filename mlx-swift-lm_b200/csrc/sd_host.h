@@ -16,8 +16,8 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
 EncodeTiledFn encode_fn();
 
 // Tensor map of `rows` rows of row_bytes at `base`, copied box_rows rows at a
-// time: whole rows, or 128 bytes of each.
-int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole = true);
+// time: whole rows, or 128 bytes of each; swizzled by the box's width, or as it is.
+int32_t encode_map(CUtensorMap* map, void* base, int row_bytes, int64_t rows, int box_rows, bool whole = true, bool swizzle = true);
 
 }  // namespace sd
 

@@ -31,6 +31,13 @@ TreeSet lookup_tree(int dtype, int bits, int D, int columns) {
   }
 }
 
+const void* (*lookup_tile(int dtype, int bits))(int, bool) {
+  const bool half = dtype == SD_F16;
+  return bits == 0 ? half ? tree_tile_e1_b0 : tree_tile_e2_b0
+         : bits == 4 ? half ? tree_tile_e1_b4 : tree_tile_e2_b4
+                     : half ? tree_tile_e1_b8 : tree_tile_e2_b8;
+}
+
 bool good_page(int P) { return P == 16 || P == 32 || P == 64 || P == 128 || P == 256; }
 
 bool any_misaligned4(std::initializer_list<const void*> list) {
@@ -44,7 +51,8 @@ struct TreeShape {
   const void* attend;
   const void* merge;
   int threads, smem_most;  // of attend
-  PagedLayout lay;
+  TileLayout lay;
+  int q_off, buf_off;
   int tile, columns;  // tokens of a tile, columns of a pair
   bool tiles;         // the tile kernel
   int ctas, seg_units;
@@ -61,13 +69,14 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   const TreeSet set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
   if (!set.attend) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   s->merge = set.merge;
-  s->tiles = g->kv_bits == 0 && g->dtype != SD_F32 && columns > kTreeColumns;
+  s->tiles = g->dtype != SD_F32 && columns > kTreeColumns;
   if (s->tiles) {
     const bool shared = columns > 128;
-    s->attend = tree_tile_kernel_for(g->dtype, D, shared);
-    s->threads = kTreeTileThreads;
+    s->attend = lookup_tile(g->dtype, g->kv_bits)(D, shared);
+    s->threads = g->kv_bits ? kTreeCodeThreads : kTreeTileThreads;
     s->smem_most = kTreeTileSmem;
-    s->lay = tree_tile_layout(batch, D, shared);
+    s->lay = tree_tile_layout(batch, D, g->kv_bits, shared);
+    s->q_off = s->lay.raw_off;
     s->tile = kTreeTileTokens;
     s->columns = shared ? 256 : 128;
     s->ctas = sms;
@@ -76,13 +85,16 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->attend = set.attend;
     s->threads = kTreeAttendThreads;
     s->smem_most = kPagedSmem;
-    s->lay = tree_layout(batch, set.columns, D, g->dtype == SD_F32 && !g->kv_bits, set.stage_bytes);
+    const PagedLayout lay = tree_layout(batch, set.columns, D, g->dtype == SD_F32 && !g->kv_bits, set.stage_bytes);
+    s->lay = TileLayout{lay.stages, 0, 0, lay.prefix_off, lay.bar_off, lay.bytes};
+    s->q_off = lay.q_off;
+    s->buf_off = lay.buf_off;
     s->tile = set.tile;
     s->columns = set.columns;
     s->ctas = 2 * sms;
     s->seg_units = kSegmentUnits;
   }
-  if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
+  if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1) || (s->tiles && g->kv_bits && s->lay.raw_stages < 2)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
   // a sequence's last pair may be almost empty; no more pairs than columns
   s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / s->columns + batch);
   s->part_floats = paged_part_floats(s->columns, D);
@@ -223,8 +235,8 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.k_data = static_cast<uint8_t*>(at(g->k_data, rows * rb));
   p.v_data = static_cast<uint8_t*>(at(g->v_data, rows * rb));
   CUtensorMap tmK, tmV;
-  if (int32_t rc = encode_map(&tmK, const_cast<uint8_t*>(p.k_data), rb, layer_rows(g), box, !s.tiles)) return rc;
-  if (int32_t rc = encode_map(&tmV, const_cast<uint8_t*>(p.v_data), rb, layer_rows(g), box, !s.tiles)) return rc;
+  if (int32_t rc = encode_map(&tmK, const_cast<uint8_t*>(p.k_data), rb, layer_rows(g), box, !s.tiles, !s.tiles || !g->kv_bits)) return rc;
+  if (int32_t rc = encode_map(&tmV, const_cast<uint8_t*>(p.v_data), rb, layer_rows(g), box, !s.tiles, !s.tiles || !g->kv_bits)) return rc;
   p.q = q;
   p.out = out;
   p.line = static_cast<int*>(workspace);
@@ -263,8 +275,9 @@ int32_t sd_paged_tree_decode(const sd_pages* g, int32_t layer, const void* q, in
   p.magic = 0x64006400u;
   p.flags = device_flags;
   p.stages = s.lay.stages;
-  p.q_off = s.lay.q_off;
-  p.buf_off = s.lay.buf_off;
+  p.raw_stages = s.lay.raw_stages;
+  p.q_off = s.q_off;
+  p.buf_off = s.buf_off;
   p.prefix_off = s.lay.prefix_off;
   p.bar_off = s.lay.bar_off;
   p.ncta = s.ctas;

@@ -1,5 +1,6 @@
 // sd_tree_tile.cu -- attention of many (node, query head) columns per sequence
-// of 16-bit pools, on the fifth-generation tensor cores. See sd_tree.cuh for what
+// on the fifth-generation tensor cores, for 16-bit pools and for codes with
+// 16-bit scales; compiled once per (SD_E, SD_BITS) pair. See sd_tree.cuh for what
 // it is a part of.
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
@@ -24,7 +25,26 @@
 // the range may hold anything and are zeroed in shared memory, and so are
 // infinities and not-a-numbers in a node's row, which a row that does see the
 // node gets back at the end.
+// Codes: the loading warp brings them as they are, with their scales, and four
+// more warps make tiles of fp16 values of them, s c + b by one packed fma each.
+// fp16 has 11 bits, three more than bf16, but a narrow range, so a tile of K, or
+// of V, is scaled by a power of two of its own -- exactly, as the scales have no
+// more than 11 bits: the largest of K goes to [2^13, 2^14), of V to [2^6, 2^14) in
+// steps of 2^8, and the scores, or weights and O, take the power back. Queries of
+// bf16 are scaled row by row in the same way.
 #include "sd_tree.cuh"
+
+#if !defined(SD_E) || !defined(SD_BITS)
+#error "SD_E and SD_BITS must be defined"
+#endif
+
+#if SD_E == 1
+using ET = __half;
+#else
+using ET = __nv_bfloat16;
+#endif
+
+#include <type_traits>
 
 namespace sd {
 
@@ -33,6 +53,7 @@ namespace {
 constexpr int kTileT = kTreeTileTokens;
 static_assert(kTileT == 64, "a row's bits of a tile are a mask's");
 constexpr int kTmemCols = 512;
+constexpr int kNoPower = -1000;  // of a tile of zeros, which takes any
 // Tensor memory columns of the first group's S, its P's two buffers, and its O; the second's are 128 on.
 constexpr int kSCol = 0, kPCol = 64, kOCol = 256;
 
@@ -98,19 +119,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
 }
 
 // --- waits: bounded; the answer is the warp's, as the tensor memory accesses are ---
-// A wait that has to go on is out of line: every instruction in the loops here is fetched again for each tile.
+// A wait that has to go on is out of line: every instruction in the loops here is fetched again for each tile. (Not in
+// the kernel for codes: a call keeps the registers from being shared out anew.)
 static __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* flags) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
 }
+template <bool CALL>
 struct Waiter {
   int* flags;
   bool dead;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) {
-    if (!dead && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) dead = !wait_on(bar, parity, flags);
+    if constexpr (CALL) {
+      if (!dead && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) dead = !wait_on(bar, parity, flags);
+    } else {
+      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
+    }
     return !dead;
   }
 };
-
 // One arrival for a warp, after what its lanes did: a barrier takes some three cycles for each, and 128 of them made
 // every signal between the warps 430 cycles late.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -153,9 +179,28 @@ __device__ __forceinline__ bool finite2(uint32_t& w) {
   return a || b;
 }
 
+// Four codes of a word as fp16 pairs.
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t magic, uint32_t (&v)[2]) {
+  v[0] = sub_f16x2(raw_u8(w, 0x5150u, magic), 0x64006400u);
+  v[1] = sub_f16x2(raw_u8(w, 0x5352u, magic), 0x64006400u);
+}
+// Codes 2 i and 2 i + 1 of a word of nibbles as an fp16 pair, the second one 16 times as large.
+__device__ __forceinline__ uint32_t codes4(uint32_t w, int i, uint32_t magic) {
+  return sub_f16x2((__byte_perm(w, 0u, 0x4040u + 0x0101u * i) & 0x00F0000Fu) | magic, 0x64006400u);
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23 & 255) - 127; }  // of a normal x > 0
+
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
   uint64_t q_full[2], s_full[2], s_free[2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer of P
+  uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages];
   uint64_t started, done;
   uint32_t tmem;
 };
@@ -163,35 +208,48 @@ static_assert(sizeof(TileBars) <= kTreeTileBarBytes, "room in the layout");
 
 }  // namespace
 
-template <typename E, int D, bool SHARED>
-__global__ void __launch_bounds__(kTreeTileThreads, 1)
+template <typename E, int BITS, int D, bool SHARED>
+__global__ void __launch_bounds__(BITS ? kTreeCodeThreads : kTreeTileThreads, 1)
 tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV) {
   constexpr int NH = D / 64, kQHalf = 128 * 128, kHalf = kTileT * 128;  // bytes of 64 dimensions of Q, of a tile
   constexpr int kQ = NH * kQHalf, kStage = NH * kHalf;
-  constexpr float kUp = __is_same(E, __half) ? 7.0f : 0.0f;  // as in a decode: fp16 weights up to 2^(kUp + kSlack)
+  constexpr int kThreads = BITS ? kTreeCodeThreads : kTreeTileThreads;
+  using T = std::conditional_t<BITS != 0, __half, E>;        // of the products' operands
+  constexpr float kUp = __is_same(T, __half) ? 7.0f : 0.0f;  // as in a decode: fp16 weights up to 2^(kUp + kSlack)
+  constexpr int kQs = tree_tile_queries(D, BITS, SHARED);    // copies of Q: one for both groups makes room for the ring
+  constexpr int kRow = BITS ? D * BITS / 8 : 1, kSb = BITS ? kTileT * (D / 64) * 2 : 0;  // bytes: a row of codes, a tile's scales
+  constexpr int kRaw = tree_raw_stage(D, BITS);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *qs = sm, *ring = sm + 2 * kQ;
+  uint8_t *qs = sm, *ring = sm + kQs * kQ, *raws = sm + p.q_off;
   TileBars* bars = reinterpret_cast<TileBars*>(sm + p.bar_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
   __shared__ float2 ml_of[2][SHARED ? 1 : 128];
+  // codes: powers of the last tiles' K and V, and whether a node's V is not finite; of the rows of Q; the warps' maxima
+  __shared__ int4 tile_pow[BITS ? kTreePows : 1];
+  __shared__ int q_pow[2][BITS ? 128 : 1];
+  __shared__ uint32_t most_of[2][2][2][4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(bars->full + i, 1);
+      mbar_init(bars->full + i, BITS ? 2 : 1);
       mbar_init(bars->empty + i, SHARED ? 2 : 1);  // groups that use the tile
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(bars->q_full + w, 4);
+      mbar_init(bars->q_full + w, kQs == 1 && w == 1 ? 8 : 4);
       mbar_init(bars->s_full + w, 1);
       mbar_init(bars->s_free + w, 4);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->o_full[w][i], 1);
         mbar_init(&bars->p_full[w][i], 4);
       }
+    }
+    for (int i = 0; i < kTreeRawStages; ++i) {
+      mbar_init(bars->raw_full + i, 33);
+      mbar_init(bars->raw_empty + i, 2);
     }
     mbar_init(&bars->started, 4);
     mbar_init(&bars->done, 2);
@@ -206,7 +264,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   griddep_wait();
   griddep_launch_dependents();
   tc_fence_before();
-  tree_line<kTreeTileThreads>(p, kTileT, units, pairs, tmp);  // with barriers
+  tree_line<kThreads>(p, kTileT, units, pairs, tmp);  // with barriers
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const Pieces pieces(p, units[p.B]);
@@ -214,8 +272,11 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   TreeWalk walk(p, units, pairs, work ? pieces.begin(blockIdx.x) : 0, work ? pieces.begin(blockIdx.x + 1) : 0);
   TreeSegment s;
   int it0 = 0;  // tiles of the segments before
-  Waiter wait{p.flags, false};
+  Waiter<BITS == 0> wait{p.flags, false};
 
+  // The registers of a launch for codes (16 warps x 128) shared out anew: 8 x 168 for the weights, 8 x 88.
+  if (warp >= 8) {
+    if constexpr (BITS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 8) {  // ---- loads ----
     const uint64_t pol = stream_policy(false);
     const int pb = min(p.P, kTileT), nb = kTileT / pb;  // rows per box, boxes per tile
@@ -247,6 +308,35 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           else if (p.flags) atomicOr(p.flags, kErrBadIndex);
         }
         const int n_box = __popc(__ballot_sync(0xffffffffu, need));
+        if constexpr (BITS) {  // K and V and their scales, as they are, in one stage
+          if (use >= p.raw_stages && !wait(bars->raw_empty + st, round ^ 1u)) break;
+          uint64_t* full = bars->raw_full + st;
+          uint8_t* stage = raws + st * kRaw;
+          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n_box * 2 * pb * kRow));
+          __syncwarp();
+          if (need) {
+            tma_load_3d(stage + lane * pb * kRow, &tmK, 0, y, 0, full, pol);
+            tma_load_3d(stage + (kTileT + lane * pb) * kRow, &tmV, 0, y, 0, full, pol);
+          }
+          constexpr int ROW = D / 64 * 2, CPA = kSb / 16;  // bytes of a token in each array of scales, 16-byte pieces of a tile
+          const uint8_t* src[4] = {static_cast<const uint8_t*>(p.k_scales), static_cast<const uint8_t*>(p.k_biases),
+                                   static_cast<const uint8_t*>(p.v_scales), static_cast<const uint8_t*>(p.v_biases)};
+          const uint32_t sb = smem_u32(stage + 2 * kTileT * kRow);
+          const int byte = lane * 16, j = min(byte / ROW / pb, nb - 1);  // the box this piece's tokens lie in
+          const int64_t kr = __shfl_sync(0xffffffffu, y, j);
+          const bool good = __shfl_sync(0xffffffffu, int(need && y != oob_row), j);
+          if (lane < CPA) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              cp_async16_zfill(sb + x * kSb + byte, good ? src[x] + (kr * ROW + byte - j * pb * ROW) : src[x], good ? 16 : 0);
+          }
+          cp_async_arrive(full);
+          ++use;
+          if (++st == p.raw_stages) {
+            st = 0;
+            round ^= 1u;
+          }
+        } else {
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (use >= p.stages && !wait(bars->empty + st, round ^ 1u)) break;
@@ -265,13 +355,17 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           }
         }
       }
+      }
     }
-    if (wait.dead)  // what is under way lands in this CTA's shared memory
-      for (int u = max(0, use - p.stages); u < use; ++u) mbar_wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u, nullptr);
+    if (wait.dead) {  // what is under way lands in this CTA's shared memory
+      uint64_t* full = BITS ? bars->raw_full : bars->full;
+      const int n = BITS ? p.raw_stages : p.stages;
+      for (int u = max(0, use - n); u < use; ++u) mbar_wait(full + u % n, uint32_t(u / n) & 1u, nullptr);
+    }
   } else if (warp == 9 || warp == 10) {  // ---- products of a group ----
     const int w = warp - 9;
     uint32_t seg = 0, k = 0;  // segments that the group took part in and tiles: the parities of its barriers
-    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + w * kQ) >> 4);
+    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + (kQs == 2 ? w * kQ : 0)) >> 4);
     const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
     const uint32_t ds = tmem + kSCol + w * 128, dp = tmem + kPCol + w * 128, dO = tmem + kOCol + w * 128;
     const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full + w);
@@ -296,7 +390,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           const uint64_t kd = kd0 + ks * (kStage >> 4);
 #pragma unroll
           for (int c = 0; c < D / 16; ++c)
-            mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<E>(kTileT, false), c > 0);
+            mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<T>(kTileT, false), c > 0);
           mma_commit(s_full);
           mma_commit(empty + ks * 8);
           ks += SHARED ? 2 : 4;
@@ -309,7 +403,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           const uint64_t v = vd0 + vs * (kStage >> 4);
           const uint32_t pp = dp + h * (kTileT / 2);
 #pragma unroll
-          for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
+          for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
           mma_commit(o_full + h * 8);
           mma_commit(empty + vs * 8);
           vs += SHARED ? 2 : 4;
@@ -321,12 +415,99 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
     mbar_wait(&bars->done, 0, p.flags);
+  } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
+    if constexpr (BITS) {
+      constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 64;  // groups, codes of 16 bytes, such pieces
+      constexpr float kTop = float((1 << BITS) - 1);
+      // Two warps for every other tile: what a tile waits for (codes, maxima, a free stage) is hidden by the other pair's.
+      // The numbers of stages are such that a stage stays with a pair.
+      const int pair = (warp - 12) >> 1, ct = (tid - 12 * 32) & 63, cw = (warp - 12) & 1;
+      while (walk.next(s)) {
+        const TreeSeq sq = tree_seq(p, s.b);
+        const int t0 = sq.begin / kTileT;
+        for (int i = s.i0; i < s.i1; ++i) {
+          const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
+          if ((t & 1) != pair) continue;
+          const int rs = t % p.raw_stages;
+          wait(bars->raw_full + rs, uint32_t(t / p.raw_stages) & 1u);
+          const uint8_t* raw = raws + rs * kRaw;
+          const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
+          // the largest value of K and of V, and whether a node's V is not finite
+          uint32_t most[2] = {0, 0};
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 2 * NG; ++e) {
+            const int x = ct + 64 * e, v = x / (kTileT * NG), at = x % (kTileT * NG), row = at / NG;
+            const float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]), bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]);
+            const float a = fmaxf(fabsf(bi), fabsf(fmaf(sc, kTop, bi)));
+            const bool in = row >= lo && row < hi, fine = a < INFINITY && fabsf(sc) < INFINITY;  // not-a-numbers are not
+            if (in && fine) most[v] = max(most[v], __float_as_uint(a));
+            odd |= v == 1 && in && row >= old && !fine;
+          }
+          most[0] = __reduce_max_sync(0xffffffffu, most[0]);
+          most[1] = __reduce_max_sync(0xffffffffu, most[1]);
+          odd = __any_sync(0xffffffffu, odd);
+          uint32_t(&mo)[2][4] = most_of[pair][t >> 1 & 1];
+          if (lane == 0) mo[cw][0] = most[0], mo[cw][1] = most[1], mo[cw][2] = odd;
+          named_barrier(4 + pair, 64);
+          const uint32_t mk = max(mo[0][0], mo[1][0]), mv = max(mo[0][1], mo[1][1]), any = mo[0][2] | mo[1][2];
+          const int ek = mk ? max(exponent(__uint_as_float(mk)) - 13, -120) : 0;
+          const int ev = mv ? max((exponent(__uint_as_float(mv)) - 6) & ~7, -120) : kNoPower;
+          if (ct == 0) tile_pow[t % kTreePows] = make_int4(ek, ev, int(any), 0);
+          const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
+#pragma unroll 1
+          for (int v = 0; v < 2; ++v) {
+            const int u = 2 * t + v, st = u % p.stages;
+            if (u >= p.stages) wait(bars->empty + st, (uint32_t(u / p.stages) & 1u) ^ 1u);
+            if (!wait.dead) {
+              const uint32_t dst = smem_u32(ring) + st * kStage;
+              const float f = v ? fv : fk;
+#pragma unroll 2
+              for (int e = 0; e < N; ++e) {
+                const int x = ct + 64 * e, row = x / CPR, c = x % CPR, el = c * EPC;  // row, piece, its first element
+                const uint4 w = *reinterpret_cast<const uint4*>(raw + (v * kTileT + row) * kRow + c * 16);
+                const int at = row * NG + el / 64;
+                float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]) * f, bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]) * f;
+                // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
+                const bool none = v && (row < lo || row >= hi || (row >= old && !(fabsf(sc) + fabsf(bi) < INFINITY)));
+                if (none) sc = bi = 0.0f;
+                const uint32_t b2 = pack2<__half>(bi, bi), s2 = pack2<__half>(sc, BITS == 8 ? sc : sc * 0.0625f);
+                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
+                  uint32_t h[4];
+                  if constexpr (BITS == 8) {
+                    uint32_t a[2], b[2];
+                    codes8(words[2 * j], p.magic, a);
+                    codes8(words[2 * j + 1], p.magic, b);
+                    h[0] = fma_f16x2(a[0], s2, b2), h[1] = fma_f16x2(a[1], s2, b2);
+                    h[2] = fma_f16x2(b[0], s2, b2), h[3] = fma_f16x2(b[1], s2, b2);
+                  } else {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) h[y] = fma_f16x2(codes4(words[j], y, p.magic), s2, b2);
+                  }
+                  const int ch = (el + 8 * j) / 8;
+                  const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                }
+              }
+              fence_proxy_async_shared();
+              warp_arrive(bars->full + st);
+              if (v) warp_arrive(bars->raw_empty + rs);
+            }
+          }
+        }
+        it0 += s.i1 - s.i0;
+      }
+    }
+  }
   } else {  // ---- weights: a row per thread ----
+    if constexpr (BITS) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
     const uint32_t ts = tmem + lanes + kSCol + w * 128, tp = tmem + lanes + kPCol + w * 128, to = tmem + lanes + kOCol + w * 128;
     const bool neg = p.scale_log2 < 0.0f;
-    const float sc = fmaxf(fabsf(p.scale_log2), 1.1754944e-38f);  // -inf times it stays -inf
+    const float scale = fmaxf(fabsf(p.scale_log2), 1.1754944e-38f);  // -inf times it stays -inf
     uint32_t k = 0;  // tiles of this group
     while (walk.next(s)) {
       const TreeSeq sq = tree_seq(p, s.b);
@@ -335,24 +516,52 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       const int t0 = sq.begin / kTileT;
       if (SHARED || s.i0 + w < s.i1) {  // Q: a thread has one 16-byte chunk of every eighth (or sixteenth) row
         constexpr int CPR = D / 8, RPT = 128 / CPR, N = 128 / RPT;
-        const uint32_t q = smem_u32(qs) + w * kQ;
+        const uint32_t q = smem_u32(qs) + (kQs == 2 ? w * kQ : 0);
         const int ch = r % CPR;
         uint4 v[N];
+        if (kQs == 2 || w == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int xx = (SHARED ? w * 128 : 0) + r / CPR + RPT * i;
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (xx < cols.n) v[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const E*>(p.q) + cols.row(xx) * D) + ch);
-        }
+          for (int i = 0; i < N; ++i) {
+            const int xx = (SHARED ? w * 128 : 0) + r / CPR + RPT * i;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (xx < cols.n) v[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const E*>(p.q) + cols.row(xx) * D) + ch);
+          }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int row = r / CPR + RPT * i;
-          const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
+          for (int i = 0; i < N; ++i) {
+            const int row = r / CPR + RPT * i;
+            if constexpr (BITS != 0) {
+              if constexpr (!__is_same(E, __half)) {  // bf16: the row's largest to [2^13, 2^14), all of its 8 bits in fp16
+                uint32_t w4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                float f[8], top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  unpack_word<E>(w4[j], f + 2 * j);
+                  top = fmaxf(top, fmaxf(fabsf(f[2 * j]), fabsf(f[2 * j + 1])));
+                }
+#pragma unroll
+                for (int j = 1; j < CPR; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
+                const int e = top > 0.0f && top < INFINITY ? min(max(exponent(top) - 13, -120), 120) : 0;
+                const float down = power(-e);
+                v[i].x = pack2<__half>(f[0] * down, f[1] * down), v[i].y = pack2<__half>(f[2] * down, f[3] * down);
+                v[i].z = pack2<__half>(f[4] * down, f[5] * down), v[i].w = pack2<__half>(f[6] * down, f[7] * down);
+                if (ch == 0) q_pow[SHARED ? w : 0][row] = e;
+              }
+            }
+            const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
+          }
         }
         fence_proxy_async_shared();
         tc_fence_before();
         warp_arrive(bars->q_full + w);
+        if (kQs == 1 && w == 0 && s.i1 - s.i0 > 1) warp_arrive(bars->q_full + 1);  // these rows are the second group's, too
+      }
+      float sq_pow = 1.0f;
+      if constexpr (BITS != 0 && !__is_same(E, __half)) {
+        // each group loads its rows, or, of one copy and for a group without tiles, the first one
+        if (SHARED) named_barrier(2 + w, 128);
+        else named_barrier(1, 256);
+        sq_pow = power(q_pow[SHARED ? w : 0][r]);
       }
       const int low = x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
       const uint64_t seen = x < cols.n ? tree_seen(p, sq, cols.node(x)) : 0;
@@ -360,6 +569,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       float m = -INFINITY, l = 0.0f;
       int steps = 0;
       bool odd = false;  // a node has a value that is not finite
+      int ref = kNoPower;  // codes: O's power
       const int n = SHARED ? s.i1 - s.i0 : (s.i1 - s.i0 + 1 - w) / 2;
 #pragma unroll 1
       for (; steps < n; ++steps, ++k) {
@@ -370,9 +580,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const bool ends = lo > 0 || old < kTileT;
         // Every group that uses the tile waits for its rows, dead or not; the second one before its own scores, which may
         // wait for the first.
-        if (SHARED && ends && w == 1) odd |= barrier_or(1, 256, false);
+        if (!BITS && SHARED && ends && w == 1) odd |= barrier_or(1, 256, false);
         const bool here = wait(bars->s_full + w, k & 1u);
-        if (ends && (!SHARED || w == 0)) {
+        if (!BITS && ends && (!SHARED || w == 0)) {
           bool mine = false;
           const int u = 2 * (it0 + tile) + 1;
           if (here && wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
@@ -395,6 +605,17 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
         if (!here) continue;
         tc_fence_after();
+        float sc = scale;
+        int ev = 0;
+        if constexpr (BITS) {
+          // What the warps that made the tile wrote of it, before its V, whose stage stays until this group's P is used.
+          const int t = it0 + tile, u = 2 * t + 1;
+          wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u);
+          const int4 pw = tile_pow[t % kTreePows];
+          sc = fminf(fmaxf(scale * sq_pow * power(pw.x), 1.1754944e-38f), 3.4e38f);
+          ev = pw.y;
+          odd |= pw.z != 0;
+        }
         uint32_t va[32], vb[32];
         tmem_ld32(ts, va);
         tmem_ld32(ts + 32, vb);
@@ -426,11 +647,17 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           mx[3] = fmaxf(fmaxf(mx[3], __uint_as_float(vb[j + 2])), __uint_as_float(vb[j + 3]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+        const bool up = BITS && ev > ref;  // O's power moves
         if (steps == 0) {
           m = top - kUp;
-        } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
-          const float fac = raise_max(m, top - kUp);
+          ref = ev;
+        } else if (__any_sync(0xffffffffu, up || top > m + (kSlack + kUp))) {
+          float fac = raise_max(m, top - kUp);
           l *= fac;
+          if (up) {
+            if (ref != kNoPower) fac *= power(max(ref - ev, -126));
+            ref = ev;
+          }
           if (wait(&bars->o_full[w][h ^ 1], ((k - 1) >> 1) & 1u)) {  // the last product
             tc_fence_after();
 #pragma unroll 1
@@ -445,6 +672,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           }
         }
         const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m, -m), sc2 = make_float2(sc, sc);
+        const float dv = BITS && ev != ref ? power(max(ev - ref, -126)) : 1.0f;  // the tile's power of V over O's
         float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         uint32_t two[32];
         auto weigh = [&](const uint32_t (&v)[32], int c) {
@@ -452,8 +680,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           for (int j = 0; j < 16; ++j) {
             float2 e = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc2, mm);
             e.x = ex2(e.x), e.y = ex2(e.y);
-            two[16 * c + j] = pack2<E>(e.x, e.y);
             sum[j & 1] = add2(sum[j & 1], e);
+            if constexpr (BITS) e.x *= dv, e.y *= dv;
+            two[16 * c + j] = pack2<T>(e.x, e.y);
           }
         };
         weigh(va, 0);
@@ -479,13 +708,25 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           const int t = sq.held + __ffsll(left) - 1, page = __ldcg(p.tables + int64_t(s.b) * p.W + t / p.P);
           if (page < 0 || page >= p.n_pages) continue;
           const int64_t row = (int64_t(page) * p.Hkv + s.h) * p.P + (t & (p.P - 1));
-          const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data) + row * (D / 2) + 16 * c;
+          if constexpr (BITS == 0) {
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data) + row * (D / 2) + 16 * c;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float f[2];
-            unpack_word<E>(__ldcg(v + j), f);
-            if (!(fabsf(f[0]) < INFINITY)) o[2 * j] = __float_as_uint(__uint_as_float(o[2 * j]) + f[0]);
-            if (!(fabsf(f[1]) < INFINITY)) o[2 * j + 1] = __float_as_uint(__uint_as_float(o[2 * j + 1]) + f[1]);
+            for (int j = 0; j < 16; ++j) {
+              float f[2];
+              unpack_word<E>(__ldcg(v + j), f);
+              if (!(fabsf(f[0]) < INFINITY)) o[2 * j] = __float_as_uint(__uint_as_float(o[2 * j]) + f[0]);
+              if (!(fabsf(f[1]) < INFINITY)) o[2 * j + 1] = __float_as_uint(__uint_as_float(o[2 * j + 1]) + f[1]);
+            }
+          } else {
+            const int64_t g = row * (D / 64) + c / 2;
+            const float sc = Elt<E>::to_f32(static_cast<const E*>(p.v_scales)[g]), bi = Elt<E>::to_f32(static_cast<const E*>(p.v_biases)[g]);
+            if (fabsf(sc) + fabsf(bi) < INFINITY) continue;
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data + row * kRow) + c * BITS;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t code = __ldcg(v + j * BITS / 32) >> (j * BITS % 32) & ((1u << BITS) - 1);
+              o[j] = __float_as_uint(__uint_as_float(o[j]) + fmaf(float(code), sc, bi));
+            }
           }
         }
       };
@@ -496,6 +737,11 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0;
+        }
+        if constexpr (BITS) {
+          const float back = ref == kNoPower ? 1.0f : power(ref);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
         }
         if (odd) add_odd(c, o);
       };
@@ -511,31 +757,28 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           }
         }
       } else {
-        // each group finishes half of the dimensions and hands the other half over, in the place of Q: no score of this
-        // segment is still to come
-        uint4* swap = reinterpret_cast<uint4*>(qs + w * kQ);  // [D / 8][128]
-        const uint4* from = reinterpret_cast<const uint4*>(qs + (1 - w) * kQ);
-        named_barrier(1, 256);
+        // each group finishes half of the dimensions and hands the other half over, 32 at a time, in the place of Q: no
+        // score of this segment is still to come
+        uint4* swap = reinterpret_cast<uint4*>(qs) + w * 8 * 128;  // [8][128]
+        const uint4* from = reinterpret_cast<const uint4*>(qs) + (1 - w) * 8 * 128;
         ml_of[w][r] = make_float2(m, l);
+        float most = 0.0f, f0 = 0.0f, f1 = 0.0f;
+        float2 ml;
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
           uint32_t o[32];
+          named_barrier(1, 256);  // Q, or what was handed over before, has been read
           load((1 - w) * (D / 64) + c, o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            swap[(8 * c + j) * 128 + r] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        }
-        named_barrier(1, 256);
-        const float2 ml = ml_of[1 - w][r];
-        const float most = fmaxf(m, ml.x), f0 = exp2_from(m, most), f1 = exp2_from(ml.x, most);
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t o[32];
+          for (int j = 0; j < 8; ++j) swap[j * 128 + r] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          named_barrier(1, 256);
+          ml = ml_of[1 - w][r];
+          most = fmaxf(m, ml.x), f0 = exp2_from(m, most), f1 = exp2_from(ml.x, most);
           load(w * (D / 64) + c, o);
           if (x < cols.n) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const uint4 z = from[(8 * c + j) * 128 + r];
+              const uint4 z = from[j * 128 + r];
               auto join = [&](uint32_t a, uint32_t b) { return fmaf(f1, __uint_as_float(b), f0 * __uint_as_float(a)); };
               reinterpret_cast<float4*>(part)[(w * (D / 8) + 8 * c + j) * 128 + x] =
                   make_float4(join(o[4 * j], z.x), join(o[4 * j + 1], z.y), join(o[4 * j + 2], z.z), join(o[4 * j + 3], z.w));
@@ -557,15 +800,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   }
 }
 
-const void* tree_tile_kernel_for(int dtype, int D, bool shared) {
-#define SD_TILE(E, DD) \
-  return shared ? reinterpret_cast<const void*>(&tree_tile_kernel<E, DD, true>) : reinterpret_cast<const void*>(&tree_tile_kernel<E, DD, false>)
-  if (dtype == 1 && D == 64) SD_TILE(__half, 64);
-  if (dtype == 1 && D == 128) SD_TILE(__half, 128);
-  if (dtype == 2 && D == 64) SD_TILE(__nv_bfloat16, 64);
-  if (dtype == 2 && D == 128) SD_TILE(__nv_bfloat16, 128);
-#undef SD_TILE
-  return nullptr;
+#define SD_NAME2(e, b) tree_tile_e##e##_b##b
+#define SD_NAME(e, b) SD_NAME2(e, b)
+const void* SD_NAME(SD_E, SD_BITS)(int D, bool shared) {
+  if (D == 64) return shared ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 64, true>)
+                             : reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 64, false>);
+  return shared ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 128, true>)
+                : reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 128, false>);
 }
 
 }  // namespace sd

@@ -79,11 +79,12 @@ def build(force: bool = False, verbose: bool = False, phase_timing: bool = False
         units.append((f"sd_inst_e{e}_b{b}.o", "sd_inst.cu", fmt, _kernel_sources("sd_inst.cu", tree | {"sd_paged.cuh", "sd_paged.h"})))
         units.append((f"sd_paged_e{e}_b{b}.o", "sd_paged_inst.cu", fmt, _kernel_sources("sd_paged_inst.cu", tree | {"sd_decode.cuh"})))
         units.append((f"sd_tree_e{e}_b{b}.o", "sd_tree_inst.cu", fmt, _kernel_sources("sd_tree_inst.cu", {"sd_decode.cuh"})))
+        if e:
+            units.append((f"sd_tree_tile_e{e}_b{b}.o", "sd_tree_tile.cu", fmt, _kernel_sources("sd_tree_tile.cu", {"sd_decode.cuh"})))
     units.append(("sd_rotary.o", "sd_rotary.cu", [],
                   _kernel_sources("sd_rotary.cu", tree | {"sd_decode.cuh", "sd_paged.cuh"})))
     units.append(("sd_draft.o", "sd_draft.cu", [],
                   _kernel_sources("sd_draft.cu", {"sd_tree.cuh", "sd_decode.cuh", "sd_paged.cuh"})))
-    units.append(("sd_tree_tile.o", "sd_tree_tile.cu", [], _kernel_sources("sd_tree_tile.cu", {"sd_decode.cuh"})))
     units += [(f"{n}.o", f"{n}.cu", [], _host_sources(f"{n}.cu")) for n in ("sd_api", "sd_pages", "sd_steps")]
     jobs = []
     for obj, src, extra, deps in units:

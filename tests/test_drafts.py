@@ -27,7 +27,7 @@ def test_struct_layout_matches_header():
 
 
 def test_attend_ctas_fit_an_sm(tmp_path):
-    """Two of the attend kernel, one of the tile kernel (with 2 KB of static shared memory), at every batch and format;
+    """Two of the attend kernel, one of the tile kernel (with at most 4 KB of static shared memory), at every batch and format;
     the parts do not overlap."""
     src = tmp_path / "layout.cpp"
     src.write_text("""#include <cuda_runtime.h>
@@ -50,11 +50,16 @@ int main() {
   all<2, 4, 64>(); all<2, 4, 128>(); all<4, 4, 64>(); all<4, 4, 128>();
   all<2, 8, 64>(); all<2, 8, 128>(); all<4, 8, 64>(); all<4, 8, 128>();
   for (int D = 64; D <= 128; D += 64)
-    for (int shared = 0; shared < 2; ++shared)
+    for (int x = 0; x < 6; ++x)
       for (int b = 1; b <= kPagedMaxBatch; ++b) {
-        const PagedLayout l = tree_tile_layout(b, D, shared);
-        if (l.stages < kTreeTileLeast || (!shared && l.stages % 4) || l.prefix_off < (2 * 128 + l.stages * kTreeTileTokens) * D * 2 ||
-            l.prefix_off + 4 * (2 * (b + 1) + 2 * (kTreeTileThreads / 32)) > l.bar_off || l.bytes + 2048 > 227 * 1024) ++bad;
+        const int bits = x / 2 * 4, shared = x % 2;
+        const TileLayout l = tree_tile_layout(b, D, bits, shared);
+        const int raw = l.raw_stages * tree_raw_stage(D, bits);
+        if (l.stages < kTreeTileLeast || l.stages > kTreeTileStages || ((bits || !shared) && l.stages % 4) || l.raw_stages % 2 || l.raw_stages > kTreeRawStages ||
+            (bits && l.raw_stages < 2) || l.raw_off < (tree_tile_queries(D, bits, shared) * 128 + l.stages * kTreeTileTokens) * D * 2 ||
+            l.raw_off % 128 || tree_raw_stage(D, bits) % 128 || l.prefix_off < l.raw_off + raw || l.bar_off % 8 ||
+            l.prefix_off + 4 * (2 * (b + 1) + 2 * ((bits ? kTreeCodeThreads : kTreeTileThreads) / 32)) > l.bar_off ||
+            l.bytes + 4096 > 227 * 1024) ++bad;
       }
   std::printf("%d", bad);
 }

@@ -3,13 +3,17 @@ plans and moved rows bit for bit against a host model, tree attention against
 64 bits.
 
 Tolerance of the attention: the framework's (_util.assert_close) where weights
-keep 16 bits or more. Where many columns share the tile kernel (16-bit pools,
-more than 16 columns a sequence) a weight p is rounded to the pool's type once,
-by at most u = eps / 2 of it, and the sum that it is divided by is made of the
-rounded ones. With A = sum p |v| / sum p, out is then off by at most
-u A + u |out| (numerator and denominator) before its own rounding of u |out|;
-scores in fp32 add less than 1e-4 of A, as do fp16 weights below 2^-14 of
-2^-7 (at most 2^-24 a token each, against a largest of 2^7).
+keep 16 bits or more. The tile kernel (16-bit pools and codes with 16-bit
+scales, more than 16 columns an average sequence) rounds a weight to the
+products' type once, by at most half a step of it: u of 16-bit pools, 2^-11 of
+codes. With A = sum p |v| / sum p that is u A of the output, besides u |out| for
+its own rounding. Codes are fp16 values there: 2^-11 |v| more of V, another
+2^-11 A, and a score is off by d = 2^-11 B at most, B = scale sum |q k| of its
+token: weights become p e^x with |x| <= d, and over their sum, which is between
+e^-d and e^d of what it was, p e^y with |y| <= 2 d, so the output moves by at
+most (e^2d - 1) A. Scores in fp32 add less than 1e-4 of A. fp16 weights below
+2^-14 are off by 2^-25 however small they are, and the largest is 2^7 at least:
+2^-32 sum |v| more, which counts where the heavy tokens' values are zero.
 """
 from __future__ import annotations
 
@@ -286,11 +290,13 @@ def test_keep_refuses_lengths_that_are_inputs(cuda):
 # ---------------------------------------------------------------------------
 
 def tree64(q, pool, tables, held, lines, scale, window=0, sinks=None):
-    """(out, sum p |v| / sum p) in fp64; lines: [[(mask, place)] per node] per sequence, rows in order."""
+    """(out, sum p |v| / sum p, (the largest scale sum |q k|, sum |v|)) in fp64; lines: [[(mask, place)] per node] per sequence, rows in order."""
     import torch
     k, v = pool.values
     hkv, D = k.shape[1], k.shape[-1]
     out, size = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    reach = torch.zeros(q.shape[:2] + (1,), dtype=torch.float64, device="cuda")
+    values = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     row = 0
     for b, (h, nodes) in enumerate(zip(held, lines)):
         n = len(nodes)
@@ -308,6 +314,9 @@ def tree64(q, pool, tables, held, lines, scale, window=0, sinks=None):
                 seen[i] &= place > p - window
         seen = seen.cuda()
         s = torch.einsum("nhgd,htd->hngt", q[row:row + n].double().view(n, hkv, -1, D), kk) * scale
+        most = torch.einsum("nhgd,htd->hngt", q[row:row + n].double().abs().view(n, hkv, -1, D), kk.abs()) * abs(scale)
+        most = torch.where(seen[None, :, None], most, 0.0).amax(-1).transpose(0, 1).reshape(n, -1, 1)
+        reach[row:row + n] = most
         s = torch.where(seen[None, :, None], s, -math.inf)  # also not-a-numbers that are not seen
         if sinks is not None:
             s = torch.cat((s, sinks.double().view(hkv, 1, -1, 1).expand(hkv, n, -1, 1)), -1)
@@ -316,20 +325,25 @@ def tree64(q, pool, tables, held, lines, scale, window=0, sinks=None):
         p = (p / p.sum(-1, keepdim=True).clamp(min=1e-300))[..., :h + n]
         vz = torch.where(seen.any(0)[None, :, None], vv, 0.0)
         out[row:row + n] = torch.einsum("hngt,htd->nhgd", p, vz).reshape(n, -1, D)
+        values[row:row + n] = (vz.abs().sum(1)[None, :, None].expand(n, hkv, q.shape[1] // hkv, D)).reshape(n, -1, D)
         size[row:row + n] = torch.einsum("hngt,htd->nhgd", p, vz.abs()).reshape(n, -1, D)
         row += n
-    return out, size
+    return out, size, (reach, values)
 
 
-def check_tree(torch, out, ref, size, dtype, tile):
+def check_tree(torch, out, ref, size, reach, dtype, tile, bits=0):
     assert torch.isfinite(out).all()
     if tile:
         u = torch.finfo(out.dtype).eps / 2
+        w = 2.0 ** -11 if bits else u
         off = (out.double() - ref).abs()
-        bound = u * (size + 2 * ref.abs()) * 1.01 + 1e-4 * size + (2.0 ** -24 if dtype == "f16" else 0.0)
+        bound = (u * ref.abs() + w * size) * 1.01 + 1e-4 * size + (2.0 ** -24 if dtype == "f16" else 0.0) + 2.0 ** -32 * reach[1]
+        if bits:
+            bound += size * (2.0 ** -11 + torch.expm1(2 * 2.0 ** -11 * reach[0]))
         assert (off <= bound).all(), f"{int((off > bound).sum())} of {off.numel()} off, worst {float((off / bound).max()):.3g}"
         rel = (off.pow(2).sum() / ref.pow(2).sum().clamp(min=1e-300)).sqrt()
-        assert rel <= u, float(rel)  # the worst case everywhere is more than what adds up in squares
+        if not bits:
+            assert rel <= u, float(rel)  # the worst case everywhere is more than what adds up in squares
     else:
         live = ref.abs().sum(-1) > 0
         if live.any():
@@ -339,7 +353,7 @@ def check_tree(torch, out, ref, size, dtype, tile):
 
 
 def uses_tiles(dtype, bits, counts, G):
-    return dtype != "f32" and not bits and -(-sum(counts) // len(counts)) * G > 16
+    return dtype != "f32" and -(-sum(counts) // len(counts)) * G > 16
 
 
 def run_tree(torch, dtype, bits, d, hkv, G, page, held, counts, window=0, sinks=False, seed=0, scale=1.0, chain=False,
@@ -379,8 +393,8 @@ def run_tree(torch, dtype, bits, d, hkv, G, page, held, counts, window=0, sinks=
     assert torch.equal(out, again)
     n = first[-1]
     assert (out[n:] == 7.0).all()
-    ref, size = tree64(q[:n], pool, tables, held, lines, 1 / math.sqrt(d), window, sk)
-    check_tree(torch, out[:n], ref, size, dtype, uses_tiles(dtype, bits, counts, G))
+    ref, size, reach = tree64(q[:n], pool, tables, held, lines, 1 / math.sqrt(d), window, sk)
+    check_tree(torch, out[:n], ref, size, reach, dtype, uses_tiles(dtype, bits, counts, G), bits)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -438,28 +452,58 @@ def test_tree_many_short_sequences(cuda, dtype, bits):
     run_tree(cuda, dtype, bits, 64, 2, 2, 16, [rng.randint(0, 90) for _ in range(300)], [rng.randint(0, 12) for _ in range(300)], seed=6)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 8), ("bf16", 4)])
 @pytest.mark.parametrize("G,d", [(2, 64), (8, 128)])
 @pytest.mark.parametrize("window", [0, 100])
-def test_tree_many_segments_per_cta(cuda, dtype, G, d, window):
+def test_tree_many_segments_per_cta(cuda, dtype, bits, G, d, window):
     """Short sequences, some of a single tile, several of them for every CTA."""
     rng = random.Random(8)
-    run_tree(cuda, dtype, 0, d, 8, G, 32, [rng.choice([0, 20, 129, rng.randint(0, 700)]) for _ in range(120)],
+    run_tree(cuda, dtype, bits, d, 8, G, 32, [rng.choice([0, 20, 129, rng.randint(0, 700)]) for _ in range(120)],
              [rng.randint(10, 40) for _ in range(120)], window=window, seed=9)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("bf16", 4)])
 @pytest.mark.parametrize("scale", [1e-3, 30.0])
-def test_tree_small_and_large_values(cuda, dtype, scale):
-    run_tree(cuda, dtype, 0, 128, 2, 4, 64, [700, 90], [33, 20], scale=scale, seed=7)
+def test_tree_small_and_large_values(cuda, dtype, bits, scale):
+    run_tree(cuda, dtype, bits, 128, 2, 4, 64, [700, 90], [33, 20], scale=scale, seed=7)
+    run_tree(cuda, dtype, bits, 64, 2, 16, 64, [700, 90], [33, 20], scale=scale, seed=8)
+
+
+@pytest.mark.parametrize("n", [9, 40])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_tree_code_tiles_of_very_different_size(cuda, bits, n):
+    """Scales of K and V that change from page to page by up to 2^60 (down, up, zero), so that the powers of tiles and of O
+    move; queries of rows that differ as much."""
+    import sparse_decode as sd
+    torch = cuda
+    hkv, G, d, page, held = 2, 4, 64, 64, 640
+    pool = Pool(torch, sd, "bf16", bits, hkv, d, page, 14, 5)
+    tables = tables_of(torch, [held + n], page, 14, 6)
+    ups = [0, -20, 3, 40, -40, 8, 9, 0, -8, 16, 0]
+    for j, u in enumerate(ups):
+        pg = int(tables[0, j])
+        for a, sign in zip(pool.arrays, (-1, 1)):  # keys and values in opposite order
+            f = 2.0 ** (u * sign if sign > 0 else min(u * sign, 2)) if j != 7 else 0.0
+            for x in a[1:]:
+                x[pg] *= f
+    for a, values in zip(pool.arrays, range(2)):
+        grow = lambda t: t.double().repeat_interleave(64, -1)  # noqa: E731
+        words = (a[0].long() & 0xFFFFFFFF)[..., None] >> (torch.arange(32 // bits, device="cuda") * bits)
+        pool.values[values] = (words & ((1 << bits) - 1)).flatten(-2).double() * grow(a[1]) + grow(a[2])
+    q = torch.randn(n, hkv * G, d, generator=gen(torch, 8), device="cuda")
+    q = (q * torch.exp2(torch.arange(n, device="cuda") % 5 * -20.0)[:, None, None]).bfloat16()
+    out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [held + n]), i32(torch, [0, n]))
+    lines = [[((2 << i) - 1, held + i) for i in range(n)]]
+    ref, size, reach = tree64(q, pool, tables, [held], lines, 1 / math.sqrt(d))
+    check_tree(torch, out, ref, size, reach, "bf16", True, bits)
 
 
 def test_tree_hidden_nodes_do_not_reach_their_siblings(cuda):
     """Two branches from one root: infinities and not-a-numbers in one branch's keys and values leave the other alone."""
     import sparse_decode as sd
     torch = cuda
-    for dtype in ("f32", "f16"):
-        pool = Pool(torch, sd, dtype, 0, 2, 64, 16, 8, 3)
+    for dtype, bits in (("f32", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("f32", 8)):
+        pool = Pool(torch, sd, dtype, bits, 2, 64, 16, 8, 3)
         tables, held = i32(torch, [[1, 4, 6, 2]]), 37
         parents = [-1, 0, 0, 1, 2, 3]
         masks = torch.tensor([m for m, _ in lineage(parents)], dtype=torch.int64, device="cuda")
@@ -469,7 +513,7 @@ def test_tree_hidden_nodes_do_not_reach_their_siblings(cuda):
         for a, x in zip(pool.arrays, (float("nan"), float("inf"))):
             for node in (2, 4):
                 t = held + node
-                a[0][int(tables[0, t // 16]), :, t % 16, 5] = x
+                a[-1][int(tables[0, t // 16]), :, t % 16, 0 if bits else 5] = x  # a value, or a group's bias
         out = call()
         for node in (0, 1, 3, 5):
             assert torch.equal(out[node], clean[node])
@@ -777,8 +821,8 @@ def test_tree_scales_of_either_sign_and_none(cuda):
         for scale in (-0.2, 0.0):
             out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [300 + n]), i32(torch, [0, n]), None, scale)
             lines = [[((2 << i) - 1, 300 + i) for i in range(n)]]
-            ref, size = tree64(q, pool, tables, [300], lines, scale)
-            check_tree(torch, out, ref, size, "bf16", n * 4 > 16)
+            ref, size, reach = tree64(q, pool, tables, [300], lines, scale)
+            check_tree(torch, out, ref, size, reach, "bf16", n * 4 > 16)
 
 
 def test_python_refusals(cuda):
