@@ -5,9 +5,10 @@
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
 // 64 tokens), P = 2^(S - m), O += P V. S, P -- the second product's left operand --
-// and O live in tensor memory, Q, K and V are 128B-swizzled tiles in shared memory (TMA, one box per page and 64 dimensions). One warp
-// loads, two groups of four warps hold a row per thread and make P, each with its
-// own S and O and a warp that issues its products:
+// and O live in tensor memory, Q, K and V are 128B-swizzled tiles in shared memory
+// (TMA, one box per page and 64 dimensions). One warp loads, two groups of four
+// warps hold a row per thread and make P, each with its own S and O and a warp that
+// issues its products:
 //   SHARED: the pair has up to 256 columns, 128 per group, and both groups use
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
@@ -274,235 +275,245 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   int it0 = 0;  // tiles of the segments before
   Waiter<BITS == 0> wait{p.flags, false};
 
-  // The registers of a launch for codes (16 warps x 128) shared out anew: 8 x 168 for the weights, 8 x 88.
+  // The registers of a launch for codes (16 warps x 128) shared out anew: 8 x 152 for the weights, 8 x 104.
   if (warp >= 8) {
-    if constexpr (BITS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 8) {  // ---- loads ----
-    const uint64_t pol = stream_policy(false);
-    const int pb = min(p.P, kTileT), nb = kTileT / pb;  // rows per box, boxes per tile
-    const int p_log = __ffs(p.P) - 1;
-    const int oob_row = int(p.n_pages * p.Hkv * p.P);  // past the tensor: TMA fills zeros
-    int use = 0, st = 0;  // stages used so far, the next one
-    uint32_t round = 0;
-    while (walk.next(s)) {
-      const TreeSeq sq = tree_seq(p, s.b);
-      const int* row = p.tables + int64_t(s.b) * p.W;
-      const int t0 = sq.begin / kTileT, last_slot = (sq.end - 1) >> p_log, first_slot = sq.begin >> p_log;
-      auto load = [&](int slot) { return slot >= first_slot && slot <= last_slot ? row[slot] : -1; };
-      int base = ((t0 + s.i0) * kTileT) >> p_log;
-      int cur = load(base + lane), nxt = load(base + 32 + lane);
-      for (int i = s.i0; i < s.i1 && !wait.dead; ++i) {
-        const int tok = (t0 + i) * kTileT;
-        if ((tok >> p_log) - base >= 32) {
-          base += 32;
-          cur = nxt;
-          nxt = load(base + 32 + lane);
-        }
-        const int tj = tok + (lane < nb ? lane : 0) * pb, off = (tj >> p_log) - base;
-        const int a = __shfl_sync(0xffffffffu, cur, off & 31), c = __shfl_sync(0xffffffffu, nxt, off & 31);
-        const int page = off < 32 ? a : c;
-        const bool need = lane < nb && tj < sq.end && tj + pb > sq.begin;
-        int y = oob_row;
-        if (need) {
-          if (page >= 0 && page < p.n_pages) y = int((int64_t(page) * p.Hkv + s.h) * p.P + (tj & (p.P - 1)));
-          else if (p.flags) atomicOr(p.flags, kErrBadIndex);
-        }
-        const int n_box = __popc(__ballot_sync(0xffffffffu, need));
-        if constexpr (BITS) {  // K and V and their scales, as they are, in one stage
-          if (use >= p.raw_stages && !wait(bars->raw_empty + st, round ^ 1u)) break;
-          uint64_t* full = bars->raw_full + st;
-          uint8_t* stage = raws + st * kRaw;
-          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n_box * 2 * pb * kRow));
-          __syncwarp();
-          if (need) {
-            tma_load_3d(stage + lane * pb * kRow, &tmK, 0, y, 0, full, pol);
-            tma_load_3d(stage + (kTileT + lane * pb) * kRow, &tmV, 0, y, 0, full, pol);
-          }
-          constexpr int ROW = D / 64 * 2, CPA = kSb / 16;  // bytes of a token in each array of scales, 16-byte pieces of a tile
-          const uint8_t* src[4] = {static_cast<const uint8_t*>(p.k_scales), static_cast<const uint8_t*>(p.k_biases),
-                                   static_cast<const uint8_t*>(p.v_scales), static_cast<const uint8_t*>(p.v_biases)};
-          const uint32_t sb = smem_u32(stage + 2 * kTileT * kRow);
-          const int byte = lane * 16, j = min(byte / ROW / pb, nb - 1);  // the box this piece's tokens lie in
-          const int64_t kr = __shfl_sync(0xffffffffu, y, j);
-          const bool good = __shfl_sync(0xffffffffu, int(need && y != oob_row), j);
-          if (lane < CPA) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              cp_async16_zfill(sb + x * kSb + byte, good ? src[x] + (kr * ROW + byte - j * pb * ROW) : src[x], good ? 16 : 0);
-          }
-          cp_async_arrive(full);
-          ++use;
-          if (++st == p.raw_stages) {
-            st = 0;
-            round ^= 1u;
-          }
-        } else {
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (use >= p.stages && !wait(bars->empty + st, round ^ 1u)) break;
-          uint64_t* full = bars->full + st;
-          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n_box * NH * pb * 128));
-          __syncwarp();
-          if (need) {
-            uint8_t* dst = ring + st * kStage + lane * pb * 128;
-#pragma unroll
-            for (int h = 0; h < NH; ++h) tma_load_3d(dst + h * kHalf, kv ? &tmV : &tmK, 0, y, h, full, pol);
-          }
-          ++use;
-          if (++st == p.stages) {
-            st = 0;
-            round ^= 1u;
-          }
-        }
-      }
-      }
-    }
-    if (wait.dead) {  // what is under way lands in this CTA's shared memory
-      uint64_t* full = BITS ? bars->raw_full : bars->full;
-      const int n = BITS ? p.raw_stages : p.stages;
-      for (int u = max(0, use - n); u < use; ++u) mbar_wait(full + u % n, uint32_t(u / n) & 1u, nullptr);
-    }
-  } else if (warp == 9 || warp == 10) {  // ---- products of a group ----
-    const int w = warp - 9;
-    uint32_t seg = 0, k = 0;  // segments that the group took part in and tiles: the parities of its barriers
-    const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + (kQs == 2 ? w * kQ : 0)) >> 4);
-    const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
-    const uint32_t ds = tmem + kSCol + w * 128, dp = tmem + kPCol + w * 128, dO = tmem + kOCol + w * 128;
-    const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full + w);
-    while (walk.next(s)) {
-      const int nt = s.i1 - s.i0, n = SHARED ? nt : (nt + 1 - w) / 2;
-      if (n > 0) {
-        // A group without tiles (a segment of one) loads no rows of Q: it could run ahead by more than a phase. The
-        // second group begins when the first has weighed its first tile: out of step, one's exponentials overlap the
-        // other's loads, maxima and stores.
-        if (w == 1 && k == 0) wait(&bars->started, 0);
-        wait(bars->q_full + w, seg++ & 1u);
-      }
-      const int u = 2 * (it0 + (SHARED ? 0 : w));
-      int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
-      // The scores of tile i + 1, then P V of tile i. The first scores follow the rows of Q: with those the group has
-      // read what it needs of its last S and O.
-#pragma unroll 1
-      for (int i = -1; i < n && !wait.dead; ++i) {
-        if (i + 1 < n) {
-          if (!wait(bars->full + ks, uint32_t(kp)) || (i >= 0 && !wait(bars->s_free + w, (k + i) & 1u))) break;
-          tc_fence_after();
-          const uint64_t kd = kd0 + ks * (kStage >> 4);
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-            mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2, product_desc<T>(kTileT, false), c > 0);
-          mma_commit(s_full);
-          mma_commit(empty + ks * 8);
-          ks += SHARED ? 2 : 4;
-          if (ks >= p.stages) ks -= p.stages, kp ^= 1;
-        }
-        if (i >= 0) {
-          const uint32_t h = (k + i) & 1u;  // buffer of P
-          if (!wait(bars->full + vs, uint32_t(vp)) || !wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u)) break;
-          tc_fence_after();
-          const uint64_t v = vd0 + vs * (kStage >> 4);
-          const uint32_t pp = dp + h * (kTileT / 2);
-#pragma unroll
-          for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
-          mma_commit(o_full + h * 8);
-          mma_commit(empty + vs * 8);
-          vs += SHARED ? 2 : 4;
-          if (vs >= p.stages) vs -= p.stages, vp ^= 1;
-        }
-      }
-      k += n;
-      it0 += nt;
-    }
-    mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
-    mbar_wait(&bars->done, 0, p.flags);
-  } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
-    if constexpr (BITS) {
-      constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 64;  // groups, codes of 16 bytes, such pieces
-      constexpr float kTop = float((1 << BITS) - 1);
-      // Two warps for every other tile: what a tile waits for (codes, maxima, a free stage) is hidden by the other pair's.
-      // The numbers of stages are such that a stage stays with a pair.
-      const int pair = (warp - 12) >> 1, ct = (tid - 12 * 32) & 63, cw = (warp - 12) & 1;
+    if constexpr (BITS) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 8) {  // ---- loads ----
+      const uint64_t pol = stream_policy(false);
+      const int pb = min(p.P, kTileT), nb = kTileT / pb;  // rows per box, boxes per tile
+      const int p_log = __ffs(p.P) - 1;
+      const int oob_row = int(p.n_pages * p.Hkv * p.P);  // past the tensor: TMA fills zeros
+      int use = 0, st = 0;  // stages used so far, the next one
+      uint32_t round = 0;
       while (walk.next(s)) {
         const TreeSeq sq = tree_seq(p, s.b);
-        const int t0 = sq.begin / kTileT;
-        for (int i = s.i0; i < s.i1; ++i) {
-          const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
-          if ((t & 1) != pair) continue;
-          const int rs = t % p.raw_stages;
-          wait(bars->raw_full + rs, uint32_t(t / p.raw_stages) & 1u);
-          const uint8_t* raw = raws + rs * kRaw;
-          const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
-          // the largest value of K and of V, and whether a node's V is not finite
-          uint32_t most[2] = {0, 0};
-          bool odd = false;
-#pragma unroll
-          for (int e = 0; e < 2 * NG; ++e) {
-            const int x = ct + 64 * e, v = x / (kTileT * NG), at = x % (kTileT * NG), row = at / NG;
-            const float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]), bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]);
-            const float a = fmaxf(fabsf(bi), fabsf(fmaf(sc, kTop, bi)));
-            const bool in = row >= lo && row < hi, fine = a < INFINITY && fabsf(sc) < INFINITY;  // not-a-numbers are not
-            if (in && fine) most[v] = max(most[v], __float_as_uint(a));
-            odd |= v == 1 && in && row >= old && !fine;
+        const int* row = p.tables + int64_t(s.b) * p.W;
+        const int t0 = sq.begin / kTileT, last_slot = (sq.end - 1) >> p_log, first_slot = sq.begin >> p_log;
+        auto load = [&](int slot) { return slot >= first_slot && slot <= last_slot ? row[slot] : -1; };
+        int base = ((t0 + s.i0) * kTileT) >> p_log;
+        int cur = load(base + lane), nxt = load(base + 32 + lane);
+        for (int i = s.i0; i < s.i1 && !wait.dead; ++i) {
+          const int tok = (t0 + i) * kTileT;
+          if ((tok >> p_log) - base >= 32) {
+            base += 32;
+            cur = nxt;
+            nxt = load(base + 32 + lane);
           }
-          most[0] = __reduce_max_sync(0xffffffffu, most[0]);
-          most[1] = __reduce_max_sync(0xffffffffu, most[1]);
-          odd = __any_sync(0xffffffffu, odd);
-          uint32_t(&mo)[2][4] = most_of[pair][t >> 1 & 1];
-          if (lane == 0) mo[cw][0] = most[0], mo[cw][1] = most[1], mo[cw][2] = odd;
-          named_barrier(4 + pair, 64);
-          const uint32_t mk = max(mo[0][0], mo[1][0]), mv = max(mo[0][1], mo[1][1]), any = mo[0][2] | mo[1][2];
-          const int ek = mk ? max(exponent(__uint_as_float(mk)) - 13, -120) : 0;
-          const int ev = mv ? max((exponent(__uint_as_float(mv)) - 6) & ~7, -120) : kNoPower;
-          if (ct == 0) tile_pow[t % kTreePows] = make_int4(ek, ev, int(any), 0);
-          const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
-#pragma unroll 1
-          for (int v = 0; v < 2; ++v) {
-            const int u = 2 * t + v, st = u % p.stages;
-            if (u >= p.stages) wait(bars->empty + st, (uint32_t(u / p.stages) & 1u) ^ 1u);
-            if (!wait.dead) {
-              const uint32_t dst = smem_u32(ring) + st * kStage;
-              const float f = v ? fv : fk;
-#pragma unroll 2
-              for (int e = 0; e < N; ++e) {
-                const int x = ct + 64 * e, row = x / CPR, c = x % CPR, el = c * EPC;  // row, piece, its first element
-                const uint4 w = *reinterpret_cast<const uint4*>(raw + (v * kTileT + row) * kRow + c * 16);
-                const int at = row * NG + el / 64;
-                float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]) * f, bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]) * f;
-                // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
-                const bool none = v && (row < lo || row >= hi || (row >= old && !(fabsf(sc) + fabsf(bi) < INFINITY)));
-                if (none) sc = bi = 0.0f;
-                const uint32_t b2 = pack2<__half>(bi, bi), s2 = pack2<__half>(sc, BITS == 8 ? sc : sc * 0.0625f);
-                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          const int tj = tok + (lane < nb ? lane : 0) * pb, off = (tj >> p_log) - base;
+          const int a = __shfl_sync(0xffffffffu, cur, off & 31), c = __shfl_sync(0xffffffffu, nxt, off & 31);
+          const int page = off < 32 ? a : c;
+          const bool need = lane < nb && tj < sq.end && tj + pb > sq.begin;
+          int y = oob_row;
+          if (need) {
+            if (page >= 0 && page < p.n_pages) y = int((int64_t(page) * p.Hkv + s.h) * p.P + (tj & (p.P - 1)));
+            else if (p.flags) atomicOr(p.flags, kErrBadIndex);
+          }
+          const int n_box = __popc(__ballot_sync(0xffffffffu, need));
+          if constexpr (BITS) {  // K and V and their scales, as they are, in one stage
+            if (use >= p.raw_stages && !wait(bars->raw_empty + st, round ^ 1u)) break;
+            uint64_t* full = bars->raw_full + st;
+            uint8_t* stage = raws + st * kRaw;
+            if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n_box * 2 * pb * kRow));
+            __syncwarp();
+            if (need) {
+              tma_load_3d(stage + lane * pb * kRow, &tmK, 0, y, 0, full, pol);
+              tma_load_3d(stage + (kTileT + lane * pb) * kRow, &tmV, 0, y, 0, full, pol);
+            }
+            constexpr int ROW = D / 64 * 2, CPA = kSb / 16;  // bytes of a token in each array of scales, 16-byte pieces of a tile
+            const uint8_t* src[4] = {static_cast<const uint8_t*>(p.k_scales), static_cast<const uint8_t*>(p.k_biases),
+                                     static_cast<const uint8_t*>(p.v_scales), static_cast<const uint8_t*>(p.v_biases)};
+            const uint32_t sb = smem_u32(stage + 2 * kTileT * kRow);
+            const int byte = lane * 16, j = min(byte / ROW / pb, nb - 1);  // the box this piece's tokens lie in
+            const int64_t kr = __shfl_sync(0xffffffffu, y, j);
+            const bool good = __shfl_sync(0xffffffffu, int(need && y != oob_row), j);
+            if (lane < CPA) {
 #pragma unroll
-                for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
-                  uint32_t h[4];
-                  if constexpr (BITS == 8) {
-                    uint32_t a[2], b[2];
-                    codes8(words[2 * j], p.magic, a);
-                    codes8(words[2 * j + 1], p.magic, b);
-                    h[0] = fma_f16x2(a[0], s2, b2), h[1] = fma_f16x2(a[1], s2, b2);
-                    h[2] = fma_f16x2(b[0], s2, b2), h[3] = fma_f16x2(b[1], s2, b2);
-                  } else {
+              for (int x = 0; x < 4; ++x)
+                cp_async16_zfill(sb + x * kSb + byte, good ? src[x] + (kr * ROW + byte - j * pb * ROW) : src[x], good ? 16 : 0);
+            }
+            cp_async_arrive(full);
+            ++use;
+            if (++st == p.raw_stages) {
+              st = 0;
+              round ^= 1u;
+            }
+          } else {
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) h[y] = fma_f16x2(codes4(words[j], y, p.magic), s2, b2);
-                  }
-                  const int ch = (el + 8 * j) / 8;
-                  const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
-                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                }
+            for (int kv = 0; kv < 2; ++kv) {
+              if (use >= p.stages && !wait(bars->empty + st, round ^ 1u)) break;
+              uint64_t* full = bars->full + st;
+              if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n_box * NH * pb * 128));
+              __syncwarp();
+              if (need) {
+                uint8_t* dst = ring + st * kStage + lane * pb * 128;
+#pragma unroll
+                for (int h = 0; h < NH; ++h) tma_load_3d(dst + h * kHalf, kv ? &tmV : &tmK, 0, y, h, full, pol);
               }
-              fence_proxy_async_shared();
-              warp_arrive(bars->full + st);
-              if (v) warp_arrive(bars->raw_empty + rs);
+              ++use;
+              if (++st == p.stages) {
+                st = 0;
+                round ^= 1u;
+              }
             }
           }
         }
-        it0 += s.i1 - s.i0;
+      }
+      if (wait.dead) {  // what is under way lands in this CTA's shared memory
+        uint64_t* full = BITS ? bars->raw_full : bars->full;
+        const int n = BITS ? p.raw_stages : p.stages;
+        for (int u = max(0, use - n); u < use; ++u) mbar_wait(full + u % n, uint32_t(u / n) & 1u, nullptr);
+      }
+    } else if (warp == 9 || warp == 10) {  // ---- products of a group ----
+      const int w = warp - 9;
+      uint32_t seg = 0, k = 0;  // segments that the group took part in and tiles: the parities of its barriers
+      const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + (kQs == 2 ? w * kQ : 0)) >> 4);
+      const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
+      const uint32_t ds = tmem + kSCol + w * 128, dp = tmem + kPCol + w * 128, dO = tmem + kOCol + w * 128;
+      const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full + w);
+      while (walk.next(s)) {
+        const int nt = s.i1 - s.i0, n = SHARED ? nt : (nt + 1 - w) / 2;
+        if (n > 0) {
+          // A group without tiles (a segment of one) loads no rows of Q: it could run ahead by more than a phase. The
+          // second group begins when the first has weighed its first tile: out of step, one's exponentials overlap the
+          // other's loads, maxima and stores.
+          if (w == 1 && k == 0) wait(&bars->started, 0);
+          wait(bars->q_full + w, seg++ & 1u);
+        }
+        const int u = 2 * (it0 + (SHARED ? 0 : w));
+        int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
+        // The scores of tile i + 1, then P V of tile i. The first scores follow the rows of Q: with those the group has
+        // read what it needs of its last S and O.
+#pragma unroll 1
+        for (int i = -1; i < n && !wait.dead; ++i) {
+          if (i + 1 < n) {
+            if (!wait(bars->full + ks, uint32_t(kp)) || (i >= 0 && !wait(bars->s_free + w, (k + i) & 1u))) break;
+            tc_fence_after();
+            const uint64_t kd = kd0 + ks * (kStage >> 4);
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c)
+              mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2,
+                       product_desc<T>(kTileT, false), c > 0);
+            mma_commit(s_full);
+            mma_commit(empty + ks * 8);
+            ks += SHARED ? 2 : 4;
+            if (ks >= p.stages) ks -= p.stages, kp ^= 1;
+          }
+          if (i >= 0) {
+            const uint32_t h = (k + i) & 1u;  // buffer of P
+            if (!wait(bars->full + vs, uint32_t(vp)) || !wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u)) break;
+            tc_fence_after();
+            const uint64_t v = vd0 + vs * (kStage >> 4);
+            const uint32_t pp = dp + h * (kTileT / 2);
+#pragma unroll
+            for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
+            mma_commit(o_full + h * 8);
+            mma_commit(empty + vs * 8);
+            vs += SHARED ? 2 : 4;
+            if (vs >= p.stages) vs -= p.stages, vp ^= 1;
+          }
+        }
+        k += n;
+        it0 += nt;
+      }
+      mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
+      mbar_wait(&bars->done, 0, p.flags);
+    } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
+      if constexpr (BITS) {
+        constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 64;  // groups, codes of 16 bytes, such pieces
+        constexpr float kTop = float((1 << BITS) - 1);
+        // Two warps for every other tile: what a tile waits for (codes, maxima, a free stage) is hidden by the other pair's.
+        // The numbers of stages are such that a stage stays with a pair.
+        const int pair = (warp - 12) >> 1, ct = (tid - 12 * 32) & 63, cw = (warp - 12) & 1;
+        while (walk.next(s)) {
+          const TreeSeq sq = tree_seq(p, s.b);
+          const int t0 = sq.begin / kTileT;
+          for (int i = s.i0; i < s.i1; ++i) {
+            const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
+            if ((t & 1) != pair) continue;
+            const int rs = t % p.raw_stages;
+            wait(bars->raw_full + rs, uint32_t(t / p.raw_stages) & 1u);
+            const uint8_t* raw = raws + rs * kRaw;
+            const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
+            // the largest value of K and of V, and whether a node's V is not finite
+            uint32_t most[2] = {0, 0};
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 2 * NG; ++e) {
+              const int x = ct + 64 * e, v = x / (kTileT * NG), at = x % (kTileT * NG), row = at / NG;
+              const float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]), bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]);
+              const float a = fmaxf(fabsf(bi), fabsf(fmaf(sc, kTop, bi)));
+              const bool in = row >= lo && row < hi, fine = a < INFINITY && fabsf(sc) < INFINITY;  // not-a-numbers are not
+              if (in && fine) most[v] = max(most[v], __float_as_uint(a));
+              odd |= v == 1 && in && row >= old && !fine;
+            }
+            most[0] = __reduce_max_sync(0xffffffffu, most[0]);
+            most[1] = __reduce_max_sync(0xffffffffu, most[1]);
+            odd = __any_sync(0xffffffffu, odd);
+            uint32_t(&mo)[2][4] = most_of[pair][t >> 1 & 1];
+            if (lane == 0) mo[cw][0] = most[0], mo[cw][1] = most[1], mo[cw][2] = odd;
+            named_barrier(4 + pair, 64);
+            const uint32_t mk = max(mo[0][0], mo[1][0]), mv = max(mo[0][1], mo[1][1]), any = mo[0][2] | mo[1][2];
+            const int ek = mk ? max(exponent(__uint_as_float(mk)) - 13, -120) : 0;
+            const int ev = mv ? max((exponent(__uint_as_float(mv)) - 6) & ~7, -120) : kNoPower;
+            if (ct == 0) tile_pow[t % kTreePows] = make_int4(ek, ev, int(any), 0);
+            const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
+#pragma unroll 1
+            for (int v = 0; v < 2; ++v) {
+              const int u = 2 * t + v, st = u % p.stages;
+              if (u >= p.stages) wait(bars->empty + st, (uint32_t(u / p.stages) & 1u) ^ 1u);
+              if (!wait.dead) {
+                const uint32_t dst = smem_u32(ring) + st * kStage;
+                const float f = v ? fv : fk;
+                constexpr int NB = N < 4 ? N : 4;  // pieces whose loads are under way together
+#pragma unroll 1
+                for (int e0 = 0; e0 < N; e0 += NB) {
+                  uint4 w[NB];
+                  uint32_t s2[NB], b2[NB];
+#pragma unroll
+                  for (int e = 0; e < NB; ++e) {
+                    const int x = ct + 64 * (e0 + e), row = x / CPR, c = x % CPR, at = row * NG + c * EPC / 64;  // row, piece
+                    w[e] = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
+                    float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]) * f;
+                    float bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]) * f;
+                    // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
+                    if (v && (row < lo || row >= hi || (row >= old && !(fabsf(sc) + fabsf(bi) < INFINITY)))) sc = bi = 0.0f;
+                    b2[e] = pack2<__half>(bi, bi), s2[e] = pack2<__half>(sc, BITS == 8 ? sc : sc * 0.0625f);
+                  }
+#pragma unroll
+                  for (int e = 0; e < NB; ++e) {
+                    const int x = ct + 64 * (e0 + e), row = x / CPR, c = x % CPR;
+                    const uint32_t words[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+#pragma unroll
+                    for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
+                      uint32_t h[4];
+                      if constexpr (BITS == 8) {
+                        uint32_t a[2], b[2];
+                        codes8(words[2 * j], p.magic, a);
+                        codes8(words[2 * j + 1], p.magic, b);
+                        h[0] = fma_f16x2(a[0], s2[e], b2[e]), h[1] = fma_f16x2(a[1], s2[e], b2[e]);
+                        h[2] = fma_f16x2(b[0], s2[e], b2[e]), h[3] = fma_f16x2(b[1], s2[e], b2[e]);
+                      } else {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) h[y] = fma_f16x2(codes4(words[j], y, p.magic), s2[e], b2[e]);
+                      }
+                      const int ch = c * EPC / 8 + j;
+                      const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+                      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    }
+                  }
+                }
+                fence_proxy_async_shared();
+                warp_arrive(bars->full + st);
+                if (v) warp_arrive(bars->raw_empty + rs);
+              }
+            }
+          }
+          it0 += s.i1 - s.i0;
+        }
       }
     }
-  }
   } else {  // ---- weights: a row per thread ----
-    if constexpr (BITS) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if constexpr (BITS) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
     const uint32_t ts = tmem + lanes + kSCol + w * 128, tp = tmem + lanes + kPCol + w * 128, to = tmem + lanes + kOCol + w * 128;
