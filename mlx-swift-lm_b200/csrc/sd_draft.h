@@ -122,9 +122,7 @@ constexpr int kTreeTileSmem = 232448 - 4096;  // beside 4 KB of static shared me
 // For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
 const void* tree_tile_e1_b0(int D, bool shared);
 const void* tree_tile_e2_b0(int D, bool shared);
-const void* tree_tile_e1_b4(int D, bool shared);
 const void* tree_tile_e2_b4(int D, bool shared);
-const void* tree_tile_e1_b8(int D, bool shared);
 const void* tree_tile_e2_b8(int D, bool shared);
 
 struct TileLayout {

@@ -32,10 +32,9 @@ TreeSet lookup_tree(int dtype, int bits, int D, int columns) {
 }
 
 const void* (*lookup_tile(int dtype, int bits))(int, bool) {
-  const bool half = dtype == SD_F16;
-  return bits == 0 ? half ? tree_tile_e1_b0 : tree_tile_e2_b0
-         : bits == 4 ? half ? tree_tile_e1_b4 : tree_tile_e2_b4
-                     : half ? tree_tile_e1_b8 : tree_tile_e2_b8;
+  if (dtype == SD_F16) return bits == 0 ? tree_tile_e1_b0 : nullptr;
+  if (dtype != SD_BF16) return nullptr;
+  return bits == 0 ? tree_tile_e2_b0 : bits == 4 ? tree_tile_e2_b4 : tree_tile_e2_b8;
 }
 
 bool good_page(int P) { return P == 16 || P == 32 || P == 64 || P == 128 || P == 256; }
@@ -69,10 +68,13 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   const TreeSet set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
   if (!set.attend) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   s->merge = set.merge;
-  s->tiles = g->dtype != SD_F32 && columns > kTreeColumns;
+  // Codes of fp16 pools are not for the tile kernel: its fp16 tiles of them cost as much as such an output's own rounding,
+  // twice over (4e-4 of the result, relative, instead of 2e-4; nothing to speak of beside bf16's 1.7e-3).
+  const auto tile_kernel = lookup_tile(g->dtype, g->kv_bits);
+  s->tiles = tile_kernel && columns > kTreeColumns;
   if (s->tiles) {
     const bool shared = columns > 128;
-    s->attend = lookup_tile(g->dtype, g->kv_bits)(D, shared);
+    s->attend = tile_kernel(D, shared);
     s->threads = g->kv_bits ? kTreeCodeThreads : kTreeTileThreads;
     s->smem_most = kTreeTileSmem;
     s->lay = tree_tile_layout(batch, D, g->kv_bits, shared);
@@ -94,7 +96,8 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->ctas = 2 * sms;
     s->seg_units = kSegmentUnits;
   }
-  if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1) || (s->tiles && g->kv_bits && s->lay.raw_stages < 2)) return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
+  if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1) || (s->tiles && g->kv_bits && s->lay.raw_stages < 2))
+    return fail(SD_ERR_SHAPE, "batch %d leaves no shared memory for the tiles", batch);
   // a sequence's last pair may be almost empty; no more pairs than columns
   s->pairs = g->n_kv_heads * std::min(int64_t(n_rows) * G, int64_t(n_rows) * G / s->columns + batch);
   s->part_floats = paged_part_floats(s->columns, D);

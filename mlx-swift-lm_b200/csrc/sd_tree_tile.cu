@@ -1,7 +1,7 @@
 // sd_tree_tile.cu -- attention of many (node, query head) columns per sequence
-// on the fifth-generation tensor cores, for 16-bit pools and for codes with
-// 16-bit scales; compiled once per (SD_E, SD_BITS) pair. See sd_tree.cuh for what
-// it is a part of.
+// on the fifth-generation tensor cores, for 16-bit pools and for codes of bf16
+// ones; compiled once per (SD_E, SD_BITS) pair. See sd_tree.cuh for what it is a
+// part of.
 //
 // A pair's columns are the rows of 128-row accumulators: S = Q K^T (128 rows x
 // 64 tokens), P = 2^(S - m), O += P V. S, P -- the second product's left operand --
@@ -28,18 +28,20 @@
 // node gets back at the end.
 // Codes: the loading warp brings them as they are, with their scales, and four
 // more warps make tiles of fp16 values of them, s c + b by one packed fma each.
-// fp16 has 11 bits, three more than bf16, but a narrow range, so a tile of K, or
-// of V, is scaled by a power of two of its own -- exactly, as the scales have no
-// more than 11 bits: the largest of K goes to [2^13, 2^14), of V to [2^6, 2^14) in
-// steps of 2^8, and the scores, or weights and O, take the power back. Queries of
-// bf16 are scaled row by row in the same way.
+// fp16 has 11 bits, three more than the bf16 of the result, but a narrow range, so a
+// tile of K, or of V, is scaled by a power of two of its own -- exactly, as bf16
+// scales have 8 bits: the largest of K goes to [2^13, 2^14), of V to [2^6, 2^14) in
+// steps of 2^8, and the scores, or weights and O, take the power back. Queries are
+// scaled row by row in the same way.
 #include "sd_tree.cuh"
 
 #if !defined(SD_E) || !defined(SD_BITS)
 #error "SD_E and SD_BITS must be defined"
 #endif
 
-#if SD_E == 1
+#if SD_E == 1 && SD_BITS != 0
+#error "codes of fp16 pools: tree_attend_kernel"
+#elif SD_E == 1
 using ET = __half;
 #else
 using ET = __nv_bfloat16;
@@ -392,7 +394,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
             for (int c = 0; c < D / 16; ++c)
               mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2,
-                       product_desc<T>(kTileT, false), c > 0);
+                     product_desc<T>(kTileT, false), c > 0);
             mma_commit(s_full);
             mma_commit(empty + ks * 8);
             ks += SHARED ? 2 : 4;
@@ -541,22 +543,21 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           for (int i = 0; i < N; ++i) {
             const int row = r / CPR + RPT * i;
             if constexpr (BITS != 0) {
-              if constexpr (!__is_same(E, __half)) {  // bf16: the row's largest to [2^13, 2^14), all of its 8 bits in fp16
-                uint32_t w4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                float f[8], top = 0.0f;
+              // bf16: the row's largest to [2^13, 2^14), all of its 8 bits in fp16
+              uint32_t w4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+              float f[8], top = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  unpack_word<E>(w4[j], f + 2 * j);
-                  top = fmaxf(top, fmaxf(fabsf(f[2 * j]), fabsf(f[2 * j + 1])));
-                }
-#pragma unroll
-                for (int j = 1; j < CPR; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
-                const int e = top > 0.0f && top < INFINITY ? min(max(exponent(top) - 13, -120), 120) : 0;
-                const float down = power(-e);
-                v[i].x = pack2<__half>(f[0] * down, f[1] * down), v[i].y = pack2<__half>(f[2] * down, f[3] * down);
-                v[i].z = pack2<__half>(f[4] * down, f[5] * down), v[i].w = pack2<__half>(f[6] * down, f[7] * down);
-                if (ch == 0) q_pow[SHARED ? w : 0][row] = e;
+              for (int j = 0; j < 4; ++j) {
+                unpack_word<E>(w4[j], f + 2 * j);
+                top = fmaxf(top, fmaxf(fabsf(f[2 * j]), fabsf(f[2 * j + 1])));
               }
+#pragma unroll
+              for (int j = 1; j < CPR; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
+              const int e = top > 0.0f && top < INFINITY ? min(max(exponent(top) - 13, -120), 120) : 0;
+              const float down = power(-e);
+              v[i].x = pack2<__half>(f[0] * down, f[1] * down), v[i].y = pack2<__half>(f[2] * down, f[3] * down);
+              v[i].z = pack2<__half>(f[4] * down, f[5] * down), v[i].w = pack2<__half>(f[6] * down, f[7] * down);
+              if (ch == 0) q_pow[SHARED ? w : 0][row] = e;
             }
             const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
@@ -568,7 +569,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         if (kQs == 1 && w == 0 && s.i1 - s.i0 > 1) warp_arrive(bars->q_full + 1);  // these rows are the second group's, too
       }
       float sq_pow = 1.0f;
-      if constexpr (BITS != 0 && !__is_same(E, __half)) {
+      if constexpr (BITS != 0) {
         // each group loads its rows, or, of one copy and for a group without tiles, the first one
         if (SHARED) named_barrier(2 + w, 128);
         else named_barrier(1, 256);

@@ -79,7 +79,7 @@ def build(force: bool = False, verbose: bool = False, phase_timing: bool = False
         units.append((f"sd_inst_e{e}_b{b}.o", "sd_inst.cu", fmt, _kernel_sources("sd_inst.cu", tree | {"sd_paged.cuh", "sd_paged.h"})))
         units.append((f"sd_paged_e{e}_b{b}.o", "sd_paged_inst.cu", fmt, _kernel_sources("sd_paged_inst.cu", tree | {"sd_decode.cuh"})))
         units.append((f"sd_tree_e{e}_b{b}.o", "sd_tree_inst.cu", fmt, _kernel_sources("sd_tree_inst.cu", {"sd_decode.cuh"})))
-        if e:
+        if e == 2 or (e == 1 and b == 0):  # codes of bf16 pools alone
             units.append((f"sd_tree_tile_e{e}_b{b}.o", "sd_tree_tile.cu", fmt, _kernel_sources("sd_tree_tile.cu", {"sd_decode.cuh"})))
     units.append(("sd_rotary.o", "sd_rotary.cu", [],
                   _kernel_sources("sd_rotary.cu", tree | {"sd_decode.cuh", "sd_paged.cuh"})))
