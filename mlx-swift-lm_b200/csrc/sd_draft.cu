@@ -63,8 +63,11 @@ __device__ __forceinline__ void store4(T* at, int64_t row, int n, const T (&v)[k
 // of which doubles how far up a node has looked, make every mask (a walk up by
 // one load per ancestor took 50 us for 64 trees of 32). The pages taken are
 // written by the same launch where its CTAs can wait until all have read what
-// is held (one cluster of at most 8), and by a second one otherwise.
-// Measured as whole calls: see the table of the operators.
+// is held (one cluster of at most 8), and by a second one otherwise, page by page:
+// neighbouring threads have neighbouring entries of the list.
+// Measured, launches in a graph: one token 2.8 us, 64 trees of 32 nodes 4.4 us,
+// 512 prompts of 2000 tokens 13 us (16.6 MB, 1.3 TB/s; it waits for bisections and
+// tables as much as for stores) and 23 us where they take their 64K pages.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int sm[];
   __shared__ int64_t sums[kPlanThreads / 32];
@@ -221,8 +224,25 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   if (gridDim.x > 1) cluster_sync();  // every CTA has read what is held
   for (int b = blockIdx.x * kPlanThreads + tid; b < p.B; b += gridDim.x * kPlanThreads) {
     const int got = (b + 1 < p.B ? base[b + 1] : pages_end) - base[b];
-    for (int i = 0; i < got; ++i) p.tables[int64_t(b) * p.W + have[b] + i] = __ldcg(p.free_pages + base[b] + i);
     if (got > 0) p.held[b] = have[b] + got;
+  }
+  // kPlanRows neighbouring pages of the list per thread
+  for (int64_t j0 = taken + (blockIdx.x * kPlanThreads + tid) * kPlanRows; j0 < pages_end;
+       j0 += gridDim.x * kPlanThreads * kPlanRows) {
+    int page[kPlanRows], b = 0, hi = p.B;
+#pragma unroll
+    for (int i = 0; i < kPlanRows; ++i)
+      if (j0 + i < pages_end) page[i] = __ldcg(p.free_pages + j0 + i);
+    while (hi - b > 1) {  // the last b with base[b] <= j0: it takes pages
+      const int mid = (b + hi) >> 1;
+      if (base[mid] <= j0) b = mid; else hi = mid;
+    }
+#pragma unroll
+    for (int i = 0; i < kPlanRows; ++i) {
+      if (j0 + i >= pages_end) break;
+      while (b + 1 < p.B && base[b + 1] <= j0 + i) ++b;
+      p.tables[int64_t(b) * p.W + have[b] + j0 + i - base[b]] = page[i];
+    }
   }
   if (blockIdx.x == 0 && tid == 0) *p.taken = pages_end;
 }

@@ -187,7 +187,7 @@ int32_t sd_paged_plan(const sd_plan* g, int32_t* device_flags, sd_stream stream)
   if (grow && !p.commit) {
     p.rows = false;
     p.commit = true;
-    return launch(fn, dim3(1), kPlanThreads, smem, st, args);
+    return launch(fn, dim3(kPlanCluster), kPlanThreads, smem, st, args, kPlanCluster);
   }
   return SD_OK;
 }

@@ -571,8 +571,8 @@ class PagePool:
         return f
 
 
-# New tokens from which on a step's positions are made on the device: on the host 250 of them cost as much as the plan's
-# call and launch, a prompt of 32K tokens 7 ms.
+# New tokens from which on a step's positions are made on the device: there a step takes the host 67 us, whatever its
+# length; with positions made on the host 56 us for 128 tokens, 71 us for 256, 4.0 ms for 32K.
 _PLAN_TOKENS = 256
 
 
