@@ -426,14 +426,15 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         // Two warps for every other tile: what a tile waits for (codes, maxima, a free stage) is hidden by the other pair's.
         // The numbers of stages are such that a stage stays with a pair.
         const int pair = (warp - 12) >> 1, ct = (tid - 12 * 32) & 63, cw = (warp - 12) & 1;
+        int rs = pair, ks = 2 * pair;  // the tile's stages: of codes, of K (V's is the next one); their phases
+        uint32_t rp = 0, kp = 0;
         while (walk.next(s)) {
           const TreeSeq sq = tree_seq(p, s.b);
           const int t0 = sq.begin / kTileT;
           for (int i = s.i0; i < s.i1; ++i) {
             const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
             if ((t & 1) != pair) continue;
-            const int rs = t % p.raw_stages;
-            wait(bars->raw_full + rs, uint32_t(t / p.raw_stages) & 1u);
+            wait(bars->raw_full + rs, rp);
             const uint8_t* raw = raws + rs * kRaw;
             const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
             // the largest value of K and of V, and whether a node's V is not finite
@@ -461,8 +462,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
 #pragma unroll 1
             for (int v = 0; v < 2; ++v) {
-              const int u = 2 * t + v, st = u % p.stages;
-              if (u >= p.stages) wait(bars->empty + st, (uint32_t(u / p.stages) & 1u) ^ 1u);
+              const int st = ks + v;
+              wait(bars->empty + st, kp ^ 1u);  // in the first phase at once
               if (!wait.dead) {
                 const uint32_t dst = smem_u32(ring) + st * kStage;
                 const float f = v ? fv : fk;
@@ -509,6 +510,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
                 if (v) warp_arrive(bars->raw_empty + rs);
               }
             }
+            if ((rs += 2) >= p.raw_stages) rs -= p.raw_stages, rp ^= 1u;
+            if ((ks += 4) >= p.stages) ks -= p.stages, kp ^= 1u;
           }
           it0 += s.i1 - s.i0;
         }
@@ -583,6 +586,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       bool odd = false;  // a node has a value that is not finite
       int ref = kNoPower;  // codes: O's power
       const int n = SHARED ? s.i1 - s.i0 : (s.i1 - s.i0 + 1 - w) / 2;
+      const int u0 = 2 * (it0 + (SHARED ? 0 : w)) + 1;
+      int vs = u0 % p.stages;  // of the tile's V
+      uint32_t vp = uint32_t(u0 / p.stages) & 1u;
 #pragma unroll 1
       for (; steps < n; ++steps, ++k) {
         const int tile = SHARED ? steps : 2 * steps + w;  // of the segment
@@ -596,10 +602,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const bool here = wait(bars->s_full + w, k & 1u);
         if (!BITS && ends && (!SHARED || w == 0)) {
           bool mine = false;
-          const int u = 2 * (it0 + tile) + 1;
-          if (here && wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u)) {
+          if (here && wait(bars->full + vs, vp)) {
             const int row = r >> 1;  // a thread has half of it
-            const uint32_t at = smem_u32(ring) + (u % p.stages) * kStage + row * 128;
+            const uint32_t at = smem_u32(ring) + vs * kStage + row * 128;
             if (row < lo || row >= old) {
 #pragma unroll 2
               for (int c = 0; c < NH * 4; ++c) {
@@ -621,13 +626,14 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         int ev = 0;
         if constexpr (BITS) {
           // What the warps that made the tile wrote of it, before its V, whose stage stays until this group's P is used.
-          const int t = it0 + tile, u = 2 * t + 1;
-          wait(bars->full + u % p.stages, uint32_t(u / p.stages) & 1u);
-          const int4 pw = tile_pow[t % kTreePows];
+          wait(bars->full + vs, vp);
+          const int4 pw = tile_pow[(it0 + tile) & (kTreePows - 1)];
           sc = fminf(fmaxf(scale * sq_pow * power(pw.x), 1.1754944e-38f), 3.4e38f);
           ev = pw.y;
           odd |= pw.z != 0;
         }
+        vs += SHARED ? 2 : 4;
+        if (vs >= p.stages) vs -= p.stages, vp ^= 1u;
         uint32_t va[32], vb[32];
         tmem_ld32(ts, va);
         tmem_ld32(ts + 32, vb);
