@@ -108,8 +108,8 @@ constexpr int kTreeTileTokens = 64;
 constexpr int kTreeTileUnits = 8;  // beginning and ending a segment, in tiles
 constexpr int kTreeTileStages = 24, kTreeTileLeast = 4;
 constexpr int kTreeTileBarBytes = 768;
-// For codes four more warps make tiles of fp16 values of them.
-constexpr int kTreeCodeThreads = 512;
+// For codes eight more warps make tiles of fp16 values of them.
+constexpr int kTreeCodeThreads = 640;
 constexpr int kTreeRawStages = 8;
 constexpr int kTreePows = 32;  // tiles whose powers are kept: more than stages hold
 static_assert(kTreePows > kTreeTileStages / 2 + 1, "a tile's powers are read while later ones are written");
@@ -136,7 +136,7 @@ constexpr TileLayout tree_tile_layout(int batch, int D, int bits, bool shared) {
   TileLayout l{};
   // Where the groups take tiles in turn, a stage stays with the K, or the V, of one of them: a wait for a stage names
   // its phase by the parity, so whoever waits has to know that the phase before is done.
-  // (Of codes, with one of the two pairs of warps that make the tiles, too.)
+  // (Of codes, with one of the two teams of warps that make the tiles, too.)
   const int by = shared && !bits ? 1 : 4;
   if (bits) {  // four tiles of values, or two, and the rest for codes, but two stages at least
     const int fit = (room - 2 * raw) / stage;

@@ -203,7 +203,7 @@ __device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
   uint64_t q_full[2], s_full[2], s_free[2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer of P
-  uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages];
+  uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages], pow_full[kTreeRawStages];
   uint64_t started, done;
   uint32_t tmem;
 };
@@ -230,15 +230,14 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
   __shared__ float2 ml_of[2][SHARED ? 1 : 128];
-  // codes: powers of the last tiles' K and V, and whether a node's V is not finite; of the rows of Q; the warps' maxima
+  // codes: powers of the last tiles' K and V, and whether a node's V is not finite; of the rows of Q
   __shared__ int4 tile_pow[BITS ? kTreePows : 1];
   __shared__ int q_pow[2][BITS ? 128 : 1];
-  __shared__ uint32_t most_of[2][2][2][4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(bars->full + i, BITS ? 2 : 1);
+      mbar_init(bars->full + i, BITS ? 4 : 1);
       mbar_init(bars->empty + i, SHARED ? 2 : 1);  // groups that use the tile
     }
     for (int w = 0; w < 2; ++w) {
@@ -252,7 +251,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     }
     for (int i = 0; i < kTreeRawStages; ++i) {
       mbar_init(bars->raw_full + i, 33);
-      mbar_init(bars->raw_empty + i, 2);
+      mbar_init(bars->raw_empty + i, 4);
+      mbar_init(bars->pow_full + i, 1);
     }
     mbar_init(&bars->started, 4);
     mbar_init(&bars->done, 2);
@@ -277,9 +277,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   int it0 = 0;  // tiles of the segments before
   Waiter<BITS == 0> wait{p.flags, false};
 
-  // The registers of a launch for codes (16 warps x 128) shared out anew: 8 x 152 for the weights, 8 x 104.
+  // The registers of a launch for codes (20 warps x 96) shared out anew: 8 x 144 for the weights, 12 x 64.
   if (warp >= 8) {
-    if constexpr (BITS) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if constexpr (BITS) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 8) {  // ---- loads ----
       const uint64_t pol = stream_policy(false);
       const int pb = min(p.P, kTileT), nb = kTileT / pb;  // rows per box, boxes per tile
@@ -419,46 +419,65 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
       mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
       mbar_wait(&bars->done, 0, p.flags);
-    } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
+    } else if (BITS && warp == 11) {  // ---- powers of the tiles of codes ----
       if constexpr (BITS) {
-        constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 64;  // groups, codes of 16 bytes, such pieces
+        constexpr int NG = D / 64;
         constexpr float kTop = float((1 << BITS) - 1);
-        // Two warps for every other tile: what a tile waits for (codes, maxima, a free stage) is hidden by the other pair's.
-        // The numbers of stages are such that a stage stays with a pair.
-        const int pair = (warp - 12) >> 1, ct = (tid - 12 * 32) & 63, cw = (warp - 12) & 1;
-        int rs = pair, ks = 2 * pair;  // the tile's stages: of codes, of K (V's is the next one); their phases
-        uint32_t rp = 0, kp = 0;
+        int rs = 0;
+        uint32_t rp = 0;
         while (walk.next(s)) {
           const TreeSeq sq = tree_seq(p, s.b);
           const int t0 = sq.begin / kTileT;
-          for (int i = s.i0; i < s.i1; ++i) {
-            const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
-            if ((t & 1) != pair) continue;
+          for (int i = s.i0; i < s.i1; ++i, ++it0) {
+            const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
             wait(bars->raw_full + rs, rp);
-            const uint8_t* raw = raws + rs * kRaw;
-            const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
+            const E* small = reinterpret_cast<const E*>(raws + rs * kRaw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
             // the largest value of K and of V, and whether a node's V is not finite
             uint32_t most[2] = {0, 0};
             bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 2 * NG; ++e) {
-              const int x = ct + 64 * e, v = x / (kTileT * NG), at = x % (kTileT * NG), row = at / NG;
+            for (int e = 0; e < 4 * NG; ++e) {
+              const int v = e / (2 * NG), at = lane + 32 * (e % (2 * NG)), row = at / NG;
               const float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]), bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]);
               const float a = fmaxf(fabsf(bi), fabsf(fmaf(sc, kTop, bi)));
               const bool in = row >= lo && row < hi, fine = a < INFINITY && fabsf(sc) < INFINITY;  // not-a-numbers are not
               if (in && fine) most[v] = max(most[v], __float_as_uint(a));
               odd |= v == 1 && in && row >= old && !fine;
             }
-            most[0] = __reduce_max_sync(0xffffffffu, most[0]);
-            most[1] = __reduce_max_sync(0xffffffffu, most[1]);
+            const uint32_t mk = __reduce_max_sync(0xffffffffu, most[0]), mv = __reduce_max_sync(0xffffffffu, most[1]);
             odd = __any_sync(0xffffffffu, odd);
-            uint32_t(&mo)[2][4] = most_of[pair][t >> 1 & 1];
-            if (lane == 0) mo[cw][0] = most[0], mo[cw][1] = most[1], mo[cw][2] = odd;
-            named_barrier(4 + pair, 64);
-            const uint32_t mk = max(mo[0][0], mo[1][0]), mv = max(mo[0][1], mo[1][1]), any = mo[0][2] | mo[1][2];
             const int ek = mk ? max(exponent(__uint_as_float(mk)) - 13, -120) : 0;
             const int ev = mv ? max((exponent(__uint_as_float(mv)) - 6) & ~7, -120) : kNoPower;
-            if (ct == 0) tile_pow[t % kTreePows] = make_int4(ek, ev, int(any), 0);
+            if (lane == 0) tile_pow[it0 & (kTreePows - 1)] = make_int4(ek, ev, int(odd), 0);
+            warp_arrive(bars->pow_full + rs);
+            if (++rs == p.raw_stages) rs = 0, rp ^= 1u;
+          }
+        }
+      }
+    } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
+      if constexpr (BITS) {
+        constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 128;  // groups, codes of 16 bytes, such pieces
+        // Four warps for every other tile: what a tile waits for (codes, a free stage) is hidden by the other four's.
+        // The numbers of stages are such that a stage stays with one of these teams.
+        const int team = (warp - 12) >> 2, ct = tid & 127;
+        // Eight lanes have the pieces of 64 dimensions of neighbouring rows: what they store at a time lies in 8 different
+        // 16-byte columns.
+        constexpr int PH = 64 / EPC;
+        auto row_of = [](int x) { return x / (8 * NG) * (8 / PH) + x / PH % (8 / PH); };
+        auto piece_of = [](int x) { return x / 8 % NG * PH + x % PH; };
+        int rs = team, ks = 2 * team;  // the tile's stages: of codes, of K (V's is the next one); their phases
+        uint32_t rp = 0, kp = 0;
+        while (walk.next(s)) {
+          const TreeSeq sq = tree_seq(p, s.b);
+          const int t0 = sq.begin / kTileT;
+          for (int i = s.i0; i < s.i1; ++i) {
+            const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
+            if ((t & 1) != team) continue;
+            wait(bars->pow_full + rs, rp);
+            const uint8_t* raw = raws + rs * kRaw;
+            const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
+            const int4 pw = tile_pow[t & (kTreePows - 1)];
+            const int ek = pw.x, ev = pw.y;
             const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
 #pragma unroll 1
             for (int v = 0; v < 2; ++v) {
@@ -467,14 +486,14 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
               if (!wait.dead) {
                 const uint32_t dst = smem_u32(ring) + st * kStage;
                 const float f = v ? fv : fk;
-                constexpr int NB = N < 4 ? N : 4;  // pieces whose loads are under way together
+                constexpr int NB = N < 2 ? N : 2;  // pieces whose loads are under way together
 #pragma unroll 1
                 for (int e0 = 0; e0 < N; e0 += NB) {
                   uint4 w[NB];
                   uint32_t s2[NB], b2[NB];
 #pragma unroll
                   for (int e = 0; e < NB; ++e) {
-                    const int x = ct + 64 * (e0 + e), row = x / CPR, c = x % CPR, at = row * NG + c * EPC / 64;  // row, piece
+                    const int x = ct + 128 * (e0 + e), row = row_of(x), c = piece_of(x), at = row * NG + c / PH;
                     w[e] = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
                     float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]) * f;
                     float bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]) * f;
@@ -484,7 +503,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
                   }
 #pragma unroll
                   for (int e = 0; e < NB; ++e) {
-                    const int x = ct + 64 * (e0 + e), row = x / CPR, c = x % CPR;
+                    const int x = ct + 128 * (e0 + e), row = row_of(x), c = piece_of(x);
                     const uint32_t words[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
 #pragma unroll
                     for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
@@ -518,7 +537,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
     }
   } else {  // ---- weights: a row per thread ----
-    if constexpr (BITS) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    if constexpr (BITS) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int w = warp >> 2, r = tid & 127;  // group, row in it
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the 32 lanes of tensor memory that this warp reaches
     const uint32_t ts = tmem + lanes + kSCol + w * 128, tp = tmem + lanes + kPCol + w * 128, to = tmem + lanes + kOCol + w * 128;
@@ -625,7 +644,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         float sc = scale;
         int ev = 0;
         if constexpr (BITS) {
-          // What the warps that made the tile wrote of it, before its V, whose stage stays until this group's P is used.
+          // Its powers were written before its V was made, whose stage stays until this group's P is used.
           wait(bars->full + vs, vp);
           const int4 pw = tile_pow[(it0 + tile) & (kTreePows - 1)];
           sc = fminf(fmaxf(scale * sq_pow * power(pw.x), 1.1754944e-38f), 3.4e38f);
