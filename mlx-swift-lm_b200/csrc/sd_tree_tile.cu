@@ -127,6 +127,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
 static __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* flags) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
 }
+constexpr uint32_t kMostTries = 1u << 22;  // 0.1 s at least
 template <bool CALL>
 struct Waiter {
   int* flags;
@@ -135,7 +136,12 @@ struct Waiter {
     if constexpr (CALL) {
       if (!dead && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) dead = !wait_on(bar, parity, flags);
     } else {
-      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
+      if (!dead && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        uint32_t tries = 0;
+        while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)) && ++tries < kMostTries) {}
+        dead = tries == kMostTries;
+        if (dead && flags) atomicOr(flags, kErrTimeout);
+      }
     }
     return !dead;
   }
@@ -187,15 +193,18 @@ __device__ __forceinline__ void codes8(uint32_t w, uint32_t magic, uint32_t (&v)
   v[0] = sub_f16x2(raw_u8(w, 0x5150u, magic), 0x64006400u);
   v[1] = sub_f16x2(raw_u8(w, 0x5352u, magic), 0x64006400u);
 }
-// Codes 2 i and 2 i + 1 of a word of nibbles as an fp16 pair, the second one 16 times as large.
-__device__ __forceinline__ uint32_t codes4(uint32_t w, int i, uint32_t magic) {
-  return sub_f16x2((__byte_perm(w, 0u, 0x4040u + 0x0101u * i) & 0x00F0000Fu) | magic, 0x64006400u);
+// Codes 0 and 4, or 1 and 5 -- as 16 times as much --, of a word of nibbles as an fp16 pair. So the tiles hold codes
+// 0 4 1 5 2 6 3 7 of every eight dimensions, as their rows of Q do, and O has its columns in that order.
+template <uint32_t WHICH>
+__device__ __forceinline__ uint32_t codes4(uint32_t w, uint32_t magic) {
+  return sub_f16x2((w & WHICH) | magic, 0x64006400u);
 }
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+__device__ __forceinline__ bool finite(float scale, float bias) { return fabsf(scale) < INFINITY && fabsf(bias) < INFINITY; }
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23 & 255) - 127; }  // of a normal x > 0
@@ -431,24 +440,53 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           for (int i = s.i0; i < s.i1; ++i, ++it0) {
             const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
             wait(bars->raw_full + rs, rp);
-            const E* small = reinterpret_cast<const E*>(raws + rs * kRaw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
-            // the largest value of K and of V, and whether a node's V is not finite
-            uint32_t most[2] = {0, 0};
+            // the largest value of K and of V, and whether a node's V is not finite; a lane has pairs of scales and biases
+            uint32_t* small = reinterpret_cast<uint32_t*>(raws + rs * kRaw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][32 NG]
+            uint32_t sc[2 * NG], bi[2 * NG], most[2] = {0, 0};
             bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 4 * NG; ++e) {
-              const int v = e / (2 * NG), at = lane + 32 * (e % (2 * NG)), row = at / NG;
-              const float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]), bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]);
-              const float a = fmaxf(fabsf(bi), fabsf(fmaf(sc, kTop, bi)));
-              const bool in = row >= lo && row < hi, fine = a < INFINITY && fabsf(sc) < INFINITY;  // not-a-numbers are not
-              if (in && fine) most[v] = max(most[v], __float_as_uint(a));
-              odd |= v == 1 && in && row >= old && !fine;
+            for (int e = 0; e < 2 * NG; ++e) {
+              const int v = e / NG, at = lane + 32 * (e % NG);
+              sc[e] = small[v * 64 * NG + at], bi[e] = small[(v * 2 + 1) * 32 * NG + at];
+              uint32_t x;
+              asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(sc[e]), "r"(BITS == 8 ? 0x437f437fu : 0x41704170u), "r"(bi[e]));
+              most[v] = __vmaxu2(most[v], __vmaxu2(x & 0x7fff7fffu, bi[e] & 0x7fff7fffu));
             }
-            const uint32_t mk = __reduce_max_sync(0xffffffffu, most[0]), mv = __reduce_max_sync(0xffffffffu, most[1]);
-            odd = __any_sync(0xffffffffu, odd);
-            const int ek = mk ? max(exponent(__uint_as_float(mk)) - 13, -120) : 0;
-            const int ev = mv ? max((exponent(__uint_as_float(mv)) - 6) & ~7, -120) : kNoPower;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) most[v] = __reduce_max_sync(0xffffffffu, max(most[v] << 16, most[v] & 0xffff0000u));
+            if (lo > 0 || old < kTileT || most[0] >= 0x7f800000u || most[1] >= 0x7f800000u) {  // what counts, one by one
+              most[0] = most[1] = 0;
+#pragma unroll 1
+              for (int e = 0; e < 4 * NG; ++e) {
+                const int v = e / (2 * NG), x = e % (2 * NG) * 32 + lane, row = x / NG;
+                __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(small) + v * 2 * kTileT * NG + x;
+                const float a = __bfloat162float(at[0]), b = __bfloat162float(at[kTileT * NG]);
+                const bool in = row >= lo && row < hi, fine = finite(a, b);
+                if (in && fine) most[v] = max(most[v], __float_as_uint(fminf(fmaxf(fabsf(b), fabsf(fmaf(a, kTop, b))), 3.4e38f)));
+                // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
+                odd |= v == 1 && in && row >= old && !fine;
+                if (v && (!in || (row >= old && !fine))) at[0] = at[kTileT * NG] = __float2bfloat16_rn(0.0f);
+              }
+              most[0] = __reduce_max_sync(0xffffffffu, most[0]), most[1] = __reduce_max_sync(0xffffffffu, most[1]);
+              odd = __any_sync(0xffffffffu, odd);
+              __syncwarp();
+#pragma unroll
+              for (int e = 0; e < 2 * NG; ++e) {
+                const int v = e / NG, at = lane + 32 * (e % NG);
+                sc[e] = small[v * 64 * NG + at], bi[e] = small[(v * 2 + 1) * 32 * NG + at];
+              }
+            }
+            const int ek = most[0] ? max(exponent(__uint_as_float(most[0])) - 13, -120) : 0;
+            const int ev = most[1] ? max((exponent(__uint_as_float(most[1])) - 6) & ~7, -120) : kNoPower;
             if (lane == 0) tile_pow[it0 & (kTreePows - 1)] = make_int4(ek, ev, int(odd), 0);
+            // scaled and in fp16, in their places
+#pragma unroll
+            for (int e = 0; e < 2 * NG; ++e) {
+              const int v = e / NG, at = lane + 32 * (e % NG);
+              const float f = v ? power(ev == kNoPower ? 0 : -ev) : power(-ek);
+              auto half2 = [&](uint32_t w) { return pack2<__half>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f); };
+              small[v * 64 * NG + at] = half2(sc[e]), small[(v * 2 + 1) * 32 * NG + at] = half2(bi[e]);
+            }
             warp_arrive(bars->pow_full + rs);
             if (++rs == p.raw_stages) rs = 0, rp ^= 1u;
           }
@@ -456,72 +494,54 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
     } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
       if constexpr (BITS) {
-        constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16, N = kTileT * CPR / 128;  // groups, codes of 16 bytes, such pieces
+        constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16;  // groups, codes of 16 bytes, such pieces of a row
         // Four warps for every other tile: what a tile waits for (codes, a free stage) is hidden by the other four's.
         // The numbers of stages are such that a stage stays with one of these teams.
         const int team = (warp - 12) >> 2, ct = tid & 127;
-        // Eight lanes have the pieces of 64 dimensions of neighbouring rows: what they store at a time lies in 8 different
-        // 16-byte columns.
-        constexpr int PH = 64 / EPC;
-        auto row_of = [](int x) { return x / (8 * NG) * (8 / PH) + x / PH % (8 / PH); };
-        auto piece_of = [](int x) { return x / 8 % NG * PH + x % PH; };
+        constexpr int PH = 64 / EPC;  // pieces of 64 dimensions: eight lanes have those of neighbouring rows, and what they
+                                      // store at a time lies in eight different 16-byte columns
         int rs = team, ks = 2 * team;  // the tile's stages: of codes, of K (V's is the next one); their phases
         uint32_t rp = 0, kp = 0;
         while (walk.next(s)) {
-          const TreeSeq sq = tree_seq(p, s.b);
-          const int t0 = sq.begin / kTileT;
-          for (int i = s.i0; i < s.i1; ++i) {
-            const int t = it0 + i - s.i0, tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
+          for (int t = it0; t < it0 + s.i1 - s.i0; ++t) {
             if ((t & 1) != team) continue;
             wait(bars->pow_full + rs, rp);
             const uint8_t* raw = raws + rs * kRaw;
-            const E* small = reinterpret_cast<const E*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
-            const int4 pw = tile_pow[t & (kTreePows - 1)];
-            const int ek = pw.x, ev = pw.y;
-            const float fk = power(-ek), fv = power(ev == kNoPower ? 0 : -ev);
+            const uint16_t* small = reinterpret_cast<const uint16_t*>(raw + 2 * kTileT * kRow);  // fp16 by now
 #pragma unroll 1
             for (int v = 0; v < 2; ++v) {
               const int st = ks + v;
               wait(bars->empty + st, kp ^ 1u);  // in the first phase at once
               if (!wait.dead) {
                 const uint32_t dst = smem_u32(ring) + st * kStage;
-                const float f = v ? fv : fk;
-                constexpr int NB = N < 2 ? N : 2;  // pieces whose loads are under way together
 #pragma unroll 1
-                for (int e0 = 0; e0 < N; e0 += NB) {
-                  uint4 w[NB];
-                  uint32_t s2[NB], b2[NB];
+                for (int x = ct; x < kTileT * CPR; x += 128) {
+                  const int row = x / (8 * NG) * (8 / PH) + x / PH % (8 / PH), half = x / 8 % NG, c = half * PH + x % PH;
+                  const uint4 w = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
+                  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                  const uint32_t s1 = small[v * 2 * kTileT * NG + row * NG + half] * 0x10001u;
+                  const uint32_t b1 = small[(v * 2 + 1) * kTileT * NG + row * NG + half] * 0x10001u;
+                  uint32_t s16;  // 2^-4 s, exact but for subnormals
+                  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s16) : "r"(s1), "r"(0x2C002C00u));
 #pragma unroll
-                  for (int e = 0; e < NB; ++e) {
-                    const int x = ct + 128 * (e0 + e), row = row_of(x), c = piece_of(x), at = row * NG + c / PH;
-                    w[e] = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
-                    float sc = Elt<E>::to_f32(small[v * 2 * kTileT * NG + at]) * f;
-                    float bi = Elt<E>::to_f32(small[(v * 2 + 1) * kTileT * NG + at]) * f;
-                    // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
-                    if (v && (row < lo || row >= hi || (row >= old && !(fabsf(sc) + fabsf(bi) < INFINITY)))) sc = bi = 0.0f;
-                    b2[e] = pack2<__half>(bi, bi), s2[e] = pack2<__half>(sc, BITS == 8 ? sc : sc * 0.0625f);
-                  }
-#pragma unroll
-                  for (int e = 0; e < NB; ++e) {
-                    const int x = ct + 128 * (e0 + e), row = row_of(x), c = piece_of(x);
-                    const uint32_t words[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
-#pragma unroll
-                    for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
-                      uint32_t h[4];
-                      if constexpr (BITS == 8) {
-                        uint32_t a[2], b[2];
-                        codes8(words[2 * j], p.magic, a);
-                        codes8(words[2 * j + 1], p.magic, b);
-                        h[0] = fma_f16x2(a[0], s2[e], b2[e]), h[1] = fma_f16x2(a[1], s2[e], b2[e]);
-                        h[2] = fma_f16x2(b[0], s2[e], b2[e]), h[3] = fma_f16x2(b[1], s2[e], b2[e]);
-                      } else {
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) h[y] = fma_f16x2(codes4(words[j], y, p.magic), s2[e], b2[e]);
-                      }
-                      const int ch = c * EPC / 8 + j;
-                      const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
-                      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                  for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
+                    uint32_t h[4];
+                    if constexpr (BITS == 8) {
+                      uint32_t a[2], b[2];
+                      codes8(words[2 * j], p.magic, a);
+                      codes8(words[2 * j + 1], p.magic, b);
+                      h[0] = fma_f16x2(a[0], s1, b1), h[1] = fma_f16x2(a[1], s1, b1);
+                      h[2] = fma_f16x2(b[0], s1, b1), h[3] = fma_f16x2(b[1], s1, b1);
+                    } else {  // two codes by one logic operation, 16 times as large every other time
+                      const uint32_t up = words[j] >> 8;
+                      h[0] = fma_f16x2(codes4<0x000F000Fu>(words[j], p.magic), s1, b1);
+                      h[1] = fma_f16x2(codes4<0x00F000F0u>(words[j], p.magic), s16, b1);
+                      h[2] = fma_f16x2(codes4<0x000F000Fu>(up, p.magic), s1, b1);
+                      h[3] = fma_f16x2(codes4<0x00F000F0u>(up, p.magic), s16, b1);
                     }
+                    const int ch = c * EPC / 8 + j;
+                    const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                   }
                 }
                 fence_proxy_async_shared();
@@ -577,8 +597,15 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
               for (int j = 1; j < CPR; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
               const int e = top > 0.0f && top < INFINITY ? min(max(exponent(top) - 13, -120), 120) : 0;
               const float down = power(-e);
-              v[i].x = pack2<__half>(f[0] * down, f[1] * down), v[i].y = pack2<__half>(f[2] * down, f[3] * down);
-              v[i].z = pack2<__half>(f[4] * down, f[5] * down), v[i].w = pack2<__half>(f[6] * down, f[7] * down);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] *= down;
+              if constexpr (BITS == 4) {  // in the order of the codes
+                v[i].x = pack2<__half>(f[0], f[4]), v[i].y = pack2<__half>(f[1], f[5]);
+                v[i].z = pack2<__half>(f[2], f[6]), v[i].w = pack2<__half>(f[3], f[7]);
+              } else {
+                v[i].x = pack2<__half>(f[0], f[1]), v[i].y = pack2<__half>(f[2], f[3]);
+                v[i].z = pack2<__half>(f[4], f[5]), v[i].w = pack2<__half>(f[6], f[7]);
+              }
               if (ch == 0) q_pow[SHARED ? w : 0][row] = e;
             }
             const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
@@ -708,8 +735,10 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             }
           }
         }
-        const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m, -m), sc2 = make_float2(sc, sc);
-        const float dv = BITS && ev != ref ? power(max(ev - ref, -126)) : 1.0f;  // the tile's power of V over O's
+        // Codes: the tile's power of V over O's, at most 1, is a part of the exponent. Below 2^-48 it makes zeros of fp16.
+        const bool none = BITS && ev < ref - 48;
+        const int dv = BITS && !none ? ev - ref : 0;
+        const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(dv - m, dv - m), sc2 = make_float2(sc, sc);
         float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         uint32_t two[32];
         auto weigh = [&](const uint32_t (&v)[32], int c) {
@@ -718,15 +747,19 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             float2 e = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc2, mm);
             e.x = ex2(e.x), e.y = ex2(e.y);
             sum[j & 1] = add2(sum[j & 1], e);
-            if constexpr (BITS) e.x *= dv, e.y *= dv;
             two[16 * c + j] = pack2<T>(e.x, e.y);
           }
         };
         weigh(va, 0);
         weigh(vb, 1);
+        if (none) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) two[j] = 0;
+        }
         // the buffer's last product is done, too: what signalled these scores was issued after it and waits for both
         tmem_st32(tp + h * (kTileT / 2), two);
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        l = BITS ? fmaf(more, power(-dv), l) : l + more;
         tc_wait_st();
         tc_fence_before();
         warp_arrive(&bars->p_full[w][h]);
@@ -757,7 +790,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           } else {
             const int64_t g = row * (D / 64) + c / 2;
             const float sc = Elt<E>::to_f32(static_cast<const E*>(p.v_scales)[g]), bi = Elt<E>::to_f32(static_cast<const E*>(p.v_biases)[g]);
-            if (fabsf(sc) + fabsf(bi) < INFINITY) continue;
+            if (finite(sc, bi)) continue;
             const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data + row * kRow) + c * BITS;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -779,6 +812,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           const float back = ref == kNoPower ? 1.0f : power(ref);
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
+        }
+        if constexpr (BITS == 4) {  // out of the order of the codes
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            const uint32_t a = o[j + 1], b = o[j + 2], c = o[j + 3], d = o[j + 4], e = o[j + 5], f = o[j + 6];
+            o[j + 4] = a, o[j + 1] = b, o[j + 5] = c, o[j + 2] = d, o[j + 6] = e, o[j + 3] = f;
+          }
         }
         if (odd) add_odd(c, o);
       };
