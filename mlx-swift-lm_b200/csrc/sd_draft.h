@@ -102,7 +102,11 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
 // of four warps, a warp that issues products for each and a loading warp.
-constexpr int kTreeColumns = 16;  // more columns than this, of an average sequence: the tile kernel
+// The rule for it: more columns, of an average sequence, than tree_attend_kernel has in one pass over the tokens, or in
+// two of 8-bit codes. Measured with 8 sequences of 8K tokens, 8 kv heads of 128, us, that kernel and this one: bf16, 16
+// columns 51 and 58, 20 columns 88 and 58; 4 bits, 16 columns 53 and 74, 20 columns 87 and 74; 8 bits, 32 columns 91 and
+// 95, 48 columns 128 and 97.
+constexpr int tree_tile_above(int bits) { return bits == 8 ? 32 : 16; }
 constexpr int kTreeTileThreads = 352;
 constexpr int kTreeTileTokens = 64;
 constexpr int kTreeTileUnits = 8;  // beginning and ending a segment, in tiles

@@ -71,7 +71,7 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   // Codes of fp16 pools are not for the tile kernel: its fp16 tiles of them cost as much as such an output's own rounding,
   // twice over (4e-4 of the result, relative, instead of 2e-4; nothing to speak of beside bf16's 1.7e-3).
   const auto tile_kernel = lookup_tile(g->dtype, g->kv_bits);
-  s->tiles = tile_kernel && columns > kTreeColumns;
+  s->tiles = tile_kernel && columns > tree_tile_above(g->kv_bits);
   if (s->tiles) {
     const bool shared = columns > 128;
     s->attend = tile_kernel(D, shared);

@@ -127,7 +127,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
 static __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* flags) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
 }
-constexpr uint32_t kMostTries = 1u << 22;  // 0.1 s at least
+constexpr uint32_t kMostTries = 1u << 22;  // tens of milliseconds at least
 template <bool CALL>
 struct Waiter {
   int* flags;
@@ -515,7 +515,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
               if (!wait.dead) {
                 const uint32_t dst = smem_u32(ring) + st * kStage;
 #pragma unroll 1
-                for (int x = ct; x < kTileT * CPR; x += 128) {
+                for (int e = 0; e < kTileT * CPR / 128; ++e) {
+                  const int x = ct + 128 * e;
                   const int row = x / (8 * NG) * (8 / PH) + x / PH % (8 / PH), half = x / 8 % NG, c = half * PH + x % PH;
                   const uint4 w = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
                   const uint32_t words[4] = {w.x, w.y, w.z, w.w};

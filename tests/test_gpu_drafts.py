@@ -3,9 +3,9 @@ plans and moved rows bit for bit against a host model, tree attention against
 64 bits.
 
 Tolerance of the attention: the framework's (_util.assert_close) where weights
-keep 16 bits or more. The tile kernel (16-bit pools and codes with 16-bit
-scales, more than 16 columns an average sequence) rounds a weight to the
-products' type once, by at most half a step of it: u of 16-bit pools, 2^-11 of
+keep 16 bits or more. The tile kernel (16-bit pools, and codes of bf16 ones;
+more than 16 columns an average sequence, 32 of 8-bit codes) rounds a weight to
+the products' type once, by at most half a step of it: u of 16-bit pools, 2^-11 of
 codes. With A = sum p |v| / sum p that is u A of the output, besides u |out| for
 its own rounding. Codes are fp16 values there: 2^-11 |v| more of V, another
 2^-11 A, and a score is off by d = 2^-11 B at most, B = scale sum |q k| of its
@@ -359,7 +359,7 @@ def check_tree(torch, out, ref, size, reach, dtype, tile, bits=0):
 
 
 def uses_tiles(dtype, bits, counts, G):
-    return (dtype == "bf16" or dtype == "f16" and not bits) and -(-sum(counts) // len(counts)) * G > 16
+    return (dtype == "bf16" or dtype == "f16" and not bits) and -(-sum(counts) // len(counts)) * G > (32 if bits == 8 else 16)
 
 
 def run_tree(torch, dtype, bits, d, hkv, G, page, held, counts, window=0, sinks=False, seed=0, scale=1.0, chain=False,
@@ -508,7 +508,7 @@ def test_tree_hidden_nodes_do_not_reach_their_siblings(cuda):
     """Two branches from one root: infinities and not-a-numbers in one branch's keys and values leave the other alone."""
     import sparse_decode as sd
     torch = cuda
-    for dtype, bits in (("f32", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("f32", 8)):
+    for dtype, bits in (("f32", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("f32", 8), ("bf16", 4), ("bf16", 0)):
         pool = Pool(torch, sd, dtype, bits, 2, 64, 16, 8, 3)
         tables, held = i32(torch, [[1, 4, 6, 2]]), 37
         parents = [-1, 0, 0, 1, 2, 3]
@@ -524,6 +524,34 @@ def test_tree_hidden_nodes_do_not_reach_their_siblings(cuda):
         for node in (0, 1, 3, 5):
             assert torch.equal(out[node], clean[node])
         assert not torch.isfinite(out[2]).any() and not torch.isfinite(out[4]).any()
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 4), ("bf16", 8), ("f16", 8), ("f32", 0), ("f32", 4)])
+@pytest.mark.parametrize("G", [2, 8])
+def test_tree_infinite_values_count_where_they_are_seen(cuda, dtype, bits, G):
+    """Keys are finite, one value (of codes: a group of 64) of node 2 is not: rows that see the node have it, all else is as before."""
+    import sparse_decode as sd
+    torch = cuda
+    pool = Pool(torch, sd, dtype, bits, 2, 128, 16, 8, 3)
+    tables, held, parents = i32(torch, [[1, 4, 6, 2]]), 37, [-1, 0, 0, 1, 2, 3]
+    masks = torch.tensor([m for m, _ in lineage(parents)], dtype=torch.int64, device="cuda")
+    q = torch.randn(6, 2 * G, 128, generator=gen(torch, 4), device="cuda").to(tdt(torch, dtype))
+    call = lambda: sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [43]), i32(torch, [0, 6]), masks).double()  # noqa: E731
+    clean = call()
+    at = (int(tables[0, (held + 2) // 16]), slice(None), (held + 2) % 16)
+    for x in (math.inf, -math.inf, math.nan):
+        pool.arrays[1][-1][at + (1 if bits else 100,)] = x
+        out = call()
+        hit = slice(64, 128) if bits else slice(100, 101)
+        for node in range(6):
+            if node in (2, 4):
+                assert torch.isnan(out[node, :, hit]).all() if x != x else (out[node, :, hit] == x).all()
+                out[node, :, hit] = clean[node, :, hit]
+        # the power that a tile of codes takes may be another one: fp16 values of half the bits at most, of small ones
+        tol = 2.0 ** -9 if dtype == "bf16" else 2.0 ** -12
+        assert torch.isfinite(out).all() and ((out - clean).abs() <= 4 * tol * clean.abs().amax()).all()
+        if not bits:
+            assert torch.equal(out, clean)
 
 
 def test_tree_reports_sequences_that_cannot_be(cuda):
