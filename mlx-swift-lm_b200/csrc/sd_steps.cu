@@ -6,6 +6,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <utility>
 
 #include "sd_draft.h"
 #include "sd_pages_host.h"
@@ -147,6 +149,19 @@ int32_t sd_paged_plan(const sd_plan* g, int32_t* device_flags, sd_stream stream)
   if (any_misaligned4({g->lengths, g->added, g->tables, g->held, g->free_pages, g->taken, g->parents, g->first, g->ends, g->seq,
                        g->positions, g->places, device_flags}) || misaligned(g->slots, 8) || misaligned(g->masks, 8))
     return fail(SD_ERR_INVALID_ARG, "an array is misaligned");
+  // every block reads the inputs, and some after another has written
+  const int64_t B = g->batch, N = g->n_rows;
+  const std::pair<const void*, int64_t> in[] = {
+      {g->lengths, 4 * B}, {g->added, 4 * B}, {g->tables, 4 * B * g->table_width}, {g->held, 4 * B},
+      {g->free_pages, 4 * int64_t(g->n_free)}, {g->taken, 4},
+      {g->parents, g->parents && B ? 4 * ((B - 1) * g->parents_stride + g->nodes) : 0}};
+  const std::pair<const void*, int64_t> to[] = {
+      {g->first, 4 * (B + 1)}, {g->ends, 4 * B}, {g->seq, 4 * N}, {g->positions, 4 * N}, {g->slots, 8 * N}, {g->places, 4 * N}, {g->masks, 8 * N}};
+  for (const auto& o : to)
+    for (const auto& i : in)
+      if (o.first && i.first && static_cast<const char*>(o.first) < static_cast<const char*>(i.first) + i.second &&
+          static_cast<const char*>(i.first) < static_cast<const char*>(o.first) + o.second)
+        return fail(SD_ERR_INVALID_ARG, "an output lies in one of the inputs");
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
   PlanParams p{};

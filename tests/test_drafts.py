@@ -93,6 +93,20 @@ def test_plan_refusals(native, kw, status):  # noqa: F811
     assert _status(native, native.sd_paged_plan(None, None, None)) == "SD_ERR_INVALID_ARG"
 
 
+def test_plan_refuses_outputs_in_its_inputs(native):  # noqa: F811
+    apart = dict(lengths=1 << 12, added=2 << 12, tables=3 << 12, held=4 << 12, free_pages=5 << 12, taken=6 << 12, n_free=5,
+                 parents=7 << 12, nodes=4, parents_stride=6, first=8 << 12, ends=9 << 12, seq=10 << 12, positions=11 << 12,
+                 slots=12 << 12, places=13 << 12, masks=14 << 12)
+    sizes = dict(lengths=8, added=8, tables=24, held=8, free_pages=20, taken=4, parents=40)
+    outs = dict(first=12, ends=8, seq=16, positions=16, slots=32, places=16, masks=32)
+    for name, own in outs.items():
+        for other, size in sizes.items():
+            step = 8 if own == 32 else 4
+            for at in (0, (size - 1) // step * step, -step):
+                plan = _plan(**{**apart, name: apart[other] + at})
+                assert _status(native, native.sd_paged_plan(plan, None, None)) == "SD_ERR_INVALID_ARG", (name, other, at)
+
+
 def _tree(native, pages=None, layer=0, q=256, n_rows=4, batch=2, hq=8, tables=256, width=3, lengths=256, first=256,  # noqa: F811
           masks=None, places=None, scale=1.0, window=0, sinks=None, out=512, work=768, size=1 << 40, flags=None):
     return _status(native, native.sd_paged_tree_decode(pages or _pages(), layer, q, n_rows, batch, hq, tables, width, lengths, first,
