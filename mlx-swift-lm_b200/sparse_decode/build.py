@@ -4,9 +4,9 @@ The library is compiled from mlx-swift-lm_b200/csrc: one object per storage
 format (sd_inst.cu and, for the paged cache, sd_paged_inst.cu and sd_tree_inst.cu,
 with SD_E/SD_BITS), the rotary and page-copy kernels (sd_rotary.cu), the plan
 and row kernels of drafted tokens (sd_draft.cu) and their attention's tile
-kernel (sd_tree_tile.cu), plus the C ABI (sd_api.cu,
-sd_pages.cu, sd_steps.cu). The CUDA runtime is linked statically, so the .so
-only needs the driver at run time.
+kernel (sd_tree_tile.cu), plus the C ABI (sd_api.cu, sd_pages.cu, sd_steps.cu).
+The CUDA runtime is linked statically, so the .so only needs the driver at run
+time.
 
 `build(phase_timing=True)` makes a second library, libsparse_decode_phases.so,
 compiled with -DSD_PHASE_TIMING: the decode kernel then writes per-phase

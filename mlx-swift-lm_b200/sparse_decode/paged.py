@@ -11,6 +11,8 @@ keep nothing between calls:
 * `copy_pages`    -- whole pages copied inside a pool, in every layer;
 * `paged_decode`  -- attention of one new token per sequence over its pages.
 
+drafts.py has the operators of steps that check drafted tokens.
+
 `PagePool` owns a pool and the map of sequences to pages (fork, copy-on-write,
 trim, free, compaction); `PagedBatch` is one step's view of some sequences,
 whose layers `attention_with_cache_update` takes as caches.
