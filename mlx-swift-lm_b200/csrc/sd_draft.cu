@@ -273,7 +273,9 @@ __device__ __forceinline__ void keep_rows(uint8_t* at, int row, const int* src, 
 // taken in order -- a thread does so with its own 16 bytes of a (head, row),
 // eight rows under way at a time, and no thread waits for another. One block
 // per (layer, sequence). Bound by HBM for many users, by latency (path, table,
-// rows: three loads one after the other) for few.
+// rows: three loads one after the other) for few. Measured in a graph, 36 layers of
+// 8 kv heads of 128: one user's 16 nodes in bf16 3.0 us (1.2 MB), 64 users' of 32 in
+// 8 bits 13 us (16.6 MB, 1.3 TB/s: 2304 short blocks, most of whose time is that chain).
 __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constant__ KeepParams p) {
   __shared__ int src[kMaxNodes], dst[kMaxNodes], count;
   const int tid = threadIdx.x, b = blockIdx.x % p.B, layer = blockIdx.x / p.B;

@@ -95,9 +95,9 @@ constexpr int kTreeHeads = 4;      // query heads that a warp takes to the nodes
 constexpr int kTreeAttendThreads = kPagedThreads + 32;  // a decode's, and a warp for the nodes
 constexpr int kTreeMergeCols = 8;  // columns of a merge block
 
-// Shared memory of an attend CTA: as a decode's, with two numbers per sequence and the columns' first tokens.
+// Shared memory of an attend CTA: as a decode's, with two numbers per sequence, the columns' first tokens and a count.
 constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
-  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 16) * 4, columns, D, dense_f32, stage_bytes);
+  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 17) * 4, columns, D, dense_f32, stage_bytes);
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups

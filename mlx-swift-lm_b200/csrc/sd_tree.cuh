@@ -15,10 +15,12 @@
 //     RT columns, and the pairs' tiles of held tokens are one line that CTAs share
 //     equally, as in a decode (sd_paged.cuh). Every segment leaves (o, m, l) in
 //     the workspace. No mask at all.
-//   * The nodes: a warp that a CTA has for it takes a row and up to four query
-//     heads at a time and attends to the visible nodes alone, reading no other
-//     node's rows -- what lies there, not-a-numbers included, does not reach it.
-//     It runs beside the tiles' warps, whose time hides its chain of loads.
+//   * The nodes: a warp takes a row and up to four query heads at a time and
+//     attends to the visible nodes alone, reading no other node's rows -- what lies
+//     there, not-a-numbers included, does not reach it. A CTA has a warp for it,
+//     beside the tiles' warps, whose time hides its chain of loads; the others come
+//     to its help when they are done (35 sequences of 8 tokens, 31 nodes of 8 heads
+//     in 8-bit codes of an fp16 pool: 120 -> 78 us).
 // tree_attend_kernel does both, and tree_merge_kernel joins a column's nodes and
 // segments in CTA order. The tile kernel of 16-bit pools (sd_tree_tile.cu) has
 // the nodes on the line, as a sequence's last tokens.
@@ -244,17 +246,22 @@ struct StoredPiece<E, 0, V> {
   }
 };
 
-// Rows and up to four query heads of one kv head at a time, number `first` and
-// every `step`-th after it; a warp calls. Lane l holds dimensions [l V, l V + V)
+// Rows and up to four query heads of one kv head at a time, the CTA's (each grid-th)
+// in turn as its warps come for them: `next`, in shared memory, counts. Which warp
+// has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
 // of q, o and the rows; scores are summed over the lanes by a butterfly that ends
 // with head l / 8's in lane l, so that lane l keeps token l % 8's of the eight
 // that are taken at a time.
 template <typename E, int BITS, int D>
-__device__ __forceinline__ void tree_nodes(const TreeParams& p, int first, int step) {
+__device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next) {
   constexpr int V = D / 32, HB = kTreeHeads;
   const int lane = threadIdx.x & 31;
   const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups, rows_end = min(__ldcg(p.first + p.B), p.N);
-  for (int64_t item = first; item < int64_t(rows_end) * per; item += step) {
+  for (;;) {
+    int turn = 0;
+    if (lane == 0) turn = atomicAdd(next, 1);
+    const int64_t item = blockIdx.x + int64_t(__shfl_sync(0xffffffffu, turn, 0)) * gridDim.x;
+    if (item >= int64_t(rows_end) * per) break;
     const int n = int(item / per), hg = int(item - int64_t(n) * per), h = hg / groups, g0 = (hg - h * groups) * HB;
     const int heads = min(HB, p.G - g0), b = tree_find(p, n);
     const TreeSeq s = tree_seq(p, b);
@@ -383,6 +390,11 @@ __device__ __forceinline__ void tree_nodes(const TreeParams& p, int first, int s
 // ---------------------------------------------------------------------------
 
 // The warps of a decode (sd_paged.cuh) with columns for heads, and one for the nodes.
+// One pass over the tokens has at most 16 columns, as a decode has heads: bound by
+// HBM for few of them, by the conversion of codes and the chain of products beside
+// it for 16, by latency for short ranges. Measured with the merge, 32 query and 8 kv
+// heads of 128: 16 sequences of 8K tokens, 4 nodes, 8 bits 54 us (2.6 TB/s), 8 of
+// them with 2 nodes 32 us; 2K tokens, 7 nodes, fp32, 8 and 2 heads of 64 16 us.
 template <typename E, int BITS, int D, int NB>
 __global__ void __launch_bounds__(kTreeAttendThreads, 2)
 tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
@@ -393,12 +405,13 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   float* qf = reinterpret_cast<float*>(sm + p.q_off);
   float* buf = reinterpret_cast<float*>(sm + p.buf_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
-  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kTreeAttendThreads / 32);
+  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kTreeAttendThreads / 32), *next = low + 16;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
   uint64_t* empty = full + kPagedMaxStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
+    *next = 0;
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(full + i, BITS ? 33 : 1);
       mbar_init(empty + i, kPagedWarps);
@@ -411,86 +424,84 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   griddep_launch_dependents();
   tree_line<kTreeAttendThreads>(p, F::kTile, units, pairs, tmp);
 
-  if (warp == kPagedWarps + 1) {
-    tree_nodes<E, BITS, D>(p, blockIdx.x, gridDim.x);
-    return;
-  }
   const Pieces pieces(p, units[p.B]);
-  if (int(blockIdx.x) >= pieces.n) return;
-  TreeWalk walk(p, units, pairs, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
-
-  if (warp == kPagedWarps) {
-    paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
-    return;
-  }
-  using A = typename PickAttend<E, BITS, D, NB, NodeCols>::type;
-  const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
-  A att;
-  TreeSegment s;
-  int it = 0, st = 0;
-  uint32_t round = 0;
-  bool dead = false;
-  while (walk.next(s)) {
-    const TreeSeq sq = tree_seq(p, s.b);
-    const NodeCols cols(p, sq, s.h, s.c);
-    const int t0 = sq.begin / F::kTile;
-    int edge = 0;  // tokens below it are not seen by every column
-    if (p.window) {
-      if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
-      named_barrier(1, 32 * kPagedWarps);
-      edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
-    }
-    att.begin(p, qf, cols, warp, lane);
-    for (int i = s.i0; i < s.i1; ++i, ++it) {
-      const int tok = (t0 + i) * F::kTile;
-      if (!dead) dead = !mbar_wait(full + st, round, p.flags);
-      if (!dead) {
-        att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, sq.begin - tok, sq.held - tok, tok < edge ? low : nullptr, tok},
-                 warp, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + st);
-      }
-      if (++st == p.stages) {
-        st = 0;
-        round ^= 1u;
-      }
-    }
-    att.end(cols.n, WarpPart<D>(buf, p.RT, warp), lane);
-    named_barrier(1, 32 * kPagedWarps);
-    // the four warps' parts, in warp order
-    float* part = tree_part(p, s.pair + blockIdx.x);
-    for (int k = tid; k < p.RT * (D / 4); k += 32 * kPagedWarps) {
-      const int d4 = k / p.RT, g = k - d4 * p.RT;
-      if (g >= cols.n) continue;
-      float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
+  if (warp <= kPagedWarps && int(blockIdx.x) < pieces.n) {
+    TreeWalk walk(p, units, pairs, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
+    if (warp == kPagedWarps) {
+      paged_produce<E, BITS, D>(p, &tmK, &tmV, sm, full, empty, walk, lane);
+    } else {
+      using A = typename PickAttend<E, BITS, D, NB, NodeCols>::type;
+      const int pb_log = __ffs(min(p.P, F::kTile)) - 1;
+      A att;
+      TreeSegment s;
+      int it = 0, st = 0;
+      uint32_t round = 0;
+      bool dead = false;
+      while (walk.next(s)) {
+        const TreeSeq sq = tree_seq(p, s.b);
+        const NodeCols cols(p, sq, s.h, s.c);
+        const int t0 = sq.begin / F::kTile;
+        int edge = 0;  // tokens below it are not seen by every column
+        if (p.window) {
+          if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
+          named_barrier(1, 32 * kPagedWarps);
+          edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
+        }
+        att.begin(p, qf, cols, warp, lane);
+        for (int i = s.i0; i < s.i1; ++i, ++it) {
+          const int tok = (t0 + i) * F::kTile;
+          if (!dead) dead = !mbar_wait(full + st, round, p.flags);
+          if (!dead) {
+            att.tile(p, qf, TileView{sm + st * F::kStageBytes, pb_log, sq.begin - tok, sq.held - tok, tok < edge ? low : nullptr, tok},
+                     warp, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + st);
+          }
+          if (++st == p.stages) {
+            st = 0;
+            round ^= 1u;
+          }
+        }
+        att.end(cols.n, WarpPart<D>(buf, p.RT, warp), lane);
+        named_barrier(1, 32 * kPagedWarps);
+        // the four warps' parts, in warp order
+        float* part = tree_part(p, s.pair + blockIdx.x);
+        for (int k = tid; k < p.RT * (D / 4); k += 32 * kPagedWarps) {
+          const int d4 = k / p.RT, g = k - d4 * p.RT;
+          if (g >= cols.n) continue;
+          float mw[kPagedWarps], M = -INFINITY, L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        mw[w] = WarpPart<D>(buf, p.RT, w).ml[2 * g];
-        M = fmaxf(M, mw[w]);
-      }
-      float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int w = 0; w < kPagedWarps; ++w) {
+            mw[w] = WarpPart<D>(buf, p.RT, w).ml[2 * g];
+            M = fmaxf(M, mw[w]);
+          }
+          float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const WarpPart<D> wp(buf, p.RT, w);
-        const float f = exp2_from(mw[w], M);
-        const float4 x = *reinterpret_cast<const float4*>(wp.o + g * (D + 4) + 4 * d4);
-        L = fmaf(f, wp.ml[2 * g + 1], L);
-        O.x = fmaf(f, x.x, O.x);
-        O.y = fmaf(f, x.y, O.y);
-        O.z = fmaf(f, x.z, O.z);
-        O.w = fmaf(f, x.w, O.w);
+          for (int w = 0; w < kPagedWarps; ++w) {
+            const WarpPart<D> wp(buf, p.RT, w);
+            const float f = exp2_from(mw[w], M);
+            const float4 x = *reinterpret_cast<const float4*>(wp.o + g * (D + 4) + 4 * d4);
+            L = fmaf(f, wp.ml[2 * g + 1], L);
+            O.x = fmaf(f, x.x, O.x);
+            O.y = fmaf(f, x.y, O.y);
+            O.z = fmaf(f, x.z, O.z);
+            O.w = fmaf(f, x.w, O.w);
+          }
+          reinterpret_cast<float4*>(part)[k] = O;
+          if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
+        }
+        named_barrier(1, 32 * kPagedWarps);
       }
-      reinterpret_cast<float4*>(part)[k] = O;
-      if (d4 == 0) *reinterpret_cast<float2*>(part + p.RT * D + 2 * g) = make_float2(M, L);
+      if (dead) drain(full, it, p.stages);
     }
-    named_barrier(1, 32 * kPagedWarps);
   }
-  if (dead) drain(full, it, p.stages);
+  tree_nodes<E, BITS, D>(p, next);
 }
 
 // Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per
 // block: a thread has one column and four dimensions, and eight segments' loads
-// under way. Bound by latency: the line, the segments' places, their loads.
+// under way. Bound by latency: the line, the segments' places, their loads. Alone
+// and with cold caches it takes 10 us for 1024 columns of 128 and 18 us for 8192.
 template <typename E, int D>
 __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(const __grid_constant__ TreeParams p) {
   constexpr int NC = kTreeMergeCols;
