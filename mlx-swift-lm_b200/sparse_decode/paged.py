@@ -454,7 +454,8 @@ class PagePool:
                  dtype: str = "bf16", kv_bits: int = 0):
         if torch is None:
             _load()
-        self._forks: dict = {}  # how often each sequence was forked
+        self._changes: dict = {}  # how often each sequence was forked, trimmed or extended
+        self._moves = 0  # compactions
         if kv_bits not in (0, 4, 8):
             raise ValueError("kv_bits must be 0, 4 or 8")
         lead = (n_layers, n_pages, n_kv_heads, page_size)
@@ -486,22 +487,32 @@ class PagePool:
     def add(self) -> int:
         s = ctypes.c_int64()
         _check(lib().sd_pagemap_add(self._h, ctypes.byref(s)))
+        self._changes[s.value] = 0
         return s.value
 
     def fork(self, seq: int) -> int:
         s = ctypes.c_int64()
         _check(lib().sd_pagemap_fork(self._h, seq, ctypes.byref(s)))
-        self._forks[seq] = self._forks.get(seq, 0) + 1
+        self._changes[s.value] = 0
+        self._changed(seq)
         return s.value
 
     def free(self, seq: int) -> None:
         _check(lib().sd_pagemap_free(self._h, seq))
-        self._forks.pop(seq, None)
+        self._changes.pop(seq, None)
 
     def trim(self, seq: int, n: int) -> int:
         t = ctypes.c_int64()
         _check(lib().sd_pagemap_trim(self._h, seq, n, ctypes.byref(t)))
+        self._changed(seq)
         return t.value
+
+    def _changed(self, seq: int) -> None:
+        self._changes[seq] += 1
+
+    def _state(self, seqs) -> list:
+        """What tells whether sequences are as they were, pages included."""
+        return [self._moves, *(self._changes.get(s) for s in seqs)]
 
     def length(self, seq: int) -> int:
         t = ctypes.c_int64()
@@ -523,6 +534,7 @@ class PagePool:
         src, dst = (ctypes.c_int32 * max(room, 1))(), (ctypes.c_int32 * max(room, 1))()
         _check(lib().sd_pagemap_compact(self._h, src, dst, room, ctypes.byref(n)))
         if n.value:
+            self._moves += 1
             copy_pages(self.pages, src[:n.value], dst[:n.value], flags=self.flags, stream=stream)
         return n.value
 
@@ -547,6 +559,7 @@ class PagePool:
             for s, k in zip(seqs, each):
                 _check(lib().sd_pagemap_extend(self._h, s, k, ctypes.byref(src), ctypes.byref(dst), ctypes.byref(n)))
                 grown.append((s, k))
+                self._changed(s)
                 if n.value:
                     copies.append((src.value, dst.value))
             batch = PagedBatch(self, list(seqs), each, stream)
@@ -618,7 +631,7 @@ class PagedBatch:
         else:
             self.positions, self.seq = rest[:tokens], rest[tokens:]
         self.host_lengths = lengths
-        self._forks = [pool._forks.get(s, 0) for s in seqs]
+        self._state = pool._state(seqs)
 
     def tree(self, parents=None, stream=None) -> "PagedBatch":
         """Make drafted tokens of the step's new ones: node i of a sequence has
@@ -630,6 +643,7 @@ class PagedBatch:
         Returns the batch."""
         from .drafts import MAX_NODES, paged_plan
         n, new = len(self.seqs), self.new
+        self._refuse_stale()
         if max(new, default=0) > MAX_NODES:
             raise ValueError(f"a tree has at most {MAX_NODES} nodes (got {max(new)})")
         if parents is None:
@@ -654,6 +668,10 @@ class PagedBatch:
         self.positions, self.seq = self.plan.positions, self.plan.seq
         return self
 
+    def _refuse_stale(self) -> None:
+        if self._state != self.pool._state(self.seqs):
+            raise ValueError("a sequence of the step was forked, trimmed, extended or moved since")
+
     def attend_tree(self, layer: int, q, scale: Optional[float] = None, **kw):
         """`paged_tree_decode` of the step's new tokens [tokens, Hq, D]."""
         from .drafts import paged_tree_decode
@@ -668,7 +686,8 @@ class PagedBatch:
         and become its next tokens, in every layer, the others are dropped. The
         step's calls must be on `stream` or waited for by it; the batch is
         stale afterwards. Refused when a sequence has changed since the step
-        was made: a fork of it shares the pages that would be written."""
+        was made (a fork of it shares the pages that would be written) or the
+        pool was compacted."""
         from .drafts import paged_keep
         pool, p, n = self.pool, self.plan, len(self.seqs)
         if p is None:
@@ -679,9 +698,7 @@ class PagedBatch:
         for x, k in zip(paths, self.new):
             if any(not 0 <= i < k for i in x) or any(a >= b for a, b in zip(x, x[1:])):
                 raise ValueError("a path names nodes in rising order")
-        if [pool._forks.get(s, 0) for s in self.seqs] != self._forks or \
-                [pool.length(s) for s in self.seqs] != self.host_lengths:
-            raise ValueError("a sequence of the step was forked, trimmed or extended since")
+        self._refuse_stale()
         wide = max(1, max(map(len, paths), default=0))
         host = [i for x in paths for i in [*x, *[-1] * (wide - len(x))]] + [len(x) for x in paths]
         dev = _upload(torch.tensor(host, dtype=torch.int32).pin_memory(), stream)

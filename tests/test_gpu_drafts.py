@@ -760,6 +760,35 @@ def test_pool_refuses_what_a_tree_cannot_be(cuda):
     assert pool.length(b) == 2 and pool.check_device() == 0
 
 
+def test_pool_refuses_stale_steps(cuda):
+    """Pages that a step's tables name may belong to others once its sequences were trimmed, freed or moved."""
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 20, 2, 64, 16)
+    a, b = pool.add(), pool.add()
+    step = pool.extend([a], 20).tree()
+    pool.trim(a, 20)
+    pool.extend([b], 5)
+    pool.extend([a], 20)  # the length that it had
+    with pytest.raises(ValueError, match="since"):
+        step.keep([[0]])
+    step = pool.extend([a], 3).tree()
+    pool.free(b)
+    assert pool.compact()
+    with pytest.raises(ValueError, match="since"):
+        step.keep([[0]])
+    with pytest.raises(ValueError, match="since"):
+        step.tree()
+    step = pool.extend([a], 3).tree()
+    step.keep([[0, 1]])
+    with pytest.raises(ValueError, match="since"):
+        step.tree()
+    step = pool.extend([a], 3).tree()
+    pool.free(a)
+    with pytest.raises(ValueError, match="since"):
+        step.keep([[0]])
+    assert pool.free_pages == 20 and pool.check_device() == 0
+
+
 def test_a_plan_on_the_device_gives_the_positions_of_the_host(cuda):
     import sparse_decode as sd
     from sparse_decode import paged
