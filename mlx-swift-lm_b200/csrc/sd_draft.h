@@ -76,8 +76,8 @@ struct TreeParams : PagedParams {
 };
 
 struct TreeSet {
-  const void* attend;  // tree_attend_kernel<E, BITS, D, blocks of columns>(TreeParams, CUtensorMap, CUtensorMap)
-  const void* merge;   // tree_merge_kernel<E, D>(TreeParams)
+  const void* attend[2];  // tree_attend_kernel<E, BITS, D, blocks of columns, help>(TreeParams, CUtensorMap, CUtensorMap)
+  const void* merge;      // tree_merge_kernel<E, D>(TreeParams)
   int tile, stage_bytes, columns;
 };
 // For at most `columns` columns a pair, or as many as there are.
@@ -95,9 +95,9 @@ constexpr int kTreeHeads = 4;      // query heads that a warp takes to the nodes
 constexpr int kTreeAttendThreads = kPagedThreads + 32;  // a decode's, and a warp for the nodes
 constexpr int kTreeMergeCols = 8;  // columns of a merge block
 
-// Shared memory of an attend CTA: as a decode's, with two numbers per sequence, the columns' first tokens and a count.
+// Shared memory of an attend CTA: as a decode's, with two numbers per sequence, the columns' first tokens and two counts.
 constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
-  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 17) * 4, columns, D, dense_f32, stage_bytes);
+  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 18) * 4, columns, D, dense_f32, stage_bytes);
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups

@@ -68,7 +68,7 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   int sms = 0;
   if (int32_t rc = sm_count(&sms)) return rc;
   const TreeSet set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
-  if (!set.attend) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
+  if (!set.merge) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   s->merge = set.merge;
   // Codes of fp16 pools are not for the tile kernel: its fp16 tiles of them cost as much as such an output's own rounding,
   // twice over (4e-4 of the result, relative, instead of 2e-4; nothing to speak of beside bf16's 1.7e-3).
@@ -86,7 +86,8 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->ctas = sms;
     s->seg_units = kTreeTileUnits;
   } else {
-    s->attend = set.attend;
+    s->ctas = 2 * sms;
+    s->attend = set.attend[int64_t(n_rows) * g->n_kv_heads * ((G + kTreeHeads - 1) / kTreeHeads) > s->ctas];
     s->threads = kTreeAttendThreads;
     s->smem_most = kPagedSmem;
     const PagedLayout lay = tree_layout(batch, set.columns, D, g->dtype == SD_F32 && !g->kv_bits, set.stage_bytes);
@@ -95,7 +96,6 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
     s->buf_off = lay.buf_off;
     s->tile = set.tile;
     s->columns = set.columns;
-    s->ctas = 2 * sms;
     s->seg_units = kSegmentUnits;
   }
   if (s->lay.stages < (s->tiles ? kTreeTileLeast : 1) || (s->tiles && g->kv_bits && s->lay.raw_stages < 2))

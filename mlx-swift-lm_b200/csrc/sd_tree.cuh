@@ -20,7 +20,7 @@
 //     there, not-a-numbers included, does not reach it. A CTA has a warp for it,
 //     beside the tiles' warps, whose time hides its chain of loads; the others come
 //     to its help when they are done (35 sequences of 8 tokens, 31 nodes of 8 heads
-//     in 8-bit codes of an fp16 pool: 120 -> 78 us).
+//     in 8-bit codes of an fp16 pool: 120 -> 75 us).
 // tree_attend_kernel does both, and tree_merge_kernel joins a column's nodes and
 // segments in CTA order. The tile kernel of 16-bit pools (sd_tree_tile.cu) has
 // the nodes on the line, as a sequence's last tokens.
@@ -247,8 +247,8 @@ struct StoredPiece<E, 0, V> {
 };
 
 // Rows and up to four query heads of one kv head at a time, the CTA's (each grid-th)
-// in turn as its warps come for them: `next`, in shared memory, counts. Which warp
-// has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
+// in turn as its warps come for them: `next`, in shared memory, counts, and has the
+// number of rows behind it. Which warp has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
 // of q, o and the rows; scores are summed over the lanes by a butterfly that ends
 // with head l / 8's in lane l, so that lane l keeps token l % 8's of the eight
 // that are taken at a time.
@@ -256,7 +256,7 @@ template <typename E, int BITS, int D>
 __device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next) {
   constexpr int V = D / 32, HB = kTreeHeads;
   const int lane = threadIdx.x & 31;
-  const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups, rows_end = min(__ldcg(p.first + p.B), p.N);
+  const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups, rows_end = next[1];
   for (;;) {
     int turn = 0;
     if (lane == 0) turn = atomicAdd(next, 1);
@@ -395,7 +395,9 @@ __device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next) {
 // it for 16, by latency for short ranges. Measured with the merge, 32 query and 8 kv
 // heads of 128: 16 sequences of 8K tokens, 4 nodes, 8 bits 54 us (2.6 TB/s), 8 of
 // them with 2 nodes 32 us; 2K tokens, 7 nodes, fp32, 8 and 2 heads of 64 16 us.
-template <typename E, int BITS, int D, int NB>
+// HELP: the warps come to the nodes' help when they are done. Where a CTA has no second row that only costs (the code
+// is larger: 2K tokens and 7 nodes in fp32 take 17.7 us instead of 16.3).
+template <typename E, int BITS, int D, int NB, bool HELP>
 __global__ void __launch_bounds__(kTreeAttendThreads, 2)
 tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV) {
@@ -422,8 +424,13 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   }
   griddep_wait();
   griddep_launch_dependents();
-  tree_line<kTreeAttendThreads>(p, F::kTile, units, pairs, tmp);
+  if (tid == 32) next[1] = min(__ldcg(p.first + p.B), p.N);
+  tree_line<kTreeAttendThreads>(p, F::kTile, units, pairs, tmp);  // with barriers
 
+  if (!HELP && warp == kPagedWarps + 1) {
+    tree_nodes<E, BITS, D>(p, next);
+    return;
+  }
   const Pieces pieces(p, units[p.B]);
   if (warp <= kPagedWarps && int(blockIdx.x) < pieces.n) {
     TreeWalk walk(p, units, pairs, pieces.begin(blockIdx.x), pieces.begin(blockIdx.x + 1));
@@ -495,7 +502,7 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
       if (dead) drain(full, it, p.stages);
     }
   }
-  tree_nodes<E, BITS, D>(p, next);
+  if constexpr (HELP) tree_nodes<E, BITS, D>(p, next);
 }
 
 // Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per

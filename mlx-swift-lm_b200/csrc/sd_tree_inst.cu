@@ -23,7 +23,8 @@ template <int D, int NB>
 static TreeSet make_tree() {
   using F = PagedFmt<sizeof(ET), SD_BITS, D>;
   TreeSet s;
-  s.attend = reinterpret_cast<const void*>(&tree_attend_kernel<ET, SD_BITS, D, NB>);
+  s.attend[0] = reinterpret_cast<const void*>(&tree_attend_kernel<ET, SD_BITS, D, NB, false>);
+  s.attend[1] = reinterpret_cast<const void*>(&tree_attend_kernel<ET, SD_BITS, D, NB, true>);
   s.merge = reinterpret_cast<const void*>(&tree_merge_kernel<ET, D>);
   s.tile = F::kTile;
   s.stage_bytes = F::kStageBytes;
