@@ -428,7 +428,7 @@ def test_tree_of_a_chain_and_without_masks(cuda, dtype, bits):
     run_tree(cuda, dtype, bits, 128, 2, 4, 64, [500, 0, 63], [9, 64, 20], causal=True, seed=4)
 
 
-@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 4)])
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 0), ("f16", 0), ("bf16", 8), ("f16", 4), ("bf16", 4)])
 @pytest.mark.parametrize("window", [1, 2, 16, 64, 65, 200])
 def test_tree_windows_and_sinks(cuda, dtype, bits, window):
     run_tree(cuda, dtype, bits, 64, 2, 4, 16, [400, 3, 150, 64, 0], [20, 12, 1, 64, 30], window=window,
@@ -441,18 +441,18 @@ def test_tree_absent_nodes_and_rows_behind_the_last(cuda, dtype, bits):
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("dtype,bits,d", [("bf16", 0, 128), ("f16", 0, 64), ("bf16", 8, 128), ("f32", 0, 64), ("f16", 4, 64)])
+@pytest.mark.parametrize("dtype,bits,d", [("bf16", 0, 128), ("f16", 0, 64), ("bf16", 8, 128), ("f32", 0, 64), ("f16", 4, 64), ("bf16", 4, 128)])
 def test_tree_page_sizes(cuda, page, dtype, bits, d):
     run_tree(cuda, dtype, bits, d, 2, 4, page, [page, 3 * page - 1, 700, 1], [16, 5, 33, 9], seed=page)
 
 
-@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 8), ("f32", 0)])
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 8), ("f32", 0), ("bf16", 4)])
 def test_tree_long_split_over_all_ctas(cuda, dtype, bits):
     run_tree(cuda, dtype, bits, 128, 2, 4, 64, [20000, 37], [33, 60], seed=1)
     run_tree(cuda, dtype, bits, 128, 1, 8, 64, [9000], [12], seed=2)
 
 
-@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 4), ("f32", 0)])
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 4), ("f32", 0), ("bf16", 4)])
 def test_tree_many_short_sequences(cuda, dtype, bits):
     rng = random.Random(5)
     run_tree(cuda, dtype, bits, 64, 2, 2, 16, [rng.randint(0, 90) for _ in range(300)], [rng.randint(0, 12) for _ in range(300)], seed=6)
