@@ -414,8 +414,10 @@ typedef struct {
 
 /* What does not fit -- the tables, the free pages, the tree, n_rows -- is cut
  * from the new tokens (first and ends say what is left) and sets bit 2 of
- * *device_flags (nullable); so do negative numbers, which count as 0, and a
- * parent that does not come before its node, which counts as absent. */
+ * *device_flags (nullable); so do negative numbers, which count as 0, a length
+ * past the sequence's table, which gets neither tokens nor pages (its end stays
+ * its length), and a parent that does not come before its node, which counts as
+ * absent. */
 int32_t sd_paged_plan(const sd_plan* plan, int32_t* device_flags, sd_stream stream);
 
 /* Attention of the new tokens of a step: q, out [n_rows, n_q_heads, D];

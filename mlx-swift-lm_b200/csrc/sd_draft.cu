@@ -53,7 +53,8 @@ __device__ __forceinline__ void store4(T* at, int64_t row, int n, const T (&v)[k
 // node i's mask has its own bit and those of its parent's mask, its place is
 // one past its parent's (the sequence's length for a root). What does not fit
 // (the table, the free pages, the tree, the rows) is cut, with an error bit,
-// so that what is planned can always be done.
+// so that what is planned can always be done; a sequence with more tokens than its
+// table holds gets nothing, so no page is written behind a table's row.
 //
 // Bound by latency up to some ten thousand rows (a launch, the lengths, the
 // table), then by its stores: 16 bytes a row, 28 with a tree. Every CTA works out all sequences'
@@ -84,14 +85,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   for (int b = b0; b < b1; ++b) {
     const int raw = __ldcg(p.lengths + b), add = __ldcg(p.added + b);
     const int l = max(raw, 0), c = p.held ? __ldcg(p.held + b) : p.W, h = max(0, min(c, p.W));
+    const bool past = l > int64_t(p.W) * p.P;  // more tokens than the table holds: neither tokens nor pages
     int n = int(max(int64_t(0), min(int64_t(max(add, 0)), min(int64_t(p.W) * p.P - l, int64_t(p.N)))));
     if (p.parents) n = min(n, p.T);
-    bad = bad || raw < 0 || n != add || h != c;
+    bad = bad || raw < 0 || n != add || h != c || past;
     len[b] = l;
     have[b] = h;
     first[b + 1] = n;
     base[b] = max(0, int((int64_t(l) + n + p.P - 1) >> p.page_shift) - h);
-    if (!p.held) base[b] = 0;
+    if (!p.held || past) base[b] = 0;
     need += base[b];
   }
   int64_t all, run = block_before(need, sums, &all);

@@ -1,0 +1,52 @@
+"""Calls of the operators around drafted tokens that their documentation allows
+and that read or wrote, once, what they should not have."""
+from __future__ import annotations
+
+import pytest
+
+from test_gpu_drafts import i32
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("take", [False, True])
+@pytest.mark.parametrize("B,at", [(2, 0), (2, 1), (5, 2), (700, 300), (4096, 4095)])
+@pytest.mark.parametrize("length,added", [(100, 0), (100, 3), (65, 0), (64, 1), ((1 << 31) - 1, 64)])
+def test_plan_of_a_length_past_its_table(cuda, B, at, length, added, take, tree):
+    """Sequence `at` has more tokens than its table's 4 pages of 16 hold (64, one more: the new one does not fit): it gets
+    neither tokens nor pages, the others theirs, and nothing is written behind its row or behind the tables."""
+    import sparse_decode as sd
+    torch = cuda
+    W, page = 4, 16
+    lengths, new, held = [3] * B, [14] * B, [1] * B  # a second page each
+    lengths[at], new[at], held[at] = length, added, 4
+    room = torch.full((B * W + 64,), -7, dtype=torch.int32, device="cuda")
+    tables = room[:B * W].view(B, W)
+    tables.copy_(torch.arange(B * W, device="cuda").view(B, W))
+    want = tables.clone()
+    free = torch.arange(5 * B, 9 * B, dtype=torch.int32, device="cuda")
+    h, taken, flags = i32(torch, held), i32(torch, [0]), i32(torch, [0])
+    grow = dict(held=h, free=free, taken=taken) if take else {}
+    others = [b for b in range(B) if b != at]
+    if take:
+        want[others, 1] = free[:B - 1]
+    up = i32(torch, list(range(-1, 63))) if tree else None
+    p = sd.paged_plan(i32(torch, lengths), i32(torch, new), tables, page, 14 * B + 9, parents=up, flags=flags, **grow)
+    assert int(flags) == 2
+    assert torch.equal(tables, want) and (room[B * W:] == -7).all()
+    if take:
+        assert h.tolist() == [4 if b == at else 2 for b in range(B)] and taken.tolist() == [B - 1]
+    first = [0]
+    for b in range(B):
+        first.append(first[-1] + (0 if b == at else 14))
+    assert p.first.tolist() == first
+    assert p.ends.tolist() == [length if b == at else 17 for b in range(B)]
+    assert p.seq.tolist() == [b for b in others for _ in range(14)] + [-1] * 23
+    assert p.positions.tolist() == [t for _ in others for t in range(3, 17)] + [-1] * 23
+    slot = want[others][:, :2].long().repeat_interleave(16, 1)[:, 3:17] * page + torch.arange(3, 17, device="cuda") % page
+    assert torch.equal(p.slots[:14 * (B - 1)], slot.flatten())
