@@ -432,7 +432,8 @@ int32_t sd_paged_plan(const sd_plan* plan, int32_t* device_flags, sd_stream stre
  * per kv head, batch <= 4096. A sequence whose numbers cannot be (rows outside
  * n_rows, more nodes, fewer tokens than nodes, more than the table holds) gives
  * zeros and sets bit 2 of *device_flags, and so does a page out of range,
- * whose tokens read as 0. Equal calls give equal bits. The workspace
+ * whose tokens read as 0. first has to rise from 0 to batch: where it falls, all
+ * rows before first[batch] give zeros. Equal calls give equal bits. The workspace
  * (sd_paged_tree_workspace bytes, 16-byte aligned, contents do not matter)
  * must not be shared by calls that may overlap. q, out: 16-byte aligned. */
 int32_t sd_paged_tree_workspace(const sd_pages* pages, int32_t batch, int32_t n_rows, int32_t n_q_heads, int64_t* bytes);

@@ -34,16 +34,19 @@
 namespace sd {
 
 // What one sequence has of a call. A sequence whose numbers cannot be is taken
-// for one without tokens, and its rows give zeros.
+// for one without tokens, and its rows give zeros. Where first falls anywhere,
+// sequences may have rows in common, more in sum than the workspace has room for:
+// then none has any (tree_line), and all rows give zeros.
 struct TreeSeq {
   int row0, n, held;  // first row, nodes, tokens before them
   int begin, end;     // the tokens on the line: from the first that any node sees, and up to the nodes or with them
-  bool bad;
+  bool bad, falls;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
   const int f0 = __ldcg(p.first + b), f1 = __ldcg(p.first + b + 1), len = __ldcg(p.lengths + b);
   const int64_t n = int64_t(f1) - f0;
   TreeSeq s;
+  s.falls = n < 0;
   s.bad = f0 < 0 || f1 > p.N || n < 0 || n > kMaxNodes || len < n || len > int64_t(p.W) * p.P;
   s.row0 = f0;
   s.n = s.bad ? 0 : int(n);
@@ -94,15 +97,17 @@ __device__ __forceinline__ uint64_t tree_seen(const TreeParams& p, const TreeSeq
   return m;
 }
 
-// Units and pairs before each sequence, by all NT threads of the block; tmp: [2 * NT / 32].
+// Units and pairs before each sequence, by all NT threads of the block; tmp: [2 * NT / 32]. No pairs at all: no row has
+// anything to see.
 template <int NT>
 __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* units, int* pairs, int* tmp) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (p.B + NT - 1) / NT, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   int u = 0, k = 0;
-  bool bad = false;
+  bool bad = false, falls = false;
   for (int b = b0; b < b1; ++b) {
     const TreeSeq s = tree_seq(p, b);
+    falls = falls || s.falls;
     const int np = tree_pairs(p, s), nu = tree_units(p, s, tile);
     bad = bad || s.bad;
     units[b + 1] = np * nu;  // of the sequence, for now
@@ -118,12 +123,13 @@ __device__ __forceinline__ void tree_line(const TreeParams& p, int tile, int* un
     if (lane >= x) iu += yu, ik += yk;
   }
   if (lane == 31) tmp[2 * warp] = iu, tmp[2 * warp + 1] = ik;
-  __syncthreads();
+  const bool none = __syncthreads_or(falls);
   u = iu - u, k = ik - k;
   for (int w = 0; w < warp; ++w) u += tmp[2 * w], k += tmp[2 * w + 1];
+  if (none) u = k = 0;
   if (tid == 0) units[0] = pairs[0] = 0;
   for (int b = b0; b < b1; ++b) {
-    u += units[b + 1], k += pairs[b + 1];
+    if (!none) u += units[b + 1], k += pairs[b + 1];
     units[b + 1] = u, pairs[b + 1] = k;
     if (blockIdx.x == 0) p.line[b + 1] = u, p.line[p.B + 2 + b] = k;  // for the merge
   }
@@ -248,12 +254,12 @@ struct StoredPiece<E, 0, V> {
 
 // Rows and up to four query heads of one kv head at a time, the CTA's (each grid-th)
 // in turn as its warps come for them: `next`, in shared memory, counts, and has the
-// number of rows behind it. Which warp has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
+// number of rows behind it. `any`: whether the call has sequences that can be. Which warp has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
 // of q, o and the rows; scores are summed over the lanes by a butterfly that ends
 // with head l / 8's in lane l, so that lane l keeps token l % 8's of the eight
 // that are taken at a time.
 template <typename E, int BITS, int D>
-__device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next) {
+__device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next, bool any) {
   constexpr int V = D / 32, HB = kTreeHeads;
   const int lane = threadIdx.x & 31;
   const int groups = (p.G + HB - 1) / HB, per = p.Hkv * groups, rows_end = next[1];
@@ -266,7 +272,7 @@ __device__ __forceinline__ void tree_nodes(const TreeParams& p, int* next) {
     const int heads = min(HB, p.G - g0), b = tree_find(p, n);
     const TreeSeq s = tree_seq(p, b);
     const int node = n - s.row0;
-    const bool mine = !s.bad && node >= 0 && node < s.n;
+    const bool mine = any && !s.bad && node >= 0 && node < s.n;
     const int64_t col0 = int64_t(n) * p.Hq + int64_t(h) * p.G + g0;  // of q, out and the nodes' parts
     float q[HB][V], o[HB][V], m[HB], l[HB];
 #pragma unroll
@@ -428,7 +434,7 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   tree_line<kTreeAttendThreads>(p, F::kTile, units, pairs, tmp);  // with barriers
 
   if (!HELP && warp == kPagedWarps + 1) {
-    tree_nodes<E, BITS, D>(p, next);
+    tree_nodes<E, BITS, D>(p, next, pairs[p.B] > 0);
     return;
   }
   const Pieces pieces(p, units[p.B]);
@@ -502,7 +508,7 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
       if (dead) drain(full, it, p.stages);
     }
   }
-  if constexpr (HELP) tree_nodes<E, BITS, D>(p, next);
+  if constexpr (HELP) tree_nodes<E, BITS, D>(p, next, pairs[p.B] > 0);
 }
 
 // Of one kv head, kTreeMergeCols neighbouring columns (row, query head) per
@@ -533,9 +539,12 @@ __global__ void __launch_bounds__(kTreeMergeCols * D / 4) tree_merge_kernel(cons
     O = __ldcg(reinterpret_cast<const float4*>(p.node_o + row * D) + d4);
   }
   const int i = n - s.row0;
+  int up = 0, u1 = 0, all = 0, pp = 0, np = 0;
   if (i >= 0 && i < s.n && s.end > s.begin) {
-    const int up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
-    const int pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
+    up = __ldcg(p.line + b), u1 = __ldcg(p.line + b + 1), all = __ldcg(p.line + p.B);
+    pp = __ldcg(p.line + p.B + 1 + b), np = __ldcg(p.line + p.B + 2 + b) - pp;
+  }
+  if (np > 0) {
     const int nu = (u1 - up) / np, y = i * p.G + g, c = y / p.RT, k = h * (np / p.Hkv) + c, at = y - c * p.RT;
     const Pieces pieces(p, all);
     const int a = up + k * nu, cta = pieces.of(a + p.seg_units), ns = pieces.of(a + nu - 1) - cta + 1;

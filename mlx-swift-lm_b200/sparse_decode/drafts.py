@@ -116,7 +116,8 @@ def paged_tree_decode(q, pages: KVPages, tables, lengths, first, masks=None, sca
     16-byte boundary), rows first[b] .. first[b + 1] of sequence b, whose
     lengths[b] tokens count them and are all stored. A row sees the tokens
     before the step and those of its sequence's new ones that its mask names
-    (None: the ones up to itself); with a window, of these the ones whose place
+    (None: the ones up to itself; `first` must not fall: then all rows give
+    zeros, with bit 2 of flags); with a window, of these the ones whose place
     is above its own less `window`. Rows from first[batch] on are left as they
     are; a row that sees nothing gives zeros.
 

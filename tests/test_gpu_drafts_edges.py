@@ -2,9 +2,12 @@
 and that read or wrote, once, what they should not have."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 from test_gpu_drafts import i32
+from test_gpu_paged import Pool, gen, tables_of, tdt
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +53,44 @@ def test_plan_of_a_length_past_its_table(cuda, B, at, length, added, take, tree)
     assert p.positions.tolist() == [t for _ in others for t in range(3, 17)] + [-1] * 23
     slot = want[others][:, :2].long().repeat_interleave(16, 1)[:, 3:17] * page + torch.arange(3, 17, device="cuda") % page
     assert torch.equal(p.slots[:14 * (B - 1)], slot.flatten())
+
+
+# ---------------------------------------------------------------------------
+# tree attention: rows that cannot be
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,bits,hkv,G,first", [
+    ("bf16", 0, 8, 4, [0, 60] * 3),                      # few columns on average: the 16-column kernel
+    ("f32", 0, 8, 4, [0, 60] * 3), ("f16", 4, 8, 4, [0, 60] * 3), ("bf16", 8, 2, 16, [0, 64] * 32 + [0]),
+    ("bf16", 0, 8, 16, [0, 60, 0, 60]), ("f16", 0, 2, 16, [0, 64, 0, 64]),  # the tile kernel
+    ("bf16", 4, 2, 16, [0, 64, 0, 64]), ("bf16", 8, 2, 16, [0, 64, 0, 64]),
+    ("bf16", 0, 2, 4, [0, 20, 40, 39, 60]), ("bf16", 0, 2, 16, [0, 20, 40, 39, 60]), ("bf16", 4, 2, 16, [0, 60, 60, 60, 59])])
+def test_tree_first_that_falls(cuda, dtype, bits, hkv, G, first):
+    """Sequences with rows in common would need more than the workspace has: all rows give zeros, with the error bit, and
+    nothing is written behind the workspace. A call whose first rises, in the same workspace, is right."""
+    import sparse_decode as sd
+    torch = cuda
+    B, n, d, page, W, guard = len(first) - 1, max(first), 64, 16, 6, 1 << 22
+    pool = Pool(torch, sd, dtype, bits, hkv, d, page, B * W, 3)
+    tables = tables_of(torch, [page * W] * B, page, B * W, 4)
+    q = torch.randn(n, hkv * G, d, generator=gen(torch, 5), device="cuda").to(tdt(torch, dtype))
+    lengths, flags, size = i32(torch, [80] * B), i32(torch, [0]), ctypes.c_int64()
+    L = sd.lib()
+    sd._check(L.sd_paged_tree_workspace(pool.pages.struct, B, n, hkv * G, size))
+    work = torch.full((size.value + guard,), 0xA5, dtype=torch.uint8, device="cuda")
+
+    def call(rows):
+        out, f = torch.full_like(q, 7.0), i32(torch, rows)
+        sd._check(L.sd_paged_tree_decode(pool.pages.struct, 0, q.data_ptr(), n, B, hkv * G, tables.data_ptr(), W,
+                                         lengths.data_ptr(), f.data_ptr(), None, None, 0.125, 0, None, out.data_ptr(),
+                                         work.data_ptr(), size.value, flags.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        got = int(flags)
+        flags.zero_()
+        assert (work[size.value:] == 0xA5).all()
+        return out, got
+    out, f = call(first)
+    assert f == 2 and not out[:first[-1]].any() and (out[first[-1]:] == 7).all()
+    rises = [min(n, -(-n // B) * b) for b in range(B + 1)]
+    out, f = call(rises)
+    want = sd.paged_tree_decode(q, pool.pages, tables, lengths, i32(torch, rises), scale=0.125)
+    assert f == 0 and torch.equal(out, want) and out.abs().amax((1, 2)).min() > 0
