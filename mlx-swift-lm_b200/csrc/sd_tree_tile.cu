@@ -13,11 +13,15 @@
 //     every tile;
 //   else: it has up to 128, both groups have the same ones, and tiles go to the
 //     groups in turn, whose parts are joined at a segment's end.
-// P has two buffers beside S, so that the scores of the next tile are made as
-// soon as this one's have been read, and P V while the next is weighed: no
-// product waits for another one to end.
-// P is one value of the element type: its products cost as much as its
-// exponentials, and a second half of it would cost as much again.
+// P has its place beside S, so that the scores of the next tile are made as
+// soon as this one's have been read, and P V while the next is weighed: only the
+// store of P waits for the product before.
+// P is two values of the element type, a high and a low half, as in the kernel for
+// few columns: 16 bits of it (22 of fp16), so that a result has its own rounding and
+// nothing else, whatever the number of columns. One half alone was half a step of
+// every weight, and a result 1.4 times as far off in the mean square (rows of bf16 up
+// to 5e-3 off the rounded exact result, 2e-3 being the tolerance); it took 154 us for
+// the largest case below instead of 180, and 38 instead of 40 for one sequence of 32K.
 //
 // The running maximum lags by up to kSlack, as in a decode; when it moves, its
 // group rescales O in tensor memory. The nodes are the sequence's last tokens: a
@@ -26,12 +30,13 @@
 // the range may hold anything and are zeroed in shared memory, and so are
 // infinities and not-a-numbers in a node's row, which a row that does see the
 // node gets back at the end.
-// Bound by the weighing warps: 64 tokens of 256 columns are 16384 exponentials,
-// 1024 cycles of an SM, and 1280 cycles of products, and take some 2000: each
-// scheduler has two such warps, whose chain (load, maxima, exponentials, store,
-// signal) leaves gaps. Measured with the merge, 32 query and 8 kv heads of 128 in
-// bf16: 4 sequences of 32K tokens with 64 nodes 153 us (0.90 PFLOP/s, 3.5 TB/s),
-// one with 32 nodes 38 us (3.6 TB/s); 4 x 32K in 4 bits with 16 nodes 117 us.
+// Bound by the weighing warps and the products: 64 tokens of 256 columns are 16384
+// exponentials, 1024 cycles of an SM, and some 1900 cycles of products, and take some
+// 2300: each scheduler has two such warps, whose chain (load, maxima, exponentials,
+// halves, store, signal) leaves gaps. Measured with the merge, 32 query and 8 kv heads
+// of 128 in bf16: 4 sequences of 32K tokens with 64 nodes 180 us (3.0 TB/s; 0.76 PFLOP/s
+// of attention, half as much again with the low halves), one with 32 nodes 40 us
+// (3.3 TB/s); 4 x 32K in 4 bits with 16 nodes 126 us.
 //
 // Codes: the loading warp brings them as they are, with their scales; a warp finds
 // the tile's powers (below) and makes the scales fp16, in their places; eight more
@@ -68,7 +73,7 @@ constexpr int kTileT = kTreeTileTokens;
 static_assert(kTileT == 64, "a row's bits of a tile are a mask's");
 constexpr int kTmemCols = 512;
 constexpr int kNoPower = -1000;  // of a tile of zeros, which takes any
-// Tensor memory columns of the first group's S, its P's two buffers, and its O; the second's are 128 on.
+// Tensor memory columns of the first group's S, its P's high and low halves, and its O; the second's are 128 on.
 constexpr int kSCol = 0, kPCol = 64, kOCol = 256;
 
 // --- tensor core pieces -----------------------------------------------------
@@ -222,7 +227,7 @@ __device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 
 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
-  uint64_t q_full[2], s_full[2], s_free[2], p_full[2][2], o_full[2][2];  // of a group; of a group's buffer of P
+  uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_full[2];  // of a group
   uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages], pow_full[kTreeRawStages];
   uint64_t started, done;
   uint32_t tmem;
@@ -264,10 +269,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       mbar_init(bars->q_full + w, kQs == 1 && w == 1 ? 8 : 4);
       mbar_init(bars->s_full + w, 1);
       mbar_init(bars->s_free + w, 4);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars->o_full[w][i], 1);
-        mbar_init(&bars->p_full[w][i], 4);
-      }
+      mbar_init(bars->o_full + w, 1);
+      mbar_init(bars->p_full + w, 4);
     }
     for (int i = 0; i < kTreeRawStages; ++i) {
       mbar_init(bars->raw_full + i, 33);
@@ -391,7 +394,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       const uint64_t q = operand_desc(0, 16, 1024) + ((smem_u32(qs) + (kQs == 2 ? w * kQ : 0)) >> 4);
       const uint64_t kd0 = operand_desc(0, 16, 1024) + (smem_u32(ring) >> 4), vd0 = operand_desc(0, kHalf, 1024) + (smem_u32(ring) >> 4);
       const uint32_t ds = tmem + kSCol + w * 128, dp = tmem + kPCol + w * 128, dO = tmem + kOCol + w * 128;
-      const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full[w]), s_full = smem_u32(bars->s_full + w);
+      const uint32_t empty = smem_u32(bars->empty), o_full = smem_u32(bars->o_full + w), s_full = smem_u32(bars->s_full + w);
       while (walk.next(s)) {
         const int nt = s.i1 - s.i0, n = SHARED ? nt : (nt + 1 - w) / 2;
         if (n > 0) {
@@ -421,14 +424,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             if (ks >= p.stages) ks -= p.stages, kp ^= 1;
           }
           if (i >= 0) {
-            const uint32_t h = (k + i) & 1u;  // buffer of P
-            if (!wait(bars->full + vs, uint32_t(vp)) || !wait(&bars->p_full[w][h], ((k + i) >> 1) & 1u)) break;
+            if (!wait(bars->full + vs, uint32_t(vp)) || !wait(bars->p_full + w, (k + i) & 1u)) break;
             tc_fence_after();
             const uint64_t v = vd0 + vs * (kStage >> 4);
-            const uint32_t pp = dp + h * (kTileT / 2);
 #pragma unroll
-            for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, pp + c * 8, v + c * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
-            mma_commit(o_full + h * 8);
+            for (int c = 0; c < kTileT / 8; ++c)  // P's high half, then its low one
+              mma_ts(dO, dp + c * 8, v + c % (kTileT / 16) * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
+            mma_commit(o_full);
             mma_commit(empty + vs * 8);
             vs += SHARED ? 2 : 4;
             if (vs >= p.stages) vs -= p.stages, vp ^= 1;
@@ -651,7 +653,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       for (; steps < n; ++steps, ++k) {
         const int tile = SHARED ? steps : 2 * steps + w;  // of the segment
         const int tok = (t0 + s.i0 + tile) * kTileT, lo = sq.begin - tok, hi = sq.end - tok;
-        const uint32_t h = k & 1u;  // buffer of P
         const int old = sq.held - tok;  // rows of the tile before the nodes'
         const bool ends = lo > 0 || old < kTileT;
         // Every group that uses the tile waits for its rows, dead or not; the second one before its own scores, which may
@@ -734,7 +735,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             if (ref != kNoPower) fac *= power(max(ref - ev, -126));
             ref = ev;
           }
-          if (wait(&bars->o_full[w][h ^ 1], ((k - 1) >> 1) & 1u)) {  // the last product
+          if (wait(bars->o_full + w, (k - 1) & 1u)) {  // the last product
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -752,36 +753,36 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const int dv = BITS && !none ? ev - ref : 0;
         const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(dv - m, dv - m), sc2 = make_float2(sc, sc);
         float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-        uint32_t two[32];
+        uint32_t high[32], low2[32];
         auto weigh = [&](const uint32_t (&v)[32], int c) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float2 e = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc2, mm);
             e.x = ex2(e.x), e.y = ex2(e.y);
             sum[j & 1] = add2(sum[j & 1], e);
-            two[16 * c + j] = pack2<T>(e.x, e.y);
+            split2<T>(e.x, e.y, high[16 * c + j], low2[16 * c + j]);
           }
         };
         weigh(va, 0);
         weigh(vb, 1);
         if (none) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) two[j] = 0;
+          for (int j = 0; j < 32; ++j) high[j] = low2[j] = 0;
         }
-        // the buffer's last product is done, too: what signalled these scores was issued after it and waits for both
-        tmem_st32(tp + h * (kTileT / 2), two);
+        if (k > 0 && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();  // what was there has been multiplied
+        tmem_st32(tp, high);
+        tmem_st32(tp + kTileT / 2, low2);
         const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         l = BITS ? fmaf(more, power(-dv), l) : l + more;
         tc_wait_st();
         tc_fence_before();
-        warp_arrive(&bars->p_full[w][h]);
+        warp_arrive(bars->p_full + w);
         if (w == 0 && k == 0) warp_arrive(&bars->started);
       }
       it0 += s.i1 - s.i0;
       // (o, m, l) of the segment
       float* part = tree_part(p, s.pair + int(blockIdx.x));
-      if (steps > 1) wait(&bars->o_full[w][k & 1u], ((k - 2) >> 1) & 1u);
-      if (steps > 0 && wait(&bars->o_full[w][(k - 1) & 1u], ((k - 1) >> 1) & 1u)) tc_fence_after();
+      if (steps > 0 && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();
       const bool has = steps > 0 && !wait.dead;
       // A node's value that is not finite counts in the rows that see it.
       auto add_odd = [&](int c, uint32_t (&o)[32]) {

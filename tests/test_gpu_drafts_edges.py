@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 
+import test_gpu_drafts as tree
 from test_gpu_drafts import i32
 from test_gpu_paged import Pool, gen, tables_of, tdt
 
@@ -94,3 +95,24 @@ def test_tree_first_that_falls(cuda, dtype, bits, hkv, G, first):
     out, f = call(rises)
     want = sd.paged_tree_decode(q, pool.pages, tables, lengths, i32(torch, rises), scale=0.125)
     assert f == 0 and torch.equal(out, want) and out.abs().amax((1, 2)).min() > 0
+
+
+# ---------------------------------------------------------------------------
+# tree attention: the same precision whatever the number of columns
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,bits,d,hkv,G,page,held,counts,more", [
+    ("bf16", 0, 128, 2, 4, 64, [3000, 5, 0, 1000], [33, 20, 64, 40], {}),
+    ("bf16", 0, 64, 2, 4, 64, [700, 90], [64, 20], {}),
+    ("bf16", 0, 128, 2, 16, 64, [20000, 37], [33, 60], {}),
+    ("bf16", 0, 128, 2, 8, 32, [400, 3, 150, 64, 0], [20, 12, 1, 64, 30], dict(window=65, sinks=True)),
+    ("f16", 0, 128, 2, 4, 64, [3000, 5, 0, 1000], [33, 20, 64, 40], {}),
+    ("f16", 0, 64, 3, 8, 16, [700, 90], [64, 20], dict(window=200)),
+    ("f16", 0, 128, 1, 16, 64, [9000], [40], {}),
+])
+def test_tree_precision_does_not_go_by_the_columns(cuda, monkeypatch, dtype, bits, d, hkv, G, page, held, counts, more):
+    """Calls with many columns have the framework's tolerance and the mean square of the result's own rounding, as those
+    with few: weights keep 16 bits or more."""
+    assert tree.uses_tiles(dtype, bits, counts, G)
+    monkeypatch.setattr(tree, "uses_tiles", lambda *a: False)
+    tree.run_tree(cuda, dtype, bits, d, hkv, G, page, held, counts, seed=G + d, **more)
