@@ -102,11 +102,13 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups
 // of four warps, a warp that issues products for each and a loading warp.
-// The rule for it: more columns, of an average sequence, than tree_attend_kernel has in one pass over the tokens, or in
-// two of 8-bit codes. Measured with 8 sequences of 8K tokens, 8 kv heads of 128, us, that kernel and this one: bf16, 16
-// columns 51 and 58, 20 columns 88 and 58; 4 bits, 16 columns 53 and 74, 20 columns 87 and 74; 8 bits, 32 columns 91 and
-// 95, 48 columns 128 and 97.
-constexpr int tree_tile_above(int bits) { return bits == 8 ? 32 : 16; }
+// The rule for it: more columns, of an average sequence, than tree_attend_kernel has in one pass over the tokens, or in two
+// of codes. Measured with 8 sequences of 8K tokens and 8 kv heads, us, that kernel and this one: bf16, heads of 128, 16
+// columns 50 and 60, 20 columns 88 and 61; of 64, 16 columns 31 and 48, 20 columns 50 and 48. 4 bits, heads of 128, 32 columns
+// 89 and 114, 40 columns 124 and 114, 64 columns 164 and 118, 128 columns 323 and 125; of 64, 40 columns 70 and 88, 64
+// columns 90 and 89, 128 columns 169 and 91; 8 bits the same within 6 us. 16 sequences of 700 tokens, 4 bits, heads of 128, 32
+// columns 45 and 42, 40 columns 70 and 45; of 64, 40 columns 35 and 32.
+constexpr int tree_tile_above(int bits) { return bits ? 32 : 16; }
 constexpr int kTreeTileThreads = 352;
 constexpr int kTreeTileTokens = 64;
 // Beginning and ending a segment, in tiles. Measured, 2 / 4 / 8 / 16: 12 windows of 1000 tokens, 168 columns, 38.9 / 31.3 /
@@ -115,18 +117,16 @@ constexpr int kTreeTileTokens = 64;
 constexpr int kTreeTileUnits = 8;
 constexpr int kTreeTileStages = 24, kTreeTileLeast = 4;
 constexpr int kTreeTileBarBytes = 768;
-// For codes eight more warps make tiles of fp16 values of them.
+// For codes eight more warps make tiles of values of them, in two halves each.
 constexpr int kTreeCodeThreads = 640;
 constexpr int kTreeRawStages = 8;
-constexpr int kTreePows = 32;  // tiles whose powers are kept: more than stages hold
-static_assert(kTreePows > kTreeTileStages / 2 + 1, "a tile's powers are read while later ones are written");
 __host__ __device__ constexpr int tree_tile_queries(int D, int bits, bool shared) { return bits && !shared && D == 128 ? 1 : 2; }
 // Codes of K and V of a tile and their scales and biases.
 __host__ __device__ constexpr int tree_raw_stage(int D, int bits) {
   return bits ? 2 * kTreeTileTokens * D * bits / 8 + 4 * kTreeTileTokens * (D / 64) * 2 : 0;
 }
 constexpr int kTreeTileSmem = 232448 - 4096;  // beside 4 KB of static shared memory
-// For rows of `shared`: up to 256 columns, else up to 128 (both groups hold them all).
+// For rows of `shared`: up to 256 columns, not for codes, else up to 128 (both groups hold them all).
 const void* tree_tile_e1_b0(int D, bool shared);
 const void* tree_tile_e2_b0(int D, bool shared);
 const void* tree_tile_e2_b4(int D, bool shared);
@@ -145,7 +145,7 @@ constexpr TileLayout tree_tile_layout(int batch, int D, int bits, bool shared) {
   // its phase by the parity, so whoever waits has to know that the phase before is done.
   // (Of codes, with one of the two teams of warps that make the tiles, too.)
   const int by = shared && !bits ? 1 : 4;
-  if (bits) {  // four tiles of values, or two, and the rest for codes, but two stages at least
+  if (bits) {  // eight tiles of halves of values, or four, and the rest for codes, but two stages at least
     const int fit = (room - 2 * raw) / stage;
     l.stages = (fit < 8 ? fit : 8) / by * by;
     l.raw_stages = (room - l.stages * stage) / raw / 2 * 2;

@@ -70,17 +70,20 @@ int32_t tree_shape(const sd_pages* g, int32_t batch, int32_t n_rows, int32_t n_q
   const TreeSet set = lookup_tree(g->dtype, g->kv_bits, D, int(std::min<int64_t>(columns, 16)));
   if (!set.merge) return fail(SD_ERR_SHAPE, "no kernel for dtype %d, bits %d, head_dim %d", g->dtype, g->kv_bits, D);
   s->merge = set.merge;
-  // Codes of fp16 pools are not for the tile kernel: its fp16 tiles of them cost as much as such an output's own rounding,
-  // twice over (4e-4 of the result, relative, instead of 2e-4; nothing to speak of beside bf16's 1.7e-3).
+  // Codes of fp16 pools are not for the tile kernel: its tiles of them, two bf16 values each, would need queries in two
+  // as well.
   const auto tile_kernel = lookup_tile(g->dtype, g->kv_bits);
-  s->tiles = tile_kernel && columns > tree_tile_above(g->kv_bits);
+  const bool shared = columns > 128 && !g->kv_bits;
+  s->lay = tree_tile_layout(batch, D, g->kv_bits, shared);
+  // Of codes a tile of K or V is two, of high and low halves, and two tiles are under way: thousands of sequences with heads
+  // of 128 leave no room for that in 8 bits.
+  s->tiles = tile_kernel && columns > tree_tile_above(g->kv_bits) && (!g->kv_bits || s->lay.stages == 8);
   if (s->tiles) {
-    const bool shared = columns > 128;
     s->attend = tile_kernel(D, shared);
     s->threads = g->kv_bits ? kTreeCodeThreads : kTreeTileThreads;
     s->smem_most = kTreeTileSmem;
-    s->lay = tree_tile_layout(batch, D, g->kv_bits, shared);
     s->q_off = s->lay.raw_off;
+    if (g->kv_bits) s->lay.stages /= 2;
     s->tile = kTreeTileTokens;
     s->columns = shared ? 256 : 128;
     s->ctas = sms;

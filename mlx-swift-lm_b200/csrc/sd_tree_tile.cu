@@ -36,19 +36,19 @@
 // halves, store, signal) leaves gaps. Measured with the merge, 32 query and 8 kv heads
 // of 128 in bf16: 4 sequences of 32K tokens with 64 nodes 180 us (3.0 TB/s; 0.76 PFLOP/s
 // of attention, half as much again with the low halves), one with 32 nodes 40 us
-// (3.3 TB/s); 4 x 32K in 4 bits with 16 nodes 126 us.
+// (3.3 TB/s); 4 x 32K in 4 bits with 16 nodes 201 us.
 //
-// Codes: the loading warp brings them as they are, with their scales; a warp finds
-// the tile's powers (below) and makes the scales fp16, in their places; eight more
-// make tiles of fp16 values, s c + b by one packed fma for two codes. A tile costs
-// some 2000 cycles there, too: these warps have the schedulers' slots in common with
-// the weighing ones. (With four of them, each looking for the powers on its own, 4 x
-// 32K in 4 bits took 146 us.)
-// fp16 has 11 bits, three more than the bf16 of the result, but a narrow range, so a
-// tile of K, or of V, is scaled by a power of two of its own -- exactly, as bf16
-// scales have 8 bits: the largest of K goes to [2^13, 2^14), of V to [2^6, 2^14) in
-// steps of 2^8, and the scores, or weights and O, take the power back. Queries are
-// scaled row by row in the same way.
+// Codes: the loading warp brings them as they are, with their scales; eight more
+// make tiles of values of them, s c + b in fp32 and then two bf16 values, a high and a low
+// half: 16 bits of a value, and fp32's range, so that a token's size does not matter to
+// another's, be it seen or not. The products are q times both halves of K, and three of
+// P and V, less the low halves' own. Bound by the converting warps: ten instructions make
+// two values, and a tile takes one of their two teams 4500 cycles, 2600 a tile with what they
+// wait for (P V first and then the next scores, which wait for the team: the other order
+// kept V's place from the team, 291 us instead of 201 for 4 x 32K in 4 bits with 16
+// nodes). One fp16 value with a power of two per tile took 126 us there, but it was
+// off by 2^-12 of every value, which keys with a large channel make 8e-3 of a result, and
+// lost a tile's small values beside a large one that a row need not even see.
 #include "sd_tree.cuh"
 
 #if !defined(SD_E) || !defined(SD_BITS)
@@ -63,8 +63,6 @@ using ET = __half;
 using ET = __nv_bfloat16;
 #endif
 
-#include <type_traits>
-
 namespace sd {
 
 namespace {
@@ -72,7 +70,6 @@ namespace {
 constexpr int kTileT = kTreeTileTokens;
 static_assert(kTileT == 64, "a row's bits of a tile are a mask's");
 constexpr int kTmemCols = 512;
-constexpr int kNoPower = -1000;  // of a tile of zeros, which takes any
 // Tensor memory columns of the first group's S, its P's high and low halves, and its O; the second's are 128 on.
 constexpr int kSCol = 0, kPCol = 64, kOCol = 256;
 
@@ -204,31 +201,34 @@ __device__ __forceinline__ bool finite2(uint32_t& w) {
   return a || b;
 }
 
-// Four codes of a word as fp16 pairs.
-__device__ __forceinline__ void codes8(uint32_t w, uint32_t magic, uint32_t (&v)[2]) {
-  v[0] = sub_f16x2(raw_u8(w, 0x5150u, magic), 0x64006400u);
-  v[1] = sub_f16x2(raw_u8(w, 0x5352u, magic), 0x64006400u);
+// Codes as floats, 2^23 + c less 2^23: two neighbouring bytes of a word, or two nibbles four apart, bits 4 i of each half,
+// as 16^i times as much. So the tiles of nibbles hold codes 0 4 1 5 2 6 3 7 of every eight dimensions, as their rows of Q
+// do, and O has its columns in that order.
+__device__ __forceinline__ float2 bytes2(uint32_t w, int i) {
+  return add2(make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 + i)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7651 + i))),
+              make_float2(-8388608.0f, -8388608.0f));
 }
-// Codes 0 and 4, or 1 and 5 -- as 16 times as much --, of a word of nibbles as an fp16 pair. So the tiles hold codes
-// 0 4 1 5 2 6 3 7 of every eight dimensions, as their rows of Q do, and O has its columns in that order.
-template <uint32_t WHICH>
-__device__ __forceinline__ uint32_t codes4(uint32_t w, uint32_t magic) {
-  return sub_f16x2((w & WHICH) | magic, 0x64006400u);
+__device__ __forceinline__ float2 nibbles2(uint32_t w, int i) {
+  return add2(make_float2(__uint_as_float((w & (15u << (4 * i))) | 0x4B000000u), __uint_as_float((w >> 16 & (15u << (4 * i))) | 0x4B000000u)),
+              make_float2(-8388608.0f, -8388608.0f));
 }
-__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
+// Two values' high halves (cut off, so that they are finite where the values are) and low ones.
+__device__ __forceinline__ void halves2(float2 x, uint32_t& high, uint32_t& low) {
+  const uint32_t a = __float_as_uint(x.x), b = __float_as_uint(x.y);
+  high = __byte_perm(a, b, 0x7632);
+  const float2 r = fma2(make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), x);
+  low = pack2<__nv_bfloat16>(r.x, r.y);
 }
-__device__ __forceinline__ bool finite(float scale, float bias) { return fabsf(scale) < INFINITY && fabsf(bias) < INFINITY; }
-// 2^e for e in [-126, 127].
-__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23 & 255) - 127; }  // of a normal x > 0
+// Whether all codes of a group stand for finite values.
+template <int BITS>
+__device__ __forceinline__ bool finite_group(float scale, float bias) {
+  return fabsf(bias) < INFINITY && fabsf(fmaf(scale, float((1 << BITS) - 1), bias)) < INFINITY;
+}
 
 struct TileBars {
   uint64_t full[kTreeTileStages], empty[kTreeTileStages];
   uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_full[2];  // of a group
-  uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages], pow_full[kTreeRawStages];
+  uint64_t raw_full[kTreeRawStages], raw_empty[kTreeRawStages];
   uint64_t started, done;
   uint32_t tmem;
 };
@@ -241,10 +241,10 @@ __global__ void __launch_bounds__(BITS ? kTreeCodeThreads : kTreeTileThreads, 1)
 tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV) {
   constexpr int NH = D / 64, kQHalf = 128 * 128, kHalf = kTileT * 128;  // bytes of 64 dimensions of Q, of a tile
-  constexpr int kQ = NH * kQHalf, kStage = NH * kHalf;
+  constexpr int kQ = NH * kQHalf, kTile = NH * kHalf, kStage = BITS ? 2 * kTile : kTile;  // of codes: high halves, then low ones
   constexpr int kThreads = BITS ? kTreeCodeThreads : kTreeTileThreads;
-  using T = std::conditional_t<BITS != 0, __half, E>;        // of the products' operands
-  constexpr float kUp = __is_same(T, __half) ? 7.0f : 0.0f;  // as in a decode: fp16 weights up to 2^(kUp + kSlack)
+  static_assert(!BITS || !SHARED, "codes: pairs of up to 128 columns, there is no room for more rows of Q beside the tiles");
+  constexpr float kUp = __is_same(E, __half) ? 7.0f : 0.0f;  // as in a decode: fp16 weights up to 2^(kUp + kSlack)
   constexpr int kQs = tree_tile_queries(D, BITS, SHARED);    // copies of Q: one for both groups makes room for the ring
   constexpr int kRow = BITS ? D * BITS / 8 : 1, kSb = BITS ? kTileT * (D / 64) * 2 : 0;  // bytes: a row of codes, a tile's scales
   constexpr int kRaw = tree_raw_stage(D, BITS);
@@ -255,9 +255,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
   int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1;
   __shared__ float2 ml_of[2][SHARED ? 1 : 128];
-  // codes: powers of the last tiles' K and V, and whether a node's V is not finite; of the rows of Q
-  __shared__ int4 tile_pow[BITS ? kTreePows : 1];
-  __shared__ int q_pow[2][BITS ? 128 : 1];
+  __shared__ int4 odd_of[2];  // codes: whether a node's V is not finite, by the four warps that made it; of two tiles
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -275,7 +273,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
     for (int i = 0; i < kTreeRawStages; ++i) {
       mbar_init(bars->raw_full + i, 33);
       mbar_init(bars->raw_empty + i, 4);
-      mbar_init(bars->pow_full + i, 1);
     }
     mbar_init(&bars->started, 4);
     mbar_init(&bars->done, 2);
@@ -407,17 +404,21 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         const int u = 2 * (it0 + (SHARED ? 0 : w));
         int ks = u % p.stages, kp = (u / p.stages) & 1, vs = (u + 1) % p.stages, vp = ((u + 1) / p.stages) & 1;
         // The scores of tile i + 1, then P V of tile i. The first scores follow the rows of Q: with those the group has
-        // read what it needs of its last S and O.
+        // read what it needs of its last S and O. Codes: P V of tile i before the scores of the next one, whose keys' place
+        // is made free by this one's scores and its values' by this P V.
 #pragma unroll 1
-        for (int i = -1; i < n && !wait.dead; ++i) {
-          if (i + 1 < n) {
-            if (!wait(bars->full + ks, uint32_t(kp)) || (i >= 0 && !wait(bars->s_free + w, (k + i) & 1u))) break;
+        for (int i = BITS ? 0 : -1; i < n && !wait.dead; ++i) {
+          const int next = BITS ? i : i + 1;
+          if (next < n) {
+            if (!wait(bars->full + ks, uint32_t(kp)) || (next > 0 && !wait(bars->s_free + w, (k + next - 1) & 1u))) break;
             tc_fence_after();
             const uint64_t kd = kd0 + ks * (kStage >> 4);
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-              mma_ss(ds, q + (c / 4) * (kQHalf >> 4) + (c % 4) * 2, kd + (c / 4) * (kHalf >> 4) + (c % 4) * 2,
-                     product_desc<T>(kTileT, false), c > 0);
+            for (int c = 0; c < kStage / kTile * (D / 16); ++c) {  // codes: K's high halves, then the low ones
+              const int cc = c % (D / 16);
+              mma_ss(ds, q + (cc / 4) * (kQHalf >> 4) + (cc % 4) * 2,
+                     kd + c / (D / 16) * (kTile >> 4) + (cc / 4) * (kHalf >> 4) + (cc % 4) * 2, product_desc<E>(kTileT, false), c > 0);
+            }
             mma_commit(s_full);
             mma_commit(empty + ks * 8);
             ks += SHARED ? 2 : 4;
@@ -429,7 +430,11 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             const uint64_t v = vd0 + vs * (kStage >> 4);
 #pragma unroll
             for (int c = 0; c < kTileT / 8; ++c)  // P's high half, then its low one
-              mma_ts(dO, dp + c * 8, v + c % (kTileT / 16) * (2048 >> 4), product_desc<T>(D, true), i > 0 || c > 0);
+              mma_ts(dO, dp + c * 8, v + c % (kTileT / 16) * (2048 >> 4), product_desc<E>(D, true), i > 0 || c > 0);
+            if constexpr (BITS != 0) {  // the high half with V's low one
+#pragma unroll
+              for (int c = 0; c < kTileT / 16; ++c) mma_ts(dO, dp + c * 8, v + (kTile >> 4) + c * (2048 >> 4), product_desc<E>(D, true), true);
+            }
             mma_commit(o_full);
             mma_commit(empty + vs * 8);
             vs += SHARED ? 2 : 4;
@@ -441,71 +446,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
       }
       mma_commit(smem_u32(&bars->done));  // no product may read shared memory that is no longer this CTA's
       mbar_wait(&bars->done, 0, p.flags);
-    } else if (BITS && warp == 11) {  // ---- powers of the tiles of codes ----
-      if constexpr (BITS) {
-        constexpr int NG = D / 64;
-        constexpr float kTop = float((1 << BITS) - 1);
-        int rs = 0;
-        uint32_t rp = 0;
-        while (walk.next(s)) {
-          const TreeSeq sq = tree_seq(p, s.b);
-          const int t0 = sq.begin / kTileT;
-          for (int i = s.i0; i < s.i1; ++i, ++it0) {
-            const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
-            wait(bars->raw_full + rs, rp);
-            // the largest value of K and of V, and whether a node's V is not finite; a lane has pairs of scales and biases
-            uint32_t* small = reinterpret_cast<uint32_t*>(raws + rs * kRaw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][32 NG]
-            uint32_t sc[2 * NG], bi[2 * NG], most[2] = {0, 0};
-            bool odd = false;
-#pragma unroll
-            for (int e = 0; e < 2 * NG; ++e) {
-              const int v = e / NG, at = lane + 32 * (e % NG);
-              sc[e] = small[v * 64 * NG + at], bi[e] = small[(v * 2 + 1) * 32 * NG + at];
-              uint32_t x;
-              asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(sc[e]), "r"(BITS == 8 ? 0x437f437fu : 0x41704170u), "r"(bi[e]));
-              most[v] = __vmaxu2(most[v], __vmaxu2(x & 0x7fff7fffu, bi[e] & 0x7fff7fffu));
-            }
-#pragma unroll
-            for (int v = 0; v < 2; ++v) most[v] = __reduce_max_sync(0xffffffffu, max(most[v] << 16, most[v] & 0xffff0000u));
-            if (lo > 0 || old < kTileT || most[0] >= 0x7f800000u || most[1] >= 0x7f800000u) {  // what counts, one by one
-              most[0] = most[1] = 0;
-#pragma unroll 1
-              for (int e = 0; e < 4 * NG; ++e) {
-                const int v = e / (2 * NG), x = e % (2 * NG) * 32 + lane, row = x / NG;
-                __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(small) + v * 2 * kTileT * NG + x;
-                const float a = __bfloat162float(at[0]), b = __bfloat162float(at[kTileT * NG]);
-                const bool in = row >= lo && row < hi, fine = finite(a, b);
-                if (in && fine) most[v] = max(most[v], __float_as_uint(fminf(fmaxf(fabsf(b), fabsf(fmaf(a, kTop, b))), 3.4e38f)));
-                // rows of V that no row sees, or a node's that is not finite (rows that see it get it back): 0 * NaN is NaN
-                odd |= v == 1 && in && row >= old && !fine;
-                if (v && (!in || (row >= old && !fine))) at[0] = at[kTileT * NG] = __float2bfloat16_rn(0.0f);
-              }
-              most[0] = __reduce_max_sync(0xffffffffu, most[0]), most[1] = __reduce_max_sync(0xffffffffu, most[1]);
-              odd = __any_sync(0xffffffffu, odd);
-              __syncwarp();
-#pragma unroll
-              for (int e = 0; e < 2 * NG; ++e) {
-                const int v = e / NG, at = lane + 32 * (e % NG);
-                sc[e] = small[v * 64 * NG + at], bi[e] = small[(v * 2 + 1) * 32 * NG + at];
-              }
-            }
-            const int ek = most[0] ? max(exponent(__uint_as_float(most[0])) - 13, -120) : 0;
-            const int ev = most[1] ? max((exponent(__uint_as_float(most[1])) - 6) & ~7, -120) : kNoPower;
-            if (lane == 0) tile_pow[it0 & (kTreePows - 1)] = make_int4(ek, ev, int(odd), 0);
-            // scaled and in fp16, in their places
-#pragma unroll
-            for (int e = 0; e < 2 * NG; ++e) {
-              const int v = e / NG, at = lane + 32 * (e % NG);
-              const float f = v ? power(ev == kNoPower ? 0 : -ev) : power(-ek);
-              auto half2 = [&](uint32_t w) { return pack2<__half>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f); };
-              small[v * 64 * NG + at] = half2(sc[e]), small[(v * 2 + 1) * 32 * NG + at] = half2(bi[e]);
-            }
-            warp_arrive(bars->pow_full + rs);
-            if (++rs == p.raw_stages) rs = 0, rp ^= 1u;
-          }
-        }
-      }
-    } else if (BITS && warp >= 12) {  // ---- codes into fp16 tiles ----
+    } else if (BITS && warp >= 12) {  // ---- codes into tiles of halves ----
       if constexpr (BITS) {
         constexpr int NG = D / 64, EPC = 128 / BITS, CPR = kRow / 16;  // groups, codes of 16 bytes, such pieces of a row
         // Four warps for every other tile: what a tile waits for (codes, a free stage) is hidden by the other four's.
@@ -516,47 +457,65 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         int rs = team, ks = 2 * team;  // the tile's stages: of codes, of K (V's is the next one); their phases
         uint32_t rp = 0, kp = 0;
         while (walk.next(s)) {
-          for (int t = it0; t < it0 + s.i1 - s.i0; ++t) {
-            if ((t & 1) != team) continue;
-            wait(bars->pow_full + rs, rp);
+          const TreeSeq sq = tree_seq(p, s.b);
+          const int t0 = sq.begin / kTileT;
+          for (int i = s.i0; i < s.i1; ++i, ++it0) {
+            if ((it0 & 1) != team) continue;
+            const int tok = (t0 + i) * kTileT, lo = sq.begin - tok, hi = sq.end - tok, old = sq.held - tok;
+            wait(bars->raw_full + rs, rp);
             const uint8_t* raw = raws + rs * kRaw;
-            const uint16_t* small = reinterpret_cast<const uint16_t*>(raw + 2 * kTileT * kRow);  // fp16 by now
+            const uint16_t* small = reinterpret_cast<const uint16_t*>(raw + 2 * kTileT * kRow);  // [K scales, K biases, V ..][64][NG]
 #pragma unroll 1
             for (int v = 0; v < 2; ++v) {
               const int st = ks + v;
               wait(bars->empty + st, kp ^ 1u);  // in the first phase at once
               if (!wait.dead) {
                 const uint32_t dst = smem_u32(ring) + st * kStage;
+                bool odd = false;
 #pragma unroll 1
                 for (int e = 0; e < kTileT * CPR / 128; ++e) {
                   const int x = ct + 128 * e;
                   const int row = x / (8 * NG) * (8 / PH) + x / PH % (8 / PH), half = x / 8 % NG, c = half * PH + x % PH;
                   const uint4 w = lds128(smem_u32(raw) + (v * kTileT + row) * kRow + c * 16);
                   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-                  const uint32_t s1 = small[v * 2 * kTileT * NG + row * NG + half] * 0x10001u;
-                  const uint32_t b1 = small[(v * 2 + 1) * kTileT * NG + row * NG + half] * 0x10001u;
-                  uint32_t s16;  // 2^-4 s, exact but for subnormals
-                  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s16) : "r"(s1), "r"(0x2C002C00u));
+                  float sc = __uint_as_float(uint32_t(small[v * 2 * kTileT * NG + row * NG + half]) << 16);
+                  float bi = __uint_as_float(uint32_t(small[(v * 2 + 1) * kTileT * NG + row * NG + half]) << 16);
+                  if (v && (row < lo || row >= hi)) sc = bi = 0.0f;  // rows that no row sees may hold anything, and 0 * NaN is NaN
+                  const bool fine = finite_group<BITS>(sc, bi), node = v && row >= old;
+                  odd |= node && !fine;
+                  const float2 b2 = make_float2(bi, bi);
 #pragma unroll
-                  for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile
-                    uint32_t h[4];
-                    if constexpr (BITS == 8) {
-                      uint32_t a[2], b[2];
-                      codes8(words[2 * j], p.magic, a);
-                      codes8(words[2 * j + 1], p.magic, b);
-                      h[0] = fma_f16x2(a[0], s1, b1), h[1] = fma_f16x2(a[1], s1, b1);
-                      h[2] = fma_f16x2(b[0], s1, b1), h[3] = fma_f16x2(b[1], s1, b1);
-                    } else {  // two codes by one logic operation, 16 times as large every other time
-                      const uint32_t up = words[j] >> 8;
-                      h[0] = fma_f16x2(codes4<0x000F000Fu>(words[j], p.magic), s1, b1);
-                      h[1] = fma_f16x2(codes4<0x00F000F0u>(words[j], p.magic), s16, b1);
-                      h[2] = fma_f16x2(codes4<0x000F000Fu>(up, p.magic), s1, b1);
-                      h[3] = fma_f16x2(codes4<0x00F000F0u>(up, p.magic), s16, b1);
+                  for (int j = 0; j < EPC / 8; ++j) {  // 16 bytes of the tile, and of the low halves'
+                    float2 f[4];
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                      const float unit = BITS == 8 ? sc : sc * (1.0f / float(1 << (4 * i4)));
+                      f[i4] = fma2(BITS == 8 ? bytes2(words[(2 * j + i4 / 2) & 3], 2 * (i4 & 1)) : nibbles2(words[j & 3], i4), make_float2(unit, unit), b2);
                     }
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) halves2(f[i4], h[i4], l[i4]);
                     const int ch = c * EPC / 8 + j;
                     const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + kTile), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
                   }
+                  if (!fine) {  // no low halves, which are infinities less themselves, and of a node what is finite: rows that
+                                // see it get the rest back
+#pragma unroll 1
+                    for (int j = 0; j < EPC / 8; ++j) {
+                      const int ch = c * EPC / 8 + j;
+                      const uint32_t to = dst + (ch / 8) * kHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+                      uint4 h = lds128(to);
+                      if (node) finite2<E>(h.x), finite2<E>(h.y), finite2<E>(h.z), finite2<E>(h.w);
+                      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h.x), "r"(h.y), "r"(h.z), "r"(h.w) : "memory");
+                      asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to + kTile), "r"(0) : "memory");
+                    }
+                  }
+                }
+                if (v) {
+                  odd = __any_sync(0xffffffffu, odd);
+                  if (lane == 0) reinterpret_cast<int*>(odd_of + team)[warp & 3] = int(odd);
                 }
                 fence_proxy_async_shared();
                 warp_arrive(bars->full + st);
@@ -566,7 +525,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             if ((rs += 2) >= p.raw_stages) rs -= p.raw_stages, rp ^= 1u;
             if ((ks += 4) >= p.stages) ks -= p.stages, kp ^= 1u;
           }
-          it0 += s.i1 - s.i0;
         }
       }
     }
@@ -598,30 +556,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const int row = r / CPR + RPT * i;
-            if constexpr (BITS != 0) {
-              // bf16: the row's largest to [2^13, 2^14), all of its 8 bits in fp16
-              uint32_t w4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-              float f[8], top = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                unpack_word<E>(w4[j], f + 2 * j);
-                top = fmaxf(top, fmaxf(fabsf(f[2 * j]), fabsf(f[2 * j + 1])));
-              }
-#pragma unroll
-              for (int j = 1; j < CPR; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
-              const int e = top > 0.0f && top < INFINITY ? min(max(exponent(top) - 13, -120), 120) : 0;
-              const float down = power(-e);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] *= down;
-              if constexpr (BITS == 4) {  // in the order of the codes
-                v[i].x = pack2<__half>(f[0], f[4]), v[i].y = pack2<__half>(f[1], f[5]);
-                v[i].z = pack2<__half>(f[2], f[6]), v[i].w = pack2<__half>(f[3], f[7]);
-              } else {
-                v[i].x = pack2<__half>(f[0], f[1]), v[i].y = pack2<__half>(f[2], f[3]);
-                v[i].z = pack2<__half>(f[4], f[5]), v[i].w = pack2<__half>(f[6], f[7]);
-              }
-              if (ch == 0) q_pow[SHARED ? w : 0][row] = e;
-            }
+            if constexpr (BITS == 4)  // in the order of the codes
+              v[i] = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
+                                __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
             const uint32_t at = q + (ch / 8) * kQHalf + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
           }
@@ -631,20 +568,12 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         warp_arrive(bars->q_full + w);
         if (kQs == 1 && w == 0 && s.i1 - s.i0 > 1) warp_arrive(bars->q_full + 1);  // these rows are the second group's, too
       }
-      float sq_pow = 1.0f;
-      if constexpr (BITS != 0) {
-        // each group loads its rows, or, of one copy and for a group without tiles, the first one
-        if (SHARED) named_barrier(2 + w, 128);
-        else named_barrier(1, 256);
-        sq_pow = power(q_pow[SHARED ? w : 0][r]);
-      }
       const int low = x < cols.n ? tree_low(p, sq, cols.node(x)) : 0;
       const uint64_t seen = x < cols.n ? tree_seen(p, sq, cols.node(x)) : 0;
       const int edge = __reduce_max_sync(0xffffffffu, low);
       float m = -INFINITY, l = 0.0f;
       int steps = 0;
       bool odd = false;  // a node has a value that is not finite
-      int ref = kNoPower;  // codes: O's power
       const int n = SHARED ? s.i1 - s.i0 : (s.i1 - s.i0 + 1 - w) / 2;
       const int u0 = 2 * (it0 + (SHARED ? 0 : w)) + 1;
       int vs = u0 % p.stages;  // of the tile's V
@@ -681,15 +610,9 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         }
         if (!here) continue;
         tc_fence_after();
-        float sc = scale;
-        int ev = 0;
-        if constexpr (BITS) {
-          // Its powers were written before its V was made, whose stage stays until this group's P is used.
-          wait(bars->full + vs, vp);
-          const int4 pw = tile_pow[(it0 + tile) & (kTreePows - 1)];
-          sc = fminf(fmaxf(scale * sq_pow * power(pw.x), 1.1754944e-38f), 3.4e38f);
-          ev = pw.y;
-          odd |= pw.z != 0;
+        if (BITS && old < kTileT && wait(bars->full + vs, vp)) {  // its stage stays until this group's P is used
+          const int4 f = odd_of[(it0 + tile) & 1];
+          odd |= (f.x | f.y | f.z | f.w) != 0;
         }
         vs += SHARED ? 2 : 4;
         if (vs >= p.stages) vs -= p.stages, vp ^= 1u;
@@ -723,18 +646,12 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           mx[2] = fmaxf(fmaxf(mx[2], __uint_as_float(vb[j])), __uint_as_float(vb[j + 1]));
           mx[3] = fmaxf(fmaxf(mx[3], __uint_as_float(vb[j + 2])), __uint_as_float(vb[j + 3]));
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        const bool up = BITS && ev > ref;  // O's power moves
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         if (steps == 0) {
           m = top - kUp;
-          ref = ev;
-        } else if (__any_sync(0xffffffffu, up || top > m + (kSlack + kUp))) {
-          float fac = raise_max(m, top - kUp);
+        } else if (__any_sync(0xffffffffu, top > m + (kSlack + kUp))) {
+          const float fac = raise_max(m, top - kUp);
           l *= fac;
-          if (up) {
-            if (ref != kNoPower) fac *= power(max(ref - ev, -126));
-            ref = ev;
-          }
           if (wait(bars->o_full + w, (k - 1) & 1u)) {  // the last product
             tc_fence_after();
 #pragma unroll 1
@@ -748,10 +665,7 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             }
           }
         }
-        // Codes: the tile's power of V over O's, at most 1, is a part of the exponent. Below 2^-48 it makes zeros of fp16.
-        const bool none = BITS && ev < ref - 48;
-        const int dv = BITS && !none ? ev - ref : 0;
-        const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(dv - m, dv - m), sc2 = make_float2(sc, sc);
+        const float2 mm = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m, -m), sc2 = make_float2(scale, scale);
         float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         uint32_t high[32], low2[32];
         auto weigh = [&](const uint32_t (&v)[32], int c) {
@@ -760,20 +674,15 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
             float2 e = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc2, mm);
             e.x = ex2(e.x), e.y = ex2(e.y);
             sum[j & 1] = add2(sum[j & 1], e);
-            split2<T>(e.x, e.y, high[16 * c + j], low2[16 * c + j]);
+            split2<E>(e.x, e.y, high[16 * c + j], low2[16 * c + j]);
           }
         };
         weigh(va, 0);
         weigh(vb, 1);
-        if (none) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) high[j] = low2[j] = 0;
-        }
         if (k > 0 && wait(bars->o_full + w, (k - 1) & 1u)) tc_fence_after();  // what was there has been multiplied
         tmem_st32(tp, high);
         tmem_st32(tp + kTileT / 2, low2);
-        const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        l = BITS ? fmaf(more, power(-dv), l) : l + more;
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_wait_st();
         tc_fence_before();
         warp_arrive(bars->p_full + w);
@@ -803,12 +712,13 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
           } else {
             const int64_t g = row * (D / 64) + c / 2;
             const float sc = Elt<E>::to_f32(static_cast<const E*>(p.v_scales)[g]), bi = Elt<E>::to_f32(static_cast<const E*>(p.v_biases)[g]);
-            if (finite(sc, bi)) continue;
+            if (finite_group<BITS>(sc, bi)) continue;
             const uint32_t* v = reinterpret_cast<const uint32_t*>(p.v_data + row * kRow) + c * BITS;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const uint32_t code = __ldcg(v + j * BITS / 32) >> (j * BITS % 32) & ((1u << BITS) - 1);
-              o[j] = __float_as_uint(__uint_as_float(o[j]) + fmaf(float(code), sc, bi));
+              const float x = fmaf(float(code), sc, bi);
+              if (!(fabsf(x) < INFINITY)) o[j] = __float_as_uint(__uint_as_float(o[j]) + x);
             }
           }
         }
@@ -820,11 +730,6 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0;
-        }
-        if constexpr (BITS) {
-          const float back = ref == kNoPower ? 1.0f : power(ref);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
         }
         if constexpr (BITS == 4) {  // out of the order of the codes
 #pragma unroll
@@ -893,10 +798,12 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #define SD_NAME2(e, b) tree_tile_e##e##_b##b
 #define SD_NAME(e, b) SD_NAME2(e, b)
 const void* SD_NAME(SD_E, SD_BITS)(int D, bool shared) {
-  if (D == 64) return shared ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 64, true>)
-                             : reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 64, false>);
-  return shared ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 128, true>)
-                : reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 128, false>);
+#if SD_BITS == 0
+  if (shared) return D == 64 ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, 0, 64, true>)
+                             : reinterpret_cast<const void*>(&tree_tile_kernel<ET, 0, 128, true>);
+#endif
+  return D == 64 ? reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 64, false>)
+                 : reinterpret_cast<const void*>(&tree_tile_kernel<ET, SD_BITS, 128, false>);
 }
 
 }  // namespace sd

@@ -3,6 +3,8 @@ and that read or wrote, once, what they should not have."""
 from __future__ import annotations
 
 import ctypes
+import math
+import random
 
 import pytest
 
@@ -116,3 +118,168 @@ def test_tree_precision_does_not_go_by_the_columns(cuda, monkeypatch, dtype, bit
     assert tree.uses_tiles(dtype, bits, counts, G)
     monkeypatch.setattr(tree, "uses_tiles", lambda *a: False)
     tree.run_tree(cuda, dtype, bits, d, hkv, G, page, held, counts, seed=G + d, **more)
+
+
+def check_codes(torch, out, ref, size, reach, dtype, tile, bits=0):
+    """Of many columns: a value of codes is two bf16 values, the first cut off, off by 2^-7 2^-8 = 2^-15 of it at most.
+    So a score is off by d = 2^-15 B, B = scale sum |q k|, and the output by (e^2d - 1) A, A = sum p |v| / sum p; values,
+    weights (2^-16) and the product of low halves that is left out (2^-8 p times 2^-7 v) are 2^-13 A more at most; then
+    half a step of the result. Most of that cancels: in the mean square nothing but that half step shows, as with few
+    columns. (Not the norm against the rounded exact result, of which one value that lies half-way makes 2e-3.)"""
+    u = torch.finfo(out.dtype).eps / 2
+    bound = 1.01 * u * ref.abs() + size * (torch.expm1(2.0 ** -14 * reach[0]) + 2.0 ** -13)
+    off = (out.double() - ref).abs()
+    assert bits and (off <= bound).all(), f"{int((off > bound).sum())} off, worst {float((off / bound).max()):.3g}"
+    assert (off.pow(2).sum() / ref.pow(2).sum()).sqrt() <= 0.65 * u
+
+
+@pytest.mark.parametrize("bits,d,hkv,G,page,held,counts,more", [
+    (4, 128, 2, 4, 64, [3000, 5, 0, 1000], [33, 20, 64, 40], {}),
+    (4, 64, 2, 16, 16, [700, 90], [64, 20], dict(window=200, sinks=True)),
+    (8, 128, 2, 4, 64, [3000, 5, 0, 1000], [33, 20, 64, 40], {}),
+    (8, 64, 2, 8, 32, [20000, 37], [33, 60], {}),
+    (8, 64, 2, 16, 64, [700, 90], [33, 20], dict(scale=1e-3)),
+])
+def test_tree_precision_of_codes_does_not_go_by_the_columns(cuda, monkeypatch, bits, d, hkv, G, page, held, counts, more):
+    assert tree.uses_tiles("bf16", bits, counts, G)
+    monkeypatch.setattr(tree, "check_tree", check_codes)
+    tree.run_tree(cuda, "bf16", bits, d, hkv, G, page, held, counts, seed=G + d, **more)
+
+
+@pytest.mark.parametrize("dtype,bits,d,G", [("bf16", 0, 128, 4), ("bf16", 0, 64, 16), ("f16", 0, 128, 8), ("bf16", 4, 128, 4),
+                                            ("bf16", 4, 64, 16), ("bf16", 8, 128, 8), ("bf16", 8, 64, 16)])
+def test_tree_scores_of_hundreds(cuda, dtype, bits, d, G):
+    """Keys and values thirty times as large: a softmax of one or a few tokens, whose weights go by errors of the scores.
+
+    The values of codes are taken as the kernel's two halves of them, so that its sums alone are off: a score by 16 steps of
+    at most 2 units 2^-23 of B, the largest scale sum |q k|, that is d = 2^-18 B, which moves the output by at most (e^2d - 1)
+    A, A = sum p |v| / sum p; weights (2^-16) and the product of low halves that is left out (2^-8 p times 2^-7 v) by less
+    than 2^-14 A; and half a step of the result. Weights below 2^-126 are none, and below 2^-117 their low halves lose bits: less
+    than 2^-125 of a value; of fp16, whose largest weight is 2^7 at least, 2^-25 of that, 2^-32. (The framework's tolerance is
+    against the rounded exact result. It does not fit here: values of codes lie half-way between two results more often than
+    not.)"""
+    import sparse_decode as sd
+    torch = cuda
+    hkv, page, held, counts = 2, 64, [700, 90], [33, 20]
+    assert tree.uses_tiles(dtype, bits, counts, G)
+    ends = [h + n for h, n in zip(held, counts)]
+    pool = Pool(torch, sd, dtype, bits, hkv, d, page, 20, 3, 30.0)
+    tables = tables_of(torch, ends, page, 20, 4)
+    if bits:
+        for i, x in enumerate(pool.values):
+            high = (x.float().view(torch.int32) & -65536).view(torch.float32)
+            pool.values[i] = high.double() + (x.float() - high).bfloat16().double()
+    q = (2 * torch.randn(sum(counts), hkv * G, d, generator=gen(torch, 5), device="cuda")).to(tdt(torch, dtype))
+    first = i32(torch, [0, counts[0], sum(counts)])
+    out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, ends), first)
+    lines = [[((2 << i) - 1, h + i) for i in range(n)] for h, n in zip(held, counts)]
+    ref, size, (reach, values) = tree.tree64(q, pool, tables, held, lines, 1 / math.sqrt(d))
+    u = torch.finfo(out.dtype).eps / 2
+    bound = 1.01 * u * ref.abs() + size * (torch.expm1(2.0 ** -17 * reach) + 2.0 ** -14) + values * 2.0 ** (-32 if dtype == "f16" else -125)
+    off = (out.double() - ref).abs()
+    assert reach.min() > 150 and (off <= bound).all(), f"{int((off > bound).sum())} off, worst {float((off / bound).max()):.3g}"
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n,d", [(40, 128), (33, 64)])
+def test_tree_codes_of_keys_with_large_channels(cuda, bits, n, d):
+    """One channel of every group is a hundred times as large as what the others spread over, so that the scores' parts cancel."""
+    import sparse_decode as sd
+    torch = cuda
+    hkv, G, page, held = 2, 4, 64, 4000
+    pool = Pool(torch, sd, "bf16", bits, hkv, d, page, 64, 5)
+    tables = tables_of(torch, [held + n], page, 64, 6)
+    (k, ks, kb), top, per = pool.arrays[0], (1 << bits) - 1, 32 // bits
+    g = gen(torch, 7)
+    codes = torch.randint(0, 2 if bits == 4 else 6, (*ks.shape[:-1], d), generator=g, device="cuda")
+    codes[..., 7::64] = top - torch.randint(0, 2 if bits == 4 else 6, codes[..., 7::64].shape, generator=g, device="cuda")
+    words = (codes.unflatten(-1, (-1, per)) << (torch.arange(per, device="cuda") * bits)).sum(-1)
+    k.copy_(torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32))
+    ks.copy_((102 + torch.rand(ks.shape, generator=g, device="cuda")) / top)
+    kb.copy_(-2 + 0.1 * torch.rand(ks.shape, generator=g, device="cuda"))
+    grow = lambda t: t.double().repeat_interleave(64, -1)  # noqa: E731
+    pool.values[0] = codes.double() * grow(ks) + grow(kb)
+    q = torch.randn(n, hkv * G, d, generator=g, device="cuda").bfloat16()
+    out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [held + n]), i32(torch, [0, n]))
+    lines = [[((2 << i) - 1, held + i) for i in range(n)]]
+    ref, size, reach = tree.tree64(q, pool, tables, [held], lines, 1 / math.sqrt(d))
+    tree.check_tree(torch, out, ref, size, reach, "bf16", False)
+
+
+# ---------------------------------------------------------------------------
+# tree attention: what a row does not see
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 0), ("f16", 0), ("bf16", 4), ("bf16", 8), ("f16", 4), ("f32", 8), ("f32", 0)])
+@pytest.mark.parametrize("G", [2, 16])
+@pytest.mark.parametrize("held", [0, 37, 200])
+@pytest.mark.parametrize("x", [2.0 ** 60, -2.0 ** 60, math.inf, -math.inf, math.nan])
+def test_tree_large_values_in_hidden_and_absent_nodes(cuda, dtype, bits, G, held, x):
+    """Two branches from one root, and nodes that do not exist: their keys and values, finite and large or not finite, leave
+    the rows alone that do not see them, bit for bit."""
+    import sparse_decode as sd
+    torch = cuda
+    if dtype == "f16" and abs(x) < math.inf:
+        x = math.copysign(2.0 ** 15, x)
+    pool = Pool(torch, sd, dtype, bits, 2, 128, 16, 16, 3)
+    tables = tables_of(torch, [held + 8], 16, 16, 4)
+    parents = [-1, 0, 0, 1, 2, 3, -2, 6]  # 2 and 4 are the other branch, 6 and 7 absent
+    masks = torch.tensor([m for m, _ in tree.lineage(parents)], dtype=torch.int64, device="cuda")
+    q = torch.randn(8, 2 * G, 128, generator=gen(torch, 4), device="cuda").to(tdt(torch, dtype))
+    call = lambda: sd.paged_tree_decode(  # noqa: E731
+        q, pool.pages, tables, i32(torch, [held + 8]), i32(torch, [0, 8]), masks)
+    clean = call()
+    for arrays in (pool.arrays[:1], pool.arrays[1:], pool.arrays):
+        saved = [a[-1].clone() for a in pool.arrays]
+        for a in arrays:
+            for node in (2, 4, 6, 7):
+                t = held + node
+                a[-1][int(tables[0, t // 16]), :, t % 16] = x  # all of a row, or every group's bias
+        out = call()
+        for a, s in zip(pool.arrays, saved):
+            a[-1].copy_(s)
+        for node in (0, 1, 3, 5, 6, 7):
+            assert torch.equal(out[node], clean[node]), node
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("G", [4, 16])
+@pytest.mark.parametrize("power", [-60, 40, 60])
+def test_tree_codes_beside_tokens_of_another_size(cuda, bits, G, power):
+    """A held token in every tile, and a node, whose values are 2^power of the others', with keys that give it no weight:
+    the others' values keep their bits. (Calls of many columns. With few, codes are the decode kernel's, which has an error
+    of 2^-28 of the largest scale.)"""
+    import sparse_decode as sd
+    torch = cuda
+    n, held, hkv, d = 9, 300, 2, 64
+    assert tree.uses_tiles("bf16", bits, [n], G)
+    pool = Pool(torch, sd, "bf16", bits, hkv, d, 64, 8, 5)
+    tables = tables_of(torch, [held + n], 64, 8, 6)
+    q = (torch.rand(n, hkv * G, d, generator=gen(torch, 7), device="cuda") + 0.5).bfloat16()
+    for t in [*range(7, held, 50), held + 2]:
+        at = (int(tables[0, t // 64]), slice(None), t % 64)
+        pool.arrays[0][1][at], pool.arrays[0][2][at] = 0.0, -40.0  # a score of -230 at most
+        for a in pool.arrays[1][1:]:
+            a[at] *= 2.0 ** power
+        pool.values[0][at] = -40.0
+        pool.values[1][at] *= 2.0 ** power
+    out = sd.paged_tree_decode(q, pool.pages, tables, i32(torch, [held + n]), i32(torch, [0, n]))
+    lines = [[((2 << i) - 1, held + i) for i in range(n)]]
+    ref, size, reach = tree.tree64(q, pool, tables, [held], lines, 1 / math.sqrt(d))
+    tree.check_tree(torch, out, ref, size, reach, "bf16", False)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B", [3400, 3500, 4096])
+def test_tree_codes_of_thousands_of_sequences(cuda, monkeypatch, bits, B):
+    """Heads of 128: what is noted of that many sequences leaves no room for the tiles of 8-bit codes, which the other kernel takes."""
+    rng = random.Random(B)
+
+    def check(torch, out, ref, size, reach, *a):
+        # The other kernel sums (p s)(c - z) and p (b + z s) apart, z the middle code: each is off by three units 2^-23 of
+        # p z |s|. z |s| is half of a group's range, 1.3 times its largest |value| at most where its codes span 200 of 255, and the
+        # largest A of a row a third of its tokens' largest or more: less than 2^-18 of the largest A, where A itself may
+        # be next to nothing.
+        check_codes(torch, out, ref, size + 2.0 ** -5 * size.amax(-1, keepdim=True), reach, *a)
+    monkeypatch.setattr(tree, "check_tree", check)
+    tree.run_tree(cuda, "bf16", bits, 128, 1, 16, 16, [rng.randint(0, 12) for _ in range(B)], [rng.choice([2, 3, 4]) for _ in range(B)], seed=5)
