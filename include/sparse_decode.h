@@ -447,6 +447,8 @@ int32_t sd_paged_tree_decode(const sd_pages* pages, int32_t layer, const void* q
  * < ... (path [batch, path_width], path_width <= SD_MAX_NODES): their rows move
  * to positions held, held + 1, ..., in every layer and array of the pool, and
  * new_lengths[b] = held + kept[b], held = ends[b] - (first[b + 1] - first[b]).
+ * Rows move as they are: that a path goes down the tree from a root, whose
+ * places its rows were rotated for, and names no absent node is the caller's.
  * Pages of two sequences must not be the same where rows move. An entry that
  * is no node or does not rise, or a page out of range, ends its sequence's
  * path there and sets bit 2 of *device_flags. new_lengths must be none of the

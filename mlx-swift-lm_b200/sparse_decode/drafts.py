@@ -166,7 +166,9 @@ def paged_keep(pages: KVPages, tables, ends, first, path, kept, *, lengths=None,
 
     tables [batch, width], ends [batch], first [batch + 1], path [batch, up to
     64], kept [batch]: int32. An entry that is no node, or does not rise, ends
-    its sequence's path and sets bit 2 of flags."""
+    its sequence's path and sets bit 2 of flags. That a path goes down the tree
+    from a root and names no absent node is the caller's (`PagedBatch.keep`
+    checks it): rows move as they are."""
     dev, i32 = pages.here(), _p._I32
     if tables.dim() != 2 or path.dim() != 2 or path.shape[0] != tables.shape[0]:
         raise ValueError("tables must be [batch, width] and path [batch, nodes]")

@@ -591,6 +591,14 @@ class PagePool:
 _PLAN_TOKENS = 256
 
 
+def _lines(parents: Sequence[int]) -> list:
+    """Of each node the bits of itself and its ancestors; 0: there is no such node."""
+    got: list = []
+    for i, up in enumerate(parents):
+        got.append(1 << i if up == -1 else 1 << i | got[up] if up >= 0 and got[up] else 0)
+    return got
+
+
 class PagedBatch:
     """One step of some sequences of a pool: `tables` [batch, width] and
     `lengths` [batch] with the step's new tokens counted in, and for the new
@@ -599,6 +607,7 @@ class PagedBatch:
     ends such a step."""
 
     plan = None  # of `tree`
+    _seen = None  # of `tree`: `_lines` of each sequence, None where the plan's masks alone have them
 
     def __init__(self, pool: PagePool, seqs: list, new: list, stream=None):
         self.pool, self.seqs, self.new = pool, seqs, new
@@ -649,12 +658,14 @@ class PagedBatch:
         if parents is None:
             parents = list(range(-1, max(new, default=0) - 1))
         host = [t - k for t, k in zip(self.host_lengths, new)] + list(new)
+        seen = None
         if not isinstance(parents, torch.Tensor):
             rows = parents if parents and not isinstance(parents[0], int) else [parents] * n
             if len(rows) != n or any(len(r) < k for r, k in zip(rows, new)):
                 raise ValueError("parents must name one for every new token")
             if any(p >= i for r, k in zip(rows, new) for i, p in enumerate(r[:k])):
                 raise ValueError("a parent comes before its node")
+            seen = [_lines(r[:k]) for r, k in zip(rows, new)]
             wide = max(1, max(new, default=0))
             host += [p for r, k in zip(rows, new) for p in [*r[:k], *[-2] * (wide - k)]]
             parents = None
@@ -665,7 +676,7 @@ class PagedBatch:
             parents = dev[2 * n:].view(n, wide)
         self.plan = paged_plan(dev[:n], dev[n:2 * n], self.tables, self.pool.pages.page_size, sum(new), parents=parents,
                                flags=self.pool.flags, stream=stream)
-        self.positions, self.seq = self.plan.positions, self.plan.seq
+        self.positions, self.seq, self._seen = self.plan.positions, self.plan.seq, seen
         return self
 
     def _refuse_stale(self) -> None:
@@ -682,9 +693,11 @@ class PagedBatch:
                                  layer=layer, flags=self.pool.flags, **kw)
 
     def keep(self, paths: Sequence[Sequence[int]], stream=None) -> None:
-        """End a tree's step: of sequence i the nodes paths[i], rising, are kept
-        and become its next tokens, in every layer, the others are dropped. The
-        step's calls must be on `stream` or waited for by it; the batch is
+        """End a tree's step: of sequence i the nodes paths[i] are kept and
+        become its next tokens, in every layer, the others are dropped. A path
+        goes down the tree from a root, node by node, as the rows were rotated
+        for these places (of a tree given as a tensor that is read from the
+        device); or it is empty. The step's calls must be on `stream` or waited for by it; the batch is
         stale afterwards. Refused when a sequence has changed since the step
         was made (a fork of it shares the pages that would be written) or the
         pool was compacted."""
@@ -699,6 +712,16 @@ class PagedBatch:
             if any(not 0 <= i < k for i in x) or any(a >= b for a, b in zip(x, x[1:])):
                 raise ValueError("a path names nodes in rising order")
         self._refuse_stale()
+        seen = self._seen
+        if seen is None:
+            _refuse_capture(stream)
+            with torch.cuda.stream(stream):
+                masks = p.masks.tolist()
+            at = [sum(self.new[:b]) for b in range(n)]
+            seen = [[m % (1 << 64) for m in masks[a:a + k]] for a, k in zip(at, self.new)]
+        for x, lines in zip(paths, seen):
+            if x and lines[x[-1]] != sum(1 << i for i in x):
+                raise ValueError(f"{x} is no way down the tree from a root")
         wide = max(1, max(map(len, paths), default=0))
         host = [i for x in paths for i in [*x, *[-1] * (wide - len(x))]] + [len(x) for x in paths]
         dev = _upload(torch.tensor(host, dtype=torch.int32).pin_memory(), stream)

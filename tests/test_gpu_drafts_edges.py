@@ -283,3 +283,46 @@ def test_tree_codes_of_thousands_of_sequences(cuda, monkeypatch, bits, B):
         check_codes(torch, out, ref, size + 2.0 ** -5 * size.amax(-1, keepdim=True), reach, *a)
     monkeypatch.setattr(tree, "check_tree", check)
     tree.run_tree(cuda, "bf16", bits, 128, 1, 16, 16, [rng.randint(0, 12) for _ in range(B)], [rng.choice([2, 3, 4]) for _ in range(B)], seed=5)
+
+
+# ---------------------------------------------------------------------------
+# keep
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("form", ["list", "lists", "one tensor", "tensors"])
+def test_pool_refuses_paths_that_are_not_in_the_tree(cuda, form):
+    """Rows are rotated for their places in the tree, and absent nodes have none: a path skips no node and ends at none that is
+    absent."""
+    import sparse_decode as sd
+    pool = sd.PagePool(1, 30, 2, 64, 16)
+    a, b = pool.add(), pool.add()
+    parents = [-1, 0, 0, 1, -2, 4, -1, 6, 2]
+    tree_of = {"list": parents, "lists": [parents, parents], "one tensor": i32(cuda, parents), "tensors": i32(cuda, [parents] * 2)}[form]
+    step = pool.extend([a, b], [9, 7]).tree(tree_of)
+    if form == "one tensor":
+        tree_of.fill_(-1)  # the step has its own
+    k = cuda.randn(16, 2, 64, device="cuda").bfloat16()
+    step.append(0, k, k)
+    for bad in ([1], [0, 3], [0, 2, 3], [0, 1, 2], [4], [0, 4], [4, 5], [0, 6], [2], [0, 1, 3, 8], [7]):
+        for paths in ([bad, [0]], [[0], bad]):
+            if max(paths[1]) < 7:
+                with pytest.raises(ValueError, match="way down"):
+                    step.keep(paths)
+    assert [pool.length(s) for s in (a, b)] == [9, 7]
+    step.keep([[0, 2, 8], [6]])
+    assert [pool.length(s) for s in (a, b)] == [3, 1] and pool.check_device() == 0
+    got = pool.batch([a]).layer(0).dense(0)[0]
+    assert cuda.equal(got.reshape(2, 3, 64), k[[0, 2, 8]].transpose(0, 1))
+
+
+def test_pool_refuses_paths_off_a_long_chain(cuda):
+    import sparse_decode as sd
+    for given in (None, i32(cuda, list(range(-1, 63)))):
+        pool = sd.PagePool(1, 30, 2, 64, 16)
+        a = pool.add()
+        step = pool.extend([a], 64).tree(given)
+        for bad in ([1], [0, 2], list(range(1, 64)), [*range(62), 63]):
+            with pytest.raises(ValueError, match="way down"):
+                step.keep([bad])
+        step.keep([list(range(64))])
+        assert pool.length(a) == 64 and pool.check_device() == 0
