@@ -95,9 +95,12 @@ constexpr int kTreeHeads = 4;      // query heads that a warp takes to the nodes
 constexpr int kTreeAttendThreads = kPagedThreads + 32;  // a decode's, and a warp for the nodes
 constexpr int kTreeMergeCols = 8;  // columns of a merge block
 
-// Shared memory of an attend CTA: as a decode's, with two numbers per sequence, the columns' first tokens and two counts.
+// Shared memory of an attend CTA: as a decode's, with two numbers per sequence and per warp, the columns' first tokens and
+// two counts (tree_attend_kernel: units, pairs, tmp, low, next).
+constexpr int kTreeLows = 16, kTreeCounts = 2;
+constexpr int tree_attend_ints(int batch) { return 2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + kTreeLows + kTreeCounts; }
 constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32, int stage_bytes) {
-  return paged_layout_of((2 * (batch + 1) + 2 * (kTreeAttendThreads / 32) + 18) * 4, columns, D, dense_f32, stage_bytes);
+  return paged_layout_of(tree_attend_ints(batch) * 4, columns, D, dense_f32, stage_bytes);
 }
 
 // The tile kernel of 16-bit pools (sd_tree_tile.cu): one CTA per SM, two groups

@@ -413,10 +413,11 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
   float* qf = reinterpret_cast<float*>(sm + p.q_off);
   float* buf = reinterpret_cast<float*>(sm + p.buf_off);
   int* units = reinterpret_cast<int*>(sm + p.prefix_off);
-  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kTreeAttendThreads / 32), *next = low + 16;
+  int *pairs = units + p.B + 1, *tmp = pairs + p.B + 1, *low = tmp + 2 * (kTreeAttendThreads / 32), *next = low + kTreeLows;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + p.bar_off);
   uint64_t* empty = full + kPagedMaxStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  static_assert(kTreeCounts == 2 && (NB * (sizeof(E) == 4 && BITS == 0 ? 4 : 8)) <= kTreeLows, "next[0] and next[1]; a token per column");
 
   if (tid == 0) {
     *next = 0;
@@ -456,9 +457,9 @@ tree_attend_kernel(const __grid_constant__ TreeParams p, const __grid_constant__
         const int t0 = sq.begin / F::kTile;
         int edge = 0;  // tokens below it are not seen by every column
         if (p.window) {
-          if (tid < 16) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
+          if (tid < kTreeLows) low[tid] = tree_low(p, sq, cols.node(min(tid, cols.n - 1)));
           named_barrier(1, 32 * kPagedWarps);
-          edge = __reduce_max_sync(0xffffffffu, low[lane & 15]);
+          edge = __reduce_max_sync(0xffffffffu, low[lane % kTreeLows]);
         }
         att.begin(p, qf, cols, warp, lane);
         for (int i = s.i0; i < s.i1; ++i, ++it) {
