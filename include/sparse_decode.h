@@ -435,7 +435,10 @@ int32_t sd_paged_plan(const sd_plan* plan, int32_t* device_flags, sd_stream stre
  * whose tokens read as 0. first has to rise from 0 to batch: where it falls, all
  * rows before first[batch] give zeros. Equal calls give equal bits. The workspace
  * (sd_paged_tree_workspace bytes, 16-byte aligned, contents do not matter)
- * must not be shared by calls that may overlap. q, out: 16-byte aligned. */
+ * must not be shared by calls that may overlap. Which kernel a call takes goes
+ * by n_rows / batch, rows of padding included: a matter of speed, not of
+ * precision. With a window, a value that is not finite of a token before the
+ * step reaches all rows of its sequence if one of them sees the token. q, out: 16-byte aligned. */
 int32_t sd_paged_tree_workspace(const sd_pages* pages, int32_t batch, int32_t n_rows, int32_t n_q_heads, int64_t* bytes);
 int32_t sd_paged_tree_decode(const sd_pages* pages, int32_t layer, const void* q, int32_t n_rows, int32_t batch,
                              int32_t n_q_heads, const int32_t* tables, int32_t table_width, const int32_t* lengths,

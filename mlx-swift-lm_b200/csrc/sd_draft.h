@@ -114,9 +114,9 @@ constexpr PagedLayout tree_layout(int batch, int columns, int D, bool dense_f32,
 constexpr int tree_tile_above(int bits) { return bits ? 32 : 16; }
 constexpr int kTreeTileThreads = 352;
 constexpr int kTreeTileTokens = 64;
-// Beginning and ending a segment, in tiles. Measured, 2 / 4 / 8 / 16: 12 windows of 1000 tokens, 168 columns, 38.9 / 31.3 /
-// 31.0 / 30.6 us; 16 ragged sequences of about 4K, 64 columns, plan to keep, 63 / 48 / 48 / 52 us; 4 x 32K in 4 bits 122 /
-// 121 / 117 / 118 us.
+// Beginning and ending a segment, in tiles. Measured, 2 / 4 / 8 / 16: 12 windows of 1000 tokens, 168 columns, 41.6 / 32.7 /
+// 30.9 / 30.5 us; 16 ragged sequences of about 4K, 64 columns, plan to keep, 78 / 60 / 52 / 60 us; one of 32K, 128 columns,
+// 43.2 / 41.8 / 39.9 / 40.3 us; 4 x 32K in 4 bits 199 / 199 / 200 / 203 us.
 constexpr int kTreeTileUnits = 8;
 constexpr int kTreeTileStages = 24, kTreeTileLeast = 4;
 constexpr int kTreeTileBarBytes = 768;

@@ -19,11 +19,11 @@
 //     attends to the visible nodes alone, reading no other node's rows -- what lies
 //     there, not-a-numbers included, does not reach it. A CTA has a warp for it,
 //     beside the tiles' warps, whose time hides its chain of loads; the others come
-//     to its help when they are done (35 sequences of 8 tokens, 31 nodes of 8 heads
-//     in 8-bit codes of an fp16 pool: 120 -> 75 us).
+//     to its help when they are done (35 sequences of 8 tokens, 31 nodes, 24 query
+//     and 3 kv heads in 8-bit codes of an fp16 pool: 120 -> 75 us).
 // tree_attend_kernel does both, and tree_merge_kernel joins a column's nodes and
-// segments in CTA order. The tile kernel of 16-bit pools (sd_tree_tile.cu) has
-// the nodes on the line, as a sequence's last tokens.
+// segments in CTA order. The tile kernel of 16-bit pools and of codes of bf16 ones
+// (sd_tree_tile.cu) has the nodes on the line, as a sequence's last tokens.
 // Results depend on no timing. Lengths, rows and tables are read on the device
 // only, so a captured graph serves growing sequences.
 #pragma once

@@ -31,12 +31,13 @@
 // infinities and not-a-numbers in a node's row, which a row that does see the
 // node gets back at the end.
 // Bound by the weighing warps and the products: 64 tokens of 256 columns are 16384
-// exponentials, 1024 cycles of an SM, and some 1900 cycles of products, and take some
-// 2300: each scheduler has two such warps, whose chain (load, maxima, exponentials,
+// exponentials, 1024 cycles of an SM, and some 1700 cycles of products, and take some
+// 2900: each scheduler has two such warps, whose chain (load, maxima, exponentials,
 // halves, store, signal) leaves gaps. Measured with the merge, 32 query and 8 kv heads
-// of 128 in bf16: 4 sequences of 32K tokens with 64 nodes 180 us (3.0 TB/s; 0.76 PFLOP/s
-// of attention, half as much again with the low halves), one with 32 nodes 40 us
-// (3.3 TB/s); 4 x 32K in 4 bits with 16 nodes 201 us.
+// of 128 in bf16: 4 sequences of 32K tokens with 64 nodes 180 to 186 us (2.9 TB/s, 0.74 PFLOP/s
+// of attention, half as much again with the low halves; 216 us at the 1500 MHz that
+// the power limit leaves when it goes on), one with 32 nodes 40 us (3.3 TB/s); 4 x 32K in
+// 4 bits with 16 nodes 200 us.
 //
 // Codes: the loading warp brings them as they are, with their scales; eight more
 // make tiles of values of them, s c + b in fp32 and then two bf16 values, a high and a low
@@ -45,7 +46,7 @@
 // P and V, less the low halves' own. Bound by the converting warps: ten instructions make
 // two values, and a tile takes one of their two teams 4500 cycles, 2600 a tile with what they
 // wait for (P V first and then the next scores, which wait for the team: the other order
-// kept V's place from the team, 291 us instead of 201 for 4 x 32K in 4 bits with 16
+// kept V's place from the team, 291 us instead of 200 for 4 x 32K in 4 bits with 16
 // nodes). One fp16 value with a power of two per tile took 126 us there, but it was
 // off by 2^-12 of every value, which keys with a large channel make 8e-3 of a result, and
 // lost a tile's small values beside a large one that a row need not even see.
