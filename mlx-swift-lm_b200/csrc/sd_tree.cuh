@@ -254,7 +254,8 @@ struct StoredPiece<E, 0, V> {
 
 // Rows and up to four query heads of one kv head at a time, the CTA's (each grid-th)
 // in turn as its warps come for them: `next`, in shared memory, counts, and has the
-// number of rows behind it. `any`: whether the call has sequences that can be. Which warp has a row changes nothing of it. Lane l holds dimensions [l V, l V + V)
+// number of rows behind it. Which warp has a row changes nothing of it. `any`:
+// whether the call has sequences that can be. Lane l holds dimensions [l V, l V + V)
 // of q, o and the rows; scores are summed over the lanes by a butterfly that ends
 // with head l / 8's in lane l, so that lane l keeps token l % 8's of the eight
 // that are taken at a time.

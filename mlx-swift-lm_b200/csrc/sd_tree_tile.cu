@@ -491,7 +491,8 @@ tree_tile_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ C
 #pragma unroll
                     for (int i4 = 0; i4 < 4; ++i4) {
                       const float unit = BITS == 8 ? sc : sc * (1.0f / float(1 << (4 * i4)));
-                      f[i4] = fma2(BITS == 8 ? bytes2(words[(2 * j + i4 / 2) & 3], 2 * (i4 & 1)) : nibbles2(words[j & 3], i4), make_float2(unit, unit), b2);
+                      const float2 code = BITS == 8 ? bytes2(words[(2 * j + i4 / 2) & 3], 2 * (i4 & 1)) : nibbles2(words[j & 3], i4);
+                      f[i4] = fma2(code, make_float2(unit, unit), b2);
                     }
                     uint32_t h[4], l[4];
 #pragma unroll
